@@ -31,6 +31,22 @@ class FmdGemmProblem(ctypes.Structure):
                 ("m", c_int64), ("n", c_int32), ("k", c_int32), ("act", c_int32), ("accumulate", c_int32)]
 
 
+class FmdHeadRotarySide(ctypes.Structure):
+    """One side (queries or keys) of fmd_head_rotary."""
+    _fields_ = [("x", c_void_p), ("g", c_void_p), ("y", c_void_p), ("w", c_void_p), ("dw", c_void_p),
+                ("row_stride", c_int64), ("head_stride", c_int64), ("g_row_stride", c_int64),
+                ("g_head_stride", c_int64), ("heads", c_int32), ("_pad", c_int32)]
+
+
+class FmdAttention(ctypes.Structure):
+    """The problem of fmd_packed_attention and fmd_packed_attention_bwd."""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("offsets", c_void_p), ("key_offsets", c_void_p),
+                ("key_counts", c_void_p), ("rows", c_int64), ("keys", c_int64), ("q_row", c_int64),
+                ("q_head", c_int64), ("k_row", c_int64), ("k_head", c_int64), ("v_row", c_int64), ("v_head", c_int64),
+                ("scale", c_float), ("type", c_int32), ("batch", c_int32), ("heads", c_int32), ("key_heads", c_int32),
+                ("dim", c_int32), ("causal", c_int32), ("_pad", c_int32)]
+
+
 _P = c_void_p  # every device pointer and the stream travel as void*
 _I64, _I32 = c_int64, c_int32
 
@@ -115,6 +131,11 @@ _SIGNATURES: dict[str, list] = {
     "fmd_nequip_self_connection": [_P, _P, _P, _P, _P, _P, _P, _I64, _I32, _P, _P, _P, _P],
     "fmd_nequip_gate": [_P, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P],
     "fmd_nequip_gate_bwd": [_P, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P],
+    "fmd_head_rotary_workspace_bytes": [_I32, POINTER(c_size_t)],
+    "fmd_head_rotary": [POINTER(FmdHeadRotarySide), _I32, _I32, _I64, _I32, _I32, _I32, c_float, _P, _P, _P, _I64,
+                        _I32, _P, c_size_t, _P, _P],
+    "fmd_packed_attention": [POINTER(FmdAttention), _P, _P, _P, _P],
+    "fmd_packed_attention_bwd": [POINTER(FmdAttention), _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P],
     "fmd_nhc_pre_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P],
     "fmd_nhc_post_pre_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P],
     "fmd_nhc_post_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P],
@@ -226,5 +247,5 @@ def flags_word(device) -> torch.Tensor:
 c_int32_t, c_int64_t = c_int32, c_int64
 c_void_p_t = c_void_p
 
-__all__ = ["FastMDLibraryError", "FmdCatPart", "call", "check", "declare", "flags_word", "lib", "ptr",
+__all__ = ["FastMDLibraryError", "FmdAttention", "FmdCatPart", "FmdHeadRotarySide", "call", "check", "declare", "flags_word", "lib", "ptr",
            "require_cuda", "stream", "c_double", "c_float", "c_int32", "c_int64", "c_void_p", "ctypes"]

@@ -51,14 +51,11 @@
 // FMD_FLAG_WAIT_TIMEOUT, waits (bounded) for its copies and MMAs in flight,
 // frees its TMEM and returns. No cluster launch and no multicast.
 
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
 #include <string.h>
 
 #include <mutex>
 
-#include "common.cuh"
+#include "sm100.cuh"
 
 namespace fmd {
 namespace {
@@ -87,7 +84,6 @@ constexpr uint32_t kACols = 2 * kStageK;   // one A buffer: x_hi then x_lo, 64 c
 constexpr uint32_t kNarrowAccCols = 64;    // n <= 64: one chunk accumulator of 64 columns
 static_assert(kAccBufs * kAccCols + kABufs * kACols <= kTmemCols, "TMEM budget");
 static_assert(kNarrowAccBufs * kNarrowAccCols + kABufs * kACols <= kTmemCols, "TMEM budget (narrow)");
-constexpr unsigned long long kWaitNs = 1000000000ull;
 
 struct Ctrl {
     uint64_t full[kMaxStages];       // TMA bytes landed (1 arrival + tx)
@@ -151,61 +147,6 @@ __device__ __forceinline__ int problem_of(const Group& G, int t, int& local) {
 
 // ------------------------------------------------------------- PTX wrappers
 
-__device__ __forceinline__ uint32_t su32(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(bar)), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(su32(bar))
-                 : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(
-                     su32(bar)),
-                 "r"(bytes)
-                 : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-__device__ __forceinline__ unsigned long long global_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-// Waits for the phase of `parity` to complete. Gives up after kWaitNs, or
-// as soon as another role of the CTA has given up (abort != 0, unless
-// `ignore_abort`); returns false then and sets the CTA's abort word.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int32_t* abort,
-                                          bool ignore_abort = false) {
-    const uint32_t a = su32(bar);
-    if (mbar_try_wait(a, parity)) return true;
-    const unsigned long long t0 = global_ns();
-    while (true) {
-        if (mbar_try_wait(a, parity)) return true;
-        if (!ignore_abort && *abort) return false;
-        if (global_ns() - t0 > kWaitNs) {
-            *abort = 1;
-            return false;
-        }
-    }
-}
-
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
@@ -228,19 +169,6 @@ __device__ __forceinline__ void bulk_wait_read_all() {
 }
 
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
-__device__ __forceinline__ void tc_fence_before() {
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-
-__device__ __forceinline__ void tc_fence_after() {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(bar))
-                 : "memory");
-}
 
 // D (=|+)= A . B^T with A [128 x 8] tf32 in TMEM (lane m, columns k) and B
 // from a shared-memory descriptor.
@@ -823,31 +751,6 @@ __global__ void wait_probe_kernel(int arrive, int32_t* flags) {
 
 // ------------------------------------------------------------------- host
 
-using EncodeTiled = PFN_cuTensorMapEncodeTiled_v12000;
-using CtxGetCurrent = PFN_cuCtxGetCurrent_v4000;
-
-struct DriverCalls {
-    EncodeTiled encode = nullptr;
-    CtxGetCurrent ctx_get_current = nullptr;
-};
-
-// Driver entry points through the runtime (no link against libcuda).
-const DriverCalls& driver_calls() {
-    static DriverCalls calls;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            calls.encode = reinterpret_cast<EncodeTiled>(p);
-        if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            calls.ctx_get_current = reinterpret_cast<CtxGetCurrent>(p);
-    });
-    return calls;
-}
-
 // [rows, cols] fp32 with row stride ld (elements), box [128 rows x 32 cols],
 // 128-byte swizzle, zero fill outside.
 CUresult encode_operand(EncodeTiled enc, CUtensorMap* map, const float* base, int64_t rows, int64_t cols,
@@ -965,15 +868,8 @@ fmd_status launch_group(const fmd_gemm_problem* problems, int32_t n_problems, in
     const DriverCalls& drv = driver_calls();
     if (drv.encode == nullptr || drv.ctx_get_current == nullptr)
         return record_error_text(FMD_ERR_CUDA, "driver entry point cuTensorMapEncodeTiled unavailable", 0);
-    // The tensor-map encoder is a driver call: a host thread on which the runtime has not yet made the
-    // primary context current (a fresh autograd worker, say) gets it bound first.
-    CUcontext current = nullptr;
-    if (drv.ctx_get_current(&current) != CUDA_SUCCESS || current == nullptr) {
-        int dev_index = 0;
-        cudaError_t err = cudaGetDevice(&dev_index);
-        if (err == cudaSuccess) err = cudaSetDevice(dev_index);
-        if (err != cudaSuccess) return record_cuda_error(err);
-    }
+    st = bind_context(drv);
+    if (st != FMD_OK) return st;
     bool narrow = true;
     for (int i = 0; i < n_problems; ++i) narrow = narrow && problems[i].n <= int32_t(kNarrowAccCols);
     GroupMaps maps;

@@ -1,0 +1,378 @@
+// Packed attention on the FP32 cores: forward, and the gradients of q and of k and v.
+//
+//   forward   s = scale q k^T (log2 units), running maximum m and sum l per row over key tiles:
+//             o = (o 2^(m - m') + 2^(s - m') v),  l likewise;  out = o / l,  lse = m + log l
+//   backward  p = exp(scale q k^T - lse),  dp = g v^T,  ds = p (dp - delta);
+//             dq = scale ds k   (one kernel, a block per tile of queries)
+//             dv = p^T g, dk = scale ds^T q   (one kernel, a block per tile of keys, over all rows that see it)
+//
+// Tiles of 64 rows x 64 keys in row-major shared memory, 256 threads, a 4 x 4 (rows ty + 16 i, columns tx + 16 j)
+// piece of every product each. A block owns its output rows and adds in one order: no atomics, the same bits every
+// time. Bound by the FP32 cores: per four values of the inner axis a thread reads 8 vectors for 64 products.
+
+#include "packed_attention.cuh"
+
+namespace fmd {
+namespace {
+
+constexpr int kM = 64, kN = 64, kThreads = 256;
+
+// rows [0, count) of src (row stride ld, dim values) into dst [64][DP + 4], zeros elsewhere
+template <typename T, int DP, typename RowOf>
+__device__ __forceinline__ void load_tile(float* dst, const T* src, int count, int dim, RowOf row_of) {
+    for (int i = threadIdx.x; i < 64 * DP; i += kThreads) {
+        const int r = i / DP, c = i - r * DP;
+        dst[r * (DP + 4) + c] = r < count && c < dim ? attn_float(src[row_of(r) + c]) : 0.0f;
+    }
+}
+
+// acc[i][j] += sum_d a[ty + 16 i][d] b[tx + 16 j][d]
+template <int DP>
+__device__ __forceinline__ void dots(const float* a, const float* b, int ty, int tx, float (&acc)[4][4]) {
+#pragma unroll 4
+    for (int d = 0; d < DP; d += 4) {
+        float4 x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * (DP + 4) + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * (DP + 4) + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
+                acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
+                acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
+                acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+            }
+    }
+}
+
+// acc[i][c] += sum_n p[ty + 16 i][n] b[n][2 tx + 32 (c / 2) + c % 2] over the 64 rows of b
+template <int DP>
+__device__ __forceinline__ void weigh(const float* p, const float* b, int ty, int tx, float (&acc)[4][DP / 16]) {
+#pragma unroll 2
+    for (int n = 0; n < 64; n += 4) {
+        float4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(p + (ty + 16 * i) * (64 + 4) + n);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) {
+                const float2 y = *reinterpret_cast<const float2*>(b + (n + u) * (DP + 4) + 2 * tx + 32 * c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float w = u == 0 ? x[i].x : u == 1 ? x[i].y : u == 2 ? x[i].z : x[i].w;
+                    acc[i][2 * c] = fmaf(w, y.x, acc[i][2 * c]);
+                    acc[i][2 * c + 1] = fmaf(w, y.y, acc[i][2 * c + 1]);
+                }
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ float sum16(float v) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+__device__ __forceinline__ float max16(float v) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// Where a packed row of the tile lies; token0: the tile's first token (of the sequence).
+struct Rows {
+    int64_t row0;
+    int group, head0, hq;
+    __device__ int64_t at(int r, int64_t row_stride, int64_t head_stride) const {
+        return (row0 + r / group) * row_stride + int64_t(head0 + r % group) * head_stride;
+    }
+    __device__ int64_t flat(int r) const { return (row0 + r / group) * hq + head0 + r % group; }
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) forward_kernel(const Attn a) {
+    extern __shared__ float smem[];
+    float* qs = smem;
+    float* ks = qs + 64 * (DP + 4);
+    float* vs = ks + 64 * (DP + 4);
+    float* ps = vs + 64 * (DP + 4);
+    const int per_tile = kM / a.group;
+    const int b = find_sequence(a.offsets, a.batch, per_tile, blockIdx.x);
+    const Span s = load_span(a, b);
+    const int64_t token0 = (int64_t(blockIdx.x) - (a.offsets[b] / per_tile + b)) * per_tile;
+    if (token0 < 0 || token0 >= s.rows) return;
+    const int tokens = int(min(int64_t(per_tile), s.rows - token0)), rows = tokens * a.group;
+    const Rows at{s.row0 + token0, a.group, int(blockIdx.y) * a.group, a.hq};
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const T* kp = static_cast<const T*>(a.k) + s.key0 * a.k_row + blockIdx.y * a.k_head;
+    const T* vp = static_cast<const T*>(a.v) + s.key0 * a.v_row + blockIdx.y * a.v_head;
+    load_tile<T, DP>(qs, static_cast<const T*>(a.q), rows, a.dim,
+                     [&](int r) { return at.at(r, a.q_row, a.q_head); });
+    int64_t limit[4];
+    float m[4], l[4], o[4][DP / 16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = ty + 16 * i;
+        limit[i] = r < rows ? seen(s, a.causal, token0 + r / a.group) : 0;
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) o[i][c] = 0.0f;
+    }
+    const int64_t end = seen(s, a.causal, token0 + tokens - 1);
+    const float scale = a.scale * kLog2e;
+    for (int64_t n0 = 0; n0 < end; n0 += kN) {
+        const int n = int(min(int64_t(kN), end - n0));
+        __syncthreads();
+        load_tile<T, DP>(ks, kp + n0 * a.k_row, n, a.dim, [&](int r) { return r * a.k_row; });
+        load_tile<T, DP>(vs, vp + n0 * a.v_row, n, a.dim, [&](int r) { return r * a.v_row; });
+        __syncthreads();
+        float x[4][4] = {};
+        dots<DP>(qs, ks, ty, tx, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[i][j] = n0 + tx + 16 * j < limit[i] ? x[i][j] * scale : -INFINITY;
+                top = fmaxf(top, x[i][j]);
+            }
+            top = fmaxf(m[i], max16(top));
+            const float base = top == -INFINITY ? 0.0f : top;  // a row with nothing yet: exp2(-inf) stays 0
+            const float keep = exp2f(m[i] - base);
+            m[i] = top;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p = exp2f(x[i][j] - base);
+                sum += p;
+                ps[(ty + 16 * i) * (64 + 4) + tx + 16 * j] = p;
+            }
+            l[i] = l[i] * keep + sum16(sum);
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) o[i][c] *= keep;
+        }
+        __syncthreads();
+        weigh<DP>(ps, vs, ty, tx, o);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = ty + 16 * i;
+        if (r >= rows) continue;
+        const float inv = l[i] > 0.0f ? 1.0f / l[i] : (l[i] == 0.0f ? 0.0f : l[i]);
+        T* out = static_cast<T*>(a.out) + at.flat(r) * a.dim;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+            const int col = 2 * tx + 32 * (c / 2) + c % 2;
+            if (col < a.dim) attn_store(out + col, o[i][c] * inv);
+        }
+        if (a.lse != nullptr && tx == 0) a.lse[at.flat(r)] = l[i] == 0.0f ? -INFINITY : m[i] * kLn2 + logf(l[i]);
+    }
+}
+
+// p and ds of one 4 x 4 piece: rows ty + 16 i of the first operand, columns tx + 16 j of the second
+__device__ __forceinline__ float weight_of(float dot, float scale, float lse2, bool there) {
+    return there ? exp2f(dot * scale - lse2) : 0.0f;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) query_gradient_kernel(const Attn a) {
+    extern __shared__ float smem[];
+    float* qs = smem;
+    float* gs = qs + 64 * (DP + 4);
+    float* ks = gs + 64 * (DP + 4);
+    float* vs = ks + 64 * (DP + 4);
+    float* ds = vs + 64 * (DP + 4);
+    const int per_tile = kM / a.group;
+    const int b = find_sequence(a.offsets, a.batch, per_tile, blockIdx.x);
+    const Span s = load_span(a, b);
+    const int64_t token0 = (int64_t(blockIdx.x) - (a.offsets[b] / per_tile + b)) * per_tile;
+    if (token0 < 0 || token0 >= s.rows) return;
+    const int tokens = int(min(int64_t(per_tile), s.rows - token0)), rows = tokens * a.group;
+    const Rows at{s.row0 + token0, a.group, int(blockIdx.y) * a.group, a.hq};
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const T* kp = static_cast<const T*>(a.k) + s.key0 * a.k_row + blockIdx.y * a.k_head;
+    const T* vp = static_cast<const T*>(a.v) + s.key0 * a.v_row + blockIdx.y * a.v_head;
+    load_tile<T, DP>(qs, static_cast<const T*>(a.q), rows, a.dim,
+                     [&](int r) { return at.at(r, a.q_row, a.q_head); });
+    load_tile<T, DP>(gs, static_cast<const T*>(a.g), rows, a.dim,
+                     [&](int r) { return at.at(r, a.g_row, a.g_head); });
+    int64_t limit[4];
+    float lse2[4], delta[4], dq[4][DP / 16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = ty + 16 * i;
+        lse2[i] = r < rows ? a.lse[at.flat(r)] * kLog2e : -INFINITY;
+        limit[i] = lse2[i] != -INFINITY ? seen(s, a.causal, token0 + r / a.group) : 0;  // an empty row has no share
+        delta[i] = r < rows ? a.delta[at.flat(r)] : 0.0f;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) dq[i][c] = 0.0f;
+    }
+    const int64_t end = seen(s, a.causal, token0 + tokens - 1);
+    const float scale = a.scale * kLog2e;
+    for (int64_t n0 = 0; n0 < end; n0 += kN) {
+        const int n = int(min(int64_t(kN), end - n0));
+        __syncthreads();
+        load_tile<T, DP>(ks, kp + n0 * a.k_row, n, a.dim, [&](int r) { return r * a.k_row; });
+        load_tile<T, DP>(vs, vp + n0 * a.v_row, n, a.dim, [&](int r) { return r * a.v_row; });
+        __syncthreads();
+        float x[4][4] = {}, y[4][4] = {};
+        dots<DP>(qs, ks, ty, tx, x);
+        dots<DP>(gs, vs, ty, tx, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool there = n0 + tx + 16 * j < limit[i];
+                const float p = weight_of(x[i][j], scale, lse2[i], there);
+                ds[(ty + 16 * i) * (64 + 4) + tx + 16 * j] = there ? p * (y[i][j] - delta[i]) : 0.0f;
+            }
+        __syncthreads();
+        weigh<DP>(ds, ks, ty, tx, dq);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = ty + 16 * i;
+        if (r >= rows) continue;
+        T* out = static_cast<T*>(a.dq) + at.flat(r) * a.dim;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+            const int col = 2 * tx + 32 * (c / 2) + c % 2;
+            if (col < a.dim) attn_store(out + col, dq[i][c] * a.scale);
+        }
+    }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) key_gradient_kernel(const Attn a) {
+    extern __shared__ float smem[];
+    float* ks = smem;
+    float* vs = ks + 64 * (DP + 4);
+    float* qs = vs + 64 * (DP + 4);
+    float* gs = qs + 64 * (DP + 4);
+    float* ps = gs + 64 * (DP + 4);
+    float* ds = ps + 64 * (64 + 4);
+    __shared__ float lse2[64], delta[64];
+    __shared__ int64_t limit[64];
+    const int b = find_sequence(a.key_offsets, a.batch, kN, blockIdx.x);
+    const Span s = load_span(a, b);
+    const int64_t n0 = (int64_t(blockIdx.x) - (a.key_offsets[b] / kN + b)) * kN;
+    if (n0 < 0 || n0 >= s.slot) return;
+    const int n = int(max(int64_t(0), min(int64_t(kN), s.keys - n0)));
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    load_tile<T, DP>(ks, static_cast<const T*>(a.k) + (s.key0 + n0) * a.k_row + blockIdx.y * a.k_head, n, a.dim,
+                     [&](int r) { return r * a.k_row; });
+    load_tile<T, DP>(vs, static_cast<const T*>(a.v) + (s.key0 + n0) * a.v_row + blockIdx.y * a.v_head, n, a.dim,
+                     [&](int r) { return r * a.v_row; });
+    float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
+    const int per_tile = kM / a.group;
+    const float scale = a.scale * kLog2e;
+    // the first token that sees key n0
+    const int64_t first = a.causal ? max(int64_t(0), n0 + s.rows - s.keys) : 0;
+    for (int64_t token0 = n > 0 ? first / per_tile * per_tile : s.rows; token0 < s.rows; token0 += per_tile) {
+        const int tokens = int(min(int64_t(per_tile), s.rows - token0)), rows = tokens * a.group;
+        const Rows at{s.row0 + token0, a.group, int(blockIdx.y) * a.group, a.hq};
+        __syncthreads();
+        load_tile<T, DP>(qs, static_cast<const T*>(a.q), rows, a.dim,
+                         [&](int r) { return at.at(r, a.q_row, a.q_head); });
+        load_tile<T, DP>(gs, static_cast<const T*>(a.g), rows, a.dim,
+                         [&](int r) { return at.at(r, a.g_row, a.g_head); });
+        if (threadIdx.x < 64) {
+            const int r = threadIdx.x;
+            lse2[r] = r < rows ? a.lse[at.flat(r)] * kLog2e : -INFINITY;
+            limit[r] = lse2[r] != -INFINITY ? seen(s, a.causal, token0 + r / a.group) : 0;
+            delta[r] = r < rows ? a.delta[at.flat(r)] : 0.0f;
+        }
+        __syncthreads();
+        float x[4][4] = {}, y[4][4] = {};
+        dots<DP>(ks, qs, ty, tx, x);
+        dots<DP>(vs, gs, ty, tx, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = ty + 16 * i, r = tx + 16 * j;
+                const bool there = key < n && n0 + key < limit[r];
+                const float p = weight_of(x[i][j], scale, lse2[r], there);
+                ps[key * (64 + 4) + r] = p;
+                ds[key * (64 + 4) + r] = there ? p * (y[i][j] - delta[r]) : 0.0f;
+            }
+        __syncthreads();
+        weigh<DP>(ps, gs, ty, tx, dv);
+        weigh<DP>(ds, qs, ty, tx, dk);
+    }
+    // every row of the slot is written: keys that no query may see have zero gradients
+    const int out_rows = int(min(int64_t(kN), s.slot - n0));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int key = ty + 16 * i;
+        if (key >= out_rows) continue;
+        const int64_t flat = ((s.key0 + n0 + key) * a.hk + blockIdx.y) * a.dim;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+            const int col = 2 * tx + 32 * (c / 2) + c % 2;
+            if (col < a.dim) {
+                attn_store(static_cast<T*>(a.dk) + flat + col, dk[i][c] * a.scale);
+                attn_store(static_cast<T*>(a.dv) + flat + col, dv[i][c]);
+            }
+        }
+    }
+}
+
+template <typename T, int DP>
+fmd_status forward_typed(const Attn& a, cudaStream_t s) {
+    const size_t bytes = size_t(3 * 64 * (DP + 4) + 64 * 68) * sizeof(float);
+    fmd_status st = grant_dynamic_smem((const void*)forward_kernel<T, DP>, bytes);
+    if (st != FMD_OK) return st;
+    const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kM / a.group)), unsigned(a.hk));
+    forward_kernel<T, DP><<<grid, kThreads, bytes, s>>>(a);
+    return check_launch();
+}
+
+template <typename T, int DP>
+fmd_status backward_typed(const Attn& a, cudaStream_t s) {
+    const size_t bytes = size_t(4 * 64 * (DP + 4) + 2 * 64 * 68) * sizeof(float);
+    fmd_status st = grant_dynamic_smem((const void*)query_gradient_kernel<T, DP>, bytes);
+    if (st == FMD_OK) st = grant_dynamic_smem((const void*)key_gradient_kernel<T, DP>, bytes);
+    if (st != FMD_OK) return st;
+    if (a.dq != nullptr && a.rows > 0) {
+        const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kM / a.group)), unsigned(a.hk));
+        query_gradient_kernel<T, DP><<<grid, kThreads, bytes, s>>>(a);
+        if ((st = check_launch()) != FMD_OK) return st;
+    }
+    if (a.dk != nullptr && a.keys > 0) {
+        const dim3 grid(unsigned(tile_bound(a.keys, a.batch, kN)), unsigned(a.hk));
+        key_gradient_kernel<T, DP><<<grid, kThreads, bytes, s>>>(a);
+        st = check_launch();
+    }
+    return st;
+}
+
+template <typename T>
+fmd_status forward_sized(const Attn& a, cudaStream_t s) {
+    return a.dim <= 32 ? forward_typed<T, 32>(a, s) : a.dim <= 64 ? forward_typed<T, 64>(a, s)
+                                                                  : forward_typed<T, 128>(a, s);
+}
+
+template <typename T>
+fmd_status backward_sized(const Attn& a, cudaStream_t s) {
+    return a.dim <= 32 ? backward_typed<T, 32>(a, s) : a.dim <= 64 ? backward_typed<T, 64>(a, s)
+                                                                   : backward_typed<T, 128>(a, s);
+}
+
+}  // namespace
+
+fmd_status attention_forward_simt(const Attn& a, int type, cudaStream_t s) {
+    return type == FMD_F32 ? forward_sized<float>(a, s) : forward_sized<__nv_bfloat16>(a, s);
+}
+
+fmd_status attention_backward_simt(const Attn& a, int type, cudaStream_t s) {
+    return type == FMD_F32 ? backward_sized<float>(a, s) : backward_sized<__nv_bfloat16>(a, s);
+}
+
+}  // namespace fmd

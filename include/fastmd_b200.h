@@ -1040,6 +1040,85 @@ FMD_API fmd_status fmd_nhc_post_pre_force(double* state, const double* masses, c
                                           int32_t f32_kick, const float* forces_f32, const double* forces_f64,
                                           const double* energy, float* positions32, void* stream);
 
+/* ------------------------------------- sequence operators (packed rows) */
+
+/* element types of the sequence operators */
+#define FMD_F32 0
+#define FMD_BF16 1
+
+/* One side (queries or keys) of fmd_head_rotary. x [rows, heads, dim] with
+ * unit stride inside a head; w [dim] or NULL (no norm); forward: y, the
+ * output, [rows, heads, dim] contiguous. Backward: g, the output's gradient,
+ * with its own strides; y, the input's gradient; dw [dim], the weight's
+ * gradient, in the weight's type (NULL: not written). heads = 0: no such side. */
+typedef struct fmd_head_rotary_side {
+    const void* x;
+    const void* g;
+    void* y;
+    const void* w;
+    void* dw;
+    int64_t row_stride, head_stride, g_row_stride, g_head_stride;
+    int32_t heads, _pad;
+} fmd_head_rotary_side;
+
+/* Workspace of the backward pass with weights. */
+FMD_API fmd_status fmd_head_rotary_workspace_bytes(int32_t dim, size_t* bytes);
+
+/* RMS norm of each head of queries and keys (sides[0], sides[1]) and the
+ * rotation of its first `rot` values by the row's position, or with backward
+ * = 1 the gradients of both:
+ *   y = turn(w x / sqrt(mean(x^2) + eps)), pairs (p, p + rot/2), or with
+ *   interleaved (2p, 2p + 1); cos, sin [table, rot / 2] float32.
+ * dim and rot multiples of 8, at most 128; FP32 arithmetic, rounded once. A
+ * position outside [0, table) raises FMD_FLAG_INDEX_RANGE and turns by
+ * cos = sin = 0. Deterministic. Bases and row and head strides must be
+ * multiples of 16 bytes, else FMD_ERR_UNSUPPORTED. No reference counterpart. */
+FMD_API fmd_status fmd_head_rotary(const fmd_head_rotary_side* sides, int32_t type, int32_t weight_type, int64_t rows,
+                                   int32_t dim, int32_t rot, int32_t interleaved, float eps, const int64_t* positions,
+                                   const float* cos, const float* sin, int64_t table, int32_t backward,
+                                   void* workspace, size_t workspace_bytes, int32_t* flags, void* stream);
+
+/* A packed-attention problem: sequence b has the tokens offsets[b] ..
+ * offsets[b + 1] - 1 of q [rows, heads, dim] and the keys key_offsets[b] ..
+ * of k, v [keys, key_heads, dim], as many as key_counts[b] says (NULL: up to
+ * key_offsets[b + 1]; the rest of the slot is never used). Query head h reads
+ * key head h / (heads / key_heads). causal: token t of m sees the first
+ * t + 1 + n - m of n keys. Offsets and counts live on the device; they start
+ * at 0, do not fall and end at rows and keys, and counts fit their slots:
+ * else FMD_FLAG_INDEX_RANGE is raised, nothing outside the arrays is touched
+ * and the results are unspecified. dim a multiple of 8 up to 128,
+ * heads / key_heads at most 64; strides in elements, unit stride inside a
+ * head; bases and strides multiples of 16 bytes, else FMD_ERR_UNSUPPORTED. */
+typedef struct fmd_attention {
+    const void* q;
+    const void* k;
+    const void* v;
+    const int64_t* offsets;
+    const int64_t* key_offsets;
+    const int64_t* key_counts;
+    int64_t rows, keys;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    float scale;
+    int32_t type, batch, heads, key_heads, dim, causal, _pad;
+} fmd_attention;
+
+/* out [rows, heads, dim] = softmax(scale q k^T) v over the keys each row
+ * sees, and lse [rows, heads] = the logarithm of the softmax's denominator
+ * (NULL: not written). A row that sees no key gets out = 0, lse = -inf. No
+ * reference counterpart (nor has the backward pass). */
+FMD_API fmd_status fmd_packed_attention(const fmd_attention* problem, void* out, float* lse, int32_t* flags,
+                                        void* stream);
+
+/* Gradients of q (dq, [rows, heads, dim], or NULL) and of k and v (dk, dv,
+ * [keys, key_heads, dim], or both NULL; slot rows behind a count get zeros)
+ * from the output's gradient g (strides g_row, g_head) and lse's, glse
+ * (NULL: none); out and lse are the forward pass's. delta [rows, heads] is
+ * workspace. Deterministic. */
+FMD_API fmd_status fmd_packed_attention_bwd(const fmd_attention* problem, const void* out, const float* lse,
+                                            const void* g, int64_t g_row, int64_t g_head, const float* glse,
+                                            float* delta, void* dq, void* dk, void* dv, int32_t* flags,
+                                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,374 @@
+"""Packed attention and its gradients against the formulas in 64 bits (GPU), and the refusals.
+
+The bounds follow the roundings: u = half the distance of neighbouring values of the stored type (2^-24 or 2^-8
+relative), t = the rounding of the weights p and their gradients for the products (2^-8 in 16 bits, none in 32), and
+e = the error of a score in FP32, at most (dim + 4) 2^-24 sum |q||k| scale, with that of exp2 and of the row sum."""
+import math
+
+import pytest
+import torch
+
+from fastmd_b200 import _lib
+from fastmd_b200.packed_attention import packed_attention
+
+gpu = pytest.mark.gpu
+F32, B16 = torch.float32, torch.bfloat16
+E32 = 2.0 ** -24
+
+
+def reference(q, k, v, offsets, key_offsets, counts, causal, scale, g=None, glse=None):
+    """Outputs, gradients and the error bound of each, in 64 bits, a sequence and a head at a time."""
+    unit = E32 if q.dtype == F32 else 2.0 ** -8
+    split = 0.0 if q.dtype == F32 else 2.0 ** -8
+    dim, group = q.shape[2], q.shape[1] // k.shape[1]
+    q, k, v = q.double(), k.double(), v.double()
+    out = {n: torch.zeros_like(t) for n, t in dict(out=q, dq=q, dk=k, dv=v).items()}
+    err = {n: torch.zeros_like(t) for n, t in out.items()}
+    lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64, device=q.device)
+    lse_err = torch.zeros_like(lse)
+    for b in range(len(offsets) - 1):
+        r = slice(offsets[b], offsets[b + 1])
+        n = counts[b] if counts is not None else key_offsets[b + 1] - key_offsets[b]
+        c = slice(key_offsets[b], key_offsets[b] + n)
+        m = r.stop - r.start
+        if m == 0 or n == 0:
+            continue
+        seen = torch.ones(m, n, dtype=torch.bool, device=q.device)
+        if causal:
+            seen = torch.arange(n, device=q.device) <= torch.arange(m, device=q.device)[:, None] + n - m
+        for h in range(q.shape[1]):
+            x, y, z = q[r, h], k[c, h // group], v[c, h // group]
+            s = torch.where(seen, scale * (x @ y.T), -math.inf)
+            top = s.amax(1, keepdim=True).nan_to_num(neginf=0.0)
+            p = torch.exp(s - top)
+            l = p.sum(1, keepdim=True)
+            lse[r, h] = (top + l.log())[:, 0]
+            p = p / l.clamp(min=1e-300)
+            # a score's error, the rounding of its difference to the maximum, exp2's (2^-22) and the row sum's
+            e = E32 * ((dim + 4) * scale * (x.abs() @ y.abs().T) + 4 * s.abs().nan_to_num(posinf=0.0) + 8)
+            e = e + (e * p).sum(1, keepdim=True) + E32 * (4 + n / 16)
+            o = p @ z
+            out["out"][r, h] = o
+            err["out"][r, h] = unit * o.abs() + (p * (split + e)) @ z.abs() + E32 * (n / 16) * (p @ z.abs())
+            lse_err[r, h] = (e * p).sum(1) + E32 * (4 + n / 16 + 4 * lse[r, h].abs().nan_to_num(posinf=0.0))
+            if g is None:
+                continue
+            w = g[r, h].double()
+            dp = w @ z.T
+            dp_err = E32 * (dim + 4) * (w.abs() @ z.abs().T)
+            delta = (w * o).sum(1, keepdim=True)
+            delta_err = (w.abs() * err["out"][r, h]).sum(1, keepdim=True) + E32 * dim * (w * o).abs().sum(1, keepdim=True)
+            if glse is not None:
+                delta = delta - glse[r, h, None].double()
+            ds = p * (dp - delta)
+            # a backward weight is exp(s - lse): the errors of both
+            we = e + lse_err[r, h, None]
+            ds_err = ds.abs() * (split + we) + p * (dp_err + delta_err + 4 * E32 * (dp.abs() + delta.abs()))
+            out["dv"][c, h // group] += p.T @ w
+            err["dv"][c, h // group] += (p * (split + we)).T @ w.abs() + E32 * (m / 16) * (p.T @ w.abs())
+            out["dq"][r, h] = scale * (ds @ y)
+            err["dq"][r, h] = scale * ((ds_err + E32 * (n / 16) * ds.abs()) @ y.abs())
+            out["dk"][c, h // group] += scale * (ds.T @ x)
+            err["dk"][c, h // group] += scale * ((ds_err + E32 * (m / 16) * ds.abs()).T @ x.abs())
+    for n in ("dq", "dk", "dv"):
+        err[n] += unit * (out[n].abs() + err[n])
+    return out, err, lse, lse_err
+
+
+def check(got, want, err, what):
+    got = got.double()
+    assert bool(torch.isfinite(got).all()), what
+    over = ((got - want).abs() - err - 1e-30).amax() if got.numel() else torch.tensor(0.0)
+    ratio = ((got - want).abs() / (err + 1e-30)).amax() if got.numel() else torch.tensor(0.0)
+    assert float(over) <= 0, f"{what}: {float(ratio):.3g} times its bound"
+
+
+def starts(sizes):
+    return [sum(sizes[:i]) for i in range(len(sizes) + 1)]
+
+
+def make(rows, slots, hq, hk, dim, dtype, seed=0, spread=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    q = (torch.randn(sum(rows), hq, dim, generator=gen) * spread).to(dtype).cuda()
+    k, v = (torch.randn(sum(slots), hk, dim, generator=gen).to(dtype).cuda() for _ in range(2))
+    g = torch.randn(q.shape, generator=gen).to(dtype).cuda()
+    return q, k, v, g
+
+
+def on_device(values):
+    return torch.tensor(values, dtype=torch.int64, device="cuda")
+
+
+def run_case(rows, slots, counts, hq, hk, dim, dtype, causal, seed=0, spread=1.0, lse_grad=False):
+    q, k, v, g = make(rows, slots, hq, hk, dim, dtype, seed, spread)
+    ro, ko = starts(rows), starts(slots)
+    if counts is not None:  # what lies behind a count is never used
+        for b, n in enumerate(counts):
+            k[ko[b] + n:ko[b + 1]] = float("nan")
+            v[ko[b] + n:ko[b + 1]] = float("inf")
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    scale = dim ** -0.5
+    out, lse = packed_attention(q, k, v, on_device(ro), on_device(ko), None if counts is None else on_device(counts),
+                                causal=causal, return_lse=True)
+    glse = torch.randn(lse.shape, generator=torch.Generator().manual_seed(9)).cuda() if lse_grad else None
+    grads = torch.autograd.grad((out, lse) if lse_grad else out, leaves, (g, glse) if lse_grad else g)
+    alone = packed_attention(q.detach(), k.detach(), v.detach(), on_device(ro), on_device(ko),
+                             None if counts is None else on_device(counts), causal=causal)
+    clean = [torch.nan_to_num(t.detach(), 0.0, 0.0, 0.0) if counts is not None else t.detach() for t in (k, v)]
+    want, err, want_lse, lse_err = reference(q.detach(), *clean, ro, ko, counts, causal, scale, g, glse)
+    check(out.detach(), want["out"], err["out"], "out")
+    check(alone, want["out"], err["out"], "out without gradients")
+    empty = torch.isinf(want_lse)
+    assert torch.equal(torch.isinf(lse), empty)
+    check(lse.detach().masked_fill(empty, 0.0), want_lse.masked_fill(empty, 0.0), lse_err, "lse")
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        check(got, want[name], err[name], name)
+
+
+SEQUENCES = {
+    "one": ([1], [1], None),
+    "atoms": ([135, 135, 135], [135, 135, 135], None),
+    "edges": ([127, 128, 129, 1, 0, 255], [127, 128, 129, 1, 0, 255], None),
+    "cross": ([5, 64, 0, 3, 200], [300, 65, 17, 0, 131], None),
+    "more_rows": ([200, 70], [90, 70], None),  # with causal the first 110 rows see nothing
+    "step": ([1, 1, 1, 1], [400, 400, 400, 400], [400, 1, 129, 0]),
+    "chunk": ([33, 33, 7], [700, 700, 700], [700, 40, 260]),
+    "long": ([1100], [1100], None),
+}
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+@pytest.mark.parametrize("causal", [False, True], ids=["all", "causal"])
+@pytest.mark.parametrize("name", list(SEQUENCES))
+def test_sequences(cuda, name, causal, dtype):
+    rows, slots, counts = SEQUENCES[name]
+    run_case(rows, slots, counts, 4, 2, 64, dtype, causal)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+@pytest.mark.parametrize("hq,hk,dim", [(1, 1, 8), (3, 1, 32), (8, 1, 128), (5, 5, 96), (6, 2, 72), (16, 4, 40),
+                                       (64, 1, 16), (24, 2, 128), (2, 2, 120)])
+def test_heads_and_sizes(cuda, hq, hk, dim, dtype):
+    run_case([70, 1, 190], [70, 1, 190], None, hq, hk, dim, dtype, True, seed=hq + dim)
+    run_case([2, 1], [150, 333], [150, 201], hq, hk, dim, dtype, True, seed=hq + dim, lse_grad=True)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+def test_large_scores(cuda, dtype):
+    """Scores of some hundreds: the running maximum moves by far more than a weight's range."""
+    run_case([300, 40], [300, 40], None, 2, 1, 64, dtype, False, spread=60.0)
+    run_case([1, 3], [900, 257], None, 4, 2, 64, dtype, False, spread=60.0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+def test_layouts_are_the_packed_ones(cuda, dtype):
+    """Views of a fused projection, a head-major tensor and an unaligned base give the packed tensor's bits."""
+    rows, hq, hk, dim = 150, 4, 2, 64
+    gen = torch.Generator().manual_seed(5)
+    fused = torch.randn(rows, hq + 2 * hk, dim, generator=gen).to(dtype).cuda()
+    parts = fused.split((hq, hk, hk), 1)
+    offsets = on_device([0, 100, 150])
+    want = packed_attention(*[p.contiguous() for p in parts], offsets, causal=True)
+    assert torch.equal(packed_attention(*parts, offsets, causal=True), want)
+    turned = [p.transpose(0, 1).contiguous().transpose(0, 1) for p in parts]
+    assert torch.equal(packed_attention(*turned, offsets, causal=True), want)
+    columns = [p.transpose(1, 2).contiguous().transpose(1, 2) for p in parts]
+    assert torch.equal(packed_attention(*columns, offsets, causal=True), want)
+    odd = torch.empty(rows * hq * dim + 1, dtype=dtype, device="cuda")
+    odd[1:] = parts[0].reshape(-1)
+    assert torch.equal(packed_attention(odd[1:].view(rows, hq, dim), *parts[1:], offsets, causal=True), want)
+    leaves = [p.detach().requires_grad_() for p in parts]
+    out = packed_attention(*leaves, offsets, causal=True)
+    spread_grad = torch.autograd.grad(out.sum(), leaves)  # an expanded gradient of stride 0
+    out = packed_attention(*leaves, offsets, causal=True)
+    full_grad = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    assert all(torch.equal(a, b) for a, b in zip(spread_grad, full_grad))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+def test_neighbours_do_not_matter(cuda, dtype):
+    """A sequence's bits are its own: the others may hold NaN and infinities, and more of them may follow."""
+    rows = [130, 77, 45]
+    q, k, v, g = make(rows, rows, 4, 2, 64, dtype, seed=3)
+    ro = starts(rows)
+
+    def whole(q, k, v, g):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = packed_attention(*leaves, on_device(ro), causal=False)
+        return out.detach(), *torch.autograd.grad(out, leaves, g)
+
+    want = whole(q, k, v, g)
+    for t, bad in ((q, "nan"), (k, "inf"), (v, "nan"), (g, "inf")):
+        t[:130] = float(bad)
+        t[207:] = float(bad)
+    got = whole(q, k, v, g)
+    for a, b in zip(got, want):
+        assert torch.equal(a[130:207], b[130:207])
+
+
+@gpu
+def test_non_finite_values_stay_visible(cuda):
+    """A row with a NaN query is NaN; the rows of other heads and tokens are not touched by it."""
+    q, k, v, _ = make([40], [40], 2, 2, 32, F32)
+    want = packed_attention(q, k, v, on_device([0, 40]))
+    q[7, 1] = float("nan")
+    got = packed_attention(q, k, v, on_device([0, 40]))
+    assert bool(torch.isnan(got[7, 1]).all())
+    q[7, 1], got[7, 1], want[7, 1] = 0, 0, 0
+    assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+def test_repeatable(cuda, dtype):
+    rows = [700, 3, 512]
+    q, k, v, g = make(rows, rows, 8, 2, 64, dtype)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    runs = []
+    for _ in range(2):
+        out = packed_attention(*leaves, on_device(starts(rows)), causal=True)
+        runs.append([out.detach(), *torch.autograd.grad(out, leaves, g)])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@gpu
+def test_gradient_against_differences(cuda):
+    """Directional derivatives of sum(out c) + sum(lse d) by central differences of the FP32 operator: a step of
+    2^-6 leaves a truncation near h^2 and a rounding near 2^-24 / h of the sum of the terms' sizes."""
+    rows = [9, 5]
+    q, k, v, c = make(rows, rows, 2, 1, 16, F32, seed=11)
+    gen = torch.Generator().manual_seed(12)
+    d = torch.randn(14, 2, generator=gen).cuda()
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    offsets, h = on_device(starts(rows)), 2.0 ** -6
+
+    def value(args):
+        out, lse = packed_attention(*args, offsets, causal=True, return_lse=True)
+        return (out * c).double().sum() + (lse * d).double().sum()
+
+    grads = torch.autograd.grad(value(leaves), leaves)
+    for i in range(3):
+        step = torch.randn(leaves[i].shape, generator=gen).cuda()
+        up, down = ([t.detach() + sign * h * step if j == i else t.detach() for j, t in enumerate(leaves)]
+                    for sign in (1, -1))
+        slope = float(value(up) - value(down)) / (2 * h)
+        size = float((grads[i].abs() * step.abs()).sum())
+        assert abs(slope - float((grads[i] * step).double().sum())) <= 2.0 ** -9 * size
+
+
+@gpu
+def test_only_what_is_asked_for(cuda):
+    q, k, v, g = make([50], [50], 2, 1, 32, B16)
+    offsets = on_device([0, 50])
+    both = [t.clone().requires_grad_() for t in (q, k, v)]
+    want = torch.autograd.grad(packed_attention(*both, offsets), both, g)
+    alone = q.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(packed_attention(alone, k, v, offsets), alone, g)[0], want[0])
+    alone = v.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(packed_attention(q, k, alone, offsets), alone, g)[0], want[2])
+    lse_only = q.clone().requires_grad_()
+    _, lse = packed_attention(lse_only, k, v, offsets, return_lse=True)
+    (dq,) = torch.autograd.grad(lse.sum(), lse_only)  # the gradient of lse alone: the mean key
+    p = torch.softmax(32 ** -0.5 * torch.einsum("thd,sd->ths", q.double(), k[:, 0].double()), -1)
+    want = 32 ** -0.5 * torch.einsum("ths,sd->thd", p, k[:, 0].double())
+    assert float((dq.double() - want).abs().max()) <= 2.0 ** -6 * float(want.abs().max())
+
+
+@gpu
+def test_captured_in_a_graph(cuda):
+    """A captured call reads offsets and counts when it is replayed."""
+    q, k, v, _ = make([1, 1], [300, 300], 4, 2, 64, B16)
+    counts = on_device([10, 300])
+    args = (q, k, v, on_device([0, 1, 2]), on_device([0, 300, 600]), counts)
+    packed_attention(*args, causal=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = packed_attention(*args, causal=True)
+    for n in ([10, 300], [299, 1], [0, 150]):
+        counts.copy_(on_device(n))
+        graph.replay()
+        assert torch.equal(out, packed_attention(*args, causal=True))
+
+
+@gpu
+def test_another_stream(cuda):
+    q, k, v, _ = make([100], [100], 2, 2, 64, B16)
+    offsets = on_device([0, 100])
+    want = packed_attention(q, k, v, offsets)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = packed_attention(q, k, v, offsets)
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+def test_bad_offsets_are_flagged(cuda, dtype):
+    """Offsets and counts that leave the arrays are held inside and flagged."""
+    q, k, v, _ = make([60], [60], 2, 2, 32, dtype)
+    word = _lib.flags_word(q.device)
+    good = on_device([0, 30, 60])
+    for offsets, key_offsets, counts in ((on_device([0, 30, 70]), good, None), (on_device([0, -5, 60]), good, None),
+                                         (good, on_device([0, 90, 60]), None), (good, good, on_device([31, 30])),
+                                         (good, good, on_device([-1, 30])), (on_device([3, 30, 60]), good, None),
+                                         (good, on_device([0, 30, 50]), None)):
+        word.zero_()
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = packed_attention(*leaves, offsets, key_offsets, counts)
+        torch.autograd.grad(out.sum(), leaves)
+        assert int(word.item()) & 1
+    word.zero_()
+    packed_attention(q, k, v, good)
+    assert int(word.item()) == 0
+
+
+@gpu
+def test_empty(cuda):
+    q, k, v, _ = make([0], [0], 2, 1, 32, B16)
+    assert packed_attention(q, k, v, on_device([0])).shape == (0, 2, 32)
+    assert packed_attention(q, k, v, on_device([0, 0, 0])).shape == (0, 2, 32)
+    q, k, v, _ = make([0], [40], 2, 1, 32, B16)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = packed_attention(*leaves, on_device([0, 0]), on_device([0, 40]))
+    grads = torch.autograd.grad(out.sum(), leaves)
+    assert not grads[1].any() and not grads[2].any()
+    q, k, v, _ = make([40], [0], 2, 1, 32, F32)
+    out, lse = packed_attention(q, k, v, on_device([0, 40]), on_device([0, 0]), return_lse=True)
+    assert not out.any() and bool((lse == -math.inf).all())
+
+
+@gpu
+def test_refusals(cuda):
+    q, k, v, _ = make([6], [6], 4, 2, 32, F32)
+    offsets = on_device([0, 6])
+    with pytest.raises(_lib.FastMDLibraryError):
+        packed_attention(q, k.cpu(), v, offsets)
+    for bad in (dict(q=q.half(), k=k.half(), v=v.half()), dict(k=k.bfloat16()), dict(v=v[:5]), dict(q=q[0]),
+                dict(q=q[..., :12], k=k[..., :12], v=v[..., :12]), dict(q=q[:, :3]), dict(offsets=offsets.int()),
+                dict(offsets=offsets[None]), dict(q=q[:5]), dict(offsets=offsets[:1]),
+                dict(key_offsets=on_device([0, 3, 6])), dict(key_counts=on_device([3, 3])),
+                dict(q=q.repeat(1, 33, 1))):
+        with pytest.raises(ValueError):
+            packed_attention(**(dict(q=q, k=k, v=v, offsets=offsets) | bad))
+
+
+def test_abi_refuses_on_the_host():
+    lib = _lib.lib()
+    base = dict(q=1 << 20, k=1 << 20, v=1 << 20, offsets=1 << 20, key_offsets=1 << 20, key_counts=None, rows=0, keys=0,
+                q_row=64, q_head=64, k_row=64, k_head=64, v_row=64, v_head=64, scale=0.125, type=1, batch=1, heads=1,
+                key_heads=1, dim=64, causal=0)
+    assert lib.fmd_packed_attention(_lib.FmdAttention(**base), None, None, None, None) == 0  # no rows
+    for bad in (dict(type=2), dict(heads=3, key_heads=2), dict(key_heads=0), dict(dim=12), dict(dim=136),
+                dict(rows=-1), dict(batch=0, rows=1), dict(rows=1, q=None), dict(keys=1, v=None),
+                dict(offsets=None), dict(heads=65)):
+        assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | bad)), None, None, None, None) == 1
+    for bad in (dict(rows=1, q=(1 << 20) + 2), dict(keys=1, k_row=65), dict(rows=1, q_head=4), dict(rows=1 << 40)):
+        assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | bad)), 1 << 20, None, None, None) == 3
+    assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | dict(rows=1))), None, None, None, None) == 1
