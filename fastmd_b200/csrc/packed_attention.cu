@@ -92,6 +92,7 @@ fmd_status fmd_packed_attention(const fmd_attention* problem, void* out, float* 
     a.out = out;
     a.lse = lse;
     a.flags = flags;
+    if (problem->type == FMD_BF16) return attention_forward_mma(a, as_stream(stream));
     return attention_forward_simt(a, problem->type, as_stream(stream));
 }
 

@@ -1,0 +1,390 @@
+// Packed attention in bfloat16 on the tensor cores: the forward pass.
+//
+//   s = q k^T;  per row a reference m and a sum l over key tiles of 128:
+//   p = 2^(c s - m), c = scale log2 e;  l += sum p;  o += p v;  out = o / l,  lse = ln 2 (m + log2 l)
+//
+// The same out and lse follow for any reference m, so m follows the row's maximum loosely: it moves (and o and l are
+// multiplied by 2^(m_old - m_new)) only when the maximum has grown by more than kSlack, which after the first tile is
+// rare. p stays below 2^kSlack, in range for bfloat16 and the FP32 sums.
+//
+// A block owns NT tiles of 128 packed rows of one key head and walks the key tiles they see:
+//   warp 0       TMA: q once, then k and v tiles through a ring of shared-memory slots
+//   warp 1       one thread issues the products: S_t = q k^T (both from shared memory, into TMEM), O_t += p v (p from
+//                TMEM); for two tiles in turn, so the tensor cores work on one tile while the other is exponentiated
+//   warps 2, 3   zero the rows behind the last key (another sequence's or an unused slot's: 0 * NaN must not happen)
+//   then 4 warps per tile: thread = row. Scores from TMEM, maximum, exp2, sum, p back over the scores as bfloat16;
+//                o rescaled in TMEM when m moves; at the end o / l to memory.
+// A score tile is only issued after the product that read the weights at its place, by the same thread, and commits
+// cover all products before them: "scores ready" therefore also says that o is at rest. The last key tile's products
+// are as narrow as its keys (multiples of 16).
+// Every wait is bounded: on expiry the block raises FMD_FLAG_WAIT_TIMEOUT, waits (bounded) for its copies and
+// products in flight, frees its TMEM and returns.
+
+#include "packed_attention_mma.cuh"
+
+namespace fmd {
+namespace {
+
+constexpr float kSlack = 8.0f;
+
+template <int KS, int NT>
+struct Shape {
+    static constexpr int kDim = 16 * KS;  // of a head, rounded up; TMA fills the rest with zeros
+    static constexpr int kPanels = (KS + 3) / 4;
+    static constexpr uint32_t kTileBytes = kPanels * kPanelBytes;
+    // NT = 1: two blocks share an SM (96 or 80 KB each); NT = 2: one block, and the ring deep
+    static constexpr int kSlots = NT == 1 ? (kPanels == 2 ? 2 : 4) : (kPanels == 2 ? 4 : 8);
+    static constexpr int kThreads = 128 + 128 * NT;
+    static constexpr uint32_t kTmem = NT == 1 ? 256 : 512;
+    static constexpr uint32_t kO = NT * 128;  // first column of the outputs, behind the score tiles
+    static constexpr size_t kBytes = size_t(NT + kSlots) * kTileBytes + 1024 + 256;
+};
+
+template <int KS, int NT>
+struct Ctrl {
+    uint64_t q_full;
+    uint64_t full[Shape<KS, NT>::kSlots], empty[Shape<KS, NT>::kSlots];
+    uint64_t scores[NT], weights[NT], done[NT];
+    uint64_t tail_here, tail;  // the last v tile has landed; its rows behind the last key are zeros
+    uint64_t drain;
+    uint32_t tmem;
+    int32_t abort;
+};
+
+struct Maps {
+    CUtensorMap q, k, v;
+};
+
+template <int KS, int NT>
+__global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
+    forward_kernel(const __grid_constant__ Maps maps, const Attn a) {
+    using S = Shape<KS, NT>;
+    extern __shared__ unsigned char raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* ring = smem + NT * S::kTileBytes;
+    __shared__ Ctrl<KS, NT> ctl;
+    volatile int32_t* abort = &ctl.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // the longest rows of a causal sequence are its last: they go first
+    const int64_t index = gridDim.x - 1 - blockIdx.x;
+    const int per_tile = kTile / a.group, per_block = NT * per_tile;
+    const int b = find_sequence(a.offsets, a.batch, per_block, index);
+    const Span s = load_span(a, b);
+    const int64_t token0 = (index - (a.offsets[b] / per_block + b)) * per_block;
+    if (token0 < 0 || token0 >= s.rows) return;
+    const int head = blockIdx.y;
+    int tokens[NT], ends[NT], counts[NT];  // tokens of each tile, the keys its last one sees, key tiles
+    int last = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        tokens[t] = int(max(int64_t(0), min(int64_t(per_tile), s.rows - token0 - t * per_tile)));
+        ends[t] = tokens[t] > 0 ? int(seen(s, a.causal, token0 + t * per_tile + tokens[t] - 1)) : 0;
+        counts[t] = (ends[t] + kTile - 1) / kTile;
+        last = max(last, counts[t]);
+    }
+    const int keys = int(s.keys);
+    // the last key tile read holds rows behind the sequence's last key
+    const bool tail = last > 0 && keys < last * kTile;
+
+    if (threadIdx.x == 0) {
+        mbar_init(&ctl.q_full, 1);
+        for (int i = 0; i < S::kSlots; ++i) {
+            mbar_init(&ctl.full[i], 1);
+            mbar_init(&ctl.empty[i], 1);
+        }
+        for (int t = 0; t < NT; ++t) {
+            mbar_init(&ctl.scores[t], 1);
+            mbar_init(&ctl.weights[t], 128);
+            mbar_init(&ctl.done[t], 1);
+        }
+        mbar_init(&ctl.tail_here, 1);
+        mbar_init(&ctl.tail, 64);
+        mbar_init(&ctl.drain, 1);
+        ctl.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&ctl.tmem)),
+                     "n"(S::kTmem)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl.tmem;
+
+    if (warp == 0) {
+        if (lane == 0 && last > 0) {
+            const uint32_t q_bytes = uint32_t(S::kPanels) * 128u * uint32_t(per_tile * a.group);
+            int tiles = 0;
+            for (int t = 0; t < NT; ++t) tiles += counts[t] > 0;
+            mbar_expect_tx(&ctl.q_full, q_bytes * tiles);
+            for (int t = 0; t < NT; ++t)
+                if (counts[t] > 0)
+                    for (int p = 0; p < S::kPanels; ++p)
+                        tma_load_4d(su32(smem + t * S::kTileBytes + p * kPanelBytes), &maps.q, &ctl.q_full, p * 64, 0,
+                                    head, int(s.row0 + token0) + t * per_tile);
+            int slot = 0, armed = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int i = 0; i < 2 * last; ++i) {  // k0, v0, k1, v1, ..
+                if (!mbar_wait(&ctl.empty[slot], phase ^ 1u, abort)) {
+                    ok = false;
+                    break;
+                }
+                mbar_expect_tx(&ctl.full[slot], S::kTileBytes);
+                for (int p = 0; p < S::kPanels; ++p)
+                    tma_load_4d(su32(ring + slot * S::kTileBytes + p * kPanelBytes), i & 1 ? &maps.v : &maps.k,
+                                &ctl.full[slot], p * 64, 0, head, int(s.key0) + (i >> 1) * kTile);
+                armed = i + 1;
+                if (++slot == S::kSlots) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (!ok) {  // the copies in flight land before the block ends
+                mbar_wait(&ctl.q_full, 0, abort, true);
+                for (int i = max(0, armed - S::kSlots); i < armed; ++i)
+                    mbar_wait(&ctl.full[i % S::kSlots], uint32_t(i / S::kSlots) & 1u, abort, true);
+            } else {  // the last slots' releases land before the block ends
+                for (int i = 0; i < S::kSlots && mbar_wait(&ctl.empty[slot], phase ^ 1u, abort); ++i)
+                    if (++slot == S::kSlots) {
+                        slot = 0;
+                        phase ^= 1u;
+                    }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && last > 0) {
+            const uint32_t o_desc = bf16_idesc(S::kDim, true);
+            int slot = 0;  // of the next k or v tile in ring order
+            uint32_t phase = 0;
+            bool ok = mbar_wait(&ctl.q_full, 0, abort), issued = false;
+            auto next = [&] {  // waits for the next tile; its place
+                const int at = slot;
+                ok = ok && mbar_wait(&ctl.full[slot], phase, abort);
+                if (++slot == S::kSlots) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
+                return at;
+            };
+            auto width = [&](int t, int j) { return min(kTile, ((ends[t] - j * kTile) + 15) & ~15); };
+            auto score = [&](int t, int j, int k_slot) {
+                tc_fence_after();
+                product_rows<KS>(tmem + t * 128u, su32(smem + t * S::kTileBytes), su32(ring + k_slot * S::kTileBytes),
+                                 bf16_idesc(width(t, j), false));
+                tc_commit(&ctl.scores[t]);
+                issued = true;
+            };
+            int k_slot = next();
+            if (ok) {
+                for (int t = 0; t < NT; ++t)
+                    if (counts[t] > 0) score(t, 0, k_slot);
+                tc_commit(&ctl.empty[k_slot]);
+            }
+            for (int j = 0; j < last && ok; ++j) {
+                const int v_slot = next();
+                if (ok && tail && j == last - 1) {
+                    mbar_arrive(&ctl.tail_here);
+                    ok = mbar_wait(&ctl.tail, 0, abort);
+                }
+                if (!ok) break;
+                bool have_k = false;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if (j < counts[t]) {
+                        ok = ok && mbar_wait(&ctl.weights[t], uint32_t(j) & 1u, abort);
+                        if (!ok) break;
+                        tc_fence_after();
+                        product_weights(tmem + S::kO + uint32_t(t) * S::kDim, tmem + t * 128u,
+                                        su32(ring + v_slot * S::kTileBytes), width(t, j) / 16, o_desc, j > 0);
+                    }
+                    if (t == NT - 1) tc_commit(&ctl.empty[v_slot]);
+                    if (j + 1 < last && !have_k) {
+                        k_slot = next();
+                        if (!ok) break;
+                        have_k = true;
+                    }
+                    if (j + 1 < counts[t]) score(t, j + 1, k_slot);
+                    else if (j + 1 == counts[t]) tc_commit(&ctl.done[t]);
+                    if (t == NT - 1 && j + 1 < last) tc_commit(&ctl.empty[k_slot]);
+                }
+            }
+            if (!ok && issued) {  // the products in flight end before TMEM is freed
+                tc_commit(&ctl.drain);
+                mbar_wait(&ctl.drain, 0, abort, true);
+            }
+        }
+    } else if (warp < 4) {
+        if (tail) {
+            if (mbar_wait(&ctl.tail_here, 0, abort)) {
+                const int first = keys - (last - 1) * kTile;
+                zero_rows(ring + ((2 * last - 1) % S::kSlots) * S::kTileBytes, S::kPanels, first, (first + 15) & ~15, threadIdx.x - 64, 64);
+                mbar_arrive(&ctl.tail);
+            }
+        }
+    } else {
+        // ---------------------------------------------------------- softmax: thread = row
+        const int t = (warp - 4) >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const uint32_t at_s = tmem + lanes + t * 128u, at_o = tmem + lanes + S::kO + uint32_t(t) * S::kDim;
+        const int token = r / a.group;
+        const bool real = token < tokens[t];
+        const int limit = real ? int(seen(s, a.causal, token0 + t * per_tile + token)) : 0;
+        const float c = a.scale * kLog2e;
+        float m = -INFINITY, l = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < counts[t]; ++j) {
+            const bool got = mbar_wait(&ctl.scores[t], uint32_t(j) & 1u, abort);
+            if (!__all_sync(0xffffffffu, got)) {  // uniform in the warp: TMEM access is .sync.aligned
+                *abort = 1;
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const int chunks = min(4, (ends[t] - j * kTile + 31) / 32);
+            const int mine = limit - j * kTile;  // columns of this tile that the row sees
+            const bool masked = __any_sync(0xffffffffu, mine < chunks * 32);
+            float x[32];
+            float top = -INFINITY;
+            for (int ch = 0; ch < chunks; ++ch) {
+                tmem_load32(at_s + ch * 32, x);
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) top = fmaxf(top, ch * 32 + i < mine ? x[i] : -INFINITY);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) top = fmaxf(top, x[i]);
+                }
+            }
+            top *= c;
+            const bool move = top > m + kSlack;  // the first finite maximum always moves: m starts at -inf
+            if (__any_sync(0xffffffffu, move)) {
+                const float keep = move ? ex2(m - top) : 1.0f;
+                if (move) m = top;
+                l *= keep;
+                if (j > 0) {
+#pragma unroll
+                    for (int ch = 0; ch < S::kDim / 32; ++ch) {
+                        float o[32];
+                        tmem_load32(at_o + ch * 32, o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] *= keep;
+                        tmem_store32(at_o + ch * 32, o);
+                    }
+                }
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+            const float2 c2 = make_float2(c, c), base2 = make_float2(-base, -base);
+            float2 sum = make_float2(0.0f, 0.0f);
+            for (int ch = 0; ch < chunks; ++ch) {
+                tmem_load32(at_s + ch * 32, x);
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = ch * 32 + i < mine ? x[i] : -INFINITY;
+                }
+                uint32_t p[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    float2 y = fma2(make_float2(x[i], x[i + 1]), c2, base2);
+                    y.x = ex2(y.x);
+                    y.y = ex2(y.y);
+                    sum = add2(sum, y);
+                    p[i / 2] = pack_bf16(y.x, y.y);
+                }
+                tmem_store16(at_s + ch * 16, p);
+            }
+            l += sum.x + sum.y;
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&ctl.weights[t]);
+        }
+        if (ok && counts[t] > 0) {
+            const bool got = mbar_wait(&ctl.done[t], 0, abort);
+            ok = __all_sync(0xffffffffu, got);
+            tc_fence_after();
+        }
+        if (ok && tokens[t] > 0) {
+            const int64_t flat = (s.row0 + token0 + t * per_tile + token) * a.hq + head * a.group + r % a.group;
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + flat * a.dim;
+            // a row without keys: zeros; a sum that is not a number stays one
+            const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+            for (int ch = 0; ch < S::kDim / 32; ++ch) {
+                float o[32];
+                if (counts[t] > 0) {
+                    tmem_load32(at_o + ch * 32, o);
+                }
+                if (!real) continue;
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (limit > 0)
+                        w = make_uint4(pack_bf16(o[i] * inv, o[i + 1] * inv), pack_bf16(o[i + 2] * inv, o[i + 3] * inv),
+                                       pack_bf16(o[i + 4] * inv, o[i + 5] * inv), pack_bf16(o[i + 6] * inv, o[i + 7] * inv));
+                    if (ch * 32 + i < a.dim) *reinterpret_cast<uint4*>(out + ch * 32 + i) = w;
+                }
+            }
+            if (real && a.lse != nullptr) a.lse[flat] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kTmem) : "memory");
+    }
+    if (threadIdx.x == 0 && ctl.abort) raise_flag(a.flags, FMD_FLAG_WAIT_TIMEOUT);
+}
+
+template <int KS, int NT>
+fmd_status launch(const Maps& maps, const Attn& a, cudaStream_t s) {
+    using S = Shape<KS, NT>;
+    const fmd_status st = grant_dynamic_smem((const void*)forward_kernel<KS, NT>, S::kBytes, true);
+    if (st != FMD_OK) return st;
+    const int64_t tiles = tile_bound(a.rows, a.batch, NT * (kTile / a.group));
+    forward_kernel<KS, NT><<<dim3(unsigned(tiles), unsigned(a.hk)), S::kThreads, S::kBytes, s>>>(maps, a);
+    return check_launch();
+}
+
+}  // namespace
+
+fmd_status encode_packed(const DriverCalls& drv, CUtensorMap* map, const void* x, int64_t rows, int hk, int group,
+                         int dim, int64_t row, int64_t head, int tokens) {
+    if (hk * group == 1) head = dim;  // the stride of an axis of one is anything
+    if (rows == 1) row = head * hk * group;
+    const cuuint64_t dims[4] = {cuuint64_t(dim), cuuint64_t(group), cuuint64_t(hk), cuuint64_t(rows)};
+    const cuuint64_t strides[3] = {cuuint64_t(head) * 2, cuuint64_t(head) * 2 * group, cuuint64_t(row) * 2};
+    const cuuint32_t box[4] = {64, cuuint32_t(group), 1, cuuint32_t(tokens)};
+    const cuuint32_t step[4] = {1, 1, 1, 1};
+    const CUresult r = drv.encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(x), dims, strides, box,
+                                  step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? FMD_OK : record_error_text(FMD_ERR_CUDA, "cuTensorMapEncodeTiled failed, CUresult", r);
+}
+
+fmd_status attention_forward_mma(const Attn& a, cudaStream_t s) {
+    const DriverCalls& drv = driver_calls();
+    if (drv.encode == nullptr || drv.ctx_get_current == nullptr)
+        return record_error_text(FMD_ERR_CUDA, "driver entry point cuTensorMapEncodeTiled unavailable", 0);
+    fmd_status st = bind_context(drv);
+    Maps maps{};
+    if (st == FMD_OK)
+        st = encode_packed(drv, &maps.q, a.q, a.rows, a.hk, a.group, a.dim, a.q_row, a.q_head, kTile / a.group);
+    if (a.keys > 0) {  // without keys nothing is loaded
+        if (st == FMD_OK) st = encode_packed(drv, &maps.k, a.k, a.keys, a.hk, 1, a.dim, a.k_row, a.k_head, kTile);
+        if (st == FMD_OK) st = encode_packed(drv, &maps.v, a.v, a.keys, a.hk, 1, a.dim, a.v_row, a.v_head, kTile);
+    }
+    if (st != FMD_OK) return st;
+    const bool two = tile_bound(a.rows, a.batch, 2 * (kTile / a.group)) * a.hk >= kNumSMs;
+    if (a.dim <= 32) return two ? launch<2, 2>(maps, a, s) : launch<2, 1>(maps, a, s);
+    if (a.dim <= 64) return two ? launch<4, 2>(maps, a, s) : launch<4, 1>(maps, a, s);
+    if (a.dim <= 96) return two ? launch<6, 2>(maps, a, s) : launch<6, 1>(maps, a, s);
+    return two ? launch<8, 2>(maps, a, s) : launch<8, 1>(maps, a, s);
+}
+
+}  // namespace fmd

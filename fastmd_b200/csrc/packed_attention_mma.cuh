@@ -1,0 +1,177 @@
+// The tensor-core pieces that the bfloat16 attention kernels share: operand tiles, descriptors, products, TMEM access.
+//
+// An operand tile is 128 rows of up to 128 values as panels of 64 values: panel p holds 128 rows of 128 bytes, in the
+// 128-byte swizzle that TMA writes. The same tile serves as a K-major operand (the product runs over its 64-value
+// rows: scores) and, read the other way, as an MN-major one (the product runs over its rows: weights times values).
+#pragma once
+
+#include "packed_attention.cuh"
+#include "sm100.cuh"
+
+namespace fmd {
+
+constexpr int kTile = 128;                           // rows of a tile: the M of every product
+constexpr uint32_t kPanelBytes = kTile * 128;        // 128 rows x 64 bfloat16
+constexpr uint32_t kPanelStep = kPanelBytes >> 4;    // in descriptor units of 16 bytes
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
+                                            int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+        "%5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(su32(bar))
+        : "memory");
+}
+
+// The upper halves of the two descriptors (the lower ones hold the address and the leading offset, in 16 bytes):
+// groups of 8 rows 1024 bytes apart, descriptor version 1, 128-byte swizzle.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+
+// An operand whose rows are the product's M or N index: a step of 16 along the row is 32 bytes (+ 2).
+__device__ __forceinline__ uint32_t rows_desc(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | (1u << 16); }
+
+// An operand whose rows are the product's inner index and whose 64-value panels are its N index (leading offset: the
+// next panel): a step of 16 rows is 2048 bytes (+ 128).
+__device__ __forceinline__ uint32_t columns_desc(uint32_t saddr) {
+    return ((saddr & 0x3FFFFu) >> 4) | (kPanelStep << 16);
+}
+
+// Instruction descriptor of kind::f16: FP32 accumulator, bfloat16 operands, M = 128, N; B transposed when its rows
+// are the inner index.
+__device__ __forceinline__ uint32_t bf16_idesc(int n, bool b_columns) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_columns ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) |
+           (uint32_t(kTile >> 4) << 24);
+}
+
+// Two steps of 16 of D [128, n] (+)= A B^T along the rows of both operands, as one statement without branches.
+__device__ __forceinline__ void mma_rows2(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 u, v, w, z;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\tadd.u32 x, %1, 2;\n\tadd.u32 y, %2, 2;\n\t"
+        "mov.b64 u, {%1, %3};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 w, {x, %3};\n\tmov.b64 z, {y, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], u, v, %4, p;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], w, z, %4, 1;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(kDescHigh), "r"(idesc), "r"(add)
+        : "memory");
+}
+
+// One step of 16 of D [128, n] (+)= P B with P in TMEM (8 columns a step), the rows of B the inner index.
+__device__ __forceinline__ void mma_weights(uint32_t d, uint32_t p, uint32_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 v;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 v, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], v, %4, p;\n\t}" ::"r"(d),
+        "r"(p), "r"(b), "r"(kDescHigh), "r"(idesc), "r"(add)
+        : "memory");
+}
+
+// D [128, n] = A B^T over KS steps of 16 along the rows of both tiles.
+template <int KS>
+__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+    const uint32_t ad = rows_desc(a), bd = rows_desc(b);
+#pragma unroll
+    for (int k = 0; k < KS; k += 2) {
+        const uint32_t off = uint32_t(k / 4) * kPanelStep + uint32_t(k % 4) * 2;
+        mma_rows2(d, ad + off, bd + off, idesc, k > 0);
+    }
+}
+
+// D [128, n] (+)= P B over `steps` (at most 8) steps of 16 rows of B, P [128, 16 steps] bfloat16 in TMEM.
+__device__ __forceinline__ void product_weights(uint32_t d, uint32_t p, uint32_t b, int steps, uint32_t idesc,
+                                                bool add) {
+    const uint32_t bd = columns_desc(b);
+    if (steps == kTile / 16) {
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k) mma_weights(d, p + 8 * k, bd + k * 128, idesc, add || k > 0);
+    } else {
+        for (int k = 0; k < steps; ++k) mma_weights(d, p + 8 * k, bd + k * 128, idesc, add || k > 0);
+    }
+}
+
+#define FMD_TMEM_R32                                                                                              \
+    "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, " \
+    "%23, %24, %25, %26, %27, %28, %29, %30, %31}"
+
+// 32 consecutive TMEM columns of this thread's lane. The load writes its registers asynchronously: the wait belongs
+// to the same statement, so that nothing between the two can copy or reuse them.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " FMD_TMEM_R32 ", [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+                   "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]),
+                   "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]),
+                   "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]),
+                   "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+                 : "r"(addr)
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const float (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " FMD_TMEM_R32 ";" ::"f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+        "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]),
+        "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]),
+        "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]),
+        "f"(v[31]), "r"(addr)
+        : "memory");
+}
+
+// 16 columns: 32 bfloat16 of this thread's lane
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// two FP32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float low, float high) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+    return r;
+}
+
+// Zeros rows [first, last) of a tile of `panels` panels (the swizzle keeps a row's 128 bytes in place), by `count`
+// threads; then visible to the tensor cores after the barrier that follows.
+__device__ __forceinline__ void zero_rows(unsigned char* tile, int panels, int first, int last, int thread, int count) {
+    const int per = (last - first) * 8;
+    for (int i = thread; i < per * panels; i += count) {
+        const int p = i / per, w = i - p * per;
+        *reinterpret_cast<uint4*>(tile + p * kPanelBytes + first * 128 + w * 16) = make_uint4(0, 0, 0, 0);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// ------------------------------------------------------------------- host
+
+// Packed rows: x [rows, key_heads, group, dim], a box of `tokens` tokens x group heads x 64 values.
+fmd_status encode_packed(const DriverCalls& drv, CUtensorMap* map, const void* x, int64_t rows, int hk, int group,
+                         int dim, int64_t row, int64_t head, int tokens);
+
+}  // namespace fmd

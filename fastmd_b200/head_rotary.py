@@ -45,8 +45,9 @@ def rotary_table(length: int, rotary_dim: int, *, base: float = 10000.0, factor:
 
 def _head_rows(x: Tensor) -> Tensor:
     """``x`` with unit stride inside a head and 16-byte rows, heads and base; copied only when needed."""
-    size = x.element_size()
-    if x.stride(2) == 1 and not (x.data_ptr() % 16 or x.stride(0) * size % 16 or x.stride(1) * size % 16):
+    row, head, unit = x.stride()
+    width = 16 // x.element_size()
+    if unit == 1 and row and head and not (row % width or head % width or x.data_ptr() % 16):
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
