@@ -127,7 +127,7 @@ fmd_status fmd_packed_attention_bwd(const fmd_attention* problem, const void* ou
         else delta_kernel<__nv_bfloat16><<<unsigned(blocks), kThreads, 0, s>>>(a, glse, delta);
         if ((st = check_launch()) != FMD_OK) return st;
     }
-    return attention_backward_simt(a, problem->type, s);
+    return problem->type == FMD_BF16 ? attention_backward_mma(a, s) : attention_backward_simt(a, problem->type, s);
 }
 
 }  // extern "C"

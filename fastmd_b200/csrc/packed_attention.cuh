@@ -100,6 +100,7 @@ __device__ __forceinline__ void attn_store(__nv_bfloat16* p, float v) { *p = __f
 
 fmd_status attention_forward_simt(const Attn& a, int type, cudaStream_t s);
 fmd_status attention_backward_simt(const Attn& a, int type, cudaStream_t s);
-fmd_status attention_forward_mma(const Attn& a, cudaStream_t s);  // bfloat16
+fmd_status attention_forward_mma(const Attn& a, cudaStream_t s);   // bfloat16
+fmd_status attention_backward_mma(const Attn& a, cudaStream_t s);  // bfloat16
 
 }  // namespace fmd

@@ -1,0 +1,623 @@
+// Packed attention in bfloat16 on the tensor cores: the gradients of q and of k and v.
+//
+//   p = exp(scale q k^T - lse),  dp = g v^T,  ds = p (dp - delta)
+//   dq = scale ds k;   dv = p^T g,  dk = scale ds^T q
+//
+// Two kernels, each of which owns the rows it writes and adds in one order, so that the gradients are the same bits on
+// every run without atomics or partial sums in memory; the price is that scores and dp are computed twice (seven
+// products for five). Both keep one side's tiles in shared memory and stream the other's:
+//
+//   queries  a block per 128 packed rows: S = q k^T, dP = g v^T, ds over dP in TMEM, dq += ds k
+//   keys     a block per 128 keys: S = k q^T and dP = v g^T with the keys in the lanes, so that p and ds are already
+//            the transposed operands: p over S, dv += p g; ds over dP, dk += ds q; lse and delta of the columns
+//            come through shared memory. The heads of a group are rows of the same tiles: their sum is the product's.
+//
+//   warp 0       TMA: the block's own tiles once, the others through a ring of shared-memory slots
+//   warp 1       one thread issues the products
+//   warps 2, 3   rows that must not count (behind a sequence's end) become zeros; keys: lse and delta of each tile
+//   warps 4-11   thread = lane; the first four warps columns 0 .. 63, the others 64 .. 127 (each overwrites only
+//                columns that it has read itself)
+//
+// Order of the products (one thread issues them, they run in order; a product that reads a TMEM operand is issued
+// before the one that overwrites it):
+//   queries  S0 dP0 | S(j+1), [ds j] dq(j), dP(j+1)       S has two buffers: exp2 of tile j + 1 runs during dq(j)
+//   keys     S0 dP0 | [p j] dv(j), S(j+1), [ds j] dk(j), dP(j+1)     exp2 of j + 1 runs during dk(j) and dP(j+1)
+// Every wait is bounded, as in the forward pass.
+
+#include "packed_attention_mma.cuh"
+
+namespace fmd {
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kWorkers = 256;
+
+template <int KS>
+struct Shape {
+    static constexpr int kDim = 16 * KS;
+    static constexpr int kPanels = (KS + 3) / 4;
+    static constexpr uint32_t kTileBytes = kPanels * kPanelBytes;
+    static constexpr int kSlots = kPanels == 2 ? 4 : 8;  // 192 or 160 KB with the two tiles that stay
+    static constexpr size_t kBytes = size_t(2 + kSlots) * kTileBytes + 1024 + 256;
+};
+
+template <int KS>
+struct Ctrl {
+    uint64_t own;  // the two tiles that stay have landed
+    uint64_t full[Shape<KS>::kSlots], empty[Shape<KS>::kSlots];
+    uint64_t scores[2], dp;      // products done
+    uint64_t p, ds;              // written by the workers
+    uint64_t stats[2], read[2];  // keys: lse and delta of a tile in shared memory; read by all worker warps
+    uint64_t tail_here, tail;    // the last tiles have landed; their rows behind the end are zeros
+    uint64_t done, drain;
+    uint32_t tmem;
+    int32_t abort;
+};
+
+struct Maps {
+    CUtensorMap q, g, k, v;
+};
+
+template <int KS>
+__device__ __forceinline__ void open_block(Ctrl<KS>& ctl, int warp) {
+    if (threadIdx.x == 0) {
+        mbar_init(&ctl.own, 1);
+        for (int i = 0; i < Shape<KS>::kSlots; ++i) {
+            mbar_init(&ctl.full[i], 1);
+            mbar_init(&ctl.empty[i], 1);
+        }
+        mbar_init(&ctl.scores[0], 1);
+        mbar_init(&ctl.scores[1], 1);
+        mbar_init(&ctl.dp, 1);
+        mbar_init(&ctl.p, kWorkers);
+        mbar_init(&ctl.ds, kWorkers);
+        mbar_init(&ctl.stats[0], 64);
+        mbar_init(&ctl.stats[1], 64);
+        mbar_init(&ctl.read[0], kWorkers / 32);
+        mbar_init(&ctl.read[1], kWorkers / 32);
+        mbar_init(&ctl.tail_here, 1);
+        mbar_init(&ctl.tail, 64);
+        mbar_init(&ctl.done, 1);
+        mbar_init(&ctl.drain, 1);
+        ctl.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&ctl.tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+}
+
+template <int KS>
+__device__ __forceinline__ void close_block(Ctrl<KS>& ctl, int warp, int32_t* flags) {
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(ctl.tmem) : "memory");
+    }
+    if (threadIdx.x == 0 && ctl.abort) raise_flag(flags, FMD_FLAG_WAIT_TIMEOUT);
+}
+
+// The ring's producer: tiles a0, b0, a1, b1, .. of `bytes` each, loaded by load(second, tile, slot address, barrier).
+template <int KS, typename Load>
+__device__ __forceinline__ void feed(Ctrl<KS>& ctl, unsigned char* ring, int tiles, uint32_t bytes, Load load) {
+    using S = Shape<KS>;
+    volatile int32_t* abort = &ctl.abort;
+    int slot = 0, armed = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int i = 0; i < 2 * tiles; ++i) {
+        if (!mbar_wait(&ctl.empty[slot], phase ^ 1u, abort)) {
+            ok = false;
+            break;
+        }
+        mbar_expect_tx(&ctl.full[slot], bytes);
+        load(i & 1, i >> 1, su32(ring + slot * S::kTileBytes), &ctl.full[slot]);
+        armed = i + 1;
+        if (++slot == S::kSlots) {
+            slot = 0;
+            phase ^= 1u;
+        }
+    }
+    if (!ok) {  // the copies in flight land before the block ends
+        mbar_wait(&ctl.own, 0, abort, true);
+        for (int i = max(0, armed - S::kSlots); i < armed; ++i)
+            mbar_wait(&ctl.full[i % S::kSlots], uint32_t(i / S::kSlots) & 1u, abort, true);
+    } else {  // the last slots' releases land before the block ends
+        for (int i = 0; i < S::kSlots && mbar_wait(&ctl.empty[slot], phase ^ 1u, abort); ++i)
+            if (++slot == S::kSlots) {
+                slot = 0;
+                phase ^= 1u;
+            }
+    }
+}
+
+// Waits for tile i of the ring (its place is i % slots); only for a thread that takes the tiles in order.
+template <int KS>
+__device__ __forceinline__ bool landed(Ctrl<KS>& ctl, int i) {
+    return mbar_wait(&ctl.full[i % Shape<KS>::kSlots], uint32_t(i / Shape<KS>::kSlots) & 1u, &ctl.abort);
+}
+
+// Writes 32 FP32 columns of TMEM times `factor` as bfloat16, as far as dim goes. loaded (the same in the whole warp):
+// the columns hold a result; keep: this row's counts, else it is zeros; real: the row exists.
+__device__ __forceinline__ void store_row(__nv_bfloat16* out, uint32_t tmem, int col0, int dim, float factor,
+                                          bool loaded, bool keep, bool real) {
+    float o[32];
+    if (loaded) tmem_load32(tmem + col0, o);
+    if (!real) return;
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (loaded && keep)
+            w = make_uint4(pack_bf16(o[i] * factor, o[i + 1] * factor), pack_bf16(o[i + 2] * factor, o[i + 3] * factor),
+                           pack_bf16(o[i + 4] * factor, o[i + 5] * factor),
+                           pack_bf16(o[i + 6] * factor, o[i + 7] * factor));
+        if (col0 + i < dim) *reinterpret_cast<uint4*>(out + col0 + i) = w;
+    }
+}
+
+// ---------------------------------------------------------------- queries
+
+template <int KS>
+__global__ void __launch_bounds__(kThreads, 1)
+    query_gradient_kernel(const __grid_constant__ Maps maps, const Attn a) {
+    using S = Shape<KS>;
+    extern __shared__ unsigned char raw[];
+    unsigned char* own = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* ring = own + 2 * S::kTileBytes;
+    __shared__ Ctrl<KS> ctl;
+    volatile int32_t* abort = &ctl.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int64_t index = gridDim.x - 1 - blockIdx.x;
+    const int per_tile = kTile / a.group;
+    const int b = find_sequence(a.offsets, a.batch, per_tile, index);
+    const Span s = load_span(a, b);
+    const int64_t token0 = (index - (a.offsets[b] / per_tile + b)) * per_tile;
+    if (token0 < 0 || token0 >= s.rows) return;
+    const int head = blockIdx.y;
+    const int tokens = int(min(int64_t(per_tile), s.rows - token0));
+    const int end = int(seen(s, a.causal, token0 + tokens - 1));
+    const int tiles = (end + kTile - 1) / kTile, keys = int(s.keys);
+    const bool tail = tiles > 0 && keys < tiles * kTile;
+    constexpr uint32_t kDp = 256, kDq = 384;  // TMEM columns: two score buffers, dP, dq
+
+    open_block<KS>(ctl, warp);
+    const uint32_t tmem = ctl.tmem;
+
+    if (warp == 0) {
+        if (lane == 0 && tiles > 0) {
+            mbar_expect_tx(&ctl.own, 2u * S::kPanels * 128u * uint32_t(per_tile * a.group));
+            for (int p = 0; p < S::kPanels; ++p) {
+                tma_load_4d(su32(own + p * kPanelBytes), &maps.q, &ctl.own, p * 64, 0, head, int(s.row0 + token0));
+                tma_load_4d(su32(own + S::kTileBytes + p * kPanelBytes), &maps.g, &ctl.own, p * 64, 0, head,
+                            int(s.row0 + token0));
+            }
+            feed<KS>(ctl, ring, tiles, S::kTileBytes, [&](int second, int j, uint32_t at, uint64_t* bar) {
+                for (int p = 0; p < S::kPanels; ++p)
+                    tma_load_4d(at + p * kPanelBytes, second ? &maps.v : &maps.k, bar, p * 64, 0, head,
+                                int(s.key0) + j * kTile);
+            });
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && tiles > 0) {
+            const uint32_t q_tile = su32(own), g_tile = su32(own + S::kTileBytes);
+            const uint32_t out_desc = bf16_idesc(S::kDim, true);
+            auto slot = [&](int i) { return su32(ring + (i % S::kSlots) * S::kTileBytes); };
+            auto width = [&](int j) { return min(kTile, (end - j * kTile + 15) & ~15); };
+            bool ok = mbar_wait(&ctl.own, 0, abort), issued = false;
+            auto scores = [&](int j) {  // into buffer j % 2
+                ok = ok && landed<KS>(ctl, 2 * j);
+                if (!ok) return;
+                tc_fence_after();
+                product_rows<KS>(tmem + uint32_t(j & 1) * 128u, q_tile, slot(2 * j), bf16_idesc(width(j), false));
+                tc_commit(&ctl.scores[j & 1]);
+                issued = true;
+            };
+            auto dp = [&](int j) {
+                ok = ok && landed<KS>(ctl, 2 * j + 1);
+                if (!ok) return;
+                tc_fence_after();
+                product_rows<KS>(tmem + kDp, g_tile, slot(2 * j + 1), bf16_idesc(width(j), false));
+                tc_commit(&ctl.dp);
+                tc_commit(&ctl.empty[(2 * j + 1) % S::kSlots]);
+            };
+            scores(0);
+            dp(0);
+            for (int j = 0; j < tiles && ok; ++j) {
+                if (j + 1 < tiles) scores(j + 1);
+                if (ok && tail && j == tiles - 1) {
+                    mbar_arrive(&ctl.tail_here);
+                    ok = mbar_wait(&ctl.tail, 0, abort);
+                }
+                ok = ok && mbar_wait(&ctl.ds, uint32_t(j) & 1u, abort);
+                if (!ok) break;
+                tc_fence_after();
+                product_weights<64>(tmem + kDq, tmem + kDp, slot(2 * j), width(j) / 16, out_desc, j > 0);
+                tc_commit(&ctl.empty[(2 * j) % S::kSlots]);
+                if (j + 1 < tiles) dp(j + 1);
+            }
+            if (ok) tc_commit(&ctl.done);
+            if (!ok && issued) {
+                tc_commit(&ctl.drain);
+                mbar_wait(&ctl.drain, 0, abort, true);
+            }
+        }
+    } else if (warp < 4) {
+        if (tail && mbar_wait(&ctl.tail_here, 0, abort)) {  // keys behind the last one: they are the inner index of dq
+            const int first = keys - (tiles - 1) * kTile;
+            zero_rows(ring + ((2 * tiles - 2) % S::kSlots) * S::kTileBytes, S::kPanels, first, (first + 15) & ~15,
+                      threadIdx.x - 64, 64);
+            mbar_arrive(&ctl.tail);
+        }
+    } else {
+        const int half = (warp - 4) >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const int token = r / a.group;
+        const bool real = token < tokens;
+        const int64_t flat = (s.row0 + token0 + token) * a.hq + head * a.group + r % a.group;
+        const float lse = real ? a.lse[flat] : -INFINITY, delta = real ? a.delta[flat] : 0.0f;
+        const int limit = lse != -INFINITY ? int(seen(s, a.causal, token0 + token)) : 0;
+        const float base = lse != -INFINITY ? -lse * kLog2e : 0.0f;
+        const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), base2 = make_float2(base, base);
+        const float2 delta2 = make_float2(-delta, -delta);
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            const int columns = end - j * kTile - 64 * half;  // of this half that some row sees
+            const int chunks = min(2, max(0, (columns + 31) / 32));
+            const int mine = limit - j * kTile - 64 * half;
+            const bool masked = __any_sync(0xffffffffu, mine < chunks * 32);
+            float p[64];
+            bool got = mbar_wait(&ctl.scores[j & 1], uint32_t(j >> 1) & 1u, abort);
+            if (!__all_sync(0xffffffffu, got)) {
+                *abort = 1;
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t at_s = tmem + lanes + uint32_t(j & 1) * 128u + uint32_t(half) * 64u;
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) {
+                if (ch < chunks) {
+                    float x[32];
+                    tmem_load32(at_s + ch * 32, x);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 y = fma2(make_float2(x[i], x[i + 1]), c2, base2);
+                        p[ch * 32 + i] = ex2(y.x);
+                        p[ch * 32 + i + 1] = ex2(y.y);
+                    }
+                }
+            }
+            got = mbar_wait(&ctl.dp, uint32_t(j) & 1u, abort);
+            if (!__all_sync(0xffffffffu, got)) {
+                *abort = 1;
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t at_d = tmem + lanes + kDp + uint32_t(half) * 64u;
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) {
+                if (ch < chunks) {
+                    float x[32];
+                    uint32_t w[16];
+                    tmem_load32(at_d + ch * 32, x);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        float2 y = add2(make_float2(x[i], x[i + 1]), delta2);
+                        y = mul2(y, make_float2(p[ch * 32 + i], p[ch * 32 + i + 1]));
+                        if (masked) {  // what a row does not see has no share, whatever its values
+                            y.x = ch * 32 + i < mine ? y.x : 0.0f;
+                            y.y = ch * 32 + i + 1 < mine ? y.y : 0.0f;
+                        }
+                        w[i / 2] = pack_bf16(y.x, y.y);
+                    }
+                    tmem_store16(at_d + ch * 16, w);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&ctl.ds);
+        }
+        if (ok && tiles > 0) {
+            const bool got = mbar_wait(&ctl.done, 0, abort);
+            ok = __all_sync(0xffffffffu, got);
+            tc_fence_after();
+        }
+        if (ok) {
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.dq) + flat * a.dim;
+            for (int col = 32 * half; col < S::kDim; col += 64)
+                store_row(out, tmem + lanes + kDq, col, a.dim, a.scale, tiles > 0, true, real);
+        }
+    }
+    close_block<KS>(ctl, warp, a.flags);
+}
+
+// ------------------------------------------------------------------- keys
+
+template <int KS>
+__global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_constant__ Maps maps, const Attn a) {
+    using S = Shape<KS>;
+    extern __shared__ unsigned char raw[];
+    unsigned char* own = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* ring = own + 2 * S::kTileBytes;
+    __shared__ Ctrl<KS> ctl;
+    // of two tiles: - lse log2 e, - delta and the number of keys that each packed row sees
+    __shared__ alignas(16) float lse_of[2][kTile], delta_of[2][kTile];
+    __shared__ alignas(16) int limit_of[2][kTile];
+    volatile int32_t* abort = &ctl.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int b = find_sequence(a.key_offsets, a.batch, kTile, blockIdx.x);
+    const Span s = load_span(a, b);
+    const int64_t key0 = (int64_t(blockIdx.x) - (a.key_offsets[b] / kTile + b)) * kTile;
+    if (key0 < 0 || key0 >= s.slot) return;
+    const int head = blockIdx.y;
+    const int per_tile = kTile / a.group, full_rows = per_tile * a.group;
+    // tiles of rows from the one that holds the first token that sees key0
+    const int64_t first = a.causal ? max(int64_t(0), key0 + s.rows - s.keys) / per_tile : 0;
+    const int64_t all = (s.rows + per_tile - 1) / per_tile;
+    const int tiles = key0 < s.keys ? int(max(int64_t(0), all - first)) : 0;
+    const int last_rows = tiles > 0 ? int(s.rows - (all - 1) * per_tile) * a.group : 0;
+    const bool tail = tiles > 0 && last_rows % 16 != 0 && last_rows < full_rows;
+    constexpr uint32_t kDp = 128, kDv = 256, kDk = 384;  // TMEM columns, the scores at 0
+
+    if (full_rows < kTile && warp >= 4)  // rows of the slots that no copy ever writes are inner rows of the products
+        for (int i = 0; i < S::kSlots; ++i)
+            zero_rows(ring + i * S::kTileBytes, S::kPanels, full_rows, kTile, threadIdx.x - 128, kWorkers);
+    open_block<KS>(ctl, warp);
+    const uint32_t tmem = ctl.tmem;
+
+    if (warp == 0) {
+        if (lane == 0 && tiles > 0) {
+            mbar_expect_tx(&ctl.own, 2u * S::kTileBytes);
+            for (int p = 0; p < S::kPanels; ++p) {
+                tma_load_4d(su32(own + p * kPanelBytes), &maps.k, &ctl.own, p * 64, 0, head, int(s.key0 + key0));
+                tma_load_4d(su32(own + S::kTileBytes + p * kPanelBytes), &maps.v, &ctl.own, p * 64, 0, head,
+                            int(s.key0 + key0));
+            }
+            feed<KS>(ctl, ring, tiles, uint32_t(S::kPanels) * 128u * full_rows,
+                     [&](int second, int j, uint32_t at, uint64_t* bar) {
+                         for (int p = 0; p < S::kPanels; ++p)
+                             tma_load_4d(at + p * kPanelBytes, second ? &maps.g : &maps.q, bar, p * 64, 0, head,
+                                         int(s.row0 + (first + j) * per_tile));
+                     });
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && tiles > 0) {
+            const uint32_t k_tile = su32(own), v_tile = su32(own + S::kTileBytes);
+            const uint32_t out_desc = bf16_idesc(S::kDim, true);
+            auto slot = [&](int i) { return su32(ring + (i % S::kSlots) * S::kTileBytes); };
+            auto width = [&](int j) { return ((j == tiles - 1 ? last_rows : full_rows) + 15) & ~15; };
+            bool ok = mbar_wait(&ctl.own, 0, abort), issued = false;
+            auto scores = [&](int j) {
+                ok = ok && landed<KS>(ctl, 2 * j);
+                if (!ok) return;
+                tc_fence_after();
+                product_rows<KS>(tmem, k_tile, slot(2 * j), bf16_idesc(width(j), false));
+                tc_commit(&ctl.scores[0]);
+                issued = true;
+            };
+            auto dp = [&](int j) {
+                ok = ok && landed<KS>(ctl, 2 * j + 1);
+                if (!ok) return;
+                tc_fence_after();
+                product_rows<KS>(tmem + kDp, v_tile, slot(2 * j + 1), bf16_idesc(width(j), false));
+                tc_commit(&ctl.dp);
+            };
+            scores(0);
+            dp(0);
+            for (int j = 0; j < tiles && ok; ++j) {
+                const int steps = width(j) / 16;
+                if (tail && j == tiles - 1) {
+                    mbar_arrive(&ctl.tail_here);
+                    ok = mbar_wait(&ctl.tail, 0, abort);
+                }
+                ok = ok && mbar_wait(&ctl.p, uint32_t(j) & 1u, abort);
+                if (!ok) break;
+                tc_fence_after();
+                product_weights<64>(tmem + kDv, tmem, slot(2 * j + 1), steps, out_desc, j > 0);
+                tc_commit(&ctl.empty[(2 * j + 1) % S::kSlots]);
+                if (j + 1 < tiles) scores(j + 1);
+                ok = ok && mbar_wait(&ctl.ds, uint32_t(j) & 1u, abort);
+                if (!ok) break;
+                tc_fence_after();
+                product_weights<64>(tmem + kDk, tmem + kDp, slot(2 * j), steps, out_desc, j > 0);
+                tc_commit(&ctl.empty[(2 * j) % S::kSlots]);
+                if (j + 1 < tiles) dp(j + 1);
+            }
+            if (ok) tc_commit(&ctl.done);
+            if (!ok && issued) {
+                tc_commit(&ctl.drain);
+                mbar_wait(&ctl.drain, 0, abort, true);
+            }
+        }
+    } else if (warp < 4) {
+        const int thread = threadIdx.x - 64;
+        bool ok = true;
+        for (int j = 0; j < tiles && ok; ++j) {
+            if (j >= 2 && !mbar_wait(&ctl.read[j & 1], uint32_t((j >> 1) - 1) & 1u, abort)) {
+                ok = false;
+                break;
+            }
+            const int64_t token0 = (first + j) * per_tile;
+            for (int r = thread; r < kTile; r += 64) {
+                const int64_t token = token0 + r / a.group;
+                float lse = -INFINITY, delta = 0.0f;
+                int limit = 0;
+                if (r < full_rows && token < s.rows) {
+                    const int64_t flat = (s.row0 + token) * a.hq + head * a.group + r % a.group;
+                    lse = a.lse[flat];
+                    delta = a.delta[flat];
+                    limit = int(max(int64_t(0), min(int64_t(kTile), seen(s, a.causal, token) - key0)));
+                }
+                const bool none = lse == -INFINITY;
+                lse_of[j & 1][r] = none ? 0.0f : -lse * kLog2e;
+                delta_of[j & 1][r] = -delta;
+                limit_of[j & 1][r] = none ? 0 : limit;
+            }
+            mbar_arrive(&ctl.stats[j & 1]);
+        }
+        if (tail && ok && mbar_wait(&ctl.tail_here, 0, abort)) {  // another sequence's rows
+            for (int i = 2 * tiles - 2; i < 2 * tiles; ++i)
+                zero_rows(ring + (i % S::kSlots) * S::kTileBytes, S::kPanels, last_rows, (last_rows + 15) & ~15, thread,
+                          64);
+            mbar_arrive(&ctl.tail);
+        }
+    } else {
+        const int half = (warp - 4) >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e);
+        const uint32_t at_s = tmem + lanes + uint32_t(half) * 64u, at_d = at_s + kDp;
+        const int here = int(min(int64_t(kTile), s.keys - key0));  // keys of this tile
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            const int rows = j == tiles - 1 ? last_rows : full_rows;
+            const int chunks = min(2, max(0, (rows - 64 * half + 31) / 32));
+            const float* nl = lse_of[j & 1] + 64 * half;
+            const float* nd = delta_of[j & 1] + 64 * half;
+            const int* lim = limit_of[j & 1] + 64 * half;
+            float p[64];
+            bool got = mbar_wait(&ctl.stats[j & 1], uint32_t(j >> 1) & 1u, abort) &&
+                       mbar_wait(&ctl.scores[0], uint32_t(j) & 1u, abort);
+            if (!__all_sync(0xffffffffu, got)) {
+                *abort = 1;
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            // a column is masked where its row sees fewer keys than the tile has, or is no row at all
+            bool masked = false;
+            if (lane < 16 * chunks) {
+                const int2 w = *reinterpret_cast<const int2*>(lim + 2 * lane);
+                masked = w.x < here || w.y < here;
+            }
+            masked = __any_sync(0xffffffffu, masked);
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) {
+                if (ch < chunks) {
+                    float x[32];
+                    uint32_t w[16];
+                    tmem_load32(at_s + ch * 32, x);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 l = *reinterpret_cast<const float2*>(nl + ch * 32 + i);
+                        float2 y = fma2(make_float2(x[i], x[i + 1]), c2, l);
+                        y.x = ex2(y.x);
+                        y.y = ex2(y.y);
+                        if (masked) {
+                            const int2 m = *reinterpret_cast<const int2*>(lim + ch * 32 + i);
+                            y.x = r < m.x ? y.x : 0.0f;
+                            y.y = r < m.y ? y.y : 0.0f;
+                        }
+                        p[ch * 32 + i] = y.x;
+                        p[ch * 32 + i + 1] = y.y;
+                        w[i / 2] = pack_bf16(y.x, y.y);
+                    }
+                    tmem_store16(at_s + ch * 16, w);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&ctl.p);
+            got = mbar_wait(&ctl.dp, uint32_t(j) & 1u, abort);
+            if (!__all_sync(0xffffffffu, got)) {
+                *abort = 1;
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) {
+                if (ch < chunks) {
+                    float x[32];
+                    uint32_t w[16];
+                    tmem_load32(at_d + ch * 32, x);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 d = *reinterpret_cast<const float2*>(nd + ch * 32 + i);
+                        float2 y = add2(make_float2(x[i], x[i + 1]), d);
+                        y = mul2(y, make_float2(p[ch * 32 + i], p[ch * 32 + i + 1]));
+                        if (masked) {  // also where dp is not a number
+                            const int2 m = *reinterpret_cast<const int2*>(lim + ch * 32 + i);
+                            y.x = r < m.x ? y.x : 0.0f;
+                            y.y = r < m.y ? y.y : 0.0f;
+                        }
+                        w[i / 2] = pack_bf16(y.x, y.y);
+                    }
+                    tmem_store16(at_d + ch * 16, w);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&ctl.ds);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl.read[j & 1]);
+        }
+        if (ok && tiles > 0) {
+            const bool got = mbar_wait(&ctl.done, 0, abort);
+            ok = __all_sync(0xffffffffu, got);
+            tc_fence_after();
+        }
+        if (ok) {
+            // the first four warps write dv, the others dk; slot rows that are no keys get zeros
+            const int64_t flat = ((s.key0 + key0 + r) * a.hk + head) * a.dim;
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(half ? a.dk : a.dv) + flat;
+            const bool real = key0 + r < s.slot;
+            for (int col = 0; col < S::kDim; col += 32)
+                store_row(out, tmem + lanes + (half ? kDk : kDv), col, a.dim, half ? a.scale : 1.0f, tiles > 0, r < here,
+                          real);
+        }
+    }
+    close_block<KS>(ctl, warp, a.flags);
+}
+
+template <int KS>
+fmd_status launch(const Maps& maps, const Attn& a, cudaStream_t s) {
+    using S = Shape<KS>;
+    fmd_status st = grant_dynamic_smem((const void*)query_gradient_kernel<KS>, S::kBytes, true);
+    if (st == FMD_OK) st = grant_dynamic_smem((const void*)key_gradient_kernel<KS>, S::kBytes, true);
+    if (st != FMD_OK) return st;
+    if (a.dq != nullptr && a.rows > 0) {
+        const int64_t tiles = tile_bound(a.rows, a.batch, kTile / a.group);
+        query_gradient_kernel<KS><<<dim3(unsigned(tiles), unsigned(a.hk)), kThreads, S::kBytes, s>>>(maps, a);
+        if ((st = check_launch()) != FMD_OK) return st;
+    }
+    if (a.dk != nullptr && a.keys > 0) {
+        const int64_t tiles = tile_bound(a.keys, a.batch, kTile);
+        key_gradient_kernel<KS><<<dim3(unsigned(tiles), unsigned(a.hk)), kThreads, S::kBytes, s>>>(maps, a);
+        st = check_launch();
+    }
+    return st;
+}
+
+}  // namespace
+
+fmd_status attention_backward_mma(const Attn& a, cudaStream_t s) {
+    const DriverCalls& drv = driver_calls();
+    if (drv.encode == nullptr || drv.ctx_get_current == nullptr)
+        return record_error_text(FMD_ERR_CUDA, "driver entry point cuTensorMapEncodeTiled unavailable", 0);
+    fmd_status st = bind_context(drv);
+    Maps maps{};
+    const int tokens = kTile / a.group;
+    if (a.rows > 0) {
+        if (st == FMD_OK) st = encode_packed(drv, &maps.q, a.q, a.rows, a.hk, a.group, a.dim, a.q_row, a.q_head, tokens);
+        if (st == FMD_OK) st = encode_packed(drv, &maps.g, a.g, a.rows, a.hk, a.group, a.dim, a.g_row, a.g_head, tokens);
+    }
+    if (a.keys > 0) {
+        if (st == FMD_OK) st = encode_packed(drv, &maps.k, a.k, a.keys, a.hk, 1, a.dim, a.k_row, a.k_head, kTile);
+        if (st == FMD_OK) st = encode_packed(drv, &maps.v, a.v, a.keys, a.hk, 1, a.dim, a.v_row, a.v_head, kTile);
+    }
+    if (st != FMD_OK) return st;
+    return a.dim <= 32 ? launch<2>(maps, a, s) : a.dim <= 64 ? launch<4>(maps, a, s)
+         : a.dim <= 96 ? launch<6>(maps, a, s) : launch<8>(maps, a, s);
+}
+
+}  // namespace fmd

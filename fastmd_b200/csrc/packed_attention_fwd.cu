@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
                         ok = ok && mbar_wait(&ctl.weights[t], uint32_t(j) & 1u, abort);
                         if (!ok) break;
                         tc_fence_after();
-                        product_weights(tmem + S::kO + uint32_t(t) * S::kDim, tmem + t * 128u,
+                        product_weights<32>(tmem + S::kO + uint32_t(t) * S::kDim, tmem + t * 128u,
                                         su32(ring + v_slot * S::kTileBytes), width(t, j) / 16, o_desc, j > 0);
                     }
                     if (t == NT - 1) tc_commit(&ctl.empty[v_slot]);

@@ -75,15 +75,19 @@ __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b,
     }
 }
 
-// D [128, n] (+)= P B over `steps` (at most 8) steps of 16 rows of B, P [128, 16 steps] bfloat16 in TMEM.
+// D [128, n] (+)= P B over `steps` (at most 8) steps of 16 rows of B, P [128, 16 steps] bfloat16 in TMEM: the first
+// four steps at p, the others at p + second.
+template <uint32_t kSecond>
 __device__ __forceinline__ void product_weights(uint32_t d, uint32_t p, uint32_t b, int steps, uint32_t idesc,
                                                 bool add) {
     const uint32_t bd = columns_desc(b);
     if (steps == kTile / 16) {
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k) mma_weights(d, p + 8 * k, bd + k * 128, idesc, add || k > 0);
+        for (int k = 0; k < kTile / 16; ++k)
+            mma_weights(d, p + 8 * (k % 4) + (k / 4) * kSecond, bd + k * 128, idesc, add || k > 0);
     } else {
-        for (int k = 0; k < steps; ++k) mma_weights(d, p + 8 * k, bd + k * 128, idesc, add || k > 0);
+        for (int k = 0; k < steps; ++k)
+            mma_weights(d, p + 8 * (k % 4) + (k / 4) * kSecond, bd + k * 128, idesc, add || k > 0);
     }
 }
 
@@ -145,6 +149,15 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 d;
     asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\t"
         "mov.b64 {%0, %1}, d;\n\t}"
         : "=f"(d.x), "=f"(d.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
