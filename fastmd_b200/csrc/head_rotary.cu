@@ -9,14 +9,15 @@
 //
 // Everything is computed in FP32 and rounded once, as the value is stored.
 //
-// What bounds it: memory. A head is D / V lanes of one 16-byte load each (V = 8 bfloat16 or 4 float32 values;
-// 4 bfloat16 where a rotated half does not divide by 8), the lanes padded to a power of two for the sums, so
-// a warp takes 32 / P heads at a time. The partner of a value in the half layout is the same value of another
-// lane (one shuffle); interleaved partners share a lane. A warp's unit is one row and kHeads heads per lane
-// group, all of the queries or all of the keys: the row's cos and sin are read once per unit, into registers,
-// and the loads of all its heads are in flight together. The backward pass keeps the weights' gradients in
-// registers over a persistent grid, sums a block's warps in shared memory in warp order and the blocks'
-// partial sums in block order in a second kernel: no atomics, the same bits every time.
+// What bounds it: memory, then the issue of instructions (about ten per value), so a lane does as little else as it
+// can. It holds two quads of a head, four whole pairs: (x_p .. x_{p+3}, x_{p+R/2} ..) or, interleaved, eight values
+// side by side, so that no pair crosses lanes and the lane needs four cosines and four sines; lanes behind the turned
+// part hold eight values and turn by (1, 0). A head is D / 8 lanes, padded to a power of two for the sums; the lane
+// groups of a warp take the heads of one row, or of several rows where a row has fewer. A warp keeps its heads (all
+// of the queries or all of the keys) and walks over the rows: weights and addresses are set up once, the next
+// position is loaded a row ahead, and the loads of all its heads are in flight together. The weights' gradients stay
+// in registers over the walk; a block adds its warps in warp order, a second kernel the blocks in block order: no
+// atomics, the same bits every time.
 
 #include <cuda_bf16.h>
 
@@ -25,10 +26,9 @@
 namespace fmd {
 namespace {
 
-constexpr int kHeads = 4;     // heads per lane group and unit: their loads are in flight together
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxDim = 128;
+constexpr int kMaxDim = 128, kMaxHeads = 1024;
 
 struct Side {
     const void* x;    // [rows, heads, D], strides row and head
@@ -36,7 +36,9 @@ struct Side {
     void* y;          // output (or the input's gradient), contiguous
     const void* w;    // [D] or null
     int64_t row, head, grow, ghead;
-    int32_t heads, units;  // units of kHeads heads per lane group
+    int32_t heads;
+    int32_t across;   // heads of a row that a warp's lane groups take at a time (a power of two)
+    int32_t units;    // warps that share a row
 };
 
 struct Args {
@@ -48,12 +50,69 @@ struct Args {
     int32_t* flags;
     int64_t rows, table;
     float eps, inv_dim;
-    int32_t dim, rot, interleaved, w_float;
+    int32_t dim, rot, w_float;
 };
 
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Pack {
-    T v[V];
+__device__ __forceinline__ void load_quad(const float* p, float (&v)[4]) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+}
+
+// the raw loads of a lane's two quads, kept packed until they are used
+template <typename T>
+struct Raw;
+
+template <>
+struct Raw<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p, int qa, int qb) {
+        a = *reinterpret_cast<const float4*>(p + qa);
+        b = *reinterpret_cast<const float4*>(p + qb);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+    static __device__ __forceinline__ void put(float* p, int qa, int qb, const float (&v)[8]) {
+        *reinterpret_cast<float4*>(p + qa) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(p + qb) = make_float4(v[4], v[5], v[6], v[7]);
+    }
+};
+
+__device__ __forceinline__ float2 halves(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+__device__ __forceinline__ uint32_t join(float low, float high) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(low, high);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <>
+struct Raw<__nv_bfloat16> {
+    uint2 a, b;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p, int qa, int qb) {
+        if (qb == qa + 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(p + qa);
+            a = make_uint2(w.x, w.y), b = make_uint2(w.z, w.w);
+        } else {
+            a = *reinterpret_cast<const uint2*>(p + qa);
+            b = *reinterpret_cast<const uint2*>(p + qb);
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const float2 f[4] = {halves(a.x), halves(a.y), halves(b.x), halves(b.y)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = f[i].x, v[2 * i + 1] = f[i].y;
+    }
+    static __device__ __forceinline__ void put(__nv_bfloat16* p, int qa, int qb, const float (&v)[8]) {
+        const uint2 a = make_uint2(join(v[0], v[1]), join(v[2], v[3])), b = make_uint2(join(v[4], v[5]), join(v[6], v[7]));
+        if (qb == qa + 4) {
+            *reinterpret_cast<uint4*>(p + qa) = make_uint4(a.x, a.y, b.x, b.y);
+        } else {
+            *reinterpret_cast<uint2*>(p + qa) = a;
+            *reinterpret_cast<uint2*>(p + qb) = b;
+        }
+    }
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -61,189 +120,172 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162f
 __device__ __forceinline__ void from_float(float& o, float v) { o = v; }
 __device__ __forceinline__ void from_float(__nv_bfloat16& o, float v) { o = __float2bfloat16_rn(v); }
 
-template <typename T, int V>
-__device__ __forceinline__ void load_weight(const Args& a, const Side& s, int c0, bool active, float (&w)[V]) {
+// Turns the lane's four pairs by their angles.
+template <bool INTER>
+__device__ __forceinline__ void turn(float (&v)[8], const float (&c)[4], const float (&s)[4]) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        w[j] = 0.0f;
-        if (s.w != nullptr && active)
-            w[j] = a.w_float ? static_cast<const float*>(s.w)[c0 + j] : to_float(static_cast<const T*>(s.w)[c0 + j]);
+    for (int i = 0; i < 4; ++i) {
+        const int p = INTER ? 2 * i : i, q = INTER ? 2 * i + 1 : i + 4;
+        const float a = v[p], b = v[q];
+        v[p] = a * c[i] - b * s[i];
+        v[q] = b * c[i] + a * s[i];
     }
 }
 
-// Turns the lane's V values by the row's angle (sign -1: back). `there` marks the lanes inside the rotated part.
-template <int V>
-__device__ __forceinline__ void turn(float (&y)[V], const float (&c)[V], const float (&s)[V], int partner, bool first,
-                                     bool there, bool interleaved, float sign) {
-    if (interleaved) {
-        if (there) {
-#pragma unroll
-            for (int j = 0; j < V; j += 2) {
-                const float p = y[j], q = y[j + 1], t = sign * s[j / 2];
-                y[j] = p * c[j / 2] - q * t;
-                y[j + 1] = q * c[j / 2] + p * t;
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float other = __shfl_sync(0xffffffffu, y[j], partner);
-        const float t = sign * (first ? -s[j] : s[j]);
-        if (there) y[j] = y[j] * c[j] + other * t;
-    }
-}
+// Blocks of an SM: the backward pass holds twice the loads and the weights' sums in registers.
+template <bool BACKWARD>
+constexpr int kResident = BACKWARD ? 2 : 3;
 
-
-template <typename T, int V, bool BACKWARD>
-__global__ void __launch_bounds__(kThreads) head_rotary_kernel(const Args a) {
+// HEADS: heads of a lane group and row whose loads are in flight together.
+template <typename T, bool INTER, bool NORM, bool BACKWARD, int HEADS>
+__global__ void __launch_bounds__(kThreads, kResident<BACKWARD>) head_rotary_kernel(const Args a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int lanes = a.dim / V;
+    const int lanes = a.dim / 8;
     int span = 1;
     while (span < lanes) span <<= 1;
     const int groups = 32 / span, group = lane / span, sub = lane % span;
     const bool active = sub < lanes;
-    const int c0 = sub * V;
     const int half = a.rot / 2;
-    const bool inter = a.interleaved != 0;
-    const bool there = active && c0 < a.rot;
-    const bool first = c0 < half;
-    const int partner = inter || !there ? lane : (first ? lane + half / V : lane - half / V);
-    const int t0 = inter ? c0 / 2 : (first ? c0 : c0 - half);
+    const bool turned = 8 * sub < a.rot;
+    const int qa = !INTER && turned ? 4 * sub : 8 * sub, qb = !INTER && turned ? half + 4 * sub : 8 * sub + 4;
+
+    // this warp's heads: unit `u` of the row's units
     const int units = a.side[0].units + a.side[1].units;
-    const int64_t total = a.rows * units;
+    const int64_t walker = int64_t(blockIdx.x) * kWarps + warp;
+    const int64_t walkers = int64_t(gridDim.x) * kWarps / units;  // warps with the same unit
+    const int64_t start = walker / units;
+    int u = int(walker - start * units);
+    const int which = u >= a.side[0].units;
+    const Side s = a.side[which];
+    if (which) u -= a.side[0].units;
+    const int across = s.across, rows_at_once = groups / across;
+    const int head0 = u * HEADS * across + group % across;
+    const int64_t row_step = walkers * rows_at_once;
 
-    float dw[2][V];
+    float w[8], dw[8];
 #pragma unroll
-    for (int j = 0; j < V; ++j) dw[0][j] = dw[1][j] = 0.0f;
-
-    for (int64_t u = int64_t(blockIdx.x) * kWarps + warp; u < total; u += int64_t(gridDim.x) * kWarps) {
-        const int64_t row = u / units;
-        int unit = int(u - row * units);
-        const int which = unit >= a.side[0].units;
-        const Side& s = a.side[which];
-        if (which) unit -= a.side[0].units;
-        const int head0 = unit * kHeads * groups + group;
-
-        Pack<T, V> x[kHeads], g[kHeads];
-        const bool need_x = !BACKWARD || s.w != nullptr;
+    for (int j = 0; j < 8; ++j) {
+        const int at = (j < 4 ? qa : qb - 4) + j;
+        dw[j] = 0.0f;
+        w[j] = 1.0f;
+        if (NORM && s.w != nullptr && active)
+            w[j] = a.w_float ? static_cast<const float*>(s.w)[at] : to_float(static_cast<const T*>(s.w)[at]);
+    }
+    const bool norm = NORM && s.w != nullptr;
+    const int64_t first = start < walkers ? start * rows_at_once + group / across : a.rows;
+    int64_t next = first < a.rows ? a.positions[first] : 0;
+    // the loop's bound is the warp's first row: its lanes stay together for the shuffles
+    for (int64_t base = start < walkers ? start * rows_at_once : a.rows; base < a.rows; base += row_step) {
+        const int64_t row = base + group / across;
+        const bool here = active && row < a.rows;
+        Raw<T> x[HEADS], g[HEADS];
 #pragma unroll
-        for (int i = 0; i < kHeads; ++i) {
-            const int h = head0 + i * groups;
-            if (active && h < s.heads) {
-                if (need_x)
-                    x[i] = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(s.x) + row * s.row +
-                                                                h * s.head + c0);
-                if (BACKWARD)
-                    g[i] = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(s.g) + row * s.grow +
-                                                                h * s.ghead + c0);
+        for (int i = 0; i < HEADS; ++i) {
+            const int h = head0 + i * across;
+            if (here && h < s.heads) {
+                if (!BACKWARD || norm) x[i].load(static_cast<const T*>(s.x) + row * s.row + h * s.head, qa, qb);
+                if (BACKWARD) g[i].load(static_cast<const T*>(s.g) + row * s.grow + h * s.ghead, qa, qb);
             }
         }
-        const int64_t pos = a.positions[row];
+        const int64_t pos = next;
+        if (row + row_step < a.rows) next = a.positions[row + row_step];
         const bool known = pos >= 0 && pos < a.table;
-        if (!known && lane == 0) raise_flag(a.flags, FMD_FLAG_INDEX_RANGE);
-        float c[V], sn[V], w[V];
+        if (!known && row < a.rows && sub == 0) raise_flag(a.flags, FMD_FLAG_INDEX_RANGE);
+        float c[4] = {1.0f, 1.0f, 1.0f, 1.0f}, sn[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (turned && here) {
+            c[0] = c[1] = c[2] = c[3] = 0.0f;
+            if (known) {
+                load_quad(a.cos + pos * half + 4 * sub, c);
+                load_quad(a.sin + pos * half + 4 * sub, sn);
+            }
+            if (BACKWARD) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) c[j] = sn[j] = 0.0f;
-        if (there && known) {
-            const float* cr = a.cos + pos * half + t0;
-            const float* sr = a.sin + pos * half + t0;
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (j < (inter ? V / 2 : V)) {
-                    c[j] = __ldg(cr + j);
-                    sn[j] = __ldg(sr + j);
-                }
+                for (int j = 0; j < 4; ++j) sn[j] = -sn[j];
+            }
         }
-        load_weight<T, V>(a, s, c0, active, w);
-
 #pragma unroll
-        for (int i = 0; i < kHeads; ++i) {
-            const int h = head0 + i * groups;
-            const bool mine = active && h < s.heads;
-            float v[V], n = 1.0f;
-            if (need_x) {
-                float sum = 0.0f;
+        for (int i = 0; i < HEADS; ++i) {
+            const int h = head0 + i * across;
+            const bool mine = here && h < s.heads;
+            if (!__any_sync(0xffffffffu, mine)) break;
+            float v[8], y[8];
+            float n = 1.0f;
+            if (!BACKWARD || norm) {
+                x[i].get(v);
+                if (norm) {
+                    float sum = 0.0f;
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    v[j] = mine ? to_float(x[i].v[j]) : 0.0f;
-                    sum += v[j] * v[j];
-                }
-                if (s.w != nullptr) {
+                    for (int j = 0; j < 8; ++j) sum += v[j] * v[j];
+                    sum = mine ? sum : 0.0f;
                     for (int o = span / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                     n = rsqrtf(sum * a.inv_dim + a.eps);
                 }
             }
-            float y[V];
             if (!BACKWARD) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) y[j] = s.w != nullptr ? v[j] * n * w[j] : v[j];
-                turn<V>(y, c, sn, partner, first, there, inter, 1.0f);
+                for (int j = 0; j < 8; ++j) y[j] = norm ? v[j] * n * w[j] : v[j];
+                turn<INTER>(y, c, sn);
             } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) y[j] = mine ? to_float(g[i].v[j]) : 0.0f;
-                turn<V>(y, c, sn, partner, first, there, inter, -1.0f);
-                if (s.w != nullptr) {
+                g[i].get(y);
+                turn<INTER>(y, c, sn);
+                if (norm) {
                     float dot = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < V; ++j) {
+                    for (int j = 0; j < 8; ++j) {
                         v[j] *= n;  // u
                         const float t = y[j] * v[j];
-                        if (which) dw[1][j] += t;
-                        else dw[0][j] += t;
+                        dw[j] += mine ? t : 0.0f;
+                        dot += t * w[j];
                         y[j] *= w[j];
-                        dot += y[j] * v[j];
                     }
+                    dot = mine ? dot : 0.0f;
                     for (int o = span / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
                     dot *= a.inv_dim;
 #pragma unroll
-                    for (int j = 0; j < V; ++j) y[j] = n * (y[j] - v[j] * dot);
+                    for (int j = 0; j < 8; ++j) y[j] = n * (y[j] - v[j] * dot);
                 }
             }
-            if (mine) {
-                Pack<T, V> o;
-#pragma unroll
-                for (int j = 0; j < V; ++j) from_float(o.v[j], y[j]);
-                *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(s.y) + (row * s.heads + h) * a.dim + c0) = o;
-            }
+            if (mine) Raw<T>::put(static_cast<T*>(s.y) + (row * s.heads + h) * a.dim, qa, qb, y);
         }
     }
 
-    if (BACKWARD && a.partial != nullptr) {
-        __shared__ float sums[kWarps][2][kMaxDim];
+    if (BACKWARD && NORM && a.partial != nullptr) {
+        __shared__ float sums[kWarps][kMaxDim];
+        __shared__ int side_of[kWarps];
 #pragma unroll
-        for (int side = 0; side < 2; ++side)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float t = dw[side][j];
-                for (int o = 16; o >= span; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-                if (group == 0 && active) sums[warp][side][c0 + j] = t;
-            }
+        for (int j = 0; j < 8; ++j) {
+            float t = dw[j];
+            for (int o = 16; o >= span; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            if (group == 0 && active) sums[warp][(j < 4 ? qa : qb - 4) + j] = t;
+        }
+        if (lane == 0) side_of[warp] = which;
         __syncthreads();
         for (int i = threadIdx.x; i < 2 * a.dim; i += kThreads) {
             const int side = i / a.dim, col = i - side * a.dim;
             float t = 0.0f;
-            for (int k = 0; k < kWarps; ++k) t += sums[k][side][col];
-            a.partial[(int64_t(blockIdx.x) * 2 + side) * a.dim + col] = t;
+            for (int k = 0; k < kWarps; ++k) t += side_of[k] == side ? sums[k][col] : 0.0f;
+            a.partial[int64_t(blockIdx.x) * 2 * a.dim + i] = t;
         }
     }
 }
 
-// dw[side][col] = the blocks' partial sums in a fixed order: warp w of a block of 8 adds blocks w, w + 8, ..,
-// then the warps are added in order. One block per 32 columns.
+// dw[side][col] = the blocks' partial sums in a fixed order: warp w of 32 adds blocks w, w + 32, .., then the warps
+// are added in order. One block per 32 columns.
 template <typename W>
-__global__ void __launch_bounds__(kThreads) weight_sum_kernel(const float* partial, int blocks, int dim, W* dq, W* dk) {
-    __shared__ float sums[kWarps][32];
+__global__ void __launch_bounds__(1024) weight_sum_kernel(const float* partial, int blocks, int dim, W* dq, W* dk) {
+    __shared__ float sums[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int i = blockIdx.x * 32 + lane;
     float t = 0.0f;
-    if (i < 2 * dim)
-        for (int b = warp; b < blocks; b += kWarps) t += partial[int64_t(b) * 2 * dim + i];
+    if (i < 2 * dim) {
+#pragma unroll 8
+        for (int b = warp; b < blocks; b += 32) t += partial[int64_t(b) * 2 * dim + i];
+    }
     sums[warp][lane] = t;
     __syncthreads();
     if (warp == 0 && i < 2 * dim) {
         float r = 0.0f;
-        for (int k = 0; k < kWarps; ++k) r += sums[k][lane];
+        for (int k = 0; k < 32; ++k) r += sums[k][lane];
         if (i < dim) {
             if (dq != nullptr) from_float(dq[i], r);
         } else if (dk != nullptr) {
@@ -252,13 +294,42 @@ __global__ void __launch_bounds__(kThreads) weight_sum_kernel(const float* parti
     }
 }
 
-constexpr int kBackwardBlocks = kNumSMs * 4;
+// Heads per lane group whose loads are in flight together: 16 bytes of each in 16 bits, 32 in 32.
+template <typename T, bool BACKWARD>
+constexpr int kHeadsOf = sizeof(T) == 2 && !BACKWARD ? 4 : 2;
 
-template <typename T, int V>
-fmd_status launch(const Args& a, bool backward, int grid, cudaStream_t s) {
-    if (backward) head_rotary_kernel<T, V, true><<<grid, kThreads, 0, s>>>(a);
-    else head_rotary_kernel<T, V, false><<<grid, kThreads, 0, s>>>(a);
+template <typename T, bool INTER, bool NORM, bool BACKWARD>
+fmd_status launch(Args& a, int* blocks, cudaStream_t s) {
+    constexpr int H = kHeadsOf<T, BACKWARD>;
+    int span = 1;
+    while (span * 8 < a.dim) span <<= 1;
+    const int groups = 32 / span;
+    int rows_at_once = groups;  // of the side that takes the fewest: its warps walk the furthest
+    for (Side& q : a.side) {
+        q.across = 1;
+        while (q.across < groups && q.across < q.heads) q.across <<= 1;
+        q.units = (q.heads + H * q.across - 1) / (H * q.across);
+        if (q.heads > 0 && groups / q.across < rows_at_once) rows_at_once = groups / q.across;
+    }
+    const int units = a.side[0].units + a.side[1].units;
+    *blocks = 0;
+    if (a.rows == 0 || units == 0) return FMD_OK;
+    // all blocks resident, and a warp at least for every unit: kMaxHeads heads are fewer units than the grid's warps
+    const int64_t wanted = ((a.rows + rows_at_once - 1) / rows_at_once * units + kWarps - 1) / kWarps;
+    const int most = kNumSMs * kResident<BACKWARD>;
+    *blocks = int(wanted < most ? wanted : most);
+    head_rotary_kernel<T, INTER, NORM, BACKWARD, H><<<*blocks, kThreads, 0, s>>>(a);
     return check_launch();
+}
+
+template <typename T>
+fmd_status launch(Args& a, bool inter, bool norm, bool backward, int* blocks, cudaStream_t s) {
+    if (backward) {
+        if (inter) return norm ? launch<T, true, true, true>(a, blocks, s) : launch<T, true, false, true>(a, blocks, s);
+        return norm ? launch<T, false, true, true>(a, blocks, s) : launch<T, false, false, true>(a, blocks, s);
+    }
+    if (inter) return norm ? launch<T, true, true, false>(a, blocks, s) : launch<T, true, false, false>(a, blocks, s);
+    return norm ? launch<T, false, true, false>(a, blocks, s) : launch<T, false, false, false>(a, blocks, s);
 }
 
 bool vector_rows(const void* p, int64_t row, int64_t head, int size) {
@@ -274,7 +345,7 @@ extern "C" {
 
 fmd_status fmd_head_rotary_workspace_bytes(int32_t dim, size_t* bytes) {
     if (bytes == nullptr || dim < 8 || dim > kMaxDim || dim % 8) return FMD_ERR_INVALID_ARGUMENT;
-    *bytes = size_t(kBackwardBlocks) * 2 * dim * sizeof(float);
+    *bytes = size_t(kNumSMs * kResident<true>) * 2 * dim * sizeof(float);
     return FMD_OK;
 }
 
@@ -287,10 +358,6 @@ fmd_status fmd_head_rotary(const fmd_head_rotary_side* sides, int32_t type, int3
         return FMD_ERR_INVALID_ARGUMENT;
     const bool norm = sides[0].w != nullptr || sides[1].w != nullptr;
     const int size = type == FMD_F32 ? 4 : 2;
-    const int v = type == FMD_F32 ? 4 : (interleaved || rot % 16 == 0) ? 8 : 4;
-    int span = 1;
-    while (span * v < dim) span <<= 1;
-    const int per_unit = 32 / span * kHeads;
     Args a{};
     bool any = false;
     for (int i = 0; i < 2; ++i) {
@@ -301,12 +368,11 @@ fmd_status fmd_head_rotary(const fmd_head_rotary_side* sides, int32_t type, int3
             if (q.y == nullptr || (!backward && q.x == nullptr) ||
                 (backward && (q.g == nullptr || (q.w != nullptr && q.x == nullptr))))
                 return FMD_ERR_INVALID_ARGUMENT;
-            if (!aligned16(q.y) || (q.x != nullptr && !vector_rows(q.x, q.row_stride, q.head_stride, size)) ||
+            if (q.heads > kMaxHeads || !aligned16(q.y) || (q.x != nullptr && !vector_rows(q.x, q.row_stride, q.head_stride, size)) ||
                 (backward && !vector_rows(q.g, q.g_row_stride, q.g_head_stride, size)))
                 return FMD_ERR_UNSUPPORTED;
         }
-        a.side[i] = Side{q.x, q.g, q.y, q.w, q.row_stride, q.head_stride, q.g_row_stride, q.g_head_stride, q.heads,
-                         (q.heads + per_unit - 1) / per_unit};
+        a.side[i] = Side{q.x, q.g, q.y, q.w, q.row_stride, q.head_stride, q.g_row_stride, q.g_head_stride, q.heads, 1, 0};
     }
     const bool weights = backward && norm;
     if (weights) {
@@ -314,9 +380,9 @@ fmd_status fmd_head_rotary(const fmd_head_rotary_side* sides, int32_t type, int3
         fmd_head_rotary_workspace_bytes(dim, &need);
         if (workspace == nullptr || workspace_bytes < need) return FMD_ERR_WORKSPACE;
     }
-    const int64_t units = rows * (a.side[0].units + a.side[1].units);
     if (rows > 0 && any && (positions == nullptr || (table > 0 && (cos == nullptr || sin == nullptr))))
         return FMD_ERR_INVALID_ARGUMENT;
+    if (rows > 0 && any && (!aligned16(cos) || !aligned16(sin))) return FMD_ERR_UNSUPPORTED;
     a.positions = positions;
     a.cos = cos;
     a.sin = sin;
@@ -328,29 +394,22 @@ fmd_status fmd_head_rotary(const fmd_head_rotary_side* sides, int32_t type, int3
     a.inv_dim = 1.0f / float(dim);
     a.dim = dim;
     a.rot = rot;
-    a.interleaved = interleaved != 0;
     a.w_float = weight_type == FMD_F32;
     const cudaStream_t s = as_stream(stream);
-    int64_t blocks = (units + kWarps - 1) / kWarps;
-    if (backward && blocks > kBackwardBlocks) blocks = kBackwardBlocks;
-    if (blocks > INT32_MAX) return FMD_ERR_UNSUPPORTED;
-    if (blocks > 0) {
-        fmd_status st;
-        if (type == FMD_F32) st = launch<float, 4>(a, backward, int(blocks), s);
-        else if (v == 8) st = launch<__nv_bfloat16, 8>(a, backward, int(blocks), s);
-        else st = launch<__nv_bfloat16, 4>(a, backward, int(blocks), s);
-        if (st != FMD_OK) return st;
-    }
+    int blocks = 0;
+    const fmd_status st = type == FMD_F32 ? launch<float>(a, interleaved != 0, norm, backward != 0, &blocks, s)
+                                          : launch<__nv_bfloat16>(a, interleaved != 0, norm, backward != 0, &blocks, s);
+    if (st != FMD_OK) return st;
     if (weights) {
         const int grid = (2 * dim + 31) / 32;
         if (weight_type == FMD_F32)
-            weight_sum_kernel<float><<<grid, kThreads, 0, s>>>(a.partial, int(blocks), dim,
-                                                               static_cast<float*>(sides[0].dw),
-                                                               static_cast<float*>(sides[1].dw));
+            weight_sum_kernel<float><<<grid, 1024, 0, s>>>(a.partial, blocks, dim,
+                                                           static_cast<float*>(sides[0].dw),
+                                                           static_cast<float*>(sides[1].dw));
         else
-            weight_sum_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(a.partial, int(blocks), dim,
-                                                                       static_cast<__nv_bfloat16*>(sides[0].dw),
-                                                                       static_cast<__nv_bfloat16*>(sides[1].dw));
+            weight_sum_kernel<__nv_bfloat16><<<grid, 1024, 0, s>>>(a.partial, blocks, dim,
+                                                                   static_cast<__nv_bfloat16*>(sides[0].dw),
+                                                                   static_cast<__nv_bfloat16*>(sides[1].dw));
         return check_launch();
     }
     return FMD_OK;

@@ -52,6 +52,11 @@ def _head_rows(x: Tensor) -> Tensor:
     return x.clone(memory_format=torch.contiguous_format)
 
 
+def _aligned(table: Tensor) -> Tensor:
+    table = table.contiguous()
+    return table.clone() if table.data_ptr() % 16 else table
+
+
 def _launch(sides, x, weight_type, rot, interleaved, eps, positions, cos, sin, backward):
     rows, _, dim = x.shape
     workspace = None
@@ -138,6 +143,8 @@ def head_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, cos: Tensor, sin: 
     rows, _, dim = q.shape
     if dim % 8 or not 8 <= dim <= 128:
         raise ValueError(f"the head size must be a multiple of 8 up to 128, got {dim}")
+    if max(q.shape[1], k.shape[1]) > 1024:
+        raise ValueError(f"at most 1024 heads, got {q.shape[1]} and {k.shape[1]}")
     if positions.shape != (rows,) or positions.dtype != torch.int64:
         raise ValueError(f"positions must be int64 [{rows}], got {positions.dtype} {tuple(positions.shape)}")
     if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
@@ -150,7 +157,7 @@ def head_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, cos: Tensor, sin: 
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise ValueError("both norm weights must have the same type")
     weights = [w if w is None or w.is_contiguous() else w.contiguous() for w in (q_weight, k_weight)]
-    args = (_head_rows(q), _head_rows(k), positions.contiguous(), cos.contiguous(), sin.contiguous(), *weights,
+    args = (_head_rows(q), _head_rows(k), positions.contiguous(), _aligned(cos), _aligned(sin), *weights,
             float(eps), bool(interleaved))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, *weights)):
         return _HeadNormRotary.apply(*args)
