@@ -134,7 +134,8 @@ _SIGNATURES: dict[str, list] = {
     "fmd_head_rotary_workspace_bytes": [_I32, POINTER(c_size_t)],
     "fmd_head_rotary": [POINTER(FmdHeadRotarySide), _I32, _I32, _I64, _I32, _I32, _I32, c_float, _P, _P, _P, _I64,
                         _I32, _P, c_size_t, _P, _P],
-    "fmd_packed_attention": [POINTER(FmdAttention), _P, _P, _P, _P],
+    "fmd_packed_attention_workspace_bytes": [POINTER(FmdAttention), POINTER(c_size_t)],
+    "fmd_packed_attention": [POINTER(FmdAttention), _P, _P, _P, c_size_t, _P, _P],
     "fmd_packed_attention_bwd": [POINTER(FmdAttention), _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P],
     "fmd_nhc_pre_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P],
     "fmd_nhc_post_pre_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P],

@@ -74,6 +74,11 @@ fmd_status check(const fmd_attention& q, Attn& a) {
     return FMD_OK;
 }
 
+size_t workspace_bytes(const Attn& a, int type) {
+    const int splits = type == FMD_BF16 ? attention_splits(a) : 1;
+    return splits > 1 ? size_t(splits) * a.rows * a.hq * (a.dim + 1) * sizeof(float) : 0;
+}
+
 }  // namespace
 }  // namespace fmd
 
@@ -81,7 +86,16 @@ using namespace fmd;
 
 extern "C" {
 
-fmd_status fmd_packed_attention(const fmd_attention* problem, void* out, float* lse, int32_t* flags, void* stream) {
+fmd_status fmd_packed_attention_workspace_bytes(const fmd_attention* problem, size_t* bytes) {
+    Attn a;
+    if (problem == nullptr || bytes == nullptr) return FMD_ERR_INVALID_ARGUMENT;
+    const fmd_status st = check(*problem, a);
+    if (st == FMD_OK) *bytes = workspace_bytes(a, problem->type);
+    return st;
+}
+
+fmd_status fmd_packed_attention(const fmd_attention* problem, void* out, float* lse, void* workspace,
+                                size_t workspace_size, int32_t* flags, void* stream) {
     Attn a;
     if (problem == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     fmd_status st = check(*problem, a);
@@ -89,9 +103,15 @@ fmd_status fmd_packed_attention(const fmd_attention* problem, void* out, float* 
     if (a.rows == 0) return FMD_OK;
     if (out == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     if (!aligned16(out)) return FMD_ERR_UNSUPPORTED;
+    if (workspace_size < workspace_bytes(a, problem->type)) return FMD_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return FMD_ERR_UNSUPPORTED;
     a.out = out;
     a.lse = lse;
     a.flags = flags;
+    if (problem->type == FMD_BF16) {
+        a.part = static_cast<float*>(workspace);
+        a.part_lse = a.part + int64_t(attention_splits(a)) * a.rows * a.hq * a.dim;
+    }
     if (problem->type == FMD_BF16) return attention_forward_mma(a, as_stream(stream));
     return attention_forward_simt(a, problem->type, as_stream(stream));
 }

@@ -32,6 +32,8 @@ struct Attn {
     void* dq;           // [rows, hq, dim] contiguous
     void* dk;           // [keys, hk, dim] contiguous
     void* dv;
+    float* part;        // [splits, rows, hq, dim] and
+    float* part_lse;    // [splits, rows, hq]: the splits of the keys, workspace
     const int64_t* offsets;      // [batch + 1] tokens
     const int64_t* key_offsets;  // [batch + 1]
     const int64_t* key_counts;   // [batch] or null: the whole slot
@@ -101,6 +103,7 @@ __device__ __forceinline__ void attn_store(__nv_bfloat16* p, float v) { *p = __f
 fmd_status attention_forward_simt(const Attn& a, int type, cudaStream_t s);
 fmd_status attention_backward_simt(const Attn& a, int type, cudaStream_t s);
 fmd_status attention_forward_mma(const Attn& a, cudaStream_t s);   // bfloat16
+int attention_splits(const Attn& a);                               // of the forward pass in bfloat16
 fmd_status attention_backward_mma(const Attn& a, cudaStream_t s);  // bfloat16
 
 }  // namespace fmd

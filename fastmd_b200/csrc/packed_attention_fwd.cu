@@ -55,7 +55,7 @@ struct Maps {
     CUtensorMap q, k, v;
 };
 
-template <int KS, int NT>
+template <int KS, int NT, bool SPLIT>
 __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
     forward_kernel(const __grid_constant__ Maps maps, const Attn a) {
     using S = Shape<KS, NT>;
@@ -83,7 +83,27 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
         counts[t] = (ends[t] + kTile - 1) / kTile;
         last = max(last, counts[t]);
     }
-    const int keys = int(s.keys);
+    // a split takes a range of the key tiles; from here on everything counts from its first key
+    int from = 0;
+    if (SPLIT) {
+        const int share = (last + int(gridDim.z) - 1) / int(gridDim.z);
+        from = min(last, int(blockIdx.z) * share) * kTile;
+        const int to = min(last, int(blockIdx.z + 1) * share) * kTile;
+        last = 0;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            ends[t] = max(0, min(ends[t], to) - from);
+            counts[t] = (ends[t] + kTile - 1) / kTile;
+            last = max(last, counts[t]);
+        }
+        if (last == 0) {  // nothing to add: a sum of zero
+            for (int r = threadIdx.x; r < tokens[0] * a.group; r += blockDim.x)
+                a.part_lse[(int64_t(blockIdx.z) * a.rows + s.row0 + token0 + r / a.group) * a.hq + head * a.group +
+                           r % a.group] = -INFINITY;
+            return;
+        }
+    }
+    const int keys = int(s.keys) - from;
     // the last key tile read holds rows behind the sequence's last key
     const bool tail = last > 0 && keys < last * kTile;
 
@@ -137,7 +157,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
                 mbar_expect_tx(&ctl.full[slot], S::kTileBytes);
                 for (int p = 0; p < S::kPanels; ++p)
                     tma_load_4d(su32(ring + slot * S::kTileBytes + p * kPanelBytes), i & 1 ? &maps.v : &maps.k,
-                                &ctl.full[slot], p * 64, 0, head, int(s.key0) + (i >> 1) * kTile);
+                                &ctl.full[slot], p * 64, 0, head, int(s.key0) + from + (i >> 1) * kTile);
                 armed = i + 1;
                 if (++slot == S::kSlots) {
                     slot = 0;
@@ -233,7 +253,9 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
         const uint32_t at_s = tmem + lanes + t * 128u, at_o = tmem + lanes + S::kO + uint32_t(t) * S::kDim;
         const int token = r / a.group;
         const bool real = token < tokens[t];
-        const int limit = real ? int(seen(s, a.causal, token0 + t * per_tile + token)) : 0;
+        // keys (from the first of the split) that the row sees
+        const int limit = real ? min(max(int(seen(s, a.causal, token0 + t * per_tile + token)) - from, 0), ends[t]) : 0;
+        const bool idle = !__any_sync(0xffffffffu, limit > 0);  // a warp without rows passes the scores on unread
         const float c = a.scale * kLog2e;
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
@@ -245,6 +267,10 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
                 break;
             }
             tc_fence_after();
+            if (idle) {
+                mbar_arrive(&ctl.weights[t]);
+                continue;
+            }
             const int chunks = min(4, (ends[t] - j * kTile + 31) / 32);
             const int mine = limit - j * kTile;  // columns of this tile that the row sees
             const bool masked = __any_sync(0xffffffffu, mine < chunks * 32);
@@ -308,26 +334,36 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
             tc_fence_after();
         }
         if (ok && tokens[t] > 0) {
-            const int64_t flat = (s.row0 + token0 + t * per_tile + token) * a.hq + head * a.group + r % a.group;
-            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + flat * a.dim;
+            int64_t flat = (s.row0 + token0 + t * per_tile + token) * a.hq + head * a.group + r % a.group;
             // a row without keys: zeros; a sum that is not a number stays one
             const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+            const float lse = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+            if (SPLIT) flat += int64_t(blockIdx.z) * a.rows * a.hq;
             for (int ch = 0; ch < S::kDim / 32; ++ch) {
                 float o[32];
-                if (counts[t] > 0) {
-                    tmem_load32(at_o + ch * 32, o);
-                }
+                if (counts[t] > 0) tmem_load32(at_o + ch * 32, o);
                 if (!real) continue;
+                if (SPLIT) {
+                    float* part = a.part + flat * a.dim + ch * 32;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        if (limit > 0 && ch * 32 + i < a.dim)
+                            *reinterpret_cast<float4*>(part + i) =
+                                make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+                    continue;
+                }
+                __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + flat * a.dim + ch * 32;
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
                     uint4 w = make_uint4(0, 0, 0, 0);
                     if (limit > 0)
                         w = make_uint4(pack_bf16(o[i] * inv, o[i + 1] * inv), pack_bf16(o[i + 2] * inv, o[i + 3] * inv),
                                        pack_bf16(o[i + 4] * inv, o[i + 5] * inv), pack_bf16(o[i + 6] * inv, o[i + 7] * inv));
-                    if (ch * 32 + i < a.dim) *reinterpret_cast<uint4*>(out + ch * 32 + i) = w;
+                    if (ch * 32 + i < a.dim) *reinterpret_cast<uint4*>(out + i) = w;
                 }
             }
-            if (real && a.lse != nullptr) a.lse[flat] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+            if (real && SPLIT) a.part_lse[flat] = lse;
+            if (real && !SPLIT && a.lse != nullptr) a.lse[flat] = lse;
         }
     }
 
@@ -341,14 +377,51 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
     if (threadIdx.x == 0 && ctl.abort) raise_flag(a.flags, FMD_FLAG_WAIT_TIMEOUT);
 }
 
-template <int KS, int NT>
-fmd_status launch(const Maps& maps, const Attn& a, cudaStream_t s) {
+// out and lse of the splits together: out = sum_z 2^(lse_z - lse) out_z. A thread per row and four values.
+__global__ void __launch_bounds__(256) join_kernel(const Attn a, int splits) {
+    const int quads = a.dim / 4;
+    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x, all = a.rows * a.hq, row = i / quads;
+    const int quad = int(i - row * quads);
+    if (row >= all) return;
+    float top = -INFINITY;
+    for (int z = 0; z < splits; ++z) top = fmaxf(top, a.part_lse[z * all + row]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    float4 o = f4_zero();
+    for (int z = 0; z < splits; ++z) {
+        const float lse = a.part_lse[z * all + row];
+        if (lse == -INFINITY) continue;  // a split without keys of this row wrote nothing else
+        const float w = exp2f((lse - base) * kLog2e);
+        const float4 v = *reinterpret_cast<const float4*>(a.part + (z * all + row) * a.dim + quad * 4);
+        sum += w;
+        o = make_float4(fmaf(w, v.x, o.x), fmaf(w, v.y, o.y), fmaf(w, v.z, o.z), fmaf(w, v.w, o.w));
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + row * a.dim + quad * 4) =
+        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    if (quad == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? -INFINITY : top + logf(sum);
+}
+
+template <int KS, int NT, bool SPLIT>
+fmd_status launch(const Maps& maps, const Attn& a, int splits, cudaStream_t s) {
     using S = Shape<KS, NT>;
-    const fmd_status st = grant_dynamic_smem((const void*)forward_kernel<KS, NT>, S::kBytes, true);
+    fmd_status st = grant_dynamic_smem((const void*)forward_kernel<KS, NT, SPLIT>, S::kBytes, true);
     if (st != FMD_OK) return st;
     const int64_t tiles = tile_bound(a.rows, a.batch, NT * (kTile / a.group));
-    forward_kernel<KS, NT><<<dim3(unsigned(tiles), unsigned(a.hk)), S::kThreads, S::kBytes, s>>>(maps, a);
+    forward_kernel<KS, NT, SPLIT>
+        <<<dim3(unsigned(tiles), unsigned(a.hk), unsigned(splits)), S::kThreads, S::kBytes, s>>>(maps, a);
+    st = check_launch();
+    if (!SPLIT || st != FMD_OK) return st;
+    const int64_t threads = a.rows * a.hq * (a.dim / 4);
+    join_kernel<<<unsigned((threads + 255) / 256), 256, 0, s>>>(a, splits);
     return check_launch();
+}
+
+template <int KS>
+fmd_status launch(const Maps& maps, const Attn& a, int splits, cudaStream_t s) {
+    if (splits > 1) return launch<KS, 1, true>(maps, a, splits, s);
+    const bool two = tile_bound(a.rows, a.batch, 2 * (kTile / a.group)) * a.hk >= kNumSMs;
+    return two ? launch<KS, 2, false>(maps, a, 1, s) : launch<KS, 1, false>(maps, a, 1, s);
 }
 
 }  // namespace
@@ -380,11 +453,20 @@ fmd_status attention_forward_mma(const Attn& a, cudaStream_t s) {
         if (st == FMD_OK) st = encode_packed(drv, &maps.v, a.v, a.keys, a.hk, 1, a.dim, a.v_row, a.v_head, kTile);
     }
     if (st != FMD_OK) return st;
-    const bool two = tile_bound(a.rows, a.batch, 2 * (kTile / a.group)) * a.hk >= kNumSMs;
-    if (a.dim <= 32) return two ? launch<2, 2>(maps, a, s) : launch<2, 1>(maps, a, s);
-    if (a.dim <= 64) return two ? launch<4, 2>(maps, a, s) : launch<4, 1>(maps, a, s);
-    if (a.dim <= 96) return two ? launch<6, 2>(maps, a, s) : launch<6, 1>(maps, a, s);
-    return two ? launch<8, 2>(maps, a, s) : launch<8, 1>(maps, a, s);
+    const int splits = attention_splits(a);
+    return a.dim <= 32 ? launch<2>(maps, a, splits, s) : a.dim <= 64 ? launch<4>(maps, a, splits, s)
+         : a.dim <= 96 ? launch<6>(maps, a, splits, s) : launch<8>(maps, a, splits, s);
+}
+
+// Splits of the keys: where the tiles of rows do not fill the SMs twice over, their keys are shared out. The lengths
+// are on the device: the host goes by the mean length of a sequence's slot, and a split has two key tiles at least.
+int attention_splits(const Attn& a) {
+    const int64_t tiles = tile_bound(a.rows, a.batch, kTile / a.group) * a.hk;
+    if (tiles == 0 || a.batch == 0) return 1;
+    const int64_t key_tiles = (a.keys / a.batch + kTile - 1) / kTile;
+    int64_t splits = 2 * kNumSMs / tiles;
+    if (splits > key_tiles / 2) splits = key_tiles / 2;
+    return splits < 1 ? 1 : splits > 64 ? 64 : int(splits);
 }
 
 }  // namespace fmd

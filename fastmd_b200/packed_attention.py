@@ -14,7 +14,7 @@ from torch import Tensor
 from torch.autograd import Function
 
 from . import _lib
-from ._lib import FmdAttention, call, ptr, stream
+from ._lib import FmdAttention, c_size_t, call, ptr, stream
 from .head_rotary import TYPES, _head_rows
 
 
@@ -29,7 +29,10 @@ def _forward(q, k, v, offsets, key_offsets, key_counts, causal, scale, lse):
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     sums = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32) if lse else None
     problem = _problem(q, k, v, offsets, key_offsets, key_counts, causal, scale)
-    call("fmd_packed_attention", problem, ptr(out), ptr(sums), ptr(_lib.flags_word(q.device)), stream(q.device))
+    nbytes = c_size_t()
+    call("fmd_packed_attention_workspace_bytes", problem, nbytes)
+    workspace = torch.empty(nbytes.value, device=q.device, dtype=torch.uint8) if nbytes.value else None
+    call("fmd_packed_attention", problem, ptr(out), ptr(sums), ptr(workspace), nbytes.value, ptr(_lib.flags_word(q.device)), stream(q.device))
     return out, sums
 
 

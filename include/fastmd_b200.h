@@ -1102,12 +1102,15 @@ typedef struct fmd_attention {
     int32_t type, batch, heads, key_heads, dim, causal, _pad;
 } fmd_attention;
 
+/* Workspace of fmd_packed_attention (0: none), from the sizes alone. */
+FMD_API fmd_status fmd_packed_attention_workspace_bytes(const fmd_attention* problem, size_t* bytes);
+
 /* out [rows, heads, dim] = softmax(scale q k^T) v over the keys each row
  * sees, and lse [rows, heads] = the logarithm of the softmax's denominator
  * (NULL: not written). A row that sees no key gets out = 0, lse = -inf. No
  * reference counterpart (nor has the backward pass). */
-FMD_API fmd_status fmd_packed_attention(const fmd_attention* problem, void* out, float* lse, int32_t* flags,
-                                        void* stream);
+FMD_API fmd_status fmd_packed_attention(const fmd_attention* problem, void* out, float* lse, void* workspace,
+                                        size_t workspace_bytes, int32_t* flags, void* stream);
 
 /* Gradients of q (dq, [rows, heads, dim], or NULL) and of k and v (dk, dv,
  * [keys, key_heads, dim], or both NULL; slot rows behind a count get zeros)

@@ -364,11 +364,11 @@ def test_abi_refuses_on_the_host():
     base = dict(q=1 << 20, k=1 << 20, v=1 << 20, offsets=1 << 20, key_offsets=1 << 20, key_counts=None, rows=0, keys=0,
                 q_row=64, q_head=64, k_row=64, k_head=64, v_row=64, v_head=64, scale=0.125, type=1, batch=1, heads=1,
                 key_heads=1, dim=64, causal=0)
-    assert lib.fmd_packed_attention(_lib.FmdAttention(**base), None, None, None, None) == 0  # no rows
+    assert lib.fmd_packed_attention(_lib.FmdAttention(**base), None, None, None, 0, None, None) == 0  # no rows
     for bad in (dict(type=2), dict(heads=3, key_heads=2), dict(key_heads=0), dict(dim=12), dict(dim=136),
                 dict(rows=-1), dict(batch=0, rows=1), dict(rows=1, q=None), dict(keys=1, v=None),
                 dict(offsets=None), dict(heads=65)):
-        assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | bad)), None, None, None, None) == 1
+        assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | bad)), None, None, None, 0, None, None) == 1
     for bad in (dict(rows=1, q=(1 << 20) + 2), dict(keys=1, k_row=65), dict(rows=1, q_head=4), dict(rows=1 << 40)):
-        assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | bad)), 1 << 20, None, None, None) == 3
-    assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | dict(rows=1))), None, None, None, None) == 1
+        assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | bad)), 1 << 20, None, None, 0, None, None) == 3
+    assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | dict(rows=1))), None, None, None, 0, None, None) == 1
