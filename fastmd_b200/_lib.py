@@ -134,9 +134,9 @@ _SIGNATURES: dict[str, list] = {
     "fmd_head_rotary_workspace_bytes": [_I32, POINTER(c_size_t)],
     "fmd_head_rotary": [POINTER(FmdHeadRotarySide), _I32, _I32, _I64, _I32, _I32, _I32, c_float, _P, _P, _P, _I64,
                         _I32, _P, c_size_t, _P, _P],
-    "fmd_packed_attention_workspace_bytes": [POINTER(FmdAttention), POINTER(c_size_t)],
+    "fmd_packed_attention_workspace_bytes": [POINTER(FmdAttention), _I32, POINTER(c_size_t)],
     "fmd_packed_attention": [POINTER(FmdAttention), _P, _P, _P, c_size_t, _P, _P],
-    "fmd_packed_attention_bwd": [POINTER(FmdAttention), _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P],
+    "fmd_packed_attention_bwd": [POINTER(FmdAttention), _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, c_size_t, _P, _P],
     "fmd_nhc_pre_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P],
     "fmd_nhc_post_pre_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P],
     "fmd_nhc_post_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P],
@@ -222,7 +222,9 @@ def ptr(tensor) -> int | None:
 
 def stream(device=None) -> int:
     """The handle of torch's current CUDA stream (kernels are launched on it)."""
-    return torch.cuda.current_stream(device).cuda_stream
+    index = getattr(device, "index", None)
+    # the raw handle: building the Stream object of current_stream() takes 2 us a call
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def require_cuda(*tensors) -> None:

@@ -8,6 +8,41 @@ namespace {
 
 constexpr int kThreads = 256;
 
+__device__ __forceinline__ float attn_float(float v) { return v; }
+__device__ __forceinline__ float attn_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+__device__ __forceinline__ void store4(float* p, float4 v) { st4(p, v); }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(p) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// out and lse of the splits of the keys together: out = sum_z exp(lse_z - lse) out_z. A thread per row and four values.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Attn a, int splits) {
+    const int quads = a.dim / 4;
+    const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x, all = a.rows * a.hq, row = i / quads;
+    const int quad = int(i - row * quads);
+    if (row >= all) return;
+    float top = -INFINITY;
+    for (int z = 0; z < splits; ++z) top = fmaxf(top, a.part_lse[z * all + row]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    float4 o = f4_zero();
+    for (int z = 0; z < splits; ++z) {
+        const float lse = a.part_lse[z * all + row];
+        if (lse == -INFINITY) continue;  // a split without keys of this row wrote nothing else
+        const float w = exp2f((lse - base) * kLog2e);
+        const float4 v = *reinterpret_cast<const float4*>(a.part + (z * all + row) * a.dim + quad * 4);
+        sum += w;
+        o = make_float4(fmaf(w, v.x, o.x), fmaf(w, v.y, o.y), fmaf(w, v.z, o.z), fmaf(w, v.w, o.w));
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+    store4(static_cast<T*>(a.out) + row * a.dim + quad * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    if (quad == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? -INFINITY : top + logf(sum);
+}
+
 // delta[row] = sum_d g out - (gradient of lse): 8 lanes per packed row, 16-byte loads.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) delta_kernel(const Attn a, const float* glse, float* delta) {
@@ -47,7 +82,7 @@ fmd_status check(const fmd_attention& q, Attn& a) {
     const int size = q.type == FMD_F32 ? 4 : 2;
     if ((q.rows > 0 && !rows16(q.q, q.q_row, q.q_head, size)) ||
         (q.keys > 0 && (!rows16(q.k, q.k_row, q.k_head, size) || !rows16(q.v, q.v_row, q.v_head, size))) ||
-        q.key_heads > 65535 || q.rows > INT32_MAX || q.keys > INT32_MAX || q.batch > (1 << 24))
+        q.key_heads > 65535 || q.rows > (1 << 29) || q.keys > (1 << 29) || q.batch > (1 << 24))
         return FMD_ERR_UNSUPPORTED;
     a = Attn{};
     a.q = q.q;
@@ -74,9 +109,31 @@ fmd_status check(const fmd_attention& q, Attn& a) {
     return FMD_OK;
 }
 
-size_t workspace_bytes(const Attn& a, int type) {
-    const int splits = type == FMD_BF16 ? attention_splits(a) : 1;
-    return splits > 1 ? size_t(splits) * a.rows * a.hq * (a.dim + 1) * sizeof(float) : 0;
+// float32 heads of up to this many values go through planes on the tensor cores
+constexpr int kPlanesDim = 64;
+
+// How the forward pass runs, from the sizes alone: its splits of the keys, and its workspace: planes, then the splits.
+struct Plan {
+    int splits;
+    size_t planes, bytes;
+};
+
+Plan plan(const Attn& a, int type) {
+    Plan p{1, 0, 0};
+    if (a.rows == 0) return p;
+    const bool planes = type == FMD_F32 && a.dim <= kPlanesDim;
+    // one block an SM by its shared memory, or two
+    if (type == FMD_BF16) p.splits = attention_splits_mma(a);
+    else p.splits = key_splits(a, (planes ? 128 : 64) / a.group, kNumSMs, 256);
+    if (planes) p.planes = attention_planes_bytes(a, false);
+    p.bytes = p.planes + (p.splits > 1 ? size_t(p.splits) * a.rows * a.hq * (a.dim + 1) * sizeof(float) : 0);
+    return p;
+}
+
+size_t delta_bytes(const Attn& a) { return (size_t(a.rows) * a.hq * sizeof(float) + 15) & ~size_t(15); }
+
+size_t backward_bytes(const Attn& a, int type) {
+    return delta_bytes(a) + (type == FMD_F32 && a.dim <= kPlanesDim ? attention_planes_bytes(a, true) : 0);
 }
 
 }  // namespace
@@ -86,16 +143,16 @@ using namespace fmd;
 
 extern "C" {
 
-fmd_status fmd_packed_attention_workspace_bytes(const fmd_attention* problem, size_t* bytes) {
+fmd_status fmd_packed_attention_workspace_bytes(const fmd_attention* problem, int32_t backward, size_t* bytes) {
     Attn a;
     if (problem == nullptr || bytes == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     const fmd_status st = check(*problem, a);
-    if (st == FMD_OK) *bytes = workspace_bytes(a, problem->type);
+    if (st == FMD_OK) *bytes = backward ? backward_bytes(a, problem->type) : plan(a, problem->type).bytes;
     return st;
 }
 
 fmd_status fmd_packed_attention(const fmd_attention* problem, void* out, float* lse, void* workspace,
-                                size_t workspace_size, int32_t* flags, void* stream) {
+                                size_t workspace_bytes, int32_t* flags, void* stream) {
     Attn a;
     if (problem == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     fmd_status st = check(*problem, a);
@@ -103,32 +160,40 @@ fmd_status fmd_packed_attention(const fmd_attention* problem, void* out, float* 
     if (a.rows == 0) return FMD_OK;
     if (out == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     if (!aligned16(out)) return FMD_ERR_UNSUPPORTED;
-    if (workspace_size < workspace_bytes(a, problem->type)) return FMD_ERR_WORKSPACE;
+    const Plan p = plan(a, problem->type);
+    if (workspace_bytes < p.bytes || (p.bytes > 0 && workspace == nullptr)) return FMD_ERR_WORKSPACE;
     if (!aligned16(workspace)) return FMD_ERR_UNSUPPORTED;
     a.out = out;
     a.lse = lse;
     a.flags = flags;
-    if (problem->type == FMD_BF16) {
-        a.part = static_cast<float*>(workspace);
-        a.part_lse = a.part + int64_t(attention_splits(a)) * a.rows * a.hq * a.dim;
-    }
-    if (problem->type == FMD_BF16) return attention_forward_mma(a, as_stream(stream));
-    return attention_forward_simt(a, problem->type, as_stream(stream));
+    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.planes);
+    a.part_lse = a.part + int64_t(p.splits) * a.rows * a.hq * a.dim;
+    const cudaStream_t s = as_stream(stream);
+    if (problem->type == FMD_BF16) st = attention_forward_mma(a, p.splits, s);
+    else if (a.dim <= kPlanesDim) st = attention_forward_planes(a, p.splits, workspace, s);
+    else st = attention_forward_simt(a, p.splits, s);
+    if (st != FMD_OK || p.splits == 1) return st;
+    const unsigned blocks = unsigned((a.rows * a.hq * (a.dim / 4) + kThreads - 1) / kThreads);
+    if (problem->type == FMD_BF16) join_kernel<__nv_bfloat16><<<blocks, kThreads, 0, s>>>(a, p.splits);
+    else join_kernel<float><<<blocks, kThreads, 0, s>>>(a, p.splits);
+    return check_launch();
 }
 
 fmd_status fmd_packed_attention_bwd(const fmd_attention* problem, const void* out, const float* lse, const void* g,
-                                    int64_t g_row, int64_t g_head, const float* glse, float* delta, void* dq, void* dk,
-                                    void* dv, int32_t* flags, void* stream) {
+                                    int64_t g_row, int64_t g_head, const float* glse, void* dq, void* dk, void* dv,
+                                    void* workspace, size_t workspace_bytes, int32_t* flags, void* stream) {
     Attn a;
     if (problem == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     fmd_status st = check(*problem, a);
     if (st != FMD_OK) return st;
     if ((dk == nullptr) != (dv == nullptr)) return FMD_ERR_INVALID_ARGUMENT;
-    if (a.rows > 0 && (out == nullptr || lse == nullptr || g == nullptr || delta == nullptr))
-        return FMD_ERR_INVALID_ARGUMENT;
+    if (a.rows > 0 && (out == nullptr || lse == nullptr || g == nullptr)) return FMD_ERR_INVALID_ARGUMENT;
+    const size_t bytes = backward_bytes(a, problem->type);
+    if (workspace_bytes < bytes || (bytes > 0 && workspace == nullptr)) return FMD_ERR_WORKSPACE;
     if ((a.rows > 0 && (!rows16(g, g_row, g_head, problem->type == FMD_F32 ? 4 : 2) || !aligned16(out))) ||
-        !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
+        !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(workspace))
         return FMD_ERR_UNSUPPORTED;
+    float* delta = static_cast<float*>(workspace);
     a.out = const_cast<void*>(out);
     a.lse = const_cast<float*>(lse);
     a.g = g;
@@ -147,7 +212,9 @@ fmd_status fmd_packed_attention_bwd(const fmd_attention* problem, const void* ou
         else delta_kernel<__nv_bfloat16><<<unsigned(blocks), kThreads, 0, s>>>(a, glse, delta);
         if ((st = check_launch()) != FMD_OK) return st;
     }
-    return problem->type == FMD_BF16 ? attention_backward_mma(a, s) : attention_backward_simt(a, problem->type, s);
+    if (problem->type == FMD_BF16) return attention_backward_mma(a, s);
+    if (a.dim <= kPlanesDim) return attention_backward_planes(a, static_cast<char*>(workspace) + delta_bytes(a), s);
+    return attention_backward_simt(a, s);
 }
 
 }  // extern "C"

@@ -95,15 +95,27 @@ __device__ __forceinline__ int64_t seen(const Span& s, bool causal, int64_t t) {
     return causal ? min(max(t + 1 + s.keys - s.rows, int64_t(0)), s.keys) : s.keys;
 }
 
-__device__ __forceinline__ float attn_float(float v) { return v; }
-__device__ __forceinline__ float attn_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void attn_store(float* p, float v) { *p = v; }
-__device__ __forceinline__ void attn_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+// Splits of the keys in the forward pass, where the tiles of `per_tile` tokens do not fill `blocks` places: the host
+// goes by the mean length of a sequence's slot (the lengths are on the device), and a split has `least` keys at least.
+inline int key_splits(const Attn& a, int per_tile, int blocks, int least) {
+    const int64_t tiles = tile_bound(a.rows, a.batch, per_tile) * a.hk;
+    if (tiles == 0 || a.batch == 0) return 1;
+    int64_t splits = blocks / tiles;
+    const int64_t most = a.keys / a.batch / least;
+    if (splits > most) splits = most;
+    return splits < 1 ? 1 : splits > 64 ? 64 : int(splits);
+}
 
-fmd_status attention_forward_simt(const Attn& a, int type, cudaStream_t s);
-fmd_status attention_backward_simt(const Attn& a, int type, cudaStream_t s);
-fmd_status attention_forward_mma(const Attn& a, cudaStream_t s);   // bfloat16
-int attention_splits(const Attn& a);                               // of the forward pass in bfloat16
-fmd_status attention_backward_mma(const Attn& a, cudaStream_t s);  // bfloat16
+// bfloat16
+int attention_splits_mma(const Attn& a);
+fmd_status attention_forward_mma(const Attn& a, int splits, cudaStream_t s);
+fmd_status attention_backward_mma(const Attn& a, cudaStream_t s);
+// float32, dim up to 64: by planes of bfloat16 in a workspace
+size_t attention_planes_bytes(const Attn& a, bool backward);
+fmd_status attention_forward_planes(const Attn& a, int splits, void* planes, cudaStream_t s);
+fmd_status attention_backward_planes(const Attn& a, void* planes, cudaStream_t s);
+// float32, wider heads
+fmd_status attention_forward_simt(const Attn& a, int splits, cudaStream_t s);
+fmd_status attention_backward_simt(const Attn& a, cudaStream_t s);
 
 }  // namespace fmd

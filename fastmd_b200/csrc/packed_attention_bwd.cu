@@ -44,7 +44,7 @@ struct Shape {
 template <int KS>
 struct Ctrl {
     uint64_t own;  // the two tiles that stay have landed
-    uint64_t full[Shape<KS>::kSlots], empty[Shape<KS>::kSlots];
+    Ring<Shape<KS>::kSlots> ring;
     uint64_t scores[2], dp;      // products done
     uint64_t p, ds;              // written by the workers
     uint64_t stats[2], read[2];  // keys: lse and delta of a tile in shared memory; read by all worker warps
@@ -62,10 +62,7 @@ template <int KS>
 __device__ __forceinline__ void open_block(Ctrl<KS>& ctl, int warp) {
     if (threadIdx.x == 0) {
         mbar_init(&ctl.own, 1);
-        for (int i = 0; i < Shape<KS>::kSlots; ++i) {
-            mbar_init(&ctl.full[i], 1);
-            mbar_init(&ctl.empty[i], 1);
-        }
+        init_ring(ctl.ring);
         mbar_init(&ctl.scores[0], 1);
         mbar_init(&ctl.scores[1], 1);
         mbar_init(&ctl.dp, 1);
@@ -82,11 +79,7 @@ __device__ __forceinline__ void open_block(Ctrl<KS>& ctl, int warp) {
         ctl.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&ctl.tmem))
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    if (warp == 1) tmem_alloc<512>(&ctl.tmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -96,52 +89,8 @@ template <int KS>
 __device__ __forceinline__ void close_block(Ctrl<KS>& ctl, int warp, int32_t* flags) {
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
-        __syncwarp();
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(ctl.tmem) : "memory");
-    }
+    if (warp == 1) tmem_free<512>(ctl.tmem);
     if (threadIdx.x == 0 && ctl.abort) raise_flag(flags, FMD_FLAG_WAIT_TIMEOUT);
-}
-
-// The ring's producer: tiles a0, b0, a1, b1, .. of `bytes` each, loaded by load(second, tile, slot address, barrier).
-template <int KS, typename Load>
-__device__ __forceinline__ void feed(Ctrl<KS>& ctl, unsigned char* ring, int tiles, uint32_t bytes, Load load) {
-    using S = Shape<KS>;
-    volatile int32_t* abort = &ctl.abort;
-    int slot = 0, armed = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int i = 0; i < 2 * tiles; ++i) {
-        if (!mbar_wait(&ctl.empty[slot], phase ^ 1u, abort)) {
-            ok = false;
-            break;
-        }
-        mbar_expect_tx(&ctl.full[slot], bytes);
-        load(i & 1, i >> 1, su32(ring + slot * S::kTileBytes), &ctl.full[slot]);
-        armed = i + 1;
-        if (++slot == S::kSlots) {
-            slot = 0;
-            phase ^= 1u;
-        }
-    }
-    if (!ok) {  // the copies in flight land before the block ends
-        mbar_wait(&ctl.own, 0, abort, true);
-        for (int i = max(0, armed - S::kSlots); i < armed; ++i)
-            mbar_wait(&ctl.full[i % S::kSlots], uint32_t(i / S::kSlots) & 1u, abort, true);
-    } else {  // the last slots' releases land before the block ends
-        for (int i = 0; i < S::kSlots && mbar_wait(&ctl.empty[slot], phase ^ 1u, abort); ++i)
-            if (++slot == S::kSlots) {
-                slot = 0;
-                phase ^= 1u;
-            }
-    }
-}
-
-// Waits for tile i of the ring (its place is i % slots); only for a thread that takes the tiles in order.
-template <int KS>
-__device__ __forceinline__ bool landed(Ctrl<KS>& ctl, int i) {
-    return mbar_wait(&ctl.full[i % Shape<KS>::kSlots], uint32_t(i / Shape<KS>::kSlots) & 1u, &ctl.abort);
 }
 
 // Writes 32 FP32 columns of TMEM times `factor` as bfloat16, as far as dim goes. loaded (the same in the whole warp):
@@ -199,10 +148,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tma_load_4d(su32(own + S::kTileBytes + p * kPanelBytes), &maps.g, &ctl.own, p * 64, 0, head,
                             int(s.row0 + token0));
             }
-            feed<KS>(ctl, ring, tiles, S::kTileBytes, [&](int second, int j, uint32_t at, uint64_t* bar) {
-                for (int p = 0; p < S::kPanels; ++p)
-                    tma_load_4d(at + p * kPanelBytes, second ? &maps.v : &maps.k, bar, p * 64, 0, head,
-                                int(s.key0) + j * kTile);
+            feed(ctl.ring, &ctl.own, abort, 2 * tiles, S::kTileBytes, [&](int i, int slot, uint64_t* bar) {
+                for (int p = 0; p < S::kPanels; ++p)  // k0, v0, k1, v1, ..
+                    tma_load_4d(su32(ring + slot * S::kTileBytes + p * kPanelBytes), i & 1 ? &maps.v : &maps.k, bar,
+                                p * 64, 0, head, int(s.key0) + (i >> 1) * kTile);
             });
         }
     } else if (warp == 1) {
@@ -213,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             auto width = [&](int j) { return min(kTile, (end - j * kTile + 15) & ~15); };
             bool ok = mbar_wait(&ctl.own, 0, abort), issued = false;
             auto scores = [&](int j) {  // into buffer j % 2
-                ok = ok && landed<KS>(ctl, 2 * j);
+                ok = ok && landed(ctl.ring, 2 * j, abort);
                 if (!ok) return;
                 tc_fence_after();
                 product_rows<KS>(tmem + uint32_t(j & 1) * 128u, q_tile, slot(2 * j), bf16_idesc(width(j), false));
@@ -221,12 +170,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 issued = true;
             };
             auto dp = [&](int j) {
-                ok = ok && landed<KS>(ctl, 2 * j + 1);
+                ok = ok && landed(ctl.ring, 2 * j + 1, abort);
                 if (!ok) return;
                 tc_fence_after();
                 product_rows<KS>(tmem + kDp, g_tile, slot(2 * j + 1), bf16_idesc(width(j), false));
                 tc_commit(&ctl.dp);
-                tc_commit(&ctl.empty[(2 * j + 1) % S::kSlots]);
+                tc_commit(&ctl.ring.empty[(2 * j + 1) % S::kSlots]);
             };
             scores(0);
             dp(0);
@@ -239,8 +188,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = ok && mbar_wait(&ctl.ds, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                product_weights<64>(tmem + kDq, tmem + kDp, slot(2 * j), width(j) / 16, out_desc, j > 0);
-                tc_commit(&ctl.empty[(2 * j) % S::kSlots]);
+                product_weights<4, 64>(tmem + kDq, tmem + kDp, slot(2 * j), width(j) / 16, out_desc, j > 0);
+                tc_commit(&ctl.ring.empty[(2 * j) % S::kSlots]);
                 if (j + 1 < tiles) dp(j + 1);
             }
             if (ok) tc_commit(&ctl.done);
@@ -252,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp < 4) {
         if (tail && mbar_wait(&ctl.tail_here, 0, abort)) {  // keys behind the last one: they are the inner index of dq
             const int first = keys - (tiles - 1) * kTile;
-            zero_rows(ring + ((2 * tiles - 2) % S::kSlots) * S::kTileBytes, S::kPanels, first, (first + 15) & ~15,
+            zero_rows(ring + ((2 * tiles - 2) % S::kSlots) * S::kTileBytes, S::kPanels, kPanelBytes, first, (first + 15) & ~15,
                       threadIdx.x - 64, 64);
             mbar_arrive(&ctl.tail);
         }
@@ -371,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
 
     if (full_rows < kTile && warp >= 4)  // rows of the slots that no copy ever writes are inner rows of the products
         for (int i = 0; i < S::kSlots; ++i)
-            zero_rows(ring + i * S::kTileBytes, S::kPanels, full_rows, kTile, threadIdx.x - 128, kWorkers);
+            zero_rows(ring + i * S::kTileBytes, S::kPanels, kPanelBytes, full_rows, kTile, threadIdx.x - 128, kWorkers);
     open_block<KS>(ctl, warp);
     const uint32_t tmem = ctl.tmem;
 
@@ -383,12 +332,12 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
                 tma_load_4d(su32(own + S::kTileBytes + p * kPanelBytes), &maps.v, &ctl.own, p * 64, 0, head,
                             int(s.key0 + key0));
             }
-            feed<KS>(ctl, ring, tiles, uint32_t(S::kPanels) * 128u * full_rows,
-                     [&](int second, int j, uint32_t at, uint64_t* bar) {
-                         for (int p = 0; p < S::kPanels; ++p)
-                             tma_load_4d(at + p * kPanelBytes, second ? &maps.g : &maps.q, bar, p * 64, 0, head,
-                                         int(s.row0 + (first + j) * per_tile));
-                     });
+            feed(ctl.ring, &ctl.own, abort, 2 * tiles, uint32_t(S::kPanels) * 128u * full_rows,
+                 [&](int i, int slot, uint64_t* bar) {
+                     for (int p = 0; p < S::kPanels; ++p)  // q0, g0, q1, g1, ..
+                         tma_load_4d(su32(ring + slot * S::kTileBytes + p * kPanelBytes), i & 1 ? &maps.g : &maps.q, bar,
+                                     p * 64, 0, head, int(s.row0 + (first + (i >> 1)) * per_tile));
+                 });
         }
     } else if (warp == 1) {
         if (lane == 0 && tiles > 0) {
@@ -398,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
             auto width = [&](int j) { return ((j == tiles - 1 ? last_rows : full_rows) + 15) & ~15; };
             bool ok = mbar_wait(&ctl.own, 0, abort), issued = false;
             auto scores = [&](int j) {
-                ok = ok && landed<KS>(ctl, 2 * j);
+                ok = ok && landed(ctl.ring, 2 * j, abort);
                 if (!ok) return;
                 tc_fence_after();
                 product_rows<KS>(tmem, k_tile, slot(2 * j), bf16_idesc(width(j), false));
@@ -406,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
                 issued = true;
             };
             auto dp = [&](int j) {
-                ok = ok && landed<KS>(ctl, 2 * j + 1);
+                ok = ok && landed(ctl.ring, 2 * j + 1, abort);
                 if (!ok) return;
                 tc_fence_after();
                 product_rows<KS>(tmem + kDp, v_tile, slot(2 * j + 1), bf16_idesc(width(j), false));
@@ -423,14 +372,14 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
                 ok = ok && mbar_wait(&ctl.p, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                product_weights<64>(tmem + kDv, tmem, slot(2 * j + 1), steps, out_desc, j > 0);
-                tc_commit(&ctl.empty[(2 * j + 1) % S::kSlots]);
+                product_weights<4, 64>(tmem + kDv, tmem, slot(2 * j + 1), steps, out_desc, j > 0);
+                tc_commit(&ctl.ring.empty[(2 * j + 1) % S::kSlots]);
                 if (j + 1 < tiles) scores(j + 1);
                 ok = ok && mbar_wait(&ctl.ds, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                product_weights<64>(tmem + kDk, tmem + kDp, slot(2 * j), steps, out_desc, j > 0);
-                tc_commit(&ctl.empty[(2 * j) % S::kSlots]);
+                product_weights<4, 64>(tmem + kDk, tmem + kDp, slot(2 * j), steps, out_desc, j > 0);
+                tc_commit(&ctl.ring.empty[(2 * j) % S::kSlots]);
                 if (j + 1 < tiles) dp(j + 1);
             }
             if (ok) tc_commit(&ctl.done);
@@ -467,8 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
         }
         if (tail && ok && mbar_wait(&ctl.tail_here, 0, abort)) {  // another sequence's rows
             for (int i = 2 * tiles - 2; i < 2 * tiles; ++i)
-                zero_rows(ring + (i % S::kSlots) * S::kTileBytes, S::kPanels, last_rows, (last_rows + 15) & ~15, thread,
-                          64);
+                zero_rows(ring + (i % S::kSlots) * S::kTileBytes, S::kPanels, kPanelBytes, last_rows,
+                          (last_rows + 15) & ~15, thread, 64);
             mbar_arrive(&ctl.tail);
         }
     } else {

@@ -1,0 +1,894 @@
+// Packed attention in float32 on the tensor cores, for heads of up to 64 values: forward and gradients.
+//
+// A float32 number is the sum of three bfloat16 ones, x = h + m + l (8 bits of the significand each; the differences
+// are exact). A product of two numbers is then nine products of which six matter, largest last:
+//   x y ~ l h' + h l' + m m' + m h' + h m' + h h'          (what is left out is below 2^-24 of x y)
+// so each FP32 product is six bfloat16 ones with FP32 sums: at the tensor cores' rate about five times what the FP32
+// cores could do. q, k, v (and g) are split once by a small kernel into three planes in memory; the weights p and ds
+// are split by the threads that compute them, into TMEM. The tensor cores' FP32 sums do not round to nearest, which
+// over thousands of keys would show: every product starts from zero, covers one tile, and the sum over tiles (with
+// the softmax's rescaling) is kept in registers.
+//
+// The forward pass is a block per 128 packed rows and key tiles of 128, the gradients as for bfloat16 (queries: a
+// block per 128 packed rows; keys: a block per 128 keys) with streamed tiles of 64, so that two stages of three planes
+// fit in shared memory beside the block's own. Roles of the warps, order of the products, masks and bounded waits are
+// those of the bfloat16 kernels. 256 workers: two threads per lane, each half of the columns.
+
+#include "packed_attention_mma.cuh"
+
+namespace fmd {
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kWorkers = 256;
+constexpr uint32_t kHalfPanel = kPanelBytes / 2;  // 64 rows
+// the plane (0: h, 1: m, 2: l) of each factor in the six products, the smallest first
+__device__ constexpr int kPlaneA[6] = {2, 0, 1, 1, 0, 0};
+__device__ constexpr int kPlaneB[6] = {0, 2, 1, 0, 1, 0};
+
+struct Maps {
+    CUtensorMap q, g, k, v;
+};
+
+// The next plane of 2 N values, two neighbours in a word; the values become what is left (exactly).
+template <int N>
+__device__ __forceinline__ void next_plane(float* y, uint32_t (&w)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        w[i] = pack_bf16(y[2 * i], y[2 * i + 1]);
+        const float2 part = unpack_bf16(w[i]);
+        const float2 left = add2(make_float2(y[2 * i], y[2 * i + 1]), make_float2(-part.x, -part.y));
+        y[2 * i] = left.x;
+        y[2 * i + 1] = left.y;
+    }
+}
+
+// N columns of TMEM (16 or 32) added to a sum in registers, which is then scaled.
+template <int N>
+__device__ __forceinline__ void drain(uint32_t addr, float (&sum)[N], float keep) {
+    float o[N];
+    if constexpr (N == 32) tmem_load32(addr, o);
+    else tmem_load16(addr, o);
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] = (sum[i] + o[i]) * keep;
+}
+
+template <int N>
+__device__ __forceinline__ void store_values(float* out, const float (&v)[N], float factor, int col0, int dim) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+        if (col0 + i < dim)
+            *reinterpret_cast<float4*>(out + col0 + i) =
+                make_float4(v[i] * factor, v[i + 1] * factor, v[i + 2] * factor, v[i + 3] * factor);
+}
+
+// ---------------------------------------------------------------- planes
+
+struct SplitArgs {
+    const float* x[4];
+    __nv_bfloat16* planes[4];  // [3][rows][heads][dim]
+    int64_t rows[4], row[4], head[4];
+    int32_t heads[4];
+    int32_t dim;
+};
+
+// 8 values a thread
+__global__ void __launch_bounds__(256) split_kernel(const SplitArgs a) {
+    const int t = blockIdx.y, per = a.dim / 8;
+    const int64_t heads = a.heads[t], all = a.rows[t] * heads * per;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += int64_t(gridDim.x) * 256) {
+        const int64_t r = i / per, row = r / heads;
+        const int c = int(i - r * per) * 8;
+        const float* x = a.x[t] + row * a.row[t] + (r - row * heads) * a.head[t] + c;
+        const float4 p = ldg4(x), q = ldg4(x + 4);
+        float v[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+        uint4* out = reinterpret_cast<uint4*>(a.planes[t] + r * a.dim + c);
+        const int64_t plane = a.rows[t] * heads * a.dim / 8;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            uint32_t w[4];
+            next_plane<4>(v, w);
+            out[i * plane] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- forward
+
+constexpr int kSlots = 3;
+constexpr uint32_t kTile3 = 3 * kPanelBytes;  // a tile of 128 rows: three planes
+constexpr size_t kForwardBytes = size_t(1 + kSlots) * kTile3 + 1024;
+
+struct ForwardCtrl {
+    uint64_t own;
+    Ring<kSlots> ring;
+    uint64_t scores[2], weights, swap, out;
+    uint64_t tail_here, tail, drain;
+    uint32_t tmem;
+    int32_t abort;
+};
+
+template <int KS, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_constant__ Maps maps, const Attn a) {
+    constexpr int kDim = 16 * KS, kMine = kDim / 2;  // output columns, and those of one half
+    constexpr uint32_t kL = 256, kO = 320;           // TMEM columns: two score buffers, p's lowest plane, the output
+    extern __shared__ unsigned char raw[];
+    unsigned char* own = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* ring = own + kTile3;
+    __shared__ ForwardCtrl ctl;
+    __shared__ float maxima[2][2][kTile], sums[2][kTile];
+    volatile int32_t* abort = &ctl.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int64_t index = gridDim.x - 1 - blockIdx.x;  // the longest rows of a causal sequence first
+    const int per_tile = kTile / a.group;
+    const int b = find_sequence(a.offsets, a.batch, per_tile, index);
+    const Span s = load_span(a, b);
+    const int64_t token0 = (index - (a.offsets[b] / per_tile + b)) * per_tile;
+    if (token0 < 0 || token0 >= s.rows) return;
+    const int head = blockIdx.y;
+    const int tokens = int(min(int64_t(per_tile), s.rows - token0));
+    int end = int(seen(s, a.causal, token0 + tokens - 1)), tiles = (end + kTile - 1) / kTile, from = 0;
+    if (SPLIT) {  // a range of the key tiles; from here on everything counts from its first key
+        const int share = (tiles + int(gridDim.z) - 1) / int(gridDim.z);
+        from = min(tiles, int(blockIdx.z) * share) * kTile;
+        end = max(0, min(end, min(tiles, int(blockIdx.z + 1) * share) * kTile) - from);
+        tiles = (end + kTile - 1) / kTile;
+        if (tiles == 0) {
+            for (int r = threadIdx.x; r < tokens * a.group; r += blockDim.x)
+                a.part_lse[(int64_t(blockIdx.z) * a.rows + s.row0 + token0 + r / a.group) * a.hq + head * a.group +
+                           r % a.group] = -INFINITY;
+            return;
+        }
+    }
+    const int keys = int(s.keys) - from;
+    const bool tail = tiles > 0 && keys < tiles * kTile;
+
+    if (threadIdx.x == 0) {
+        mbar_init(&ctl.own, 1);
+        init_ring(ctl.ring);
+        mbar_init(&ctl.scores[0], 1);
+        mbar_init(&ctl.scores[1], 1);
+        mbar_init(&ctl.weights, kWorkers);
+        mbar_init(&ctl.swap, kWorkers);
+        mbar_init(&ctl.out, 1);
+        mbar_init(&ctl.tail_here, 1);
+        mbar_init(&ctl.tail, 64);
+        mbar_init(&ctl.drain, 1);
+        ctl.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc<512>(&ctl.tmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl.tmem;
+
+    if (warp == 0) {
+        if (lane == 0 && tiles > 0) {
+            mbar_expect_tx(&ctl.own, 3u * 128u * uint32_t(per_tile * a.group));
+            for (int p = 0; p < 3; ++p)
+                tma_load_4d(su32(own + p * kPanelBytes), &maps.q, &ctl.own, 0, 0, head,
+                            int(p * a.rows + s.row0 + token0));
+            feed(ctl.ring, &ctl.own, abort, 2 * tiles, kTile3, [&](int i, int slot, uint64_t* bar) {
+                for (int p = 0; p < 3; ++p)  // k0, v0, k1, v1, ..
+                    tma_load_4d(su32(ring + slot * kTile3 + p * kPanelBytes), i & 1 ? &maps.v : &maps.k, bar, 0, 0, head,
+                                int(p * a.keys + s.key0) + from + (i >> 1) * kTile);
+            });
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && tiles > 0) {
+            const uint32_t o_desc = bf16_idesc(kDim, true);
+            auto slot = [&](int i) { return su32(ring + (i % kSlots) * kTile3); };
+            auto width = [&](int j) { return min(kTile, (end - j * kTile + 15) & ~15); };
+            bool ok = mbar_wait(&ctl.own, 0, abort), issued = false;
+            auto scores = [&](int j) {
+                ok = ok && landed(ctl.ring, 2 * j, abort);
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t d = tmem + uint32_t(j & 1) * 128u, q = su32(own), k = slot(2 * j);
+                const uint32_t desc = bf16_idesc(width(j), false);
+#pragma unroll
+                for (int i = 0; i < 6; ++i)
+                    product_rows<KS>(d, q + kPlaneA[i] * kPanelBytes, k + kPlaneB[i] * kPanelBytes, desc, i > 0);
+                tc_commit(&ctl.scores[j & 1]);
+                tc_commit(&ctl.ring.empty[(2 * j) % kSlots]);
+                issued = true;
+            };
+            scores(0);
+            for (int j = 0; j < tiles && ok; ++j) {
+                if (j + 1 < tiles) scores(j + 1);
+                ok = ok && landed(ctl.ring, 2 * j + 1, abort);
+                if (ok && tail && j == tiles - 1) {
+                    mbar_arrive(&ctl.tail_here);
+                    ok = mbar_wait(&ctl.tail, 0, abort);
+                }
+                ok = ok && mbar_wait(&ctl.weights, uint32_t(j) & 1u, abort);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t p = tmem + uint32_t(j & 1) * 128u, v = slot(2 * j + 1);
+                const int steps = width(j) / 16;
+#pragma unroll
+                for (int i = 0; i < 6; ++i) {
+                    const uint32_t at = v + kPlaneB[i] * kPanelBytes;
+                    if (kPlaneA[i] == 2) product_weights<4, 32>(tmem + kO, tmem + kL, at, steps, o_desc, i > 0);
+                    else product_weights<4, 64>(tmem + kO, p + 32u * kPlaneA[i], at, steps, o_desc, i > 0);
+                }
+                tc_commit(&ctl.out);
+                tc_commit(&ctl.ring.empty[(2 * j + 1) % kSlots]);
+            }
+            if (!ok && issued) {
+                tc_commit(&ctl.drain);
+                mbar_wait(&ctl.drain, 0, abort, true);
+            }
+        }
+    } else if (warp < 4) {
+        if (tail && mbar_wait(&ctl.tail_here, 0, abort)) {
+            const int first = keys - (tiles - 1) * kTile;
+            zero_rows(ring + ((2 * tiles - 1) % kSlots) * kTile3, 3, kPanelBytes, first, (first + 15) & ~15,
+                      threadIdx.x - 64, 64);
+            mbar_arrive(&ctl.tail);
+        }
+    } else {
+        const int half = (warp - 4) >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const int token = r / a.group;
+        const bool real = token < tokens;
+        const int limit = real ? min(max(int(seen(s, a.causal, token0 + token)) - from, 0), end) : 0;
+        const float c = a.scale * kLog2e;
+        const uint32_t at_o = tmem + lanes + kO + uint32_t(half * kMine);
+        float m = -INFINITY, l = 0.0f, o[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) o[i] = 0.0f;
+        bool ok = true;
+        auto all = [&](bool got) {  // uniform in the warp: TMEM access is .sync.aligned
+            ok = __all_sync(0xffffffffu, got);
+            if (!ok) *abort = 1;
+            tc_fence_after();
+            return ok;
+        };
+        for (int j = 0; j < tiles; ++j) {
+            if (!all(mbar_wait(&ctl.scores[j & 1], uint32_t(j >> 1) & 1u, abort))) break;
+            const uint32_t at_s = tmem + lanes + uint32_t(j & 1) * 128u + uint32_t(half) * 64u;
+            const int columns = end - j * kTile - 64 * half, mine = limit - j * kTile - 64 * half;
+            float x[2][32];
+            float top = -INFINITY;
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) {
+                if (32 * ch < columns) {
+                    tmem_load32(at_s + ch * 32, x[ch]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[ch][i] = -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    x[ch][i] = ch * 32 + i < mine ? x[ch][i] : -INFINITY;
+                    top = fmaxf(top, x[ch][i]);
+                }
+            }
+            // the row's maximum over both halves
+            maxima[j & 1][half][r] = top;
+            mbar_arrive(&ctl.swap);
+            if (!all(mbar_wait(&ctl.swap, uint32_t(j) & 1u, abort))) break;
+            top = fmaxf(m, fmaxf(top, maxima[j & 1][1 - half][r]) * c);
+            const float base = top == -INFINITY ? 0.0f : top;
+            const float keep = ex2(m - base);
+            m = top;
+            const float2 c2 = make_float2(c, c), base2 = make_float2(-base, -base);
+            float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 y = fma2(make_float2(x[ch][i], x[ch][i + 1]), c2, base2);
+                    x[ch][i] = ex2(y.x);
+                    x[ch][i + 1] = ex2(y.y);
+                    sum = add2(sum, make_float2(x[ch][i], x[ch][i + 1]));
+                }
+            }
+            l = l * keep + (sum.x + sum.y);
+            if (j > 0) {  // the last tile's output, against the old maximum; then p may overwrite its weights
+                if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
+                drain<kMine>(at_o, o, keep);
+            }
+            const uint32_t at_l = tmem + lanes + kL + uint32_t(half) * 32u;
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) {
+                if (32 * ch < columns) {
+                    uint32_t w[16];
+                    next_plane<16>(x[ch], w);
+                    tmem_store16(at_s + ch * 16, w);
+                    next_plane<16>(x[ch], w);
+                    tmem_store16(at_s + 32 + ch * 16, w);
+                    next_plane<16>(x[ch], w);
+                    tmem_store16(at_l + ch * 16, w);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&ctl.weights);
+        }
+        if (ok && tiles > 0) {
+            sums[half][r] = l;
+            mbar_arrive(&ctl.swap);
+            if (all(mbar_wait(&ctl.out, uint32_t(tiles - 1) & 1u, abort) &&
+                    mbar_wait(&ctl.swap, uint32_t(tiles) & 1u, abort))) {
+                drain<kMine>(at_o, o, 1.0f);
+                l = sums[0][r] + sums[1][r];
+            }
+        }
+        if (ok && real) {
+            int64_t flat = (s.row0 + token0 + token) * a.hq + head * a.group + r % a.group;
+            const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+            const float lse = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+            if (SPLIT) flat += int64_t(blockIdx.z) * a.rows * a.hq;
+            if (limit == 0) {
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) o[i] = 0.0f;
+            }
+            store_values<kMine>((SPLIT ? a.part : static_cast<float*>(a.out)) + flat * a.dim, o, inv, half * kMine, a.dim);
+            if (half == 0 && SPLIT) a.part_lse[flat] = lse;
+            if (half == 0 && !SPLIT && a.lse != nullptr) a.lse[flat] = lse;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_free<512>(tmem);
+    if (threadIdx.x == 0 && ctl.abort) raise_flag(a.flags, FMD_FLAG_WAIT_TIMEOUT);
+}
+
+// --------------------------------------------------------------- gradients
+
+constexpr int kStream = 64;                     // rows of a streamed tile
+constexpr int kStreamSlots = 4;
+constexpr uint32_t kSlot3 = 3 * kHalfPanel;
+constexpr size_t kBackwardBytes = 2 * size_t(kTile3) + kStreamSlots * size_t(kSlot3) + 1024;
+
+struct BackwardCtrl {
+    uint64_t own;
+    Ring<kStreamSlots> ring;
+    uint64_t scores[2], dp[2];
+    uint64_t weights, out;
+    uint64_t stats[2], read[2];
+    uint64_t tail_here, tail, drain;
+    uint32_t tmem;
+    int32_t abort;
+};
+
+__device__ __forceinline__ void open_block(BackwardCtrl& ctl, int warp) {
+    if (threadIdx.x == 0) {
+        mbar_init(&ctl.own, 1);
+        init_ring(ctl.ring);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ctl.scores[i], 1);
+            mbar_init(&ctl.dp[i], 1);
+            mbar_init(&ctl.stats[i], 64);
+            mbar_init(&ctl.read[i], kWorkers / 32);
+        }
+        mbar_init(&ctl.weights, kWorkers);
+        mbar_init(&ctl.out, 1);
+        mbar_init(&ctl.tail_here, 1);
+        mbar_init(&ctl.tail, 64);
+        mbar_init(&ctl.drain, 1);
+        ctl.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc<512>(&ctl.tmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+}
+
+__device__ __forceinline__ void close_block(BackwardCtrl& ctl, int warp, int32_t* flags) {
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_free<512>(ctl.tmem);
+    if (threadIdx.x == 0 && ctl.abort) raise_flag(flags, FMD_FLAG_WAIT_TIMEOUT);
+}
+
+// D [128, n] = the six products of two operands of three planes, along their rows.
+template <int KS>
+__device__ __forceinline__ void product6(uint32_t d, uint32_t a, uint32_t b, uint32_t b_plane, uint32_t idesc) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i)
+        product_rows<KS>(d, a + kPlaneA[i] * kPanelBytes, b + kPlaneB[i] * b_plane, idesc, i > 0);
+}
+
+// D [128, n] = the six products of weights over a tile's columns (planes h and m at w, l at low) and a streamed tile.
+__device__ __forceinline__ void weigh6(uint32_t d, uint32_t w, uint32_t low, uint32_t b, int steps, uint32_t idesc) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+        const uint32_t at = b + kPlaneB[i] * kHalfPanel;
+        if (kPlaneA[i] == 2) product_weights<2, 16>(d, low, at, steps, idesc, i > 0);
+        else product_weights<2, 32>(d, w + 16u * kPlaneA[i], at, steps, idesc, i > 0);
+    }
+}
+
+// The three planes of a thread's 32 weights: h and m over the columns it has read, l beside.
+__device__ __forceinline__ void store_planes(uint32_t w, uint32_t low, float (&y)[32]) {
+    uint32_t plane[16];
+    next_plane<16>(y, plane);
+    tmem_store16(w, plane);
+    next_plane<16>(y, plane);
+    tmem_store16(w + 16, plane);
+    next_plane<16>(y, plane);
+    tmem_store16(low, plane);
+}
+
+template <int KS>
+__global__ void __launch_bounds__(kThreads, 1)
+    query_gradient_kernel(const __grid_constant__ Maps maps, const Attn a) {
+    constexpr int kDim = 16 * KS, kMine = kDim / 2;
+    constexpr uint32_t kDp = 128, kL = 256, kDq = 320;  // TMEM columns: two score buffers, two of dP, ds's l, dq
+    extern __shared__ unsigned char raw[];
+    unsigned char* own = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* ring = own + 2 * kTile3;
+    __shared__ BackwardCtrl ctl;
+    volatile int32_t* abort = &ctl.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int64_t index = gridDim.x - 1 - blockIdx.x;
+    const int per_tile = kTile / a.group;
+    const int b = find_sequence(a.offsets, a.batch, per_tile, index);
+    const Span s = load_span(a, b);
+    const int64_t token0 = (index - (a.offsets[b] / per_tile + b)) * per_tile;
+    if (token0 < 0 || token0 >= s.rows) return;
+    const int head = blockIdx.y;
+    const int tokens = int(min(int64_t(per_tile), s.rows - token0));
+    const int end = int(seen(s, a.causal, token0 + tokens - 1));
+    const int tiles = (end + kStream - 1) / kStream, keys = int(s.keys);
+    const bool tail = tiles > 0 && keys < tiles * kStream;
+
+    open_block(ctl, warp);
+    const uint32_t tmem = ctl.tmem;
+
+    if (warp == 0) {
+        if (lane == 0 && tiles > 0) {
+            mbar_expect_tx(&ctl.own, 2u * 3u * 128u * uint32_t(per_tile * a.group));
+            for (int p = 0; p < 3; ++p) {
+                const int row = int(p * a.rows + s.row0 + token0);
+                tma_load_4d(su32(own + p * kPanelBytes), &maps.q, &ctl.own, 0, 0, head, row);
+                tma_load_4d(su32(own + kTile3 + p * kPanelBytes), &maps.g, &ctl.own, 0, 0, head, row);
+            }
+            feed(ctl.ring, &ctl.own, abort, 2 * tiles, kSlot3, [&](int i, int slot, uint64_t* bar) {
+                for (int p = 0; p < 3; ++p)  // k0, v0, k1, v1, ..
+                    tma_load_4d(su32(ring + slot * kSlot3 + p * kHalfPanel), i & 1 ? &maps.v : &maps.k, bar, 0, 0, head,
+                                int(p * a.keys + s.key0) + (i >> 1) * kStream);
+            });
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && tiles > 0) {
+            const uint32_t out_desc = bf16_idesc(kDim, true);
+            auto slot = [&](int i) { return su32(ring + (i % kStreamSlots) * kSlot3); };
+            auto width = [&](int j) { return min(kStream, (end - j * kStream + 15) & ~15); };
+            bool ok = mbar_wait(&ctl.own, 0, abort), issued = false;
+            auto both = [&](int j) {  // scores and dP of tile j
+                ok = ok && landed(ctl.ring, 2 * j, abort) && landed(ctl.ring, 2 * j + 1, abort);
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t at = tmem + uint32_t(j & 1) * kStream, desc = bf16_idesc(width(j), false);
+                product6<KS>(at, su32(own), slot(2 * j), kHalfPanel, desc);
+                tc_commit(&ctl.scores[j & 1]);
+                product6<KS>(at + kDp, su32(own + kTile3), slot(2 * j + 1), kHalfPanel, desc);
+                tc_commit(&ctl.dp[j & 1]);
+                tc_commit(&ctl.ring.empty[(2 * j + 1) % kStreamSlots]);
+                issued = true;
+            };
+            both(0);
+            for (int j = 0; j < tiles && ok; ++j) {
+                if (j + 1 < tiles) both(j + 1);
+                if (ok && tail && j == tiles - 1) {
+                    mbar_arrive(&ctl.tail_here);
+                    ok = mbar_wait(&ctl.tail, 0, abort);
+                }
+                ok = ok && mbar_wait(&ctl.weights, uint32_t(j) & 1u, abort);
+                if (!ok) break;
+                tc_fence_after();
+                weigh6(tmem + kDq, tmem + kDp + uint32_t(j & 1) * kStream, tmem + kL, slot(2 * j), width(j) / 16,
+                       out_desc);
+                tc_commit(&ctl.out);
+                tc_commit(&ctl.ring.empty[(2 * j) % kStreamSlots]);
+            }
+            if (!ok && issued) {
+                tc_commit(&ctl.drain);
+                mbar_wait(&ctl.drain, 0, abort, true);
+            }
+        }
+    } else if (warp < 4) {
+        if (tail && mbar_wait(&ctl.tail_here, 0, abort)) {
+            const int first = keys - (tiles - 1) * kStream;
+            zero_rows(ring + ((2 * tiles - 2) % kStreamSlots) * kSlot3, 3, kHalfPanel, first, (first + 15) & ~15,
+                      threadIdx.x - 64, 64);
+            mbar_arrive(&ctl.tail);
+        }
+    } else {
+        const int half = (warp - 4) >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const int token = r / a.group;
+        const bool real = token < tokens;
+        const int64_t flat = (s.row0 + token0 + token) * a.hq + head * a.group + r % a.group;
+        const float lse = real ? a.lse[flat] : -INFINITY, delta = real ? a.delta[flat] : 0.0f;
+        const int limit = lse != -INFINITY ? int(seen(s, a.causal, token0 + token)) : 0;
+        const float base = lse != -INFINITY ? -lse * kLog2e : 0.0f;
+        const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), base2 = make_float2(base, base);
+        const float2 delta2 = make_float2(-delta, -delta);
+        const uint32_t at_q = tmem + lanes + kDq + uint32_t(half * kMine);
+        float dq[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) dq[i] = 0.0f;
+        bool ok = true;
+        auto all = [&](bool got) {
+            ok = __all_sync(0xffffffffu, got);
+            if (!ok) *abort = 1;
+            tc_fence_after();
+            return ok;
+        };
+        for (int j = 0; j < tiles; ++j) {
+            const int mine = limit - j * kStream - 32 * half;
+            const bool any = end - j * kStream - 32 * half > 0;
+            const uint32_t at = tmem + lanes + uint32_t(j & 1) * kStream + uint32_t(half) * 32u;
+            float p[32], x[32];
+            if (!all(mbar_wait(&ctl.scores[j & 1], uint32_t(j >> 1) & 1u, abort))) break;
+            if (any) {
+                tmem_load32(at, p);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 y = fma2(make_float2(p[i], p[i + 1]), c2, base2);
+                    p[i] = ex2(y.x);
+                    p[i + 1] = ex2(y.y);
+                }
+            }
+            if (!all(mbar_wait(&ctl.dp[j & 1], uint32_t(j >> 1) & 1u, abort))) break;
+            if (any) {
+                tmem_load32(at + kDp, x);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 y = mul2(add2(make_float2(x[i], x[i + 1]), delta2), make_float2(p[i], p[i + 1]));
+                    x[i] = i < mine ? y.x : 0.0f;
+                    x[i + 1] = i + 1 < mine ? y.y : 0.0f;
+                }
+            }
+            if (j > 0) {
+                if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
+                drain<kMine>(at_q, dq, 1.0f);
+            }
+            if (any) store_planes(at + kDp, tmem + lanes + kL + uint32_t(half) * 16u, x);
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&ctl.weights);
+        }
+        if (ok && tiles > 0 && all(mbar_wait(&ctl.out, uint32_t(tiles - 1) & 1u, abort))) drain<kMine>(at_q, dq, 1.0f);
+        if (ok && real) store_values<kMine>(static_cast<float*>(a.dq) + flat * a.dim, dq, a.scale, half * kMine, a.dim);
+    }
+    close_block(ctl, warp, a.flags);
+}
+
+template <int KS>
+__global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_constant__ Maps maps, const Attn a) {
+    constexpr int kDim = 16 * KS;
+    constexpr uint32_t kDp = 128, kPl = 256, kDl = 288, kDv = 320, kDk = 384;  // TMEM columns
+    extern __shared__ unsigned char raw[];
+    unsigned char* own = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* ring = own + 2 * kTile3;
+    __shared__ BackwardCtrl ctl;
+    // of two tiles: - lse log2 e, - delta and the number of keys that each packed row sees
+    __shared__ alignas(16) float lse_of[2][kStream], delta_of[2][kStream];
+    __shared__ alignas(16) int limit_of[2][kStream];
+    volatile int32_t* abort = &ctl.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int b = find_sequence(a.key_offsets, a.batch, kTile, blockIdx.x);
+    const Span s = load_span(a, b);
+    const int64_t key0 = (int64_t(blockIdx.x) - (a.key_offsets[b] / kTile + b)) * kTile;
+    if (key0 < 0 || key0 >= s.slot) return;
+    const int head = blockIdx.y;
+    const int per_tile = kStream / a.group, full_rows = per_tile * a.group;
+    const int64_t first = a.causal ? max(int64_t(0), key0 + s.rows - s.keys) / per_tile : 0;
+    const int64_t count = (s.rows + per_tile - 1) / per_tile;
+    const int tiles = key0 < s.keys ? int(max(int64_t(0), count - first)) : 0;
+    const int last_rows = tiles > 0 ? int(s.rows - (count - 1) * per_tile) * a.group : 0;
+    const bool tail = tiles > 0 && last_rows % 16 != 0 && last_rows < full_rows;
+
+    if (full_rows < kStream && warp >= 4)  // rows of the slots that no copy ever writes are inner rows of the products
+        for (int i = 0; i < kStreamSlots; ++i)
+            zero_rows(ring + i * kSlot3, 3, kHalfPanel, full_rows, kStream, threadIdx.x - 128, kWorkers);
+    open_block(ctl, warp);
+    const uint32_t tmem = ctl.tmem;
+
+    if (warp == 0) {
+        if (lane == 0 && tiles > 0) {
+            mbar_expect_tx(&ctl.own, 2u * kTile3);
+            for (int p = 0; p < 3; ++p) {
+                const int row = int(p * a.keys + s.key0 + key0);
+                tma_load_4d(su32(own + p * kPanelBytes), &maps.k, &ctl.own, 0, 0, head, row);
+                tma_load_4d(su32(own + kTile3 + p * kPanelBytes), &maps.v, &ctl.own, 0, 0, head, row);
+            }
+            feed(ctl.ring, &ctl.own, abort, 2 * tiles, 3u * 128u * full_rows, [&](int i, int slot, uint64_t* bar) {
+                for (int p = 0; p < 3; ++p)  // q0, g0, q1, g1, ..
+                    tma_load_4d(su32(ring + slot * kSlot3 + p * kHalfPanel), i & 1 ? &maps.g : &maps.q, bar, 0, 0, head,
+                                int(p * a.rows + s.row0 + (first + (i >> 1)) * per_tile));
+            });
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && tiles > 0) {
+            const uint32_t out_desc = bf16_idesc(kDim, true);
+            auto slot = [&](int i) { return su32(ring + (i % kStreamSlots) * kSlot3); };
+            auto width = [&](int j) { return ((j == tiles - 1 ? last_rows : full_rows) + 15) & ~15; };
+            bool ok = mbar_wait(&ctl.own, 0, abort), issued = false;
+            auto both = [&](int j) {
+                ok = ok && landed(ctl.ring, 2 * j, abort) && landed(ctl.ring, 2 * j + 1, abort);
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t at = tmem + uint32_t(j & 1) * kStream, desc = bf16_idesc(width(j), false);
+                product6<KS>(at, su32(own), slot(2 * j), kHalfPanel, desc);
+                tc_commit(&ctl.scores[j & 1]);
+                product6<KS>(at + kDp, su32(own + kTile3), slot(2 * j + 1), kHalfPanel, desc);
+                tc_commit(&ctl.dp[j & 1]);
+                issued = true;
+            };
+            both(0);
+            for (int j = 0; j < tiles && ok; ++j) {
+                if (j + 1 < tiles) both(j + 1);
+                if (ok && tail && j == tiles - 1) {
+                    mbar_arrive(&ctl.tail_here);
+                    ok = mbar_wait(&ctl.tail, 0, abort);
+                }
+                ok = ok && mbar_wait(&ctl.weights, uint32_t(j) & 1u, abort);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t at = tmem + uint32_t(j & 1) * kStream;
+                weigh6(tmem + kDv, at, tmem + kPl, slot(2 * j + 1), width(j) / 16, out_desc);
+                weigh6(tmem + kDk, at + kDp, tmem + kDl, slot(2 * j), width(j) / 16, out_desc);
+                tc_commit(&ctl.out);
+                tc_commit(&ctl.ring.empty[(2 * j) % kStreamSlots]);
+                tc_commit(&ctl.ring.empty[(2 * j + 1) % kStreamSlots]);
+            }
+            if (!ok && issued) {
+                tc_commit(&ctl.drain);
+                mbar_wait(&ctl.drain, 0, abort, true);
+            }
+        }
+    } else if (warp < 4) {
+        const int r = threadIdx.x - 64;
+        bool ok = true;
+        for (int j = 0; j < tiles && ok; ++j) {
+            if (j >= 2 && !mbar_wait(&ctl.read[j & 1], uint32_t((j >> 1) - 1) & 1u, abort)) {
+                ok = false;
+                break;
+            }
+            const int64_t token = (first + j) * per_tile + r / a.group;
+            float lse = -INFINITY, delta = 0.0f;
+            int limit = 0;
+            if (r < full_rows && token < s.rows) {
+                const int64_t flat = (s.row0 + token) * a.hq + head * a.group + r % a.group;
+                lse = a.lse[flat];
+                delta = a.delta[flat];
+                limit = int(max(int64_t(0), min(int64_t(kTile), seen(s, a.causal, token) - key0)));
+            }
+            const bool none = lse == -INFINITY;
+            lse_of[j & 1][r] = none ? 0.0f : -lse * kLog2e;
+            delta_of[j & 1][r] = -delta;
+            limit_of[j & 1][r] = none ? 0 : limit;
+            mbar_arrive(&ctl.stats[j & 1]);
+        }
+        if (tail && ok && mbar_wait(&ctl.tail_here, 0, abort)) {
+            for (int i = 2 * tiles - 2; i < 2 * tiles; ++i)
+                zero_rows(ring + (i % kStreamSlots) * kSlot3, 3, kHalfPanel, last_rows, (last_rows + 15) & ~15, r, 64);
+            mbar_arrive(&ctl.tail);
+        }
+    } else {
+        const int half = (warp - 4) >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e);
+        // the first four warps keep the sum of dv, the others that of dk
+        const uint32_t at_out = tmem + lanes + (half ? kDk : kDv);
+        float out[kDim / 32][32];
+#pragma unroll
+        for (int i = 0; i < kDim; ++i) out[i / 32][i % 32] = 0.0f;
+        bool ok = true;
+        auto all = [&](bool got) {
+            ok = __all_sync(0xffffffffu, got);
+            if (!ok) *abort = 1;
+            tc_fence_after();
+            return ok;
+        };
+        auto drain_all = [&] {
+#pragma unroll
+            for (int i = 0; i < kDim / 32; ++i) drain<32>(at_out + 32 * i, out[i], 1.0f);
+        };
+        for (int j = 0; j < tiles; ++j) {
+            const int rows = j == tiles - 1 ? last_rows : full_rows;
+            const bool any = rows > 32 * half;
+            const float* nl = lse_of[j & 1] + 32 * half;
+            const float* nd = delta_of[j & 1] + 32 * half;
+            const int* lim = limit_of[j & 1] + 32 * half;
+            const uint32_t at = tmem + lanes + uint32_t(j & 1) * kStream + uint32_t(half) * 32u;
+            float p[32], x[32];
+            if (!all(mbar_wait(&ctl.stats[j & 1], uint32_t(j >> 1) & 1u, abort) &&
+                     mbar_wait(&ctl.scores[j & 1], uint32_t(j >> 1) & 1u, abort)))
+                break;
+            if (any) {
+                tmem_load32(at, p);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 y = fma2(make_float2(p[i], p[i + 1]), c2, *reinterpret_cast<const float2*>(nl + i));
+                    const int2 m = *reinterpret_cast<const int2*>(lim + i);
+                    p[i] = r < m.x ? ex2(y.x) : 0.0f;
+                    p[i + 1] = r < m.y ? ex2(y.y) : 0.0f;
+                }
+            }
+            if (!all(mbar_wait(&ctl.dp[j & 1], uint32_t(j >> 1) & 1u, abort))) break;
+            if (any) {
+                tmem_load32(at + kDp, x);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 d = *reinterpret_cast<const float2*>(nd + i);
+                    const int2 m = *reinterpret_cast<const int2*>(lim + i);
+                    const float2 y = mul2(add2(make_float2(x[i], x[i + 1]), d), make_float2(p[i], p[i + 1]));
+                    x[i] = r < m.x ? y.x : 0.0f;
+                    x[i + 1] = r < m.y ? y.y : 0.0f;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl.read[j & 1]);
+            // the last products have read their weights and may be added before the next ones start
+            if (j > 0 && !all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
+            if (any) {
+                store_planes(at, tmem + lanes + kPl + uint32_t(half) * 16u, p);
+                store_planes(at + kDp, tmem + lanes + kDl + uint32_t(half) * 16u, x);
+            }
+            if (j > 0) drain_all();
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&ctl.weights);
+        }
+        if (ok && tiles > 0 && all(mbar_wait(&ctl.out, uint32_t(tiles - 1) & 1u, abort))) drain_all();
+        if (ok && key0 + r < s.slot) {  // slot rows that are no keys get zeros
+            float* row = static_cast<float*>(half ? a.dk : a.dv) + ((s.key0 + key0 + r) * a.hk + head) * a.dim;
+            const bool keep = key0 + r < s.keys;
+#pragma unroll
+            for (int i = 0; i < kDim / 32; ++i) {
+                if (!keep) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) out[i][e] = 0.0f;
+                }
+                store_values<32>(row, out[i], half ? a.scale : 1.0f, 32 * i, a.dim);
+            }
+        }
+    }
+    close_block(ctl, warp, a.flags);
+}
+
+// ------------------------------------------------------------------- host
+
+// The planes of up to four tensors, one behind the other in the workspace; their tensor maps' base addresses.
+struct Planes {
+    SplitArgs args{};
+    int count = 0;
+    __nv_bfloat16* next;
+
+    explicit Planes(void* workspace) : next(static_cast<__nv_bfloat16*>(workspace)) {}
+
+    const __nv_bfloat16* add(const void* x, int64_t rows, int heads, int64_t row, int64_t head, int dim) {
+        __nv_bfloat16* const planes = next;
+        args.x[count] = static_cast<const float*>(x);
+        args.planes[count] = planes;
+        args.rows[count] = rows;
+        args.heads[count] = heads;
+        args.row[count] = row;
+        args.head[count] = head;
+        args.dim = dim;
+        ++count;
+        next += 3 * rows * heads * dim;
+        return planes;
+    }
+
+    fmd_status launch(cudaStream_t s) const {
+        int64_t most = 0;
+        for (int i = 0; i < count; ++i) {
+            const int64_t n = args.rows[i] * args.heads[i] * (args.dim / 8);
+            most = n > most ? n : most;
+        }
+        if (most == 0) return FMD_OK;
+        split_kernel<<<dim3(unsigned(grid_for(most, 256)), unsigned(count)), 256, 0, s>>>(args);
+        return check_launch();
+    }
+};
+
+fmd_status encode_planes(const DriverCalls& drv, CUtensorMap* map, const void* planes, int64_t rows, int hk, int group,
+                         int dim, int tokens) {
+    return encode_packed(drv, map, planes, 3 * rows, hk, group, dim, int64_t(hk) * group * dim, dim, tokens);
+}
+
+template <int KS>
+fmd_status launch_forward(const Maps& maps, const Attn& a, int splits, cudaStream_t s) {
+    const void* kernel = splits > 1 ? (const void*)forward_kernel<KS, true> : (const void*)forward_kernel<KS, false>;
+    const fmd_status st = grant_dynamic_smem(kernel, kForwardBytes, true);
+    if (st != FMD_OK) return st;
+    const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kTile / a.group)), unsigned(a.hk), unsigned(splits));
+    if (splits > 1) forward_kernel<KS, true><<<grid, kThreads, kForwardBytes, s>>>(maps, a);
+    else forward_kernel<KS, false><<<grid, kThreads, kForwardBytes, s>>>(maps, a);
+    return check_launch();
+}
+
+template <int KS>
+fmd_status launch_backward(const Maps& queries, const Maps& keys, const Attn& a, cudaStream_t s) {
+    fmd_status st = grant_dynamic_smem((const void*)query_gradient_kernel<KS>, kBackwardBytes, true);
+    if (st == FMD_OK) st = grant_dynamic_smem((const void*)key_gradient_kernel<KS>, kBackwardBytes, true);
+    if (st != FMD_OK) return st;
+    if (a.dq != nullptr && a.rows > 0) {
+        const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kTile / a.group)), unsigned(a.hk));
+        query_gradient_kernel<KS><<<grid, kThreads, kBackwardBytes, s>>>(queries, a);
+        if ((st = check_launch()) != FMD_OK) return st;
+    }
+    if (a.dk != nullptr && a.keys > 0) {
+        const dim3 grid(unsigned(tile_bound(a.keys, a.batch, kTile)), unsigned(a.hk));
+        key_gradient_kernel<KS><<<grid, kThreads, kBackwardBytes, s>>>(keys, a);
+        st = check_launch();
+    }
+    return st;
+}
+
+}  // namespace
+
+size_t attention_planes_bytes(const Attn& a, bool backward) {
+    const size_t values = size_t(a.rows) * a.hq * (backward ? 2 : 1) + size_t(a.keys) * a.hk * 2;
+    return (values * a.dim * 3 * sizeof(__nv_bfloat16) + 15) & ~size_t(15);
+}
+
+fmd_status attention_forward_planes(const Attn& a, int splits, void* workspace, cudaStream_t s) {
+    const DriverCalls& drv = driver_calls();
+    if (drv.encode == nullptr || drv.ctx_get_current == nullptr)
+        return record_error_text(FMD_ERR_CUDA, "driver entry point cuTensorMapEncodeTiled unavailable", 0);
+    fmd_status st = bind_context(drv);
+    Maps maps{};
+    Planes planes(workspace);
+    if (st == FMD_OK)
+        st = encode_planes(drv, &maps.q, planes.add(a.q, a.rows, a.hq, a.q_row, a.q_head, a.dim), a.rows, a.hk, a.group,
+                           a.dim, kTile / a.group);
+    if (a.keys > 0) {
+        if (st == FMD_OK)
+            st = encode_planes(drv, &maps.k, planes.add(a.k, a.keys, a.hk, a.k_row, a.k_head, a.dim), a.keys, a.hk, 1,
+                               a.dim, kTile);
+        if (st == FMD_OK)
+            st = encode_planes(drv, &maps.v, planes.add(a.v, a.keys, a.hk, a.v_row, a.v_head, a.dim), a.keys, a.hk, 1,
+                               a.dim, kTile);
+    }
+    if (st == FMD_OK) st = planes.launch(s);
+    if (st != FMD_OK) return st;
+    return a.dim <= 32 ? launch_forward<2>(maps, a, splits, s) : launch_forward<4>(maps, a, splits, s);
+}
+
+fmd_status attention_backward_planes(const Attn& a, void* workspace, cudaStream_t s) {
+    const DriverCalls& drv = driver_calls();
+    if (drv.encode == nullptr || drv.ctx_get_current == nullptr)
+        return record_error_text(FMD_ERR_CUDA, "driver entry point cuTensorMapEncodeTiled unavailable", 0);
+    fmd_status st = bind_context(drv);
+    Maps queries{}, keys{};  // own tiles of 128 rows and streamed ones of 64, of the one kernel and of the other
+    Planes planes(workspace);
+    if (a.rows > 0) {
+        const void* q = planes.add(a.q, a.rows, a.hq, a.q_row, a.q_head, a.dim);
+        const void* g = planes.add(a.g, a.rows, a.hq, a.g_row, a.g_head, a.dim);
+        for (int i = 0; i < 2 && st == FMD_OK; ++i) {
+            Maps& maps = i ? keys : queries;
+            const int tokens = (i ? kStream : kTile) / a.group;
+            st = encode_planes(drv, &maps.q, q, a.rows, a.hk, a.group, a.dim, tokens);
+            if (st == FMD_OK) st = encode_planes(drv, &maps.g, g, a.rows, a.hk, a.group, a.dim, tokens);
+        }
+    }
+    if (a.keys > 0) {
+        const void* k = planes.add(a.k, a.keys, a.hk, a.k_row, a.k_head, a.dim);
+        const void* v = planes.add(a.v, a.keys, a.hk, a.v_row, a.v_head, a.dim);
+        for (int i = 0; i < 2 && st == FMD_OK; ++i) {
+            Maps& maps = i ? keys : queries;
+            st = encode_planes(drv, &maps.k, k, a.keys, a.hk, 1, a.dim, i ? kTile : kStream);
+            if (st == FMD_OK) st = encode_planes(drv, &maps.v, v, a.keys, a.hk, 1, a.dim, i ? kTile : kStream);
+        }
+    }
+    if (st == FMD_OK) st = planes.launch(s);
+    if (st != FMD_OK) return st;
+    return a.dim <= 32 ? launch_backward<2>(queries, keys, a, s) : launch_backward<4>(queries, keys, a, s);
+}
+
+}  // namespace fmd

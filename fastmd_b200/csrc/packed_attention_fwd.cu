@@ -43,7 +43,7 @@ struct Shape {
 template <int KS, int NT>
 struct Ctrl {
     uint64_t q_full;
-    uint64_t full[Shape<KS, NT>::kSlots], empty[Shape<KS, NT>::kSlots];
+    Ring<Shape<KS, NT>::kSlots> ring;
     uint64_t scores[NT], weights[NT], done[NT];
     uint64_t tail_here, tail;  // the last v tile has landed; its rows behind the last key are zeros
     uint64_t drain;
@@ -109,10 +109,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
 
     if (threadIdx.x == 0) {
         mbar_init(&ctl.q_full, 1);
-        for (int i = 0; i < S::kSlots; ++i) {
-            mbar_init(&ctl.full[i], 1);
-            mbar_init(&ctl.empty[i], 1);
-        }
+        init_ring(ctl.ring);
         for (int t = 0; t < NT; ++t) {
             mbar_init(&ctl.scores[t], 1);
             mbar_init(&ctl.weights[t], 128);
@@ -124,12 +121,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
         ctl.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&ctl.tmem)),
-                     "n"(S::kTmem)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    if (warp == 1) tmem_alloc<S::kTmem>(&ctl.tmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -146,35 +138,11 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
                     for (int p = 0; p < S::kPanels; ++p)
                         tma_load_4d(su32(smem + t * S::kTileBytes + p * kPanelBytes), &maps.q, &ctl.q_full, p * 64, 0,
                                     head, int(s.row0 + token0) + t * per_tile);
-            int slot = 0, armed = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int i = 0; i < 2 * last; ++i) {  // k0, v0, k1, v1, ..
-                if (!mbar_wait(&ctl.empty[slot], phase ^ 1u, abort)) {
-                    ok = false;
-                    break;
-                }
-                mbar_expect_tx(&ctl.full[slot], S::kTileBytes);
-                for (int p = 0; p < S::kPanels; ++p)
-                    tma_load_4d(su32(ring + slot * S::kTileBytes + p * kPanelBytes), i & 1 ? &maps.v : &maps.k,
-                                &ctl.full[slot], p * 64, 0, head, int(s.key0) + from + (i >> 1) * kTile);
-                armed = i + 1;
-                if (++slot == S::kSlots) {
-                    slot = 0;
-                    phase ^= 1u;
-                }
-            }
-            if (!ok) {  // the copies in flight land before the block ends
-                mbar_wait(&ctl.q_full, 0, abort, true);
-                for (int i = max(0, armed - S::kSlots); i < armed; ++i)
-                    mbar_wait(&ctl.full[i % S::kSlots], uint32_t(i / S::kSlots) & 1u, abort, true);
-            } else {  // the last slots' releases land before the block ends
-                for (int i = 0; i < S::kSlots && mbar_wait(&ctl.empty[slot], phase ^ 1u, abort); ++i)
-                    if (++slot == S::kSlots) {
-                        slot = 0;
-                        phase ^= 1u;
-                    }
-            }
+            feed(ctl.ring, &ctl.q_full, abort, 2 * last, S::kTileBytes, [&](int i, int slot, uint64_t* bar) {
+                for (int p = 0; p < S::kPanels; ++p)  // k0, v0, k1, v1, ..
+                    tma_load_4d(su32(ring + slot * S::kTileBytes + p * kPanelBytes), i & 1 ? &maps.v : &maps.k, bar,
+                                p * 64, 0, head, int(s.key0) + from + (i >> 1) * kTile);
+            });
         }
     } else if (warp == 1) {
         if (lane == 0 && last > 0) {
@@ -184,7 +152,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
             bool ok = mbar_wait(&ctl.q_full, 0, abort), issued = false;
             auto next = [&] {  // waits for the next tile; its place
                 const int at = slot;
-                ok = ok && mbar_wait(&ctl.full[slot], phase, abort);
+                ok = ok && mbar_wait(&ctl.ring.full[slot], phase, abort);
                 if (++slot == S::kSlots) {
                     slot = 0;
                     phase ^= 1u;
@@ -203,7 +171,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
             if (ok) {
                 for (int t = 0; t < NT; ++t)
                     if (counts[t] > 0) score(t, 0, k_slot);
-                tc_commit(&ctl.empty[k_slot]);
+                tc_commit(&ctl.ring.empty[k_slot]);
             }
             for (int j = 0; j < last && ok; ++j) {
                 const int v_slot = next();
@@ -219,10 +187,10 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
                         ok = ok && mbar_wait(&ctl.weights[t], uint32_t(j) & 1u, abort);
                         if (!ok) break;
                         tc_fence_after();
-                        product_weights<32>(tmem + S::kO + uint32_t(t) * S::kDim, tmem + t * 128u,
+                        product_weights<4, 32>(tmem + S::kO + uint32_t(t) * S::kDim, tmem + t * 128u,
                                         su32(ring + v_slot * S::kTileBytes), width(t, j) / 16, o_desc, j > 0);
                     }
-                    if (t == NT - 1) tc_commit(&ctl.empty[v_slot]);
+                    if (t == NT - 1) tc_commit(&ctl.ring.empty[v_slot]);
                     if (j + 1 < last && !have_k) {
                         k_slot = next();
                         if (!ok) break;
@@ -230,7 +198,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
                     }
                     if (j + 1 < counts[t]) score(t, j + 1, k_slot);
                     else if (j + 1 == counts[t]) tc_commit(&ctl.done[t]);
-                    if (t == NT - 1 && j + 1 < last) tc_commit(&ctl.empty[k_slot]);
+                    if (t == NT - 1 && j + 1 < last) tc_commit(&ctl.ring.empty[k_slot]);
                 }
             }
             if (!ok && issued) {  // the products in flight end before TMEM is freed
@@ -242,7 +210,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
         if (tail) {
             if (mbar_wait(&ctl.tail_here, 0, abort)) {
                 const int first = keys - (last - 1) * kTile;
-                zero_rows(ring + ((2 * last - 1) % S::kSlots) * S::kTileBytes, S::kPanels, first, (first + 15) & ~15, threadIdx.x - 64, 64);
+                zero_rows(ring + ((2 * last - 1) % S::kSlots) * S::kTileBytes, S::kPanels, kPanelBytes, first, (first + 15) & ~15, threadIdx.x - 64, 64);
                 mbar_arrive(&ctl.tail);
             }
         }
@@ -369,51 +337,18 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
-        __syncwarp();
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kTmem) : "memory");
-    }
+    if (warp == 1) tmem_free<S::kTmem>(tmem);
     if (threadIdx.x == 0 && ctl.abort) raise_flag(a.flags, FMD_FLAG_WAIT_TIMEOUT);
-}
-
-// out and lse of the splits together: out = sum_z 2^(lse_z - lse) out_z. A thread per row and four values.
-__global__ void __launch_bounds__(256) join_kernel(const Attn a, int splits) {
-    const int quads = a.dim / 4;
-    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x, all = a.rows * a.hq, row = i / quads;
-    const int quad = int(i - row * quads);
-    if (row >= all) return;
-    float top = -INFINITY;
-    for (int z = 0; z < splits; ++z) top = fmaxf(top, a.part_lse[z * all + row]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
-    float4 o = f4_zero();
-    for (int z = 0; z < splits; ++z) {
-        const float lse = a.part_lse[z * all + row];
-        if (lse == -INFINITY) continue;  // a split without keys of this row wrote nothing else
-        const float w = exp2f((lse - base) * kLog2e);
-        const float4 v = *reinterpret_cast<const float4*>(a.part + (z * all + row) * a.dim + quad * 4);
-        sum += w;
-        o = make_float4(fmaf(w, v.x, o.x), fmaf(w, v.y, o.y), fmaf(w, v.z, o.z), fmaf(w, v.w, o.w));
-    }
-    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + row * a.dim + quad * 4) =
-        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
-    if (quad == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? -INFINITY : top + logf(sum);
 }
 
 template <int KS, int NT, bool SPLIT>
 fmd_status launch(const Maps& maps, const Attn& a, int splits, cudaStream_t s) {
     using S = Shape<KS, NT>;
-    fmd_status st = grant_dynamic_smem((const void*)forward_kernel<KS, NT, SPLIT>, S::kBytes, true);
+    const fmd_status st = grant_dynamic_smem((const void*)forward_kernel<KS, NT, SPLIT>, S::kBytes, true);
     if (st != FMD_OK) return st;
     const int64_t tiles = tile_bound(a.rows, a.batch, NT * (kTile / a.group));
     forward_kernel<KS, NT, SPLIT>
         <<<dim3(unsigned(tiles), unsigned(a.hk), unsigned(splits)), S::kThreads, S::kBytes, s>>>(maps, a);
-    st = check_launch();
-    if (!SPLIT || st != FMD_OK) return st;
-    const int64_t threads = a.rows * a.hq * (a.dim / 4);
-    join_kernel<<<unsigned((threads + 255) / 256), 256, 0, s>>>(a, splits);
     return check_launch();
 }
 
@@ -440,7 +375,7 @@ fmd_status encode_packed(const DriverCalls& drv, CUtensorMap* map, const void* x
     return r == CUDA_SUCCESS ? FMD_OK : record_error_text(FMD_ERR_CUDA, "cuTensorMapEncodeTiled failed, CUresult", r);
 }
 
-fmd_status attention_forward_mma(const Attn& a, cudaStream_t s) {
+fmd_status attention_forward_mma(const Attn& a, int splits, cudaStream_t s) {
     const DriverCalls& drv = driver_calls();
     if (drv.encode == nullptr || drv.ctx_get_current == nullptr)
         return record_error_text(FMD_ERR_CUDA, "driver entry point cuTensorMapEncodeTiled unavailable", 0);
@@ -453,20 +388,10 @@ fmd_status attention_forward_mma(const Attn& a, cudaStream_t s) {
         if (st == FMD_OK) st = encode_packed(drv, &maps.v, a.v, a.keys, a.hk, 1, a.dim, a.v_row, a.v_head, kTile);
     }
     if (st != FMD_OK) return st;
-    const int splits = attention_splits(a);
     return a.dim <= 32 ? launch<2>(maps, a, splits, s) : a.dim <= 64 ? launch<4>(maps, a, splits, s)
          : a.dim <= 96 ? launch<6>(maps, a, splits, s) : launch<8>(maps, a, splits, s);
 }
 
-// Splits of the keys: where the tiles of rows do not fill the SMs twice over, their keys are shared out. The lengths
-// are on the device: the host goes by the mean length of a sequence's slot, and a split has two key tiles at least.
-int attention_splits(const Attn& a) {
-    const int64_t tiles = tile_bound(a.rows, a.batch, kTile / a.group) * a.hk;
-    if (tiles == 0 || a.batch == 0) return 1;
-    const int64_t key_tiles = (a.keys / a.batch + kTile - 1) / kTile;
-    int64_t splits = 2 * kNumSMs / tiles;
-    if (splits > key_tiles / 2) splits = key_tiles / 2;
-    return splits < 1 ? 1 : splits > 64 ? 64 : int(splits);
-}
+int attention_splits_mma(const Attn& a) { return key_splits(a, kTile / a.group, 2 * kNumSMs, 2 * kTile); }
 
 }  // namespace fmd

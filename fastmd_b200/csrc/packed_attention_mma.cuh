@@ -64,30 +64,30 @@ __device__ __forceinline__ void mma_weights(uint32_t d, uint32_t p, uint32_t b, 
         : "memory");
 }
 
-// D [128, n] = A B^T over KS steps of 16 along the rows of both tiles.
+// D [128, n] (+)= A B^T over KS steps of 16 along the rows of both tiles.
 template <int KS>
-__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add = false) {
     const uint32_t ad = rows_desc(a), bd = rows_desc(b);
 #pragma unroll
     for (int k = 0; k < KS; k += 2) {
         const uint32_t off = uint32_t(k / 4) * kPanelStep + uint32_t(k % 4) * 2;
-        mma_rows2(d, ad + off, bd + off, idesc, k > 0);
+        mma_rows2(d, ad + off, bd + off, idesc, add || k > 0);
     }
 }
 
-// D [128, n] (+)= P B over `steps` (at most 8) steps of 16 rows of B, P [128, 16 steps] bfloat16 in TMEM: the first
-// four steps at p, the others at p + second.
-template <uint32_t kSecond>
+// D [128, n] (+)= P B over `steps` (at most 2 HALF) steps of 16 rows of B, P [128, 16 steps] bfloat16 in TMEM: the
+// first HALF steps at p, the others at p + kSecond.
+template <int HALF, uint32_t kSecond>
 __device__ __forceinline__ void product_weights(uint32_t d, uint32_t p, uint32_t b, int steps, uint32_t idesc,
                                                 bool add) {
     const uint32_t bd = columns_desc(b);
-    if (steps == kTile / 16) {
+    if (steps == 2 * HALF) {
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-            mma_weights(d, p + 8 * (k % 4) + (k / 4) * kSecond, bd + k * 128, idesc, add || k > 0);
+        for (int k = 0; k < 2 * HALF; ++k)
+            mma_weights(d, p + 8 * (k % HALF) + (k / HALF) * kSecond, bd + k * 128, idesc, add || k > 0);
     } else {
         for (int k = 0; k < steps; ++k)
-            mma_weights(d, p + 8 * (k % 4) + (k / 4) * kSecond, bd + k * 128, idesc, add || k > 0);
+            mma_weights(d, p + 8 * (k % HALF) + (k / HALF) * kSecond, bd + k * 128, idesc, add || k > 0);
     }
 }
 
@@ -106,6 +106,17 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
                    "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
                  : "r"(addr)
                  : "memory");
+}
+
+// 16 columns, in the same way
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(addr)
+        : "memory");
 }
 
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const float (&v)[32]) {
@@ -164,21 +175,95 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     return d;
 }
 
+__device__ __forceinline__ float2 unpack_bf16(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float low, float high) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
     return r;
 }
 
-// Zeros rows [first, last) of a tile of `panels` panels (the swizzle keeps a row's 128 bytes in place), by `count`
-// threads; then visible to the tensor cores after the barrier that follows.
-__device__ __forceinline__ void zero_rows(unsigned char* tile, int panels, int first, int last, int thread, int count) {
+// Zeros rows [first, last) of `panels` panels that lie `stride` bytes apart (the swizzle keeps a row's 128 bytes in
+// place), by `count` threads; then visible to the tensor cores after the barrier that follows.
+__device__ __forceinline__ void zero_rows(unsigned char* tile, int panels, uint32_t stride, int first, int last,
+                                          int thread, int count) {
     const int per = (last - first) * 8;
     for (int i = thread; i < per * panels; i += count) {
         const int p = i / per, w = i - p * per;
-        *reinterpret_cast<uint4*>(tile + p * kPanelBytes + first * 128 + w * 16) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(tile + p * stride + first * 128 + w * 16) = make_uint4(0, 0, 0, 0);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// A ring of shared-memory slots that TMA fills in order.
+template <int SLOTS>
+struct Ring {
+    uint64_t full[SLOTS], empty[SLOTS];
+};
+
+template <int SLOTS>
+__device__ __forceinline__ void init_ring(Ring<SLOTS>& ring) {
+    for (int i = 0; i < SLOTS; ++i) {
+        mbar_init(&ring.full[i], 1);
+        mbar_init(&ring.empty[i], 1);
+    }
+}
+
+// The producer (one thread): `count` tiles of `bytes` each, tile i by load(i, slot, barrier). `own`: the barrier of
+// the copies that the caller has started before.
+template <int SLOTS, typename Load>
+__device__ __forceinline__ void feed(Ring<SLOTS>& ring, uint64_t* own, volatile int32_t* abort, int count,
+                                     uint32_t bytes, Load load) {
+    int slot = 0, armed = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int i = 0; i < count; ++i) {
+        if (!mbar_wait(&ring.empty[slot], phase ^ 1u, abort)) {
+            ok = false;
+            break;
+        }
+        mbar_expect_tx(&ring.full[slot], bytes);
+        load(i, slot, &ring.full[slot]);
+        armed = i + 1;
+        if (++slot == SLOTS) {
+            slot = 0;
+            phase ^= 1u;
+        }
+    }
+    if (!ok) {  // the copies in flight land before the block ends
+        mbar_wait(own, 0, abort, true);
+        for (int i = max(0, armed - SLOTS); i < armed; ++i)
+            mbar_wait(&ring.full[i % SLOTS], uint32_t(i / SLOTS) & 1u, abort, true);
+    } else {  // the last slots' releases land before the block ends
+        for (int i = 0; i < SLOTS && mbar_wait(&ring.empty[slot], phase ^ 1u, abort); ++i)
+            if (++slot == SLOTS) {
+                slot = 0;
+                phase ^= 1u;
+            }
+    }
+}
+
+// Waits for tile i; only for a thread that takes the tiles of each slot in order.
+template <int SLOTS>
+__device__ __forceinline__ bool landed(Ring<SLOTS>& ring, int i, volatile int32_t* abort) {
+    return mbar_wait(&ring.full[i % SLOTS], uint32_t(i / SLOTS) & 1u, abort);
+}
+
+// The block's TMEM: COLUMNS of it, by one whole warp; the address through shared memory.
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_alloc(uint32_t* address) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(address)), "n"(COLUMNS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_free(uint32_t address) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "n"(COLUMNS) : "memory");
 }
 
 // ------------------------------------------------------------------- host

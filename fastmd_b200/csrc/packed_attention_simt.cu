@@ -1,4 +1,5 @@
-// Packed attention on the FP32 cores: forward, and the gradients of q and of k and v.
+// Packed attention in float32 on the FP32 cores, for heads of more than 64 values: forward, and the gradients of q and
+// of k and v. (Smaller heads take the tensor cores: three planes of a wider tile do not fit in shared memory.)
 //
 //   forward   s = scale q k^T (log2 units), running maximum m and sum l per row over key tiles:
 //             o = (o 2^(m - m') + 2^(s - m') v),  l likewise;  out = o / l,  lse = m + log l
@@ -15,27 +16,26 @@
 namespace fmd {
 namespace {
 
-constexpr int kM = 64, kN = 64, kThreads = 256;
+constexpr int kM = 64, kN = 64, kThreads = 256, kDim = 128;
 
-// rows [0, count) of src (row stride ld, dim values) into dst [64][DP + 4], zeros elsewhere
-template <typename T, int DP, typename RowOf>
-__device__ __forceinline__ void load_tile(float* dst, const T* src, int count, int dim, RowOf row_of) {
-    for (int i = threadIdx.x; i < 64 * DP; i += kThreads) {
-        const int r = i / DP, c = i - r * DP;
-        dst[r * (DP + 4) + c] = r < count && c < dim ? attn_float(src[row_of(r) + c]) : 0.0f;
+// rows [0, count) of src (row stride ld, dim values) into dst [64][kDim + 4], zeros elsewhere
+template <typename RowOf>
+__device__ __forceinline__ void load_tile(float* dst, const float* src, int count, int dim, RowOf row_of) {
+    for (int i = threadIdx.x; i < 64 * kDim; i += kThreads) {
+        const int r = i / kDim, c = i - r * kDim;
+        dst[r * (kDim + 4) + c] = r < count && c < dim ? src[row_of(r) + c] : 0.0f;
     }
 }
 
 // acc[i][j] += sum_d a[ty + 16 i][d] b[tx + 16 j][d]
-template <int DP>
 __device__ __forceinline__ void dots(const float* a, const float* b, int ty, int tx, float (&acc)[4][4]) {
 #pragma unroll 4
-    for (int d = 0; d < DP; d += 4) {
+    for (int d = 0; d < kDim; d += 4) {
         float4 x[4], y[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * (DP + 4) + d);
+        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * (kDim + 4) + d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * (DP + 4) + d);
+        for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * (kDim + 4) + d);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -49,8 +49,7 @@ __device__ __forceinline__ void dots(const float* a, const float* b, int ty, int
 }
 
 // acc[i][c] += sum_n p[ty + 16 i][n] b[n][2 tx + 32 (c / 2) + c % 2] over the 64 rows of b
-template <int DP>
-__device__ __forceinline__ void weigh(const float* p, const float* b, int ty, int tx, float (&acc)[4][DP / 16]) {
+__device__ __forceinline__ void weigh(const float* p, const float* b, int ty, int tx, float (&acc)[4][kDim / 16]) {
 #pragma unroll 2
     for (int n = 0; n < 64; n += 4) {
         float4 x[4];
@@ -59,8 +58,8 @@ __device__ __forceinline__ void weigh(const float* p, const float* b, int ty, in
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
 #pragma unroll
-            for (int c = 0; c < DP / 32; ++c) {
-                const float2 y = *reinterpret_cast<const float2*>(b + (n + u) * (DP + 4) + 2 * tx + 32 * c);
+            for (int c = 0; c < kDim / 32; ++c) {
+                const float2 y = *reinterpret_cast<const float2*>(b + (n + u) * (kDim + 4) + 2 * tx + 32 * c);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float w = u == 0 ? x[i].x : u == 1 ? x[i].y : u == 2 ? x[i].z : x[i].w;
@@ -94,13 +93,13 @@ struct Rows {
     __device__ int64_t flat(int r) const { return (row0 + r / group) * hq + head0 + r % group; }
 };
 
-template <typename T, int DP>
+template <bool SPLIT>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const Attn a) {
     extern __shared__ float smem[];
     float* qs = smem;
-    float* ks = qs + 64 * (DP + 4);
-    float* vs = ks + 64 * (DP + 4);
-    float* ps = vs + 64 * (DP + 4);
+    float* ks = qs + 64 * (kDim + 4);
+    float* vs = ks + 64 * (kDim + 4);
+    float* ps = vs + 64 * (kDim + 4);
     const int per_tile = kM / a.group;
     const int b = find_sequence(a.offsets, a.batch, per_tile, blockIdx.x);
     const Span s = load_span(a, b);
@@ -109,12 +108,12 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Attn a) {
     const int tokens = int(min(int64_t(per_tile), s.rows - token0)), rows = tokens * a.group;
     const Rows at{s.row0 + token0, a.group, int(blockIdx.y) * a.group, a.hq};
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const T* kp = static_cast<const T*>(a.k) + s.key0 * a.k_row + blockIdx.y * a.k_head;
-    const T* vp = static_cast<const T*>(a.v) + s.key0 * a.v_row + blockIdx.y * a.v_head;
-    load_tile<T, DP>(qs, static_cast<const T*>(a.q), rows, a.dim,
+    const float* kp = static_cast<const float*>(a.k) + s.key0 * a.k_row + blockIdx.y * a.k_head;
+    const float* vp = static_cast<const float*>(a.v) + s.key0 * a.v_row + blockIdx.y * a.v_head;
+    load_tile(qs, static_cast<const float*>(a.q), rows, a.dim,
                      [&](int r) { return at.at(r, a.q_row, a.q_head); });
     int64_t limit[4];
-    float m[4], l[4], o[4][DP / 16];
+    float m[4], l[4], o[4][kDim / 16];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = ty + 16 * i;
@@ -122,18 +121,23 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Attn a) {
         m[i] = -INFINITY;
         l[i] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) o[i][c] = 0.0f;
+        for (int c = 0; c < kDim / 16; ++c) o[i][c] = 0.0f;
     }
-    const int64_t end = seen(s, a.causal, token0 + tokens - 1);
+    int64_t end = seen(s, a.causal, token0 + tokens - 1), from = 0;
+    if (SPLIT) {  // a range of the key tiles
+        const int64_t share = (((end + kN - 1) / kN + gridDim.z - 1) / gridDim.z) * kN;
+        from = min(end, blockIdx.z * share);
+        end = min(end, from + share);
+    }
     const float scale = a.scale * kLog2e;
-    for (int64_t n0 = 0; n0 < end; n0 += kN) {
+    for (int64_t n0 = from; n0 < end; n0 += kN) {
         const int n = int(min(int64_t(kN), end - n0));
         __syncthreads();
-        load_tile<T, DP>(ks, kp + n0 * a.k_row, n, a.dim, [&](int r) { return r * a.k_row; });
-        load_tile<T, DP>(vs, vp + n0 * a.v_row, n, a.dim, [&](int r) { return r * a.v_row; });
+        load_tile(ks, kp + n0 * a.k_row, n, a.dim, [&](int r) { return r * a.k_row; });
+        load_tile(vs, vp + n0 * a.v_row, n, a.dim, [&](int r) { return r * a.v_row; });
         __syncthreads();
         float x[4][4] = {};
-        dots<DP>(qs, ks, ty, tx, x);
+        dots(qs, ks, ty, tx, x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float top = -INFINITY;
@@ -155,23 +159,25 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Attn a) {
             }
             l[i] = l[i] * keep + sum16(sum);
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) o[i][c] *= keep;
+            for (int c = 0; c < kDim / 16; ++c) o[i][c] *= keep;
         }
         __syncthreads();
-        weigh<DP>(ps, vs, ty, tx, o);
+        weigh(ps, vs, ty, tx, o);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = ty + 16 * i;
         if (r >= rows) continue;
         const float inv = l[i] > 0.0f ? 1.0f / l[i] : (l[i] == 0.0f ? 0.0f : l[i]);
-        T* out = static_cast<T*>(a.out) + at.flat(r) * a.dim;
+        const int64_t flat = at.flat(r) + (SPLIT ? int64_t(blockIdx.z) * a.rows * a.hq : 0);
+        float* out = (SPLIT ? a.part : static_cast<float*>(a.out)) + flat * a.dim;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) {
+        for (int c = 0; c < kDim / 16; ++c) {
             const int col = 2 * tx + 32 * (c / 2) + c % 2;
-            if (col < a.dim) attn_store(out + col, o[i][c] * inv);
+            if (col < a.dim) out[col] = o[i][c] * inv;
         }
-        if (a.lse != nullptr && tx == 0) a.lse[at.flat(r)] = l[i] == 0.0f ? -INFINITY : m[i] * kLn2 + logf(l[i]);
+        float* lse = SPLIT ? a.part_lse : a.lse;
+        if (lse != nullptr && tx == 0) lse[flat] = l[i] == 0.0f ? -INFINITY : m[i] * kLn2 + logf(l[i]);
     }
 }
 
@@ -180,14 +186,13 @@ __device__ __forceinline__ float weight_of(float dot, float scale, float lse2, b
     return there ? exp2f(dot * scale - lse2) : 0.0f;
 }
 
-template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const Attn a) {
     extern __shared__ float smem[];
     float* qs = smem;
-    float* gs = qs + 64 * (DP + 4);
-    float* ks = gs + 64 * (DP + 4);
-    float* vs = ks + 64 * (DP + 4);
-    float* ds = vs + 64 * (DP + 4);
+    float* gs = qs + 64 * (kDim + 4);
+    float* ks = gs + 64 * (kDim + 4);
+    float* vs = ks + 64 * (kDim + 4);
+    float* ds = vs + 64 * (kDim + 4);
     const int per_tile = kM / a.group;
     const int b = find_sequence(a.offsets, a.batch, per_tile, blockIdx.x);
     const Span s = load_span(a, b);
@@ -196,14 +201,14 @@ __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const Attn a) 
     const int tokens = int(min(int64_t(per_tile), s.rows - token0)), rows = tokens * a.group;
     const Rows at{s.row0 + token0, a.group, int(blockIdx.y) * a.group, a.hq};
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const T* kp = static_cast<const T*>(a.k) + s.key0 * a.k_row + blockIdx.y * a.k_head;
-    const T* vp = static_cast<const T*>(a.v) + s.key0 * a.v_row + blockIdx.y * a.v_head;
-    load_tile<T, DP>(qs, static_cast<const T*>(a.q), rows, a.dim,
+    const float* kp = static_cast<const float*>(a.k) + s.key0 * a.k_row + blockIdx.y * a.k_head;
+    const float* vp = static_cast<const float*>(a.v) + s.key0 * a.v_row + blockIdx.y * a.v_head;
+    load_tile(qs, static_cast<const float*>(a.q), rows, a.dim,
                      [&](int r) { return at.at(r, a.q_row, a.q_head); });
-    load_tile<T, DP>(gs, static_cast<const T*>(a.g), rows, a.dim,
+    load_tile(gs, static_cast<const float*>(a.g), rows, a.dim,
                      [&](int r) { return at.at(r, a.g_row, a.g_head); });
     int64_t limit[4];
-    float lse2[4], delta[4], dq[4][DP / 16];
+    float lse2[4], delta[4], dq[4][kDim / 16];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = ty + 16 * i;
@@ -211,19 +216,19 @@ __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const Attn a) 
         limit[i] = lse2[i] != -INFINITY ? seen(s, a.causal, token0 + r / a.group) : 0;  // an empty row has no share
         delta[i] = r < rows ? a.delta[at.flat(r)] : 0.0f;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) dq[i][c] = 0.0f;
+        for (int c = 0; c < kDim / 16; ++c) dq[i][c] = 0.0f;
     }
     const int64_t end = seen(s, a.causal, token0 + tokens - 1);
     const float scale = a.scale * kLog2e;
     for (int64_t n0 = 0; n0 < end; n0 += kN) {
         const int n = int(min(int64_t(kN), end - n0));
         __syncthreads();
-        load_tile<T, DP>(ks, kp + n0 * a.k_row, n, a.dim, [&](int r) { return r * a.k_row; });
-        load_tile<T, DP>(vs, vp + n0 * a.v_row, n, a.dim, [&](int r) { return r * a.v_row; });
+        load_tile(ks, kp + n0 * a.k_row, n, a.dim, [&](int r) { return r * a.k_row; });
+        load_tile(vs, vp + n0 * a.v_row, n, a.dim, [&](int r) { return r * a.v_row; });
         __syncthreads();
         float x[4][4] = {}, y[4][4] = {};
-        dots<DP>(qs, ks, ty, tx, x);
-        dots<DP>(gs, vs, ty, tx, y);
+        dots(qs, ks, ty, tx, x);
+        dots(gs, vs, ty, tx, y);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -233,29 +238,28 @@ __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const Attn a) 
                 ds[(ty + 16 * i) * (64 + 4) + tx + 16 * j] = there ? p * (y[i][j] - delta[i]) : 0.0f;
             }
         __syncthreads();
-        weigh<DP>(ds, ks, ty, tx, dq);
+        weigh(ds, ks, ty, tx, dq);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = ty + 16 * i;
         if (r >= rows) continue;
-        T* out = static_cast<T*>(a.dq) + at.flat(r) * a.dim;
+        float* out = static_cast<float*>(a.dq) + at.flat(r) * a.dim;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) {
+        for (int c = 0; c < kDim / 16; ++c) {
             const int col = 2 * tx + 32 * (c / 2) + c % 2;
-            if (col < a.dim) attn_store(out + col, dq[i][c] * a.scale);
+            if (col < a.dim) out[col] = dq[i][c] * a.scale;
         }
     }
 }
 
-template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads) key_gradient_kernel(const Attn a) {
     extern __shared__ float smem[];
     float* ks = smem;
-    float* vs = ks + 64 * (DP + 4);
-    float* qs = vs + 64 * (DP + 4);
-    float* gs = qs + 64 * (DP + 4);
-    float* ps = gs + 64 * (DP + 4);
+    float* vs = ks + 64 * (kDim + 4);
+    float* qs = vs + 64 * (kDim + 4);
+    float* gs = qs + 64 * (kDim + 4);
+    float* ps = gs + 64 * (kDim + 4);
     float* ds = ps + 64 * (64 + 4);
     __shared__ float lse2[64], delta[64];
     __shared__ int64_t limit[64];
@@ -265,11 +269,11 @@ __global__ void __launch_bounds__(kThreads) key_gradient_kernel(const Attn a) {
     if (n0 < 0 || n0 >= s.slot) return;
     const int n = int(max(int64_t(0), min(int64_t(kN), s.keys - n0)));
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    load_tile<T, DP>(ks, static_cast<const T*>(a.k) + (s.key0 + n0) * a.k_row + blockIdx.y * a.k_head, n, a.dim,
+    load_tile(ks, static_cast<const float*>(a.k) + (s.key0 + n0) * a.k_row + blockIdx.y * a.k_head, n, a.dim,
                      [&](int r) { return r * a.k_row; });
-    load_tile<T, DP>(vs, static_cast<const T*>(a.v) + (s.key0 + n0) * a.v_row + blockIdx.y * a.v_head, n, a.dim,
+    load_tile(vs, static_cast<const float*>(a.v) + (s.key0 + n0) * a.v_row + blockIdx.y * a.v_head, n, a.dim,
                      [&](int r) { return r * a.v_row; });
-    float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
+    float dk[4][kDim / 16] = {}, dv[4][kDim / 16] = {};
     const int per_tile = kM / a.group;
     const float scale = a.scale * kLog2e;
     // the first token that sees key n0
@@ -278,9 +282,9 @@ __global__ void __launch_bounds__(kThreads) key_gradient_kernel(const Attn a) {
         const int tokens = int(min(int64_t(per_tile), s.rows - token0)), rows = tokens * a.group;
         const Rows at{s.row0 + token0, a.group, int(blockIdx.y) * a.group, a.hq};
         __syncthreads();
-        load_tile<T, DP>(qs, static_cast<const T*>(a.q), rows, a.dim,
+        load_tile(qs, static_cast<const float*>(a.q), rows, a.dim,
                          [&](int r) { return at.at(r, a.q_row, a.q_head); });
-        load_tile<T, DP>(gs, static_cast<const T*>(a.g), rows, a.dim,
+        load_tile(gs, static_cast<const float*>(a.g), rows, a.dim,
                          [&](int r) { return at.at(r, a.g_row, a.g_head); });
         if (threadIdx.x < 64) {
             const int r = threadIdx.x;
@@ -290,8 +294,8 @@ __global__ void __launch_bounds__(kThreads) key_gradient_kernel(const Attn a) {
         }
         __syncthreads();
         float x[4][4] = {}, y[4][4] = {};
-        dots<DP>(ks, qs, ty, tx, x);
-        dots<DP>(vs, gs, ty, tx, y);
+        dots(ks, qs, ty, tx, x);
+        dots(vs, gs, ty, tx, y);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -303,8 +307,8 @@ __global__ void __launch_bounds__(kThreads) key_gradient_kernel(const Attn a) {
                 ds[key * (64 + 4) + r] = there ? p * (y[i][j] - delta[r]) : 0.0f;
             }
         __syncthreads();
-        weigh<DP>(ps, gs, ty, tx, dv);
-        weigh<DP>(ds, qs, ty, tx, dk);
+        weigh(ps, gs, ty, tx, dv);
+        weigh(ds, qs, ty, tx, dk);
     }
     // every row of the slot is written: keys that no query may see have zero gradients
     const int out_rows = int(min(int64_t(kN), s.slot - n0));
@@ -314,65 +318,45 @@ __global__ void __launch_bounds__(kThreads) key_gradient_kernel(const Attn a) {
         if (key >= out_rows) continue;
         const int64_t flat = ((s.key0 + n0 + key) * a.hk + blockIdx.y) * a.dim;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) {
+        for (int c = 0; c < kDim / 16; ++c) {
             const int col = 2 * tx + 32 * (c / 2) + c % 2;
             if (col < a.dim) {
-                attn_store(static_cast<T*>(a.dk) + flat + col, dk[i][c] * a.scale);
-                attn_store(static_cast<T*>(a.dv) + flat + col, dv[i][c]);
+                static_cast<float*>(a.dk)[flat + col] = dk[i][c] * a.scale;
+                static_cast<float*>(a.dv)[flat + col] = dv[i][c];
             }
         }
     }
 }
 
-template <typename T, int DP>
-fmd_status forward_typed(const Attn& a, cudaStream_t s) {
-    const size_t bytes = size_t(3 * 64 * (DP + 4) + 64 * 68) * sizeof(float);
-    fmd_status st = grant_dynamic_smem((const void*)forward_kernel<T, DP>, bytes);
+}  // namespace
+
+fmd_status attention_forward_simt(const Attn& a, int splits, cudaStream_t s) {
+    const size_t bytes = size_t(3 * 64 * (kDim + 4) + 64 * 68) * sizeof(float);
+    const void* kernel = splits > 1 ? (const void*)forward_kernel<true> : (const void*)forward_kernel<false>;
+    const fmd_status st = grant_dynamic_smem(kernel, bytes);
     if (st != FMD_OK) return st;
-    const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kM / a.group)), unsigned(a.hk));
-    forward_kernel<T, DP><<<grid, kThreads, bytes, s>>>(a);
+    const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kM / a.group)), unsigned(a.hk), unsigned(splits));
+    if (splits > 1) forward_kernel<true><<<grid, kThreads, bytes, s>>>(a);
+    else forward_kernel<false><<<grid, kThreads, bytes, s>>>(a);
     return check_launch();
 }
 
-template <typename T, int DP>
-fmd_status backward_typed(const Attn& a, cudaStream_t s) {
-    const size_t bytes = size_t(4 * 64 * (DP + 4) + 2 * 64 * 68) * sizeof(float);
-    fmd_status st = grant_dynamic_smem((const void*)query_gradient_kernel<T, DP>, bytes);
-    if (st == FMD_OK) st = grant_dynamic_smem((const void*)key_gradient_kernel<T, DP>, bytes);
+fmd_status attention_backward_simt(const Attn& a, cudaStream_t s) {
+    const size_t bytes = size_t(4 * 64 * (kDim + 4) + 2 * 64 * 68) * sizeof(float);
+    fmd_status st = grant_dynamic_smem((const void*)query_gradient_kernel, bytes);
+    if (st == FMD_OK) st = grant_dynamic_smem((const void*)key_gradient_kernel, bytes);
     if (st != FMD_OK) return st;
     if (a.dq != nullptr && a.rows > 0) {
         const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kM / a.group)), unsigned(a.hk));
-        query_gradient_kernel<T, DP><<<grid, kThreads, bytes, s>>>(a);
+        query_gradient_kernel<<<grid, kThreads, bytes, s>>>(a);
         if ((st = check_launch()) != FMD_OK) return st;
     }
     if (a.dk != nullptr && a.keys > 0) {
         const dim3 grid(unsigned(tile_bound(a.keys, a.batch, kN)), unsigned(a.hk));
-        key_gradient_kernel<T, DP><<<grid, kThreads, bytes, s>>>(a);
+        key_gradient_kernel<<<grid, kThreads, bytes, s>>>(a);
         st = check_launch();
     }
     return st;
-}
-
-template <typename T>
-fmd_status forward_sized(const Attn& a, cudaStream_t s) {
-    return a.dim <= 32 ? forward_typed<T, 32>(a, s) : a.dim <= 64 ? forward_typed<T, 64>(a, s)
-                                                                  : forward_typed<T, 128>(a, s);
-}
-
-template <typename T>
-fmd_status backward_sized(const Attn& a, cudaStream_t s) {
-    return a.dim <= 32 ? backward_typed<T, 32>(a, s) : a.dim <= 64 ? backward_typed<T, 64>(a, s)
-                                                                   : backward_typed<T, 128>(a, s);
-}
-
-}  // namespace
-
-fmd_status attention_forward_simt(const Attn& a, int type, cudaStream_t s) {
-    return type == FMD_F32 ? forward_sized<float>(a, s) : forward_sized<__nv_bfloat16>(a, s);
-}
-
-fmd_status attention_backward_simt(const Attn& a, int type, cudaStream_t s) {
-    return type == FMD_F32 ? backward_sized<float>(a, s) : backward_sized<__nv_bfloat16>(a, s);
 }
 
 }  // namespace fmd

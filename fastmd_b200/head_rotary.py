@@ -57,33 +57,35 @@ def _aligned(table: Tensor) -> Tensor:
     return table.clone() if table.data_ptr() % 16 else table
 
 
-def _launch(sides, x, weight_type, rot, interleaved, eps, positions, cos, sin, backward):
+def _like(x: Tensor) -> Tensor:
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _launch(sides, x, weight, cos, sin, positions, interleaved, eps, backward):
     rows, _, dim = x.shape
-    workspace = None
-    if backward and any(s.w for s in sides):
+    length, half = cos.shape
+    device = x.device
+    workspace, size = None, 0
+    if backward and weight is not None:
         nbytes = ctypes.c_size_t()
-        call("fmd_head_rotary_workspace_bytes", dim, ctypes.byref(nbytes))
-        workspace = torch.empty(nbytes.value, device=x.device, dtype=torch.uint8)
-    call("fmd_head_rotary", sides, TYPES[x.dtype], TYPES[weight_type], rows, dim, rot, interleaved, eps,
-         ptr(positions), ptr(cos), ptr(sin), cos.shape[0], backward, ptr(workspace),
-         0 if workspace is None else workspace.numel(), ptr(_lib.flags_word(x.device)), stream(x.device))
-
-
-def _weight_type(x: Tensor, *weights) -> torch.dtype:
-    return next((w.dtype for w in weights if w is not None), x.dtype)
+        call("fmd_head_rotary_workspace_bytes", dim, nbytes)
+        size = nbytes.value
+        workspace = torch.empty(size, device=device, dtype=torch.uint8)
+    kind = TYPES[x.dtype]
+    call("fmd_head_rotary", sides, kind, kind if weight is None else TYPES[weight.dtype], rows, dim, 2 * half,
+         interleaved, eps, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), length, backward, ptr(workspace), size,
+         ptr(_lib.flags_word(device)), stream(device))
 
 
 def _forward(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved):
-    outs = []
-    sides = (FmdHeadRotarySide * 2)()
-    for side, x, w in zip(sides, (q, k), (q_weight, k_weight)):
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        side.x, side.y, side.w, side.heads = ptr(x), ptr(y), ptr(w), x.shape[1]
-        side.row_stride, side.head_stride = x.stride(0), x.stride(1)
-        outs.append(y)
-    _launch(sides, q, _weight_type(q, q_weight, k_weight), 2 * cos.shape[1], interleaved, eps, positions, cos, sin,
-            False)
-    return tuple(outs)
+    q_out, k_out = _like(q), _like(k)
+    sides = (FmdHeadRotarySide * 2)(
+        FmdHeadRotarySide(q.data_ptr(), None, q_out.data_ptr(), ptr(q_weight), None, q.stride(0), q.stride(1), 0, 0,
+                          q.shape[1]),
+        FmdHeadRotarySide(k.data_ptr(), None, k_out.data_ptr(), ptr(k_weight), None, k.stride(0), k.stride(1), 0, 0,
+                          k.shape[1]))
+    _launch(sides, q, q_weight if q_weight is not None else k_weight, cos, sin, positions, interleaved, eps, False)
+    return q_out, k_out
 
 
 class _HeadNormRotary(Function):
@@ -100,24 +102,21 @@ class _HeadNormRotary(Function):
     def backward(ctx, gq, gk):
         q, k, positions, cos, sin, q_weight, k_weight = ctx.saved_tensors
         sides = (FmdHeadRotarySide * 2)()
-        grads, kept = [], []
-        for i, (side, x, g, w) in enumerate(zip(sides, (q, k), (gq, gk), (q_weight, k_weight))):
-            needed = ctx.needs_input_grad[i] or (w is not None and ctx.needs_input_grad[5 + i])
-            if not needed:  # heads = 0: this side is left out
+        grads, kept, weight = [], [], None
+        for i, (x, g, w) in enumerate(((q, gq, q_weight), (k, gk, k_weight))):
+            if not (ctx.needs_input_grad[i] or ctx.needs_input_grad[5 + i]):  # heads = 0: this side is left out
                 grads.append((None, None))
                 continue
             g = _head_rows(g)
-            dx = torch.empty(g.shape, device=g.device, dtype=g.dtype)
-            dw = torch.empty_like(w) if w is not None else None
-            side.g, side.y, side.w, side.dw, side.heads = ptr(g), ptr(dx), ptr(w), ptr(dw), g.shape[1]
-            side.g_row_stride, side.g_head_stride = g.stride(0), g.stride(1)
-            if x is not None:
-                side.x, side.row_stride, side.head_stride = ptr(x), x.stride(0), x.stride(1)
+            dx, dw = _like(g), torch.empty_like(w) if w is not None else None
+            weight = w if w is not None else weight
+            sides[i] = FmdHeadRotarySide(ptr(x), g.data_ptr(), dx.data_ptr(), ptr(w), ptr(dw),
+                                         x.stride(0) if x is not None else 0, x.stride(1) if x is not None else 0,
+                                         g.stride(0), g.stride(1), g.shape[1])
             grads.append((dx, dw))
             kept.append(g)
         if kept:
-            _launch(sides, kept[0], _weight_type(kept[0], q_weight, k_weight), 2 * cos.shape[1], ctx.interleaved,
-                    ctx.eps, positions, cos, sin, True)
+            _launch(sides, kept[0], weight, cos, sin, positions, ctx.interleaved, ctx.eps, True)
         (dq, dwq), (dk, dwk) = grads
         return dq, dk, None, None, None, dwq, dwk, None, None
 

@@ -15,7 +15,7 @@ from torch.autograd import Function
 
 from . import _lib
 from ._lib import FmdAttention, c_size_t, call, ptr, stream
-from .head_rotary import TYPES, _head_rows
+from .head_rotary import TYPES, _head_rows, _like
 
 
 def _problem(q, k, v, offsets, key_offsets, key_counts, causal, scale) -> FmdAttention:
@@ -25,14 +25,21 @@ def _problem(q, k, v, offsets, key_offsets, key_counts, causal, scale) -> FmdAtt
                         q.shape[2], causal)
 
 
-def _forward(q, k, v, offsets, key_offsets, key_counts, causal, scale, lse):
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    sums = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32) if lse else None
-    problem = _problem(q, k, v, offsets, key_offsets, key_counts, causal, scale)
+def _workspace(problem: FmdAttention, backward: bool, device) -> tuple[Tensor | None, int]:
     nbytes = c_size_t()
-    call("fmd_packed_attention_workspace_bytes", problem, nbytes)
-    workspace = torch.empty(nbytes.value, device=q.device, dtype=torch.uint8) if nbytes.value else None
-    call("fmd_packed_attention", problem, ptr(out), ptr(sums), ptr(workspace), nbytes.value, ptr(_lib.flags_word(q.device)), stream(q.device))
+    call("fmd_packed_attention_workspace_bytes", problem, backward, nbytes)
+    size = nbytes.value
+    return (torch.empty(size, device=device, dtype=torch.uint8) if size else None), size
+
+
+def _forward(q, k, v, offsets, key_offsets, key_counts, causal, scale, lse):
+    device = q.device
+    out = _like(q)
+    sums = torch.empty(q.shape[:2], device=device, dtype=torch.float32) if lse else None
+    problem = _problem(q, k, v, offsets, key_offsets, key_counts, causal, scale)
+    workspace, size = _workspace(problem, False, device)
+    call("fmd_packed_attention", problem, out.data_ptr(), ptr(sums), ptr(workspace), size,
+         _lib.flags_word(device).data_ptr(), stream(device))
     return out, sums
 
 
@@ -52,14 +59,13 @@ class _PackedAttention(Function):
             return (None,) * 8
         g = torch.zeros_like(out) if g is None else _head_rows(g)
         glse = glse.contiguous() if glse is not None else None
-        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if ctx.needs_input_grad[0] else None
-        dk = dv = None
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (k, v))
-        delta = torch.empty_like(lse)
+        dq = _like(q) if ctx.needs_input_grad[0] else None
+        dk, dv = (_like(k), _like(v)) if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else (None, None)
         problem = _problem(q, k, v, offsets, key_offsets, key_counts, ctx.causal, ctx.scale)
-        call("fmd_packed_attention_bwd", problem, ptr(out), ptr(lse), ptr(g), g.stride(0), g.stride(1), ptr(glse),
-             ptr(delta), ptr(dq), ptr(dk), ptr(dv), ptr(_lib.flags_word(q.device)), stream(q.device))
+        workspace, size = _workspace(problem, True, q.device)
+        call("fmd_packed_attention_bwd", problem, out.data_ptr(), lse.data_ptr(), g.data_ptr(), g.stride(0),
+             g.stride(1), ptr(glse), ptr(dq), ptr(dk), ptr(dv), ptr(workspace), size,
+             _lib.flags_word(q.device).data_ptr(), stream(q.device))
         return dq, dk, dv, None, None, None, None, None
 
 

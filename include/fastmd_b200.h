@@ -1087,7 +1087,7 @@ FMD_API fmd_status fmd_head_rotary(const fmd_head_rotary_side* sides, int32_t ty
  * at 0, do not fall and end at rows and keys, and counts fit their slots:
  * else FMD_FLAG_INDEX_RANGE is raised, nothing outside the arrays is touched
  * and the results are unspecified. dim a multiple of 8 up to 128,
- * heads / key_heads at most 64; strides in elements, unit stride inside a
+ * heads / key_heads at most 64, rows and keys at most 2^29; strides in elements, unit stride inside a
  * head; bases and strides multiples of 16 bytes, else FMD_ERR_UNSUPPORTED. */
 typedef struct fmd_attention {
     const void* q;
@@ -1102,8 +1102,11 @@ typedef struct fmd_attention {
     int32_t type, batch, heads, key_heads, dim, causal, _pad;
 } fmd_attention;
 
-/* Workspace of fmd_packed_attention (0: none), from the sizes alone. */
-FMD_API fmd_status fmd_packed_attention_workspace_bytes(const fmd_attention* problem, size_t* bytes);
+/* Workspace of fmd_packed_attention (backward = 0) or of
+ * fmd_packed_attention_bwd (1), 0 for none, from the sizes alone; it starts
+ * at a multiple of 16 bytes. */
+FMD_API fmd_status fmd_packed_attention_workspace_bytes(const fmd_attention* problem, int32_t backward,
+                                                        size_t* bytes);
 
 /* out [rows, heads, dim] = softmax(scale q k^T) v over the keys each row
  * sees, and lse [rows, heads] = the logarithm of the softmax's denominator
@@ -1115,12 +1118,11 @@ FMD_API fmd_status fmd_packed_attention(const fmd_attention* problem, void* out,
 /* Gradients of q (dq, [rows, heads, dim], or NULL) and of k and v (dk, dv,
  * [keys, key_heads, dim], or both NULL; slot rows behind a count get zeros)
  * from the output's gradient g (strides g_row, g_head) and lse's, glse
- * (NULL: none); out and lse are the forward pass's. delta [rows, heads] is
- * workspace. Deterministic. */
+ * (NULL: none); out and lse are the forward pass's. Deterministic. */
 FMD_API fmd_status fmd_packed_attention_bwd(const fmd_attention* problem, const void* out, const float* lse,
                                             const void* g, int64_t g_row, int64_t g_head, const float* glse,
-                                            float* delta, void* dq, void* dk, void* dv, int32_t* flags,
-                                            void* stream);
+                                            void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                            int32_t* flags, void* stream);
 
 #ifdef __cplusplus
 }
