@@ -3,6 +3,11 @@
 //   p = exp(scale q k^T - lse),  dp = g v^T,  ds = p (dp - delta)
 //   dq = scale ds k;   dv = p^T g,  dk = scale ds^T q
 //
+// p is rounded to bfloat16 for its product with g, as for that with v in the forward pass: its roundings average out
+// to about that of the stored result. Those of ds would count for more, because sums over ds cancel (a row's adds up
+// to zero), and took the error of dq and dk to 1.5 times that of rounding the result alone; so ds is kept in two planes,
+// ds = h + m of 16 significant bits, at the price of one more product each.
+//
 // Two kernels, each of which owns the rows it writes and adds in one order, so that the gradients are the same bits on
 // every run without atomics or partial sums in memory; the price is that scores and dp are computed twice (seven
 // products for five). Both keep one side's tiles in shared memory and stream the other's:
@@ -111,6 +116,28 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* out, uint32_t tmem, int
     }
 }
 
+// The two planes of ds over the columns of dP that the thread has read: of each 32, 16 and 16.
+template <int N>
+__device__ __forceinline__ void store_planes(uint32_t at, float (&ds)[N], int chunks) {
+#pragma unroll
+    for (int ch = 0; ch < N / 32; ++ch) {
+        if (ch < chunks) {
+            uint32_t w[16];
+            next_plane<16>(ds + 32 * ch, w);
+            tmem_store16(at + ch * 32, w);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = pack_bf16(ds[32 * ch + 2 * i], ds[32 * ch + 2 * i + 1]);
+            tmem_store16(at + ch * 32 + 16, w);
+        }
+    }
+}
+
+// D (+)= ds B with ds in two planes, 16 columns each of every 32 that they replace: the lower one first.
+__device__ __forceinline__ void product_planes(uint32_t d, uint32_t ds, uint32_t b, int steps, uint32_t idesc, bool add) {
+    product_weights<8, 2, 32>(d, ds + 16, b, steps, idesc, add);
+    product_weights<8, 2, 32>(d, ds, b, steps, idesc, true);
+}
+
 // ---------------------------------------------------------------- queries
 
 template <int KS>
@@ -188,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = ok && mbar_wait(&ctl.ds, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                product_weights<4, 64>(tmem + kDq, tmem + kDp, slot(2 * j), width(j) / 16, out_desc, j > 0);
+                product_planes(tmem + kDq, tmem + kDp, slot(2 * j), width(j) / 16, out_desc, j > 0);
                 tc_commit(&ctl.ring.empty[(2 * j) % S::kSlots]);
                 if (j + 1 < tiles) dp(j + 1);
             }
@@ -231,17 +258,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc_fence_after();
             const uint32_t at_s = tmem + lanes + uint32_t(j & 1) * 128u + uint32_t(half) * 64u;
+            if (chunks > 0) {
+                tmem_load64(at_s, p);
 #pragma unroll
-            for (int ch = 0; ch < 2; ++ch) {
-                if (ch < chunks) {
-                    float x[32];
-                    tmem_load32(at_s + ch * 32, x);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 y = fma2(make_float2(x[i], x[i + 1]), c2, base2);
-                        p[ch * 32 + i] = ex2(y.x);
-                        p[ch * 32 + i + 1] = ex2(y.y);
-                    }
+                for (int i = 0; i < 64; i += 2) {
+                    const float2 y = fma2(make_float2(p[i], p[i + 1]), c2, base2);
+                    p[i] = ex2(y.x);
+                    p[i + 1] = ex2(y.y);
                 }
             }
             got = mbar_wait(&ctl.dp, uint32_t(j) & 1u, abort);
@@ -252,24 +275,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc_fence_after();
             const uint32_t at_d = tmem + lanes + kDp + uint32_t(half) * 64u;
+            if (chunks > 0) {
+                float x[64];
+                tmem_load64(at_d, x);
 #pragma unroll
-            for (int ch = 0; ch < 2; ++ch) {
-                if (ch < chunks) {
-                    float x[32];
-                    uint32_t w[16];
-                    tmem_load32(at_d + ch * 32, x);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        float2 y = add2(make_float2(x[i], x[i + 1]), delta2);
-                        y = mul2(y, make_float2(p[ch * 32 + i], p[ch * 32 + i + 1]));
-                        if (masked) {  // what a row does not see has no share, whatever its values
-                            y.x = ch * 32 + i < mine ? y.x : 0.0f;
-                            y.y = ch * 32 + i + 1 < mine ? y.y : 0.0f;
-                        }
-                        w[i / 2] = pack_bf16(y.x, y.y);
+                for (int i = 0; i < 64; i += 2) {
+                    float2 y = add2(make_float2(x[i], x[i + 1]), delta2);
+                    y = mul2(y, make_float2(p[i], p[i + 1]));
+                    if (masked) {  // what a row does not see has no share, whatever its values
+                        y.x = i < mine ? y.x : 0.0f;
+                        y.y = i + 1 < mine ? y.y : 0.0f;
                     }
-                    tmem_store16(at_d + ch * 16, w);
+                    x[i] = y.x;
+                    x[i + 1] = y.y;
                 }
+                store_planes(at_d, x, chunks);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -372,13 +392,13 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
                 ok = ok && mbar_wait(&ctl.p, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                product_weights<4, 64>(tmem + kDv, tmem, slot(2 * j + 1), steps, out_desc, j > 0);
+                product_weights<8, 4, 64>(tmem + kDv, tmem, slot(2 * j + 1), steps, out_desc, j > 0);
                 tc_commit(&ctl.ring.empty[(2 * j + 1) % S::kSlots]);
                 if (j + 1 < tiles) scores(j + 1);
                 ok = ok && mbar_wait(&ctl.ds, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                product_weights<4, 64>(tmem + kDk, tmem + kDp, slot(2 * j), steps, out_desc, j > 0);
+                product_planes(tmem + kDk, tmem + kDp, slot(2 * j), steps, out_desc, j > 0);
                 tc_commit(&ctl.ring.empty[(2 * j) % S::kSlots]);
                 if (j + 1 < tiles) dp(j + 1);
             }
@@ -487,7 +507,6 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
             for (int ch = 0; ch < 2; ++ch) {
                 if (ch < chunks) {
                     float x[32];
-                    uint32_t w[16];
                     tmem_load32(at_d + ch * 32, x);
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
@@ -499,9 +518,10 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
                             y.x = r < m.x ? y.x : 0.0f;
                             y.y = r < m.y ? y.y : 0.0f;
                         }
-                        w[i / 2] = pack_bf16(y.x, y.y);
+                        x[i] = y.x;
+                        x[i + 1] = y.y;
                     }
-                    tmem_store16(at_d + ch * 16, w);
+                    store_planes(at_d + ch * 32, x, 1);
                 }
             }
             tmem_wait_st();

@@ -30,19 +30,6 @@ struct Maps {
     CUtensorMap q, g, k, v;
 };
 
-// The next plane of 2 N values, two neighbours in a word; the values become what is left (exactly).
-template <int N>
-__device__ __forceinline__ void next_plane(float* y, uint32_t (&w)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        w[i] = pack_bf16(y[2 * i], y[2 * i + 1]);
-        const float2 part = unpack_bf16(w[i]);
-        const float2 left = add2(make_float2(y[2 * i], y[2 * i + 1]), make_float2(-part.x, -part.y));
-        y[2 * i] = left.x;
-        y[2 * i + 1] = left.y;
-    }
-}
-
 // N columns of TMEM (16 or 32) added to a sum in registers, which is then scaled.
 template <int N>
 __device__ __forceinline__ void drain(uint32_t addr, float (&sum)[N], float keep) {
@@ -111,7 +98,7 @@ struct ForwardCtrl {
 template <int KS, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_constant__ Maps maps, const Attn a) {
     constexpr int kDim = 16 * KS, kMine = kDim / 2;  // output columns, and those of one half
-    constexpr uint32_t kL = 256, kO = 320;           // TMEM columns: two score buffers, p's lowest plane, the output
+    constexpr uint32_t kL = 256, kO = 384;           // TMEM columns, two buffers each: scores, p's lowest plane, output
     extern __shared__ unsigned char raw[];
     unsigned char* own = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     unsigned char* ring = own + kTile3;
@@ -211,8 +198,9 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
 #pragma unroll
                 for (int i = 0; i < 6; ++i) {
                     const uint32_t at = v + kPlaneB[i] * kPanelBytes;
-                    if (kPlaneA[i] == 2) product_weights<4, 32>(tmem + kO, tmem + kL, at, steps, o_desc, i > 0);
-                    else product_weights<4, 64>(tmem + kO, p + 32u * kPlaneA[i], at, steps, o_desc, i > 0);
+                    const uint32_t o = tmem + kO + uint32_t(j & 1) * 64u, low = tmem + kL + uint32_t(j & 1) * 64u;
+                    if (kPlaneA[i] == 2) product_weights<8, 4, 32>(o, low, at, steps, o_desc, i > 0);
+                    else product_weights<8, 4, 64>(o, p + 32u * kPlaneA[i], at, steps, o_desc, i > 0);
                 }
                 tc_commit(&ctl.out);
                 tc_commit(&ctl.ring.empty[(2 * j + 1) % kSlots]);
@@ -251,22 +239,11 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
             if (!all(mbar_wait(&ctl.scores[j & 1], uint32_t(j >> 1) & 1u, abort))) break;
             const uint32_t at_s = tmem + lanes + uint32_t(j & 1) * 128u + uint32_t(half) * 64u;
             const int columns = end - j * kTile - 64 * half, mine = limit - j * kTile - 64 * half;
-            float x[2][32];
-            float top = -INFINITY;
+            float x[64];
+            tmem_load64(at_s, x);  // columns behind the products' width hold anything: no row sees them
 #pragma unroll
-            for (int ch = 0; ch < 2; ++ch) {
-                if (32 * ch < columns) {
-                    tmem_load32(at_s + ch * 32, x[ch]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) x[ch][i] = -INFINITY;
-                }
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    x[ch][i] = ch * 32 + i < mine ? x[ch][i] : -INFINITY;
-                    top = fmaxf(top, x[ch][i]);
-                }
-            }
+            for (int i = 0; i < 64; ++i) x[i] = i < mine ? x[i] : -INFINITY;
+            float top = largest(x);
             // the row's maximum over both halves
             maxima[j & 1][half][r] = top;
             mbar_arrive(&ctl.swap);
@@ -276,45 +253,42 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
             const float keep = ex2(m - base);
             m = top;
             const float2 c2 = make_float2(c, c), base2 = make_float2(-base, -base);
-            float2 sum = make_float2(0.0f, 0.0f);
+            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-            for (int ch = 0; ch < 2; ++ch) {
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float2 y = fma2(make_float2(x[ch][i], x[ch][i + 1]), c2, base2);
-                    x[ch][i] = ex2(y.x);
-                    x[ch][i + 1] = ex2(y.y);
-                    sum = add2(sum, make_float2(x[ch][i], x[ch][i + 1]));
-                }
+            for (int i = 0; i < 64; i += 2) {
+                const float2 y = fma2(make_float2(x[i], x[i + 1]), c2, base2);
+                x[i] = ex2(y.x);
+                x[i + 1] = ex2(y.y);
+                sum[(i / 2) & 1] = add2(sum[(i / 2) & 1], make_float2(x[i], x[i + 1]));
             }
-            l = l * keep + (sum.x + sum.y);
-            if (j > 0) {  // the last tile's output, against the old maximum; then p may overwrite its weights
-                if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
-                drain<kMine>(at_o, o, keep);
-            }
-            const uint32_t at_l = tmem + lanes + kL + uint32_t(half) * 32u;
+            l = l * keep + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+            const uint32_t at_l = tmem + lanes + kL + uint32_t(j & 1) * 64u + uint32_t(half) * 32u;
 #pragma unroll
             for (int ch = 0; ch < 2; ++ch) {
                 if (32 * ch < columns) {
                     uint32_t w[16];
-                    next_plane<16>(x[ch], w);
+                    next_plane<16>(x + 32 * ch, w);
                     tmem_store16(at_s + ch * 16, w);
-                    next_plane<16>(x[ch], w);
+                    next_plane<16>(x + 32 * ch, w);
                     tmem_store16(at_s + 32 + ch * 16, w);
-                    next_plane<16>(x[ch], w);
+                    next_plane<16>(x + 32 * ch, w);
                     tmem_store16(at_l + ch * 16, w);
                 }
             }
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&ctl.weights);
+            if (j > 0) {  // the last tile's output, against the old maximum, while this one's products run
+                if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
+                drain<kMine>(at_o + uint32_t((j - 1) & 1) * 64u, o, keep);
+            }
         }
         if (ok && tiles > 0) {
             sums[half][r] = l;
             mbar_arrive(&ctl.swap);
             if (all(mbar_wait(&ctl.out, uint32_t(tiles - 1) & 1u, abort) &&
                     mbar_wait(&ctl.swap, uint32_t(tiles) & 1u, abort))) {
-                drain<kMine>(at_o, o, 1.0f);
+                drain<kMine>(at_o + uint32_t((tiles - 1) & 1) * 64u, o, 1.0f);
                 l = sums[0][r] + sums[1][r];
             }
         }
@@ -400,8 +374,8 @@ __device__ __forceinline__ void weigh6(uint32_t d, uint32_t w, uint32_t low, uin
 #pragma unroll
     for (int i = 0; i < 6; ++i) {
         const uint32_t at = b + kPlaneB[i] * kHalfPanel;
-        if (kPlaneA[i] == 2) product_weights<2, 16>(d, low, at, steps, idesc, i > 0);
-        else product_weights<2, 32>(d, w + 16u * kPlaneA[i], at, steps, idesc, i > 0);
+        if (kPlaneA[i] == 2) product_weights<4, 2, 16>(d, low, at, steps, idesc, i > 0);
+        else product_weights<4, 2, 32>(d, w + 16u * kPlaneA[i], at, steps, idesc, i > 0);
     }
 }
 
@@ -420,7 +394,7 @@ template <int KS>
 __global__ void __launch_bounds__(kThreads, 1)
     query_gradient_kernel(const __grid_constant__ Maps maps, const Attn a) {
     constexpr int kDim = 16 * KS, kMine = kDim / 2;
-    constexpr uint32_t kDp = 128, kL = 256, kDq = 320;  // TMEM columns: two score buffers, two of dP, ds's l, dq
+    constexpr uint32_t kDp = 128, kL = 256, kDq = 320;  // TMEM columns, two buffers each: scores, dP, ds's l, dq
     extern __shared__ unsigned char raw[];
     unsigned char* own = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     unsigned char* ring = own + 2 * kTile3;
@@ -485,8 +459,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = ok && mbar_wait(&ctl.weights, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                weigh6(tmem + kDq, tmem + kDp + uint32_t(j & 1) * kStream, tmem + kL, slot(2 * j), width(j) / 16,
-                       out_desc);
+                weigh6(tmem + kDq + uint32_t(j & 1) * 64u, tmem + kDp + uint32_t(j & 1) * kStream,
+                       tmem + kL + uint32_t(j & 1) * 32u, slot(2 * j), width(j) / 16, out_desc);
                 tc_commit(&ctl.out);
                 tc_commit(&ctl.ring.empty[(2 * j) % kStreamSlots]);
             }
@@ -549,16 +523,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     x[i + 1] = i + 1 < mine ? y.y : 0.0f;
                 }
             }
-            if (j > 0) {
-                if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
-                drain<kMine>(at_q, dq, 1.0f);
-            }
-            if (any) store_planes(at + kDp, tmem + lanes + kL + uint32_t(half) * 16u, x);
+            if (any) store_planes(at + kDp, tmem + lanes + kL + uint32_t(j & 1) * 32u + uint32_t(half) * 16u, x);
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&ctl.weights);
+            if (j > 0) {  // the last tile's product, while this one's runs
+                if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
+                drain<kMine>(at_q + uint32_t((j - 1) & 1) * 64u, dq, 1.0f);
+            }
         }
-        if (ok && tiles > 0 && all(mbar_wait(&ctl.out, uint32_t(tiles - 1) & 1u, abort))) drain<kMine>(at_q, dq, 1.0f);
+        if (ok && tiles > 0 && all(mbar_wait(&ctl.out, uint32_t(tiles - 1) & 1u, abort)))
+            drain<kMine>(at_q + uint32_t((tiles - 1) & 1) * 64u, dq, 1.0f);
         if (ok && real) store_values<kMine>(static_cast<float*>(a.dq) + flat * a.dim, dq, a.scale, half * kMine, a.dim);
     }
     close_block(ctl, warp, a.flags);
@@ -567,7 +542,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int KS>
 __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_constant__ Maps maps, const Attn a) {
     constexpr int kDim = 16 * KS;
-    constexpr uint32_t kDp = 128, kPl = 256, kDl = 288, kDv = 320, kDk = 384;  // TMEM columns
+    // TMEM columns: two buffers each of scores, dP and the lowest planes of p and ds; dv, dk
+    constexpr uint32_t kDp = 128, kPl = 256, kDl = 320, kDv = 384, kDk = 448;
     extern __shared__ unsigned char raw[];
     unsigned char* own = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     unsigned char* ring = own + 2 * kTile3;
@@ -638,8 +614,9 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t at = tmem + uint32_t(j & 1) * kStream;
-                weigh6(tmem + kDv, at, tmem + kPl, slot(2 * j + 1), width(j) / 16, out_desc);
-                weigh6(tmem + kDk, at + kDp, tmem + kDl, slot(2 * j), width(j) / 16, out_desc);
+                const uint32_t low = uint32_t(j & 1) * 32u;
+                weigh6(tmem + kDv, at, tmem + kPl + low, slot(2 * j + 1), width(j) / 16, out_desc);
+                weigh6(tmem + kDk, at + kDp, tmem + kDl + low, slot(2 * j), width(j) / 16, out_desc);
                 tc_commit(&ctl.out);
                 tc_commit(&ctl.ring.empty[(2 * j) % kStreamSlots]);
                 tc_commit(&ctl.ring.empty[(2 * j + 1) % kStreamSlots]);
@@ -732,13 +709,15 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&ctl.read[j & 1]);
-            // the last products have read their weights and may be added before the next ones start
-            if (j > 0 && !all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
             if (any) {
-                store_planes(at, tmem + lanes + kPl + uint32_t(half) * 16u, p);
-                store_planes(at + kDp, tmem + lanes + kDl + uint32_t(half) * 16u, x);
+                const uint32_t low = lanes + uint32_t(j & 1) * 32u + uint32_t(half) * 16u;
+                store_planes(at, tmem + kPl + low, p);
+                store_planes(at + kDp, tmem + kDl + low, x);
             }
-            if (j > 0) drain_all();
+            if (j > 0) {  // the last products are added before the next ones start over
+                if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
+                drain_all();
+            }
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&ctl.weights);

@@ -11,6 +11,7 @@
 //   warp 0       TMA: q once, then k and v tiles through a ring of shared-memory slots
 //   warp 1       one thread issues the products: S_t = q k^T (both from shared memory, into TMEM), O_t += p v (p from
 //                TMEM); for two tiles in turn, so the tensor cores work on one tile while the other is exponentiated
+//                (a thread for each tile let their products mix and cost 15 %)
 //   warps 2, 3   zero the rows behind the last key (another sequence's or an unused slot's: 0 * NaN must not happen)
 //   then 4 warps per tile: thread = row. Scores from TMEM, maximum, exp2, sum, p back over the scores as bfloat16;
 //                o rescaled in TMEM when m moves; at the end o / l to memory.
@@ -54,6 +55,16 @@ struct Ctrl {
 struct Maps {
     CUtensorMap q, k, v;
 };
+
+__device__ __forceinline__ void load_scores(uint32_t addr, float (&x)[64]) { tmem_load64(addr, x); }
+__device__ __forceinline__ void load_scores(uint32_t addr, float (&x)[128]) { tmem_load128(addr, x); }
+
+// What a row does not see is as if it were not there.
+template <int N>
+__device__ __forceinline__ void hide(float (&x)[N], int mine) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = i < mine ? x[i] : -INFINITY;
+}
 
 template <int KS, int NT, bool SPLIT>
 __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
@@ -187,7 +198,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
                         ok = ok && mbar_wait(&ctl.weights[t], uint32_t(j) & 1u, abort);
                         if (!ok) break;
                         tc_fence_after();
-                        product_weights<4, 32>(tmem + S::kO + uint32_t(t) * S::kDim, tmem + t * 128u,
+                        product_weights<8, 4, 32>(tmem + S::kO + uint32_t(t) * S::kDim, tmem + t * 128u,
                                         su32(ring + v_slot * S::kTileBytes), width(t, j) / 16, o_desc, j > 0);
                     }
                     if (t == NT - 1) tc_commit(&ctl.ring.empty[v_slot]);
@@ -214,8 +225,9 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
                 mbar_arrive(&ctl.tail);
             }
         }
-    } else {
+    } else if (warp >= 4) {
         // ---------------------------------------------------------- softmax: thread = row
+        constexpr int kLoad = NT == 2 ? 128 : 64;
         const int t = (warp - 4) >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         const uint32_t at_s = tmem + lanes + t * 128u, at_o = tmem + lanes + S::kO + uint32_t(t) * S::kDim;
@@ -239,20 +251,18 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
                 mbar_arrive(&ctl.weights[t]);
                 continue;
             }
-            const int chunks = min(4, (ends[t] - j * kTile + 31) / 32);
-            const int mine = limit - j * kTile;  // columns of this tile that the row sees
-            const bool masked = __any_sync(0xffffffffu, mine < chunks * 32);
-            float x[32];
+            const int seen_here = min(kTile, ends[t] - j * kTile);  // columns that some row sees
+            const int mine = limit - j * kTile;                     // that this row sees
+            const bool masked = __any_sync(0xffffffffu, mine < kTile);
+            // the scores stay in registers where a thread may have them all; two blocks an SM read them twice, by halves
+            float x[kLoad];
             float top = -INFINITY;
-            for (int ch = 0; ch < chunks; ++ch) {
-                tmem_load32(at_s + ch * 32, x);
-                if (masked) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) top = fmaxf(top, ch * 32 + i < mine ? x[i] : -INFINITY);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) top = fmaxf(top, x[i]);
-                }
+            for (int part = 0; part < kTile / kLoad; ++part) {
+                if (part * kLoad >= seen_here) break;
+                load_scores(at_s + part * kLoad, x);
+                if (masked) hide(x, mine - part * kLoad);
+                top = fmaxf(top, largest(x));
             }
             top *= c;
             const bool move = top > m + kSlack;  // the first finite maximum always moves: m starts at -inf
@@ -261,37 +271,42 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
                 if (move) m = top;
                 l *= keep;
                 if (j > 0) {
+#pragma unroll 1
+                    for (int ch = 0; ch < S::kDim / 16; ++ch) {
+                        float o[16];
+                        tmem_load16(at_o + ch * 16, o);
 #pragma unroll
-                    for (int ch = 0; ch < S::kDim / 32; ++ch) {
-                        float o[32];
-                        tmem_load32(at_o + ch * 32, o);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] *= keep;
-                        tmem_store32(at_o + ch * 32, o);
+                        for (int i = 0; i < 16; ++i) o[i] *= keep;
+                        tmem_store16(at_o + ch * 16, reinterpret_cast<const uint32_t(&)[16]>(o));
                     }
                 }
             }
             const float base = m == -INFINITY ? 0.0f : m;
             const float2 c2 = make_float2(c, c), base2 = make_float2(-base, -base);
-            float2 sum = make_float2(0.0f, 0.0f);
-            for (int ch = 0; ch < chunks; ++ch) {
-                tmem_load32(at_s + ch * 32, x);
-                if (masked) {
+            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] = ch * 32 + i < mine ? x[i] : -INFINITY;
+            for (int part = 0; part < kTile / kLoad; ++part) {
+                if (part * kLoad >= seen_here) break;
+                if (kLoad < kTile) {
+                    load_scores(at_s + part * kLoad, x);
+                    if (masked) hide(x, mine - part * kLoad);
                 }
-                uint32_t p[16];
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    float2 y = fma2(make_float2(x[i], x[i + 1]), c2, base2);
-                    y.x = ex2(y.x);
-                    y.y = ex2(y.y);
-                    sum = add2(sum, y);
-                    p[i / 2] = pack_bf16(y.x, y.y);
+                for (int ch = 0; ch < kLoad; ch += 32) {
+                    if (part * kLoad + ch >= seen_here) break;
+                    uint32_t p[16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        float2 y = fma2(make_float2(x[ch + i], x[ch + i + 1]), c2, base2);
+                        y.x = ex2(y.x);
+                        y.y = ex2(y.y);
+                        sum[(i / 2) & 1] = add2(sum[(i / 2) & 1], y);
+                        p[i / 2] = pack_bf16(y.x, y.y);
+                    }
+                    tmem_store16(at_s + (part * kLoad + ch) / 2, p);
                 }
-                tmem_store16(at_s + ch * 16, p);
             }
-            l += sum.x + sum.y;
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&ctl.weights[t]);

@@ -75,19 +75,19 @@ __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b,
     }
 }
 
-// D [128, n] (+)= P B over `steps` (at most 2 HALF) steps of 16 rows of B, P [128, 16 steps] bfloat16 in TMEM: the
-// first HALF steps at p, the others at p + kSecond.
-template <int HALF, uint32_t kSecond>
+// D [128, n] (+)= P B over `steps` (at most STEPS) steps of 16 rows of B, P [128, 16 steps] bfloat16 in TMEM: groups of
+// GROUP steps, kNext columns apart.
+template <int STEPS, int GROUP, uint32_t kNext>
 __device__ __forceinline__ void product_weights(uint32_t d, uint32_t p, uint32_t b, int steps, uint32_t idesc,
                                                 bool add) {
     const uint32_t bd = columns_desc(b);
-    if (steps == 2 * HALF) {
+    if (steps == STEPS) {
 #pragma unroll
-        for (int k = 0; k < 2 * HALF; ++k)
-            mma_weights(d, p + 8 * (k % HALF) + (k / HALF) * kSecond, bd + k * 128, idesc, add || k > 0);
+        for (int k = 0; k < STEPS; ++k)
+            mma_weights(d, p + 8 * (k % GROUP) + (k / GROUP) * kNext, bd + k * 128, idesc, add || k > 0);
     } else {
         for (int k = 0; k < steps; ++k)
-            mma_weights(d, p + 8 * (k % HALF) + (k / HALF) * kSecond, bd + k * 128, idesc, add || k > 0);
+            mma_weights(d, p + 8 * (k % GROUP) + (k / GROUP) * kNext, bd + k * 128, idesc, add || k > 0);
     }
 }
 
@@ -106,6 +106,66 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
                    "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
                  : "r"(addr)
                  : "memory");
+}
+
+#define FMD_TMEM_R64 \
+    "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, " \
+    "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, " \
+    "%42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, " \
+    "%62, %63}"
+
+// 64 columns, in the same way
+__device__ __forceinline__ void tmem_load64(uint32_t addr, float (&v)[64]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 " FMD_TMEM_R64 ", [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+          "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+          "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]),
+          "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+          "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]), "=f"(v[32]), "=f"(v[33]), "=f"(v[34]),
+          "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]), "=f"(v[40]), "=f"(v[41]),
+          "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]), "=f"(v[48]),
+          "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
+          "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]),
+          "=f"(v[63])
+        : "r"(addr)
+        : "memory");
+}
+
+#define FMD_TMEM_R128 \
+    "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, " \
+    "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, " \
+    "%42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, " \
+    "%62, %63, %64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, %80, %81, " \
+    "%82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, %96, %97, %98, %99, %100, " \
+    "%101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, " \
+    "%117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}"
+
+// 128 columns, in the same way
+__device__ __forceinline__ void tmem_load128(uint32_t addr, float (&v)[128]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x128.b32 " FMD_TMEM_R128 ", [%128];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+          "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+          "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]),
+          "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+          "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]), "=f"(v[32]), "=f"(v[33]), "=f"(v[34]),
+          "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]), "=f"(v[40]), "=f"(v[41]),
+          "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]), "=f"(v[48]),
+          "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
+          "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]),
+          "=f"(v[63]), "=f"(v[64]), "=f"(v[65]), "=f"(v[66]), "=f"(v[67]), "=f"(v[68]), "=f"(v[69]),
+          "=f"(v[70]), "=f"(v[71]), "=f"(v[72]), "=f"(v[73]), "=f"(v[74]), "=f"(v[75]), "=f"(v[76]),
+          "=f"(v[77]), "=f"(v[78]), "=f"(v[79]), "=f"(v[80]), "=f"(v[81]), "=f"(v[82]), "=f"(v[83]),
+          "=f"(v[84]), "=f"(v[85]), "=f"(v[86]), "=f"(v[87]), "=f"(v[88]), "=f"(v[89]), "=f"(v[90]),
+          "=f"(v[91]), "=f"(v[92]), "=f"(v[93]), "=f"(v[94]), "=f"(v[95]), "=f"(v[96]), "=f"(v[97]),
+          "=f"(v[98]), "=f"(v[99]), "=f"(v[100]), "=f"(v[101]), "=f"(v[102]), "=f"(v[103]),
+          "=f"(v[104]), "=f"(v[105]), "=f"(v[106]), "=f"(v[107]), "=f"(v[108]), "=f"(v[109]),
+          "=f"(v[110]), "=f"(v[111]), "=f"(v[112]), "=f"(v[113]), "=f"(v[114]), "=f"(v[115]),
+          "=f"(v[116]), "=f"(v[117]), "=f"(v[118]), "=f"(v[119]), "=f"(v[120]), "=f"(v[121]),
+          "=f"(v[122]), "=f"(v[123]), "=f"(v[124]), "=f"(v[125]), "=f"(v[126]), "=f"(v[127])
+        : "r"(addr)
+        : "memory");
 }
 
 // 16 columns, in the same way
@@ -175,6 +235,15 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     return d;
 }
 
+// The largest of N values: four chains, not one of N dependent steps.
+template <int N>
+__device__ __forceinline__ float largest(const float (&x)[N]) {
+    float t[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+    for (int i = 4; i < N; ++i) t[i & 3] = fmaxf(t[i & 3], x[i]);
+    return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+}
+
 __device__ __forceinline__ float2 unpack_bf16(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
@@ -183,6 +252,19 @@ __device__ __forceinline__ uint32_t pack_bf16(float low, float high) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
     return r;
+}
+
+// The next plane of 2 N values, two neighbours in a word; the values become what is left (exactly).
+template <int N>
+__device__ __forceinline__ void next_plane(float* y, uint32_t (&w)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        w[i] = pack_bf16(y[2 * i], y[2 * i + 1]);
+        const float2 part = unpack_bf16(w[i]);
+        const float2 left = add2(make_float2(y[2 * i], y[2 * i + 1]), make_float2(-part.x, -part.y));
+        y[2 * i] = left.x;
+        y[2 * i + 1] = left.y;
+    }
 }
 
 // Zeros rows [first, last) of `panels` panels that lie `stride` bytes apart (the swizzle keeps a row's 128 bytes in
