@@ -182,47 +182,58 @@ __global__ void __launch_bounds__(kThreads, 1)
             });
         }
     } else if (warp == 1) {
-        if (lane == 0 && tiles > 0) {
-            const uint32_t q_tile = su32(own), g_tile = su32(own + S::kTileBytes);
+        if (tiles > 0) {
+            const uint32_t base = uniform(tmem), own_at = uniform(su32(own)), first_slot = uniform(su32(ring));
             const uint32_t out_desc = bf16_idesc(S::kDim, true);
-            auto slot = [&](int i) { return su32(ring + (i % S::kSlots) * S::kTileBytes); };
-            auto width = [&](int j) { return min(kTile, (end - j * kTile + 15) & ~15); };
-            bool ok = mbar_wait(&ctl.own, 0, abort), issued = false;
+            const int count = uniform(tiles), last_key = uniform(end);
+            const bool zeroed = uniform(int(tail));
+            auto slot = [&](int i) { return first_slot + uint32_t(i % S::kSlots) * S::kTileBytes; };
+            auto width = [&](int j) { return min(kTile, (last_key - j * kTile + 15) & ~15); };
+            bool ok = warp_wait(&ctl.own, 0, abort), issued = false;
             auto scores = [&](int j) {  // into buffer j % 2
                 ok = ok && landed(ctl.ring, 2 * j, abort);
                 if (!ok) return;
                 tc_fence_after();
-                product_rows<KS>(tmem + uint32_t(j & 1) * 128u, q_tile, slot(2 * j), bf16_idesc(width(j), false));
-                tc_commit(&ctl.scores[j & 1]);
+                const uint32_t desc = bf16_idesc(width(j), false);
+                if (elect_one()) {
+                    product_rows<KS>(base + uint32_t(j & 1) * 128u, own_at, slot(2 * j), desc);
+                    tc_commit(&ctl.scores[j & 1]);
+                }
                 issued = true;
             };
             auto dp = [&](int j) {
                 ok = ok && landed(ctl.ring, 2 * j + 1, abort);
                 if (!ok) return;
                 tc_fence_after();
-                product_rows<KS>(tmem + kDp, g_tile, slot(2 * j + 1), bf16_idesc(width(j), false));
-                tc_commit(&ctl.dp);
-                tc_commit(&ctl.ring.empty[(2 * j + 1) % S::kSlots]);
+                const uint32_t desc = bf16_idesc(width(j), false);
+                if (elect_one()) {
+                    product_rows<KS>(base + kDp, own_at + S::kTileBytes, slot(2 * j + 1), desc);
+                    tc_commit(&ctl.dp);
+                    tc_commit(&ctl.ring.empty[(2 * j + 1) % S::kSlots]);
+                }
             };
             scores(0);
             dp(0);
-            for (int j = 0; j < tiles && ok; ++j) {
-                if (j + 1 < tiles) scores(j + 1);
-                if (ok && tail && j == tiles - 1) {
-                    mbar_arrive(&ctl.tail_here);
-                    ok = mbar_wait(&ctl.tail, 0, abort);
+            for (int j = 0; j < count && ok; ++j) {
+                if (j + 1 < count) scores(j + 1);
+                if (ok && zeroed && j == count - 1) {
+                    if (elect_one()) mbar_arrive(&ctl.tail_here);
+                    ok = warp_wait(&ctl.tail, 0, abort);
                 }
-                ok = ok && mbar_wait(&ctl.ds, uint32_t(j) & 1u, abort);
+                ok = ok && warp_wait(&ctl.ds, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                product_planes(tmem + kDq, tmem + kDp, slot(2 * j), width(j) / 16, out_desc, j > 0);
-                tc_commit(&ctl.ring.empty[(2 * j) % S::kSlots]);
-                if (j + 1 < tiles) dp(j + 1);
+                const int steps = width(j) / 16;
+                if (elect_one()) {
+                    product_planes(base + kDq, base + kDp, slot(2 * j), steps, out_desc, j > 0);
+                    if (j + 1 == count) tc_commit(&ctl.done);
+                    tc_commit(&ctl.ring.empty[(2 * j) % S::kSlots]);
+                }
+                if (j + 1 < count) dp(j + 1);
             }
-            if (ok) tc_commit(&ctl.done);
             if (!ok && issued) {
-                tc_commit(&ctl.drain);
-                mbar_wait(&ctl.drain, 0, abort, true);
+                if (elect_one()) tc_commit(&ctl.drain);
+                warp_wait(&ctl.drain, 0, abort, true);
             }
         }
     } else if (warp < 4) {
@@ -360,52 +371,64 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
                  });
         }
     } else if (warp == 1) {
-        if (lane == 0 && tiles > 0) {
-            const uint32_t k_tile = su32(own), v_tile = su32(own + S::kTileBytes);
+        if (tiles > 0) {
+            const uint32_t base = uniform(tmem), own_at = uniform(su32(own)), first_slot = uniform(su32(ring));
             const uint32_t out_desc = bf16_idesc(S::kDim, true);
-            auto slot = [&](int i) { return su32(ring + (i % S::kSlots) * S::kTileBytes); };
-            auto width = [&](int j) { return ((j == tiles - 1 ? last_rows : full_rows) + 15) & ~15; };
-            bool ok = mbar_wait(&ctl.own, 0, abort), issued = false;
+            const int count = uniform(tiles), rows_last = uniform(last_rows), rows_full = uniform(full_rows);
+            const bool zeroed = uniform(int(tail));
+            auto slot = [&](int i) { return first_slot + uint32_t(i % S::kSlots) * S::kTileBytes; };
+            auto width = [&](int j) { return ((j == count - 1 ? rows_last : rows_full) + 15) & ~15; };
+            bool ok = warp_wait(&ctl.own, 0, abort), issued = false;
             auto scores = [&](int j) {
                 ok = ok && landed(ctl.ring, 2 * j, abort);
                 if (!ok) return;
                 tc_fence_after();
-                product_rows<KS>(tmem, k_tile, slot(2 * j), bf16_idesc(width(j), false));
-                tc_commit(&ctl.scores[0]);
+                const uint32_t desc = bf16_idesc(width(j), false);
+                if (elect_one()) {
+                    product_rows<KS>(base, own_at, slot(2 * j), desc);
+                    tc_commit(&ctl.scores[0]);
+                }
                 issued = true;
             };
             auto dp = [&](int j) {
                 ok = ok && landed(ctl.ring, 2 * j + 1, abort);
                 if (!ok) return;
                 tc_fence_after();
-                product_rows<KS>(tmem + kDp, v_tile, slot(2 * j + 1), bf16_idesc(width(j), false));
-                tc_commit(&ctl.dp);
+                const uint32_t desc = bf16_idesc(width(j), false);
+                if (elect_one()) {
+                    product_rows<KS>(base + kDp, own_at + S::kTileBytes, slot(2 * j + 1), desc);
+                    tc_commit(&ctl.dp);
+                }
             };
             scores(0);
             dp(0);
-            for (int j = 0; j < tiles && ok; ++j) {
+            for (int j = 0; j < count && ok; ++j) {
                 const int steps = width(j) / 16;
-                if (tail && j == tiles - 1) {
-                    mbar_arrive(&ctl.tail_here);
-                    ok = mbar_wait(&ctl.tail, 0, abort);
+                if (zeroed && j == count - 1) {
+                    if (elect_one()) mbar_arrive(&ctl.tail_here);
+                    ok = warp_wait(&ctl.tail, 0, abort);
                 }
-                ok = ok && mbar_wait(&ctl.p, uint32_t(j) & 1u, abort);
+                ok = ok && warp_wait(&ctl.p, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                product_weights<8, 4, 64>(tmem + kDv, tmem, slot(2 * j + 1), steps, out_desc, j > 0);
-                tc_commit(&ctl.ring.empty[(2 * j + 1) % S::kSlots]);
-                if (j + 1 < tiles) scores(j + 1);
-                ok = ok && mbar_wait(&ctl.ds, uint32_t(j) & 1u, abort);
+                if (elect_one()) {
+                    product_weights<8, 4, 64>(base + kDv, base, slot(2 * j + 1), steps, out_desc, j > 0);
+                    tc_commit(&ctl.ring.empty[(2 * j + 1) % S::kSlots]);
+                }
+                if (j + 1 < count) scores(j + 1);
+                ok = ok && warp_wait(&ctl.ds, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                product_planes(tmem + kDk, tmem + kDp, slot(2 * j), steps, out_desc, j > 0);
-                tc_commit(&ctl.ring.empty[(2 * j) % S::kSlots]);
-                if (j + 1 < tiles) dp(j + 1);
+                if (elect_one()) {
+                    product_planes(base + kDk, base + kDp, slot(2 * j), steps, out_desc, j > 0);
+                    if (j + 1 == count) tc_commit(&ctl.done);
+                    tc_commit(&ctl.ring.empty[(2 * j) % S::kSlots]);
+                }
+                if (j + 1 < count) dp(j + 1);
             }
-            if (ok) tc_commit(&ctl.done);
             if (!ok && issued) {
-                tc_commit(&ctl.drain);
-                mbar_wait(&ctl.drain, 0, abort, true);
+                if (elect_one()) tc_commit(&ctl.drain);
+                warp_wait(&ctl.drain, 0, abort, true);
             }
         }
     } else if (warp < 4) {

@@ -49,6 +49,24 @@ __device__ __forceinline__ void store_values(float* out, const float (&v)[N], fl
                 make_float4(v[i] * factor, v[i + 1] * factor, v[i + 2] * factor, v[i + 3] * factor);
 }
 
+// D [128, n] = the six products of two operands of three planes, along their rows.
+template <int KS>
+__device__ __forceinline__ void product6(uint32_t d, uint32_t a, uint32_t b, uint32_t b_plane, uint32_t idesc) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i)
+        product_rows<KS>(d, a + kPlaneA[i] * kPanelBytes, b + kPlaneB[i] * b_plane, idesc, i > 0);
+}
+
+// D [128, n] = the six products of weights over a tile's columns (planes h and m at w, l at low) and a streamed tile.
+__device__ __forceinline__ void weigh6(uint32_t d, uint32_t w, uint32_t low, uint32_t b, int steps, uint32_t idesc) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+        const uint32_t at = b + kPlaneB[i] * kHalfPanel;
+        if (kPlaneA[i] == 2) product_weights<4, 2, 16>(d, low, at, steps, idesc, i > 0);
+        else product_weights<4, 2, 32>(d, w + 16u * kPlaneA[i], at, steps, idesc, i > 0);
+    }
+}
+
 // ---------------------------------------------------------------- planes
 
 struct SplitArgs {
@@ -164,50 +182,54 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
             });
         }
     } else if (warp == 1) {
-        if (lane == 0 && tiles > 0) {
+        if (tiles > 0) {
+            const uint32_t base = uniform(tmem), own_at = uniform(su32(own)), first_slot = uniform(su32(ring));
             const uint32_t o_desc = bf16_idesc(kDim, true);
-            auto slot = [&](int i) { return su32(ring + (i % kSlots) * kTile3); };
-            auto width = [&](int j) { return min(kTile, (end - j * kTile + 15) & ~15); };
-            bool ok = mbar_wait(&ctl.own, 0, abort), issued = false;
+            const int count = uniform(tiles), last_key = uniform(end);
+            const bool zeroed = uniform(int(tail));
+            auto slot = [&](int i) { return first_slot + uint32_t(i % kSlots) * kTile3; };
+            auto width = [&](int j) { return min(kTile, (last_key - j * kTile + 15) & ~15); };
+            bool ok = warp_wait(&ctl.own, 0, abort), issued = false;
             auto scores = [&](int j) {
                 ok = ok && landed(ctl.ring, 2 * j, abort);
                 if (!ok) return;
                 tc_fence_after();
-                const uint32_t d = tmem + uint32_t(j & 1) * 128u, q = su32(own), k = slot(2 * j);
                 const uint32_t desc = bf16_idesc(width(j), false);
-#pragma unroll
-                for (int i = 0; i < 6; ++i)
-                    product_rows<KS>(d, q + kPlaneA[i] * kPanelBytes, k + kPlaneB[i] * kPanelBytes, desc, i > 0);
-                tc_commit(&ctl.scores[j & 1]);
-                tc_commit(&ctl.ring.empty[(2 * j) % kSlots]);
+                if (elect_one()) {
+                    product6<KS>(base + uint32_t(j & 1) * 128u, own_at, slot(2 * j), kPanelBytes, desc);
+                    tc_commit(&ctl.scores[j & 1]);
+                    tc_commit(&ctl.ring.empty[(2 * j) % kSlots]);
+                }
                 issued = true;
             };
             scores(0);
-            for (int j = 0; j < tiles && ok; ++j) {
-                if (j + 1 < tiles) scores(j + 1);
+            for (int j = 0; j < count && ok; ++j) {
+                if (j + 1 < count) scores(j + 1);
                 ok = ok && landed(ctl.ring, 2 * j + 1, abort);
-                if (ok && tail && j == tiles - 1) {
-                    mbar_arrive(&ctl.tail_here);
-                    ok = mbar_wait(&ctl.tail, 0, abort);
+                if (ok && zeroed && j == count - 1) {
+                    if (elect_one()) mbar_arrive(&ctl.tail_here);
+                    ok = warp_wait(&ctl.tail, 0, abort);
                 }
-                ok = ok && mbar_wait(&ctl.weights, uint32_t(j) & 1u, abort);
+                ok = ok && warp_wait(&ctl.weights, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t p = tmem + uint32_t(j & 1) * 128u, v = slot(2 * j + 1);
+                const uint32_t odd = uint32_t(j & 1);
+                const uint32_t o = base + kO + odd * 64u, p = base + odd * 128u, low = base + kL + odd * 64u;
                 const int steps = width(j) / 16;
+                if (elect_one()) {
 #pragma unroll
-                for (int i = 0; i < 6; ++i) {
-                    const uint32_t at = v + kPlaneB[i] * kPanelBytes;
-                    const uint32_t o = tmem + kO + uint32_t(j & 1) * 64u, low = tmem + kL + uint32_t(j & 1) * 64u;
-                    if (kPlaneA[i] == 2) product_weights<8, 4, 32>(o, low, at, steps, o_desc, i > 0);
-                    else product_weights<8, 4, 64>(o, p + 32u * kPlaneA[i], at, steps, o_desc, i > 0);
+                    for (int i = 0; i < 6; ++i) {
+                        const uint32_t at = slot(2 * j + 1) + kPlaneB[i] * kPanelBytes;
+                        if (kPlaneA[i] == 2) product_weights<8, 4, 32>(o, low, at, steps, o_desc, i > 0);
+                        else product_weights<8, 4, 64>(o, p + 32u * kPlaneA[i], at, steps, o_desc, i > 0);
+                    }
+                    tc_commit(&ctl.out);
+                    tc_commit(&ctl.ring.empty[(2 * j + 1) % kSlots]);
                 }
-                tc_commit(&ctl.out);
-                tc_commit(&ctl.ring.empty[(2 * j + 1) % kSlots]);
             }
             if (!ok && issued) {
-                tc_commit(&ctl.drain);
-                mbar_wait(&ctl.drain, 0, abort, true);
+                if (elect_one()) tc_commit(&ctl.drain);
+                warp_wait(&ctl.drain, 0, abort, true);
             }
         }
     } else if (warp < 4) {
@@ -361,24 +383,6 @@ __device__ __forceinline__ void close_block(BackwardCtrl& ctl, int warp, int32_t
     if (threadIdx.x == 0 && ctl.abort) raise_flag(flags, FMD_FLAG_WAIT_TIMEOUT);
 }
 
-// D [128, n] = the six products of two operands of three planes, along their rows.
-template <int KS>
-__device__ __forceinline__ void product6(uint32_t d, uint32_t a, uint32_t b, uint32_t b_plane, uint32_t idesc) {
-#pragma unroll
-    for (int i = 0; i < 6; ++i)
-        product_rows<KS>(d, a + kPlaneA[i] * kPanelBytes, b + kPlaneB[i] * b_plane, idesc, i > 0);
-}
-
-// D [128, n] = the six products of weights over a tile's columns (planes h and m at w, l at low) and a streamed tile.
-__device__ __forceinline__ void weigh6(uint32_t d, uint32_t w, uint32_t low, uint32_t b, int steps, uint32_t idesc) {
-#pragma unroll
-    for (int i = 0; i < 6; ++i) {
-        const uint32_t at = b + kPlaneB[i] * kHalfPanel;
-        if (kPlaneA[i] == 2) product_weights<4, 2, 16>(d, low, at, steps, idesc, i > 0);
-        else product_weights<4, 2, 32>(d, w + 16u * kPlaneA[i], at, steps, idesc, i > 0);
-    }
-}
-
 // The three planes of a thread's 32 weights: h and m over the columns it has read, l beside.
 __device__ __forceinline__ void store_planes(uint32_t w, uint32_t low, float (&y)[32]) {
     uint32_t plane[16];
@@ -432,41 +436,50 @@ __global__ void __launch_bounds__(kThreads, 1)
             });
         }
     } else if (warp == 1) {
-        if (lane == 0 && tiles > 0) {
+        if (tiles > 0) {
+            const uint32_t base = uniform(tmem), own_at = uniform(su32(own)), first_slot = uniform(su32(ring));
             const uint32_t out_desc = bf16_idesc(kDim, true);
-            auto slot = [&](int i) { return su32(ring + (i % kStreamSlots) * kSlot3); };
-            auto width = [&](int j) { return min(kStream, (end - j * kStream + 15) & ~15); };
-            bool ok = mbar_wait(&ctl.own, 0, abort), issued = false;
+            const int count = uniform(tiles), last_key = uniform(end);
+            auto width = [&](int j) { return min(kStream, (last_key - j * kStream + 15) & ~15); };
+            const bool zeroed = uniform(int(tail));
+            auto slot = [&](int i) { return first_slot + uint32_t(i % kStreamSlots) * kSlot3; };
+            bool ok = warp_wait(&ctl.own, 0, abort), issued = false;
             auto both = [&](int j) {  // scores and dP of tile j
                 ok = ok && landed(ctl.ring, 2 * j, abort) && landed(ctl.ring, 2 * j + 1, abort);
                 if (!ok) return;
                 tc_fence_after();
-                const uint32_t at = tmem + uint32_t(j & 1) * kStream, desc = bf16_idesc(width(j), false);
-                product6<KS>(at, su32(own), slot(2 * j), kHalfPanel, desc);
-                tc_commit(&ctl.scores[j & 1]);
-                product6<KS>(at + kDp, su32(own + kTile3), slot(2 * j + 1), kHalfPanel, desc);
-                tc_commit(&ctl.dp[j & 1]);
-                tc_commit(&ctl.ring.empty[(2 * j + 1) % kStreamSlots]);
+                const uint32_t at = base + uint32_t(j & 1) * kStream, desc = bf16_idesc(width(j), false);
+                if (elect_one()) {
+                    product6<KS>(at, own_at, slot(2 * j), kHalfPanel, desc);
+                    tc_commit(&ctl.scores[j & 1]);
+                    product6<KS>(at + kDp, own_at + kTile3, slot(2 * j + 1), kHalfPanel, desc);
+                    tc_commit(&ctl.dp[j & 1]);
+                    tc_commit(&ctl.ring.empty[(2 * j + 1) % kStreamSlots]);
+                }
                 issued = true;
             };
             both(0);
-            for (int j = 0; j < tiles && ok; ++j) {
-                if (j + 1 < tiles) both(j + 1);
-                if (ok && tail && j == tiles - 1) {
-                    mbar_arrive(&ctl.tail_here);
-                    ok = mbar_wait(&ctl.tail, 0, abort);
+            for (int j = 0; j < count && ok; ++j) {
+                if (j + 1 < count) both(j + 1);
+                if (ok && zeroed && j == count - 1) {
+                    if (elect_one()) mbar_arrive(&ctl.tail_here);
+                    ok = warp_wait(&ctl.tail, 0, abort);
                 }
-                ok = ok && mbar_wait(&ctl.weights, uint32_t(j) & 1u, abort);
+                ok = ok && warp_wait(&ctl.weights, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                weigh6(tmem + kDq + uint32_t(j & 1) * 64u, tmem + kDp + uint32_t(j & 1) * kStream,
-                       tmem + kL + uint32_t(j & 1) * 32u, slot(2 * j), width(j) / 16, out_desc);
-                tc_commit(&ctl.out);
-                tc_commit(&ctl.ring.empty[(2 * j) % kStreamSlots]);
+                const int steps = width(j) / 16;
+                const uint32_t odd = uint32_t(j & 1);
+                if (elect_one()) {
+                    weigh6(base + kDq + odd * 64u, base + kDp + odd * kStream, base + kL + odd * 32u, slot(2 * j), steps,
+                           out_desc);
+                    tc_commit(&ctl.out);
+                    tc_commit(&ctl.ring.empty[(2 * j) % kStreamSlots]);
+                }
             }
             if (!ok && issued) {
-                tc_commit(&ctl.drain);
-                mbar_wait(&ctl.drain, 0, abort, true);
+                if (elect_one()) tc_commit(&ctl.drain);
+                warp_wait(&ctl.drain, 0, abort, true);
             }
         }
     } else if (warp < 4) {
@@ -587,43 +600,51 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
             });
         }
     } else if (warp == 1) {
-        if (lane == 0 && tiles > 0) {
+        if (tiles > 0) {
+            const uint32_t base = uniform(tmem), own_at = uniform(su32(own)), first_slot = uniform(su32(ring));
             const uint32_t out_desc = bf16_idesc(kDim, true);
-            auto slot = [&](int i) { return su32(ring + (i % kStreamSlots) * kSlot3); };
-            auto width = [&](int j) { return ((j == tiles - 1 ? last_rows : full_rows) + 15) & ~15; };
-            bool ok = mbar_wait(&ctl.own, 0, abort), issued = false;
-            auto both = [&](int j) {
+            const int count = uniform(tiles), rows_last = uniform(last_rows), rows_full = uniform(full_rows);
+            auto width = [&](int j) { return ((j == count - 1 ? rows_last : rows_full) + 15) & ~15; };
+            const bool zeroed = uniform(int(tail));
+            auto slot = [&](int i) { return first_slot + uint32_t(i % kStreamSlots) * kSlot3; };
+            bool ok = warp_wait(&ctl.own, 0, abort), issued = false;
+            auto both = [&](int j) {  // scores and dP of tile j
                 ok = ok && landed(ctl.ring, 2 * j, abort) && landed(ctl.ring, 2 * j + 1, abort);
                 if (!ok) return;
                 tc_fence_after();
-                const uint32_t at = tmem + uint32_t(j & 1) * kStream, desc = bf16_idesc(width(j), false);
-                product6<KS>(at, su32(own), slot(2 * j), kHalfPanel, desc);
-                tc_commit(&ctl.scores[j & 1]);
-                product6<KS>(at + kDp, su32(own + kTile3), slot(2 * j + 1), kHalfPanel, desc);
-                tc_commit(&ctl.dp[j & 1]);
+                const uint32_t at = base + uint32_t(j & 1) * kStream, desc = bf16_idesc(width(j), false);
+                if (elect_one()) {
+                    product6<KS>(at, own_at, slot(2 * j), kHalfPanel, desc);
+                    tc_commit(&ctl.scores[j & 1]);
+                    product6<KS>(at + kDp, own_at + kTile3, slot(2 * j + 1), kHalfPanel, desc);
+                    tc_commit(&ctl.dp[j & 1]);
+                }
                 issued = true;
             };
             both(0);
-            for (int j = 0; j < tiles && ok; ++j) {
-                if (j + 1 < tiles) both(j + 1);
-                if (ok && tail && j == tiles - 1) {
-                    mbar_arrive(&ctl.tail_here);
-                    ok = mbar_wait(&ctl.tail, 0, abort);
+            for (int j = 0; j < count && ok; ++j) {
+                if (j + 1 < count) both(j + 1);
+                if (ok && zeroed && j == count - 1) {
+                    if (elect_one()) mbar_arrive(&ctl.tail_here);
+                    ok = warp_wait(&ctl.tail, 0, abort);
                 }
-                ok = ok && mbar_wait(&ctl.weights, uint32_t(j) & 1u, abort);
+                ok = ok && warp_wait(&ctl.weights, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t at = tmem + uint32_t(j & 1) * kStream;
-                const uint32_t low = uint32_t(j & 1) * 32u;
-                weigh6(tmem + kDv, at, tmem + kPl + low, slot(2 * j + 1), width(j) / 16, out_desc);
-                weigh6(tmem + kDk, at + kDp, tmem + kDl + low, slot(2 * j), width(j) / 16, out_desc);
-                tc_commit(&ctl.out);
-                tc_commit(&ctl.ring.empty[(2 * j) % kStreamSlots]);
-                tc_commit(&ctl.ring.empty[(2 * j + 1) % kStreamSlots]);
+                const int steps = width(j) / 16;
+                const uint32_t odd = uint32_t(j & 1);
+                if (elect_one()) {
+                    const uint32_t at = base + odd * kStream, low = odd * 32u;
+                    weigh6(base + kDv, at, base + kPl + low, slot(2 * j + 1), steps, out_desc);
+                    weigh6(base + kDk, at + kDp, base + kDl + low, slot(2 * j), steps, out_desc);
+                    tc_commit(&ctl.out);
+                    tc_commit(&ctl.ring.empty[(2 * j) % kStreamSlots]);
+                    tc_commit(&ctl.ring.empty[(2 * j + 1) % kStreamSlots]);
+                }
             }
             if (!ok && issued) {
-                tc_commit(&ctl.drain);
-                mbar_wait(&ctl.drain, 0, abort, true);
+                if (elect_one()) tc_commit(&ctl.drain);
+                warp_wait(&ctl.drain, 0, abort, true);
             }
         }
     } else if (warp < 4) {

@@ -156,76 +156,74 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
             });
         }
     } else if (warp == 1) {
-        if (lane == 0 && last > 0) {
+        if (last > 0) {
+            const uint32_t base = uniform(tmem), q_tile = uniform(su32(smem)), first_slot = uniform(su32(ring));
             const uint32_t o_desc = bf16_idesc(S::kDim, true);
-            int slot = 0;  // of the next k or v tile in ring order
-            uint32_t phase = 0;
-            bool ok = mbar_wait(&ctl.q_full, 0, abort), issued = false;
-            auto next = [&] {  // waits for the next tile; its place
-                const int at = slot;
-                ok = ok && mbar_wait(&ctl.ring.full[slot], phase, abort);
-                if (++slot == S::kSlots) {
-                    slot = 0;
-                    phase ^= 1u;
-                }
-                return at;
-            };
-            auto width = [&](int t, int j) { return min(kTile, ((ends[t] - j * kTile) + 15) & ~15); };
-            auto score = [&](int t, int j, int k_slot) {
+            const int tiles = uniform(last);
+            const bool zeroed = uniform(int(tail));
+            int count[NT], end[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                count[t] = uniform(counts[t]);
+                end[t] = uniform(ends[t]);
+            }
+            auto slot = [&](int i) { return first_slot + uint32_t(i % S::kSlots) * S::kTileBytes; };
+            auto width = [&](int t, int j) { return min(kTile, (end[t] - j * kTile + 15) & ~15); };
+            bool ok = warp_wait(&ctl.q_full, 0, abort), issued = false;
+            auto score = [&](int t, int j) {
                 tc_fence_after();
-                product_rows<KS>(tmem + t * 128u, su32(smem + t * S::kTileBytes), su32(ring + k_slot * S::kTileBytes),
-                                 bf16_idesc(width(t, j), false));
-                tc_commit(&ctl.scores[t]);
+                const uint32_t desc = bf16_idesc(width(t, j), false);
+                if (elect_one()) {
+                    product_rows<KS>(base + t * 128u, q_tile + t * S::kTileBytes, slot(2 * j), desc);
+                    tc_commit(&ctl.scores[t]);
+                    if (t == NT - 1 || j >= count[NT - 1]) tc_commit(&ctl.ring.empty[(2 * j) % S::kSlots]);
+                }
                 issued = true;
             };
-            int k_slot = next();
-            if (ok) {
-                for (int t = 0; t < NT; ++t)
-                    if (counts[t] > 0) score(t, 0, k_slot);
-                tc_commit(&ctl.ring.empty[k_slot]);
-            }
-            for (int j = 0; j < last && ok; ++j) {
-                const int v_slot = next();
-                if (ok && tail && j == last - 1) {
-                    mbar_arrive(&ctl.tail_here);
-                    ok = mbar_wait(&ctl.tail, 0, abort);
+            ok = ok && landed(ctl.ring, 0, abort);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                if (ok && count[t] > 0) score(t, 0);
+            for (int j = 0; j < tiles && ok; ++j) {
+                ok = landed(ctl.ring, 2 * j + 1, abort);
+                if (ok && zeroed && j == tiles - 1) {
+                    if (elect_one()) mbar_arrive(&ctl.tail_here);
+                    ok = warp_wait(&ctl.tail, 0, abort);
                 }
-                if (!ok) break;
-                bool have_k = false;
+                bool next = false;  // the next k tile has landed
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    if (j < counts[t]) {
-                        ok = ok && mbar_wait(&ctl.weights[t], uint32_t(j) & 1u, abort);
-                        if (!ok) break;
-                        tc_fence_after();
-                        product_weights<8, 4, 32>(tmem + S::kO + uint32_t(t) * S::kDim, tmem + t * 128u,
-                                        su32(ring + v_slot * S::kTileBytes), width(t, j) / 16, o_desc, j > 0);
+                    if (j >= count[t]) continue;
+                    ok = ok && warp_wait(&ctl.weights[t], uint32_t(j) & 1u, abort);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const int steps = width(t, j) / 16;
+                    if (elect_one()) {
+                        product_weights<8, 4, 32>(base + S::kO + uint32_t(t) * S::kDim, base + t * 128u, slot(2 * j + 1),
+                                                  steps, o_desc, j > 0);
+                        if (j + 1 == count[t]) tc_commit(&ctl.done[t]);
+                        if (t == NT - 1 || j >= count[NT - 1]) tc_commit(&ctl.ring.empty[(2 * j + 1) % S::kSlots]);
                     }
-                    if (t == NT - 1) tc_commit(&ctl.ring.empty[v_slot]);
-                    if (j + 1 < last && !have_k) {
-                        k_slot = next();
-                        if (!ok) break;
-                        have_k = true;
-                    }
-                    if (j + 1 < counts[t]) score(t, j + 1, k_slot);
-                    else if (j + 1 == counts[t]) tc_commit(&ctl.done[t]);
-                    if (t == NT - 1 && j + 1 < last) tc_commit(&ctl.ring.empty[k_slot]);
+                    if (j + 1 >= count[t]) continue;
+                    if (!next) ok = landed(ctl.ring, 2 * j + 2, abort);
+                    if (!ok) break;
+                    next = true;
+                    score(t, j + 1);
                 }
             }
             if (!ok && issued) {  // the products in flight end before TMEM is freed
-                tc_commit(&ctl.drain);
-                mbar_wait(&ctl.drain, 0, abort, true);
+                if (elect_one()) tc_commit(&ctl.drain);
+                warp_wait(&ctl.drain, 0, abort, true);
             }
         }
     } else if (warp < 4) {
-        if (tail) {
-            if (mbar_wait(&ctl.tail_here, 0, abort)) {
-                const int first = keys - (last - 1) * kTile;
-                zero_rows(ring + ((2 * last - 1) % S::kSlots) * S::kTileBytes, S::kPanels, kPanelBytes, first, (first + 15) & ~15, threadIdx.x - 64, 64);
-                mbar_arrive(&ctl.tail);
-            }
+        if (tail && mbar_wait(&ctl.tail_here, 0, abort)) {
+            const int first = keys - (last - 1) * kTile;
+            zero_rows(ring + ((2 * last - 1) % S::kSlots) * S::kTileBytes, S::kPanels, kPanelBytes, first,
+                      (first + 15) & ~15, threadIdx.x - 64, 64);
+            mbar_arrive(&ctl.tail);
         }
-    } else if (warp >= 4) {
+    } else {
         // ---------------------------------------------------------- softmax: thread = row
         constexpr int kLoad = NT == 2 ? 128 : 64;
         const int t = (warp - 4) >> 2, r = threadIdx.x & 127;

@@ -23,6 +23,24 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// The products are issued by one thread of a warp whose lanes all walk through the same waits: only there, with every
+// operand the same in all lanes, does the compiler keep descriptors and addresses in uniform registers. Under a branch
+// on the lane each product took about 115 cycles to issue, twice what the tensor cores need for it.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// mbar_wait by a whole warp: true when every lane has seen the phase complete.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int32_t* abort,
+                                          bool ignore_abort = false) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, ignore_abort));
+}
+
 // The upper halves of the two descriptors (the lower ones hold the address and the leading offset, in 16 bytes):
 // groups of 8 rows 1024 bytes apart, descriptor version 1, 128-byte swizzle.
 constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
@@ -327,10 +345,10 @@ __device__ __forceinline__ void feed(Ring<SLOTS>& ring, uint64_t* own, volatile 
     }
 }
 
-// Waits for tile i; only for a thread that takes the tiles of each slot in order.
+// Waits (a whole warp) for tile i; only for a warp that takes the tiles of each slot in order.
 template <int SLOTS>
 __device__ __forceinline__ bool landed(Ring<SLOTS>& ring, int i, volatile int32_t* abort) {
-    return mbar_wait(&ring.full[i % SLOTS], uint32_t(i / SLOTS) & 1u, abort);
+    return warp_wait(&ring.full[i % SLOTS], uint32_t(i / SLOTS) & 1u, abort);
 }
 
 // The block's TMEM: COLUMNS of it, by one whole warp; the address through shared memory.
