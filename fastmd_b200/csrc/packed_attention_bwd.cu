@@ -71,8 +71,8 @@ __device__ __forceinline__ void open_block(Ctrl<KS>& ctl, int warp) {
         mbar_init(&ctl.scores[0], 1);
         mbar_init(&ctl.scores[1], 1);
         mbar_init(&ctl.dp, 1);
-        mbar_init(&ctl.p, kWorkers);
-        mbar_init(&ctl.ds, kWorkers);
+        mbar_init(&ctl.p, kWorkers / 32);
+        mbar_init(&ctl.ds, kWorkers / 32);
         mbar_init(&ctl.stats[0], 64);
         mbar_init(&ctl.stats[1], 64);
         mbar_init(&ctl.read[0], kWorkers / 32);
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&ctl.ds);
+            warp_arrive(&ctl.ds);
         }
         if (ok && tiles > 0) {
             const bool got = mbar_wait(&ctl.done, 0, abort);
@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&ctl.p);
+            warp_arrive(&ctl.p);
             got = mbar_wait(&ctl.dp, uint32_t(j) & 1u, abort);
             if (!__all_sync(0xffffffffu, got)) {
                 *abort = 1;
@@ -549,8 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&ctl.ds);
-            __syncwarp();
+            warp_arrive(&ctl.ds);
             if (lane == 0) mbar_arrive(&ctl.read[j & 1]);
         }
         if (ok && tiles > 0) {

@@ -154,8 +154,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
         init_ring(ctl.ring);
         mbar_init(&ctl.scores[0], 1);
         mbar_init(&ctl.scores[1], 1);
-        mbar_init(&ctl.weights, kWorkers);
-        mbar_init(&ctl.swap, kWorkers);
+        mbar_init(&ctl.weights, kWorkers / 32);
+        mbar_init(&ctl.swap, kWorkers / 32);
         mbar_init(&ctl.out, 1);
         mbar_init(&ctl.tail_here, 1);
         mbar_init(&ctl.tail, 64);
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
             float top = largest(x);
             // the row's maximum over both halves
             maxima[j & 1][half][r] = top;
-            mbar_arrive(&ctl.swap);
+            warp_arrive(&ctl.swap);
             if (!all(mbar_wait(&ctl.swap, uint32_t(j) & 1u, abort))) break;
             top = fmaxf(m, fmaxf(top, maxima[j & 1][1 - half][r]) * c);
             const float base = top == -INFINITY ? 0.0f : top;
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&ctl.weights);
+            warp_arrive(&ctl.weights);
             if (j > 0) {  // the last tile's output, against the old maximum, while this one's products run
                 if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
                 drain<kMine>(at_o + uint32_t((j - 1) & 1) * 64u, o, keep);
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
         }
         if (ok && tiles > 0) {
             sums[half][r] = l;
-            mbar_arrive(&ctl.swap);
+            warp_arrive(&ctl.swap);
             if (all(mbar_wait(&ctl.out, uint32_t(tiles - 1) & 1u, abort) &&
                     mbar_wait(&ctl.swap, uint32_t(tiles) & 1u, abort))) {
                 drain<kMine>(at_o + uint32_t((tiles - 1) & 1) * 64u, o, 1.0f);
@@ -362,7 +362,7 @@ __device__ __forceinline__ void open_block(BackwardCtrl& ctl, int warp) {
             mbar_init(&ctl.stats[i], 64);
             mbar_init(&ctl.read[i], kWorkers / 32);
         }
-        mbar_init(&ctl.weights, kWorkers);
+        mbar_init(&ctl.weights, kWorkers / 32);
         mbar_init(&ctl.out, 1);
         mbar_init(&ctl.tail_here, 1);
         mbar_init(&ctl.tail, 64);
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (any) store_planes(at + kDp, tmem + lanes + kL + uint32_t(j & 1) * 32u + uint32_t(half) * 16u, x);
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&ctl.weights);
+            warp_arrive(&ctl.weights);
             if (j > 0) {  // the last tile's product, while this one's runs
                 if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
                 drain<kMine>(at_q + uint32_t((j - 1) & 1) * 64u, dq, 1.0f);
@@ -728,8 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
                     x[i + 1] = r < m.y ? y.y : 0.0f;
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl.read[j & 1]);
+            warp_arrive(&ctl.read[j & 1]);
             if (any) {
                 const uint32_t low = lanes + uint32_t(j & 1) * 32u + uint32_t(half) * 16u;
                 store_planes(at, tmem + kPl + low, p);
@@ -741,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&ctl.weights);
+            warp_arrive(&ctl.weights);
         }
         if (ok && tiles > 0 && all(mbar_wait(&ctl.out, uint32_t(tiles - 1) & 1u, abort))) drain_all();
         if (ok && key0 + r < s.slot) {  // slot rows that are no keys get zeros

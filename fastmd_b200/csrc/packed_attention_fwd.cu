@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
         init_ring(ctl.ring);
         for (int t = 0; t < NT; ++t) {
             mbar_init(&ctl.scores[t], 1);
-            mbar_init(&ctl.weights[t], 128);
+            mbar_init(&ctl.weights[t], 4);
             mbar_init(&ctl.done[t], 1);
         }
         mbar_init(&ctl.tail_here, 1);
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
             }
             tc_fence_after();
             if (idle) {
-                mbar_arrive(&ctl.weights[t]);
+                warp_arrive(&ctl.weights[t]);
                 continue;
             }
             const int seen_here = min(kTile, ends[t] - j * kTile);  // columns that some row sees
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&ctl.weights[t]);
+            warp_arrive(&ctl.weights[t]);
         }
         if (ok && counts[t] > 0) {
             const bool got = mbar_wait(&ctl.done[t], 0, abort);

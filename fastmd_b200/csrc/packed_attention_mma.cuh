@@ -41,6 +41,12 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, ignore_abort));
 }
 
+// One arrival for a warp, after all its lanes have come this far (32 arrivals on one barrier go one by one).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 // The upper halves of the two descriptors (the lower ones hold the address and the leading offset, in 16 bytes):
 // groups of 8 rows 1024 bytes apart, descriptor version 1, 128-byte swizzle.
 constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
