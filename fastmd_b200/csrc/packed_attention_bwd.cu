@@ -37,19 +37,21 @@ namespace {
 constexpr int kThreads = 384;
 constexpr int kWorkers = 256;
 
-template <int KS>
+template <int KS, bool KEYS>
 struct Shape {
     static constexpr int kDim = 16 * KS;
     static constexpr int kPanels = (KS + 3) / 4;
     static constexpr uint32_t kTileBytes = kPanels * kPanelBytes;
-    static constexpr int kSlots = kPanels == 2 ? 4 : 8;  // 192 or 160 KB with the two tiles that stay
+    // as many as fit beside the two tiles that stay (and, for the keys, lse and delta): with five a tile's copy need
+    // not wait for the products of the one before
+    static constexpr int kSlots = kPanels == 1 ? 8 : KEYS ? 4 : 5;
     static constexpr size_t kBytes = size_t(2 + kSlots) * kTileBytes + 1024 + 256;
 };
 
-template <int KS>
+template <int KS, bool KEYS>
 struct Ctrl {
     uint64_t own;  // the two tiles that stay have landed
-    Ring<Shape<KS>::kSlots> ring;
+    Ring<Shape<KS, KEYS>::kSlots> ring;
     uint64_t scores[2], dp;      // products done
     uint64_t p, ds;              // written by the workers
     uint64_t stats[2], read[2];  // keys: lse and delta of a tile in shared memory; read by all worker warps
@@ -63,8 +65,8 @@ struct Maps {
     CUtensorMap q, g, k, v;
 };
 
-template <int KS>
-__device__ __forceinline__ void open_block(Ctrl<KS>& ctl, int warp) {
+template <int KS, bool KEYS>
+__device__ __forceinline__ void open_block(Ctrl<KS, KEYS>& ctl, int warp) {
     if (threadIdx.x == 0) {
         mbar_init(&ctl.own, 1);
         init_ring(ctl.ring);
@@ -90,8 +92,8 @@ __device__ __forceinline__ void open_block(Ctrl<KS>& ctl, int warp) {
     tc_fence_after();
 }
 
-template <int KS>
-__device__ __forceinline__ void close_block(Ctrl<KS>& ctl, int warp, int32_t* flags) {
+template <int KS, bool KEYS>
+__device__ __forceinline__ void close_block(Ctrl<KS, KEYS>& ctl, int warp, int32_t* flags) {
     tc_fence_before();
     __syncthreads();
     if (warp == 1) tmem_free<512>(ctl.tmem);
@@ -143,11 +145,11 @@ __device__ __forceinline__ void product_planes(uint32_t d, uint32_t ds, uint32_t
 template <int KS>
 __global__ void __launch_bounds__(kThreads, 1)
     query_gradient_kernel(const __grid_constant__ Maps maps, const Attn a) {
-    using S = Shape<KS>;
+    using S = Shape<KS, false>;
     extern __shared__ unsigned char raw[];
     unsigned char* own = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     unsigned char* ring = own + 2 * S::kTileBytes;
-    __shared__ Ctrl<KS> ctl;
+    __shared__ Ctrl<KS, false> ctl;
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -164,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool tail = tiles > 0 && keys < tiles * kTile;
     constexpr uint32_t kDp = 256, kDq = 384;  // TMEM columns: two score buffers, dP, dq
 
-    open_block<KS>(ctl, warp);
+    open_block(ctl, warp);
     const uint32_t tmem = ctl.tmem;
 
     if (warp == 0) {
@@ -317,18 +319,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 store_row(out, tmem + lanes + kDq, col, a.dim, a.scale, tiles > 0, true, real);
         }
     }
-    close_block<KS>(ctl, warp, a.flags);
+    close_block(ctl, warp, a.flags);
 }
 
 // ------------------------------------------------------------------- keys
 
 template <int KS>
 __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_constant__ Maps maps, const Attn a) {
-    using S = Shape<KS>;
+    using S = Shape<KS, true>;
     extern __shared__ unsigned char raw[];
     unsigned char* own = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     unsigned char* ring = own + 2 * S::kTileBytes;
-    __shared__ Ctrl<KS> ctl;
+    __shared__ Ctrl<KS, true> ctl;
     // of two tiles: - lse log2 e, - delta and the number of keys that each packed row sees
     __shared__ alignas(16) float lse_of[2][kTile], delta_of[2][kTile];
     __shared__ alignas(16) int limit_of[2][kTile];
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
     if (full_rows < kTile && warp >= 4)  // rows of the slots that no copy ever writes are inner rows of the products
         for (int i = 0; i < S::kSlots; ++i)
             zero_rows(ring + i * S::kTileBytes, S::kPanels, kPanelBytes, full_rows, kTile, threadIdx.x - 128, kWorkers);
-    open_block<KS>(ctl, warp);
+    open_block(ctl, warp);
     const uint32_t tmem = ctl.tmem;
 
     if (warp == 0) {
@@ -567,23 +569,23 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
                           real);
         }
     }
-    close_block<KS>(ctl, warp, a.flags);
+    close_block(ctl, warp, a.flags);
 }
 
 template <int KS>
 fmd_status launch(const Maps& maps, const Attn& a, cudaStream_t s) {
-    using S = Shape<KS>;
-    fmd_status st = grant_dynamic_smem((const void*)query_gradient_kernel<KS>, S::kBytes, true);
-    if (st == FMD_OK) st = grant_dynamic_smem((const void*)key_gradient_kernel<KS>, S::kBytes, true);
+    constexpr size_t query_bytes = Shape<KS, false>::kBytes, key_bytes = Shape<KS, true>::kBytes;
+    fmd_status st = grant_dynamic_smem((const void*)query_gradient_kernel<KS>, query_bytes, true);
+    if (st == FMD_OK) st = grant_dynamic_smem((const void*)key_gradient_kernel<KS>, key_bytes, true);
     if (st != FMD_OK) return st;
     if (a.dq != nullptr && a.rows > 0) {
         const int64_t tiles = tile_bound(a.rows, a.batch, kTile / a.group);
-        query_gradient_kernel<KS><<<dim3(unsigned(tiles), unsigned(a.hk)), kThreads, S::kBytes, s>>>(maps, a);
+        query_gradient_kernel<KS><<<dim3(unsigned(tiles), unsigned(a.hk)), kThreads, query_bytes, s>>>(maps, a);
         if ((st = check_launch()) != FMD_OK) return st;
     }
     if (a.dk != nullptr && a.keys > 0) {
         const int64_t tiles = tile_bound(a.keys, a.batch, kTile);
-        key_gradient_kernel<KS><<<dim3(unsigned(tiles), unsigned(a.hk)), kThreads, S::kBytes, s>>>(maps, a);
+        key_gradient_kernel<KS><<<dim3(unsigned(tiles), unsigned(a.hk)), kThreads, key_bytes, s>>>(maps, a);
         st = check_launch();
     }
     return st;

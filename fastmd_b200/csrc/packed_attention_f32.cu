@@ -176,9 +176,11 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
                 tma_load_4d(su32(own + p * kPanelBytes), &maps.q, &ctl.own, 0, 0, head,
                             int(p * a.rows + s.row0 + token0));
             feed(ctl.ring, &ctl.own, abort, 2 * tiles, kTile3, [&](int i, int slot, uint64_t* bar) {
-                for (int p = 0; p < 3; ++p)  // k0, v0, k1, v1, ..
-                    tma_load_4d(su32(ring + slot * kTile3 + p * kPanelBytes), i & 1 ? &maps.v : &maps.k, bar, 0, 0, head,
-                                int(p * a.keys + s.key0) + from + (i >> 1) * kTile);
+                const bool last = i == 2 * tiles - 1, v = last || (i > 0 && i % 2 == 0);
+                const int j = last ? tiles - 1 : v ? i / 2 - 1 : (i + 1) / 2;
+                for (int p = 0; p < 3; ++p)
+                    tma_load_4d(su32(ring + slot * kTile3 + p * kPanelBytes), v ? &maps.v : &maps.k, bar, 0, 0, head,
+                                int(p * a.keys + s.key0) + from + j * kTile);
             });
         }
     } else if (warp == 1) {
@@ -187,25 +189,28 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
             const uint32_t o_desc = bf16_idesc(kDim, true);
             const int count = uniform(tiles), last_key = uniform(end);
             const bool zeroed = uniform(int(tail));
+            // two key tiles ahead of the values: k0 k1 v0 k2 v1 .. k(n-1) v(n-2) v(n-1)
+            auto key_at = [&](int j) { return j > 0 ? 2 * j - 1 : 0; };
+            auto value_at = [&](int j) { return j + 1 < count ? 2 * j + 2 : 2 * j + 1; };
             auto slot = [&](int i) { return first_slot + uint32_t(i % kSlots) * kTile3; };
             auto width = [&](int j) { return min(kTile, (last_key - j * kTile + 15) & ~15); };
             bool ok = warp_wait(&ctl.own, 0, abort), issued = false;
             auto scores = [&](int j) {
-                ok = ok && landed(ctl.ring, 2 * j, abort);
+                ok = ok && landed(ctl.ring, key_at(j), abort);
                 if (!ok) return;
                 tc_fence_after();
                 const uint32_t desc = bf16_idesc(width(j), false);
                 if (elect_one()) {
-                    product6<KS>(base + uint32_t(j & 1) * 128u, own_at, slot(2 * j), kPanelBytes, desc);
+                    product6<KS>(base + uint32_t(j & 1) * 128u, own_at, slot(key_at(j)), kPanelBytes, desc);
                     tc_commit(&ctl.scores[j & 1]);
-                    tc_commit(&ctl.ring.empty[(2 * j) % kSlots]);
+                    tc_commit(&ctl.ring.empty[key_at(j) % kSlots]);
                 }
                 issued = true;
             };
             scores(0);
+            if (count > 1) scores(1);
             for (int j = 0; j < count && ok; ++j) {
-                if (j + 1 < count) scores(j + 1);
-                ok = ok && landed(ctl.ring, 2 * j + 1, abort);
+                ok = landed(ctl.ring, value_at(j), abort);
                 if (ok && zeroed && j == count - 1) {
                     if (elect_one()) mbar_arrive(&ctl.tail_here);
                     ok = warp_wait(&ctl.tail, 0, abort);
@@ -219,13 +224,14 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
                 if (elect_one()) {
 #pragma unroll
                     for (int i = 0; i < 6; ++i) {
-                        const uint32_t at = slot(2 * j + 1) + kPlaneB[i] * kPanelBytes;
+                        const uint32_t at = slot(value_at(j)) + kPlaneB[i] * kPanelBytes;
                         if (kPlaneA[i] == 2) product_weights<8, 4, 32>(o, low, at, steps, o_desc, i > 0);
                         else product_weights<8, 4, 64>(o, p + 32u * kPlaneA[i], at, steps, o_desc, i > 0);
                     }
                     tc_commit(&ctl.out);
-                    tc_commit(&ctl.ring.empty[(2 * j + 1) % kSlots]);
+                    tc_commit(&ctl.ring.empty[value_at(j) % kSlots]);
                 }
+                if (j + 2 < count) scores(j + 2);  // over this tile's weights, behind the product that reads them
             }
             if (!ok && issued) {
                 if (elect_one()) tc_commit(&ctl.drain);
@@ -337,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
 // --------------------------------------------------------------- gradients
 
 constexpr int kStream = 64;                     // rows of a streamed tile
-constexpr int kStreamSlots = 4;
+constexpr int kStreamSlots = 5;                 // a tile's copy need not wait for the products of the one before
 constexpr uint32_t kSlot3 = 3 * kHalfPanel;
 constexpr size_t kBackwardBytes = 2 * size_t(kTile3) + kStreamSlots * size_t(kSlot3) + 1024;
 
