@@ -10,9 +10,13 @@
 // the softmax's rescaling) is kept in registers.
 //
 // The forward pass is a block per 128 packed rows and key tiles of 128, the gradients as for bfloat16 (queries: a
-// block per 128 packed rows; keys: a block per 128 keys) with streamed tiles of 64, so that two stages of three planes
-// fit in shared memory beside the block's own. Roles of the warps, order of the products, masks and bounded waits are
-// those of the bfloat16 kernels. 256 workers: two threads per lane, each half of the columns.
+// block per 128 packed rows; keys: a block per 128 keys) with streamed tiles of 64. There the block's own planes are in
+// TMEM: a product of 64 columns takes 32 cycles so and 48 with both operands in shared memory, and shared memory holds
+// four stages. Roles of the warps, masks and bounded waits are those of the bfloat16 kernels. 256 workers: two threads
+// per lane, each half of the columns. Order of the products:
+//   forward  S0 S1 | [p j] o(j), S(j+2)
+//   queries  S0 dP0 | S(j+1) dP(j+1), [ds j] dq(j)
+//   keys     S0 dP0 | [p j] dv(j), S(j+1), [ds j] dk(j), dP(j+1)
 
 #include "packed_attention_mma.cuh"
 
@@ -28,6 +32,11 @@ __device__ constexpr int kPlaneB[6] = {0, 2, 1, 0, 1, 0};
 
 struct Maps {
     CUtensorMap q, g, k, v;
+};
+
+// the planes in memory, for the rows that a block keeps
+struct Own {
+    const __nv_bfloat16 *q, *g, *k, *v;
 };
 
 // N columns of TMEM (16 or 32) added to a sum in registers, which is then scaled.
@@ -57,12 +66,26 @@ __device__ __forceinline__ void product6(uint32_t d, uint32_t a, uint32_t b, uin
         product_rows<KS>(d, a + kPlaneA[i] * kPanelBytes, b + kPlaneB[i] * b_plane, idesc, i > 0);
 }
 
-// D [128, n] = the six products of weights over a tile's columns (planes h and m at w, l at low) and a streamed tile.
+// The same with the first operand's planes in TMEM (8 KS columns each) and a streamed tile of 64 rows.
+template <int KS>
+__device__ __forceinline__ void product6_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+        const uint32_t bd = rows_desc(b + kPlaneB[i] * kHalfPanel);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+            mma_weights(d, a + 8u * (kPlaneA[i] * KS + k), bd + 2 * k, idesc, i > 0 || k > 0);
+    }
+}
+
+// D [128, n] = the six products of weights over a tile's 64 columns (planes h and m at w, 16 columns each of every 32
+// that they replace; l at low, 16 columns of every kLow) and a streamed tile.
+template <uint32_t kLow>
 __device__ __forceinline__ void weigh6(uint32_t d, uint32_t w, uint32_t low, uint32_t b, int steps, uint32_t idesc) {
 #pragma unroll
     for (int i = 0; i < 6; ++i) {
         const uint32_t at = b + kPlaneB[i] * kHalfPanel;
-        if (kPlaneA[i] == 2) product_weights<4, 2, 16>(d, low, at, steps, idesc, i > 0);
+        if (kPlaneA[i] == 2) product_weights<4, 2, kLow>(d, low, at, steps, idesc, i > 0);
         else product_weights<4, 2, 32>(d, w + 16u * kPlaneA[i], at, steps, idesc, i > 0);
     }
 }
@@ -343,16 +366,17 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
 // --------------------------------------------------------------- gradients
 
 constexpr int kStream = 64;                     // rows of a streamed tile
-constexpr int kStreamSlots = 5;                 // a tile's copy need not wait for the products of the one before
+constexpr int kStreamSlots = 8;
 constexpr uint32_t kSlot3 = 3 * kHalfPanel;
-constexpr size_t kBackwardBytes = 2 * size_t(kTile3) + kStreamSlots * size_t(kSlot3) + 1024;
+constexpr size_t kBackwardBytes = kStreamSlots * size_t(kSlot3) + 1024;
 
 struct BackwardCtrl {
-    uint64_t own;
+    uint64_t own;                // the block's own planes are in TMEM
     Ring<kStreamSlots> ring;
-    uint64_t scores[2], dp[2];
-    uint64_t weights, out;
-    uint64_t stats[2], read[2];
+    uint64_t scores[2], dp[2];   // products done
+    uint64_t p, ds;              // written by the workers
+    uint64_t out;
+    uint64_t stats[2], read[2];  // keys: lse and delta of a tile in shared memory; read by all worker warps
     uint64_t tail_here, tail, drain;
     uint32_t tmem;
     int32_t abort;
@@ -360,7 +384,7 @@ struct BackwardCtrl {
 
 __device__ __forceinline__ void open_block(BackwardCtrl& ctl, int warp) {
     if (threadIdx.x == 0) {
-        mbar_init(&ctl.own, 1);
+        mbar_init(&ctl.own, kWorkers / 32);
         init_ring(ctl.ring);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctl.scores[i], 1);
@@ -368,7 +392,8 @@ __device__ __forceinline__ void open_block(BackwardCtrl& ctl, int warp) {
             mbar_init(&ctl.stats[i], 64);
             mbar_init(&ctl.read[i], kWorkers / 32);
         }
-        mbar_init(&ctl.weights, kWorkers / 32);
+        mbar_init(&ctl.p, kWorkers / 32);
+        mbar_init(&ctl.ds, kWorkers / 32);
         mbar_init(&ctl.out, 1);
         mbar_init(&ctl.tail_here, 1);
         mbar_init(&ctl.tail, 64);
@@ -389,6 +414,25 @@ __device__ __forceinline__ void close_block(BackwardCtrl& ctl, int warp, int32_t
     if (threadIdx.x == 0 && ctl.abort) raise_flag(flags, FMD_FLAG_WAIT_TIMEOUT);
 }
 
+// A worker's row of one tensor: its three planes into TMEM, 8 KS columns each; zeros where there is no row.
+template <int KS>
+__device__ __forceinline__ void load_own(uint32_t at, const __nv_bfloat16* row, int64_t plane, int dim, bool real) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+#pragma unroll
+        for (int c = 0; c < KS; c += 2) {  // 32 values: 16 columns
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (real && 16 * c + 8 * i < dim) v = *reinterpret_cast<const uint4*>(row + p * plane + 16 * c + 8 * i);
+                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+            }
+            tmem_store16(at + uint32_t(8 * (p * KS + c)), w);
+        }
+    }
+}
+
 // The three planes of a thread's 32 weights: h and m over the columns it has read, l beside.
 __device__ __forceinline__ void store_planes(uint32_t w, uint32_t low, float (&y)[32]) {
     uint32_t plane[16];
@@ -402,12 +446,12 @@ __device__ __forceinline__ void store_planes(uint32_t w, uint32_t low, float (&y
 
 template <int KS>
 __global__ void __launch_bounds__(kThreads, 1)
-    query_gradient_kernel(const __grid_constant__ Maps maps, const Attn a) {
+    query_gradient_kernel(const __grid_constant__ Maps maps, const Attn a, const Own own) {
     constexpr int kDim = 16 * KS, kMine = kDim / 2;
-    constexpr uint32_t kDp = 128, kL = 256, kDq = 320;  // TMEM columns, two buffers each: scores, dP, ds's l, dq
+    // TMEM columns: two buffers of scores (then of ds's lowest plane) and of dP (then ds's other planes), dq, q, g
+    constexpr uint32_t kDp = 128, kDq = 256, kQ = 320, kG = 416;
     extern __shared__ unsigned char raw[];
-    unsigned char* own = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    unsigned char* ring = own + 2 * kTile3;
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     __shared__ BackwardCtrl ctl;
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -429,12 +473,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 0) {
         if (lane == 0 && tiles > 0) {
-            mbar_expect_tx(&ctl.own, 2u * 3u * 128u * uint32_t(per_tile * a.group));
-            for (int p = 0; p < 3; ++p) {
-                const int row = int(p * a.rows + s.row0 + token0);
-                tma_load_4d(su32(own + p * kPanelBytes), &maps.q, &ctl.own, 0, 0, head, row);
-                tma_load_4d(su32(own + kTile3 + p * kPanelBytes), &maps.g, &ctl.own, 0, 0, head, row);
-            }
             feed(ctl.ring, &ctl.own, abort, 2 * tiles, kSlot3, [&](int i, int slot, uint64_t* bar) {
                 for (int p = 0; p < 3; ++p)  // k0, v0, k1, v1, ..
                     tma_load_4d(su32(ring + slot * kSlot3 + p * kHalfPanel), i & 1 ? &maps.v : &maps.k, bar, 0, 0, head,
@@ -443,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1) {
         if (tiles > 0) {
-            const uint32_t base = uniform(tmem), own_at = uniform(su32(own)), first_slot = uniform(su32(ring));
+            const uint32_t base = uniform(tmem), first_slot = uniform(su32(ring));
             const uint32_t out_desc = bf16_idesc(kDim, true);
             const int count = uniform(tiles), last_key = uniform(end);
             auto width = [&](int j) { return min(kStream, (last_key - j * kStream + 15) & ~15); };
@@ -456,9 +494,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_fence_after();
                 const uint32_t at = base + uint32_t(j & 1) * kStream, desc = bf16_idesc(width(j), false);
                 if (elect_one()) {
-                    product6<KS>(at, own_at, slot(2 * j), kHalfPanel, desc);
+                    product6_tmem<KS>(at, base + kQ, slot(2 * j), desc);
                     tc_commit(&ctl.scores[j & 1]);
-                    product6<KS>(at + kDp, own_at + kTile3, slot(2 * j + 1), kHalfPanel, desc);
+                    product6_tmem<KS>(at + kDp, base + kG, slot(2 * j + 1), desc);
                     tc_commit(&ctl.dp[j & 1]);
                     tc_commit(&ctl.ring.empty[(2 * j + 1) % kStreamSlots]);
                 }
@@ -471,14 +509,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (elect_one()) mbar_arrive(&ctl.tail_here);
                     ok = warp_wait(&ctl.tail, 0, abort);
                 }
-                ok = ok && warp_wait(&ctl.weights, uint32_t(j) & 1u, abort);
+                ok = ok && warp_wait(&ctl.ds, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
                 const int steps = width(j) / 16;
                 const uint32_t odd = uint32_t(j & 1);
                 if (elect_one()) {
-                    weigh6(base + kDq + odd * 64u, base + kDp + odd * kStream, base + kL + odd * 32u, slot(2 * j), steps,
-                           out_desc);
+                    weigh6<32>(base + kDq, base + kDp + odd * kStream, base + odd * kStream, slot(2 * j), steps, out_desc);
                     tc_commit(&ctl.out);
                     tc_commit(&ctl.ring.empty[(2 * j) % kStreamSlots]);
                 }
@@ -510,6 +547,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         float dq[kMine];
 #pragma unroll
         for (int i = 0; i < kMine; ++i) dq[i] = 0.0f;
+        if (tiles > 0) {  // the first four warps bring q, the others g
+            const int64_t plane = a.rows * a.hq * a.dim;
+            load_own<KS>(tmem + lanes + (half ? kG : kQ), (half ? own.g : own.q) + flat * a.dim, plane, a.dim, real);
+            tmem_wait_st();
+            tc_fence_before();
+            warp_arrive(&ctl.own);
+        }
         bool ok = true;
         auto all = [&](bool got) {
             ok = __all_sync(0xffffffffu, got);
@@ -542,30 +586,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                     x[i + 1] = i + 1 < mine ? y.y : 0.0f;
                 }
             }
-            if (any) store_planes(at + kDp, tmem + lanes + kL + uint32_t(j & 1) * 32u + uint32_t(half) * 16u, x);
+            if (j > 0) {  // the last tile's product is added before this one's starts over
+                if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
+                drain<kMine>(at_q, dq, 1.0f);
+            }
+            if (any) store_planes(at + kDp, at, x);
             tmem_wait_st();
             tc_fence_before();
-            warp_arrive(&ctl.weights);
-            if (j > 0) {  // the last tile's product, while this one's runs
-                if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
-                drain<kMine>(at_q + uint32_t((j - 1) & 1) * 64u, dq, 1.0f);
-            }
+            warp_arrive(&ctl.ds);
         }
         if (ok && tiles > 0 && all(mbar_wait(&ctl.out, uint32_t(tiles - 1) & 1u, abort)))
-            drain<kMine>(at_q + uint32_t((tiles - 1) & 1) * 64u, dq, 1.0f);
+            drain<kMine>(at_q, dq, 1.0f);
         if (ok && real) store_values<kMine>(static_cast<float*>(a.dq) + flat * a.dim, dq, a.scale, half * kMine, a.dim);
     }
     close_block(ctl, warp, a.flags);
 }
 
 template <int KS>
-__global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_constant__ Maps maps, const Attn a) {
+__global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_constant__ Maps maps, const Attn a, const Own own) {
     constexpr int kDim = 16 * KS;
-    // TMEM columns: two buffers each of scores, dP and the lowest planes of p and ds; dv, dk
-    constexpr uint32_t kDp = 128, kPl = 256, kDl = 320, kDv = 384, kDk = 448;
+    // TMEM columns: scores (then p's planes h and m), dP (then ds's), the lowest planes of p and ds, dv, dk, k, v
+    constexpr uint32_t kDp = 64, kPl = 128, kDl = 160, kDv = 192, kDk = 256, kK = 320, kV = 416;
     extern __shared__ unsigned char raw[];
-    unsigned char* own = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    unsigned char* ring = own + 2 * kTile3;
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     __shared__ BackwardCtrl ctl;
     // of two tiles: - lse log2 e, - delta and the number of keys that each packed row sees
     __shared__ alignas(16) float lse_of[2][kStream], delta_of[2][kStream];
@@ -593,12 +636,6 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
 
     if (warp == 0) {
         if (lane == 0 && tiles > 0) {
-            mbar_expect_tx(&ctl.own, 2u * kTile3);
-            for (int p = 0; p < 3; ++p) {
-                const int row = int(p * a.keys + s.key0 + key0);
-                tma_load_4d(su32(own + p * kPanelBytes), &maps.k, &ctl.own, 0, 0, head, row);
-                tma_load_4d(su32(own + kTile3 + p * kPanelBytes), &maps.v, &ctl.own, 0, 0, head, row);
-            }
             feed(ctl.ring, &ctl.own, abort, 2 * tiles, 3u * 128u * full_rows, [&](int i, int slot, uint64_t* bar) {
                 for (int p = 0; p < 3; ++p)  // q0, g0, q1, g1, ..
                     tma_load_4d(su32(ring + slot * kSlot3 + p * kHalfPanel), i & 1 ? &maps.g : &maps.q, bar, 0, 0, head,
@@ -607,46 +644,59 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
         }
     } else if (warp == 1) {
         if (tiles > 0) {
-            const uint32_t base = uniform(tmem), own_at = uniform(su32(own)), first_slot = uniform(su32(ring));
+            const uint32_t base = uniform(tmem), first_slot = uniform(su32(ring));
             const uint32_t out_desc = bf16_idesc(kDim, true);
             const int count = uniform(tiles), rows_last = uniform(last_rows), rows_full = uniform(full_rows);
-            auto width = [&](int j) { return ((j == count - 1 ? rows_last : rows_full) + 15) & ~15; };
             const bool zeroed = uniform(int(tail));
             auto slot = [&](int i) { return first_slot + uint32_t(i % kStreamSlots) * kSlot3; };
+            auto width = [&](int j) { return ((j == count - 1 ? rows_last : rows_full) + 15) & ~15; };
             bool ok = warp_wait(&ctl.own, 0, abort), issued = false;
-            auto both = [&](int j) {  // scores and dP of tile j
-                ok = ok && landed(ctl.ring, 2 * j, abort) && landed(ctl.ring, 2 * j + 1, abort);
+            auto scores = [&](int j) {
+                ok = ok && landed(ctl.ring, 2 * j, abort);
                 if (!ok) return;
                 tc_fence_after();
-                const uint32_t at = base + uint32_t(j & 1) * kStream, desc = bf16_idesc(width(j), false);
+                const uint32_t desc = bf16_idesc(width(j), false);
                 if (elect_one()) {
-                    product6<KS>(at, own_at, slot(2 * j), kHalfPanel, desc);
-                    tc_commit(&ctl.scores[j & 1]);
-                    product6<KS>(at + kDp, own_at + kTile3, slot(2 * j + 1), kHalfPanel, desc);
-                    tc_commit(&ctl.dp[j & 1]);
+                    product6_tmem<KS>(base, base + kK, slot(2 * j), desc);
+                    tc_commit(&ctl.scores[0]);
                 }
                 issued = true;
             };
-            both(0);
+            auto dp = [&](int j) {
+                ok = ok && landed(ctl.ring, 2 * j + 1, abort);
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t desc = bf16_idesc(width(j), false);
+                if (elect_one()) {
+                    product6_tmem<KS>(base + kDp, base + kV, slot(2 * j + 1), desc);
+                    tc_commit(&ctl.dp[0]);
+                }
+            };
+            scores(0);
+            dp(0);
             for (int j = 0; j < count && ok; ++j) {
-                if (j + 1 < count) both(j + 1);
-                if (ok && zeroed && j == count - 1) {
+                const int steps = width(j) / 16;
+                if (zeroed && j == count - 1) {
                     if (elect_one()) mbar_arrive(&ctl.tail_here);
                     ok = warp_wait(&ctl.tail, 0, abort);
                 }
-                ok = ok && warp_wait(&ctl.weights, uint32_t(j) & 1u, abort);
+                ok = ok && warp_wait(&ctl.p, uint32_t(j) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
-                const int steps = width(j) / 16;
-                const uint32_t odd = uint32_t(j & 1);
                 if (elect_one()) {
-                    const uint32_t at = base + odd * kStream, low = odd * 32u;
-                    weigh6(base + kDv, at, base + kPl + low, slot(2 * j + 1), steps, out_desc);
-                    weigh6(base + kDk, at + kDp, base + kDl + low, slot(2 * j), steps, out_desc);
-                    tc_commit(&ctl.out);
-                    tc_commit(&ctl.ring.empty[(2 * j) % kStreamSlots]);
+                    weigh6<16>(base + kDv, base, base + kPl, slot(2 * j + 1), steps, out_desc);
                     tc_commit(&ctl.ring.empty[(2 * j + 1) % kStreamSlots]);
                 }
+                if (j + 1 < count) scores(j + 1);
+                ok = ok && warp_wait(&ctl.ds, uint32_t(j) & 1u, abort);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    weigh6<16>(base + kDk, base + kDp, base + kDl, slot(2 * j), steps, out_desc);
+                    if (j + 1 == count) tc_commit(&ctl.out);
+                    tc_commit(&ctl.ring.empty[(2 * j) % kStreamSlots]);
+                }
+                if (j + 1 < count) dp(j + 1);
             }
             if (!ok && issued) {
                 if (elect_one()) tc_commit(&ctl.drain);
@@ -690,6 +740,13 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
         float out[kDim / 32][32];
 #pragma unroll
         for (int i = 0; i < kDim; ++i) out[i / 32][i % 32] = 0.0f;
+        if (tiles > 0) {  // the first four warps bring k, the others v
+            const int64_t at = ((s.key0 + key0 + r) * a.hk + head) * a.dim, plane = a.keys * a.hk * a.dim;
+            load_own<KS>(tmem + lanes + (half ? kV : kK), (half ? own.v : own.k) + at, plane, a.dim, key0 + r < s.keys);
+            tmem_wait_st();
+            tc_fence_before();
+            warp_arrive(&ctl.own);
+        }
         bool ok = true;
         auto all = [&](bool got) {
             ok = __all_sync(0xffffffffu, got);
@@ -707,10 +764,10 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
             const float* nl = lse_of[j & 1] + 32 * half;
             const float* nd = delta_of[j & 1] + 32 * half;
             const int* lim = limit_of[j & 1] + 32 * half;
-            const uint32_t at = tmem + lanes + uint32_t(j & 1) * kStream + uint32_t(half) * 32u;
+            const uint32_t at = tmem + lanes + uint32_t(half) * 32u, low = tmem + lanes + uint32_t(half) * 16u;
             float p[32], x[32];
             if (!all(mbar_wait(&ctl.stats[j & 1], uint32_t(j >> 1) & 1u, abort) &&
-                     mbar_wait(&ctl.scores[j & 1], uint32_t(j >> 1) & 1u, abort)))
+                     mbar_wait(&ctl.scores[0], uint32_t(j) & 1u, abort)))
                 break;
             if (any) {
                 tmem_load32(at, p);
@@ -718,11 +775,18 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
                 for (int i = 0; i < 32; i += 2) {
                     const float2 y = fma2(make_float2(p[i], p[i + 1]), c2, *reinterpret_cast<const float2*>(nl + i));
                     const int2 m = *reinterpret_cast<const int2*>(lim + i);
-                    p[i] = r < m.x ? ex2(y.x) : 0.0f;
-                    p[i + 1] = r < m.y ? ex2(y.y) : 0.0f;
+                    p[i] = x[i] = r < m.x ? ex2(y.x) : 0.0f;
+                    p[i + 1] = x[i + 1] = r < m.y ? ex2(y.y) : 0.0f;
                 }
+                store_planes(at, low + kPl, x);
             }
-            if (!all(mbar_wait(&ctl.dp[j & 1], uint32_t(j >> 1) & 1u, abort))) break;
+            // the scores were issued behind the last tile's dv, dP behind its dk: each is complete, and added here
+            // before the products that start over
+            if (j > 0 && half == 0) drain_all();
+            tmem_wait_st();
+            tc_fence_before();
+            warp_arrive(&ctl.p);
+            if (!all(mbar_wait(&ctl.dp[0], uint32_t(j) & 1u, abort))) break;
             if (any) {
                 tmem_load32(at + kDp, x);
 #pragma unroll
@@ -733,22 +797,15 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
                     x[i] = r < m.x ? y.x : 0.0f;
                     x[i + 1] = r < m.y ? y.y : 0.0f;
                 }
+                store_planes(at + kDp, low + kDl, x);
             }
-            warp_arrive(&ctl.read[j & 1]);
-            if (any) {
-                const uint32_t low = lanes + uint32_t(j & 1) * 32u + uint32_t(half) * 16u;
-                store_planes(at, tmem + kPl + low, p);
-                store_planes(at + kDp, tmem + kDl + low, x);
-            }
-            if (j > 0) {  // the last products are added before the next ones start over
-                if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
-                drain_all();
-            }
+            if (j > 0 && half == 1) drain_all();
             tmem_wait_st();
             tc_fence_before();
-            warp_arrive(&ctl.weights);
+            warp_arrive(&ctl.ds);
+            if (lane == 0) mbar_arrive(&ctl.read[j & 1]);
         }
-        if (ok && tiles > 0 && all(mbar_wait(&ctl.out, uint32_t(tiles - 1) & 1u, abort))) drain_all();
+        if (ok && tiles > 0 && all(mbar_wait(&ctl.out, 0, abort))) drain_all();
         if (ok && key0 + r < s.slot) {  // slot rows that are no keys get zeros
             float* row = static_cast<float*>(half ? a.dk : a.dv) + ((s.key0 + key0 + r) * a.hk + head) * a.dim;
             const bool keep = key0 + r < s.keys;
@@ -818,18 +875,18 @@ fmd_status launch_forward(const Maps& maps, const Attn& a, int splits, cudaStrea
 }
 
 template <int KS>
-fmd_status launch_backward(const Maps& queries, const Maps& keys, const Attn& a, cudaStream_t s) {
+fmd_status launch_backward(const Maps& maps, const Attn& a, const Own& own, cudaStream_t s) {
     fmd_status st = grant_dynamic_smem((const void*)query_gradient_kernel<KS>, kBackwardBytes, true);
     if (st == FMD_OK) st = grant_dynamic_smem((const void*)key_gradient_kernel<KS>, kBackwardBytes, true);
     if (st != FMD_OK) return st;
     if (a.dq != nullptr && a.rows > 0) {
         const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kTile / a.group)), unsigned(a.hk));
-        query_gradient_kernel<KS><<<grid, kThreads, kBackwardBytes, s>>>(queries, a);
+        query_gradient_kernel<KS><<<grid, kThreads, kBackwardBytes, s>>>(maps, a, own);
         if ((st = check_launch()) != FMD_OK) return st;
     }
     if (a.dk != nullptr && a.keys > 0) {
         const dim3 grid(unsigned(tile_bound(a.keys, a.batch, kTile)), unsigned(a.hk));
-        key_gradient_kernel<KS><<<grid, kThreads, kBackwardBytes, s>>>(keys, a);
+        key_gradient_kernel<KS><<<grid, kThreads, kBackwardBytes, s>>>(maps, a, own);
         st = check_launch();
     }
     return st;
@@ -870,30 +927,25 @@ fmd_status attention_backward_planes(const Attn& a, void* workspace, cudaStream_
     if (drv.encode == nullptr || drv.ctx_get_current == nullptr)
         return record_error_text(FMD_ERR_CUDA, "driver entry point cuTensorMapEncodeTiled unavailable", 0);
     fmd_status st = bind_context(drv);
-    Maps queries{}, keys{};  // own tiles of 128 rows and streamed ones of 64, of the one kernel and of the other
+    Maps maps{};  // of streamed tiles of 64 rows; a block reads its own rows by itself
+    Own own{};
     Planes planes(workspace);
     if (a.rows > 0) {
-        const void* q = planes.add(a.q, a.rows, a.hq, a.q_row, a.q_head, a.dim);
-        const void* g = planes.add(a.g, a.rows, a.hq, a.g_row, a.g_head, a.dim);
-        for (int i = 0; i < 2 && st == FMD_OK; ++i) {
-            Maps& maps = i ? keys : queries;
-            const int tokens = (i ? kStream : kTile) / a.group;
-            st = encode_planes(drv, &maps.q, q, a.rows, a.hk, a.group, a.dim, tokens);
-            if (st == FMD_OK) st = encode_planes(drv, &maps.g, g, a.rows, a.hk, a.group, a.dim, tokens);
-        }
+        const int tokens = kStream / a.group;
+        own.q = planes.add(a.q, a.rows, a.hq, a.q_row, a.q_head, a.dim);
+        own.g = planes.add(a.g, a.rows, a.hq, a.g_row, a.g_head, a.dim);
+        if (st == FMD_OK) st = encode_planes(drv, &maps.q, own.q, a.rows, a.hk, a.group, a.dim, tokens);
+        if (st == FMD_OK) st = encode_planes(drv, &maps.g, own.g, a.rows, a.hk, a.group, a.dim, tokens);
     }
     if (a.keys > 0) {
-        const void* k = planes.add(a.k, a.keys, a.hk, a.k_row, a.k_head, a.dim);
-        const void* v = planes.add(a.v, a.keys, a.hk, a.v_row, a.v_head, a.dim);
-        for (int i = 0; i < 2 && st == FMD_OK; ++i) {
-            Maps& maps = i ? keys : queries;
-            st = encode_planes(drv, &maps.k, k, a.keys, a.hk, 1, a.dim, i ? kTile : kStream);
-            if (st == FMD_OK) st = encode_planes(drv, &maps.v, v, a.keys, a.hk, 1, a.dim, i ? kTile : kStream);
-        }
+        own.k = planes.add(a.k, a.keys, a.hk, a.k_row, a.k_head, a.dim);
+        own.v = planes.add(a.v, a.keys, a.hk, a.v_row, a.v_head, a.dim);
+        if (st == FMD_OK) st = encode_planes(drv, &maps.k, own.k, a.keys, a.hk, 1, a.dim, kStream);
+        if (st == FMD_OK) st = encode_planes(drv, &maps.v, own.v, a.keys, a.hk, 1, a.dim, kStream);
     }
     if (st == FMD_OK) st = planes.launch(s);
     if (st != FMD_OK) return st;
-    return a.dim <= 32 ? launch_backward<2>(queries, keys, a, s) : launch_backward<4>(queries, keys, a, s);
+    return a.dim <= 32 ? launch_backward<2>(maps, a, own, s) : launch_backward<4>(maps, a, own, s);
 }
 
 }  // namespace fmd
