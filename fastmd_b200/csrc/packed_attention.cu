@@ -18,29 +18,60 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
         make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// out and lse of the splits of the keys together: out = sum_z exp(lse_z - lse) out_z. A thread per row and four values.
-template <typename T>
+// out and lse of the splits of the keys together: out = sum_z exp(lse_z - lse) out_z. A warp per row, four values a
+// lane; with many splits PARTS warps share a row's (their loads are what the time goes to).
+template <typename T, int PARTS>
 __global__ void __launch_bounds__(kThreads) join_kernel(const Attn a, int splits) {
-    const int quads = a.dim / 4;
-    const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x, all = a.rows * a.hq, row = i / quads;
-    const int quad = int(i - row * quads);
-    if (row >= all) return;
-    float top = -INFINITY;
-    for (int z = 0; z < splits; ++z) top = fmaxf(top, a.part_lse[z * all + row]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
+    constexpr int kWarps = kThreads / 32;
+    __shared__ float4 sums[kWarps][32];
+    __shared__ float weights[kWarps];
+    const int quad = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % PARTS;
+    const int64_t row = int64_t(blockIdx.x) * (kWarps / PARTS) + warp / PARTS, all = a.rows * a.hq;
+    float top = -INFINITY, sum = 0.0f;
     float4 o = f4_zero();
-    for (int z = 0; z < splits; ++z) {
-        const float lse = a.part_lse[z * all + row];
-        if (lse == -INFINITY) continue;  // a split without keys of this row wrote nothing else
-        const float w = exp2f((lse - base) * kLog2e);
-        const float4 v = *reinterpret_cast<const float4*>(a.part + (z * all + row) * a.dim + quad * 4);
-        sum += w;
-        o = make_float4(fmaf(w, v.x, o.x), fmaf(w, v.y, o.y), fmaf(w, v.z, o.z), fmaf(w, v.w, o.w));
+    if (row < all) {
+        for (int z = quad; z < splits; z += 32) top = fmaxf(top, a.part_lse[z * all + row]);
+#pragma unroll
+        for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+        const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll 4
+        for (int z = part; z < splits; z += PARTS) {
+            const float lse = a.part_lse[z * all + row];
+            if (lse == -INFINITY) continue;  // a split without keys of this row wrote nothing else
+            const float w = exp2f((lse - base) * kLog2e);
+            sum += w;
+            if (quad * 4 < a.dim) {
+                const float4 v = *reinterpret_cast<const float4*>(a.part + (z * all + row) * a.dim + quad * 4);
+                o = make_float4(fmaf(w, v.x, o.x), fmaf(w, v.y, o.y), fmaf(w, v.z, o.z), fmaf(w, v.w, o.w));
+            }
+        }
     }
+    if (PARTS > 1) {
+        sums[warp][quad] = o;
+        if (quad == 0) weights[warp] = sum;
+        __syncthreads();
+        if (part > 0) return;
+#pragma unroll
+        for (int i = 1; i < PARTS; ++i) {
+            o = f4_add(o, sums[warp + i][quad]);
+            sum += weights[warp + i];
+        }
+    }
+    if (row >= all) return;
     const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-    store4(static_cast<T*>(a.out) + row * a.dim + quad * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    if (quad * 4 < a.dim)
+        store4(static_cast<T*>(a.out) + row * a.dim + quad * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     if (quad == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? -INFINITY : top + logf(sum);
+}
+
+template <typename T>
+fmd_status join(const Attn& a, int splits, cudaStream_t s) {
+    const int parts = splits >= 16 ? 8 : 1, rows_each = kThreads / 32 / parts;
+    const int64_t blocks = (a.rows * a.hq + rows_each - 1) / rows_each;
+    if (blocks > INT32_MAX) return FMD_ERR_UNSUPPORTED;
+    if (parts == 8) join_kernel<T, 8><<<unsigned(blocks), kThreads, 0, s>>>(a, splits);
+    else join_kernel<T, 1><<<unsigned(blocks), kThreads, 0, s>>>(a, splits);
+    return check_launch();
 }
 
 // delta[row] = sum_d g out - (gradient of lse): 8 lanes per packed row, 16-byte loads.
@@ -173,10 +204,7 @@ fmd_status fmd_packed_attention(const fmd_attention* problem, void* out, float* 
     else if (a.dim <= kPlanesDim) st = attention_forward_planes(a, p.splits, workspace, s);
     else st = attention_forward_simt(a, p.splits, s);
     if (st != FMD_OK || p.splits == 1) return st;
-    const unsigned blocks = unsigned((a.rows * a.hq * (a.dim / 4) + kThreads - 1) / kThreads);
-    if (problem->type == FMD_BF16) join_kernel<__nv_bfloat16><<<blocks, kThreads, 0, s>>>(a, p.splits);
-    else join_kernel<float><<<blocks, kThreads, 0, s>>>(a, p.splits);
-    return check_launch();
+    return problem->type == FMD_BF16 ? join<__nv_bfloat16>(a, p.splits, s) : join<float>(a, p.splits, s);
 }
 
 fmd_status fmd_packed_attention_bwd(const fmd_attention* problem, const void* out, const float* lse, const void* g,
