@@ -53,64 +53,52 @@ struct Args {
     int32_t dim, rot, w_float;
 };
 
-__device__ __forceinline__ void load_quad(const float* p, float (&v)[4]) {
-    const float4 f = *reinterpret_cast<const float4*>(p);
-    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-}
-
-// the raw loads of a lane's two quads, kept packed until they are used
+// A lane's two quads as they are in memory, kept packed until they are used; then as four pairs of neighbours.
 template <typename T>
 struct Raw;
 
 template <>
 struct Raw<float> {
     float4 a, b;
-    __device__ __forceinline__ void load(const float* p, int qa, int qb) {
-        a = *reinterpret_cast<const float4*>(p + qa);
-        b = *reinterpret_cast<const float4*>(p + qb);
+    __device__ __forceinline__ void load(const float* p, int gap) {
+        a = *reinterpret_cast<const float4*>(p);
+        b = *reinterpret_cast<const float4*>(p + gap);
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    __device__ __forceinline__ void zero() { a = b = f4_zero(); }
+    __device__ __forceinline__ void get(float2 (&v)[4]) const {
+        v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w);
+        v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
     }
-    static __device__ __forceinline__ void put(float* p, int qa, int qb, const float (&v)[8]) {
-        *reinterpret_cast<float4*>(p + qa) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(p + qb) = make_float4(v[4], v[5], v[6], v[7]);
+    static __device__ __forceinline__ void put(float* p, int gap, const float2 (&v)[4]) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        *reinterpret_cast<float4*>(p + gap) = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
     }
 };
-
-__device__ __forceinline__ float2 halves(uint32_t w) {
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-
-__device__ __forceinline__ uint32_t join(float low, float high) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(low, high);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
 
 template <>
 struct Raw<__nv_bfloat16> {
     uint2 a, b;
-    __device__ __forceinline__ void load(const __nv_bfloat16* p, int qa, int qb) {
-        if (qb == qa + 4) {
-            const uint4 w = *reinterpret_cast<const uint4*>(p + qa);
+    __device__ __forceinline__ void load(const __nv_bfloat16* p, int gap) {
+        if (gap == 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(p);
             a = make_uint2(w.x, w.y), b = make_uint2(w.z, w.w);
         } else {
-            a = *reinterpret_cast<const uint2*>(p + qa);
-            b = *reinterpret_cast<const uint2*>(p + qb);
+            a = *reinterpret_cast<const uint2*>(p);
+            b = *reinterpret_cast<const uint2*>(p + gap);
         }
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        const float2 f[4] = {halves(a.x), halves(a.y), halves(b.x), halves(b.y)};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[2 * i] = f[i].x, v[2 * i + 1] = f[i].y;
+    __device__ __forceinline__ void zero() { a = b = make_uint2(0, 0); }
+    __device__ __forceinline__ void get(float2 (&v)[4]) const {
+        v[0] = unpack_bf16(a.x), v[1] = unpack_bf16(a.y), v[2] = unpack_bf16(b.x), v[3] = unpack_bf16(b.y);
     }
-    static __device__ __forceinline__ void put(__nv_bfloat16* p, int qa, int qb, const float (&v)[8]) {
-        const uint2 a = make_uint2(join(v[0], v[1]), join(v[2], v[3])), b = make_uint2(join(v[4], v[5]), join(v[6], v[7]));
-        if (qb == qa + 4) {
-            *reinterpret_cast<uint4*>(p + qa) = make_uint4(a.x, a.y, b.x, b.y);
+    static __device__ __forceinline__ void put(__nv_bfloat16* p, int gap, const float2 (&v)[4]) {
+        const uint2 a = make_uint2(pack_bf16(v[0].x, v[0].y), pack_bf16(v[1].x, v[1].y));
+        const uint2 b = make_uint2(pack_bf16(v[2].x, v[2].y), pack_bf16(v[3].x, v[3].y));
+        if (gap == 4) {
+            *reinterpret_cast<uint4*>(p) = make_uint4(a.x, a.y, b.x, b.y);
         } else {
-            *reinterpret_cast<uint2*>(p + qa) = a;
-            *reinterpret_cast<uint2*>(p + qb) = b;
+            *reinterpret_cast<uint2*>(p) = a;
+            *reinterpret_cast<uint2*>(p + gap) = b;
         }
     }
 };
@@ -120,16 +108,35 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162f
 __device__ __forceinline__ void from_float(float& o, float v) { o = v; }
 __device__ __forceinline__ void from_float(__nv_bfloat16& o, float v) { o = __float2bfloat16_rn(v); }
 
-// Turns the lane's four pairs by their angles.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// Turns the lane's four pairs: c and s hold the four cosines and sines, two and two (s negated to turn back).
 template <bool INTER>
-__device__ __forceinline__ void turn(float (&v)[8], const float (&c)[4], const float (&s)[4]) {
+__device__ __forceinline__ void turn(float2 (&v)[4], const float2 (&c)[2], const float2 (&s)[2]) {
+    if (INTER) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int p = INTER ? 2 * i : i, q = INTER ? 2 * i + 1 : i + 4;
-        const float a = v[p], b = v[q];
-        v[p] = a * c[i] - b * s[i];
-        v[q] = b * c[i] + a * s[i];
+        for (int i = 0; i < 4; ++i) {
+            const float ci = i & 1 ? c[i / 2].y : c[i / 2].x, si = i & 1 ? s[i / 2].y : s[i / 2].x;
+            v[i] = fma2(v[i], both(ci), mul2(make_float2(v[i].y, v[i].x), make_float2(-si, si)));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float2 a = v[i], b = v[i + 2];
+            v[i] = fma2(a, c[i], mul2(b, make_float2(-s[i].x, -s[i].y)));
+            v[i + 2] = fma2(b, c[i], mul2(a, s[i]));
+        }
     }
+}
+
+// The sum of the pairwise products of a lane, over the lanes of a head.
+__device__ __forceinline__ float dot(const float2 (&a)[4], const float2 (&b)[4], int span) {
+    float2 t = mul2(a[0], b[0]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) t = fma2(a[i], b[i], t);
+    float sum = t.x + t.y;
+    for (int o = span / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
 }
 
 // Blocks of an SM: the backward pass holds twice the loads and the weights' sums in registers.
@@ -147,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, kResident<BACKWARD>) head_rotary_ker
     const bool active = sub < lanes;
     const int half = a.rot / 2;
     const bool turned = 8 * sub < a.rot;
-    const int qa = !INTER && turned ? 4 * sub : 8 * sub, qb = !INTER && turned ? half + 4 * sub : 8 * sub + 4;
+    const int qa = !INTER && turned ? 4 * sub : 8 * sub, gap = !INTER && turned ? half : 4;  // the second quad
 
     // this warp's heads: unit `u` of the row's units
     const int units = a.side[0].units + a.side[1].units;
@@ -162,91 +169,90 @@ __global__ void __launch_bounds__(kThreads, kResident<BACKWARD>) head_rotary_ker
     const int head0 = u * HEADS * across + group % across;
     const int64_t row_step = walkers * rows_at_once;
 
-    float w[8], dw[8];
+    float2 w[4], dw[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int at = (j < 4 ? qa : qb - 4) + j;
-        dw[j] = 0.0f;
-        w[j] = 1.0f;
-        if (NORM && s.w != nullptr && active)
-            w[j] = a.w_float ? static_cast<const float*>(s.w)[at] : to_float(static_cast<const T*>(s.w)[at]);
+    for (int j = 0; j < 4; ++j) {
+        dw[j] = both(0.0f);
+        w[j] = both(1.0f);
+        if (NORM && s.w != nullptr && active) {
+            const int at = qa + (j < 2 ? 2 * j : gap + 2 * j - 4);
+            if (a.w_float) w[j] = make_float2(static_cast<const float*>(s.w)[at], static_cast<const float*>(s.w)[at + 1]);
+            else w[j] = make_float2(to_float(static_cast<const T*>(s.w)[at]), to_float(static_cast<const T*>(s.w)[at + 1]));
+        }
     }
     const bool norm = NORM && s.w != nullptr;
-    const int64_t first = start < walkers ? start * rows_at_once + group / across : a.rows;
-    int64_t next = first < a.rows ? a.positions[first] : 0;
+    // addresses are set up once and move by the walk's step
+    int64_t row = start * rows_at_once + group / across;
+    const T* x = static_cast<const T*>(s.x) + row * s.row + head0 * s.head + qa;
+    const T* g = static_cast<const T*>(s.g) + row * s.grow + head0 * s.ghead + qa;
+    T* y = static_cast<T*>(s.y) + (row * s.heads + head0) * a.dim + qa;
+    const int64_t x_step = row_step * s.row, g_step = row_step * s.grow, y_step = row_step * s.heads * a.dim;
+    const int64_t x_head = across * s.head, g_head = across * s.ghead;
+    const int y_head = across * a.dim;
+    int64_t next = start < walkers && row < a.rows ? a.positions[row] : 0;
     // the loop's bound is the warp's first row: its lanes stay together for the shuffles
-    for (int64_t base = start < walkers ? start * rows_at_once : a.rows; base < a.rows; base += row_step) {
-        const int64_t row = base + group / across;
+    for (int64_t base = start < walkers ? row - group / across : a.rows; base < a.rows; base += row_step) {
         const bool here = active && row < a.rows;
-        Raw<T> x[HEADS], g[HEADS];
+        Raw<T> xs[HEADS], gs[HEADS];
 #pragma unroll
         for (int i = 0; i < HEADS; ++i) {
-            const int h = head0 + i * across;
-            if (here && h < s.heads) {
-                if (!BACKWARD || norm) x[i].load(static_cast<const T*>(s.x) + row * s.row + h * s.head, qa, qb);
-                if (BACKWARD) g[i].load(static_cast<const T*>(s.g) + row * s.grow + h * s.ghead, qa, qb);
+            const bool mine = here && head0 + i * across < s.heads;
+            if (!BACKWARD || norm) {
+                if (mine) xs[i].load(x + i * x_head, gap);
+                else xs[i].zero();
+            }
+            if (BACKWARD) {
+                if (mine) gs[i].load(g + i * g_head, gap);
+                else gs[i].zero();
             }
         }
         const int64_t pos = next;
         if (row + row_step < a.rows) next = a.positions[row + row_step];
         const bool known = pos >= 0 && pos < a.table;
         if (!known && row < a.rows && sub == 0) raise_flag(a.flags, FMD_FLAG_INDEX_RANGE);
-        float c[4] = {1.0f, 1.0f, 1.0f, 1.0f}, sn[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float2 c[2] = {both(1.0f), both(1.0f)}, sn[2] = {both(0.0f), both(0.0f)};
         if (turned && here) {
-            c[0] = c[1] = c[2] = c[3] = 0.0f;
+            float4 cf = f4_zero(), sf = f4_zero();
             if (known) {
-                load_quad(a.cos + pos * half + 4 * sub, c);
-                load_quad(a.sin + pos * half + 4 * sub, sn);
+                cf = ldg4(a.cos + pos * half + 4 * sub);
+                sf = ldg4(a.sin + pos * half + 4 * sub);
             }
-            if (BACKWARD) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sn[j] = -sn[j];
-            }
+            const float sign = BACKWARD ? -1.0f : 1.0f;
+            c[0] = make_float2(cf.x, cf.y), c[1] = make_float2(cf.z, cf.w);
+            sn[0] = make_float2(sign * sf.x, sign * sf.y), sn[1] = make_float2(sign * sf.z, sign * sf.w);
         }
 #pragma unroll
         for (int i = 0; i < HEADS; ++i) {
-            const int h = head0 + i * across;
-            const bool mine = here && h < s.heads;
-            if (!__any_sync(0xffffffffu, mine)) break;
-            float v[8], y[8];
+            if (u * HEADS * across + i * across >= s.heads) break;  // the same for the whole warp
+            float2 v[4], o[4];
             float n = 1.0f;
-            if (!BACKWARD || norm) {
-                x[i].get(v);
-                if (norm) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) sum += v[j] * v[j];
-                    sum = mine ? sum : 0.0f;
-                    for (int o = span / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    n = rsqrtf(sum * a.inv_dim + a.eps);
-                }
-            }
+            if (!BACKWARD || norm) xs[i].get(v);
+            if (norm) n = rsqrtf(dot(v, v, span) * a.inv_dim + a.eps);
             if (!BACKWARD) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = norm ? v[j] * n * w[j] : v[j];
-                turn<INTER>(y, c, sn);
+                for (int j = 0; j < 4; ++j) o[j] = norm ? mul2(v[j], mul2(both(n), w[j])) : v[j];
+                turn<INTER>(o, c, sn);
             } else {
-                g[i].get(y);
-                turn<INTER>(y, c, sn);
+                gs[i].get(o);
+                turn<INTER>(o, c, sn);
                 if (norm) {
-                    float dot = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        v[j] *= n;  // u
-                        const float t = y[j] * v[j];
-                        dw[j] += mine ? t : 0.0f;
-                        dot += t * w[j];
-                        y[j] *= w[j];
+                    for (int j = 0; j < 4; ++j) {
+                        v[j] = mul2(v[j], both(n));  // u; zero, as its gradient, in lanes without a head
+                        dw[j] = fma2(o[j], v[j], dw[j]);
+                        o[j] = mul2(o[j], w[j]);
                     }
-                    dot = mine ? dot : 0.0f;
-                    for (int o = span / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-                    dot *= a.inv_dim;
+                    const float mean = -dot(o, v, span) * a.inv_dim;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) y[j] = n * (y[j] - v[j] * dot);
+                    for (int j = 0; j < 4; ++j) o[j] = mul2(both(n), fma2(v[j], both(mean), o[j]));
                 }
             }
-            if (mine) Raw<T>::put(static_cast<T*>(s.y) + (row * s.heads + h) * a.dim, qa, qb, y);
+            if (here && head0 + i * across < s.heads) Raw<T>::put(y + i * y_head, gap, o);
         }
+        row += row_step;
+        x += x_step;
+        g += g_step;
+        y += y_step;
     }
 
     if (BACKWARD && NORM && a.partial != nullptr) {
@@ -254,9 +260,9 @@ __global__ void __launch_bounds__(kThreads, kResident<BACKWARD>) head_rotary_ker
         __shared__ int side_of[kWarps];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float t = dw[j];
+            float t = j & 1 ? dw[j / 2].y : dw[j / 2].x;
             for (int o = 16; o >= span; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-            if (group == 0 && active) sums[warp][(j < 4 ? qa : qb - 4) + j] = t;
+            if (group == 0 && active) sums[warp][qa + (j < 4 ? j : gap + j - 4)] = t;
         }
         if (lane == 0) side_of[warp] = which;
         __syncthreads();
