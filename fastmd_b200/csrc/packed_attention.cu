@@ -113,7 +113,10 @@ fmd_status check(const fmd_attention& q, Attn& a) {
     const int size = q.type == FMD_F32 ? 4 : 2;
     if ((q.rows > 0 && !rows16(q.q, q.q_row, q.q_head, size)) ||
         (q.keys > 0 && (!rows16(q.k, q.k_row, q.k_head, size) || !rows16(q.v, q.v_row, q.v_head, size))) ||
-        q.key_heads > 65535 || q.rows > (1 << 29) || q.keys > (1 << 29) || q.batch > (1 << 24))
+        q.rows > (1 << 29) || q.keys > (1 << 29) || q.batch > (1 << 24) ||
+        // a block per tile (of 64 rows at least) and key head
+        tile_bound(q.rows, q.batch, 64 / (q.heads / q.key_heads)) > INT32_MAX / q.key_heads ||
+        tile_bound(q.keys, q.batch, 64) > INT32_MAX / q.key_heads)
         return FMD_ERR_UNSUPPORTED;
     a = Attn{};
     a.q = q.q;

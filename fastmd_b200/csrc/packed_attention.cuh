@@ -8,7 +8,8 @@
 // sequence and a place in it with the monotone map  first(b) = offsets[b] / per_tile + b : sequence b owns the
 // indexes first(b) .. first(b + 1) - 1, which are never fewer than its tiles (floor(x + n) - floor(x) + 1 >=
 // ceil(n) for lengths in tiles); an index past its tiles has nothing to do. So a launch needs no list of tiles, no
-// copy to the host and no maximum length.
+// copy to the host and no maximum length. With few sequences the indexes are dealt out heaviest tile first instead
+// (find_place): blocks start in order, and a long tile that starts last is waited for by the whole GPU.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -20,6 +21,7 @@ namespace fmd {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kRowTile = 128;  // packed rows, or keys, of a tile on the tensor cores
 
 struct Attn {
     const void* q;      // [rows, hq, dim]
@@ -85,9 +87,90 @@ __device__ __forceinline__ Span load_span(const Attn& a, int b) {
     }
     // packed rows no sequence holds would stay unwritten: the offsets have to cover them all
     bad = bad || (b == 0 && (r0 != 0 || k0 != 0)) || (b == a.batch - 1 && (r1 != a.rows || k1 != a.keys));
-    if (bad && (threadIdx.x & 31) == 0) raise_flag(a.flags, FMD_FLAG_INDEX_RANGE);
+    if (bad) raise_flag(a.flags, FMD_FLAG_INDEX_RANGE);
     s.keys = n;
     return s;
+}
+
+// Tiles of a sequence whose work is at least `level` units, all of them for level 0. KEYS: tiles of `per` keys, their
+// work the tokens that see the first one, the heavy ones at the front; else tiles of `per` tokens, their work the keys
+// that the last one sees, the heavy ones at the end.
+template <bool KEYS>
+__device__ __forceinline__ int tiles_of(const Span& s, bool causal, int per, int unit, int level) {
+    const int rows = int(s.rows), keys = int(s.keys);
+    const int all = ((KEYS ? int(s.slot) : rows) + per - 1) / per;
+    if (level == 0) return all;
+    const int least = (level - 1) * unit + 1;
+    if (keys < least && !KEYS) return 0;
+    if (KEYS) {
+        if (rows < least || keys == 0) return 0;
+        return causal ? (keys < least ? 0 : (keys - least) / per + 1) : (keys + per - 1) / per;
+    }
+    const int token = least - keys + rows;  // tokens up to here see fewer keys
+    return !causal || token <= 0 ? all : all - (token + per - 1) / per + 1;
+}
+
+// A block's sequence and its tile in it (from its first row or key); b < 0: nothing to do.
+struct Place {
+    int b, tile;
+};
+
+// Sequences that a warp sorts by, one a lane. With more of them the blocks are many and even out by themselves, and the
+// longer search cost more than it gave (64 sequences of 135 rows: dk and dv 66 -> 75 us).
+constexpr int kSorted = 32;
+
+// The index-th tile, heaviest first where there are at most kSorted sequences. All 32 lanes of a warp.
+template <bool KEYS>
+__device__ __forceinline__ Place find_place(const Attn& a, int per, int index, int places) {
+    const int lane = threadIdx.x & 31;
+    if (a.batch > kSorted) {
+        const int64_t* offsets = KEYS ? a.key_offsets : a.offsets;
+        if (!KEYS) index = places - 1 - index;  // a causal sequence's last rows see the most
+        const int b = find_sequence(offsets, a.batch, per, index);
+        const int64_t tile = index - (offsets[b] / per + b);
+        const Span s = load_span(a, b);
+        return tile < 0 || tile * per >= (KEYS ? s.slot : s.rows) ? Place{-1, 0} : Place{b, int(tile)};
+    }
+    const int unit = KEYS ? kRowTile / a.group : kRowTile;
+    const Span s = lane < a.batch ? load_span(a, lane) : Span{};
+    auto mine = [&](int level) { return tiles_of<KEYS>(s, a.causal, per, unit, level); };
+    auto count = [&](int level) { return int(__reduce_add_sync(0xffffffffu, unsigned(mine(level)))); };
+    if (index >= count(0)) return Place{-1, 0};
+    // the highest level with more than `index` tiles
+    int low = 0, high = int(__reduce_max_sync(0xffffffffu, unsigned((KEYS ? s.rows : s.keys) / unit + 1)));
+    while (low < high) {
+        const int mid = (low + high + 1) / 2;
+        if (count(mid) > index) low = mid;
+        else high = mid - 1;
+    }
+    // the rank among the tiles of this very level, which go by sequence
+    const int here = mine(low), above = mine(low + 1);
+    int before = here - above;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+    }
+    before -= here - above;
+    const int rank = index - int(__reduce_add_sync(0xffffffffu, unsigned(above)));
+    const int b = __ffs(__ballot_sync(0xffffffffu, rank >= before && rank < before + here - above)) - 1;
+    const int first = KEYS ? above : mine(0) - here;
+    return Place{b, __shfl_sync(0xffffffffu, first + rank - before, b)};
+}
+
+// The same for a whole block: its first warp looks, all get the answer. Blocks count through the key heads first, so
+// that the order holds for all heads together; `head` is the block's.
+template <bool KEYS>
+__device__ __forceinline__ Place block_place(const Attn& a, int per, int* head) {
+    __shared__ Place place;
+    const int index = int(blockIdx.x / unsigned(a.hk));
+    *head = int(blockIdx.x - unsigned(index) * unsigned(a.hk));
+    if (threadIdx.x < 32) {
+        const Place p = find_place<KEYS>(a, per, index, int(gridDim.x / unsigned(a.hk)));
+        if (threadIdx.x == 0) place = p;
+    }
+    __syncthreads();
+    return place;
 }
 
 // Keys that token t (of the span) sees: all, or with causal those up to its place counted from the end.

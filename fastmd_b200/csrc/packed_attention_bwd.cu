@@ -153,13 +153,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int64_t index = gridDim.x - 1 - blockIdx.x;
     const int per_tile = kTile / a.group;
-    const int b = find_sequence(a.offsets, a.batch, per_tile, index);
-    const Span s = load_span(a, b);
-    const int64_t token0 = (index - (a.offsets[b] / per_tile + b)) * per_tile;
-    if (token0 < 0 || token0 >= s.rows) return;
-    const int head = blockIdx.y;
+    int head;
+    const Place place = block_place<false>(a, per_tile, &head);
+    if (place.b < 0) return;
+    const Span s = load_span(a, place.b);
+    const int64_t token0 = int64_t(place.tile) * per_tile;
     const int tokens = int(min(int64_t(per_tile), s.rows - token0));
     const int end = int(seen(s, a.causal, token0 + tokens - 1));
     const int tiles = (end + kTile - 1) / kTile, keys = int(s.keys);
@@ -337,11 +336,11 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int b = find_sequence(a.key_offsets, a.batch, kTile, blockIdx.x);
-    const Span s = load_span(a, b);
-    const int64_t key0 = (int64_t(blockIdx.x) - (a.key_offsets[b] / kTile + b)) * kTile;
-    if (key0 < 0 || key0 >= s.slot) return;
-    const int head = blockIdx.y;
+    int head;
+    const Place place = block_place<true>(a, kTile, &head);
+    if (place.b < 0) return;
+    const Span s = load_span(a, place.b);
+    const int64_t key0 = int64_t(place.tile) * kTile;
     const int per_tile = kTile / a.group, full_rows = per_tile * a.group;
     // tiles of rows from the one that holds the first token that sees key0
     const int64_t first = a.causal ? max(int64_t(0), key0 + s.rows - s.keys) / per_tile : 0;
@@ -580,12 +579,12 @@ fmd_status launch(const Maps& maps, const Attn& a, cudaStream_t s) {
     if (st != FMD_OK) return st;
     if (a.dq != nullptr && a.rows > 0) {
         const int64_t tiles = tile_bound(a.rows, a.batch, kTile / a.group);
-        query_gradient_kernel<KS><<<dim3(unsigned(tiles), unsigned(a.hk)), kThreads, query_bytes, s>>>(maps, a);
+        query_gradient_kernel<KS><<<unsigned(tiles * a.hk), kThreads, query_bytes, s>>>(maps, a);
         if ((st = check_launch()) != FMD_OK) return st;
     }
     if (a.dk != nullptr && a.keys > 0) {
         const int64_t tiles = tile_bound(a.keys, a.batch, kTile);
-        key_gradient_kernel<KS><<<dim3(unsigned(tiles), unsigned(a.hk)), kThreads, key_bytes, s>>>(maps, a);
+        key_gradient_kernel<KS><<<unsigned(tiles * a.hk), kThreads, key_bytes, s>>>(maps, a);
         st = check_launch();
     }
     return st;

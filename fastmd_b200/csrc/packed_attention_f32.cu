@@ -148,13 +148,12 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int64_t index = gridDim.x - 1 - blockIdx.x;  // the longest rows of a causal sequence first
     const int per_tile = kTile / a.group;
-    const int b = find_sequence(a.offsets, a.batch, per_tile, index);
-    const Span s = load_span(a, b);
-    const int64_t token0 = (index - (a.offsets[b] / per_tile + b)) * per_tile;
-    if (token0 < 0 || token0 >= s.rows) return;
-    const int head = blockIdx.y;
+    int head;
+    const Place place = block_place<false>(a, per_tile, &head);
+    if (place.b < 0) return;
+    const Span s = load_span(a, place.b);
+    const int64_t token0 = int64_t(place.tile) * per_tile;
     const int tokens = int(min(int64_t(per_tile), s.rows - token0));
     int end = int(seen(s, a.causal, token0 + tokens - 1)), tiles = (end + kTile - 1) / kTile, from = 0;
     if (SPLIT) {  // a range of the key tiles; from here on everything counts from its first key
@@ -456,13 +455,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int64_t index = gridDim.x - 1 - blockIdx.x;
     const int per_tile = kTile / a.group;
-    const int b = find_sequence(a.offsets, a.batch, per_tile, index);
-    const Span s = load_span(a, b);
-    const int64_t token0 = (index - (a.offsets[b] / per_tile + b)) * per_tile;
-    if (token0 < 0 || token0 >= s.rows) return;
-    const int head = blockIdx.y;
+    int head;
+    const Place place = block_place<false>(a, per_tile, &head);
+    if (place.b < 0) return;
+    const Span s = load_span(a, place.b);
+    const int64_t token0 = int64_t(place.tile) * per_tile;
     const int tokens = int(min(int64_t(per_tile), s.rows - token0));
     const int end = int(seen(s, a.causal, token0 + tokens - 1));
     const int tiles = (end + kStream - 1) / kStream, keys = int(s.keys);
@@ -616,11 +614,11 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int b = find_sequence(a.key_offsets, a.batch, kTile, blockIdx.x);
-    const Span s = load_span(a, b);
-    const int64_t key0 = (int64_t(blockIdx.x) - (a.key_offsets[b] / kTile + b)) * kTile;
-    if (key0 < 0 || key0 >= s.slot) return;
-    const int head = blockIdx.y;
+    int head;
+    const Place place = block_place<true>(a, kTile, &head);
+    if (place.b < 0) return;
+    const Span s = load_span(a, place.b);
+    const int64_t key0 = int64_t(place.tile) * kTile;
     const int per_tile = kStream / a.group, full_rows = per_tile * a.group;
     const int64_t first = a.causal ? max(int64_t(0), key0 + s.rows - s.keys) / per_tile : 0;
     const int64_t count = (s.rows + per_tile - 1) / per_tile;
@@ -868,7 +866,7 @@ fmd_status launch_forward(const Maps& maps, const Attn& a, int splits, cudaStrea
     const void* kernel = splits > 1 ? (const void*)forward_kernel<KS, true> : (const void*)forward_kernel<KS, false>;
     const fmd_status st = grant_dynamic_smem(kernel, kForwardBytes, true);
     if (st != FMD_OK) return st;
-    const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kTile / a.group)), unsigned(a.hk), unsigned(splits));
+    const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kTile / a.group) * a.hk), 1, unsigned(splits));
     if (splits > 1) forward_kernel<KS, true><<<grid, kThreads, kForwardBytes, s>>>(maps, a);
     else forward_kernel<KS, false><<<grid, kThreads, kForwardBytes, s>>>(maps, a);
     return check_launch();
@@ -880,12 +878,12 @@ fmd_status launch_backward(const Maps& maps, const Attn& a, const Own& own, cuda
     if (st == FMD_OK) st = grant_dynamic_smem((const void*)key_gradient_kernel<KS>, kBackwardBytes, true);
     if (st != FMD_OK) return st;
     if (a.dq != nullptr && a.rows > 0) {
-        const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kTile / a.group)), unsigned(a.hk));
+        const unsigned grid = unsigned(tile_bound(a.rows, a.batch, kTile / a.group) * a.hk);
         query_gradient_kernel<KS><<<grid, kThreads, kBackwardBytes, s>>>(maps, a, own);
         if ((st = check_launch()) != FMD_OK) return st;
     }
     if (a.dk != nullptr && a.keys > 0) {
-        const dim3 grid(unsigned(tile_bound(a.keys, a.batch, kTile)), unsigned(a.hk));
+        const unsigned grid = unsigned(tile_bound(a.keys, a.batch, kTile) * a.hk);
         key_gradient_kernel<KS><<<grid, kThreads, kBackwardBytes, s>>>(maps, a, own);
         st = check_launch();
     }

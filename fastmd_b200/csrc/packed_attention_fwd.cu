@@ -77,14 +77,12 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    // the longest rows of a causal sequence are its last: they go first
-    const int64_t index = gridDim.x - 1 - blockIdx.x;
     const int per_tile = kTile / a.group, per_block = NT * per_tile;
-    const int b = find_sequence(a.offsets, a.batch, per_block, index);
-    const Span s = load_span(a, b);
-    const int64_t token0 = (index - (a.offsets[b] / per_block + b)) * per_block;
-    if (token0 < 0 || token0 >= s.rows) return;
-    const int head = blockIdx.y;
+    int head;
+    const Place place = block_place<false>(a, per_block, &head);
+    if (place.b < 0) return;
+    const Span s = load_span(a, place.b);
+    const int64_t token0 = int64_t(place.tile) * per_block;
     int tokens[NT], ends[NT], counts[NT];  // tokens of each tile, the keys its last one sees, key tiles
     int last = 0;
 #pragma unroll
@@ -361,7 +359,7 @@ fmd_status launch(const Maps& maps, const Attn& a, int splits, cudaStream_t s) {
     if (st != FMD_OK) return st;
     const int64_t tiles = tile_bound(a.rows, a.batch, NT * (kTile / a.group));
     forward_kernel<KS, NT, SPLIT>
-        <<<dim3(unsigned(tiles), unsigned(a.hk), unsigned(splits)), S::kThreads, S::kBytes, s>>>(maps, a);
+        <<<dim3(unsigned(tiles * a.hk), 1, unsigned(splits)), S::kThreads, S::kBytes, s>>>(maps, a);
     return check_launch();
 }
 

@@ -10,7 +10,7 @@
 
 namespace fmd {
 
-constexpr int kTile = 128;                           // rows of a tile: the M of every product
+constexpr int kTile = kRowTile;                      // the M of every product
 constexpr uint32_t kPanelBytes = kTile * 128;        // 128 rows x 64 bfloat16
 constexpr uint32_t kPanelStep = kPanelBytes >> 4;    // in descriptor units of 16 bytes
 

@@ -101,15 +101,16 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Attn a) {
     float* vs = ks + 64 * (kDim + 4);
     float* ps = vs + 64 * (kDim + 4);
     const int per_tile = kM / a.group;
-    const int b = find_sequence(a.offsets, a.batch, per_tile, blockIdx.x);
-    const Span s = load_span(a, b);
-    const int64_t token0 = (int64_t(blockIdx.x) - (a.offsets[b] / per_tile + b)) * per_tile;
-    if (token0 < 0 || token0 >= s.rows) return;
+    int head;
+    const Place place = block_place<false>(a, per_tile, &head);
+    if (place.b < 0) return;
+    const Span s = load_span(a, place.b);
+    const int64_t token0 = int64_t(place.tile) * per_tile;
     const int tokens = int(min(int64_t(per_tile), s.rows - token0)), rows = tokens * a.group;
-    const Rows at{s.row0 + token0, a.group, int(blockIdx.y) * a.group, a.hq};
+    const Rows at{s.row0 + token0, a.group, head * a.group, a.hq};
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const float* kp = static_cast<const float*>(a.k) + s.key0 * a.k_row + blockIdx.y * a.k_head;
-    const float* vp = static_cast<const float*>(a.v) + s.key0 * a.v_row + blockIdx.y * a.v_head;
+    const float* kp = static_cast<const float*>(a.k) + s.key0 * a.k_row + head * a.k_head;
+    const float* vp = static_cast<const float*>(a.v) + s.key0 * a.v_row + head * a.v_head;
     load_tile(qs, static_cast<const float*>(a.q), rows, a.dim,
                      [&](int r) { return at.at(r, a.q_row, a.q_head); });
     int64_t limit[4];
@@ -194,15 +195,16 @@ __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const Attn a) 
     float* vs = ks + 64 * (kDim + 4);
     float* ds = vs + 64 * (kDim + 4);
     const int per_tile = kM / a.group;
-    const int b = find_sequence(a.offsets, a.batch, per_tile, blockIdx.x);
-    const Span s = load_span(a, b);
-    const int64_t token0 = (int64_t(blockIdx.x) - (a.offsets[b] / per_tile + b)) * per_tile;
-    if (token0 < 0 || token0 >= s.rows) return;
+    int head;
+    const Place place = block_place<false>(a, per_tile, &head);
+    if (place.b < 0) return;
+    const Span s = load_span(a, place.b);
+    const int64_t token0 = int64_t(place.tile) * per_tile;
     const int tokens = int(min(int64_t(per_tile), s.rows - token0)), rows = tokens * a.group;
-    const Rows at{s.row0 + token0, a.group, int(blockIdx.y) * a.group, a.hq};
+    const Rows at{s.row0 + token0, a.group, head * a.group, a.hq};
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const float* kp = static_cast<const float*>(a.k) + s.key0 * a.k_row + blockIdx.y * a.k_head;
-    const float* vp = static_cast<const float*>(a.v) + s.key0 * a.v_row + blockIdx.y * a.v_head;
+    const float* kp = static_cast<const float*>(a.k) + s.key0 * a.k_row + head * a.k_head;
+    const float* vp = static_cast<const float*>(a.v) + s.key0 * a.v_row + head * a.v_head;
     load_tile(qs, static_cast<const float*>(a.q), rows, a.dim,
                      [&](int r) { return at.at(r, a.q_row, a.q_head); });
     load_tile(gs, static_cast<const float*>(a.g), rows, a.dim,
@@ -263,15 +265,16 @@ __global__ void __launch_bounds__(kThreads) key_gradient_kernel(const Attn a) {
     float* ds = ps + 64 * (64 + 4);
     __shared__ float lse2[64], delta[64];
     __shared__ int64_t limit[64];
-    const int b = find_sequence(a.key_offsets, a.batch, kN, blockIdx.x);
-    const Span s = load_span(a, b);
-    const int64_t n0 = (int64_t(blockIdx.x) - (a.key_offsets[b] / kN + b)) * kN;
-    if (n0 < 0 || n0 >= s.slot) return;
+    int head;
+    const Place place = block_place<true>(a, kN, &head);
+    if (place.b < 0) return;
+    const Span s = load_span(a, place.b);
+    const int64_t n0 = int64_t(place.tile) * kN;
     const int n = int(max(int64_t(0), min(int64_t(kN), s.keys - n0)));
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    load_tile(ks, static_cast<const float*>(a.k) + (s.key0 + n0) * a.k_row + blockIdx.y * a.k_head, n, a.dim,
+    load_tile(ks, static_cast<const float*>(a.k) + (s.key0 + n0) * a.k_row + head * a.k_head, n, a.dim,
                      [&](int r) { return r * a.k_row; });
-    load_tile(vs, static_cast<const float*>(a.v) + (s.key0 + n0) * a.v_row + blockIdx.y * a.v_head, n, a.dim,
+    load_tile(vs, static_cast<const float*>(a.v) + (s.key0 + n0) * a.v_row + head * a.v_head, n, a.dim,
                      [&](int r) { return r * a.v_row; });
     float dk[4][kDim / 16] = {}, dv[4][kDim / 16] = {};
     const int per_tile = kM / a.group;
@@ -280,7 +283,7 @@ __global__ void __launch_bounds__(kThreads) key_gradient_kernel(const Attn a) {
     const int64_t first = a.causal ? max(int64_t(0), n0 + s.rows - s.keys) : 0;
     for (int64_t token0 = n > 0 ? first / per_tile * per_tile : s.rows; token0 < s.rows; token0 += per_tile) {
         const int tokens = int(min(int64_t(per_tile), s.rows - token0)), rows = tokens * a.group;
-        const Rows at{s.row0 + token0, a.group, int(blockIdx.y) * a.group, a.hq};
+        const Rows at{s.row0 + token0, a.group, head * a.group, a.hq};
         __syncthreads();
         load_tile(qs, static_cast<const float*>(a.q), rows, a.dim,
                          [&](int r) { return at.at(r, a.q_row, a.q_head); });
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(kThreads) key_gradient_kernel(const Attn a) {
     for (int i = 0; i < 4; ++i) {
         const int key = ty + 16 * i;
         if (key >= out_rows) continue;
-        const int64_t flat = ((s.key0 + n0 + key) * a.hk + blockIdx.y) * a.dim;
+        const int64_t flat = ((s.key0 + n0 + key) * a.hk + head) * a.dim;
 #pragma unroll
         for (int c = 0; c < kDim / 16; ++c) {
             const int col = 2 * tx + 32 * (c / 2) + c % 2;
@@ -335,7 +338,7 @@ fmd_status attention_forward_simt(const Attn& a, int splits, cudaStream_t s) {
     const void* kernel = splits > 1 ? (const void*)forward_kernel<true> : (const void*)forward_kernel<false>;
     const fmd_status st = grant_dynamic_smem(kernel, bytes);
     if (st != FMD_OK) return st;
-    const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kM / a.group)), unsigned(a.hk), unsigned(splits));
+    const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kM / a.group) * a.hk), 1, unsigned(splits));
     if (splits > 1) forward_kernel<true><<<grid, kThreads, bytes, s>>>(a);
     else forward_kernel<false><<<grid, kThreads, bytes, s>>>(a);
     return check_launch();
@@ -347,12 +350,12 @@ fmd_status attention_backward_simt(const Attn& a, cudaStream_t s) {
     if (st == FMD_OK) st = grant_dynamic_smem((const void*)key_gradient_kernel, bytes);
     if (st != FMD_OK) return st;
     if (a.dq != nullptr && a.rows > 0) {
-        const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kM / a.group)), unsigned(a.hk));
+        const unsigned grid = unsigned(tile_bound(a.rows, a.batch, kM / a.group) * a.hk);
         query_gradient_kernel<<<grid, kThreads, bytes, s>>>(a);
         if ((st = check_launch()) != FMD_OK) return st;
     }
     if (a.dk != nullptr && a.keys > 0) {
-        const dim3 grid(unsigned(tile_bound(a.keys, a.batch, kN)), unsigned(a.hk));
+        const unsigned grid = unsigned(tile_bound(a.keys, a.batch, kN) * a.hk);
         key_gradient_kernel<<<grid, kThreads, bytes, s>>>(a);
         st = check_launch();
     }
