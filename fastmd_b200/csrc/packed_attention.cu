@@ -158,7 +158,7 @@ Plan plan(const Attn& a, int type) {
     const bool planes = type == FMD_F32 && a.dim <= kPlanesDim;
     // one block an SM by its shared memory, or two
     if (type == FMD_BF16) p.splits = attention_splits_mma(a);
-    else p.splits = key_splits(a, (planes ? 128 : 64) / a.group, kNumSMs, 256);
+    else p.splits = key_splits(a, (planes ? 128 : 64) / a.group, kNumSMs, planes ? 128 : 64);
     if (planes) p.planes = attention_planes_bytes(a, false);
     p.bytes = p.planes + (p.splits > 1 ? size_t(p.splits) * a.rows * a.hq * (a.dim + 1) * sizeof(float) : 0);
     return p;

@@ -178,15 +178,25 @@ __device__ __forceinline__ int64_t seen(const Span& s, bool causal, int64_t t) {
     return causal ? min(max(t + 1 + s.keys - s.rows, int64_t(0)), s.keys) : s.keys;
 }
 
-// Splits of the keys in the forward pass, where the tiles of `per_tile` tokens do not fill `blocks` places: the host
-// goes by the mean length of a sequence's slot (the lengths are on the device), and a split has `least` keys at least.
-inline int key_splits(const Attn& a, int per_tile, int blocks, int least) {
+// Splits of the keys in the forward pass, for `blocks` places and key tiles of `tile`: the number that ends first when a
+// block takes two tiles' time besides its own and the join as much again. The host goes by the mean length of a
+// sequence's slot (the lengths are on the device); where the tiles of rows fill the places four times over they are not
+// split.
+inline int key_splits(const Attn& a, int per_tile, int blocks, int tile) {
     const int64_t tiles = tile_bound(a.rows, a.batch, per_tile) * a.hk;
-    if (tiles == 0 || a.batch == 0) return 1;
-    int64_t splits = blocks / tiles;
-    const int64_t most = a.keys / a.batch / least;
-    if (splits > most) splits = most;
-    return splits < 1 ? 1 : splits > 64 ? 64 : int(splits);
+    if (tiles == 0 || a.batch == 0 || tiles >= 4 * int64_t(blocks)) return 1;
+    const int64_t keys = (a.keys / a.batch + tile - 1) / tile;  // key tiles of a mean sequence
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int64_t splits = 1; splits <= 64 && (splits == 1 || 2 * splits <= keys); ++splits) {
+        const int64_t rounds = (tiles * splits + blocks - 1) / blocks;
+        const int64_t time = rounds * ((keys + splits - 1) / splits + 2) + (splits > 1 ? 2 : 0);
+        if (time < least) {
+            least = time;
+            best = int(splits);
+        }
+    }
+    return best;
 }
 
 // bfloat16

@@ -363,11 +363,13 @@ fmd_status launch(const Maps& maps, const Attn& a, int splits, cudaStream_t s) {
     return check_launch();
 }
 
+// Two tiles a block, which read each key tile once, where that still gives every SM a block; else one, two blocks an SM.
+bool two_tiles(const Attn& a) { return tile_bound(a.rows, a.batch, 2 * (kTile / a.group)) * a.hk >= kNumSMs; }
+
 template <int KS>
 fmd_status launch(const Maps& maps, const Attn& a, int splits, cudaStream_t s) {
     if (splits > 1) return launch<KS, 1, true>(maps, a, splits, s);
-    const bool two = tile_bound(a.rows, a.batch, 2 * (kTile / a.group)) * a.hk >= kNumSMs;
-    return two ? launch<KS, 2, false>(maps, a, 1, s) : launch<KS, 1, false>(maps, a, 1, s);
+    return two_tiles(a) ? launch<KS, 2, false>(maps, a, 1, s) : launch<KS, 1, false>(maps, a, 1, s);
 }
 
 }  // namespace
@@ -403,6 +405,6 @@ fmd_status attention_forward_mma(const Attn& a, int splits, cudaStream_t s) {
          : a.dim <= 96 ? launch<6>(maps, a, splits, s) : launch<8>(maps, a, splits, s);
 }
 
-int attention_splits_mma(const Attn& a) { return key_splits(a, kTile / a.group, 2 * kNumSMs, 2 * kTile); }
+int attention_splits_mma(const Attn& a) { return two_tiles(a) ? 1 : key_splits(a, kTile / a.group, 2 * kNumSMs, kTile); }
 
 }  // namespace fmd

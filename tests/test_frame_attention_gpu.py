@@ -1,0 +1,90 @@
+"""The example model of logged frames: its packed form, its step form and plain torch operations agree (GPU)."""
+import importlib.util
+
+import pytest
+import torch
+
+from conftest import ROOT
+
+gpu = pytest.mark.gpu
+
+
+def load():
+    spec = importlib.util.spec_from_file_location("frame_attention", ROOT / "examples" / "frame_attention.py")
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def test_the_made_up_log_on_the_host():
+    frames, steps, offsets = load().made_up_log(5, 9, 3, device="cpu")
+    assert frames.shape == (int(offsets[-1]), 3) and steps.shape == (int(offsets[-1]),)
+    assert all(int(steps[a]) == 0 for a in offsets[:-1]) and int(offsets.diff().max()) <= 9
+
+
+def plain_forward(model, frames, steps, offsets):
+    """The model in 64 bits with elementary operations, a replica at a time."""
+    wide = {n: p.detach().double() for n, p in model.named_parameters()}
+    cos, sin = (t.double() for t in model.table)
+    out = []
+    for a, b in zip(offsets.tolist(), offsets.tolist()[1:]):
+        x = frames[a:b].double() @ wide["embed.weight"].T + wide["embed.bias"]
+        c, s = cos[steps[a:b]][:, None], sin[steps[a:b]][:, None]
+        for i, block in enumerate(model.blocks):
+            w = {n.split(".", 2)[2]: p for n, p in wide.items() if n.startswith(f"blocks.{i}.")}
+            h = torch.nn.functional.layer_norm(x, x.shape[-1:], w["norm_in.weight"], w["norm_in.bias"])
+            q, k, v = (h @ w["qkv.weight"].T).unflatten(1, (-1, block.dim)).split(block.sizes, 1)
+
+            def turned(y, weight):
+                y = y / (y.square().mean(-1, keepdim=True) + 1e-6).sqrt() * weight
+                one, two = y.chunk(2, -1)
+                return torch.cat((one * c - two * s, two * c + one * s), -1)
+
+            q, k = turned(q, w["q_weight"]), turned(k, w["k_weight"])
+            k, v = (t.repeat_interleave(q.shape[1] // t.shape[1], 1) for t in (k, v))
+            score = torch.einsum("ihd,jhd->hij", q, k) * block.dim ** -0.5
+            score = score.masked_fill(torch.ones(b - a, b - a, device=x.device).triu(1).bool(), float("-inf"))
+            x = x + torch.einsum("hij,jhd->ihd", score.softmax(-1), v).flatten(1) @ w["out.weight"].T
+            h = torch.nn.functional.layer_norm(x, x.shape[-1:], w["norm_mlp.weight"], w["norm_mlp.bias"])
+            h = torch.nn.functional.silu(h @ w["mlp.0.weight"].T + w["mlp.0.bias"])
+            x = x + h @ w["mlp.2.weight"].T + w["mlp.2.bias"]
+        out.append(x @ wide["read.weight"].T + wide["read.bias"])
+    return torch.cat(out)
+
+
+@gpu
+def test_packed_steps_and_plain_agree(cuda):
+    """float32: two layers of a few hundred FP32 roundings each, of values of size one, stay below 1e-4."""
+    example = load()
+    torch.manual_seed(1)
+    model = example.FrameModel(4, device="cuda")
+    frames, steps, offsets = example.made_up_log(6, 150, 4)
+    whole = model(frames, steps, offsets).detach()
+    want = plain_forward(model, frames, steps, offsets)
+    assert float((whole.double() - want).abs().max()) <= 1e-4
+    cache = model.new_cache(6, 160)
+    shortest = int(offsets.diff().min())
+    for i in range(shortest):
+        rows = offsets[:-1] + i
+        got = model.step(frames[rows], steps[rows], cache)
+        assert float((got.double() - want[rows]).abs().max()) <= 1e-4
+    assert cache["counts"].tolist() == [shortest] * 6
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_training_lowers_the_loss(cuda, dtype):
+    example = load()
+    torch.manual_seed(2)
+    model = example.FrameModel(4, device="cuda", dtype=getattr(torch, dtype))
+    log = example.made_up_log(8, 100, 4, dtype=getattr(torch, dtype))
+    optimizer = torch.optim.AdamW(model.parameters(), lr=1e-3)
+    losses = []
+    for _ in range(15):
+        optimizer.zero_grad()
+        loss = example.next_frame_loss(model, *log)
+        loss.backward()
+        assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in model.parameters())
+        optimizer.step()
+        losses.append(float(loss.detach()))
+    assert losses[-1] < 0.7 * losses[0]
