@@ -18,59 +18,104 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
         make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// out and lse of the splits of the keys together: out = sum_z exp(lse_z - lse) out_z. A warp per row, four values a
-// lane; with many splits PARTS warps share a row's (their loads are what the time goes to).
-template <typename T, int PARTS>
+// out and lse of the splits of the keys together: out = sum_z exp(lse_z - lse) out_z. Many splits: a block per row, 32
+// threads of four values each, times eight that share the splits (their loads are what the time goes to).
+template <typename T>
 __global__ void __launch_bounds__(kThreads) join_kernel(const Attn a, int splits) {
-    constexpr int kWarps = kThreads / 32;
-    __shared__ float4 sums[kWarps][32];
-    __shared__ float weights[kWarps];
-    const int quad = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % PARTS;
-    const int64_t row = int64_t(blockIdx.x) * (kWarps / PARTS) + warp / PARTS, all = a.rows * a.hq;
+    constexpr int kParts = kThreads / 32;
+    __shared__ float4 sums[kParts][32];
+    __shared__ float weights[kParts];
+    const int quad = threadIdx.x & 31, part = threadIdx.x >> 5;
+    const int64_t row = blockIdx.x, all = a.rows * a.hq;
     float top = -INFINITY, sum = 0.0f;
+    for (int z = quad; z < splits; z += 32) top = fmaxf(top, a.part_lse[z * all + row]);
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+    const float base = top == -INFINITY ? 0.0f : top;
     float4 o = f4_zero();
-    if (row < all) {
-        for (int z = quad; z < splits; z += 32) top = fmaxf(top, a.part_lse[z * all + row]);
-#pragma unroll
-        for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-        const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll 4
-        for (int z = part; z < splits; z += PARTS) {
-            const float lse = a.part_lse[z * all + row];
-            if (lse == -INFINITY) continue;  // a split without keys of this row wrote nothing else
-            const float w = exp2f((lse - base) * kLog2e);
-            sum += w;
-            if (quad * 4 < a.dim) {
-                const float4 v = *reinterpret_cast<const float4*>(a.part + (z * all + row) * a.dim + quad * 4);
-                o = make_float4(fmaf(w, v.x, o.x), fmaf(w, v.y, o.y), fmaf(w, v.z, o.z), fmaf(w, v.w, o.w));
-            }
+    for (int z = part; z < splits; z += kParts) {
+        const float lse = a.part_lse[z * all + row];
+        if (lse == -INFINITY) continue;  // a split without keys of this row wrote nothing else
+        const float w = exp2f((lse - base) * kLog2e);
+        sum += w;
+        if (quad * 4 < a.dim) {
+            const float4 v = *reinterpret_cast<const float4*>(a.part + (z * all + row) * a.dim + quad * 4);
+            o = make_float4(fmaf(w, v.x, o.x), fmaf(w, v.y, o.y), fmaf(w, v.z, o.z), fmaf(w, v.w, o.w));
         }
     }
-    if (PARTS > 1) {
-        sums[warp][quad] = o;
-        if (quad == 0) weights[warp] = sum;
-        __syncthreads();
-        if (part > 0) return;
+    sums[part][quad] = o;
+    if (quad == 0) weights[part] = sum;
+    __syncthreads();
+    if (part > 0) return;
 #pragma unroll
-        for (int i = 1; i < PARTS; ++i) {
-            o = f4_add(o, sums[warp + i][quad]);
-            sum += weights[warp + i];
-        }
+    for (int i = 1; i < kParts; ++i) {
+        o = f4_add(o, sums[i][quad]);
+        sum += weights[i];
     }
-    if (row >= all) return;
     const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
     if (quad * 4 < a.dim)
         store4(static_cast<T*>(a.out) + row * a.dim + quad * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     if (quad == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? -INFINITY : top + logf(sum);
 }
 
+// The same for few splits: a thread per row and four values.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_few_kernel(const Attn a, int splits) {
+    const int quads = a.dim / 4;
+    const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x, all = a.rows * a.hq, row = i / quads;
+    const int quad = int(i - row * quads);
+    if (row >= all) return;
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll 4
+    for (int z = 0; z < splits; ++z) top = fmaxf(top, a.part_lse[z * all + row]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float4 o = f4_zero();
+#pragma unroll 4
+    for (int z = 0; z < splits; ++z) {
+        const float lse = a.part_lse[z * all + row];
+        if (lse == -INFINITY) continue;
+        const float w = exp2f((lse - base) * kLog2e);
+        const float4 v = *reinterpret_cast<const float4*>(a.part + (z * all + row) * a.dim + quad * 4);
+        sum += w;
+        o = make_float4(fmaf(w, v.x, o.x), fmaf(w, v.y, o.y), fmaf(w, v.z, o.z), fmaf(w, v.w, o.w));
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+    store4(static_cast<T*>(a.out) + row * a.dim + quad * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    if (quad == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? -INFINITY : top + logf(sum);
+}
+
 template <typename T>
 fmd_status join(const Attn& a, int splits, cudaStream_t s) {
-    const int parts = splits >= 16 ? 8 : 1, rows_each = kThreads / 32 / parts;
-    const int64_t blocks = (a.rows * a.hq + rows_each - 1) / rows_each;
+    const bool many = splits >= 16;
+    const int64_t all = a.rows * a.hq, blocks = many ? all : (all * (a.dim / 4) + kThreads - 1) / kThreads;
     if (blocks > INT32_MAX) return FMD_ERR_UNSUPPORTED;
-    if (parts == 8) join_kernel<T, 8><<<unsigned(blocks), kThreads, 0, s>>>(a, splits);
-    else join_kernel<T, 1><<<unsigned(blocks), kThreads, 0, s>>>(a, splits);
+    if (many) join_kernel<T><<<unsigned(blocks), kThreads, 0, s>>>(a, splits);
+    else join_few_kernel<T><<<unsigned(blocks), kThreads, 0, s>>>(a, splits);
+    return check_launch();
+}
+
+// out[i] = the sum of the splits' parts, four values a thread; y: a second pair of arrays.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) add_kernel(const float* part0, const float* part1, T* out0, T* out1,
+                                                       int64_t values, int splits) {
+    const float* part = blockIdx.y ? part1 : part0;
+    T* out = blockIdx.y ? out1 : out0;
+    const int64_t i = (int64_t(blockIdx.x) * kThreads + threadIdx.x) * 4;
+    if (i >= values) return;
+    float4 sum = f4_zero();
+#pragma unroll 4
+    for (int z = 0; z < splits; ++z) sum = f4_add(sum, *reinterpret_cast<const float4*>(part + z * values + i));
+    store4(out + i, sum);
+}
+
+template <typename T>
+fmd_status add(const float* part0, const float* part1, void* out0, void* out1, int64_t values, int splits,
+               cudaStream_t s) {
+    const int64_t blocks = (values / 4 + kThreads - 1) / kThreads;
+    if (blocks > INT32_MAX) return FMD_ERR_UNSUPPORTED;
+    add_kernel<T><<<dim3(unsigned(blocks), out1 != nullptr ? 2 : 1), kThreads, 0, s>>>(
+        part0, part1, static_cast<T*>(out0), static_cast<T*>(out1), values, splits);
     return check_launch();
 }
 
@@ -166,8 +211,25 @@ Plan plan(const Attn& a, int type) {
 
 size_t delta_bytes(const Attn& a) { return (size_t(a.rows) * a.hq * sizeof(float) + 15) & ~size_t(15); }
 
-size_t backward_bytes(const Attn& a, int type) {
-    return delta_bytes(a) + (type == FMD_F32 && a.dim <= kPlanesDim ? attention_planes_bytes(a, true) : 0);
+// How the backward pass runs, and its workspace: delta, planes, then the splits' parts.
+struct BackwardPlan {
+    BackwardSplits splits;
+    size_t delta, planes, dq, dkv, bytes;
+};
+
+BackwardPlan backward_plan(const Attn& a, int type, bool dq, bool dkv) {
+    BackwardPlan p{{1, 1}, delta_bytes(a), 0, 0, 0, 0};
+    const bool planes = type == FMD_F32 && a.dim <= kPlanesDim;
+    if (planes) p.planes = attention_planes_bytes(a, true);
+    if (type == FMD_BF16 || planes) {
+        const int stream = planes ? 64 : 128;  // rows of a streamed tile
+        if (dq) p.splits.queries = key_splits(a, 128 / a.group, kNumSMs, stream);
+        if (dkv) p.splits.keys = row_splits(a, stream / a.group, kNumSMs, 128);
+    }
+    if (p.splits.queries > 1) p.dq = size_t(p.splits.queries) * a.rows * a.hq * a.dim * sizeof(float);
+    if (p.splits.keys > 1) p.dkv = size_t(p.splits.keys) * a.keys * a.hk * a.dim * sizeof(float);
+    p.bytes = p.delta + p.planes + p.dq + 2 * p.dkv;
+    return p;
 }
 
 }  // namespace
@@ -181,7 +243,7 @@ fmd_status fmd_packed_attention_workspace_bytes(const fmd_attention* problem, in
     Attn a;
     if (problem == nullptr || bytes == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     const fmd_status st = check(*problem, a);
-    if (st == FMD_OK) *bytes = backward ? backward_bytes(a, problem->type) : plan(a, problem->type).bytes;
+    if (st == FMD_OK) *bytes = backward ? backward_plan(a, problem->type, true, true).bytes : plan(a, problem->type).bytes;
     return st;
 }
 
@@ -219,8 +281,8 @@ fmd_status fmd_packed_attention_bwd(const fmd_attention* problem, const void* ou
     if (st != FMD_OK) return st;
     if ((dk == nullptr) != (dv == nullptr)) return FMD_ERR_INVALID_ARGUMENT;
     if (a.rows > 0 && (out == nullptr || lse == nullptr || g == nullptr)) return FMD_ERR_INVALID_ARGUMENT;
-    const size_t bytes = backward_bytes(a, problem->type);
-    if (workspace_bytes < bytes || (bytes > 0 && workspace == nullptr)) return FMD_ERR_WORKSPACE;
+    const BackwardPlan p = backward_plan(a, problem->type, dq != nullptr, dk != nullptr);
+    if (workspace_bytes < p.bytes || (p.bytes > 0 && workspace == nullptr)) return FMD_ERR_WORKSPACE;
     if ((a.rows > 0 && (!rows16(g, g_row, g_head, problem->type == FMD_F32 ? 4 : 2) || !aligned16(out))) ||
         !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(workspace))
         return FMD_ERR_UNSUPPORTED;
@@ -243,9 +305,22 @@ fmd_status fmd_packed_attention_bwd(const fmd_attention* problem, const void* ou
         else delta_kernel<__nv_bfloat16><<<unsigned(blocks), kThreads, 0, s>>>(a, glse, delta);
         if ((st = check_launch()) != FMD_OK) return st;
     }
-    if (problem->type == FMD_BF16) return attention_backward_mma(a, s);
-    if (a.dim <= kPlanesDim) return attention_backward_planes(a, static_cast<char*>(workspace) + delta_bytes(a), s);
-    return attention_backward_simt(a, s);
+    char* at = static_cast<char*>(workspace) + p.delta;
+    a.part = reinterpret_cast<float*>(at + p.planes);
+    a.part_dk = reinterpret_cast<float*>(at + p.planes + p.dq);
+    a.part_dv = reinterpret_cast<float*>(at + p.planes + p.dq + p.dkv);
+    if (problem->type == FMD_BF16) st = attention_backward_mma(a, p.splits, s);
+    else if (a.dim <= kPlanesDim) st = attention_backward_planes(a, p.splits, at, s);
+    else st = attention_backward_simt(a, s);
+    const int64_t q_values = a.rows * a.hq * a.dim, k_values = a.keys * a.hk * a.dim;
+    const bool bf16 = problem->type == FMD_BF16;
+    if (st == FMD_OK && p.splits.queries > 1 && q_values > 0)
+        st = bf16 ? add<__nv_bfloat16>(a.part, nullptr, dq, nullptr, q_values, p.splits.queries, s)
+                  : add<float>(a.part, nullptr, dq, nullptr, q_values, p.splits.queries, s);
+    if (st == FMD_OK && p.splits.keys > 1 && k_values > 0)
+        st = bf16 ? add<__nv_bfloat16>(a.part_dk, a.part_dv, dk, dv, k_values, p.splits.keys, s)
+                  : add<float>(a.part_dk, a.part_dv, dk, dv, k_values, p.splits.keys, s);
+    return st;
 }
 
 }  // extern "C"

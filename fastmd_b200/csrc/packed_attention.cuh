@@ -34,8 +34,10 @@ struct Attn {
     void* dq;           // [rows, hq, dim] contiguous
     void* dk;           // [keys, hk, dim] contiguous
     void* dv;
-    float* part;        // [splits, rows, hq, dim] and
-    float* part_lse;    // [splits, rows, hq]: the splits of the keys, workspace
+    float* part;        // [splits, rows, hq, dim]: outputs, or gradients of q, of the splits of the keys (workspace)
+    float* part_lse;    // [splits, rows, hq]
+    float* part_dk;     // [splits, keys, hk, dim]: gradients of the splits of the rows (workspace)
+    float* part_dv;
     const int64_t* offsets;      // [batch + 1] tokens
     const int64_t* key_offsets;  // [batch + 1]
     const int64_t* key_counts;   // [batch] or null: the whole slot
@@ -178,19 +180,16 @@ __device__ __forceinline__ int64_t seen(const Span& s, bool causal, int64_t t) {
     return causal ? min(max(t + 1 + s.keys - s.rows, int64_t(0)), s.keys) : s.keys;
 }
 
-// Splits of the keys in the forward pass, for `blocks` places and key tiles of `tile`: the number that ends first when a
-// block takes two tiles' time besides its own and the join as much again. The host goes by the mean length of a
-// sequence's slot (the lengths are on the device); where the tiles of rows fill the places four times over they are not
-// split.
-inline int key_splits(const Attn& a, int per_tile, int blocks, int tile) {
-    const int64_t tiles = tile_bound(a.rows, a.batch, per_tile) * a.hk;
-    if (tiles == 0 || a.batch == 0 || tiles >= 4 * int64_t(blocks)) return 1;
-    const int64_t keys = (a.keys / a.batch + tile - 1) / tile;  // key tiles of a mean sequence
+// Splits of the axis that blocks walk along, for `blocks` places and `tiles` blocks of `length` steps each: the number
+// that ends first when a block takes two steps' time besides its own and adding up the splits as much again. Where the
+// blocks fill the places four times over they are not split.
+inline int split_count(int64_t tiles, int64_t length, int blocks) {
+    if (tiles == 0 || tiles >= 4 * int64_t(blocks)) return 1;
     int best = 1;
     int64_t least = INT64_MAX;
-    for (int64_t splits = 1; splits <= 64 && (splits == 1 || 2 * splits <= keys); ++splits) {
+    for (int64_t splits = 1; splits <= 64 && (splits == 1 || 2 * splits <= length); ++splits) {
         const int64_t rounds = (tiles * splits + blocks - 1) / blocks;
-        const int64_t time = rounds * ((keys + splits - 1) / splits + 2) + (splits > 1 ? 2 : 0);
+        const int64_t time = rounds * ((length + splits - 1) / splits + 2) + (splits > 1 ? 2 : 0);
         if (time < least) {
             least = time;
             best = int(splits);
@@ -199,14 +198,32 @@ inline int key_splits(const Attn& a, int per_tile, int blocks, int tile) {
     return best;
 }
 
+// Of the keys, for tiles of `per_tile` tokens. The host goes by the mean length of a sequence's slot: the lengths are on
+// the device.
+inline int key_splits(const Attn& a, int per_tile, int blocks, int tile) {
+    if (a.batch == 0) return 1;
+    return split_count(tile_bound(a.rows, a.batch, per_tile) * a.hk, (a.keys / a.batch + tile - 1) / tile, blocks);
+}
+
+// Of the rows, for tiles of `tile` keys that walk over tiles of `per_tile` tokens.
+inline int row_splits(const Attn& a, int per_tile, int blocks, int tile) {
+    if (a.batch == 0) return 1;
+    return split_count(tile_bound(a.keys, a.batch, tile) * a.hk, (a.rows / a.batch + per_tile - 1) / per_tile, blocks);
+}
+
+// Blocks along z of the two gradient kernels; more than one: each writes its part in FP32.
+struct BackwardSplits {
+    int queries, keys;
+};
+
 // bfloat16
 int attention_splits_mma(const Attn& a);
 fmd_status attention_forward_mma(const Attn& a, int splits, cudaStream_t s);
-fmd_status attention_backward_mma(const Attn& a, cudaStream_t s);
+fmd_status attention_backward_mma(const Attn& a, BackwardSplits splits, cudaStream_t s);
 // float32, dim up to 64: by planes of bfloat16 in a workspace
 size_t attention_planes_bytes(const Attn& a, bool backward);
 fmd_status attention_forward_planes(const Attn& a, int splits, void* planes, cudaStream_t s);
-fmd_status attention_backward_planes(const Attn& a, void* planes, cudaStream_t s);
+fmd_status attention_backward_planes(const Attn& a, BackwardSplits splits, void* planes, cudaStream_t s);
 // float32, wider heads
 fmd_status attention_forward_simt(const Attn& a, int splits, cudaStream_t s);
 fmd_status attention_backward_simt(const Attn& a, cudaStream_t s);

@@ -100,21 +100,30 @@ __device__ __forceinline__ void close_block(Ctrl<KS, KEYS>& ctl, int warp, int32
     if (threadIdx.x == 0 && ctl.abort) raise_flag(flags, FMD_FLAG_WAIT_TIMEOUT);
 }
 
-// Writes 32 FP32 columns of TMEM times `factor` as bfloat16, as far as dim goes. loaded (the same in the whole warp):
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+    st4(p, make_float4(v[0], v[1], v[2], v[3]));
+    st4(p + 4, make_float4(v[4], v[5], v[6], v[7]));
+}
+
+// Writes 32 FP32 columns of TMEM times `factor` as T, as far as dim goes. loaded (the same in the whole warp):
 // the columns hold a result; keep: this row's counts, else it is zeros; real: the row exists.
-__device__ __forceinline__ void store_row(__nv_bfloat16* out, uint32_t tmem, int col0, int dim, float factor,
-                                          bool loaded, bool keep, bool real) {
+template <typename T>
+__device__ __forceinline__ void store_row(T* out, uint32_t tmem, int col0, int dim, float factor, bool loaded, bool keep,
+                                          bool real) {
     float o[32];
     if (loaded) tmem_load32(tmem + col0, o);
     if (!real) return;
 #pragma unroll
     for (int i = 0; i < 32; i += 8) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (loaded && keep)
-            w = make_uint4(pack_bf16(o[i] * factor, o[i + 1] * factor), pack_bf16(o[i + 2] * factor, o[i + 3] * factor),
-                           pack_bf16(o[i + 4] * factor, o[i + 5] * factor),
-                           pack_bf16(o[i + 6] * factor, o[i + 7] * factor));
-        if (col0 + i < dim) *reinterpret_cast<uint4*>(out + col0 + i) = w;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = loaded && keep ? o[i + e] * factor : 0.0f;
+        if (col0 + i < dim) store8(out + col0 + i, v);
     }
 }
 
@@ -160,8 +169,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Span s = load_span(a, place.b);
     const int64_t token0 = int64_t(place.tile) * per_tile;
     const int tokens = int(min(int64_t(per_tile), s.rows - token0));
-    const int end = int(seen(s, a.causal, token0 + tokens - 1));
-    const int tiles = (end + kTile - 1) / kTile, keys = int(s.keys);
+    int end = int(seen(s, a.causal, token0 + tokens - 1)), tiles = (end + kTile - 1) / kTile, from = 0;
+    if (gridDim.z > 1) {  // a range of the key tiles; from here on everything counts from its first key
+        const int share = (tiles + int(gridDim.z) - 1) / int(gridDim.z);
+        from = min(tiles, int(blockIdx.z) * share) * kTile;
+        end = max(0, min(end, min(tiles, int(blockIdx.z + 1) * share) * kTile) - from);
+        tiles = (end + kTile - 1) / kTile;
+    }
+    const int keys = int(s.keys) - from;
     const bool tail = tiles > 0 && keys < tiles * kTile;
     constexpr uint32_t kDp = 256, kDq = 384;  // TMEM columns: two score buffers, dP, dq
 
@@ -179,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             feed(ctl.ring, &ctl.own, abort, 2 * tiles, S::kTileBytes, [&](int i, int slot, uint64_t* bar) {
                 for (int p = 0; p < S::kPanels; ++p)  // k0, v0, k1, v1, ..
                     tma_load_4d(su32(ring + slot * S::kTileBytes + p * kPanelBytes), i & 1 ? &maps.v : &maps.k, bar,
-                                p * 64, 0, head, int(s.key0) + (i >> 1) * kTile);
+                                p * 64, 0, head, int(s.key0) + from + (i >> 1) * kTile);
             });
         }
     } else if (warp == 1) {
@@ -251,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool real = token < tokens;
         const int64_t flat = (s.row0 + token0 + token) * a.hq + head * a.group + r % a.group;
         const float lse = real ? a.lse[flat] : -INFINITY, delta = real ? a.delta[flat] : 0.0f;
-        const int limit = lse != -INFINITY ? int(seen(s, a.causal, token0 + token)) : 0;
+        const int limit = lse != -INFINITY ? min(max(int(seen(s, a.causal, token0 + token)) - from, 0), end) : 0;
         const float base = lse != -INFINITY ? -lse * kLog2e : 0.0f;
         const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), base2 = make_float2(base, base);
         const float2 delta2 = make_float2(-delta, -delta);
@@ -313,9 +328,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
         }
         if (ok) {
-            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.dq) + flat * a.dim;
-            for (int col = 32 * half; col < S::kDim; col += 64)
-                store_row(out, tmem + lanes + kDq, col, a.dim, a.scale, tiles > 0, true, real);
+            const int64_t at = flat * a.dim, part = int64_t(blockIdx.z) * a.rows * a.hq * a.dim;
+            for (int col = 32 * half; col < S::kDim; col += 64) {
+                if (gridDim.z > 1)
+                    store_row(a.part + part + at, tmem + lanes + kDq, col, a.dim, a.scale, tiles > 0, true, real);
+                else
+                    store_row(static_cast<__nv_bfloat16*>(a.dq) + at, tmem + lanes + kDq, col, a.dim, a.scale, tiles > 0,
+                              true, real);
+            }
         }
     }
     close_block(ctl, warp, a.flags);
@@ -343,10 +363,15 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
     const int64_t key0 = int64_t(place.tile) * kTile;
     const int per_tile = kTile / a.group, full_rows = per_tile * a.group;
     // tiles of rows from the one that holds the first token that sees key0
-    const int64_t first = a.causal ? max(int64_t(0), key0 + s.rows - s.keys) / per_tile : 0;
+    int64_t first = a.causal ? max(int64_t(0), key0 + s.rows - s.keys) / per_tile : 0;
     const int64_t all = (s.rows + per_tile - 1) / per_tile;
-    const int tiles = key0 < s.keys ? int(max(int64_t(0), all - first)) : 0;
-    const int last_rows = tiles > 0 ? int(s.rows - (all - 1) * per_tile) * a.group : 0;
+    int tiles = key0 < s.keys ? int(max(int64_t(0), all - first)) : 0;
+    if (gridDim.z > 1) {  // a range of them
+        const int share = (tiles + int(gridDim.z) - 1) / int(gridDim.z), skip = min(tiles, int(blockIdx.z) * share);
+        first += skip;
+        tiles = min(tiles, skip + share) - skip;
+    }
+    const int last_rows = tiles > 0 ? int(min(int64_t(per_tile), s.rows - (first + tiles - 1) * per_tile)) * a.group : 0;
     const bool tail = tiles > 0 && last_rows % 16 != 0 && last_rows < full_rows;
     constexpr uint32_t kDp = 128, kDv = 256, kDk = 384;  // TMEM columns, the scores at 0
 
@@ -561,30 +586,37 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
         if (ok) {
             // the first four warps write dv, the others dk; slot rows that are no keys get zeros
             const int64_t flat = ((s.key0 + key0 + r) * a.hk + head) * a.dim;
-            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(half ? a.dk : a.dv) + flat;
+            const int64_t part = int64_t(blockIdx.z) * a.keys * a.hk * a.dim;
             const bool real = key0 + r < s.slot;
-            for (int col = 0; col < S::kDim; col += 32)
-                store_row(out, tmem + lanes + (half ? kDk : kDv), col, a.dim, half ? a.scale : 1.0f, tiles > 0, r < here,
-                          real);
+            const uint32_t from = tmem + lanes + (half ? kDk : kDv);
+            const float factor = half ? a.scale : 1.0f;
+            for (int col = 0; col < S::kDim; col += 32) {
+                if (gridDim.z > 1)
+                    store_row((half ? a.part_dk : a.part_dv) + part + flat, from, col, a.dim, factor, tiles > 0, r < here,
+                              real);
+                else
+                    store_row(static_cast<__nv_bfloat16*>(half ? a.dk : a.dv) + flat, from, col, a.dim, factor, tiles > 0,
+                              r < here, real);
+            }
         }
     }
     close_block(ctl, warp, a.flags);
 }
 
 template <int KS>
-fmd_status launch(const Maps& maps, const Attn& a, cudaStream_t s) {
+fmd_status launch(const Maps& maps, const Attn& a, BackwardSplits splits, cudaStream_t s) {
     constexpr size_t query_bytes = Shape<KS, false>::kBytes, key_bytes = Shape<KS, true>::kBytes;
     fmd_status st = grant_dynamic_smem((const void*)query_gradient_kernel<KS>, query_bytes, true);
     if (st == FMD_OK) st = grant_dynamic_smem((const void*)key_gradient_kernel<KS>, key_bytes, true);
     if (st != FMD_OK) return st;
     if (a.dq != nullptr && a.rows > 0) {
         const int64_t tiles = tile_bound(a.rows, a.batch, kTile / a.group);
-        query_gradient_kernel<KS><<<unsigned(tiles * a.hk), kThreads, query_bytes, s>>>(maps, a);
+        query_gradient_kernel<KS><<<dim3(unsigned(tiles * a.hk), 1, unsigned(splits.queries)), kThreads, query_bytes, s>>>(maps, a);
         if ((st = check_launch()) != FMD_OK) return st;
     }
     if (a.dk != nullptr && a.keys > 0) {
         const int64_t tiles = tile_bound(a.keys, a.batch, kTile);
-        key_gradient_kernel<KS><<<unsigned(tiles * a.hk), kThreads, key_bytes, s>>>(maps, a);
+        key_gradient_kernel<KS><<<dim3(unsigned(tiles * a.hk), 1, unsigned(splits.keys)), kThreads, key_bytes, s>>>(maps, a);
         st = check_launch();
     }
     return st;
@@ -592,7 +624,7 @@ fmd_status launch(const Maps& maps, const Attn& a, cudaStream_t s) {
 
 }  // namespace
 
-fmd_status attention_backward_mma(const Attn& a, cudaStream_t s) {
+fmd_status attention_backward_mma(const Attn& a, BackwardSplits splits, cudaStream_t s) {
     const DriverCalls& drv = driver_calls();
     if (drv.encode == nullptr || drv.ctx_get_current == nullptr)
         return record_error_text(FMD_ERR_CUDA, "driver entry point cuTensorMapEncodeTiled unavailable", 0);
@@ -608,8 +640,8 @@ fmd_status attention_backward_mma(const Attn& a, cudaStream_t s) {
         if (st == FMD_OK) st = encode_packed(drv, &maps.v, a.v, a.keys, a.hk, 1, a.dim, a.v_row, a.v_head, kTile);
     }
     if (st != FMD_OK) return st;
-    return a.dim <= 32 ? launch<2>(maps, a, s) : a.dim <= 64 ? launch<4>(maps, a, s)
-         : a.dim <= 96 ? launch<6>(maps, a, s) : launch<8>(maps, a, s);
+    return a.dim <= 32 ? launch<2>(maps, a, splits, s) : a.dim <= 64 ? launch<4>(maps, a, splits, s)
+         : a.dim <= 96 ? launch<6>(maps, a, splits, s) : launch<8>(maps, a, splits, s);
 }
 
 }  // namespace fmd

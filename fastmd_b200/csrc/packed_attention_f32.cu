@@ -462,8 +462,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Span s = load_span(a, place.b);
     const int64_t token0 = int64_t(place.tile) * per_tile;
     const int tokens = int(min(int64_t(per_tile), s.rows - token0));
-    const int end = int(seen(s, a.causal, token0 + tokens - 1));
-    const int tiles = (end + kStream - 1) / kStream, keys = int(s.keys);
+    int end = int(seen(s, a.causal, token0 + tokens - 1)), tiles = (end + kStream - 1) / kStream, from = 0;
+    if (gridDim.z > 1) {  // a range of the key tiles; from here on everything counts from its first key
+        const int share = (tiles + int(gridDim.z) - 1) / int(gridDim.z);
+        from = min(tiles, int(blockIdx.z) * share) * kStream;
+        end = max(0, min(end, min(tiles, int(blockIdx.z + 1) * share) * kStream) - from);
+        tiles = (end + kStream - 1) / kStream;
+    }
+    const int keys = int(s.keys) - from;
     const bool tail = tiles > 0 && keys < tiles * kStream;
 
     open_block(ctl, warp);
@@ -474,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             feed(ctl.ring, &ctl.own, abort, 2 * tiles, kSlot3, [&](int i, int slot, uint64_t* bar) {
                 for (int p = 0; p < 3; ++p)  // k0, v0, k1, v1, ..
                     tma_load_4d(su32(ring + slot * kSlot3 + p * kHalfPanel), i & 1 ? &maps.v : &maps.k, bar, 0, 0, head,
-                                int(p * a.keys + s.key0) + (i >> 1) * kStream);
+                                int(p * a.keys + s.key0) + from + (i >> 1) * kStream);
             });
         }
     } else if (warp == 1) {
@@ -537,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool real = token < tokens;
         const int64_t flat = (s.row0 + token0 + token) * a.hq + head * a.group + r % a.group;
         const float lse = real ? a.lse[flat] : -INFINITY, delta = real ? a.delta[flat] : 0.0f;
-        const int limit = lse != -INFINITY ? int(seen(s, a.causal, token0 + token)) : 0;
+        const int limit = lse != -INFINITY ? min(max(int(seen(s, a.causal, token0 + token)) - from, 0), end) : 0;
         const float base = lse != -INFINITY ? -lse * kLog2e : 0.0f;
         const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), base2 = make_float2(base, base);
         const float2 delta2 = make_float2(-delta, -delta);
@@ -595,7 +601,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (ok && tiles > 0 && all(mbar_wait(&ctl.out, uint32_t(tiles - 1) & 1u, abort)))
             drain<kMine>(at_q, dq, 1.0f);
-        if (ok && real) store_values<kMine>(static_cast<float*>(a.dq) + flat * a.dim, dq, a.scale, half * kMine, a.dim);
+        float* out = gridDim.z > 1 ? a.part + int64_t(blockIdx.z) * a.rows * a.hq * a.dim : static_cast<float*>(a.dq);
+        if (ok && real) store_values<kMine>(out + flat * a.dim, dq, a.scale, half * kMine, a.dim);
     }
     close_block(ctl, warp, a.flags);
 }
@@ -620,10 +627,15 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
     const Span s = load_span(a, place.b);
     const int64_t key0 = int64_t(place.tile) * kTile;
     const int per_tile = kStream / a.group, full_rows = per_tile * a.group;
-    const int64_t first = a.causal ? max(int64_t(0), key0 + s.rows - s.keys) / per_tile : 0;
-    const int64_t count = (s.rows + per_tile - 1) / per_tile;
-    const int tiles = key0 < s.keys ? int(max(int64_t(0), count - first)) : 0;
-    const int last_rows = tiles > 0 ? int(s.rows - (count - 1) * per_tile) * a.group : 0;
+    int64_t first = a.causal ? max(int64_t(0), key0 + s.rows - s.keys) / per_tile : 0;
+    const int64_t all = (s.rows + per_tile - 1) / per_tile;
+    int tiles = key0 < s.keys ? int(max(int64_t(0), all - first)) : 0;
+    if (gridDim.z > 1) {  // a range of them
+        const int share = (tiles + int(gridDim.z) - 1) / int(gridDim.z), skip = min(tiles, int(blockIdx.z) * share);
+        first += skip;
+        tiles = min(tiles, skip + share) - skip;
+    }
+    const int last_rows = tiles > 0 ? int(min(int64_t(per_tile), s.rows - (first + tiles - 1) * per_tile)) * a.group : 0;
     const bool tail = tiles > 0 && last_rows % 16 != 0 && last_rows < full_rows;
 
     if (full_rows < kStream && warp >= 4)  // rows of the slots that no copy ever writes are inner rows of the products
@@ -805,7 +817,9 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
         }
         if (ok && tiles > 0 && all(mbar_wait(&ctl.out, 0, abort))) drain_all();
         if (ok && key0 + r < s.slot) {  // slot rows that are no keys get zeros
-            float* row = static_cast<float*>(half ? a.dk : a.dv) + ((s.key0 + key0 + r) * a.hk + head) * a.dim;
+            float* row = gridDim.z > 1 ? (half ? a.part_dk : a.part_dv) + int64_t(blockIdx.z) * a.keys * a.hk * a.dim
+                                       : static_cast<float*>(half ? a.dk : a.dv);
+            row += ((s.key0 + key0 + r) * a.hk + head) * a.dim;
             const bool keep = key0 + r < s.keys;
 #pragma unroll
             for (int i = 0; i < kDim / 32; ++i) {
@@ -873,17 +887,17 @@ fmd_status launch_forward(const Maps& maps, const Attn& a, int splits, cudaStrea
 }
 
 template <int KS>
-fmd_status launch_backward(const Maps& maps, const Attn& a, const Own& own, cudaStream_t s) {
+fmd_status launch_backward(const Maps& maps, const Attn& a, const Own& own, BackwardSplits splits, cudaStream_t s) {
     fmd_status st = grant_dynamic_smem((const void*)query_gradient_kernel<KS>, kBackwardBytes, true);
     if (st == FMD_OK) st = grant_dynamic_smem((const void*)key_gradient_kernel<KS>, kBackwardBytes, true);
     if (st != FMD_OK) return st;
     if (a.dq != nullptr && a.rows > 0) {
-        const unsigned grid = unsigned(tile_bound(a.rows, a.batch, kTile / a.group) * a.hk);
+        const dim3 grid(unsigned(tile_bound(a.rows, a.batch, kTile / a.group) * a.hk), 1, unsigned(splits.queries));
         query_gradient_kernel<KS><<<grid, kThreads, kBackwardBytes, s>>>(maps, a, own);
         if ((st = check_launch()) != FMD_OK) return st;
     }
     if (a.dk != nullptr && a.keys > 0) {
-        const unsigned grid = unsigned(tile_bound(a.keys, a.batch, kTile) * a.hk);
+        const dim3 grid(unsigned(tile_bound(a.keys, a.batch, kTile) * a.hk), 1, unsigned(splits.keys));
         key_gradient_kernel<KS><<<grid, kThreads, kBackwardBytes, s>>>(maps, a, own);
         st = check_launch();
     }
@@ -920,7 +934,7 @@ fmd_status attention_forward_planes(const Attn& a, int splits, void* workspace, 
     return a.dim <= 32 ? launch_forward<2>(maps, a, splits, s) : launch_forward<4>(maps, a, splits, s);
 }
 
-fmd_status attention_backward_planes(const Attn& a, void* workspace, cudaStream_t s) {
+fmd_status attention_backward_planes(const Attn& a, BackwardSplits splits, void* workspace, cudaStream_t s) {
     const DriverCalls& drv = driver_calls();
     if (drv.encode == nullptr || drv.ctx_get_current == nullptr)
         return record_error_text(FMD_ERR_CUDA, "driver entry point cuTensorMapEncodeTiled unavailable", 0);
@@ -943,7 +957,7 @@ fmd_status attention_backward_planes(const Attn& a, void* workspace, cudaStream_
     }
     if (st == FMD_OK) st = planes.launch(s);
     if (st != FMD_OK) return st;
-    return a.dim <= 32 ? launch_backward<2>(maps, a, own, s) : launch_backward<4>(maps, a, own, s);
+    return a.dim <= 32 ? launch_backward<2>(maps, a, own, splits, s) : launch_backward<4>(maps, a, own, splits, s);
 }
 
 }  // namespace fmd

@@ -1103,8 +1103,8 @@ typedef struct fmd_attention {
 } fmd_attention;
 
 /* Workspace of fmd_packed_attention (backward = 0) or of
- * fmd_packed_attention_bwd (1), 0 for none, from the sizes alone; it starts
- * at a multiple of 16 bytes. */
+ * fmd_packed_attention_bwd (1, for all three gradients), 0 for none, from
+ * the sizes alone; it starts at a multiple of 16 bytes. */
 FMD_API fmd_status fmd_packed_attention_workspace_bytes(const fmd_attention* problem, int32_t backward,
                                                         size_t* bytes);
 
