@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    dependents_may_start();
     const int per_tile = kTile / a.group;
     int head;
     const Place place = block_place<false>(a, per_tile, &head);
@@ -358,7 +359,10 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
 
     int head;
     const Place place = block_place<true>(a, kTile, &head);
-    if (place.b < 0) return;
+    if (place.b < 0) {
+        wait_for_previous();
+        return;
+    }
     const Span s = load_span(a, place.b);
     const int64_t key0 = int64_t(place.tile) * kTile;
     const int per_tile = kTile / a.group, full_rows = per_tile * a.group;
@@ -600,6 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
             }
         }
     }
+    wait_for_previous();
     close_block(ctl, warp, a.flags);
 }
 
@@ -615,8 +620,9 @@ fmd_status launch(const Maps& maps, const Attn& a, BackwardSplits splits, cudaSt
         if ((st = check_launch()) != FMD_OK) return st;
     }
     if (a.dk != nullptr && a.keys > 0) {
-        const int64_t tiles = tile_bound(a.keys, a.batch, kTile);
-        key_gradient_kernel<KS><<<dim3(unsigned(tiles * a.hk), 1, unsigned(splits.keys)), kThreads, key_bytes, s>>>(maps, a);
+        const dim3 grid(unsigned(tile_bound(a.keys, a.batch, kTile) * a.hk), 1, unsigned(splits.keys));
+        if (a.dq != nullptr && a.rows > 0) return launch_early(key_gradient_kernel<KS>, grid, kThreads, key_bytes, s, maps, a);
+        key_gradient_kernel<KS><<<grid, kThreads, key_bytes, s>>>(maps, a);
         st = check_launch();
     }
     return st;

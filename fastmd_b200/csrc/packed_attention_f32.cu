@@ -455,6 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    dependents_may_start();
     const int per_tile = kTile / a.group;
     int head;
     const Place place = block_place<false>(a, per_tile, &head);
@@ -623,7 +624,10 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
 
     int head;
     const Place place = block_place<true>(a, kTile, &head);
-    if (place.b < 0) return;
+    if (place.b < 0) {
+        wait_for_previous();
+        return;
+    }
     const Span s = load_span(a, place.b);
     const int64_t key0 = int64_t(place.tile) * kTile;
     const int per_tile = kStream / a.group, full_rows = per_tile * a.group;
@@ -831,6 +835,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
             }
         }
     }
+    wait_for_previous();
     close_block(ctl, warp, a.flags);
 }
 
@@ -898,6 +903,8 @@ fmd_status launch_backward(const Maps& maps, const Attn& a, const Own& own, Back
     }
     if (a.dk != nullptr && a.keys > 0) {
         const dim3 grid(unsigned(tile_bound(a.keys, a.batch, kTile) * a.hk), 1, unsigned(splits.keys));
+        if (a.dq != nullptr && a.rows > 0)
+            return launch_early(key_gradient_kernel<KS>, grid, kThreads, kBackwardBytes, s, maps, a, own);
         key_gradient_kernel<KS><<<grid, kThreads, kBackwardBytes, s>>>(maps, a, own);
         st = check_launch();
     }

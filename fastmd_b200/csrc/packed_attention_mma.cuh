@@ -334,7 +334,33 @@ __device__ __forceinline__ void tmem_free(uint32_t address) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "n"(COLUMNS) : "memory");
 }
 
+// The kernel of the keys' gradients follows that of the queries' without depending on it: it is launched so that its
+// blocks start as soon as every block of the first has (dependents_may_start), and fill the SMs that the first one's
+// end leaves idle. Its last block waits for the first kernel before it ends (wait_for_previous), so that what follows in
+// the stream finds both complete.
+__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void wait_for_previous() {
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.z == gridDim.z - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ------------------------------------------------------------------- host
+
+// Launches `kernel` so that it may start before the one ahead of it in the stream is complete.
+template <typename... Params, typename... Given>
+fmd_status launch_early(void (*kernel)(Params...), dim3 grid, int threads, size_t bytes, cudaStream_t s, Given... given) {
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(unsigned(threads));
+    config.dynamicSmemBytes = bytes;
+    config.stream = s;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, Params(given)...);
+    return err == cudaSuccess ? check_launch() : record_cuda_error(err);
+}
 
 // Packed rows: x [rows, key_heads, group, dim], a box of `tokens` tokens x group heads x 64 values.
 fmd_status encode_packed(const DriverCalls& drv, CUtensorMap* map, const void* x, int64_t rows, int hk, int group,
