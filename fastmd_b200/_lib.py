@@ -187,7 +187,10 @@ def check(status: int, what: str) -> None:
 
 # kernels each entry point launches (for the launch count of a step); the default is one
 KERNELS_PER_CALL = {"fmd_refilter_edges": 2, "fmd_refilter_edges_noalloc": 2, "fmd_mace_message_bwd": 2,
-                    "fmd_mace_edge_virial": 2, "fmd_reverse_pairs": 5, "fmd_line_graph": 6, "fmd_column_sum": 2}
+                    "fmd_mace_edge_virial": 2, "fmd_reverse_pairs": 5, "fmd_line_graph": 6, "fmd_column_sum": 2,
+                    # queries, keys and the row sums before them; planes and splits of an axis add some
+                    "fmd_packed_attention_bwd": 3, "fmd_packed_attention_workspace_bytes": 0,
+                    "fmd_head_rotary_workspace_bytes": 0}
 
 
 def fused_step_kernels(n_layers: int) -> int:
