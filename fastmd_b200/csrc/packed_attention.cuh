@@ -13,7 +13,6 @@
 #pragma once
 
 #include <cuda_bf16.h>
-#include <float.h>
 
 #include "common.cuh"
 

@@ -18,6 +18,14 @@
 // A score tile is only issued after the product that read the weights at its place, by the same thread, and commits
 // cover all products before them: "scores ready" therefore also says that o is at rest. The last key tile's products
 // are as narrow as its keys (multiples of 16).
+//
+// Measured: one causal sequence of 10,000, 16 heads on 2 key heads of 128: 431 us, 950 TFLOP/s of the 1,650 that a
+// library product reaches; the tensor cores are 50 % busy and so is the special-function unit (a tile of 128 x 128 takes
+// 1,024 cycles of products and 1,024 of exponentials, and 2,300 in all: what remains is the hand-over between the two).
+// A cubic on the FMA pipes for a quarter of the exponentials cost 15 % instead of saving. 33 new rows of 8 sequences
+// behind up to 5,000 keys, four splits: 43 us; one new row of 3 sequences against 20,000 to 60,000 keys, 24 splits:
+// 72 us, 3.4 TB/s (the splits of the longest sequence are what it ends with).
+//
 // Every wait is bounded: on expiry the block raises FMD_FLAG_WAIT_TIMEOUT, waits (bounded) for its copies and
 // products in flight, frees its TMEM and returns.
 

@@ -203,16 +203,6 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_store32(uint32_t addr, const float (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " FMD_TMEM_R32 ";" ::"f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
-        "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]),
-        "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]),
-        "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]),
-        "f"(v[31]), "r"(addr)
-        : "memory");
-}
-
 // 16 columns: 32 bfloat16 of this thread's lane
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
     asm volatile(

@@ -21,9 +21,10 @@ constexpr int kM = 64, kN = 64, kThreads = 256, kDim = 128;
 // rows [0, count) of src (row stride ld, dim values) into dst [64][kDim + 4], zeros elsewhere
 template <typename RowOf>
 __device__ __forceinline__ void load_tile(float* dst, const float* src, int count, int dim, RowOf row_of) {
-    for (int i = threadIdx.x; i < 64 * kDim; i += kThreads) {
-        const int r = i / kDim, c = i - r * kDim;
-        dst[r * (kDim + 4) + c] = r < count && c < dim ? src[row_of(r) + c] : 0.0f;
+#pragma unroll
+    for (int i = threadIdx.x; i < 64 * kDim / 4; i += kThreads) {
+        const int r = i / (kDim / 4), c = i % (kDim / 4) * 4;
+        st4(dst + r * (kDim + 4) + c, r < count && c < dim ? ldg4(src + row_of(r) + c) : f4_zero());
     }
 }
 
@@ -48,7 +49,10 @@ __device__ __forceinline__ void dots(const float* a, const float* b, int ty, int
     }
 }
 
-// acc[i][c] += sum_n p[ty + 16 i][n] b[n][2 tx + 32 (c / 2) + c % 2] over the 64 rows of b
+// column c of a thread's kDim / 16
+__device__ __forceinline__ int column(int tx, int c) { return 4 * tx + 64 * (c / 4) + c % 4; }
+
+// acc[i][c] += sum_n p[ty + 16 i][n] b[n][column(tx, c)] over the 64 rows of b
 __device__ __forceinline__ void weigh(const float* p, const float* b, int ty, int tx, float (&acc)[4][kDim / 16]) {
 #pragma unroll 2
     for (int n = 0; n < 64; n += 4) {
@@ -58,13 +62,15 @@ __device__ __forceinline__ void weigh(const float* p, const float* b, int ty, in
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
 #pragma unroll
-            for (int c = 0; c < kDim / 32; ++c) {
-                const float2 y = *reinterpret_cast<const float2*>(b + (n + u) * (kDim + 4) + 2 * tx + 32 * c);
+            for (int c = 0; c < kDim / 64; ++c) {
+                const float4 y = *reinterpret_cast<const float4*>(b + (n + u) * (kDim + 4) + 4 * tx + 64 * c);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float w = u == 0 ? x[i].x : u == 1 ? x[i].y : u == 2 ? x[i].z : x[i].w;
-                    acc[i][2 * c] = fmaf(w, y.x, acc[i][2 * c]);
-                    acc[i][2 * c + 1] = fmaf(w, y.y, acc[i][2 * c + 1]);
+                    acc[i][4 * c] = fmaf(w, y.x, acc[i][4 * c]);
+                    acc[i][4 * c + 1] = fmaf(w, y.y, acc[i][4 * c + 1]);
+                    acc[i][4 * c + 2] = fmaf(w, y.z, acc[i][4 * c + 2]);
+                    acc[i][4 * c + 3] = fmaf(w, y.w, acc[i][4 * c + 3]);
                 }
             }
         }
@@ -174,7 +180,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Attn a) {
         float* out = (SPLIT ? a.part : static_cast<float*>(a.out)) + flat * a.dim;
 #pragma unroll
         for (int c = 0; c < kDim / 16; ++c) {
-            const int col = 2 * tx + 32 * (c / 2) + c % 2;
+            const int col = column(tx, c);
             if (col < a.dim) out[col] = o[i][c] * inv;
         }
         float* lse = SPLIT ? a.part_lse : a.lse;
@@ -249,7 +255,7 @@ __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const Attn a) 
         float* out = static_cast<float*>(a.dq) + at.flat(r) * a.dim;
 #pragma unroll
         for (int c = 0; c < kDim / 16; ++c) {
-            const int col = 2 * tx + 32 * (c / 2) + c % 2;
+            const int col = column(tx, c);
             if (col < a.dim) out[col] = dq[i][c] * a.scale;
         }
     }
@@ -322,7 +328,7 @@ __global__ void __launch_bounds__(kThreads) key_gradient_kernel(const Attn a) {
         const int64_t flat = ((s.key0 + n0 + key) * a.hk + head) * a.dim;
 #pragma unroll
         for (int c = 0; c < kDim / 16; ++c) {
-            const int col = 2 * tx + 32 * (c / 2) + c % 2;
+            const int col = column(tx, c);
             if (col < a.dim) {
                 static_cast<float*>(a.dk)[flat + col] = dk[i][c] * a.scale;
                 static_cast<float*>(a.dv)[flat + col] = dv[i][c];

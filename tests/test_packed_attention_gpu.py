@@ -296,6 +296,62 @@ def test_captured_in_a_graph(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+def test_gradients_captured_in_a_graph(cuda, dtype):
+    """Forward and backward in one graph: replays give the eager pass's bits for new values."""
+    rows = [200, 1, 90]
+    q, k, v, g = make(rows, rows, 4, 2, 64, dtype)
+    leaves, offsets = [t.requires_grad_() for t in (q, k, v)], on_device(starts(rows))
+
+    def step():
+        out = packed_attention(*leaves, offsets, causal=True)
+        return out.detach(), *torch.autograd.grad(out, leaves, g)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in (21, 22):
+        with torch.no_grad():
+            for t, new in zip((*leaves, g), make(rows, rows, 4, 2, 64, dtype, seed)):
+                t.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, step()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+@pytest.mark.parametrize("causal", [False, True], ids=["all", "causal"])
+def test_many_sequences(cuda, causal, dtype):
+    """More sequences than a warp ranks, empty ones and single rows among them."""
+    rows = [(37 * b * b + 11 * b) % 150 if b % 7 else b % 2 for b in range(75)]
+    run_case(rows, rows, None, 4, 2, 32, dtype, causal)
+
+
+@gpu
+def test_a_cache_past_32_bits(cuda):
+    """Slots whose values lie more than 2^32 bytes and 2^31 elements into the cache are read as those of a small one."""
+    rows, dim, slot = 20_000_000, 128, 300
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.empty(rows, 1, dim, dtype=B16, device="cuda") for _ in range(2))
+    ends = [torch.randn(slot, 1, dim, generator=gen, device="cuda").to(B16) for _ in range(2)]
+    k[-slot:], v[-slot:] = ends
+    k[:50], v[:50] = ends[0][:50], ends[1][:50]
+    q = torch.randn(2, 4, dim, generator=gen, device="cuda").to(B16)
+    got = packed_attention(q, k, v, on_device([0, 1, 2]), on_device([0, rows - slot, rows]), on_device([50, 277]))
+    small = [torch.cat((e[:50], e)) for e in ends]
+    want = packed_attention(q, *small, on_device([0, 1, 2]), on_device([0, 50, 50 + slot]), on_device([50, 277]))
+    # another number of splits: the roundings of the sums differ, not the values
+    assert float((got.double() - want.double()).abs().max()) <= 2.0 ** -7 * float(want.abs().max())
+
+
+@gpu
 def test_another_stream(cuda):
     q, k, v, _ = make([100], [100], 2, 2, 64, B16)
     offsets = on_device([0, 100])
