@@ -151,7 +151,7 @@ bool rows16(const void* p, int64_t row, int64_t head, int size) {
 fmd_status check(const fmd_attention& q, Attn& a) {
     if ((q.type != FMD_F32 && q.type != FMD_BF16) || q.rows < 0 || q.keys < 0 || q.batch < 0 || q.heads < 1 ||
         q.key_heads < 1 || q.heads % q.key_heads || q.heads / q.key_heads > 64 || q.dim < 8 || q.dim > 128 ||
-        q.dim % 8 || (q.batch > 0 && (q.offsets == nullptr || q.key_offsets == nullptr)) ||
+        q.dim % 8 || !(q.scale >= 0.0f && q.scale <= 3.0e38f) || (q.batch > 0 && (q.offsets == nullptr || q.key_offsets == nullptr)) ||
         (q.batch == 0 && (q.rows > 0 || q.keys > 0)) || (q.rows > 0 && q.q == nullptr) ||
         (q.keys > 0 && (q.k == nullptr || q.v == nullptr)))
         return FMD_ERR_INVALID_ARGUMENT;
@@ -221,11 +221,9 @@ BackwardPlan backward_plan(const Attn& a, int type, bool dq, bool dkv) {
     BackwardPlan p{{1, 1}, delta_bytes(a), 0, 0, 0, 0};
     const bool planes = type == FMD_F32 && a.dim <= kPlanesDim;
     if (planes) p.planes = attention_planes_bytes(a, true);
-    if (type == FMD_BF16 || planes) {
-        const int stream = planes ? 64 : 128;  // rows of a streamed tile
-        if (dq) p.splits.queries = key_splits(a, 128 / a.group, kNumSMs, stream);
-        if (dkv) p.splits.keys = row_splits(a, stream / a.group, kNumSMs, 128);
-    }
+    const int own = type == FMD_BF16 || planes ? 128 : 64, stream = type == FMD_BF16 ? 128 : 64;  // rows of the tiles
+    if (dq) p.splits.queries = key_splits(a, own / a.group, kNumSMs, stream);
+    if (dkv) p.splits.keys = row_splits(a, stream / a.group, kNumSMs, own);
     if (p.splits.queries > 1) p.dq = size_t(p.splits.queries) * a.rows * a.hq * a.dim * sizeof(float);
     if (p.splits.keys > 1) p.dkv = size_t(p.splits.keys) * a.keys * a.hk * a.dim * sizeof(float);
     p.bytes = p.delta + p.planes + p.dq + 2 * p.dkv;
@@ -311,7 +309,7 @@ fmd_status fmd_packed_attention_bwd(const fmd_attention* problem, const void* ou
     a.part_dv = reinterpret_cast<float*>(at + p.planes + p.dq + p.dkv);
     if (problem->type == FMD_BF16) st = attention_backward_mma(a, p.splits, s);
     else if (a.dim <= kPlanesDim) st = attention_backward_planes(a, p.splits, at, s);
-    else st = attention_backward_simt(a, s);
+    else st = attention_backward_simt(a, p.splits, s);
     const int64_t q_values = a.rows * a.hq * a.dim, k_values = a.keys * a.hk * a.dim;
     const bool bf16 = problem->type == FMD_BF16;
     if (st == FMD_OK && p.splits.queries > 1 && q_values > 0)

@@ -225,6 +225,6 @@ fmd_status attention_forward_planes(const Attn& a, int splits, void* planes, cud
 fmd_status attention_backward_planes(const Attn& a, BackwardSplits splits, void* planes, cudaStream_t s);
 // float32, wider heads
 fmd_status attention_forward_simt(const Attn& a, int splits, cudaStream_t s);
-fmd_status attention_backward_simt(const Attn& a, cudaStream_t s);
+fmd_status attention_backward_simt(const Attn& a, BackwardSplits splits, cudaStream_t s);
 
 }  // namespace fmd

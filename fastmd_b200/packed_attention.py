@@ -82,7 +82,8 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offse
 
     q ``[rows, heads, dim]``, k and v ``[keys, key_heads, dim]``, float32 or bfloat16; query head ``h`` reads key head
     ``h // (heads // key_heads)``. ``dim`` is a multiple of 8 up to 128. Strides are free; tensors whose heads have no
-    unit stride or do not start at multiples of 16 bytes are copied first. ``scale`` defaults to ``dim ** -0.5``.
+    unit stride or do not start at multiples of 16 bytes are copied first. ``scale`` (not negative) defaults to
+    ``dim ** -0.5``.
 
     Sequence ``b`` has the rows ``offsets[b] .. offsets[b + 1] - 1`` and the keys ``key_offsets[b] ..`` (default:
     the same offsets), all up to ``key_offsets[b + 1]`` or the first ``key_counts[b]`` of them: a cache gives each
@@ -122,8 +123,10 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offse
         key_offsets = _check_offsets("key_offsets", key_offsets, (batch + 1,))
     if key_counts is not None:
         key_counts = _check_offsets("key_counts", key_counts, (batch,))
-    args = (_head_rows(q), _head_rows(k), _head_rows(v), offsets, key_offsets, key_counts, bool(causal),
-            dim ** -0.5 if scale is None else float(scale))
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 <= scale < float("inf"):
+        raise ValueError(f"scale must be finite and not negative, got {scale}")
+    args = (_head_rows(q), _head_rows(k), _head_rows(v), offsets, key_offsets, key_counts, bool(causal), scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _PackedAttention.apply(*args)
     else:

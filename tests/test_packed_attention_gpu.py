@@ -280,6 +280,17 @@ def test_only_what_is_asked_for(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+@pytest.mark.parametrize("scale", [0.0, 0.7])
+def test_scale(cuda, scale, dtype):
+    """A scale of its own; 0 takes the mean of the values."""
+    q, k, v, _ = make([150], [150], 2, 1, 64, dtype)
+    got = packed_attention(q, k, v, on_device([0, 150]), scale=scale)
+    want, err, _, _ = reference(q, k, v, [0, 150], [0, 150], None, False, scale)
+    check(got, want["out"], err["out"], "out")
+
+
+@gpu
 def test_captured_in_a_graph(cuda):
     """A captured call reads offsets and counts when it is replayed."""
     q, k, v, _ = make([1, 1], [300, 300], 4, 2, 64, B16)
@@ -410,7 +421,7 @@ def test_refusals(cuda):
                 dict(q=q[..., :12], k=k[..., :12], v=v[..., :12]), dict(q=q[:, :3]), dict(offsets=offsets.int()),
                 dict(offsets=offsets[None]), dict(q=q[:5]), dict(offsets=offsets[:1]),
                 dict(key_offsets=on_device([0, 3, 6])), dict(key_counts=on_device([3, 3])),
-                dict(q=q.repeat(1, 33, 1))):
+                dict(q=q.repeat(1, 33, 1)), dict(scale=-0.1), dict(scale=float("nan")), dict(scale=float("inf"))):
         with pytest.raises(ValueError):
             packed_attention(**(dict(q=q, k=k, v=v, offsets=offsets) | bad))
 
@@ -423,7 +434,7 @@ def test_abi_refuses_on_the_host():
     assert lib.fmd_packed_attention(_lib.FmdAttention(**base), None, None, None, 0, None, None) == 0  # no rows
     for bad in (dict(type=2), dict(heads=3, key_heads=2), dict(key_heads=0), dict(dim=12), dict(dim=136),
                 dict(rows=-1), dict(batch=0, rows=1), dict(rows=1, q=None), dict(keys=1, v=None),
-                dict(offsets=None), dict(heads=65)):
+                dict(offsets=None), dict(heads=65), dict(scale=-1.0), dict(scale=math.nan)):
         assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | bad)), None, None, None, 0, None, None) == 1
     for bad in (dict(rows=1, q=(1 << 20) + 2), dict(keys=1, k_row=65), dict(rows=1, q_head=4), dict(rows=1 << 40)):
         assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | bad)), 1 << 20, None, None, 0, None, None) == 3
