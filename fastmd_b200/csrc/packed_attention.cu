@@ -1,6 +1,8 @@
 // C entry points of packed attention: argument checks, the choice of kernels, and the row sums that the backward
 // pass starts from.
 
+#include <cfloat>
+
 #include "packed_attention.cuh"
 
 namespace fmd {
@@ -151,7 +153,7 @@ bool rows16(const void* p, int64_t row, int64_t head, int size) {
 fmd_status check(const fmd_attention& q, Attn& a) {
     if ((q.type != FMD_F32 && q.type != FMD_BF16) || q.rows < 0 || q.keys < 0 || q.batch < 0 || q.heads < 1 ||
         q.key_heads < 1 || q.heads % q.key_heads || q.heads / q.key_heads > 64 || q.dim < 8 || q.dim > 128 ||
-        q.dim % 8 || !(q.scale >= 0.0f && q.scale <= 3.0e38f) || (q.batch > 0 && (q.offsets == nullptr || q.key_offsets == nullptr)) ||
+        q.dim % 8 || !(q.scale >= 0.0f && q.scale <= 1.0e38f) || (q.batch > 0 && (q.offsets == nullptr || q.key_offsets == nullptr)) ||
         (q.batch == 0 && (q.rows > 0 || q.keys > 0)) || (q.rows > 0 && q.q == nullptr) ||
         (q.keys > 0 && (q.k == nullptr || q.v == nullptr)))
         return FMD_ERR_INVALID_ARGUMENT;
@@ -178,7 +180,8 @@ fmd_status check(const fmd_attention& q, Attn& a) {
     a.k_head = q.k_head;
     a.v_row = q.v_row;
     a.v_head = q.v_head;
-    a.scale = q.scale;
+    // The smallest normal number stands for 0: a masked score is -inf before it is scaled, and -inf * 0 is not a number.
+    a.scale = fmaxf(q.scale, FLT_MIN);
     a.batch = q.batch;
     a.hq = q.heads;
     a.hk = q.key_heads;

@@ -124,8 +124,8 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offse
     if key_counts is not None:
         key_counts = _check_offsets("key_counts", key_counts, (batch,))
     scale = dim ** -0.5 if scale is None else float(scale)
-    if not 0.0 <= scale < float("inf"):
-        raise ValueError(f"scale must be finite and not negative, got {scale}")
+    if not 0.0 <= scale <= 1e38:
+        raise ValueError(f"scale must be between 0 and 1e38, got {scale}")
     args = (_head_rows(q), _head_rows(k), _head_rows(v), offsets, key_offsets, key_counts, bool(causal), scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _PackedAttention.apply(*args)

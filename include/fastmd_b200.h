@@ -1086,9 +1086,9 @@ FMD_API fmd_status fmd_head_rotary(const fmd_head_rotary_side* sides, int32_t ty
  * t + 1 + n - m of n keys. Offsets and counts live on the device; they start
  * at 0, do not fall and end at rows and keys, and counts fit their slots:
  * else FMD_FLAG_INDEX_RANGE is raised, nothing outside the arrays is touched
- * and the results are unspecified. scale finite and not negative, dim a
- * multiple of 8 up to 128, heads / key_heads at most 64, rows and keys at most 2^29; strides in elements, unit stride inside a
- * head; bases and strides multiples of 16 bytes, else FMD_ERR_UNSUPPORTED. */
+ * and the results are unspecified. scale between 0 and 1e38, dim a
+ * multiple of 8 up to 128, heads / key_heads at most 64, rows and keys at
+ * most 2^29; strides in elements, unit stride inside a head; bases and strides multiples of 16 bytes, else FMD_ERR_UNSUPPORTED. */
 typedef struct fmd_attention {
     const void* q;
     const void* k;

@@ -291,6 +291,23 @@ def test_scale(cuda, scale, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,dim", [(F32, 64), (F32, 128), (B16, 64)], ids=["f32", "f32_wide", "b16"])
+def test_scale_of_zero_gradients(cuda, dtype, dim):
+    """Scores that do not count: queries and keys get nothing, each value the mean of the gradients. The tail of a tile
+    is masked, so a masked score times 0 would show."""
+    q, k, v, g = make([150], [150], 2, 1, dim, dtype)
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    out = packed_attention(*leaves, on_device([0, 150]), scale=0.0)
+    out.backward(g)
+    assert float(leaves[0].grad.abs().max()) < 1e-30 and float(leaves[1].grad.abs().max()) < 1e-30
+    want = g.double().sum((0, 1)) / 150
+    # 300 rounded products a sum, and the rounding of 1/150 and of the result
+    unit = 2.0 ** -8 if dtype == B16 else 2.0 ** -20
+    err = 2 * unit * g.double().abs().sum((0, 1)) / 150
+    assert bool(((leaves[2].grad.double() - want).abs() <= err).all())
+
+
+@gpu
 def test_captured_in_a_graph(cuda):
     """A captured call reads offsets and counts when it is replayed."""
     q, k, v, _ = make([1, 1], [300, 300], 4, 2, 64, B16)
