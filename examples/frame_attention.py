@@ -69,21 +69,26 @@ class FrameModel(nn.Module):
         return self.read(x)
 
     def new_cache(self, replicas: int, capacity: int):
-        """Room for `capacity` frames of each replica: a slot per replica, filled as far as its count."""
+        """Room for the last `capacity` frames of each replica: a slot per replica, filled as far as its count."""
+        if capacity < 1:
+            raise ValueError(f"a cache needs room for a frame, got {capacity}")
         weight = self.embed.weight
         shape = (replicas * capacity, self.blocks[0].sizes[1], self.blocks[0].dim)
         layers = [tuple(torch.zeros(shape, device=weight.device, dtype=weight.dtype) for _ in "kv")
                   for _ in self.blocks]
         starts = torch.arange(replicas + 1, device=weight.device) * capacity
         return {"layers": layers, "starts": starts, "counts": torch.zeros_like(starts[1:]),
+                "frames": torch.zeros_like(starts[1:]), "capacity": capacity,
                 "rows": torch.arange(replicas + 1, device=weight.device)}
 
     @torch.no_grad()
     def step(self, frames, steps, cache):
-        """Predictions after one new frame ``[replicas, features]`` of every replica; the cache grows by it. No length
-        is read on the host, so the call can be captured in a CUDA graph and replayed."""
-        at = cache["starts"][:-1] + cache["counts"]
-        cache["counts"] += 1
+        """Predictions after one new frame ``[replicas, features]`` of every replica; the cache grows by it. In a full
+        slot it takes the oldest frame's place: a new row sees all keys of its slot, and their order does not count. No
+        length is read on the host, so the call can be captured in a CUDA graph and replayed."""
+        at = cache["starts"][:-1] + cache["frames"] % cache["capacity"]
+        cache["frames"] += 1
+        torch.clamp(cache["frames"], max=cache["capacity"], out=cache["counts"])
         x = self.embed(frames)
         for block, (keys, values) in zip(self.blocks, cache["layers"]):
             q, k, v = block.heads(x, steps, self.table)

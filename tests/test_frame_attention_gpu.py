@@ -88,3 +88,43 @@ def test_training_lowers_the_loss(cuda, dtype):
         optimizer.step()
         losses.append(float(loss.detach()))
     assert losses[-1] < 0.7 * losses[0]
+
+
+def plain_operators(example, monkeypatch):
+    """Stand-ins on the host for the two operators of the step form (queries and keys as they are, plain attention)."""
+
+    def attend(q, k, v, offsets, key_offsets, key_counts, causal):
+        out = []
+        for b in range(q.shape[0]):
+            at = slice(int(key_offsets[b]), int(key_offsets[b] + key_counts[b]))
+            x, y = (t[at].repeat_interleave(q.shape[1] // k.shape[1], 1) for t in (k, v))
+            weight = torch.softmax(torch.einsum("hd,jhd->hj", q[b], x) * q.shape[2] ** -0.5, 1)
+            out.append(torch.einsum("hj,jhd->hd", weight, y))
+        return torch.stack(out)
+
+    monkeypatch.setattr(example, "packed_attention", attend)
+    monkeypatch.setattr(example, "head_norm_rotary", lambda q, k, *rest: (q, k))
+
+
+def test_a_full_cache_keeps_the_last_frames_on_the_host(monkeypatch):
+    """More frames than a slot holds: the oldest make room, in their own slot, and the prediction is that of a fresh
+    cache that has read the last ones alone."""
+    example = load()
+    plain_operators(example, monkeypatch)
+    torch.manual_seed(3)
+    model = example.FrameModel(3, width=16, heads=2, key_heads=1, dim=8, layers=1, device="cpu")
+    frames, at = torch.randn(7, 2, 3), torch.arange(7)[:, None].expand(7, 2)
+    cache = model.new_cache(2, 4)
+    for i in range(7):
+        got = model.step(frames[i], at[i], cache)
+    assert cache["counts"].tolist() == [4, 4]
+    fresh = model.new_cache(2, 4)
+    for i in range(3, 7):
+        want = model.step(frames[i], at[i], fresh)
+    # one layer: what is kept of a frame does not depend on the frames before it; sums of four terms in another order
+    assert torch.allclose(got, want, atol=1e-5)
+
+
+def test_a_cache_without_room_is_refused_on_the_host():
+    with pytest.raises(ValueError):
+        load().FrameModel(3, width=16, heads=2, key_heads=1, dim=8, layers=1, device="cpu").new_cache(2, 0)
