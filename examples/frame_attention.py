@@ -129,7 +129,7 @@ def main(argv=None):
     args = parser.parse_args(argv)
     torch.manual_seed(0)
     dtype = getattr(torch, args.dtype)
-    model = FrameModel(4, device="cuda", dtype=dtype)
+    model = FrameModel(4, device="cuda", dtype=dtype, max_steps=max(10_000, args.longest))
     log = made_up_log(args.replicas, args.longest, 4, dtype=dtype)
     optimizer = torch.optim.AdamW(model.parameters(), lr=1e-3)
     for i in range(args.steps):

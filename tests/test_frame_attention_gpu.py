@@ -128,3 +128,20 @@ def test_a_full_cache_keeps_the_last_frames_on_the_host(monkeypatch):
 def test_a_cache_without_room_is_refused_on_the_host():
     with pytest.raises(ValueError):
         load().FrameModel(3, width=16, heads=2, key_heads=1, dim=8, layers=1, device="cpu").new_cache(2, 0)
+
+
+def test_the_table_covers_the_longest_history_on_the_host(monkeypatch):
+    """A position outside the table would be flagged and its row not turned."""
+    example = load()
+
+    class Seen(Exception):
+        pass
+
+    def record(*args, max_steps=10_000, **kwargs):
+        raise Seen(max_steps)
+
+    monkeypatch.setattr(example, "FrameModel", record)
+    for longest in (500, 10_001, 20_000):
+        with pytest.raises(Seen) as seen:
+            example.main(["--longest", str(longest)])
+        assert seen.value.args[0] >= longest
