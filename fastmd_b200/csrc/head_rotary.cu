@@ -229,10 +229,14 @@ __global__ void __launch_bounds__(kThreads, kResident<NORM, BACKWARD>) head_rota
 #pragma unroll
         for (int i = 0; i < HEADS; ++i) {
             if (u * HEADS * across + i * across >= s.heads) break;  // the same for the whole warp
+            const bool mine = here && head0 + i * across < s.heads;
             float2 v[4], o[4];
             float n = 1.0f;
             if (!BACKWARD || norm) xs[i].get(v);
-            if (norm) n = rsqrtf(dot(v, v, span) * a.inv_dim + a.eps);
+            if (norm) {
+                n = rsqrtf(dot(v, v, span) * a.inv_dim + a.eps);
+                if (BACKWARD && !mine) n = 0.0f;  // with eps = 0 it is infinite there, and zeros times it no numbers
+            }
             if (!BACKWARD) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[j] = norm ? mul2(v[j], mul2(both(n), w[j])) : v[j];
@@ -252,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, kResident<NORM, BACKWARD>) head_rota
                     for (int j = 0; j < 4; ++j) o[j] = mul2(both(n), fma2(v[j], both(mean), o[j]));
                 }
             }
-            if (here && head0 + i * across < s.heads) Raw<T>::put(y + i * y_head, gap, o);
+            if (mine) Raw<T>::put(y + i * y_head, gap, o);
         }
         row += row_step;
         x += x_step;

@@ -207,3 +207,29 @@ def test_abi_refuses_on_the_host():
     args[12] = 1
     assert lib.fmd_head_rotary(*args) == 4  # the backward pass with weights needs its workspace
     assert head_rotary.TYPES[torch.float32] == 0
+
+
+@gpu
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "pairs"])
+@pytest.mark.parametrize("rows,hq,hk,dim,dtype", [(7, 3, 1, 96, torch.bfloat16), (13, 5, 6, 64, torch.float32),
+                                                  (1, 3, 3, 32, torch.float32), (33, 1, 7, 48, torch.bfloat16)])
+def test_gradients_without_an_eps(cuda, rows, hq, hk, dim, dtype, interleaved):
+    """eps = 0: the lanes without a head or a row, which divide nothing by nothing, have no share in the sums. The
+    bounds are those of test_forward_and_gradients: eps does not add a rounding."""
+    q, k, positions, cos, sin, (wq, wk) = make(rows, hq, hk, dim, dim, dtype, True, seed=rows)
+    leaves = [t.detach().requires_grad_() for t in (q, k, wq, wk)]
+    out = head_norm_rotary(*leaves[:2], positions, cos, sin, *leaves[2:], eps=0.0, interleaved=interleaved)
+    gen = torch.Generator().manual_seed(1)
+    g = [torch.randn(o.shape, generator=gen).to(dtype).cuda() for o in out]
+    grads = torch.autograd.grad(out, leaves, g)
+    wide = [t.detach().double().requires_grad_() for t in leaves]
+    ref = [head64(x, w, cos[positions], sin[positions], interleaved, 0.0) for x, w in zip(wide[:2], wide[2:])]
+    ref_grads = torch.autograd.grad(ref, wide, [t.double() for t in g])
+    for got, want in zip(list(out) + list(grads[:2]), list(ref) + list(ref_grads[:2])):
+        bound = unit(dtype) * want.abs() + 16 * 2.0 ** -24 * (want.abs().amax(-1, keepdim=True) + 1)
+        assert bool(((got.double() - want).abs() <= bound).all())
+    for got, want, x, gx in zip(grads[2:], ref_grads[2:], wide[:2], g):
+        terms = rows * x.shape[1]
+        size = 3.0 * math.sqrt(dim) * gx.double().abs().amax()
+        bound = unit(dtype) * want.abs() + 2.0 ** -24 * min(terms, 64) * terms * size
+        assert bool(((got.double() - want).abs() <= bound).all())
