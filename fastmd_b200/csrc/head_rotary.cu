@@ -369,7 +369,8 @@ fmd_status fmd_head_rotary(const fmd_head_rotary_side* sides, int32_t type, int3
                            const float* cos, const float* sin, int64_t table, int32_t backward, void* workspace,
                            size_t workspace_bytes, int32_t* flags, void* stream) {
     if (sides == nullptr || rows < 0 || dim < 8 || dim > kMaxDim || dim % 8 || rot < 8 || rot > dim || rot % 8 ||
-        table < 0 || (type != FMD_F32 && type != FMD_BF16) || (weight_type != type && weight_type != FMD_F32))
+        table < 0 || (type != FMD_F32 && type != FMD_BF16) || (weight_type != type && weight_type != FMD_F32) ||
+        !(eps >= 0.0f && eps <= 1.0e38f))
         return FMD_ERR_INVALID_ARGUMENT;
     const bool norm = sides[0].w != nullptr || sides[1].w != nullptr;
     const int size = type == FMD_F32 ? 4 : 2;

@@ -128,10 +128,10 @@ def head_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, cos: Tensor, sin: 
     rows that are not 16-byte aligned are copied first).
 
     With its weight ``[dim]`` (float32 or the type of q and k; None: no norm) a head is divided by
-    ``sqrt(mean(x^2) + eps)`` and multiplied by the weight. Then its first ``2 * cos.shape[1]`` values are turned by
-    row ``positions[row]`` (int64) of the float32 tables: pairs ``(p, p + half)``, or ``(2p, 2p + 1)`` with
-    ``interleaved``. ``dim`` is a multiple of 8 up to 128, the turned part a multiple of 8 up to ``dim``. A position
-    outside the table raises ``FMD_FLAG_INDEX_RANGE`` in the device's flags word and the turned part is zero.
+    ``sqrt(mean(x^2) + eps)`` (``eps`` not negative) and multiplied by the weight. Then its first
+    ``2 * cos.shape[1]`` values are turned by row ``positions[row]`` (int64) of the float32 tables: pairs
+    ``(p, p + half)``, or ``(2p, 2p + 1)`` with ``interleaved``. ``dim`` is a multiple of 8 up to 128, the turned part a
+    multiple of 8 up to ``dim``. A position outside the table raises ``FMD_FLAG_INDEX_RANGE`` in the device's flags word and the turned part is zero.
     Differentiable in q, k and the weights, with the same bits on every run; computed in 32 bits, rounded once."""
     _lib.require_cuda(q, k, positions, cos, sin, q_weight, k_weight)
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
@@ -155,9 +155,12 @@ def head_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, cos: Tensor, sin: 
             raise ValueError(f"a norm weight must be [{dim}] in float32 or the type of q and k")
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise ValueError("both norm weights must have the same type")
+    eps = float(eps)
+    if not 0.0 <= eps <= 1e38:
+        raise ValueError(f"eps must be between 0 and 1e38, got {eps}")
     weights = [w if w is None or w.is_contiguous() else w.contiguous() for w in (q_weight, k_weight)]
     args = (_head_rows(q), _head_rows(k), positions.contiguous(), _aligned(cos), _aligned(sin), *weights,
-            float(eps), bool(interleaved))
+            eps, bool(interleaved))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, *weights)):
         return _HeadNormRotary.apply(*args)
     return _forward(*args)

@@ -1069,9 +1069,9 @@ FMD_API fmd_status fmd_head_rotary_workspace_bytes(int32_t dim, size_t* bytes);
  * = 1 the gradients of both:
  *   y = turn(w x / sqrt(mean(x^2) + eps)), pairs (p, p + rot/2), or with
  *   interleaved (2p, 2p + 1); cos, sin [table, rot / 2] float32.
- * dim and rot multiples of 8, at most 128; at most 1024 heads a side; FP32 arithmetic, rounded once. A
- * position outside [0, table) raises FMD_FLAG_INDEX_RANGE and turns by
- * cos = sin = 0. Deterministic. Bases (the tables' too) and row and head
+ * dim and rot multiples of 8, at most 128; at most 1024 heads a side; eps
+ * between 0 and 1e38; FP32 arithmetic, rounded once. A position outside
+ * [0, table) raises FMD_FLAG_INDEX_RANGE and turns by cos = sin = 0. Deterministic. Bases (the tables' too) and row and head
  * strides must be multiples of 16 bytes, else FMD_ERR_UNSUPPORTED. No reference counterpart. */
 FMD_API fmd_status fmd_head_rotary(const fmd_head_rotary_side* sides, int32_t type, int32_t weight_type, int64_t rows,
                                    int32_t dim, int32_t rot, int32_t interleaved, float eps, const int64_t* positions,

@@ -233,3 +233,17 @@ def test_gradients_without_an_eps(cuda, rows, hq, hk, dim, dtype, interleaved):
         size = 3.0 * math.sqrt(dim) * gx.double().abs().amax()
         bound = unit(dtype) * want.abs() + 2.0 ** -24 * min(terms, 64) * terms * size
         assert bool(((got.double() - want).abs() <= bound).all())
+
+
+@gpu
+@pytest.mark.parametrize("eps", [-1e-6, float("nan"), float("inf"), 1e39])
+def test_an_eps_that_is_none_is_refused(cuda, eps):
+    q, k, positions, cos, sin, (wq, wk) = make(4, 2, 1, 16, 16, torch.float32, True)
+    with pytest.raises(ValueError):
+        head_norm_rotary(q, k, positions, cos, sin, wq, wk, eps=eps)
+
+
+@pytest.mark.parametrize("eps", [-1e-6, float("nan"), float("inf")])
+def test_abi_refuses_an_eps_that_is_none(eps):
+    sides = (_lib.FmdHeadRotarySide * 2)()
+    assert _lib.lib().fmd_head_rotary(sides, 0, 0, 0, 64, 64, 0, eps, None, None, None, 0, 0, None, 0, None, None) == 1
