@@ -14,6 +14,7 @@ from torch import Tensor
 from torch.autograd import Function
 
 from . import _lib
+from ._first_order import first_order
 from ._lib import FmdHeadRotarySide, call, ptr, stream
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1}
@@ -118,6 +119,7 @@ class _HeadNormRotary(Function):
         if kept:
             _launch(sides, kept[0], weight, cos, sin, positions, ctx.interleaved, ctx.eps, True)
         (dq, dwq), (dk, dwk) = grads
+        dq, dk, dwq, dwk = first_order("head_norm_rotary", (dq, dk, dwq, dwk), (gq, gk, q, k, q_weight, k_weight))
         return dq, dk, None, None, None, dwq, dwk, None, None
 
 
@@ -131,8 +133,10 @@ def head_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, cos: Tensor, sin: 
     ``sqrt(mean(x^2) + eps)`` (``eps`` not negative) and multiplied by the weight. Then its first
     ``2 * cos.shape[1]`` values are turned by row ``positions[row]`` (int64) of the float32 tables: pairs
     ``(p, p + half)``, or ``(2p, 2p + 1)`` with ``interleaved``. ``dim`` is a multiple of 8 up to 128, the turned part a
-    multiple of 8 up to ``dim``. A position outside the table raises ``FMD_FLAG_INDEX_RANGE`` in the device's flags word and the turned part is zero.
-    Differentiable in q, k and the weights, with the same bits on every run; computed in 32 bits, rounded once."""
+    multiple of 8 up to ``dim``. A position outside the table raises ``FMD_FLAG_INDEX_RANGE`` in the device's flags word
+    and the turned part is zero.
+    Differentiable in q, k and the weights (first derivatives: a second one raises), with the same bits on every run;
+    computed in 32 bits, rounded once."""
     _lib.require_cuda(q, k, positions, cos, sin, q_weight, k_weight)
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError("q and k must be [rows, heads, dim] with the same rows and dim, got "

@@ -14,6 +14,7 @@ from torch import Tensor
 from torch.autograd import Function
 
 from . import _lib
+from ._first_order import first_order
 from ._lib import FmdAttention, c_size_t, call, ptr, stream
 from .head_rotary import TYPES, _head_rows, _like
 
@@ -57,6 +58,7 @@ class _PackedAttention(Function):
         q, k, v, offsets, key_offsets, key_counts, out, lse = ctx.saved_tensors
         if g is None and glse is None:
             return (None,) * 8
+        inputs = (g, glse, q, k, v)
         g = torch.zeros_like(out) if g is None else _head_rows(g)
         glse = glse.contiguous() if glse is not None else None
         dq = _like(q) if ctx.needs_input_grad[0] else None
@@ -66,7 +68,7 @@ class _PackedAttention(Function):
         call("fmd_packed_attention_bwd", problem, out.data_ptr(), lse.data_ptr(), g.data_ptr(), g.stride(0),
              g.stride(1), ptr(glse), ptr(dq), ptr(dk), ptr(dv), ptr(workspace), size,
              _lib.flags_word(q.device).data_ptr(), stream(q.device))
-        return dq, dk, dv, None, None, None, None, None
+        return *first_order("packed_attention", (dq, dk, dv), inputs), None, None, None, None, None
 
 
 def _check_offsets(name: str, t: Tensor, shape: tuple) -> Tensor:
@@ -94,10 +96,10 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offse
     device's flags word.
 
     ``return_lse`` also returns float32 ``[rows, heads]``: the logarithm of each row's softmax denominator (-inf for
-    a row that sees no key). Both are differentiable in q, k and v, with the same bits on every run. Scores, softmax
-    and sums are held in 32 bits. For bfloat16, weights and their gradients are rounded to bfloat16 for the products
-    with v, k and q, as those themselves are. A key that a row does not see has no part in it, but a value that is
-    not finite may reach rows of its own sequence that do not see it (0 * inf)."""
+    a row that sees no key). Both are differentiable in q, k and v (first derivatives: a second one raises), with the
+    same bits on every run. Scores, softmax and sums are held in 32 bits. For bfloat16, weights and their gradients are
+    rounded to bfloat16 for the products with v, k and q, as those themselves are. A key that a row does not see has no
+    part in it, but a value that is not finite may reach rows of its own sequence that do not see it (0 * inf)."""
     _lib.require_cuda(q, k, v, offsets, key_offsets, key_counts)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
         raise ValueError("q must be [rows, heads, dim] and k and v the same [keys, key_heads, dim], got "

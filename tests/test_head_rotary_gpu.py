@@ -247,3 +247,24 @@ def test_an_eps_that_is_none_is_refused(cuda, eps):
 def test_abi_refuses_an_eps_that_is_none(eps):
     sides = (_lib.FmdHeadRotarySide * 2)()
     assert _lib.lib().fmd_head_rotary(sides, 0, 0, 0, 64, 64, 0, eps, None, None, None, 0, 0, None, 0, None, None) == 1
+
+
+@gpu
+@pytest.mark.parametrize("norm", [False, True], ids=["turn", "norm"])
+def test_a_second_derivative_is_refused(cuda, norm):
+    """Gradients taken with create_graph are first derivatives: to differentiate them raises and drops no term, with a
+    gradient that depends on the inputs and with one that does not. Where nothing is differentiated again they are the
+    same."""
+    q, k, positions, cos, sin, (wq, wk) = make(5, 2, 1, 16, 16, torch.float32, norm)
+    leaves = [t.detach().requires_grad_() for t in (q, k, wq, wk) if t is not None]
+    out = head_norm_rotary(leaves[0], leaves[1], positions, cos, sin, *leaves[2:])
+    once = torch.autograd.grad(out[0].sum() + out[1].sum(), leaves, retain_graph=True)
+    again = torch.autograd.grad(out[0].sum() + out[1].sum(), leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(once, again))
+    if norm:  # without a norm the gradient is the same for all inputs: no second derivative is lost
+        with pytest.raises(RuntimeError, match="first derivatives"):
+            torch.autograd.grad(again[0].sum() + leaves[0].square().sum(), leaves[0])
+    (dq,) = torch.autograd.grad(head_norm_rotary(leaves[0], leaves[1], positions, cos, sin, *leaves[2:])[0].square().sum(),
+                                leaves[0], create_graph=True)
+    with pytest.raises(RuntimeError, match="first derivatives"):
+        (dq.square().sum() + leaves[0].square().sum()).backward()

@@ -456,3 +456,23 @@ def test_abi_refuses_on_the_host():
     for bad in (dict(rows=1, q=(1 << 20) + 2), dict(keys=1, k_row=65), dict(rows=1, q_head=4), dict(rows=1 << 40)):
         assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | bad)), 1 << 20, None, None, 0, None, None) == 3
     assert lib.fmd_packed_attention(_lib.FmdAttention(**(base | dict(rows=1))), None, None, None, 0, None, None) == 1
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+def test_a_second_derivative_is_refused(cuda, dtype):
+    """Gradients taken with create_graph are first derivatives: to differentiate them raises and drops no term, with a
+    gradient that depends on the inputs and with one that does not. Where nothing is differentiated again they are the
+    same."""
+    q, k, v, g = make([30], [30], 2, 1, 32, dtype)
+    leaves, offsets = [t.requires_grad_() for t in (q, k, v)], on_device([0, 30])
+    out, lse = packed_attention(*leaves, offsets, return_lse=True)
+    once = torch.autograd.grad(out, leaves, g, retain_graph=True)
+    again = torch.autograd.grad(out, leaves, g, create_graph=True, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(once, again))
+    for i in range(3):
+        with pytest.raises(RuntimeError, match="first derivatives"):
+            torch.autograd.grad(again[i].sum() + leaves[0].square().sum(), leaves[0], retain_graph=True)
+    (dq,) = torch.autograd.grad(lse.square().sum(), leaves[0], create_graph=True)
+    with pytest.raises(RuntimeError, match="first derivatives"):
+        (dq.square().sum() + leaves[0].square().sum()).backward()
