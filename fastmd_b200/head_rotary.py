@@ -14,7 +14,7 @@ from torch import Tensor
 from torch.autograd import Function
 
 from . import _lib
-from ._first_order import first_order
+from ._first_order import first_order, has_tangent
 from ._lib import FmdHeadRotarySide, call, ptr, stream
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1}
@@ -135,7 +135,7 @@ def head_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, cos: Tensor, sin: 
     ``(p, p + half)``, or ``(2p, 2p + 1)`` with ``interleaved``. ``dim`` is a multiple of 8 up to 128, the turned part a
     multiple of 8 up to ``dim``. A position outside the table raises ``FMD_FLAG_INDEX_RANGE`` in the device's flags word
     and the turned part is zero.
-    Differentiable in q, k and the weights (first derivatives: a second one raises), with the same bits on every run;
+    Differentiable in q, k and the weights (first derivatives in reverse mode: others raise), with the same bits on every run;
     computed in 32 bits, rounded once."""
     _lib.require_cuda(q, k, positions, cos, sin, q_weight, k_weight)
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
@@ -165,7 +165,9 @@ def head_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, cos: Tensor, sin: 
     weights = [w if w is None or w.is_contiguous() else w.contiguous() for w in (q_weight, k_weight)]
     args = (_head_rows(q), _head_rows(k), positions.contiguous(), _aligned(cos), _aligned(sin), *weights,
             eps, bool(interleaved))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, *weights)):
+    trains = (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
+              or (k_weight is not None and k_weight.requires_grad))
+    if (trains and torch.is_grad_enabled()) or has_tangent(q, k, cos, sin, q_weight, k_weight):
         return _HeadNormRotary.apply(*args)
     return _forward(*args)
 

@@ -14,7 +14,7 @@ from torch import Tensor
 from torch.autograd import Function
 
 from . import _lib
-from ._first_order import first_order
+from ._first_order import first_order, has_tangent
 from ._lib import FmdAttention, c_size_t, call, ptr, stream
 from .head_rotary import TYPES, _head_rows, _like
 
@@ -96,7 +96,7 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offse
     device's flags word.
 
     ``return_lse`` also returns float32 ``[rows, heads]``: the logarithm of each row's softmax denominator (-inf for
-    a row that sees no key). Both are differentiable in q, k and v (first derivatives: a second one raises), with the
+    a row that sees no key). Both are differentiable in q, k and v (first derivatives in reverse mode: others raise), with the
     same bits on every run. Scores, softmax and sums are held in 32 bits. For bfloat16, weights and their gradients are
     rounded to bfloat16 for the products with v, k and q, as those themselves are. A key that a row does not see has no
     part in it, but a value that is not finite may reach rows of its own sequence that do not see it (0 * inf)."""
@@ -129,7 +129,7 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offse
     if not 0.0 <= scale <= 1e38:
         raise ValueError(f"scale must be between 0 and 1e38, got {scale}")
     args = (_head_rows(q), _head_rows(k), _head_rows(v), offsets, key_offsets, key_counts, bool(causal), scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or has_tangent(q, k, v):
         out, lse = _PackedAttention.apply(*args)
     else:
         out, lse = _forward(*args, return_lse)

@@ -1,9 +1,9 @@
 """Gradients that have no derivative of their own say so, on the host."""
 import pytest
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
-from fastmd_b200._first_order import first_order
+from fastmd_b200._first_order import first_order, has_tangent
 
 
 class Square(Function):
@@ -42,3 +42,14 @@ def test_what_does_not_pass_through_it_is_free():
     (dx,) = torch.autograd.grad(Square.apply(x).sum(), x, create_graph=True)
     (dw,) = torch.autograd.grad((dx * w).sum(), w)
     assert torch.equal(dw, dx.detach())
+
+
+def test_a_tangent_is_seen():
+    x = torch.tensor([3.0])
+    assert not has_tangent(x, None)
+    with forward_ad.dual_level():
+        assert not has_tangent(x, None)
+        dual = forward_ad.make_dual(x, torch.ones(1))
+        assert has_tangent(None, x, dual)
+        with pytest.raises(RuntimeError):  # an autograd function without a forward-mode rule refuses it
+            Square.apply(dual)

@@ -3,6 +3,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from fastmd_b200 import _lib, head_rotary
 from fastmd_b200.head_rotary import head_norm_rotary, rotary_table
@@ -268,3 +269,19 @@ def test_a_second_derivative_is_refused(cuda, norm):
                                 leaves[0], create_graph=True)
     with pytest.raises(RuntimeError, match="first derivatives"):
         (dq.square().sum() + leaves[0].square().sum()).backward()
+
+
+@gpu
+def test_forward_mode_is_refused(cuda):
+    """A tangent on any input raises: it is not passed by."""
+    q, k, positions, cos, sin, (wq, wk) = make(5, 2, 1, 16, 16, torch.float32, True)
+    args = [q, k, positions, cos, sin, wq, wk]
+    with forward_ad.dual_level():
+        for i in (0, 1, 3, 4, 5, 6):
+            dual = list(args)
+            dual[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(RuntimeError):
+                head_norm_rotary(*dual)
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                head_norm_rotary(*dual)
+        head_norm_rotary(*args)

@@ -7,6 +7,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from fastmd_b200 import _lib
 from fastmd_b200.packed_attention import packed_attention
@@ -476,3 +477,18 @@ def test_a_second_derivative_is_refused(cuda, dtype):
     (dq,) = torch.autograd.grad(lse.square().sum(), leaves[0], create_graph=True)
     with pytest.raises(RuntimeError, match="first derivatives"):
         (dq.square().sum() + leaves[0].square().sum()).backward()
+
+
+@gpu
+def test_forward_mode_is_refused(cuda):
+    """A tangent on any of the three raises: it is not passed by."""
+    args, offsets = make([20], [20], 2, 1, 32, F32)[:3], on_device([0, 20])
+    with forward_ad.dual_level():
+        for i in range(3):
+            dual = list(args)
+            dual[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(RuntimeError):
+                packed_attention(*dual, offsets)
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                packed_attention(*dual, offsets, return_lse=True)
+        packed_attention(*args, offsets)
