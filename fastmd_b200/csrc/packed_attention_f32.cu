@@ -1,7 +1,8 @@
 // Packed attention in float32 on the tensor cores, for heads of up to 64 values: forward and gradients.
 //
 // A float32 number is the sum of three bfloat16 ones, x = h + m + l (8 bits of the significand each; the differences
-// are exact). A product of two numbers is then nine products of which six matter, largest last:
+// are exact; an infinity has no such sum, and its products are no numbers). A product of two numbers is then nine
+// products of which six matter, largest last:
 //   x y ~ l h' + h l' + m m' + m h' + h m' + h h'          (what is left out is below 2^-24 of x y)
 // so each FP32 product is six bfloat16 ones with FP32 sums: at the tensor cores' rate about five times what the FP32
 // cores could do. q, k, v (and g) are split once by a small kernel into three planes in memory; the weights p and ds
@@ -105,6 +106,8 @@ struct SplitArgs {
     int32_t dim;
 };
 
+constexpr float kBf16Max = 3.38953139e38f;  // (2 - 2^-7) 2^127
+
 // 8 values a thread
 __global__ void __launch_bounds__(256) split_kernel(const SplitArgs a) {
     const int t = blockIdx.y, per = a.dim / 8;
@@ -117,9 +120,20 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitArgs a) {
         float v[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
         uint4* out = reinterpret_cast<uint4*>(a.planes[t] + r * a.dim + c);
         const int64_t plane = a.rows[t] * heads * a.dim / 8;
+        uint32_t w[4];
+        // the first plane is held to the largest bfloat16: beyond it finite numbers would round to an infinity, and what
+        // it leaves of them (2^120 at most) is exact all the same
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            uint32_t w[4];
+        for (int j = 0; j < 4; ++j) {
+            w[j] = pack_bf16(fminf(fmaxf(v[2 * j], -kBf16Max), kBf16Max),
+                             fminf(fmaxf(v[2 * j + 1], -kBf16Max), kBf16Max));
+            const float2 part = unpack_bf16(w[j]);
+            v[2 * j] -= part.x;
+            v[2 * j + 1] -= part.y;
+        }
+        out[0] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+        for (int i = 1; i < 3; ++i) {
             next_plane<4>(v, w);
             out[i * plane] = make_uint4(w[0], w[1], w[2], w[3]);
         }

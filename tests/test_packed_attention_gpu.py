@@ -492,3 +492,37 @@ def test_forward_mode_is_refused(cuda):
             with torch.no_grad(), pytest.raises(RuntimeError):
                 packed_attention(*dual, offsets, return_lse=True)
         packed_attention(*args, offsets)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_values_at_the_end_of_float32(cuda, dim):
+    """Finite values whose nearest bfloat16 is an infinity. A row of one key returns its value: a weight of 1 and, in
+    planes, three exact products of it, which the sum may cut below 2^-22 each. Keys of zero score zero whatever the
+    query holds: the mean of the values."""
+    top = torch.finfo(F32).max
+    q, k, v, _ = make([3], [3], 2, 1, dim, F32)
+    v[:, :, 0], v[:, :, 1], v[:, :, 2] = top, -top, 3.3961775e38
+    one = on_device([0, 1, 2, 3])  # three sequences of a row
+    got = packed_attention(q, k, v, one)
+    want = v.double().expand(3, 2, dim)
+    assert bool(((got.double() - want).abs() <= 2.0 ** -20 * want.abs()).all())
+    q, k, v, _ = make([3], [3], 2, 1, dim, F32)
+    q[:, :, 0], q[:, :, 1], k[:] = top, -top, 0.0
+    got = packed_attention(q, k, v, on_device([0, 3]))
+    want = v.double().mean(0, keepdim=True).expand(3, 2, dim)
+    assert bool(((got.double() - want).abs() <= 2.0 ** -20 * v.double().abs().amax(0)).all())
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_infinite_values_stay_not_finite(cuda, dim):
+    """An infinite value leaves no finite number in its column of the rows that see it, and the other columns and the
+    rows of other key heads as they are."""
+    q, k, v, _ = make([40], [40], 4, 2, dim, F32)
+    want = packed_attention(q, k, v, on_device([0, 40]))
+    v[7, 1, 5] = float("inf")
+    got = packed_attention(q, k, v, on_device([0, 40]))
+    assert not bool(torch.isfinite(got[:, 2:, 5]).any())
+    got[:, 2:, 5] = want[:, 2:, 5]
+    assert torch.equal(got, want)
