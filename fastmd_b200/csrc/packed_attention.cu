@@ -144,6 +144,8 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const Attn a, const flo
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (i < a.rows * a.hq && lane == 0) delta[i] = glse != nullptr ? sum - glse[i] : sum;
+    for (int64_t b = int64_t(blockIdx.x) * kThreads + threadIdx.x; b < a.batch; b += int64_t(gridDim.x) * kThreads)
+        check_sequence(a, b);
 }
 
 bool rows16(const void* p, int64_t row, int64_t head, int size) {

@@ -93,6 +93,17 @@ __device__ __forceinline__ Span load_span(const Attn& a, int b) {
     return s;
 }
 
+// Sequences that a warp sorts by, one a lane. With more of them the blocks are many and even out by themselves, and the
+// longer search cost more than it gave (64 sequences of 135 rows: dk and dv 66 -> 75 us).
+constexpr int kSorted = 32;
+
+// Looks at sequence b, where there are more than a warp sorts (else every block looks at all): a search among offsets
+// that fall may pass a sequence by. The forward kernels do this (they have a block for every sequence at least), and the
+// backward pass does it beside its row sums: in both gradient kernels too it took 2 % of 64 sequences of 135.
+__device__ __forceinline__ void check_sequence(const Attn& a, int64_t b) {
+    if (a.batch > kSorted && b < a.batch) load_span(a, int(b));
+}
+
 // Tiles of a sequence whose work is at least `level` units, all of them for level 0. KEYS: tiles of `per` keys, their
 // work the tokens that see the first one, the heavy ones at the front; else tiles of `per` tokens, their work the keys
 // that the last one sees, the heavy ones at the end.
@@ -115,10 +126,6 @@ __device__ __forceinline__ int tiles_of(const Span& s, bool causal, int per, int
 struct Place {
     int b, tile;
 };
-
-// Sequences that a warp sorts by, one a lane. With more of them the blocks are many and even out by themselves, and the
-// longer search cost more than it gave (64 sequences of 135 rows: dk and dv 66 -> 75 us).
-constexpr int kSorted = 32;
 
 // The index-th tile, heaviest first where there are at most kSorted sequences. All 32 lanes of a warp.
 template <bool KEYS>
@@ -160,8 +167,8 @@ __device__ __forceinline__ Place find_place(const Attn& a, int per, int index, i
 }
 
 // The same for a whole block: its first warp looks, all get the answer. Blocks count through the key heads first, so
-// that the order holds for all heads together; `head` is the block's.
-template <bool KEYS>
+// that the order holds for all heads together; `head` is the block's. CHECK: the offsets have not been looked at before.
+template <bool KEYS, bool CHECK = false>
 __device__ __forceinline__ Place block_place(const Attn& a, int per, int* head) {
     __shared__ Place place;
     const int index = int(blockIdx.x / unsigned(a.hk));
@@ -169,6 +176,8 @@ __device__ __forceinline__ Place block_place(const Attn& a, int per, int* head) 
     if (threadIdx.x < 32) {
         const Place p = find_place<KEYS>(a, per, index, int(gridDim.x / unsigned(a.hk)));
         if (threadIdx.x == 0) place = p;
+    } else if (CHECK && threadIdx.x == 32 && *head == 0 && blockIdx.z == 0) {
+        check_sequence(a, index);
     }
     __syncthreads();
     return place;

@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
 
     const int per_tile = kTile / a.group;
     int head;
-    const Place place = block_place<false>(a, per_tile, &head);
+    const Place place = block_place<false, true>(a, per_tile, &head);
     if (place.b < 0) return;
     const Span s = load_span(a, place.b);
     const int64_t token0 = int64_t(place.tile) * per_tile;

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(Shape<KS, NT>::kThreads, NT == 1 ? 2 : 1)
 
     const int per_tile = kTile / a.group, per_block = NT * per_tile;
     int head;
-    const Place place = block_place<false>(a, per_block, &head);
+    const Place place = block_place<false, true>(a, per_block, &head);
     if (place.b < 0) return;
     const Span s = load_span(a, place.b);
     const int64_t token0 = int64_t(place.tile) * per_block;

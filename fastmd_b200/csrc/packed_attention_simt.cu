@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Attn a) {
     float* ps = vs + 64 * (kDim + 4);
     const int per_tile = kM / a.group;
     int head;
-    const Place place = block_place<false>(a, per_tile, &head);
+    const Place place = block_place<false, true>(a, per_tile, &head);
     if (place.b < 0) return;
     const Span s = load_span(a, place.b);
     const int64_t token0 = int64_t(place.tile) * per_tile;

@@ -526,3 +526,28 @@ def test_infinite_values_stay_not_finite(cuda, dim):
     assert not bool(torch.isfinite(got[:, 2:, 5]).any())
     got[:, 2:, 5] = want[:, 2:, 5]
     assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,dim", [(F32, 32), (F32, 96), (B16, 32)], ids=["f32", "f32_wide", "b16"])
+def test_offsets_that_fall_among_many_are_flagged(cuda, dtype, dim):
+    """Forty sequences: one offset far ahead of its neighbours, whose sequence no tile's search ends at."""
+    q, k, v, _ = make([2000], [2000], 1, 1, dim, dtype)
+    good = torch.arange(41) * 50
+    bad = good.clone()
+    bad[5] = 1900
+    word = _lib.flags_word(q.device)
+    word.zero_()
+    packed_attention(q, k, v, good.cuda())
+    assert int(word.item()) == 0
+    packed_attention(q, k, v, bad.cuda(), good.cuda())
+    assert int(word.item()) & 1
+    word.zero_()
+    packed_attention(q, k, v, good.cuda(), bad.cuda())
+    assert int(word.item()) & 1
+    leaf = q.clone().requires_grad_()
+    out = packed_attention(leaf, k, v, bad.cuda(), good.cuda())
+    word.zero_()
+    torch.autograd.grad(out.sum(), leaf)  # the backward pass by itself
+    assert int(word.item()) & 1
+    word.zero_()
