@@ -223,11 +223,16 @@ def ptr(tensor) -> int | None:
     return tensor.data_ptr()
 
 
+# the raw handle: building the Stream object of current_stream() takes 2 us a call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream(device=None) -> int:
-    """The handle of torch's current CUDA stream (kernels are launched on it)."""
-    index = getattr(device, "index", None)
-    # the raw handle: building the Stream object of current_stream() takes 2 us a call
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+    """The handle of torch's current CUDA stream of ``device`` (a ``torch.device``, its number or name; default: the
+    current device). Kernels are launched on it."""
+    if _raw_stream is not None and isinstance(device, torch.device) and device.index is not None:
+        return _raw_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def require_cuda(*tensors) -> None:
