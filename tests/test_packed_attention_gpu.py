@@ -551,3 +551,27 @@ def test_offsets_that_fall_among_many_are_flagged(cuda, dtype, dim):
     torch.autograd.grad(out.sum(), leaf)  # the backward pass by itself
     assert int(word.item()) & 1
     word.zero_()
+
+
+def takes_two_tiles(rows, slots, hq, hk):
+    """The rule of the forward pass in 16 bits: two tiles of rows a block."""
+    blocks = (sum(rows) // (2 * (128 // (hq // hk))) + len(rows)) * hk
+    return blocks >= 148 and sum(slots) // len(rows) >= 1024
+
+
+@gpu
+@pytest.mark.parametrize("causal", [False, True], ids=["all", "causal"])
+@pytest.mark.parametrize("rows,slots,counts,hq,hk,dim", [
+    ([2100, 1301], [2100, 1301], None, 16, 8, 64),  # last tiles of 52 and 21 rows; blocks without a second tile
+    ([2100, 1301], [2100, 1301], None, 12, 12, 128),
+    ([2100, 1301], [2100, 1301], None, 24, 8, 32),  # 42 tokens of three heads: rows of a tile that hold nothing
+    ([1000, 1500], [1700, 1033], None, 30, 5, 96),  # 21 tokens of six heads; more keys than rows and the reverse
+    ([1430, 1300], [1100, 1030], None, 16, 8, 72),  # causal: 330 rows see nothing, a first tile among them
+    ([700, 1300, 0, 1], [1500, 1300, 1400, 1200], [1333, 1300, 5, 0], 32, 4, 64),
+    ([1153] * 30, [1153] * 30, None, 2, 2, 40),
+    ([1040 + b % 5 for b in range(40)], [1040 + b % 5 for b in range(40)], None, 2, 1, 128),
+], ids=["pairs", "single", "three", "six", "more_rows", "cache", "thirty", "forty"])
+def test_two_tiles_a_block(cuda, rows, slots, counts, hq, hk, dim, causal):
+    """Long sequences in 16 bits: the tiles of a block share their keys and may see different numbers of them."""
+    assert takes_two_tiles(rows, slots, hq, hk)
+    run_case(rows, slots, counts, hq, hk, dim, B16, causal, seed=dim)
