@@ -149,7 +149,9 @@ constexpr size_t kForwardBytes = size_t(1 + kSlots) * kTile3 + 1024;
 struct ForwardCtrl {
     uint64_t own;
     Ring<kSlots> ring;
-    uint64_t scores[2], weights, swap, out;
+    // two barriers for weights and outputs by turns: the workers may be done with the next tile's weights before the
+    // issuing warp, which waits for v to land first, has looked at this one's, and a phase that is run over is never seen
+    uint64_t scores[2], weights[2], swap, out[2];
     uint64_t tail_here, tail, drain;
     uint32_t tmem;
     int32_t abort;
@@ -193,11 +195,12 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
     if (threadIdx.x == 0) {
         mbar_init(&ctl.own, 1);
         init_ring(ctl.ring);
-        mbar_init(&ctl.scores[0], 1);
-        mbar_init(&ctl.scores[1], 1);
-        mbar_init(&ctl.weights, kWorkers / 32);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ctl.scores[i], 1);
+            mbar_init(&ctl.weights[i], kWorkers / 32);
+            mbar_init(&ctl.out[i], 1);
+        }
         mbar_init(&ctl.swap, kWorkers / 32);
-        mbar_init(&ctl.out, 1);
         mbar_init(&ctl.tail_here, 1);
         mbar_init(&ctl.tail, 64);
         mbar_init(&ctl.drain, 1);
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
                     if (elect_one()) mbar_arrive(&ctl.tail_here);
                     ok = warp_wait(&ctl.tail, 0, abort);
                 }
-                ok = ok && warp_wait(&ctl.weights, uint32_t(j) & 1u, abort);
+                ok = ok && warp_wait(&ctl.weights[j & 1], uint32_t(j >> 1) & 1u, abort);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t odd = uint32_t(j & 1);
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
                         if (kPlaneA[i] == 2) product_weights<8, 4, 32>(o, low, at, steps, o_desc, i > 0);
                         else product_weights<8, 4, 64>(o, p + 32u * kPlaneA[i], at, steps, o_desc, i > 0);
                     }
-                    tc_commit(&ctl.out);
+                    tc_commit(&ctl.out[j & 1]);
                     tc_commit(&ctl.ring.empty[value_at(j) % kSlots]);
                 }
                 if (j + 2 < count) scores(j + 2);  // over this tile's weights, behind the product that reads them
@@ -346,16 +349,16 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
             }
             tmem_wait_st();
             tc_fence_before();
-            warp_arrive(&ctl.weights);
+            warp_arrive(&ctl.weights[j & 1]);
             if (j > 0) {  // the last tile's output, against the old maximum, while this one's products run
-                if (!all(mbar_wait(&ctl.out, uint32_t(j - 1) & 1u, abort))) break;
+                if (!all(mbar_wait(&ctl.out[(j - 1) & 1], uint32_t((j - 1) >> 1) & 1u, abort))) break;
                 drain<kMine>(at_o + uint32_t((j - 1) & 1) * 64u, o, keep);
             }
         }
         if (ok && tiles > 0) {
             sums[half][r] = l;
             warp_arrive(&ctl.swap);
-            if (all(mbar_wait(&ctl.out, uint32_t(tiles - 1) & 1u, abort) &&
+            if (all(mbar_wait(&ctl.out[(tiles - 1) & 1], uint32_t((tiles - 1) >> 1) & 1u, abort) &&
                     mbar_wait(&ctl.swap, uint32_t(tiles) & 1u, abort))) {
                 drain<kMine>(at_o + uint32_t((tiles - 1) & 1) * 64u, o, 1.0f);
                 l = sums[0][r] + sums[1][r];

@@ -575,3 +575,25 @@ def test_two_tiles_a_block(cuda, rows, slots, counts, hq, hk, dim, causal):
     """Long sequences in 16 bits: the tiles of a block share their keys and may see different numbers of them."""
     assert takes_two_tiles(rows, slots, hq, hk)
     run_case(rows, slots, counts, hq, hk, dim, B16, causal, seed=dim)
+
+
+@gpu
+@pytest.mark.parametrize("batch,slot,hq,hk,dim", [(64, 2000, 8, 2, 64), (3, 40_000, 32, 4, 64), (64, 1500, 4, 4, 32)])
+def test_rows_against_long_caches_in_float32(cuda, batch, slot, hq, hk, dim):
+    """Keys and values that come from memory late (caches larger than L2, read by all blocks at once): no wait runs out,
+    in many passes, and all have the same bits."""
+    gen = torch.Generator(device="cuda").manual_seed(batch)
+    q, k, v = (torch.randn(n, h, dim, generator=gen, device="cuda") for n, h in ((batch, hq), (batch * slot, hk),
+                                                                               (batch * slot, hk)))
+    rows, keys = list(range(batch + 1)), starts([slot] * batch)
+    args = (q, k, v, on_device(rows), on_device(keys), on_device([slot] * batch))
+    word = _lib.flags_word(q.device)
+    word.zero_()
+    first = packed_attention(*args, causal=True)
+    others = torch.empty(2 ** 26, device="cuda")
+    for _ in range(20):
+        others.zero_()  # 256 MB: the caches leave L2
+        assert torch.equal(packed_attention(*args, causal=True), first)
+    assert int(word.item()) == 0
+    want, err, _, _ = reference(q, k, v, rows, keys, None, True, dim ** -0.5)
+    check(first, want["out"], err["out"], "out")
