@@ -41,8 +41,8 @@ struct Shape {
     static constexpr int kDim = 16 * KS;  // of a head, rounded up; TMA fills the rest with zeros
     static constexpr int kPanels = (KS + 3) / 4;
     static constexpr uint32_t kTileBytes = kPanels * kPanelBytes;
-    // NT = 1: two blocks share an SM (96 or 80 KB each); NT = 2: one block, and the ring deep
-    static constexpr int kSlots = NT == 1 ? (kPanels == 2 ? 2 : 4) : (kPanels == 2 ? 4 : 8);
+    // NT = 1: two blocks share an SM (96 or 80 KB each); NT = 2 (two panels): one block, and the ring deep
+    static constexpr int kSlots = NT == 1 && kPanels == 2 ? 2 : 4;
     static constexpr int kThreads = 128 + 128 * NT;
     static constexpr uint32_t kTmem = NT == 1 ? 256 : 512;
     static constexpr uint32_t kO = NT * 128;  // first column of the outputs, behind the score tiles
@@ -371,18 +371,27 @@ fmd_status launch(const Maps& maps, const Attn& a, int splits, cudaStream_t s) {
     return check_launch();
 }
 
-// Two tiles a block, which read each key tile once, where that gives every SM a block and a mean sequence has eight key
-// tiles; else one tile, two blocks an SM: the one hides what the other takes to start and end. One sequence of 10,000:
-// 440 us against 456; 64 of 135, forward and backward: 164 against 159.
+// Two tiles a block, which read each key tile once, for heads of more than 64 values where that gives every SM a block and a
+// mean sequence has eight key tiles; else one tile, two blocks an SM: the one hides what the other takes to start and end.
+// us with two tiles and with one, launches back to back until the clocks have settled, heads / key heads x values:
+//   1 x 10,000 causal   16/2 x 128: 434, 441    16/2 x 72: 379, 447    16/4 x 64: 364, 349    16/4 x 32: 346, 333
+//   8 x 3,000           16/4 x 128: 678, 688    16/4 x 96: 607, 628     8/2 x 64: 312, 282     8/8 x 32: 304, 282
+//   24 x 1,024          16/4 x 128: 282, 277    16/4 x 96: 257, 252     8/2 x 64: 128, 113
+// (a few launches on a GPU at rest gain less by two: 128 values, 388 and 379, 24 x 1,024 272 and 247). With fewer blocks
+// than SMs (1 x 2,500, 8/8 x 128) 54 and 62, causal 54 and 48.
+constexpr int kTwoTilesDim = 64;
+
 bool two_tiles(const Attn& a) {
-    return a.batch > 0 && tile_bound(a.rows, a.batch, 2 * (kTile / a.group)) * a.hk >= kNumSMs &&
+    return a.dim > kTwoTilesDim && a.batch > 0 && tile_bound(a.rows, a.batch, 2 * (kTile / a.group)) * a.hk >= kNumSMs &&
            a.keys / a.batch >= 8 * kTile;
 }
 
 template <int KS>
 fmd_status launch(const Maps& maps, const Attn& a, int splits, cudaStream_t s) {
     if (splits > 1) return launch<KS, 1, true>(maps, a, splits, s);
-    return two_tiles(a) ? launch<KS, 2, false>(maps, a, 1, s) : launch<KS, 1, false>(maps, a, 1, s);
+    if constexpr (16 * KS > kTwoTilesDim)
+        if (two_tiles(a)) return launch<KS, 2, false>(maps, a, 1, s);
+    return launch<KS, 1, false>(maps, a, 1, s);
 }
 
 }  // namespace

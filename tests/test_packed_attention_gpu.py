@@ -554,7 +554,7 @@ def test_offsets_that_fall_among_many_are_flagged(cuda, dtype, dim):
 
 
 def takes_two_tiles(rows, slots, hq, hk):
-    """The rule of the forward pass in 16 bits: two tiles of rows a block."""
+    """The rule of the forward pass in 16 bits for heads of more than 64 values: two tiles of rows a block."""
     blocks = (sum(rows) // (2 * (128 // (hq // hk))) + len(rows)) * hk
     return blocks >= 148 and sum(slots) // len(rows) >= 1024
 
@@ -569,8 +569,13 @@ def takes_two_tiles(rows, slots, hq, hk):
     ([1430, 1300], [1100, 1030], None, 16, 8, 72),  # causal: 330 rows see nothing, a first tile among them
     ([700, 1300, 0, 1], [1500, 1300, 1400, 1200], [1333, 1300, 5, 0], 32, 4, 64),
     ([1153] * 30, [1153] * 30, None, 2, 2, 40),
+    ([2100, 1301], [2100, 1301], None, 24, 8, 72),
+    ([2100, 1301], [2100, 1301], None, 16, 8, 120),
+    ([700, 1300, 0, 1], [1500, 1300, 1400, 1200], [1333, 1300, 5, 0], 32, 4, 128),
+    ([1153] * 30, [1153] * 30, None, 2, 2, 96),
     ([1040 + b % 5 for b in range(40)], [1040 + b % 5 for b in range(40)], None, 2, 1, 128),
-], ids=["pairs", "single", "three", "six", "more_rows", "cache", "thirty", "forty"])
+], ids=["pairs", "single", "three", "six", "more_rows", "cache", "thirty", "three_wide", "pairs_wide",
+        "cache_wide", "thirty_wide", "forty"])
 def test_two_tiles_a_block(cuda, rows, slots, counts, hq, hk, dim, causal):
     """Long sequences in 16 bits: the tiles of a block share their keys and may see different numbers of them."""
     assert takes_two_tiles(rows, slots, hq, hk)
