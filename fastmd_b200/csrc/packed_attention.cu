@@ -20,8 +20,8 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
         make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// out and lse of the splits of the keys together: out = sum_z exp(lse_z - lse) out_z. Many splits: a block per row, 32
-// threads of four values each, times eight that share the splits (their loads are what the time goes to).
+// out and lse of the splits of the keys together: out = sum_z exp(lse_z - lse) out_z. Many splits of few rows: a block
+// per row, 32 threads of four values each, times eight that share the splits (their loads are what the time goes to).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) join_kernel(const Attn a, int splits) {
     constexpr int kParts = kThreads / 32;
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Attn a, int splits
     if (quad == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? -INFINITY : top + logf(sum);
 }
 
-// The same for few splits: a thread per row and four values.
+// The same for few splits of many rows: a thread per row and four values.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) join_few_kernel(const Attn a, int splits) {
     const int quads = a.dim / 4;
@@ -87,10 +87,16 @@ __global__ void __launch_bounds__(kThreads) join_few_kernel(const Attn a, int sp
     if (quad == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? -INFINITY : top + logf(sum);
 }
 
+// A block per row where its eight parts have enough splits each for the rows that an SM has to take, about 128 rows a
+// split at the most; else a thread per four values. us of the whole call, by blocks and by threads:
+//   rows    64, splits 14: 18.4, 22.0     128,  8: 17.8, 19.5     512,  2: 38.6, 39.0     512, 32: 24.0, 33.8
+//   rows 1,024, splits  4: 22.2, 20.8   1,024,  7: 26.9, 27.0   1,024, 10: 23.4, 24.4   1,024, 32: 26.7, 33.9
+//   rows 2,048, splits  6: 34.1, 31.0   2,048, 14: 43.7, 42.2   1,536, 18: 36.2, 38.2   4,224,  4: 51.7, 42.7
 template <typename T>
 fmd_status join(const Attn& a, int splits, cudaStream_t s) {
-    const bool many = splits >= 16;
-    const int64_t all = a.rows * a.hq, blocks = many ? all : (all * (a.dim / 4) + kThreads - 1) / kThreads;
+    const int64_t all = a.rows * a.hq;
+    const bool many = all <= 128 * int64_t(splits);
+    const int64_t blocks = many ? all : (all * (a.dim / 4) + kThreads - 1) / kThreads;
     if (blocks > INT32_MAX) return FMD_ERR_UNSUPPORTED;
     if (many) join_kernel<T><<<unsigned(blocks), kThreads, 0, s>>>(a, splits);
     else join_few_kernel<T><<<unsigned(blocks), kThreads, 0, s>>>(a, splits);
