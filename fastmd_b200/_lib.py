@@ -188,7 +188,8 @@ def check(status: int, what: str) -> None:
 # kernels each entry point launches (for the launch count of a step); the default is one
 KERNELS_PER_CALL = {"fmd_refilter_edges": 2, "fmd_refilter_edges_noalloc": 2, "fmd_mace_message_bwd": 2,
                     "fmd_mace_edge_virial": 2, "fmd_reverse_pairs": 5, "fmd_line_graph": 6, "fmd_column_sum": 2,
-                    # queries, keys and the row sums before them; planes and splits of an axis add some
+                    # the least: float32 planes, splits of an axis and the weights' gradients add one each
+                    # (attention backward: queries, keys and the row sums before them)
                     "fmd_packed_attention_bwd": 3, "fmd_packed_attention_workspace_bytes": 0,
                     "fmd_head_rotary_workspace_bytes": 0}
 

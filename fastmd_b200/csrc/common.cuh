@@ -36,6 +36,11 @@ inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Rows of heads that 16-byte accesses reach: base and strides (in elements of `size` bytes) multiples of 16 bytes.
+inline bool vector_rows(const void* p, int64_t row, int64_t head, int size) {
+    return aligned16(p) && (row * size) % 16 == 0 && (head * size) % 16 == 0;
+}
+
 // Grid size for a grid-stride loop over `work` items with `threads` per CTA:
 // enough CTAs to cover the work, capped at `per_sm` resident CTAs on every SM.
 inline int grid_for(int64_t work, int threads, int per_sm = 8) {

@@ -347,10 +347,6 @@ fmd_status launch(Args& a, bool inter, bool norm, bool backward, int* blocks, cu
     return norm ? launch<T, false, true, false>(a, blocks, s) : launch<T, false, false, false>(a, blocks, s);
 }
 
-bool vector_rows(const void* p, int64_t row, int64_t head, int size) {
-    return aligned16(p) && (row * size) % 16 == 0 && (head * size) % 16 == 0;
-}
-
 }  // namespace
 }  // namespace fmd
 

@@ -127,7 +127,9 @@ fmd_status add(const float* part0, const float* part1, void* out0, void* out1, i
     return check_launch();
 }
 
-// delta[row] = sum_d g out - (gradient of lse): 8 lanes per packed row, 16-byte loads.
+// delta[row] = sum_d g out - (gradient of lse): 8 lanes per packed row, 16-byte loads. out is read as it was stored: in 16
+// bits each product carries the rounding of its value (2^-9 of it at most), which over a head's values averages out to less
+// than the rounding of the stored gradients; to keep an FP32 copy would double what the forward pass writes.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) delta_kernel(const Attn a, const float* glse, float* delta) {
     constexpr int kV = 16 / sizeof(T);
@@ -154,10 +156,6 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const Attn a, const flo
         check_sequence(a, b);
 }
 
-bool rows16(const void* p, int64_t row, int64_t head, int size) {
-    return aligned16(p) && (row * size) % 16 == 0 && (head * size) % 16 == 0;
-}
-
 fmd_status check(const fmd_attention& q, Attn& a) {
     if ((q.type != FMD_F32 && q.type != FMD_BF16) || q.rows < 0 || q.keys < 0 || q.batch < 0 || q.heads < 1 ||
         q.key_heads < 1 || q.heads % q.key_heads || q.heads / q.key_heads > 64 || q.dim < 8 || q.dim > 128 ||
@@ -166,8 +164,8 @@ fmd_status check(const fmd_attention& q, Attn& a) {
         (q.keys > 0 && (q.k == nullptr || q.v == nullptr)))
         return FMD_ERR_INVALID_ARGUMENT;
     const int size = q.type == FMD_F32 ? 4 : 2;
-    if ((q.rows > 0 && !rows16(q.q, q.q_row, q.q_head, size)) ||
-        (q.keys > 0 && (!rows16(q.k, q.k_row, q.k_head, size) || !rows16(q.v, q.v_row, q.v_head, size))) ||
+    if ((q.rows > 0 && !vector_rows(q.q, q.q_row, q.q_head, size)) ||
+        (q.keys > 0 && (!vector_rows(q.k, q.k_row, q.k_head, size) || !vector_rows(q.v, q.v_row, q.v_head, size))) ||
         q.rows > (1 << 29) || q.keys > (1 << 29) || q.batch > (1 << 24) ||
         // a block per tile (of 64 rows at least) and key head
         tile_bound(q.rows, q.batch, 64 / (q.heads / q.key_heads)) > INT32_MAX / q.key_heads ||
@@ -199,7 +197,10 @@ fmd_status check(const fmd_attention& q, Attn& a) {
     return FMD_OK;
 }
 
-// float32 heads of up to this many values go through planes on the tensor cores
+// float32 heads of up to this many values go through planes on the tensor cores, wider ones stay on the FP32 cores, whose
+// kernels are also right for every size. Forward, us by planes and on the FP32 cores: 64 slots of 2,000 keys, 2 key heads of
+// 64, one new row of 8 heads each 104 and 393, 32 rows 109 and 785, 128 rows 232 and 2,573. All rows of k and v are split,
+// filled or not, since the host knows no count: with a tenth filled 73 and 44 for one row, 113 and 245 for 128.
 constexpr int kPlanesDim = 64;
 
 // How the forward pass runs, from the sizes alone: its splits of the keys, and its workspace: planes, then the splits.
@@ -292,7 +293,7 @@ fmd_status fmd_packed_attention_bwd(const fmd_attention* problem, const void* ou
     if (a.rows > 0 && (out == nullptr || lse == nullptr || g == nullptr)) return FMD_ERR_INVALID_ARGUMENT;
     const BackwardPlan p = backward_plan(a, problem->type, dq != nullptr, dk != nullptr);
     if (workspace_bytes < p.bytes || (p.bytes > 0 && workspace == nullptr)) return FMD_ERR_WORKSPACE;
-    if ((a.rows > 0 && (!rows16(g, g_row, g_head, problem->type == FMD_F32 ? 4 : 2) || !aligned16(out))) ||
+    if ((a.rows > 0 && (!vector_rows(g, g_row, g_head, problem->type == FMD_F32 ? 4 : 2) || !aligned16(out))) ||
         !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(workspace))
         return FMD_ERR_UNSUPPORTED;
     float* delta = static_cast<float*>(workspace);

@@ -9,8 +9,9 @@
 // ds = h + m of 16 significant bits, at the price of one more product each.
 //
 // Two kernels, each of which owns the rows it writes and adds in one order, so that the gradients are the same bits on
-// every run without atomics or partial sums in memory; the price is that scores and dp are computed twice (seven
-// products for five). Both keep one side's tiles in shared memory and stream the other's:
+// every run without atomics; the price is that scores and dp are computed twice (seven products for five). Where the
+// blocks do not fill the GPU the axis they walk along is shared out: each part is then written in FP32 and a third kernel
+// adds the parts in their order. Both keep one side's tiles in shared memory and stream the other's:
 //
 //   queries  a block per 128 packed rows: S = q k^T, dP = g v^T, ds over dP in TMEM, dq += ds k
 //   keys     a block per 128 keys: S = k q^T and dP = v g^T with the keys in the lanes, so that p and ds are already

@@ -1,4 +1,4 @@
-// The tensor-core pieces that the bfloat16 attention kernels share: operand tiles, descriptors, products, TMEM access.
+// The tensor-core pieces that the attention kernels share, bfloat16 ones and those in planes of float32: operand tiles, descriptors, products, TMEM access.
 //
 // An operand tile is 128 rows of up to 128 values as panels of 64 values: panel p holds 128 rows of 128 bytes, in the
 // 128-byte swizzle that TMA writes. The same tile serves as a K-major operand (the product runs over its 64-value

@@ -1,5 +1,7 @@
 // Packed attention in float32 on the FP32 cores, for heads of more than 64 values: forward, and the gradients of q and
-// of k and v. (Smaller heads take the tensor cores: three planes of a wider tile do not fit in shared memory.)
+// of k and v. (Smaller heads take the tensor cores, in three planes. Those kernels hold their tiles in full width; for wider
+// heads the forward pass would have to keep q's planes in TMEM and stream keys by 64, the gradients to work on half a head at
+// a time. That is not built.)
 //
 //   forward   s = scale q k^T (log2 units), running maximum m and sum l per row over key tiles:
 //             o = (o 2^(m - m') + 2^(s - m') v),  l likewise;  out = o / l,  lse = m + log l
