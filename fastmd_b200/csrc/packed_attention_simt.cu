@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Attn a) {
         __syncthreads();
         float x[4][4] = {};
         dots(qs, ks, ty, tx, x);
+        float keep[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float top = -INFINITY;
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Attn a) {
             }
             top = fmaxf(m[i], max16(top));
             const float base = top == -INFINITY ? 0.0f : top;  // a row with nothing yet: exp2(-inf) stays 0
-            const float keep = exp2f(m[i] - base);
+            keep[i] = exp2f(m[i] - base);
             m[i] = top;
             float sum = 0.0f;
 #pragma unroll
@@ -168,12 +169,16 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Attn a) {
                 sum += p;
                 ps[(ty + 16 * i) * (64 + 4) + tx + 16 * j] = p;
             }
-            l[i] = l[i] * keep + sum16(sum);
-#pragma unroll
-            for (int c = 0; c < kDim / 16; ++c) o[i][c] *= keep;
+            l[i] = l[i] * keep[i] + sum16(sum);
         }
         __syncthreads();
-        weigh(ps, vs, ty, tx, o);
+        // a tile's sum starts from zero: n keys are n / 64 + 64 additions in a row, not n
+        float tile[4][kDim / 16] = {};
+        weigh(ps, vs, ty, tx, tile);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < kDim / 16; ++c) o[i][c] = fmaf(o[i][c], keep[i], tile[i][c]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

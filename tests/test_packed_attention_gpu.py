@@ -620,3 +620,23 @@ def test_gradients_of_few_keys_in_16_bits(cuda, rows, hq, hk, dim, causal):
     for name, got in zip(("dq", "dk"), grads):
         rounding = (want[name].to(B16).double() - want[name]).norm()
         assert float((got.double() - want[name]).norm()) <= 1.3 * float(rounding), name
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 72])
+def test_sums_over_many_keys_in_float32(cuda, dim):
+    """Values near 1 and 4,000 keys in one walk: 4,000 additions in a row would leave 0.29 sqrt(4000 / 3) = 11 units of 2^-24
+    (root mean square), the tiles' sums one after the other 1.3 (tiles of 64), as much again in the denominator, and the
+    last operations about one each: 5 in all."""
+    batch, slot, heads = 64, 4000, 8
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    q, k, v = (torch.randn(n, heads, dim, generator=gen, device="cuda") for n in (batch, batch * slot, batch * slot))
+    v = 1.0 + 0.1 * v
+    got = packed_attention(q, k, v, on_device(list(range(batch + 1))), on_device(starts([slot] * batch)))
+    square = 0.0
+    for b in range(0, batch, 8):
+        x, y = (t[b * slot:(b + 1) * slot].double() for t in (k, v))
+        p = torch.softmax(dim ** -0.5 * torch.einsum("hd,jhd->hj", q[b].double(), x), 1)
+        want = torch.einsum("hj,jhd->hd", p, y)
+        square += float(((got[b].double() - want) / want).square().mean()) / (batch // 8)
+    assert math.sqrt(square) <= 5 * E32
