@@ -361,6 +361,7 @@ fmd_status fmd_packed_attention_bwd(const fmd_attention* problem, const void* ou
     a.dk = dk;
     a.dv = dv;
     a.flags = flags;
+    a.lse_gradient = glse != nullptr;
     const cudaStream_t s = as_stream(stream);
     if (a.rows > 0) {
         const int64_t blocks = (a.rows * a.hq * 8 + kThreads - 1) / kThreads;

@@ -45,6 +45,7 @@ struct Attn {
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, g_row, g_head;
     float scale;
     int32_t batch, hq, hk, group, dim, causal;
+    int32_t lse_gradient;  // backward: lse has a gradient too
 };
 
 // The sequence of one block: its tokens [row0, row0 + rows), its keys [key0, key0 + keys), of a slot of `slot` rows.
@@ -187,6 +188,10 @@ __device__ __forceinline__ Place block_place(const Attn& a, int per, int* head) 
 __device__ __forceinline__ int64_t seen(const Span& s, bool causal, int64_t t) {
     return causal ? min(max(t + 1 + s.keys - s.rows, int64_t(0)), s.keys) : s.keys;
 }
+
+// Whether the scores of a row that sees `keys` keys have a gradient: the softmax of one score is 1 whatever the score, and
+// p (dp - delta) would leave the rounding of two equal numbers' difference.
+__device__ __forceinline__ bool scores_count(const Attn& a, int64_t keys) { return keys > 1 || a.lse_gradient; }
 
 // Splits of the axis that blocks walk along, for `blocks` places and `tiles` blocks of `length` steps each: the number
 // that ends first when a block takes two steps' time besides its own and adding up the splits as much again. Where the

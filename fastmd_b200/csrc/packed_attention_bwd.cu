@@ -273,7 +273,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool real = token < tokens;
         const int64_t flat = (s.row0 + token0 + token) * a.hq + head * a.group + r % a.group;
         const float lse = real ? a.lse[flat] : -INFINITY, delta = real ? a.delta[flat] : 0.0f;
-        const int limit = lse != -INFINITY ? min(max(int(seen(s, a.causal, token0 + token)) - from, 0), end) : 0;
+        const int64_t keys_seen = seen(s, a.causal, token0 + token);
+        const int limit =
+            lse != -INFINITY && scores_count(a, keys_seen) ? min(max(int(keys_seen) - from, 0), end) : 0;
         const float base = lse != -INFINITY ? -lse * kLog2e : 0.0f;
         const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), base2 = make_float2(base, base);
         const float2 delta2 = make_float2(-delta, -delta);
@@ -600,13 +602,14 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
             const bool real = key0 + r < s.slot;
             const uint32_t from = tmem + lanes + (half ? kDk : kDv);
             const float factor = half ? a.scale : 1.0f;
+            const bool keep = r < here && !(half && !scores_count(a, s.keys));
             for (int col = 0; col < S::kDim; col += 32) {
                 if (gridDim.z > 1)
-                    store_row((half ? a.part_dk : a.part_dv) + part + flat, from, col, a.dim, factor, tiles > 0, r < here,
+                    store_row((half ? a.part_dk : a.part_dv) + part + flat, from, col, a.dim, factor, tiles > 0, keep,
                               real);
                 else
                     store_row(static_cast<__nv_bfloat16*>(half ? a.dk : a.dv) + flat, from, col, a.dim, factor, tiles > 0,
-                              r < here, real);
+                              keep, real);
             }
         }
     }

@@ -566,7 +566,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool real = token < tokens;
         const int64_t flat = (s.row0 + token0 + token) * a.hq + head * a.group + r % a.group;
         const float lse = real ? a.lse[flat] : -INFINITY, delta = real ? a.delta[flat] : 0.0f;
-        const int limit = lse != -INFINITY ? min(max(int(seen(s, a.causal, token0 + token)) - from, 0), end) : 0;
+        const int64_t keys_seen = seen(s, a.causal, token0 + token);
+        const int limit =
+            lse != -INFINITY && scores_count(a, keys_seen) ? min(max(int(keys_seen) - from, 0), end) : 0;
         const float base = lse != -INFINITY ? -lse * kLog2e : 0.0f;
         const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), base2 = make_float2(base, base);
         const float2 delta2 = make_float2(-delta, -delta);
@@ -846,7 +848,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_gradient_kernel(const __grid_
             float* row = gridDim.z > 1 ? (half ? a.part_dk : a.part_dv) + int64_t(blockIdx.z) * a.keys * a.hk * a.dim
                                        : static_cast<float*>(half ? a.dk : a.dv);
             row += ((s.key0 + key0 + r) * a.hk + head) * a.dim;
-            const bool keep = key0 + r < s.keys;
+            const bool keep = key0 + r < s.keys && !(half && !scores_count(a, s.keys));
 #pragma unroll
             for (int i = 0; i < kDim / 32; ++i) {
                 if (!keep) {

@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(kThreads) query_gradient_kernel(const Attn a) 
         const int r = ty + 16 * i;
         lse2[i] = r < rows ? a.lse[at.flat(r)] * kLog2e : -INFINITY;
         limit[i] = lse2[i] != -INFINITY ? seen(s, a.causal, token0 + r / a.group) : 0;  // an empty row has no share
+        if (!scores_count(a, limit[i])) limit[i] = 0;
         delta[i] = r < rows ? a.delta[at.flat(r)] : 0.0f;
 #pragma unroll
         for (int c = 0; c < kDim / 16; ++c) dq[i][c] = 0.0f;
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(kThreads) key_gradient_kernel(const Attn a) {
         for (int c = 0; c < kDim / 16; ++c) {
             const int col = column(tx, c);
             if (col < a.dim) {
-                dk_out[flat + col] = dk[i][c] * a.scale;
+                dk_out[flat + col] = scores_count(a, s.keys) ? dk[i][c] * a.scale : 0.0f;
                 dv_out[flat + col] = dv[i][c];
             }
         }

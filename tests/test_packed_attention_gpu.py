@@ -640,3 +640,26 @@ def test_sums_over_many_keys_in_float32(cuda, dim):
         want = torch.einsum("hj,jhd->hd", p, y)
         square += float(((got[b].double() - want) / want).square().mean()) / (batch // 8)
     assert math.sqrt(square) <= 5 * E32
+
+
+@gpu
+@pytest.mark.parametrize("dtype,dim", [(F32, 32), (F32, 128), (B16, 64)], ids=["f32", "f32_wide", "b16"])
+@pytest.mark.parametrize("causal", [False, True], ids=["all", "causal"])
+def test_one_key_has_no_gradient_of_its_score(cuda, causal, dtype, dim):
+    """The softmax of one score is 1: rows that see one key give nothing to queries and keys, to the bit, and a key that is
+    alone gets nothing; with a gradient of lse they get that."""
+    rows, slots = [1, 1, 5, 3, 1], [1, 4, 5, 1, 1]
+    q, k, v, g = make(rows, slots, 6, 2, dim, dtype, seed=dim)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    ro, ko = starts(rows), starts(slots)
+    out, lse = packed_attention(*leaves, on_device(ro), on_device(ko), causal=causal, return_lse=True)
+    dq, dk, dv = torch.autograd.grad(out, leaves, g, retain_graph=True)
+    alone_q = [0, 7, 8, 9, 10] + ([2] if causal else [])  # causal: the first of five frames, and two rows that see nothing
+    assert not dq[alone_q].any() and not dk[[0, 10, 11]].any()
+    assert bool(dq[1].any()) and bool(dq[3:7].any()) and bool(dk[1:10].any()) and bool(dv[[0, 10, 11]].any())
+    glse = torch.randn(lse.shape, generator=torch.Generator().manual_seed(2)).cuda()
+    dq, dk, _ = torch.autograd.grad((out, lse), leaves, (g, glse))
+    want, err, _, _ = reference(q.detach(), k.detach(), v.detach(), ro, ko, None, causal, dim ** -0.5, g, glse)
+    check(dq, want["dq"], err["dq"], "dq")
+    check(dk, want["dk"], err["dk"], "dk")
+    assert bool(dq[0].any()) and bool(dk[0].any())
