@@ -19,7 +19,7 @@
 // in registers over the walk; a block adds its warps in warp order, a second kernel the blocks in block order: no
 // atomics, the same bits every time.
 //
-// Measured: 32,000 rows of 16 + 4 heads of 128, bfloat16: forward 80 us (4.1 TB/s), backward 137 us (3.6 TB/s) of
+// Measured: 32,000 rows of 16 + 4 heads of 128, bfloat16: forward 83 us (3.9 TB/s), backward 139 us (3.5 TB/s) of
 // the 50 and 75 us that the bytes take at the copy rate of 6.55 TB/s; what is left is latency (a third of the warps
 // fit, issue slots 57 and 48 % busy). 10,007 rows of 24 heads of 96 without a norm: 16 us (5.9 TB/s).
 
