@@ -100,10 +100,10 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, key_offse
     with the same bits on every run. Scores, softmax and sums are held in 32 bits. For bfloat16, weights are rounded to
     bfloat16 for their products with v and the output's gradient, their gradients to 16 significant bits for those with
     k and q, and the backward pass goes by the output as it is stored where a row sees more than 16 keys: errors are up
-    to 1.4 times that of rounding an exact result. A key that a row does not see has no part in it, but a value that is not finite may reach rows of its
-    own sequence that do not see it (0 * inf), and in float32 with ``dim`` up to 64 an infinity gives NaN where the
-    formula may have an infinity. There a call also reads all rows of k and v, filled or not, and needs a workspace of
-    one and a half times their bytes."""
+    to 1.4 times that of rounding an exact result. A key that a row does not see has no part in it, but a value that is
+    not finite may reach rows of its own sequence that do not see it (0 * inf), and in float32 with ``dim`` up to 64 an
+    infinity gives NaN where the formula may have an infinity. There a call also reads all rows of k and v, filled or
+    not, and needs a workspace of one and a half times their bytes."""
     _lib.require_cuda(q, k, v, offsets, key_offsets, key_counts)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
         raise ValueError("q must be [rows, heads, dim] and k and v the same [keys, key_heads, dim], got "
