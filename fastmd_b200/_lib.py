@@ -6,6 +6,7 @@ the package.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from ctypes import POINTER, c_double, c_float, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
@@ -45,6 +46,14 @@ class FmdAttention(ctypes.Structure):
                 ("q_head", c_int64), ("k_row", c_int64), ("k_head", c_int64), ("v_row", c_int64), ("v_head", c_int64),
                 ("scale", c_float), ("type", c_int32), ("batch", c_int32), ("heads", c_int32), ("key_heads", c_int32),
                 ("dim", c_int32), ("causal", c_int32), ("_pad", c_int32)]
+
+
+class FmdFeedForward(ctypes.Structure):
+    """The problem of fmd_gated_feed_forward and fmd_gated_feed_forward_bwd."""
+    _fields_ = [("x", c_void_p), ("gate", c_void_p), ("up", c_void_p), ("down", c_void_p), ("rows", c_int64),
+                ("x_row", c_int64), ("gate_row", c_int64), ("up_row", c_int64), ("down_row", c_int64),
+                ("width", c_int32), ("hidden", c_int32), ("out", c_int32), ("type", c_int32), ("activation", c_int32),
+                ("_pad", c_int32)]
 
 
 _P = c_void_p  # every device pointer and the stream travel as void*
@@ -137,6 +146,9 @@ _SIGNATURES: dict[str, list] = {
     "fmd_packed_attention_workspace_bytes": [POINTER(FmdAttention), _I32, POINTER(c_size_t)],
     "fmd_packed_attention": [POINTER(FmdAttention), _P, _P, _P, c_size_t, _P, _P],
     "fmd_packed_attention_bwd": [POINTER(FmdAttention), _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, c_size_t, _P, _P],
+    "fmd_gated_feed_forward_bytes": [POINTER(FmdFeedForward), _I32, POINTER(c_size_t), POINTER(c_size_t)],
+    "fmd_gated_feed_forward": [POINTER(FmdFeedForward), _P, _I32, _P, c_size_t, _P, c_size_t, _P, _P],
+    "fmd_gated_feed_forward_bwd": [POINTER(FmdFeedForward), _P, c_size_t, _P, _I64, _P, _P, _P, _P, _P, c_size_t, _P, _P],
     "fmd_nhc_pre_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P],
     "fmd_nhc_post_pre_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P],
     "fmd_nhc_post_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P],
@@ -191,7 +203,9 @@ KERNELS_PER_CALL = {"fmd_refilter_edges": 2, "fmd_refilter_edges_noalloc": 2, "f
                     # the least: float32 planes, splits of an axis and the weights' gradients add one each
                     # (attention backward: queries, keys and the row sums before them)
                     "fmd_packed_attention_bwd": 3, "fmd_packed_attention_workspace_bytes": 0,
-                    "fmd_head_rotary_workspace_bytes": 0}
+                    "fmd_head_rotary_workspace_bytes": 0,
+                    # up and down; hidden, input and weights (float32 planes and shares of a sum add one each)
+                    "fmd_gated_feed_forward": 2, "fmd_gated_feed_forward_bwd": 3, "fmd_gated_feed_forward_bytes": 0}
 
 
 def fused_step_kernels(n_layers: int) -> int:
@@ -236,6 +250,14 @@ def stream(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """A context in which ``device`` is the current one, for launches on tensors that may lie elsewhere."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def require_cuda(*tensors) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
@@ -259,5 +281,5 @@ def flags_word(device) -> torch.Tensor:
 c_int32_t, c_int64_t = c_int32, c_int64
 c_void_p_t = c_void_p
 
-__all__ = ["FastMDLibraryError", "FmdAttention", "FmdCatPart", "FmdHeadRotarySide", "call", "check", "declare", "flags_word", "lib", "ptr",
+__all__ = ["FastMDLibraryError", "FmdAttention", "FmdCatPart", "FmdFeedForward", "FmdHeadRotarySide", "call", "check", "declare", "flags_word", "lib", "on_device", "ptr",
            "require_cuda", "stream", "c_double", "c_float", "c_int32", "c_int64", "c_void_p", "ctypes"]

@@ -1,0 +1,910 @@
+// Gated feed-forward block and its backward pass, as products on the tensor cores with the rest of the block in them.
+//
+//   a = x Wg^T, b = x Wu^T, h = act(a) b, y = h Wd^T              x [rows, width], Wg, Wu [hidden, width], Wd [out, hidden]
+//   dh = g Wd;  da = dh (b act'(a)), db = dh act(a)
+//   dx = da Wg + db Wu;  dWg = da^T x, dWu = db^T x, dWd = g^T h
+//
+// Five products, each a kernel of the one form below; they differ in how operands lie and in what follows the sums:
+//   up       x [Wg; Wu]^T: a tile's columns are half a's and half b's, so that h follows where the sums are; where a
+//            backward pass follows, b act'(a) and act(a) are kept in FP32
+//   down     h Wd^T
+//   hidden   g Wd, times what was kept: da and db
+//   input    [da, db] [Wg; Wu]: one sum over both
+//   weights  da^T x, db^T x, g^T h: three problems of one launch
+//
+// Roundings: h, da and db are operands of further products and are stored in bfloat16; each costs the result as much as its
+// own last rounding, 1.4 of it in all. What the gradients are multiplied by stays in FP32, which would add as much again.
+//
+// float32: every operand is three planes of bfloat16 (x = x0 + x1 + x2, 24 bits) and a product is the six of its planes
+// that count: x0 w0 apart from the five small ones, because the tensor cores cut off what does not fit as they add. For the
+// same reason sums are taken out of TMEM and added up in registers every kSegment steps of 64.
+//
+// A block walks over tiles of 128 x bn: warp 0 loads operands by TMA through a ring of slots (64 values of the inner index
+// each), one thread of warp 1 issues the products, warps 4 to 11 take the sums from one of two accumulators in TMEM while
+// the other one is filled: thread = row and half of the columns.
+//
+// Every wait is bounded: on expiry the block raises FMD_FLAG_WAIT_TIMEOUT, waits (bounded) for its copies and products in
+// flight, frees its TMEM and returns.
+
+#include <cuda_bf16.h>
+
+#include "tensor_cores.cuh"
+
+namespace fmd {
+namespace {
+
+constexpr int kThreads = 384, kWorkers = 256;
+constexpr int kM = 128, kK = 64;
+constexpr uint32_t kTileA = kM * kK * 2, kPanel = 64 * kK * 2;  // bytes of an operand's tile, of 64 columns of it
+constexpr int kMostSlots = 8;
+constexpr size_t kRingBytes = 224 * 1024;
+constexpr int kSegment = 2;
+constexpr float kBf16Max = 3.38953139e38f;
+
+enum Kind { kUp, kDown, kHidden, kInput, kWeights };
+
+// One product [m, n] of a launch.
+struct Problem {
+    void* out;
+    float* part;  // [splits, m, part_row]: sums of the splits
+    int64_t m, n, part_row;
+    int32_t a, b;  // maps
+    int32_t m_tiles, n_tiles;
+};
+
+struct Args {
+    Problem problem[3];
+    int32_t problems, splits, tiles;
+    int32_t steps, turn;  // of 64 along the inner index; from step `turn` on the second pair of maps (kInput)
+    int32_t bn, slots, act;
+    // h, da and db: [planes][rows][row]; what is kept: [rows][row] FP32
+    __nv_bfloat16 *h, *da, *db;
+    float *slope, *level;
+    int64_t row, plane;
+    int32_t* flags;
+};
+
+struct Maps {
+    CUtensorMap a[3], b[3];
+};
+
+struct Ctrl {
+    uint64_t full[kMostSlots], empty[kMostSlots];
+    uint64_t sums[2], taken[2];
+    uint64_t drain;
+    uint32_t tmem;
+    int32_t abort;
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(su32(bar))
+        : "memory");
+}
+
+// Two steps of 16 of D (+)= A B^T; `astep`, `bstep`: how far a step is, in descriptor units.
+template <int ASTEP, int BSTEP>
+__device__ __forceinline__ void mma2(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 u, v, w, z;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\tadd.u32 x, %1, %6;\n\tadd.u32 y, %2, %7;\n\t"
+        "mov.b64 u, {%1, %3};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 w, {x, %3};\n\tmov.b64 z, {y, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], u, v, %4, p;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], w, z, %4, 1;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(kDescHigh), "r"(idesc), "r"(add), "n"(ASTEP), "n"(BSTEP)
+        : "memory");
+}
+
+// The place of tile t: its problem, rows and columns, and the steps of its share of the inner index.
+struct Place {
+    int problem, m, n, split, from, to;
+};
+
+__device__ __forceinline__ Place place_of(const Args& g, int t) {
+    Place p;
+    p.problem = 0;
+    while (p.problem + 1 < g.problems) {
+        const int here = g.problem[p.problem].m_tiles * g.problem[p.problem].n_tiles * g.splits;
+        if (t < here) break;
+        t -= here;
+        ++p.problem;
+    }
+    const Problem& q = g.problem[p.problem];
+    const int all = q.m_tiles * q.n_tiles;
+    p.split = t / all;
+    t -= p.split * all;
+    p.m = t / q.n_tiles;
+    p.n = t - p.m * q.n_tiles;
+    const int share = (g.steps + g.splits - 1) / g.splits;
+    p.from = min(g.steps, p.split * share);
+    p.to = min(g.steps, p.from + share);
+    return p;
+}
+
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// act(a) and act'(a). EXACT: to FP32's last bits; else to 2^-20 or so, for results in 16 bits.
+template <bool EXACT>
+__device__ __forceinline__ void activate(int act, float a, float& value, float& slope) {
+    if (act == FMD_FEED_SILU) {
+        const float turn = EXACT ? 1.0f / (1.0f + expf(-a)) : rcp(1.0f + ex2(-1.4426950408889634f * a));
+        value = a * turn;
+        slope = turn + value * (1.0f - turn);
+        if (fabsf(a) == INFINITY) {
+            value = a > 0.0f ? a : 0.0f;
+            slope = a > 0.0f ? 1.0f : 0.0f;
+        }
+    } else {
+        const float share = 0.5f * erfcf(-0.7071067811865476f * a);
+        value = a * share;
+        slope = share + a * (0.3989422804014327f * (EXACT ? expf(-0.5f * a * a) : ex2(-0.7213475204444817f * a * a)));
+        if (fabsf(a) == INFINITY) {
+            value = a > 0.0f ? a : 0.0f;
+            slope = a > 0.0f ? 1.0f : 0.0f;
+        }
+    }
+}
+
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float* v) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
+__device__ __forceinline__ void store8(float* p, const float* v) {
+    st4(p, make_float4(v[0], v[1], v[2], v[3]));
+    st4(p + 4, make_float4(v[4], v[5], v[6], v[7]));
+}
+
+__device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+
+// N values of a row from column `col` on, as far as `n`: by eights where rows start at multiples of 16 bytes.
+template <int N, typename T>
+__device__ __forceinline__ void store_row(T* row, int64_t col, int64_t n, bool vector, const float* v) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
+        if (vector) {
+            if (col + i < n) store8(row + col + i, v + i);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col + i + e < n) store1(row + col + i + e, v[i + e]);
+        }
+    }
+}
+
+// Eight values as P planes.
+template <int P>
+__device__ __forceinline__ void store_planes8(__nv_bfloat16* p, int64_t plane, const float* v) {
+    if constexpr (P == 1) {
+        store8(p, v);
+    } else {
+        float left[8];
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // held to the largest bfloat16: finite values stay finite in the first plane
+            w[i] = pack_bf16(fminf(fmaxf(v[2 * i], -kBf16Max), kBf16Max), fminf(fmaxf(v[2 * i + 1], -kBf16Max), kBf16Max));
+            const float2 part = unpack_bf16(w[i]);
+            left[2 * i] = v[2 * i] - part.x;
+            left[2 * i + 1] = v[2 * i + 1] - part.y;
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+        for (int i = 1; i < P; ++i) {
+            next_plane<4>(left, w);
+            *reinterpret_cast<uint4*>(p + i * plane) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+// What follows the sums of 64 columns of one row: of kUp 32 of a and 32 of b, whose place among the hidden units is col.
+template <int KIND, int P>
+__device__ __forceinline__ void finish(const Args& g, const Problem& q, const Place& p, int64_t row, int64_t col,
+                                       float (&v)[64]) {
+    using T = typename std::conditional<P == 1, __nv_bfloat16, float>::type;
+    if constexpr (KIND == kUp) {
+        const bool kept = g.slope != nullptr;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+            if (col + i >= q.n) break;  // rows are padded to multiples of 8, and get zeros there
+            float h[8], slope[8], level[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                activate<P == 3>(g.act, v[i + e], level[e], slope[e]);
+                h[e] = level[e] * v[32 + i + e];
+                slope[e] *= v[32 + i + e];
+            }
+            const int64_t at = row * g.row + col + i;
+            store_planes8<P>(g.h + at, g.plane, h);
+            if (kept) {
+                store8(g.slope + at, slope);
+                store8(g.level + at, level);
+            }
+        }
+    } else if constexpr (KIND == kHidden) {
+#pragma unroll
+        for (int i = 0; i < 64; i += 8) {
+            if (col + i >= q.n) break;
+            const int64_t at = row * g.row + col + i;
+            float da[8], db[8];
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const float4 s = ldg4(g.slope + at + e), l = ldg4(g.level + at + e);
+                da[e] = v[i + e] * s.x;
+                da[e + 1] = v[i + e + 1] * s.y;
+                da[e + 2] = v[i + e + 2] * s.z;
+                da[e + 3] = v[i + e + 3] * s.w;
+                db[e] = v[i + e] * l.x;
+                db[e + 1] = v[i + e + 1] * l.y;
+                db[e + 2] = v[i + e + 2] * l.z;
+                db[e + 3] = v[i + e + 3] * l.w;
+            }
+            store_planes8<P>(g.da + at, g.plane, da);
+            store_planes8<P>(g.db + at, g.plane, db);
+        }
+    } else if (g.splits > 1) {
+        store_row<64>(q.part + (int64_t(p.split) * q.m + row) * q.part_row, col, q.n, true, v);
+    } else {
+        store_row<64>(static_cast<T*>(q.out) + row * q.n, col, q.n, q.n % 8 == 0, v);
+    }
+}
+
+template <int KIND, int P>
+__global__ void __launch_bounds__(kThreads, 1) feed_kernel(const __grid_constant__ Maps maps, const Args g) {
+    constexpr bool kColumnsA = KIND == kWeights, kColumnsB = KIND == kHidden || KIND == kInput || KIND == kWeights;
+    extern __shared__ unsigned char raw[];
+    const uint32_t ring = (su32(raw) + 1023u) & ~1023u;
+    __shared__ Ctrl ctl;
+    volatile int32_t* abort = &ctl.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t tile_b = uint32_t(g.bn) * 128u, slot_bytes = P * (kTileA + tile_b);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kMostSlots; ++i) {
+            mbar_init(&ctl.full[i], 1);
+            mbar_init(&ctl.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ctl.sums[i], 1);
+            mbar_init(&ctl.taken[i], kWorkers / 32);
+        }
+        mbar_init(&ctl.drain, 1);
+        ctl.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc<512>(&ctl.tmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl.tmem;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int slot = 0;
+            uint32_t phase = 0, armed = 0;  // armed: slots with a copy that nobody may have waited for
+            bool ok = true;
+            for (int t = blockIdx.x; t < g.tiles && ok; t += gridDim.x) {
+                const Place p = place_of(g, t);
+                const Problem& q = g.problem[p.problem];
+                const int m0 = p.m * kM, n0 = p.n * (KIND == kUp ? g.bn / 2 : g.bn);
+                for (int step = p.from; step < p.to; ++step) {
+                    if (!mbar_wait(&ctl.empty[slot], phase ^ 1u, abort)) {
+                        ok = false;
+                        break;
+                    }
+                    uint64_t* bar = &ctl.full[slot];
+                    mbar_expect_tx(bar, slot_bytes);
+                    armed |= 1u << slot;
+                    const uint32_t at = ring + uint32_t(slot) * slot_bytes;
+                    const bool second = KIND == kInput && step >= g.turn;
+                    const int k0 = (second ? step - g.turn : step) * kK;
+                    const CUtensorMap *ma = &maps.a[second ? 1 : q.a], *mb = &maps.b[second ? 1 : q.b];
+                    for (int i = 0; i < P; ++i) {
+                        const uint32_t a = at + i * kTileA, b = at + P * kTileA + uint32_t(i) * tile_b;
+                        if (kColumnsA) {
+                            tma_load_3d(a, ma, bar, m0, k0, i);
+                            tma_load_3d(a + kPanel, ma, bar, m0 + 64, k0, i);
+                        } else {
+                            tma_load_3d(a, ma, bar, k0, m0, i);
+                        }
+                        if (KIND == kUp) {
+                            tma_load_3d(b, &maps.b[0], bar, k0, n0, i);
+                            tma_load_3d(b + tile_b / 2, &maps.b[1], bar, k0, n0, i);
+                        } else if (kColumnsB) {
+                            for (int c = 0; c < g.bn / 64; ++c)
+                                tma_load_3d(b + c * kPanel, mb, bar, n0 + 64 * c, k0, i);
+                        } else {
+                            tma_load_3d(b, mb, bar, k0, n0, i);
+                        }
+                    }
+                    if (++slot == g.slots) {
+                        slot = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            // the block ends after the copies in flight and, where all went well, after the products that read them
+            for (int i = 0; i < g.slots; ++i) {
+                const uint32_t turns = phase + (i < slot ? 1u : 0u);  // parity of the number of uses of slot i
+                if (!(armed >> i & 1u)) continue;
+                if (ok) ok = mbar_wait(&ctl.empty[i], (turns ^ 1u) & 1u, abort);
+                if (!ok) mbar_wait(&ctl.full[i], (turns ^ 1u) & 1u, abort, true);
+            }
+        }
+    } else if (warp == 1) {
+        const uint32_t base = uniform(tmem), first = uniform(ring), bytes = uniform(slot_bytes), b_bytes = uniform(tile_b);
+        const int slots = uniform(g.slots), bn = uniform(g.bn);
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (kColumnsA ? 1u << 15 : 0u) |
+                               (kColumnsB ? 1u << 16 : 0u) | (uint32_t(bn >> 3) << 17) | (uint32_t(kM >> 4) << 24);
+        constexpr int kStepA = kColumnsA ? 128 : 2, kStepB = kColumnsB ? 128 : 2;
+        auto desc = [](uint32_t at, bool columns) {
+            return ((at & 0x3FFFFu) >> 4) | (columns ? (kPanel >> 4) << 16 : 1u << 16);
+        };
+        int slot = 0, unit = 0;
+        uint32_t phase = 0;
+        bool ok = true, issued = false;
+        for (int t = blockIdx.x; t < g.tiles && ok; t += gridDim.x) {
+            const Place p = place_of(g, t);
+            const int from = uniform(p.from), to = uniform(p.to);
+            for (int start = from; start < to && ok; ++unit) {
+                const int end = P == 1 ? to : min(to, start + kSegment);
+                const uint32_t d = base + uint32_t(unit & 1) * 256u;
+                ok = warp_wait(&ctl.taken[unit & 1], (uint32_t(unit >> 1) & 1u) ^ 1u, abort);
+                for (int step = start; step < end && ok; ++step) {
+                    ok = warp_wait(&ctl.full[slot], phase, abort);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t at = first + uint32_t(slot) * bytes;
+                    if (elect_one()) {
+                        const uint32_t a = desc(at, kColumnsA), b = desc(at + P * kTileA, kColumnsB);
+                        const bool add = step > start;
+                        if (P == 1) {
+                            mma2<kStepA, kStepB>(d, a, b, idesc, add);
+                            mma2<kStepA, kStepB>(d, a + 2 * kStepA, b + 2 * kStepB, idesc, true);
+                        } else {  // the small products first, into sums of their own
+                            constexpr int kPa[6] = {2, 1, 0, 1, 0, 0}, kPb[6] = {0, 1, 2, 0, 1, 0};
+#pragma unroll
+                            for (int i = 0; i < 6; ++i) {
+                                const uint32_t x = a + kPa[i] * (kTileA >> 4), y = b + kPb[i] * (b_bytes >> 4);
+                                const uint32_t to_sum = i < 5 ? d + 128 : d;
+                                mma2<kStepA, kStepB>(to_sum, x, y, idesc, add || (i > 0 && i < 5));
+                                mma2<kStepA, kStepB>(to_sum, x + 2 * kStepA, y + 2 * kStepB, idesc, true);
+                            }
+                        }
+                        tc_commit(&ctl.empty[slot]);
+                        if (step + 1 == end) tc_commit(&ctl.sums[unit & 1]);
+                    }
+                    issued = true;
+                    if (++slot == slots) {
+                        slot = 0;
+                        phase ^= 1u;
+                    }
+                }
+                start = end;
+            }
+        }
+        if (!ok && issued) {  // the products in flight end before TMEM is freed
+            if (elect_one()) tc_commit(&ctl.drain);
+            warp_wait(&ctl.drain, 0, abort, true);
+        }
+    } else if (warp >= 4) {
+        const int half = (warp - 4) >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        int unit = 0;
+        bool ok = true;
+        auto wait = [&]() {  // uniform in the warp: TMEM access is .sync.aligned
+            const bool got = mbar_wait(&ctl.sums[unit & 1], uint32_t(unit >> 1) & 1u, abort);
+            if (!__all_sync(0xffffffffu, got)) {
+                *abort = 1;
+                return false;
+            }
+            tc_fence_after();
+            return true;
+        };
+        auto done = [&]() {
+            tc_fence_before();
+            warp_arrive(&ctl.taken[unit & 1]);
+            ++unit;
+        };
+        // columns of TMEM and of the result that this thread's 64 sums of round `it` begin at
+        auto first_of = [&](int it) { return KIND == kUp ? half * (g.bn / 4) + it * 32 : half * (g.bn / 2) + it * 64; };
+        auto load = [&](uint32_t at, int col, float (&v)[64]) {
+            if (KIND == kUp) {
+                tmem_load32(at + col, reinterpret_cast<float(&)[32]>(v[0]));
+                tmem_load32(at + g.bn / 2 + col, reinterpret_cast<float(&)[32]>(v[32]));
+            } else {
+                tmem_load64(at + col, v);
+            }
+        };
+        for (int t = blockIdx.x; t < g.tiles && ok; t += gridDim.x) {
+            const Place p = place_of(g, t);
+            const Problem& q = g.problem[p.problem];
+            const int64_t row = int64_t(p.m) * kM + r, n0 = int64_t(p.n) * (KIND == kUp ? g.bn / 2 : g.bn);
+            if (p.from >= p.to) {  // a split without a share: sums of zero
+                float v[64] = {};
+                for (int it = 0; it < g.bn / 128; ++it)
+                    if (row < q.m) finish<KIND, P>(g, q, p, row, n0 + first_of(it), v);
+                continue;
+            }
+            if constexpr (P == 1) {
+                if (!(ok = wait())) break;
+                const uint32_t at = tmem + lanes + uint32_t(unit & 1) * 256u;
+                const int rounds = g.bn / 128;
+                for (int it = 0; it < rounds; ++it) {
+                    float v[64];
+                    load(at, first_of(it), v);
+                    if (it + 1 == rounds) done();
+                    if (row < q.m) finish<KIND, P>(g, q, p, row, n0 + first_of(it), v);
+                }
+            } else {
+                float sum[64] = {};
+                for (int start = p.from; start < p.to; start += kSegment) {
+                    if (!(ok = wait())) break;
+                    const uint32_t at = tmem + lanes + uint32_t(unit & 1) * 256u;
+#pragma unroll
+                    for (int j = 0; j < 64; j += 32) {
+                        const uint32_t col = uint32_t(first_of(0)) + (KIND == kUp && j > 0 ? g.bn / 2 : j);
+                        float big[32], small[32];
+                        tmem_load32(at + col, big);
+                        tmem_load32(at + 128 + col, small);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sum[j + i] += big[i] + small[i];
+                    }
+                    done();
+                }
+                if (!ok) break;
+                if (row < q.m) finish<KIND, P>(g, q, p, row, n0 + first_of(0), sum);
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_free<512>(tmem);
+    if (threadIdx.x == 0 && ctl.abort) raise_flag(g.flags, FMD_FLAG_WAIT_TIMEOUT);
+}
+
+// ------------------------------------------------------------------- planes and sums of splits
+
+// float32 [rows, columns] as three planes [3][rows][row] of bfloat16, up to four arrays (blockIdx.y).
+struct SplitArgs {
+    const float* x[4];
+    __nv_bfloat16* to[4];
+    int64_t rows[4], from_row[4], row[4];
+    int32_t columns[4];
+};
+
+__global__ void __launch_bounds__(256) split_kernel(const SplitArgs a) {
+    const int t = blockIdx.y, per = int(a.row[t] / 8), n = a.columns[t];
+    const int64_t all = a.rows[t] * per, plane = a.rows[t] * a.row[t];
+    const bool vector = a.from_row[t] % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x[t]) & 15u) == 0;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += int64_t(gridDim.x) * 256) {
+        const int64_t row = i / per;
+        const int c = int(i - row * per) * 8;
+        const float* x = a.x[t] + row * a.from_row[t] + c;
+        float v[8];
+        if (vector && c + 8 <= n) {
+            const float4 p = ldg4(x), q = ldg4(x + 4);
+            v[0] = p.x, v[1] = p.y, v[2] = p.z, v[3] = p.w, v[4] = q.x, v[5] = q.y, v[6] = q.z, v[7] = q.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = c + e < n ? x[e] : 0.0f;
+        }
+        store_planes8<3>(a.to[t] + row * a.row[t] + c, plane, v);
+    }
+}
+
+// out [m, n] = the sum of the splits' parts, in their order; a thread per four columns, blockIdx.y: the problem.
+template <typename T>
+__global__ void __launch_bounds__(256) add_kernel(const Args g) {
+    const Problem& q = g.problem[blockIdx.y];
+    const int64_t per = (q.n + 3) / 4, all = q.m * per;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += int64_t(gridDim.x) * 256) {
+        const int64_t row = i / per;
+        const int64_t col = (i - row * per) * 4;
+        float4 sum = f4_zero();
+#pragma unroll 4
+        for (int z = 0; z < g.splits; ++z)
+            sum = f4_add(sum, *reinterpret_cast<const float4*>(q.part + (int64_t(z) * q.m + row) * q.part_row + col));
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+        T* out = static_cast<T*>(q.out) + row * q.n + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < q.n) store1(out + e, v[e]);
+    }
+}
+
+// ------------------------------------------------------------------- host
+
+// A matrix of bfloat16 as TMA reads it: `planes` of [rows, columns] with rows `row` apart.
+struct Matrix {
+    const void* data;
+    int64_t rows, columns, row;
+    int planes;
+};
+
+fmd_status encode(CUtensorMap* map, const Matrix& x, int box_rows) {
+    const DriverCalls& drv = driver_calls();
+    const int64_t row = x.rows == 1 ? (x.columns + 7) / 8 * 8 : x.row;
+    const cuuint64_t dims[3] = {cuuint64_t(x.columns), cuuint64_t(x.rows), cuuint64_t(x.planes)};
+    const cuuint64_t strides[2] = {cuuint64_t(row) * 2, cuuint64_t(x.planes == 1 ? row * x.rows : x.row * x.rows) * 2};
+    const cuuint32_t box[3] = {64, cuuint32_t(box_rows), 1}, step[3] = {1, 1, 1};
+    const CUresult r = drv.encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(x.data), dims, strides, box,
+                                  step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? FMD_OK : record_error_text(FMD_ERR_CUDA, "cuTensorMapEncodeTiled failed, CUresult", r);
+}
+
+int64_t round_up(int64_t v, int64_t unit) { return (v + unit - 1) / unit * unit; }
+
+// How a product runs: columns of a tile, and shares of the inner index.
+struct Plan {
+    int bn, splits;
+};
+
+// The time of a launch in steps of 128 x 256 x 64: rounds of blocks, each its tile's steps and, besides, about four for
+// its start and end (its output for kinds that write much); the shares' sums are written and read again.
+Plan plan(const int64_t* m, const int64_t* n, int problems, int64_t steps, int planes, bool can_split) {
+    Plan best{128, 1};
+    double least = 1e300;
+    for (int bn = 128; bn <= (planes == 1 ? 256 : 128); bn *= 2) {
+        int64_t tiles = 0;
+        for (int i = 0; i < problems; ++i) tiles += ((m[i] + kM - 1) / kM) * ((n[i] + bn - 1) / bn);
+        for (int splits = 1; splits <= (can_split ? 64 : 1) && (splits == 1 || 4 * splits <= steps); ++splits) {
+            const int64_t rounds = (tiles * splits + kNumSMs - 1) / kNumSMs;
+            const double step = (planes == 1 ? 1.0 : 6.0) * (bn == 256 ? 1.0 : 0.6);
+            const double time = rounds * (((steps + splits - 1) / splits) * step + 4.0) + (splits > 1 ? 16.0 + splits : 0.0);
+            if (time < least) {
+                least = time;
+                best = Plan{bn, splits};
+            }
+        }
+    }
+    return best;
+}
+
+struct Sizes {
+    int64_t rows, width, hidden, out;
+    int planes;  // 3: float32
+    int64_t hidden_row, width_row, out_row;  // of the arrays made here
+};
+
+template <int KIND, int P>
+fmd_status launch(const Maps& maps, const Args& g, cudaStream_t s) {
+    constexpr size_t bytes = kRingBytes + 1024;
+    const fmd_status st = grant_dynamic_smem((const void*)feed_kernel<KIND, P>, bytes, true);
+    if (st != FMD_OK) return st;
+    feed_kernel<KIND, P><<<unsigned(g.tiles < kNumSMs ? g.tiles : kNumSMs), kThreads, bytes, s>>>(maps, g);
+    return check_launch();
+}
+
+template <int KIND>
+fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args& g, const Plan& p, cudaStream_t s) {
+    Maps maps{};
+    const bool columns_a = KIND == kWeights, columns_b = KIND == kHidden || KIND == kInput || KIND == kWeights;
+    for (int i = 0; i < operands; ++i) {
+        fmd_status st = FMD_OK;
+        if (a[i].data != nullptr) st = encode(&maps.a[i], a[i], columns_a ? kK : kM);
+        if (st == FMD_OK && b[i].data != nullptr)
+            st = encode(&maps.b[i], b[i], columns_b ? kK : KIND == kUp ? p.bn / 2 : p.bn);
+        if (st != FMD_OK) return st;
+    }
+    g.bn = p.bn;
+    g.splits = p.splits;
+    const int slots = int(kRingBytes / (planes * (kTileA + p.bn * 128)));
+    g.slots = slots < kMostSlots ? slots : kMostSlots;
+    g.tiles = 0;
+    for (int i = 0; i < g.problems; ++i) {
+        Problem& q = g.problem[i];
+        const int columns = KIND == kUp ? p.bn / 2 : p.bn;
+        q.m_tiles = int((q.m + kM - 1) / kM);
+        q.n_tiles = int((q.n + columns - 1) / columns);
+        q.part_row = round_up(q.n, 8);
+        g.tiles += q.m_tiles * q.n_tiles * p.splits;
+    }
+    if (g.tiles == 0) return FMD_OK;
+    fmd_status st = planes == 1 ? launch<KIND, 1>(maps, g, s) : launch<KIND, 3>(maps, g, s);
+    if (st != FMD_OK || p.splits == 1) return st;
+    int64_t most = 0;
+    for (int i = 0; i < g.problems; ++i) {
+        const int64_t all = g.problem[i].m * ((g.problem[i].n + 3) / 4);
+        most = all > most ? all : most;
+    }
+    const dim3 grid(unsigned(grid_for(most, 256)), unsigned(g.problems));
+    if (planes == 1) add_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(g);
+    else add_kernel<float><<<grid, 256, 0, s>>>(g);
+    return check_launch();
+}
+
+int64_t steps_of(int64_t k) { return (k + kK - 1) / kK; }
+
+size_t part_bytes(const Plan& p, int64_t m, int64_t n) {
+    return p.splits > 1 ? size_t(p.splits) * m * round_up(n, 8) * sizeof(float) : 0;
+}
+
+Plan down_plan(const Sizes& z) { return plan(&z.rows, &z.out, 1, steps_of(z.hidden), z.planes, true); }
+Plan input_plan(const Sizes& z) { return plan(&z.rows, &z.width, 1, 2 * steps_of(z.hidden), z.planes, true); }
+Plan weights_plan(const Sizes& z) {
+    const int64_t m[3] = {z.hidden, z.hidden, z.out}, n[3] = {z.width, z.width, z.hidden};
+    return plan(m, n, 3, steps_of(z.rows), z.planes, true);
+}
+
+// Arrays in one buffer, each at a multiple of 256 bytes.
+struct Layout {
+    size_t bytes = 0;
+    size_t take(size_t n) {
+        const size_t at = bytes;
+        bytes += (n + 255) / 256 * 256;
+        return at;
+    }
+};
+
+// What the forward pass keeps for the backward pass: h, FP32 factors, and in float32 the planes of what it was given.
+struct Kept {
+    size_t h, slope, level, x, gate, up, down, bytes;
+};
+
+Kept kept_layout(const Sizes& z, bool factors) {
+    Layout at;
+    Kept k{};
+    const size_t hidden = size_t(z.rows) * z.hidden_row;
+    k.h = at.take(hidden * z.planes * 2);
+    if (factors) {
+        k.slope = at.take(hidden * 4);
+        k.level = at.take(hidden * 4);
+    }
+    if (z.planes == 3) {
+        k.x = at.take(size_t(z.rows) * z.width_row * 6);
+        k.gate = at.take(size_t(z.hidden) * z.width_row * 6);
+        k.up = at.take(size_t(z.hidden) * z.width_row * 6);
+        k.down = at.take(size_t(z.out) * z.hidden_row * 6);
+    }
+    k.bytes = at.bytes;
+    return k;
+}
+
+// The backward pass's workspace: da, db, the planes of g, and sums of splits (of one product at a time).
+struct Scratch {
+    size_t da, db, g, part, bytes;
+};
+
+Scratch scratch_layout(const Sizes& z) {
+    Layout at;
+    Scratch k{};
+    const size_t hidden = size_t(z.rows) * z.hidden_row * z.planes * 2;
+    k.da = at.take(hidden);
+    k.db = at.take(hidden);
+    if (z.planes == 3) k.g = at.take(size_t(z.rows) * z.out_row * 6);
+    const Plan w = weights_plan(z);
+    const size_t weights = 2 * part_bytes(w, z.hidden, z.width) + part_bytes(w, z.out, z.hidden);
+    const size_t input = part_bytes(input_plan(z), z.rows, z.width);
+    k.part = at.take(weights > input ? weights : input);
+    k.bytes = at.bytes;
+    return k;
+}
+
+fmd_status check(const fmd_feed_forward& f, Sizes& z) {
+    if ((f.type != FMD_F32 && f.type != FMD_BF16) || (f.activation != FMD_FEED_SILU && f.activation != FMD_FEED_GELU) ||
+        f.rows < 0 || f.width < 1 || f.hidden < 1 || f.out < 1 || (f.rows > 0 && f.x == nullptr) || f.gate == nullptr ||
+        f.up == nullptr || f.down == nullptr || (f.rows > 1 && f.x_row < f.width) ||
+        (f.hidden > 1 && (f.gate_row < f.width || f.up_row < f.width)) || (f.out > 1 && f.down_row < f.hidden))
+        return FMD_ERR_INVALID_ARGUMENT;
+    if (f.rows > (1 << 28) || f.width > (1 << 20) || f.hidden > (1 << 20) || f.out > (1 << 20)) return FMD_ERR_UNSUPPORTED;
+    if (f.type == FMD_BF16 &&
+        ((f.rows > 0 && !vector_rows(f.x, f.rows > 1 ? f.x_row : 0, 0, 2)) ||
+         !vector_rows(f.gate, f.hidden > 1 ? f.gate_row : 0, 0, 2) || !vector_rows(f.up, f.hidden > 1 ? f.up_row : 0, 0, 2) ||
+         !vector_rows(f.down, f.out > 1 ? f.down_row : 0, 0, 2)))
+        return FMD_ERR_UNSUPPORTED;
+    z = Sizes{f.rows, f.width, f.hidden, f.out, f.type == FMD_F32 ? 3 : 1, round_up(f.hidden, 8), round_up(f.width, 8),
+              round_up(f.out, 8)};
+    // tiles are counted in 32 bits
+    if (((z.rows + 127) / 128) * ((z.hidden + 63) / 64 + (z.width + 63) / 64 + (z.out + 63) / 64) * 64 > INT32_MAX)
+        return FMD_ERR_UNSUPPORTED;
+    return FMD_OK;
+}
+
+fmd_status ready() {
+    const DriverCalls& drv = driver_calls();
+    if (drv.encode == nullptr || drv.ctx_get_current == nullptr)
+        return record_error_text(FMD_ERR_CUDA, "driver entry point cuTensorMapEncodeTiled unavailable", 0);
+    return bind_context(drv);
+}
+
+void add_split(SplitArgs& a, int& count, const void* x, void* to, int64_t rows, int64_t columns, int64_t from_row,
+               int64_t row) {
+    a.x[count] = static_cast<const float*>(x);
+    a.to[count] = static_cast<__nv_bfloat16*>(to);
+    a.rows[count] = rows;
+    a.columns[count] = int32_t(columns);
+    a.from_row[count] = from_row;
+    a.row[count++] = row;
+}
+
+fmd_status split(const SplitArgs& a, int count, cudaStream_t s) {
+    int64_t most = 0;
+    for (int i = 0; i < count; ++i) most = a.rows[i] * (a.row[i] / 8) > most ? a.rows[i] * (a.row[i] / 8) : most;
+    split_kernel<<<dim3(unsigned(grid_for(most, 256)), unsigned(count)), 256, 0, s>>>(a);
+    return check_launch();
+}
+
+// x and the weights as the products read them.
+struct Inputs {
+    Matrix x, gate, up, down;
+};
+
+Inputs inputs_of(const fmd_feed_forward& f, const Sizes& z, const Kept& k, char* kept) {
+    if (z.planes == 1)
+        return Inputs{{f.x, z.rows, z.width, f.x_row, 1}, {f.gate, z.hidden, z.width, f.gate_row, 1},
+                      {f.up, z.hidden, z.width, f.up_row, 1}, {f.down, z.out, z.hidden, f.down_row, 1}};
+    return Inputs{{kept + k.x, z.rows, z.width, z.width_row, 3}, {kept + k.gate, z.hidden, z.width, z.width_row, 3},
+                  {kept + k.up, z.hidden, z.width, z.width_row, 3}, {kept + k.down, z.out, z.hidden, z.hidden_row, 3}};
+}
+
+}  // namespace
+}  // namespace fmd
+
+using namespace fmd;
+
+extern "C" {
+
+fmd_status fmd_gated_feed_forward_bytes(const fmd_feed_forward* problem, int32_t backward, size_t* kept,
+                                        size_t* workspace) {
+    Sizes z;
+    if (problem == nullptr || kept == nullptr || workspace == nullptr) return FMD_ERR_INVALID_ARGUMENT;
+    const fmd_status st = check(*problem, z);
+    if (st != FMD_OK) return st;
+    *kept = kept_layout(z, backward != 0).bytes;
+    if (backward) *workspace = z.rows > 0 ? scratch_layout(z).bytes : 0;
+    else *workspace = part_bytes(down_plan(z), z.rows, z.out);
+    return FMD_OK;
+}
+
+fmd_status fmd_gated_feed_forward(const fmd_feed_forward* problem, void* y, int32_t keep, void* kept, size_t kept_bytes,
+                                  void* workspace, size_t workspace_bytes, int32_t* flags, void* stream) {
+    Sizes z;
+    if (problem == nullptr) return FMD_ERR_INVALID_ARGUMENT;
+    fmd_status st = check(*problem, z);
+    if (st != FMD_OK || z.rows == 0) return st;
+    const Kept k = kept_layout(z, keep != 0);
+    const Plan down = down_plan(z);
+    if (y == nullptr) return FMD_ERR_INVALID_ARGUMENT;
+    if (kept_bytes < k.bytes || kept == nullptr || workspace_bytes < part_bytes(down, z.rows, z.out) ||
+        (down.splits > 1 && workspace == nullptr))
+        return FMD_ERR_WORKSPACE;
+    if (!aligned16(y) || !aligned16(kept) || !aligned16(workspace)) return FMD_ERR_UNSUPPORTED;
+    if ((st = ready()) != FMD_OK) return st;
+    const cudaStream_t s = as_stream(stream);
+    char* at = static_cast<char*>(kept);
+    const fmd_feed_forward& f = *problem;
+    const Inputs in = inputs_of(f, z, k, at);
+    if (z.planes == 3) {
+        SplitArgs a{};
+        int count = 0;
+        add_split(a, count, f.x, at + k.x, z.rows, z.width, f.x_row, z.width_row);
+        add_split(a, count, f.gate, at + k.gate, z.hidden, z.width, f.gate_row, z.width_row);
+        add_split(a, count, f.up, at + k.up, z.hidden, z.width, f.up_row, z.width_row);
+        add_split(a, count, f.down, at + k.down, z.out, z.hidden, f.down_row, z.hidden_row);
+        if ((st = split(a, count, s)) != FMD_OK) return st;
+    }
+    Args g{};
+    g.problems = 1;
+    g.flags = flags;
+    g.act = f.activation;
+    g.h = reinterpret_cast<__nv_bfloat16*>(at + k.h);
+    g.row = z.hidden_row;
+    g.plane = z.rows * z.hidden_row;
+    if (keep) {
+        g.slope = reinterpret_cast<float*>(at + k.slope);
+        g.level = reinterpret_cast<float*>(at + k.level);
+    }
+    g.problem[0].m = z.rows;
+    g.problem[0].n = z.hidden;
+    g.steps = int(steps_of(z.width));
+    {
+        const Matrix a[2] = {in.x, {}}, b[2] = {in.gate, in.up};
+        const int64_t twice = 2 * z.hidden;  // two columns of sums for one of h
+        if ((st = run<kUp>(z.planes, a, b, 2, g, plan(&z.rows, &twice, 1, g.steps, z.planes, false), s)) != FMD_OK) return st;
+    }
+    g.problem[0].n = z.out;
+    g.problem[0].out = y;
+    g.problem[0].part = static_cast<float*>(workspace);
+    g.steps = int(steps_of(z.hidden));
+    const Matrix h{at + k.h, z.rows, z.hidden, z.hidden_row, z.planes};
+    return run<kDown>(z.planes, &h, &in.down, 1, g, down, s);
+}
+
+fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kept, size_t kept_bytes, const void* g,
+                                      int64_t g_row, void* dx, void* dgate, void* dup, void* ddown, void* workspace,
+                                      size_t workspace_bytes, int32_t* flags, void* stream) {
+    Sizes z;
+    if (problem == nullptr) return FMD_ERR_INVALID_ARGUMENT;
+    fmd_status st = check(*problem, z);
+    if (st != FMD_OK) return st;
+    const fmd_feed_forward& f = *problem;
+    const cudaStream_t s = as_stream(stream);
+    const int size = z.planes == 1 ? 2 : 4;
+    if (z.rows == 0) {  // nothing was summed
+        void* const out[3] = {dgate, dup, ddown};
+        const int64_t values[3] = {z.hidden * z.width, z.hidden * z.width, z.out * z.hidden};
+        for (int i = 0; i < 3; ++i) {
+            if (out[i] == nullptr) continue;
+            const cudaError_t err = cudaMemsetAsync(out[i], 0, size_t(values[i]) * size, s);
+            if (err != cudaSuccess) return record_cuda_error(err);
+        }
+        return FMD_OK;
+    }
+    const Kept k = kept_layout(z, true);
+    const Scratch w = scratch_layout(z);
+    if (g == nullptr || (z.rows > 1 && g_row < z.out)) return FMD_ERR_INVALID_ARGUMENT;
+    if (kept == nullptr || kept_bytes < k.bytes || workspace == nullptr || workspace_bytes < w.bytes)
+        return FMD_ERR_WORKSPACE;
+    if (!aligned16(kept) || !aligned16(workspace) || !aligned16(dx) || !aligned16(dgate) || !aligned16(dup) ||
+        !aligned16(ddown) || (z.planes == 1 && !vector_rows(g, z.rows > 1 ? g_row : 0, 0, 2)))
+        return FMD_ERR_UNSUPPORTED;
+    if ((st = ready()) != FMD_OK) return st;
+    char *at = static_cast<char*>(kept), *own = static_cast<char*>(workspace);
+    const Inputs in = inputs_of(f, z, k, at);
+    Matrix gm{g, z.rows, z.out, g_row, 1};
+    if (z.planes == 3) {
+        SplitArgs a{};
+        int count = 0;
+        add_split(a, count, g, own + w.g, z.rows, z.out, g_row, z.out_row);
+        if ((st = split(a, count, s)) != FMD_OK) return st;
+        gm = Matrix{own + w.g, z.rows, z.out, z.out_row, 3};
+    }
+    Args args{};
+    args.flags = flags;
+    args.row = z.hidden_row;
+    args.plane = z.rows * z.hidden_row;
+    args.slope = reinterpret_cast<float*>(at + k.slope);
+    args.level = reinterpret_cast<float*>(at + k.level);
+    args.da = reinterpret_cast<__nv_bfloat16*>(own + w.da);
+    args.db = reinterpret_cast<__nv_bfloat16*>(own + w.db);
+    float* part = reinterpret_cast<float*>(own + w.part);
+    if (dx != nullptr || dgate != nullptr || dup != nullptr) {
+        args.problems = 1;
+        args.problem[0].m = z.rows;
+        args.problem[0].n = z.hidden;
+        args.steps = int(steps_of(z.out));
+        st = run<kHidden>(z.planes, &gm, &in.down, 1, args,
+                          plan(&z.rows, &z.hidden, 1, args.steps, z.planes, false), s);
+        if (st != FMD_OK) return st;
+    }
+    const Matrix da{own + w.da, z.rows, z.hidden, z.hidden_row, z.planes}, db{own + w.db, z.rows, z.hidden, z.hidden_row, z.planes};
+    if (dx != nullptr) {
+        args.problems = 1;
+        args.problem[0].n = z.width;
+        args.problem[0].out = dx;
+        args.problem[0].part = part;
+        args.turn = int(steps_of(z.hidden));
+        args.steps = 2 * args.turn;
+        const Matrix a[2] = {da, db}, b[2] = {in.gate, in.up};
+        if ((st = run<kInput>(z.planes, a, b, 2, args, input_plan(z), s)) != FMD_OK) return st;
+    }
+    // the products of the weights' gradients that are asked for
+    const Plan p = weights_plan(z);
+    const Matrix h{at + k.h, z.rows, z.hidden, z.hidden_row, z.planes};
+    const Matrix a[3] = {da, db, gm}, b[3] = {in.x, in.x, h};
+    void* const out[3] = {dgate, dup, ddown};
+    args.problems = 0;
+    for (int i = 0; i < 3; ++i) {
+        if (out[i] == nullptr) continue;
+        Problem& q = args.problem[args.problems++];
+        q = Problem{};
+        q.out = out[i];
+        q.m = i < 2 ? z.hidden : z.out;
+        q.n = i < 2 ? z.width : z.hidden;
+        q.part = part;
+        q.a = q.b = i;
+        part += part_bytes(p, q.m, q.n) / sizeof(float);
+    }
+    args.steps = int(steps_of(z.rows));
+    return args.problems > 0 ? run<kWeights>(z.planes, a, b, 3, args, p, s) : FMD_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,129 @@
+"""A gated feed-forward block, ``(act(x gate^T) * (x up^T)) down^T``, and its backward pass.
+
+The other half of a block that attends (``packed_attention``, ``decay_attention``): both first projections, the activation
+and the product are one kernel, the last projection another, and the backward pass three. The kernels are
+``fmd_gated_feed_forward`` / ``fmd_gated_feed_forward_bwd`` (fastmd_b200/csrc/gated_feed_forward.cu). CUDA tensors only:
+there is no CPU path.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+from torch.autograd import Function
+
+from . import _lib
+from ._first_order import first_order, has_tangent
+from ._lib import FmdFeedForward, c_size_t, call, on_device, ptr, stream
+from .head_rotary import TYPES
+
+ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _rows(x: Tensor) -> Tensor:
+    """``x`` with unit stride inside a row and, in 16 bits, rows that start at multiples of 16 bytes; copied only when
+    needed."""
+    row, unit = x.stride()
+    rows, columns = x.shape
+    whole = (unit == 1 or columns == 1) and (row >= columns or rows <= 1)
+    if x.dtype == torch.float32:
+        return x if whole else x.contiguous()
+    if whole and not (x.data_ptr() % 16 or (row % 8 and rows > 1)):
+        return x
+    room = torch.empty(rows, (columns + 7) // 8 * 8, device=x.device, dtype=x.dtype)
+    return room[:, :columns].copy_(x)
+
+
+def _problem(x, gate, up, down, activation) -> FmdFeedForward:
+    return FmdFeedForward(x.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(), x.shape[0], x.stride(0),
+                          gate.stride(0), up.stride(0), down.stride(0), x.shape[1], gate.shape[0], down.shape[0],
+                          TYPES[x.dtype], activation)
+
+
+def _bytes(problem: FmdFeedForward, backward: bool) -> tuple[int, int]:
+    kept, workspace = c_size_t(), c_size_t()
+    call("fmd_gated_feed_forward_bytes", problem, backward, kept, workspace)
+    return kept.value, workspace.value
+
+
+def _room(size: int, device) -> Tensor | None:
+    return torch.empty(size, device=device, dtype=torch.uint8) if size else None
+
+
+def _forward(x, gate, up, down, activation, keep):
+    device = x.device
+    y = torch.empty(x.shape[0], down.shape[0], device=device, dtype=x.dtype)
+    problem = _problem(x, gate, up, down, activation)
+    size, more = _bytes(problem, False)
+    if keep:
+        size, _ = _bytes(problem, True)
+    kept, workspace = _room(size, device), _room(more, device)
+    call("fmd_gated_feed_forward", problem, y.data_ptr(), keep, ptr(kept), size, ptr(workspace), more,
+         _lib.flags_word(device).data_ptr(), stream(device))
+    return y, kept
+
+
+class _GatedFeedForward(Function):
+    @staticmethod
+    def forward(ctx, x, gate, up, down, activation):
+        y, kept = _forward(x, gate, up, down, activation, True)
+        ctx.save_for_backward(x, gate, up, down, kept)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        x, gate, up, down, kept = ctx.saved_tensors
+        like, device = (x, gate, up, down), x.device
+        inputs = (g, *like)
+        g = _rows(g)
+        grads = [torch.empty(t.shape, device=device, dtype=t.dtype) if need else None
+                 for t, need in zip(like, ctx.needs_input_grad)]
+        problem = _problem(x, gate, up, down, ctx.activation)
+        _, size = _bytes(problem, True)
+        workspace = _room(size, device)
+        call("fmd_gated_feed_forward_bwd", problem, ptr(kept), 0 if kept is None else kept.numel(), g.data_ptr(), g.stride(0),
+             *(ptr(t) for t in grads), ptr(workspace), size, _lib.flags_word(device).data_ptr(), stream(device))
+        return *first_order("gated_feed_forward", grads, inputs), None
+
+
+def gated_feed_forward(x: Tensor, gate: Tensor, up: Tensor, down: Tensor, *, activation: str = "silu") -> Tensor:
+    """``(act(x gate^T) * (x up^T)) down^T``: ``[.., width] -> [.., out]``.
+
+    x ``[.., width]``, gate and up ``[hidden, width]``, down ``[out, hidden]`` (as ``torch.nn.Linear`` keeps its weights),
+    all float32 or all bfloat16. ``activation``: ``"silu"``, ``a / (1 + e^-a)``, or ``"gelu"``, ``a (1 + erf(a / sqrt 2)) /
+    2``. Sizes are free, and so are strides; in bfloat16, rows that do not start at multiples of 16 bytes are copied first
+    (keep weights of odd width in padded storage to save that).
+
+    Differentiable in all four (first derivatives in reverse mode: others raise), with the same bits on every run. Sums are
+    held in 32 bits; in bfloat16 the gated product and the gradients of the two projections are rounded to bfloat16 as
+    operands of the next product, each of which costs a result about as much as its own rounding. In float32 each product
+    is six of bfloat16 planes; an infinity gives NaN where the formula may have an infinity. For the backward pass a call
+    keeps 10 bytes a row and hidden unit (float32: 14, and one and a half times the bytes of x and the weights)."""
+    _lib.require_cuda(x, gate, up, down)
+    if x.dim() < 1 or gate.dim() != 2 or up.shape != gate.shape or down.dim() != 2 or x.shape[-1] != gate.shape[1] \
+            or down.shape[1] != gate.shape[0]:
+        raise ValueError("x must be [.., width], gate and up [hidden, width] and down [out, hidden], got "
+                         f"{tuple(x.shape)}, {tuple(gate.shape)}, {tuple(up.shape)} and {tuple(down.shape)}")
+    if x.dtype not in TYPES or not x.dtype == gate.dtype == up.dtype == down.dtype:
+        raise ValueError("x and the weights must all be float32 or bfloat16, got "
+                         f"{x.dtype}, {gate.dtype}, {up.dtype} and {down.dtype}")
+    if not x.device == gate.device == up.device == down.device:
+        raise ValueError("x and the weights must be on one device")
+    if min(gate.shape) < 1 or down.shape[0] < 1 or max(*gate.shape, down.shape[0]) > 2 ** 20:
+        raise ValueError(f"width, hidden and out must be between 1 and 2^20, got {gate.shape[1]}, {gate.shape[0]} and "
+                         f"{down.shape[0]}")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
+    shape = (*x.shape[:-1], down.shape[0])
+    flat = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+    args = (_rows(flat), _rows(gate), _rows(up), _rows(down), ACTIVATIONS[activation])
+    trains = x.requires_grad or gate.requires_grad or up.requires_grad or down.requires_grad
+    with on_device(x.device):
+        if (trains and torch.is_grad_enabled()) or has_tangent(x, gate, up, down):
+            y = _GatedFeedForward.apply(*args)
+        else:
+            y, _ = _forward(*args, False)
+    return y if x.dim() == 2 else y.view(shape)
+
+
+__all__ = ["gated_feed_forward"]

@@ -1124,6 +1124,47 @@ FMD_API fmd_status fmd_packed_attention_bwd(const fmd_attention* problem, const 
                                             void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                                             int32_t* flags, void* stream);
 
+/* activations of the gated feed-forward block */
+#define FMD_FEED_SILU 0
+#define FMD_FEED_GELU 1 /* a (1 + erf(a / sqrt 2)) / 2 */
+
+/* A gated feed-forward block, y = (act(x gate^T) * (x up^T)) down^T: x [rows,
+ * width], gate and up [hidden, width], down [out, hidden], with unit stride
+ * inside a row; *_row: the row strides in elements. In bfloat16 bases and row
+ * strides are multiples of 16 bytes, else FMD_ERR_UNSUPPORTED; in float32
+ * they are anything. Sizes up to 2^20, rows up to 2^28. */
+typedef struct fmd_feed_forward {
+    const void* x;
+    const void* gate;
+    const void* up;
+    const void* down;
+    int64_t rows, x_row, gate_row, up_row, down_row;
+    int32_t width, hidden, out, type, activation, _pad;
+} fmd_feed_forward;
+
+/* From the sizes alone: `kept`, the bytes that the forward pass fills (with
+ * backward = 1 for fmd_gated_feed_forward_bwd, else as scratch of its own),
+ * and `workspace`: of the forward pass (backward = 0) or of the backward pass
+ * (1). Both buffers start at a multiple of 16 bytes. The forward pass's
+ * workspace is the same whether it keeps or not. */
+FMD_API fmd_status fmd_gated_feed_forward_bytes(const fmd_feed_forward* problem, int32_t backward, size_t* kept,
+                                                size_t* workspace);
+
+/* y [rows, out] contiguous. keep = 1: `kept` is left for the backward pass.
+ * FP32 sums, deterministic; h = act(..) * (..) is rounded to the type before
+ * the last product. No reference counterpart (nor has the backward pass). */
+FMD_API fmd_status fmd_gated_feed_forward(const fmd_feed_forward* problem, void* y, int32_t keep, void* kept,
+                                          size_t kept_bytes, void* workspace, size_t workspace_bytes, int32_t* flags,
+                                          void* stream);
+
+/* The gradients of x, gate, up and down (contiguous, each may be NULL) from
+ * g [rows, out], rows g_row apart, and what the forward pass of the same
+ * problem kept (which is not changed). The same bits on every run. */
+FMD_API fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kept, size_t kept_bytes,
+                                              const void* g, int64_t g_row, void* dx, void* dgate, void* dup,
+                                              void* ddown, void* workspace, size_t workspace_bytes, int32_t* flags,
+                                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif
