@@ -13,11 +13,11 @@ query and key heads, and softmax attention over packed sequences: learned models
 logged frames).
 """
 from fastmd_b200 import (  # noqa: F401
-    _lib, decomposed_indexed_cat_silu_linear, dispatch, energy_derivative, gated_feed_forward, gated_ln, gpu_nhc, graph, head_rotary,
+    _lib, decay_attention, decomposed_indexed_cat_silu_linear, dispatch, energy_derivative, gated_feed_forward, gated_ln, gpu_nhc, graph, head_rotary,
     line_graph, mace,
     md_protocol, model_graph, nequip, ops, packed_attention, pair_aggregate, residual_add, segment_attention, skin_topology, units, whole_step,
     wide_gemm)
 
-__all__ = ["decomposed_indexed_cat_silu_linear", "dispatch", "energy_derivative", "gated_feed_forward", "gated_ln", "gpu_nhc", "graph",
+__all__ = ["decay_attention", "decomposed_indexed_cat_silu_linear", "dispatch", "energy_derivative", "gated_feed_forward", "gated_ln", "gpu_nhc", "graph",
            "head_rotary", "line_graph", "mace", "md_protocol", "model_graph", "nequip", "ops", "packed_attention", "pair_aggregate", "residual_add",
            "segment_attention", "skin_topology", "units", "whole_step", "wide_gemm"]

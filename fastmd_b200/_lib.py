@@ -56,6 +56,14 @@ class FmdFeedForward(ctypes.Structure):
                 ("_pad", c_int32)]
 
 
+class FmdDecay(ctypes.Structure):
+    """The problem of fmd_decay_attention, its backward pass and its step."""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("log_decay", c_void_p), ("offsets", c_void_p),
+                ("rows", c_int64), ("q_row", c_int64), ("q_head", c_int64), ("k_row", c_int64), ("k_head", c_int64),
+                ("v_row", c_int64), ("v_head", c_int64), ("scale", c_float), ("type", c_int32), ("batch", c_int32),
+                ("heads", c_int32), ("dim", c_int32), ("_pad", c_int32)]
+
+
 _P = c_void_p  # every device pointer and the stream travel as void*
 _I64, _I32 = c_int64, c_int32
 
@@ -149,6 +157,10 @@ _SIGNATURES: dict[str, list] = {
     "fmd_gated_feed_forward_bytes": [POINTER(FmdFeedForward), _I32, POINTER(c_size_t), POINTER(c_size_t)],
     "fmd_gated_feed_forward": [POINTER(FmdFeedForward), _P, _I32, _P, c_size_t, _P, c_size_t, _P, _P],
     "fmd_gated_feed_forward_bwd": [POINTER(FmdFeedForward), _P, c_size_t, _P, _I64, _P, _P, _P, _P, _P, c_size_t, _P, _P],
+    "fmd_decay_attention_workspace_bytes": [POINTER(FmdDecay), _I32, POINTER(c_size_t)],
+    "fmd_decay_attention": [POINTER(FmdDecay), _P, _P, _P, _P, c_size_t, _P, _P],
+    "fmd_decay_attention_bwd": [POINTER(FmdDecay), _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, c_size_t, _P, _P],
+    "fmd_decay_attention_step": [POINTER(FmdDecay), _P, _P, _P],
     "fmd_nhc_pre_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P],
     "fmd_nhc_post_pre_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P],
     "fmd_nhc_post_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P],
@@ -205,7 +217,9 @@ KERNELS_PER_CALL = {"fmd_refilter_edges": 2, "fmd_refilter_edges_noalloc": 2, "f
                     "fmd_packed_attention_bwd": 3, "fmd_packed_attention_workspace_bytes": 0,
                     "fmd_head_rotary_workspace_bytes": 0,
                     # up and down; hidden, input and weights (float32 planes and shares of a sum add one each)
-                    "fmd_gated_feed_forward": 2, "fmd_gated_feed_forward_bwd": 3, "fmd_gated_feed_forward_bytes": 0}
+                    "fmd_gated_feed_forward": 2, "fmd_gated_feed_forward_bwd": 3, "fmd_gated_feed_forward_bytes": 0,
+                    # segments add two a pass
+                    "fmd_decay_attention_bwd": 3, "fmd_decay_attention_workspace_bytes": 0}
 
 
 def fused_step_kernels(n_layers: int) -> int:
@@ -281,5 +295,5 @@ def flags_word(device) -> torch.Tensor:
 c_int32_t, c_int64_t = c_int32, c_int64
 c_void_p_t = c_void_p
 
-__all__ = ["FastMDLibraryError", "FmdAttention", "FmdCatPart", "FmdFeedForward", "FmdHeadRotarySide", "call", "check", "declare", "flags_word", "lib", "on_device", "ptr",
+__all__ = ["FastMDLibraryError", "FmdAttention", "FmdCatPart", "FmdDecay", "FmdFeedForward", "FmdHeadRotarySide", "call", "check", "declare", "flags_word", "lib", "on_device", "ptr",
            "require_cuda", "stream", "c_double", "c_float", "c_int32", "c_int64", "c_void_p", "ctypes"]

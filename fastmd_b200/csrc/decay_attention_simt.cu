@@ -1,0 +1,264 @@
+// Decay attention on the FP32 cores.
+//
+// A block of 256 threads walks over the chunks of 64 rows of one segment and head; the chunk's rows of a, b and c and the
+// matrix lie in shared memory in FP32, padded to DP columns. A thread owns pieces of 4 x 4 pairs, of 4 rows x DP / 16
+// values of the output, and of DP / 16 x DP / 16 of the matrix, which it also keeps in registers.
+
+#include "decay_attention.cuh"
+
+namespace fmd {
+namespace {
+
+constexpr int kThreads = 256, kChunk = 64;
+
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <int DP>
+struct Tiles {
+    static constexpr int kLd = DP + 4;
+    static constexpr int kPer = DP / 16;
+    static constexpr size_t kStates = size_t(2 * kChunk * kLd + kChunk) * 4;
+    static constexpr size_t kRows = size_t(3 * kChunk * kLd + DP * kLd + kChunk * (kChunk + 4) + kChunk) * 4;
+};
+
+// `count` rows from `row0` on, zeros behind them and behind dim.
+template <int DP, typename T>
+__device__ __forceinline__ void load_rows(float* to, const void* from, int64_t row0, int64_t row, int64_t offset, int count,
+                                          int dim) {
+    for (int i = threadIdx.x; i < kChunk * DP / 4; i += kThreads) {
+        const int r = i / (DP / 4), c = i % (DP / 4) * 4;
+        float4 v = f4_zero();
+        if (r < count && c < dim) {
+            const T* p = static_cast<const T*>(from) + (row0 + r) * row + offset + c;
+            v = make_float4(as_float(p[0]), as_float(p[1]), as_float(p[2]), as_float(p[3]));
+        }
+        st4(to + r * Tiles<DP>::kLd + c, v);
+    }
+}
+
+template <int PER>
+__device__ __forceinline__ void load_piece(const float* p, float (&v)[PER]) {
+#pragma unroll
+    for (int i = 0; i < PER; i += (PER < 4 ? 2 : 4)) {
+        if constexpr (PER < 4) {
+            const float2 x = *reinterpret_cast<const float2*>(p + i);
+            v[i] = x.x;
+            v[i + 1] = x.y;
+        } else {
+            const float4 x = *reinterpret_cast<const float4*>(p + i);
+            v[i] = x.x;
+            v[i + 1] = x.y;
+            v[i + 2] = x.z;
+            v[i + 3] = x.w;
+        }
+    }
+}
+
+// state += sum_j w_j b_j c_j^T over the chunk, the piece of rows ty PER .. and columns tx PER ..
+template <int DP>
+__device__ __forceinline__ void add_outer(const float* b, const float* c, const float* weight, int count, int ty, int tx,
+                                          float (&state)[DP / 16][DP / 16]) {
+    constexpr int kPer = DP / 16, kLd = Tiles<DP>::kLd;
+#pragma unroll 2
+    for (int j = 0; j < count; ++j) {
+        float x[kPer], y[kPer];
+        load_piece<kPer>(b + j * kLd + ty * kPer, x);
+        load_piece<kPer>(c + j * kLd + tx * kPer, y);
+        const float w = weight[j];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            x[i] *= w;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) state[i][e] = fmaf(x[i], y[e], state[i][e]);
+        }
+    }
+}
+
+// The rows of the next chunk of a stretch: `done` rows lie behind the walk.
+__device__ __forceinline__ int64_t chunk_row(const Decay& d, const Stretch& s, int64_t done, int count) {
+    return d.later ? s.row0 + s.rows - done - count : s.row0 + done;
+}
+
+template <int DP, typename T>
+__global__ void __launch_bounds__(kThreads) states_kernel(const Decay d) {
+    constexpr int kPer = DP / 16, kLd = Tiles<DP>::kLd;
+    extern __shared__ float smem[];
+    float *b = smem, *c = b + kChunk * kLd, *weight = c + kChunk * kLd;
+    const int head = blockIdx.x % d.heads;
+    const Stretch s = stretch_of(d, blockIdx.x / d.heads);
+    if (s.rows == 0) return;
+    const float l2 = log2_decay(d, head);
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    float state[kPer][kPer] = {};
+    for (int64_t done = 0; done < s.rows; done += kChunk) {
+        const int count = int(min(int64_t(kChunk), s.rows - done));
+        const int64_t row = chunk_row(d, s, done, count);
+        __syncthreads();
+        load_rows<DP, T>(b, d.b, row, d.b_row, head * d.b_head, count, d.dim);
+        load_rows<DP, T>(c, d.c, row, d.c_row, head * d.c_head, count, d.dim);
+        if (threadIdx.x < kChunk) {
+            const int j = threadIdx.x;
+            weight[j] = j < count ? d.add * exp2f(float(d.later ? j + 1 : count - 1 - j) * l2) : 0.0f;
+        }
+        __syncthreads();
+        const float keep = exp2f(float(count) * l2);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) state[i][e] *= keep;
+        add_outer<DP>(b, c, weight, count, ty, tx, state);
+    }
+    float* out = d.states + (s.index * d.heads + head) * d.dim * d.dim;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+            if (ty * kPer + i < d.dim && tx * kPer + e < d.dim) out[(ty * kPer + i) * d.dim + tx * kPer + e] = state[i][e];
+}
+
+template <int DP, typename T>
+__global__ void __launch_bounds__(kThreads) rows_kernel(const Decay d, bool carried) {
+    constexpr int kPer = DP / 16, kLd = Tiles<DP>::kLd, kPairs = kChunk + 4;
+    extern __shared__ float smem[];
+    float *a = smem, *b = a + kChunk * kLd, *c = b + kChunk * kLd, *matrix = c + kChunk * kLd, *pairs = matrix + DP * kLd,
+          *weight = pairs + kChunk * kPairs;
+    const int head = blockIdx.x % d.heads;
+    const int64_t index = blockIdx.x / d.heads;
+    if (head == 0 && threadIdx.x == 32 && index < d.batch) check_offsets(d, index);
+    const Stretch s = stretch_of(d, index);
+    if (s.rows == 0) return;
+    const float l2 = log2_decay(d, head);
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    float state[kPer][kPer] = {};
+    const float* start = carried ? d.states + (index * d.heads + head) * d.dim * d.dim
+                         : d.start != nullptr ? d.start + (int64_t(s.b) * d.heads + head) * d.dim * d.dim : nullptr;
+    const bool turn = !carried && d.transposed;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            const int r = ty * kPer + i, col = tx * kPer + e;
+            if (start != nullptr && r < d.dim && col < d.dim) state[i][e] = start[turn ? col * d.dim + r : r * d.dim + col];
+            matrix[r * kLd + col] = state[i][e];
+        }
+    for (int64_t done = 0; done < s.rows; done += kChunk) {
+        const int count = int(min(int64_t(kChunk), s.rows - done));
+        const int64_t row = chunk_row(d, s, done, count);
+        __syncthreads();
+        load_rows<DP, T>(a, d.a, row, d.a_row, head * d.a_head, count, d.dim);
+        load_rows<DP, T>(b, d.b, row, d.b_row, head * d.b_head, count, d.dim);
+        load_rows<DP, T>(c, d.c, row, d.c_row, head * d.c_head, count, d.dim);
+        if (threadIdx.x < kChunk) {
+            const int j = threadIdx.x;
+            weight[j] = j < count ? d.add * exp2f(float(d.later ? j + 1 : count - 1 - j) * l2) : 0.0f;
+        }
+        __syncthreads();
+        float dot[4][4] = {};
+#pragma unroll 2
+        for (int x = 0; x < DP; x += 4) {
+            float4 p[4], q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * kLd + x);
+                q[i] = *reinterpret_cast<const float4*>(b + (tx + 16 * i) * kLd + x);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    dot[i][j] = fmaf(p[i].x, q[j].x, dot[i][j]);
+                    dot[i][j] = fmaf(p[i].y, q[j].y, dot[i][j]);
+                    dot[i][j] = fmaf(p[i].z, q[j].z, dot[i][j]);
+                    dot[i][j] = fmaf(p[i].w, q[j].w, dot[i][j]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int t = ty + 16 * i, u = tx + 16 * j, gap = d.later ? u - t : t - u;
+                pairs[t * kPairs + u] = gap >= 0 && u < count ? d.near * dot[i][j] * exp2f(float(gap) * l2) : 0.0f;
+            }
+        __syncthreads();
+        float far[4][kPer] = {}, near[4][kPer] = {};
+#pragma unroll 2
+        for (int x = 0; x < DP; ++x) {
+            float y[kPer];
+            load_piece<kPer>(matrix + x * kLd + tx * kPer, y);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = a[(ty + 16 * i) * kLd + x];
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) far[i][e] = fmaf(p, y[e], far[i][e]);
+            }
+        }
+#pragma unroll 2
+        for (int j = 0; j < count; ++j) {
+            float y[kPer];
+            load_piece<kPer>(c + j * kLd + tx * kPer, y);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = pairs[(ty + 16 * i) * kPairs + j];
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) near[i][e] = fmaf(p, y[e], near[i][e]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = ty + 16 * i;
+            if (t >= count) continue;
+            const float reach = d.far * exp2f(float(d.later ? count - 1 - t : t + 1) * l2);
+            T* out = static_cast<T*>(d.out) + ((row + t) * d.heads + head) * d.dim;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                const float v = fmaf(reach, far[i][e], near[i][e]);
+                if (tx * kPer + e < d.dim) {
+                    if constexpr (sizeof(T) == 2) out[tx * kPer + e] = __float2bfloat16_rn(v);
+                    else out[tx * kPer + e] = v;
+                }
+            }
+        }
+        const float keep = exp2f(float(count) * l2);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) state[i][e] *= keep;
+        add_outer<DP>(b, c, weight, count, ty, tx, state);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) matrix[(ty * kPer + i) * kLd + tx * kPer + e] = state[i][e];
+    }
+}
+
+template <int DP, typename T>
+fmd_status launch(const Decay& d, bool states, bool carried, cudaStream_t s) {
+    const size_t bytes = states ? Tiles<DP>::kStates : Tiles<DP>::kRows;
+    const void* kernel = states ? (const void*)states_kernel<DP, T> : (const void*)rows_kernel<DP, T>;
+    const fmd_status st = grant_dynamic_smem(kernel, bytes, true);
+    if (st != FMD_OK) return st;
+    const unsigned blocks = unsigned(decay_segments(d) * d.heads);
+    if (states) states_kernel<DP, T><<<blocks, kThreads, bytes, s>>>(d);
+    else rows_kernel<DP, T><<<blocks, kThreads, bytes, s>>>(d, carried);
+    return check_launch();
+}
+
+template <typename T>
+fmd_status launch_for(const Decay& d, bool states, bool carried, cudaStream_t s) {
+    return d.dim <= 32 ? launch<32, T>(d, states, carried, s) : d.dim <= 64 ? launch<64, T>(d, states, carried, s)
+                                                                            : launch<128, T>(d, states, carried, s);
+}
+
+}  // namespace
+
+fmd_status decay_states_simt(const Decay& d, bool bf16, cudaStream_t s) {
+    return bf16 ? launch_for<__nv_bfloat16>(d, true, false, s) : launch_for<float>(d, true, false, s);
+}
+
+fmd_status decay_rows_simt(const Decay& d, bool bf16, bool carried, cudaStream_t s) {
+    return bf16 ? launch_for<__nv_bfloat16>(d, false, carried, s) : launch_for<float>(d, false, carried, s);
+}
+
+}  // namespace fmd

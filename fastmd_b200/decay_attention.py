@@ -1,0 +1,177 @@
+"""Linear attention over packed sequences with a decay for each head, its gradients and its form for single rows.
+
+Where ``packed_attention`` reads all that a replica has logged, ``decay_attention`` carries it along as one matrix a head, so
+that a log may go on for ever: a new row costs the same whatever came before. ``decay_attention`` takes whole sequences or
+chunks that follow a state; ``decay_attention_step`` takes one new row of every sequence. No call reads a length on the
+host, so every call can be captured in a CUDA graph. The kernels are ``fmd_decay_attention`` and ``_bwd``, ``_step``
+(fastmd_b200/csrc/decay_attention*.cu). CUDA tensors only: there is no CPU path.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+from torch.autograd import Function
+
+from . import _lib
+from ._first_order import first_order, has_tangent
+from ._lib import FmdDecay, c_size_t, call, on_device, ptr, stream
+from .head_rotary import TYPES, _head_rows, _like
+
+
+def _problem(q, k, v, log_decay, offsets, scale) -> FmdDecay:
+    return FmdDecay(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), ptr(offsets), q.shape[0], q.stride(0),
+                    q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), scale, TYPES[q.dtype],
+                    offsets.shape[0] - 1 if offsets is not None else 0, q.shape[1], q.shape[2])
+
+
+def _workspace(problem: FmdDecay, after: bool, device) -> tuple[Tensor | None, int]:
+    nbytes = c_size_t()
+    call("fmd_decay_attention_workspace_bytes", problem, after, nbytes)
+    size = nbytes.value
+    return (torch.empty(size, device=device, dtype=torch.uint8) if size else None), size
+
+
+def _states(q: Tensor, offsets: Tensor) -> Tensor:
+    return torch.empty(offsets.shape[0] - 1, q.shape[1], q.shape[2], q.shape[2], device=q.device, dtype=torch.float32)
+
+
+def _forward(q, k, v, log_decay, offsets, state, scale, keep):
+    device = q.device
+    out, after = _like(q), _states(q, offsets) if keep else None
+    problem = _problem(q, k, v, log_decay, offsets, scale)
+    workspace, size = _workspace(problem, keep, device)
+    call("fmd_decay_attention", problem, ptr(state), out.data_ptr(), ptr(after), ptr(workspace), size,
+         _lib.flags_word(device).data_ptr(), stream(device))
+    return out, after
+
+
+class _DecayAttention(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, offsets, state, scale, keep):
+        out, after = _forward(q, k, v, log_decay, offsets, state, scale, keep)
+        ctx.save_for_backward(q, k, v, log_decay, offsets, state)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return out, after
+
+    @staticmethod
+    def backward(ctx, g, gafter):
+        q, k, v, log_decay, offsets, state = ctx.saved_tensors
+        if g is None and gafter is None:
+            return (None,) * 8
+        inputs = (g, gafter, q, k, v, state)
+        g = torch.zeros_like(q, memory_format=torch.contiguous_format) if g is None else _head_rows(g)
+        gafter = _aligned_state(gafter)
+        need = ctx.needs_input_grad
+        dq, dk, dv = (_like(t) if n else None for t, n in zip((q, k, v), need))
+        dstate = torch.empty_like(state) if need[5] else None
+        problem = _problem(q, k, v, log_decay, offsets, ctx.scale)
+        workspace, size = _workspace(problem, need[5], q.device)
+        call("fmd_decay_attention_bwd", problem, ptr(state), g.data_ptr(), g.stride(0), g.stride(1), ptr(gafter), ptr(dq),
+             ptr(dk), ptr(dv), ptr(dstate), ptr(workspace), size, _lib.flags_word(q.device).data_ptr(), stream(q.device))
+        dq, dk, dv, dstate = first_order("decay_attention", (dq, dk, dv, dstate), inputs)
+        return dq, dk, dv, None, None, dstate, None, None
+
+
+def _aligned_state(state: Tensor | None) -> Tensor | None:
+    if state is None:
+        return None
+    state = state.contiguous()
+    return state.clone() if state.data_ptr() % 16 else state
+
+
+def _check(q, k, v, log_decay, scale) -> float:
+    if q.dim() != 3 or k.shape != q.shape or v.shape != q.shape:
+        raise ValueError("q, k and v must all be [rows, heads, dim], got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    if q.dtype not in TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q, k and v must all be float32 or bfloat16, got {q.dtype}, {k.dtype} and {v.dtype}")
+    heads, dim = q.shape[1:]
+    if dim % 8 or not 8 <= dim <= 128:
+        raise ValueError(f"the head size must be a multiple of 8 up to 128, got {dim}")
+    if not 1 <= heads <= 1024:
+        raise ValueError(f"between 1 and 1024 heads, got {heads}")
+    if log_decay.shape != (heads,) or log_decay.dtype != torch.float32:
+        raise ValueError(f"log_decay must be float32 [{heads}], got {log_decay.dtype} {tuple(log_decay.shape)}")
+    if not q.device == k.device == v.device == log_decay.device:
+        raise ValueError("q, k, v and log_decay must be on one device")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 <= scale <= 1e38:
+        raise ValueError(f"scale must be between 0 and 1e38, got {scale}")
+    return scale
+
+
+def _check_state(state, batch, q) -> None:
+    shape = (batch, q.shape[1], q.shape[2], q.shape[2])
+    if tuple(state.shape) != shape or state.dtype != torch.float32:
+        raise ValueError(f"state must be float32 {list(shape)}, got {state.dtype} {list(state.shape)}")
+    if state.device != q.device:
+        raise ValueError("state must be on the device of q")
+
+
+def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, offsets: Tensor, state: Tensor | None = None, *,
+                    scale: float | None = None, return_state: bool = False) -> Tensor | tuple[Tensor, Tensor]:
+    """``out_t = scale * q_t S_t`` with ``S_t = exp(log_decay) S_{t-1} + k_t v_t^T``: ``[rows, heads, dim]``.
+
+    q, k and v ``[rows, heads, dim]``, float32 or bfloat16; ``dim`` is a multiple of 8 up to 128. Strides are free; tensors
+    whose heads have no unit stride or do not start at multiples of 16 bytes are copied first. Sequence ``b`` has the rows
+    ``offsets[b] .. offsets[b + 1] - 1`` (int64 on the device; offsets that do not start at 0, fall or end elsewhere than
+    at the last row raise ``FMD_FLAG_INDEX_RANGE`` in the device's flags word). ``log_decay`` is float32 ``[heads]``, at
+    most 0 (0: nothing is forgotten; values above count as 0, values below -10,000 as that); it is given, not learned:
+    where it requires a gradient the call raises. ``scale`` (not negative) defaults to ``dim ** -0.5``.
+
+    ``state``: float32 ``[sequences, heads, dim, dim]``, k's index first: the matrices before the first rows (default:
+    zeros). ``return_state`` also returns those behind the last rows, from which a later call or
+    ``decay_attention_step`` goes on; a sequence without rows keeps its own.
+
+    Differentiable in q, k, v and ``state`` (first derivatives in reverse mode: others raise), with the same bits on every
+    run. Sums and matrices are held in 32 bits."""
+    _lib.require_cuda(q, k, v, log_decay, offsets, state)
+    scale = _check(q, k, v, log_decay, scale)
+    if offsets.dim() != 1 or offsets.shape[0] < 1 or offsets.dtype != torch.int64:
+        raise ValueError(f"offsets must be int64 [sequences + 1], got {offsets.dtype} {tuple(offsets.shape)}")
+    if offsets.device != q.device:
+        raise ValueError("offsets must be on the device of q")
+    if offsets.shape[0] == 1 and q.shape[0]:
+        raise ValueError("rows without a sequence: offsets holds one value")
+    if state is not None:
+        _check_state(state, offsets.shape[0] - 1, q)
+    if torch.is_grad_enabled() and log_decay.requires_grad:
+        raise ValueError("log_decay has no gradient here: pass it detached")
+    args = (_head_rows(q), _head_rows(k), _head_rows(v), log_decay.contiguous(), offsets.contiguous(), _aligned_state(state),
+            scale, bool(return_state))
+    trains = q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)
+    with on_device(q.device):
+        if (torch.is_grad_enabled() and trains) or has_tangent(q, k, v, log_decay, state):
+            out, after = _DecayAttention.apply(*args)
+        else:
+            out, after = _forward(*args)
+    return (out, after) if return_state else out
+
+
+def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, *,
+                         scale: float | None = None) -> Tensor:
+    """One new row of every sequence: ``state = exp(log_decay) state + k v^T`` in place, ``out = scale * q state``.
+
+    q, k and v ``[sequences, heads, dim]`` and ``log_decay`` as for ``decay_attention``; any strides. ``state`` is
+    contiguous float32 ``[sequences, heads, dim, dim]`` and is the caller's: it moves on by a row each call. Not
+    differentiable: where an argument requires a gradient the call raises (``decay_attention`` takes single rows too)."""
+    _lib.require_cuda(q, k, v, log_decay, state)
+    scale = _check(q, k, v, log_decay, scale)
+    _check_state(state, q.shape[0], q)
+    if not state.is_contiguous() or state.data_ptr() % 16:
+        raise ValueError("state must be contiguous and start at a multiple of 16 bytes: it is changed in place")
+    tensors = (q, k, v, log_decay, state)
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or has_tangent(*tensors):
+        raise ValueError("decay_attention_step has no gradient: call it under torch.no_grad(), or decay_attention")
+    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+    out = _like(q)
+    with on_device(q.device):
+        call("fmd_decay_attention_step", _problem(q, k, v, log_decay.contiguous(), None, scale), state.data_ptr(),
+             out.data_ptr(), stream(q.device))
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
+    return out
+
+
+__all__ = ["decay_attention", "decay_attention_step"]

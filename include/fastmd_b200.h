@@ -1165,6 +1165,50 @@ FMD_API fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, v
                                               void* ddown, void* workspace, size_t workspace_bytes, int32_t* flags,
                                               void* stream);
 
+/* Linear attention with a decay for each head: S_t = e^log_decay S_{t-1} +
+ * k_t v_t^T, out_t = scale q_t S_t over the rows offsets[b] .. offsets[b + 1]
+ * - 1 of sequence b. q, k, v [rows, heads, dim] with unit stride inside a
+ * head; log_decay [heads], at most 0 (what is above counts as 0, what is
+ * below -10,000 as that); states [batch, heads, dim, dim] FP32, rows of k's
+ * index, columns of v's. Offsets live on the device, start at 0, do not fall
+ * and end at rows: else FMD_FLAG_INDEX_RANGE is raised, nothing outside the
+ * arrays is touched and the results are unspecified. dim a multiple of 8 up
+ * to 128, scale between 0 and 1e38, rows at most 2^29, heads at most 1024;
+ * bases and strides multiples of 16 bytes, else FMD_ERR_UNSUPPORTED. */
+typedef struct fmd_decay {
+    const void* q;
+    const void* k;
+    const void* v;
+    const float* log_decay;
+    const int64_t* offsets;
+    int64_t rows, q_row, q_head, k_row, k_head, v_row, v_head;
+    float scale;
+    int32_t type, batch, heads, dim, _pad;
+} fmd_decay;
+
+/* Workspace of the forward pass, or of the backward pass, where the matrix
+ * behind the last row (the gradient of the first state) is asked for
+ * (after = 1) or not; 0 for none. It starts at a multiple of 16 bytes. */
+FMD_API fmd_status fmd_decay_attention_workspace_bytes(const fmd_decay* problem, int32_t after, size_t* bytes);
+
+/* out [rows, heads, dim] and `after`, the states behind the last rows (NULL:
+ * not written), from the states before the first ones (NULL: zeros). No
+ * reference counterpart (nor have the others). */
+FMD_API fmd_status fmd_decay_attention(const fmd_decay* problem, const float* state, void* out, float* after,
+                                       void* workspace, size_t workspace_bytes, int32_t* flags, void* stream);
+
+/* Gradients of q, k, v (contiguous) and of the first states, each may be
+ * NULL, from those of out (g, strides g_row, g_head) and of the last states
+ * (gafter, NULL: none). Deterministic. */
+FMD_API fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state, const void* g, int64_t g_row,
+                                           int64_t g_head, const float* gafter, void* dq, void* dk, void* dv,
+                                           float* dstate, void* workspace, size_t workspace_bytes, int32_t* flags,
+                                           void* stream);
+
+/* One row of each of `rows` sequences: state [rows, heads, dim, dim] moves on
+ * in place. offsets and batch are not used; any strides. */
+FMD_API fmd_status fmd_decay_attention_step(const fmd_decay* problem, float* state, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
