@@ -156,7 +156,7 @@ fmd_status mix(Decay d, bool bf16, void* workspace, cudaStream_t s) {
     fmd_status st = FMD_OK;
     if (carried && d.batch > 0) {
         d.states = static_cast<float*>(workspace);
-        if (d.rows > 0) st = decay_states_simt(d, bf16, s);
+        if (d.rows > 0) st = bf16 ? decay_states_mma(d, s) : decay_states_simt(d, s);
         if (st != FMD_OK) return st;
         const int64_t blocks = int64_t(d.batch) * d.heads;
         if (blocks > INT32_MAX) return FMD_ERR_UNSUPPORTED;
@@ -165,7 +165,7 @@ fmd_status mix(Decay d, bool bf16, void* workspace, cudaStream_t s) {
         if ((st = check_launch()) != FMD_OK) return st;
     }
     if (d.rows == 0 || d.out == nullptr) return FMD_OK;
-    return decay_rows_simt(d, bf16, carried, s);
+    return bf16 ? decay_rows_mma(d, carried, s) : decay_rows_simt(d, carried, s);
 }
 
 size_t mix_bytes(Decay d, bool after) {

@@ -79,8 +79,12 @@ __host__ __device__ inline int64_t decay_segments(const Decay& d) {
     return d.length >= kWhole ? d.batch : d.rows / d.length + d.batch;
 }
 
-// carried: a segment starts from its place in `states`, else from `start`
-fmd_status decay_states_simt(const Decay& d, bool bf16, cudaStream_t s);
-fmd_status decay_rows_simt(const Decay& d, bool bf16, bool carried, cudaStream_t s);
+// What the segments add to the matrix, and the rows. carried: a segment starts from its place in `states`, else from
+// `start`. bfloat16:
+fmd_status decay_states_mma(const Decay& d, cudaStream_t s);
+fmd_status decay_rows_mma(const Decay& d, bool carried, cudaStream_t s);
+// float32
+fmd_status decay_states_simt(const Decay& d, cudaStream_t s);
+fmd_status decay_rows_simt(const Decay& d, bool carried, cudaStream_t s);
 
 }  // namespace fmd

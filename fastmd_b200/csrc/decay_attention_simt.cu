@@ -1,4 +1,4 @@
-// Decay attention on the FP32 cores.
+// Decay attention in float32, on the FP32 cores.
 //
 // A block of 256 threads walks over the chunks of 64 rows of one segment and head; the chunk's rows of a, b and c and the
 // matrix lie in shared memory in FP32, padded to DP columns. A thread owns pieces of 4 x 4 pairs, of 4 rows x DP / 16
@@ -11,27 +11,22 @@ namespace {
 
 constexpr int kThreads = 256, kChunk = 64;
 
-__device__ __forceinline__ float as_float(float v) { return v; }
-__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-
 template <int DP>
 struct Tiles {
     static constexpr int kLd = DP + 4;
-    static constexpr int kPer = DP / 16;
     static constexpr size_t kStates = size_t(2 * kChunk * kLd + kChunk) * 4;
     static constexpr size_t kRows = size_t(3 * kChunk * kLd + DP * kLd + kChunk * (kChunk + 4) + kChunk) * 4;
 };
 
 // `count` rows from `row0` on, zeros behind them and behind dim.
-template <int DP, typename T>
+template <int DP>
 __device__ __forceinline__ void load_rows(float* to, const void* from, int64_t row0, int64_t row, int64_t offset, int count,
                                           int dim) {
     for (int i = threadIdx.x; i < kChunk * DP / 4; i += kThreads) {
         const int r = i / (DP / 4), c = i % (DP / 4) * 4;
         float4 v = f4_zero();
         if (r < count && c < dim) {
-            const T* p = static_cast<const T*>(from) + (row0 + r) * row + offset + c;
-            v = make_float4(as_float(p[0]), as_float(p[1]), as_float(p[2]), as_float(p[3]));
+            v = ldg4(static_cast<const float*>(from) + (row0 + r) * row + offset + c);
         }
         st4(to + r * Tiles<DP>::kLd + c, v);
     }
@@ -80,7 +75,7 @@ __device__ __forceinline__ int64_t chunk_row(const Decay& d, const Stretch& s, i
     return d.later ? s.row0 + s.rows - done - count : s.row0 + done;
 }
 
-template <int DP, typename T>
+template <int DP>
 __global__ void __launch_bounds__(kThreads) states_kernel(const Decay d) {
     constexpr int kPer = DP / 16, kLd = Tiles<DP>::kLd;
     extern __shared__ float smem[];
@@ -95,8 +90,8 @@ __global__ void __launch_bounds__(kThreads) states_kernel(const Decay d) {
         const int count = int(min(int64_t(kChunk), s.rows - done));
         const int64_t row = chunk_row(d, s, done, count);
         __syncthreads();
-        load_rows<DP, T>(b, d.b, row, d.b_row, head * d.b_head, count, d.dim);
-        load_rows<DP, T>(c, d.c, row, d.c_row, head * d.c_head, count, d.dim);
+        load_rows<DP>(b, d.b, row, d.b_row, head * d.b_head, count, d.dim);
+        load_rows<DP>(c, d.c, row, d.c_row, head * d.c_head, count, d.dim);
         if (threadIdx.x < kChunk) {
             const int j = threadIdx.x;
             weight[j] = j < count ? d.add * exp2f(float(d.later ? j + 1 : count - 1 - j) * l2) : 0.0f;
@@ -117,7 +112,7 @@ __global__ void __launch_bounds__(kThreads) states_kernel(const Decay d) {
             if (ty * kPer + i < d.dim && tx * kPer + e < d.dim) out[(ty * kPer + i) * d.dim + tx * kPer + e] = state[i][e];
 }
 
-template <int DP, typename T>
+template <int DP>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const Decay d, bool carried) {
     constexpr int kPer = DP / 16, kLd = Tiles<DP>::kLd, kPairs = kChunk + 4;
     extern __shared__ float smem[];
@@ -146,9 +141,9 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Decay d, bool carr
         const int count = int(min(int64_t(kChunk), s.rows - done));
         const int64_t row = chunk_row(d, s, done, count);
         __syncthreads();
-        load_rows<DP, T>(a, d.a, row, d.a_row, head * d.a_head, count, d.dim);
-        load_rows<DP, T>(b, d.b, row, d.b_row, head * d.b_head, count, d.dim);
-        load_rows<DP, T>(c, d.c, row, d.c_row, head * d.c_head, count, d.dim);
+        load_rows<DP>(a, d.a, row, d.a_row, head * d.a_head, count, d.dim);
+        load_rows<DP>(b, d.b, row, d.b_row, head * d.b_head, count, d.dim);
+        load_rows<DP>(c, d.c, row, d.c_row, head * d.c_head, count, d.dim);
         if (threadIdx.x < kChunk) {
             const int j = threadIdx.x;
             weight[j] = j < count ? d.add * exp2f(float(d.later ? j + 1 : count - 1 - j) * l2) : 0.0f;
@@ -209,14 +204,10 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Decay d, bool carr
             const int t = ty + 16 * i;
             if (t >= count) continue;
             const float reach = d.far * exp2f(float(d.later ? count - 1 - t : t + 1) * l2);
-            T* out = static_cast<T*>(d.out) + ((row + t) * d.heads + head) * d.dim;
+            float* out = static_cast<float*>(d.out) + ((row + t) * d.heads + head) * d.dim;
 #pragma unroll
             for (int e = 0; e < kPer; ++e) {
-                const float v = fmaf(reach, far[i][e], near[i][e]);
-                if (tx * kPer + e < d.dim) {
-                    if constexpr (sizeof(T) == 2) out[tx * kPer + e] = __float2bfloat16_rn(v);
-                    else out[tx * kPer + e] = v;
-                }
+                if (tx * kPer + e < d.dim) out[tx * kPer + e] = fmaf(reach, far[i][e], near[i][e]);
             }
         }
         const float keep = exp2f(float(count) * l2);
@@ -233,32 +224,27 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Decay d, bool carr
     }
 }
 
-template <int DP, typename T>
+template <int DP>
 fmd_status launch(const Decay& d, bool states, bool carried, cudaStream_t s) {
     const size_t bytes = states ? Tiles<DP>::kStates : Tiles<DP>::kRows;
-    const void* kernel = states ? (const void*)states_kernel<DP, T> : (const void*)rows_kernel<DP, T>;
+    const void* kernel = states ? (const void*)states_kernel<DP> : (const void*)rows_kernel<DP>;
     const fmd_status st = grant_dynamic_smem(kernel, bytes, true);
     if (st != FMD_OK) return st;
     const unsigned blocks = unsigned(decay_segments(d) * d.heads);
-    if (states) states_kernel<DP, T><<<blocks, kThreads, bytes, s>>>(d);
-    else rows_kernel<DP, T><<<blocks, kThreads, bytes, s>>>(d, carried);
+    if (states) states_kernel<DP><<<blocks, kThreads, bytes, s>>>(d);
+    else rows_kernel<DP><<<blocks, kThreads, bytes, s>>>(d, carried);
     return check_launch();
 }
 
-template <typename T>
 fmd_status launch_for(const Decay& d, bool states, bool carried, cudaStream_t s) {
-    return d.dim <= 32 ? launch<32, T>(d, states, carried, s) : d.dim <= 64 ? launch<64, T>(d, states, carried, s)
-                                                                            : launch<128, T>(d, states, carried, s);
+    return d.dim <= 32 ? launch<32>(d, states, carried, s) : d.dim <= 64 ? launch<64>(d, states, carried, s)
+                                                                         : launch<128>(d, states, carried, s);
 }
 
 }  // namespace
 
-fmd_status decay_states_simt(const Decay& d, bool bf16, cudaStream_t s) {
-    return bf16 ? launch_for<__nv_bfloat16>(d, true, false, s) : launch_for<float>(d, true, false, s);
-}
+fmd_status decay_states_simt(const Decay& d, cudaStream_t s) { return launch_for(d, true, false, s); }
 
-fmd_status decay_rows_simt(const Decay& d, bool bf16, bool carried, cudaStream_t s) {
-    return bf16 ? launch_for<__nv_bfloat16>(d, false, carried, s) : launch_for<float>(d, false, carried, s);
-}
+fmd_status decay_rows_simt(const Decay& d, bool carried, cudaStream_t s) { return launch_for(d, false, carried, s); }
 
 }  // namespace fmd
