@@ -37,7 +37,7 @@ constexpr int kThreads = 384, kWorkers = 256;
 constexpr int kM = 128, kK = 64;
 constexpr uint32_t kTileA = kM * kK * 2, kPanel = 64 * kK * 2;  // bytes of an operand's tile, of 64 columns of it
 constexpr int kMostSlots = 8;
-constexpr size_t kRingBytes = 224 * 1024;
+constexpr size_t kRingBytes = 192 * 1024, kScratch = 4096;  // kScratch: of each warp that stores
 constexpr int kSegment = 2;
 constexpr float kBf16Max = 3.38953139e38f;
 
@@ -150,107 +150,139 @@ __device__ __forceinline__ void activate(int act, float a, float& value, float& 
     }
 }
 
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float* v) {
-    *reinterpret_cast<uint4*>(p) =
-        make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-}
-
-__device__ __forceinline__ void store8(float* p, const float* v) {
-    st4(p, make_float4(v[0], v[1], v[2], v[3]));
-    st4(p + 4, make_float4(v[4], v[5], v[6], v[7]));
-}
-
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 
-// N values of a row from column `col` on, as far as `n`: by eights where rows start at multiples of 16 bytes.
-template <int N, typename T>
-__device__ __forceinline__ void store_row(T* row, int64_t col, int64_t n, bool vector, const float* v) {
+// A thread holds a row of the sums, memory wants rows side by side: what a warp stores or loads goes through 4 KB of shared
+// memory of its own, W pieces of 16 bytes a row, so that W lanes reach into one row. The pieces of a row are turned by the
+// row's number, which keeps the banks apart both ways.
+template <int W>
+__device__ __forceinline__ uint4* piece_at(unsigned char* scratch, int row, int piece) {
+    const int turn = W == 8 ? row & 7 : (row >> 1) & 3;
+    return reinterpret_cast<uint4*>(scratch + (row * W + (piece ^ turn)) * 16);
+}
+
+// The first `pieces` of each of the first `rows` rows to `to` and on, rows `stride` bytes apart.
+template <int W>
+__device__ __forceinline__ void put_rows(unsigned char* scratch, const uint4* w, void* to, int64_t stride, int rows, int pieces) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < N; i += 8) {
-        if (vector) {
-            if (col + i < n) store8(row + col + i, v + i);
-        } else {
+    for (int i = 0; i < W; ++i) *piece_at<W>(scratch, lane, i) = w[i];
+    __syncwarp();
+    char* p = static_cast<char*>(to) + (lane % W) * 16;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (col + i + e < n) store1(row + col + i + e, v[i + e]);
-        }
+    for (int i = 0; i < W; ++i) {
+        const int row = i * (32 / W) + lane / W;
+        const uint4 x = *piece_at<W>(scratch, row, lane % W);
+        if (row < rows && lane % W < pieces) *reinterpret_cast<uint4*>(p + row * stride) = x;
     }
 }
 
-// Eight values as P planes.
+// 32 columns of FP32 of 32 rows: the loads (a lane holds pieces of eight rows) ..
+__device__ __forceinline__ void fetch_rows(const float* from, int64_t stride, int rows, int pieces, float4 (&x)[8]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int row = i * 4 + lane / 8;
+        x[i] = row < rows && lane % 8 < pieces ? ldg4(from + row * stride + (lane % 8) * 4) : f4_zero();
+    }
+}
+
+// .. and the turn to a row a lane.
+__device__ __forceinline__ void turn_rows(unsigned char* scratch, const float4 (&x)[8], float (&v)[32]) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<float4*>(piece_at<8>(scratch, i * 4 + lane / 8, lane % 8)) = x[i];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(piece_at<8>(scratch, lane, i));
+        v[4 * i] = y.x, v[4 * i + 1] = y.y, v[4 * i + 2] = y.z, v[4 * i + 3] = y.w;
+    }
+}
+
+__device__ __forceinline__ uint4 pack8(const float* v) {
+    return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
+// Eight values' first plane; `v` becomes what is left of them. Held to the largest bfloat16: finite values stay finite.
+__device__ __forceinline__ uint4 first_plane8(float* v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = pack_bf16(fminf(fmaxf(v[2 * i], -kBf16Max), kBf16Max), fminf(fmaxf(v[2 * i + 1], -kBf16Max), kBf16Max));
+        const float2 part = unpack_bf16(w[i]);
+        v[2 * i] -= part.x;
+        v[2 * i + 1] -= part.y;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ uint4 next_plane8(float* v) {
+    uint32_t w[4];
+    next_plane<4>(v, w);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 32 values a row as P planes, `plane` values apart; rows are padded to multiples of 8 columns. The values are used up.
 template <int P>
-__device__ __forceinline__ void store_planes8(__nv_bfloat16* p, int64_t plane, const float* v) {
-    if constexpr (P == 1) {
-        store8(p, v);
-    } else {
-        float left[8];
-        uint32_t w[4];
+__device__ __forceinline__ void put_planes(unsigned char* scratch, float (&v)[32], __nv_bfloat16* to, int64_t row,
+                                           int64_t plane, int rows, int pieces) {
+    uint4 w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // held to the largest bfloat16: finite values stay finite in the first plane
-            w[i] = pack_bf16(fminf(fmaxf(v[2 * i], -kBf16Max), kBf16Max), fminf(fmaxf(v[2 * i + 1], -kBf16Max), kBf16Max));
-            const float2 part = unpack_bf16(w[i]);
-            left[2 * i] = v[2 * i] - part.x;
-            left[2 * i + 1] = v[2 * i + 1] - part.y;
-        }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int q = 0; q < P; ++q) {
 #pragma unroll
-        for (int i = 1; i < P; ++i) {
-            next_plane<4>(left, w);
-            *reinterpret_cast<uint4*>(p + i * plane) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        for (int i = 0; i < 4; ++i)
+            w[i] = P == 1 ? pack8(v + 8 * i) : q == 0 ? first_plane8(v + 8 * i) : next_plane8(v + 8 * i);
+        put_rows<4>(scratch, w, to + q * plane, row * 2, rows, pieces);
     }
 }
 
-// What follows the sums of 64 columns of one row: of kUp 32 of a and 32 of b, whose place among the hidden units is col.
-template <int KIND, int P>
-__device__ __forceinline__ void finish(const Args& g, const Problem& q, const Place& p, int64_t row, int64_t col,
-                                       float (&v)[64]) {
-    using T = typename std::conditional<P == 1, __nv_bfloat16, float>::type;
-    if constexpr (KIND == kUp) {
-        const bool kept = g.slope != nullptr;
+__device__ __forceinline__ void put_floats(unsigned char* scratch, const float* v, float* to, int64_t row, int rows,
+                                           int pieces) {
+    uint4 w[8];
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-            if (col + i >= q.n) break;  // rows are padded to multiples of 8, and get zeros there
-            float h[8], slope[8], level[8];
+    for (int i = 0; i < 8; ++i)
+        w[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                          __float_as_uint(v[4 * i + 3]));
+    put_rows<8>(scratch, w, to, row * 4, rows, pieces);
+}
+
+// 64 columns from `col` of a result's rows, `n` columns wide; rows start anywhere unless `vector`.
+template <typename T>
+__device__ __forceinline__ void put_result(unsigned char* scratch, const float (&v)[64], T* to, int64_t col, int64_t n,
+                                           int64_t row, int rows, bool vector) {
+    const int left = int(min(int64_t(64), n - col)), lane = threadIdx.x & 31;
+    if (left <= 0) return;
+    to += col;
+    if (vector) {
+        if constexpr (sizeof(T) == 2) {
+            uint4 w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                activate<P == 3>(g.act, v[i + e], level[e], slope[e]);
-                h[e] = level[e] * v[32 + i + e];
-                slope[e] *= v[32 + i + e];
-            }
-            const int64_t at = row * g.row + col + i;
-            store_planes8<P>(g.h + at, g.plane, h);
-            if (kept) {
-                store8(g.slope + at, slope);
-                store8(g.level + at, level);
-            }
+            for (int i = 0; i < 8; ++i) w[i] = pack8(v + 8 * i);
+            put_rows<8>(scratch, w, to, row * 2, rows, left / 8);
+        } else {
+            put_floats(scratch, v, to, row, rows, left / 4);
+            if (left > 32) put_floats(scratch, v + 32, to + 32, row, rows, left / 4 - 8);
         }
-    } else if constexpr (KIND == kHidden) {
+        return;
+    }
 #pragma unroll
-        for (int i = 0; i < 64; i += 8) {
-            if (col + i >= q.n) break;
-            const int64_t at = row * g.row + col + i;
-            float da[8], db[8];
+    for (int part = 0; part < 64; part += 32) {  // a row of 33 words: lanes side by side in a row or in a column
+        float* cells = reinterpret_cast<float*>(scratch);
 #pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const float4 s = ldg4(g.slope + at + e), l = ldg4(g.level + at + e);
-                da[e] = v[i + e] * s.x;
-                da[e + 1] = v[i + e + 1] * s.y;
-                da[e + 2] = v[i + e + 2] * s.z;
-                da[e + 3] = v[i + e + 3] * s.w;
-                db[e] = v[i + e] * l.x;
-                db[e + 1] = v[i + e + 1] * l.y;
-                db[e + 2] = v[i + e + 2] * l.z;
-                db[e + 3] = v[i + e + 3] * l.w;
-            }
-            store_planes8<P>(g.da + at, g.plane, da);
-            store_planes8<P>(g.db + at, g.plane, db);
+        for (int turn = 0; turn < 32; turn += 16) {
+            __syncwarp();
+            if (lane >= turn && lane < turn + 16)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) cells[(lane - turn) * 33 + i] = v[part + i];
+            __syncwarp();
+            for (int r = 0; r < 16 && turn + r < rows; ++r)
+                if (part + lane < left) store1(to + (turn + r) * row + part + lane, cells[r * 33 + lane]);
         }
-    } else if (g.splits > 1) {
-        store_row<64>(q.part + (int64_t(p.split) * q.m + row) * q.part_row, col, q.n, true, v);
-    } else {
-        store_row<64>(static_cast<T*>(q.out) + row * q.n, col, q.n, q.n % 8 == 0, v);
     }
 }
 
@@ -393,7 +425,10 @@ __global__ void __launch_bounds__(kThreads, 1) feed_kernel(const __grid_constant
             warp_wait(&ctl.drain, 0, abort, true);
         }
     } else if (warp >= 4) {
-        const int half = (warp - 4) >> 2, r = threadIdx.x & 127;
+        using T = typename std::conditional<P == 1, __nv_bfloat16, float>::type;
+        const int half = (warp - 4) >> 2;
+        unsigned char* scratch = raw + (ring - su32(raw)) + kRingBytes + (warp - 4) * kScratch;
+        float4 ahead[8];
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         int unit = 0;
         bool ok = true;
@@ -421,25 +456,83 @@ __global__ void __launch_bounds__(kThreads, 1) feed_kernel(const __grid_constant
                 tmem_load64(at + col, v);
             }
         };
+        // kHidden: the factors of the next 32 columns are on their way while the last ones are stored
+        auto fetch = [&](const float* factor, int64_t row0, int64_t col, int rows, int64_t n) {
+            const int pieces = int(max(int64_t(0), min(int64_t(8), (n - col + 7) / 8 * 2)));
+            fetch_rows(factor + row0 * g.row + col, g.row, rows, pieces, ahead);
+        };
+        auto spread = [&](const Problem& q, int64_t row0, int rows, int64_t col, int64_t after, const float* v) {
+            const int pieces = int(max(int64_t(0), min(int64_t(4), (q.n - col + 7) / 8)));
+            const int64_t at = row0 * g.row + col;
+            float x[32];
+            turn_rows(scratch, ahead, x);
+            fetch(g.level, row0, col, rows, q.n);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] *= v[i];
+            put_planes<P>(scratch, x, g.da + at, g.row, g.plane, rows, pieces);
+            turn_rows(scratch, ahead, x);
+            fetch(g.slope, row0, after, rows, q.n);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] *= v[i];
+            put_planes<P>(scratch, x, g.db + at, g.row, g.plane, rows, pieces);
+        };
+        // What follows the sums of 64 columns (kUp: 32 of a, 32 of b) from column `col` of the result (the hidden units).
+        auto finish = [&](const Problem& q, const Place& p, int64_t row0, int rows, int64_t col, float(&v)[64]) {
+            if constexpr (KIND == kUp) {
+                const int pieces = int(max(int64_t(0), min(int64_t(4), (q.n - col + 7) / 8)));
+                float h[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    float level, slope;
+                    activate<P == 3>(g.act, v[i], level, slope);
+                    h[i] = level * v[32 + i];
+                    v[i] = level;
+                    v[32 + i] *= slope;
+                }
+                const int64_t at = row0 * g.row + col;
+                put_planes<P>(scratch, h, g.h + at, g.row, g.plane, rows, pieces);
+                if (g.slope != nullptr) {
+                    put_floats(scratch, v + 32, g.slope + at, g.row, rows, 2 * pieces);
+                    put_floats(scratch, v, g.level + at, g.row, rows, 2 * pieces);
+                }
+            } else if constexpr (KIND == kHidden) {
+                spread(q, row0, rows, col, col + 32, v);
+                spread(q, row0, rows, col + 32, q.n, v + 32);
+            } else if (g.splits > 1) {
+                put_result(scratch, v, q.part + (int64_t(p.split) * q.m + row0) * q.part_row, col, q.part_row, q.part_row, rows,
+                           true);
+            } else {
+                put_result(scratch, v, static_cast<T*>(q.out) + row0 * q.n, col, q.n, q.n, rows, q.n % 8 == 0);
+            }
+        };
         for (int t = blockIdx.x; t < g.tiles && ok; t += gridDim.x) {
             const Place p = place_of(g, t);
             const Problem& q = g.problem[p.problem];
-            const int64_t row = int64_t(p.m) * kM + r, n0 = int64_t(p.n) * (KIND == kUp ? g.bn / 2 : g.bn);
+            const int64_t row0 = int64_t(p.m) * kM + (warp & 3) * 32, n0 = int64_t(p.n) * (KIND == kUp ? g.bn / 2 : g.bn);
+            const int rows = int(max(int64_t(0), min(int64_t(32), q.m - row0)));
+            if constexpr (KIND == kHidden) fetch(g.slope, row0, n0 + first_of(0), rows, q.n);
             if (p.from >= p.to) {  // a split without a share: sums of zero
                 float v[64] = {};
-                for (int it = 0; it < g.bn / 128; ++it)
-                    if (row < q.m) finish<KIND, P>(g, q, p, row, n0 + first_of(it), v);
+                for (int it = 0; it < g.bn / 128; ++it) finish(q, p, row0, rows, n0 + first_of(it), v);
                 continue;
             }
             if constexpr (P == 1) {
                 if (!(ok = wait())) break;
                 const uint32_t at = tmem + lanes + uint32_t(unit & 1) * 256u;
-                const int rounds = g.bn / 128;
+                const int rounds = g.bn / (KIND == kHidden ? 64 : 128);
                 for (int it = 0; it < rounds; ++it) {
-                    float v[64];
-                    load(at, first_of(it), v);
-                    if (it + 1 == rounds) done();
-                    if (row < q.m) finish<KIND, P>(g, q, p, row, n0 + first_of(it), v);
+                    if constexpr (KIND == kHidden) {
+                        float v[32];
+                        const int col = first_of(0) + it * 32;
+                        tmem_load32(at + col, v);
+                        if (it + 1 == rounds) done();
+                        spread(q, row0, rows, n0 + col, it + 1 == rounds ? q.n : n0 + col + 32, v);
+                    } else {
+                        float v[64];
+                        load(at, first_of(it), v);
+                        if (it + 1 == rounds) done();
+                        finish(q, p, row0, rows, n0 + first_of(it), v);
+                    }
                 }
             } else {
                 float sum[64] = {};
@@ -458,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) feed_kernel(const __grid_constant
                     done();
                 }
                 if (!ok) break;
-                if (row < q.m) finish<KIND, P>(g, q, p, row, n0 + first_of(0), sum);
+                finish(q, p, row0, rows, n0 + first_of(0), sum);
             }
         }
     }
@@ -495,7 +588,10 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = c + e < n ? x[e] : 0.0f;
         }
-        store_planes8<3>(a.to[t] + row * a.row[t] + c, plane, v);
+        uint4* to = reinterpret_cast<uint4*>(a.to[t] + row * a.row[t] + c);
+        to[0] = first_plane8(v);
+        to[plane / 8] = next_plane8(v);
+        to[plane / 4] = next_plane8(v);
     }
 }
 
@@ -576,7 +672,7 @@ struct Sizes {
 
 template <int KIND, int P>
 fmd_status launch(const Maps& maps, const Args& g, cudaStream_t s) {
-    constexpr size_t bytes = kRingBytes + 1024;
+    constexpr size_t bytes = kRingBytes + kWorkers / 32 * kScratch + 1024;
     const fmd_status st = grant_dynamic_smem((const void*)feed_kernel<KIND, P>, bytes, true);
     if (st != FMD_OK) return st;
     feed_kernel<KIND, P><<<unsigned(g.tiles < kNumSMs ? g.tiles : kNumSMs), kThreads, bytes, s>>>(maps, g);
