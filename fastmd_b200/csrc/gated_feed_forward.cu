@@ -19,9 +19,9 @@
 // that count: x0 w0 apart from the five small ones, because the tensor cores cut off what does not fit as they add. For the
 // same reason sums are taken out of TMEM and added up in registers every kSegment steps of 64.
 //
-// A block walks over tiles of 128 x bn: warp 0 loads operands by TMA through a ring of slots (64 values of the inner index
-// each), one thread of warp 1 issues the products, warps 4 to 11 take the sums from one of two accumulators in TMEM while
-// the other one is filled: thread = row and half of the columns.
+// A block walks over tiles of 128 x bn: one warp loads operands by TMA through a ring of slots (64 values of the inner index
+// each), one thread of another issues the products, 8 or 16 take the sums from one of two accumulators in TMEM while the
+// other one is filled: thread = row and part of the columns.
 //
 // Every wait is bounded: on expiry the block raises FMD_FLAG_WAIT_TIMEOUT, waits (bounded) for its copies and products in
 // flight, frees its TMEM and returns.
@@ -33,15 +33,24 @@
 namespace fmd {
 namespace {
 
-constexpr int kThreads = 384, kWorkers = 256;
 constexpr int kM = 128, kK = 64;
 constexpr uint32_t kTileA = kM * kK * 2, kPanel = 64 * kK * 2;  // bytes of an operand's tile, of 64 columns of it
 constexpr int kMostSlots = 8;
-constexpr size_t kRingBytes = 192 * 1024, kScratch = 4096;  // kScratch: of each warp that stores
+constexpr size_t kScratch = 4096;  // of each warp that stores
 constexpr int kSegment = 2;
 constexpr float kBf16Max = 3.38953139e38f;
 
 enum Kind { kUp, kDown, kHidden, kInput, kWeights };
+
+// Warps that take the sums: sixteen where much follows them, which eight did not get through in the time of a tile's products
+// (up of 32,000 x 1,024 x 4,096 with its factors 718 us, hidden 923); float32 has six times the products and needs the slots.
+template <int KIND, int P>
+struct Shape {
+    static constexpr int kWarps = P == 1 && (KIND == kUp || KIND == kHidden) ? 16 : 8;
+    static constexpr int kThreads = 64 + 32 * kWarps;  // the takers first: a warp's part of TMEM goes by its number
+    static constexpr size_t kRing = 224 * 1024 - kWarps * kScratch;
+    static constexpr size_t kBytes = 225 * 1024;
+};
 
 // One product [m, n] of a launch.
 struct Problem {
@@ -82,6 +91,10 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(su32(bar))
         : "memory");
 }
+
+__device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[16]) { tmem_load16(at, v); }
+__device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[32]) { tmem_load32(at, v); }
+__device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[64]) { tmem_load64(at, v); }
 
 // Two steps of 16 of D (+)= A B^T; `astep`, `bstep`: how far a step is, in descriptor units.
 template <int ASTEP, int BSTEP>
@@ -131,22 +144,16 @@ __device__ __forceinline__ float rcp(float x) {
 // act(a) and act'(a). EXACT: to FP32's last bits; else to 2^-20 or so, for results in 16 bits.
 template <bool EXACT>
 __device__ __forceinline__ void activate(int act, float a, float& value, float& slope) {
+    // held where a factor of 0 stands for the limit, so that an infinity gives its limit too
+    const float low = fmaxf(a, -1.0e18f), held = fminf(low, 1.0e18f);
     if (act == FMD_FEED_SILU) {
         const float turn = EXACT ? 1.0f / (1.0f + expf(-a)) : rcp(1.0f + ex2(-1.4426950408889634f * a));
-        value = a * turn;
-        slope = turn + value * (1.0f - turn);
-        if (fabsf(a) == INFINITY) {
-            value = a > 0.0f ? a : 0.0f;
-            slope = a > 0.0f ? 1.0f : 0.0f;
-        }
+        value = low * turn;
+        slope = fmaf(held * turn, 1.0f - turn, turn);
     } else {
         const float share = 0.5f * erfcf(-0.7071067811865476f * a);
-        value = a * share;
-        slope = share + a * (0.3989422804014327f * (EXACT ? expf(-0.5f * a * a) : ex2(-0.7213475204444817f * a * a)));
-        if (fabsf(a) == INFINITY) {
-            value = a > 0.0f ? a : 0.0f;
-            slope = a > 0.0f ? 1.0f : 0.0f;
-        }
+        value = low * share;
+        slope = fmaf(held, 0.3989422804014327f * (EXACT ? expf(-0.5f * a * a) : ex2(-0.7213475204444817f * a * a)), share);
     }
 }
 
@@ -158,8 +165,8 @@ __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 // row's number, which keeps the banks apart both ways.
 template <int W>
 __device__ __forceinline__ uint4* piece_at(unsigned char* scratch, int row, int piece) {
-    const int turn = W == 8 ? row & 7 : (row >> 1) & 3;
-    return reinterpret_cast<uint4*>(scratch + (row * W + (piece ^ turn)) * 16);
+    constexpr int kShift = W == 8 ? 0 : W == 4 ? 1 : 2;
+    return reinterpret_cast<uint4*>(scratch + (row * W + (piece ^ (row >> kShift & (W - 1)))) * 16);
 }
 
 // The first `pieces` of each of the first `rows` rows to `to` and on, rows `stride` bytes apart.
@@ -170,22 +177,25 @@ __device__ __forceinline__ void put_rows(unsigned char* scratch, const uint4* w,
 #pragma unroll
     for (int i = 0; i < W; ++i) *piece_at<W>(scratch, lane, i) = w[i];
     __syncwarp();
-    char* p = static_cast<char*>(to) + (lane % W) * 16;
+    if (lane % W >= pieces) return;
+    char* p = static_cast<char*>(to) + (lane / W) * stride + (lane % W) * 16;
+    const int left = rows - lane / W;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        const int row = i * (32 / W) + lane / W;
-        const uint4 x = *piece_at<W>(scratch, row, lane % W);
-        if (row < rows && lane % W < pieces) *reinterpret_cast<uint4*>(p + row * stride) = x;
+        if (i * (32 / W) < left)
+            *reinterpret_cast<uint4*>(p) = *piece_at<W>(scratch, i * (32 / W) + lane / W, lane % W);
+        p += (32 / W) * stride;
     }
 }
 
 // 32 columns of FP32 of 32 rows: the loads (a lane holds pieces of eight rows) ..
 __device__ __forceinline__ void fetch_rows(const float* from, int64_t stride, int rows, int pieces, float4 (&x)[8]) {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, left = lane % 8 < pieces ? rows - lane / 8 : 0;
+    const float* p = from + (lane / 8) * stride + (lane % 8) * 4;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int row = i * 4 + lane / 8;
-        x[i] = row < rows && lane % 8 < pieces ? ldg4(from + row * stride + (lane % 8) * 4) : f4_zero();
+        x[i] = i * 4 < left ? ldg4(p) : f4_zero();
+        p += 4 * stride;
     }
 }
 
@@ -227,51 +237,53 @@ __device__ __forceinline__ uint4 next_plane8(float* v) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 32 values a row as P planes, `plane` values apart; rows are padded to multiples of 8 columns. The values are used up.
-template <int P>
-__device__ __forceinline__ void put_planes(unsigned char* scratch, float (&v)[32], __nv_bfloat16* to, int64_t row,
-                                           int64_t plane, int rows, int pieces) {
-    uint4 w[4];
+// N values a row as P planes, `plane` values apart; rows are padded to multiples of 8 columns. The values are used up.
+template <int P, int N>
+__device__ __forceinline__ void put_planes(unsigned char* scratch, float* v, __nv_bfloat16* to, int64_t row, int64_t plane,
+                                           int rows, int columns) {
+    uint4 w[N / 8];
 #pragma unroll
     for (int q = 0; q < P; ++q) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < N / 8; ++i)
             w[i] = P == 1 ? pack8(v + 8 * i) : q == 0 ? first_plane8(v + 8 * i) : next_plane8(v + 8 * i);
-        put_rows<4>(scratch, w, to + q * plane, row * 2, rows, pieces);
+        put_rows<N / 8>(scratch, w, to + q * plane, row * 2, rows, (columns + 7) / 8);
     }
 }
 
+// N values a row in FP32, as far as `columns` (rounded up to a multiple of 4).
+template <int N>
 __device__ __forceinline__ void put_floats(unsigned char* scratch, const float* v, float* to, int64_t row, int rows,
-                                           int pieces) {
-    uint4 w[8];
+                                           int columns) {
+    uint4 w[N / 4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < N / 4; ++i)
         w[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
                           __float_as_uint(v[4 * i + 3]));
-    put_rows<8>(scratch, w, to, row * 4, rows, pieces);
+    put_rows<N / 4>(scratch, w, to, row * 4, rows, (columns + 3) / 4);
 }
 
-// 64 columns from `col` of a result's rows, `n` columns wide; rows start anywhere unless `vector`.
-template <typename T>
-__device__ __forceinline__ void put_result(unsigned char* scratch, const float (&v)[64], T* to, int64_t col, int64_t n,
-                                           int64_t row, int rows, bool vector) {
-    const int left = int(min(int64_t(64), n - col)), lane = threadIdx.x & 31;
-    if (left <= 0) return;
-    to += col;
+// N columns of a result's rows, `columns` of which exist; rows start anywhere unless `vector`.
+template <int N, typename T>
+__device__ __forceinline__ void put_result(unsigned char* scratch, const float (&v)[N], T* to, int64_t row, int rows, int columns,
+                                           bool vector) {
+    const int lane = threadIdx.x & 31;
+    if (columns <= 0) return;
     if (vector) {
         if constexpr (sizeof(T) == 2) {
-            uint4 w[8];
+            uint4 w[N / 8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = pack8(v + 8 * i);
-            put_rows<8>(scratch, w, to, row * 2, rows, left / 8);
+            for (int i = 0; i < N / 8; ++i) w[i] = pack8(v + 8 * i);
+            put_rows<N / 8>(scratch, w, to, row * 2, rows, columns / 8);
         } else {
-            put_floats(scratch, v, to, row, rows, left / 4);
-            if (left > 32) put_floats(scratch, v + 32, to + 32, row, rows, left / 4 - 8);
+#pragma unroll
+            for (int i = 0; i < N; i += 32)
+                if (columns > i) put_floats<32>(scratch, v + i, to + i, row, rows, columns - i);
         }
         return;
     }
 #pragma unroll
-    for (int part = 0; part < 64; part += 32) {  // a row of 33 words: lanes side by side in a row or in a column
+    for (int part = 0; part < N; part += 32) {  // a row of 33 words: lanes side by side in a row or in a column
         float* cells = reinterpret_cast<float*>(scratch);
 #pragma unroll
         for (int turn = 0; turn < 32; turn += 16) {
@@ -281,13 +293,15 @@ __device__ __forceinline__ void put_result(unsigned char* scratch, const float (
                 for (int i = 0; i < 32; ++i) cells[(lane - turn) * 33 + i] = v[part + i];
             __syncwarp();
             for (int r = 0; r < 16 && turn + r < rows; ++r)
-                if (part + lane < left) store1(to + (turn + r) * row + part + lane, cells[r * 33 + lane]);
+                if (part + lane < columns) store1(to + (turn + r) * row + part + lane, cells[r * 33 + lane]);
         }
     }
 }
 
-template <int KIND, int P>
-__global__ void __launch_bounds__(kThreads, 1) feed_kernel(const __grid_constant__ Maps maps, const Args g) {
+// W: columns of the sums that a warp takes at a time (64 where bn = 256; kUp: half of them a's, half b's).
+template <int KIND, int P, int W>
+__global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const __grid_constant__ Maps maps, const Args g) {
+    using S = Shape<KIND, P>;
     constexpr bool kColumnsA = KIND == kWeights, kColumnsB = KIND == kHidden || KIND == kInput || KIND == kWeights;
     extern __shared__ unsigned char raw[];
     const uint32_t ring = (su32(raw) + 1023u) & ~1023u;
@@ -303,19 +317,19 @@ __global__ void __launch_bounds__(kThreads, 1) feed_kernel(const __grid_constant
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctl.sums[i], 1);
-            mbar_init(&ctl.taken[i], kWorkers / 32);
+            mbar_init(&ctl.taken[i], S::kWarps);
         }
         mbar_init(&ctl.drain, 1);
         ctl.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) tmem_alloc<512>(&ctl.tmem);
+    if (warp == S::kWarps + 1) tmem_alloc<512>(&ctl.tmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl.tmem;
 
-    if (warp == 0) {
+    if (warp == S::kWarps) {
         if (lane == 0) {
             int slot = 0;
             uint32_t phase = 0, armed = 0;  // armed: slots with a copy that nobody may have waited for
@@ -368,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) feed_kernel(const __grid_constant
                 if (!ok) mbar_wait(&ctl.full[i], (turns ^ 1u) & 1u, abort, true);
             }
         }
-    } else if (warp == 1) {
+    } else if (warp > S::kWarps) {
         const uint32_t base = uniform(tmem), first = uniform(ring), bytes = uniform(slot_bytes), b_bytes = uniform(tile_b);
         const int slots = uniform(g.slots), bn = uniform(g.bn);
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (kColumnsA ? 1u << 15 : 0u) |
@@ -424,11 +438,11 @@ __global__ void __launch_bounds__(kThreads, 1) feed_kernel(const __grid_constant
             if (elect_one()) tc_commit(&ctl.drain);
             warp_wait(&ctl.drain, 0, abort, true);
         }
-    } else if (warp >= 4) {
+    } else {
         using T = typename std::conditional<P == 1, __nv_bfloat16, float>::type;
-        const int half = (warp - 4) >> 2;
-        unsigned char* scratch = raw + (ring - su32(raw)) + kRingBytes + (warp - 4) * kScratch;
-        float4 ahead[8];
+        constexpr int kGroups = S::kWarps / 4, kStep = KIND == kUp ? W / 2 : W;  // kStep: columns of the result a unit
+        const int group = warp >> 2, units = g.bn / W;
+        unsigned char* scratch = raw + (ring - su32(raw)) + S::kRing + warp * kScratch;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         int unit = 0;
         bool ok = true;
@@ -446,63 +460,60 @@ __global__ void __launch_bounds__(kThreads, 1) feed_kernel(const __grid_constant
             warp_arrive(&ctl.taken[unit & 1]);
             ++unit;
         };
-        // columns of TMEM and of the result that this thread's 64 sums of round `it` begin at
-        auto first_of = [&](int it) { return KIND == kUp ? half * (g.bn / 4) + it * 32 : half * (g.bn / 2) + it * 64; };
-        auto load = [&](uint32_t at, int col, float (&v)[64]) {
-            if (KIND == kUp) {
-                tmem_load32(at + col, reinterpret_cast<float(&)[32]>(v[0]));
-                tmem_load32(at + g.bn / 2 + col, reinterpret_cast<float(&)[32]>(v[32]));
-            } else {
-                tmem_load64(at + col, v);
-            }
-        };
         // kHidden: the factors of the next 32 columns are on their way while the last ones are stored
+        float4 ahead[8];
         auto fetch = [&](const float* factor, int64_t row0, int64_t col, int rows, int64_t n) {
             const int pieces = int(max(int64_t(0), min(int64_t(8), (n - col + 7) / 8 * 2)));
             fetch_rows(factor + row0 * g.row + col, g.row, rows, pieces, ahead);
         };
-        auto spread = [&](const Problem& q, int64_t row0, int rows, int64_t col, int64_t after, const float* v) {
-            const int pieces = int(max(int64_t(0), min(int64_t(4), (q.n - col + 7) / 8)));
+        // dh of 32 columns by `take(i, v)`, 16 at a time
+        auto spread = [&](const Problem& q, int64_t row0, int rows, int64_t col, int64_t after, auto take, auto taken) {
+            const int columns = int(max(int64_t(0), min(int64_t(32), q.n - col)));
             const int64_t at = row0 * g.row + col;
             float x[32];
             turn_rows(scratch, ahead, x);
             fetch(g.level, row0, col, rows, q.n);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] *= v[i];
-            put_planes<P>(scratch, x, g.da + at, g.row, g.plane, rows, pieces);
+            take(x);
+            put_planes<P, 32>(scratch, x, g.da + at, g.row, g.plane, rows, columns);
             turn_rows(scratch, ahead, x);
             fetch(g.slope, row0, after, rows, q.n);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] *= v[i];
-            put_planes<P>(scratch, x, g.db + at, g.row, g.plane, rows, pieces);
+            take(x);
+            taken();
+            put_planes<P, 32>(scratch, x, g.db + at, g.row, g.plane, rows, columns);
         };
-        // What follows the sums of 64 columns (kUp: 32 of a, 32 of b) from column `col` of the result (the hidden units).
-        auto finish = [&](const Problem& q, const Place& p, int64_t row0, int rows, int64_t col, float(&v)[64]) {
+        // What follows the W sums of column `col` and on (kUp: of the hidden units).
+        auto finish = [&](const Problem& q, const Place& p, int64_t row0, int rows, int64_t col, float(&v)[W]) {
             if constexpr (KIND == kUp) {
-                const int pieces = int(max(int64_t(0), min(int64_t(4), (q.n - col + 7) / 8)));
-                float h[32];
+                constexpr int kH = W / 2;
+                const int columns = int(max(int64_t(0), min(int64_t(kH), q.n - col)));
+                const int64_t at = row0 * g.row + col;
+                uint4 first[kH / 8];
+                float h[P == 3 ? kH : 8];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
+                for (int i = 0; i < kH; ++i) {
                     float level, slope;
                     activate<P == 3>(g.act, v[i], level, slope);
-                    h[i] = level * v[32 + i];
+                    h[P == 3 ? i : i % 8] = level * v[kH + i];
                     v[i] = level;
-                    v[32 + i] *= slope;
+                    v[kH + i] *= slope;
+                    if (P == 1 && i % 8 == 7) first[i / 8] = pack8(h);
                 }
-                const int64_t at = row0 * g.row + col;
-                put_planes<P>(scratch, h, g.h + at, g.row, g.plane, rows, pieces);
+                if constexpr (P == 1)
+                    put_rows<kH / 8>(scratch, first, g.h + at, g.row * 2, rows, (columns + 7) / 8);
+                else
+                    put_planes<P, kH>(scratch, h, g.h + at, g.row, g.plane, rows, columns);
                 if (g.slope != nullptr) {
-                    put_floats(scratch, v + 32, g.slope + at, g.row, rows, 2 * pieces);
-                    put_floats(scratch, v, g.level + at, g.row, rows, 2 * pieces);
+                    put_floats<kH>(scratch, v + kH, g.slope + at, g.row, rows, (columns + 7) & ~7);
+                    put_floats<kH>(scratch, v, g.level + at, g.row, rows, (columns + 7) & ~7);
                 }
-            } else if constexpr (KIND == kHidden) {
-                spread(q, row0, rows, col, col + 32, v);
-                spread(q, row0, rows, col + 32, q.n, v + 32);
-            } else if (g.splits > 1) {
-                put_result(scratch, v, q.part + (int64_t(p.split) * q.m + row0) * q.part_row, col, q.part_row, q.part_row, rows,
-                           true);
-            } else {
-                put_result(scratch, v, static_cast<T*>(q.out) + row0 * q.n, col, q.n, q.n, rows, q.n % 8 == 0);
+            } else if constexpr (KIND != kHidden) {
+                const bool parts = g.splits > 1;
+                const int64_t n = parts ? q.part_row : q.n;
+                const int columns = int(max(int64_t(0), min(int64_t(W), n - col)));
+                if (parts)
+                    put_result<W>(scratch, v, q.part + (int64_t(p.split) * q.m + row0) * n + col, n, rows, columns, true);
+                else
+                    put_result<W>(scratch, v, static_cast<T*>(q.out) + row0 * n + col, n, rows, columns, n % 8 == 0);
             }
         };
         for (int t = blockIdx.x; t < g.tiles && ok; t += gridDim.x) {
@@ -510,55 +521,90 @@ __global__ void __launch_bounds__(kThreads, 1) feed_kernel(const __grid_constant
             const Problem& q = g.problem[p.problem];
             const int64_t row0 = int64_t(p.m) * kM + (warp & 3) * 32, n0 = int64_t(p.n) * (KIND == kUp ? g.bn / 2 : g.bn);
             const int rows = int(max(int64_t(0), min(int64_t(32), q.m - row0)));
-            if constexpr (KIND == kHidden) fetch(g.slope, row0, n0 + first_of(0), rows, q.n);
+            if (KIND == kHidden && group < units) fetch(g.slope, row0, n0 + group * kStep, rows, q.n);
             if (p.from >= p.to) {  // a split without a share: sums of zero
-                float v[64] = {};
-                for (int it = 0; it < g.bn / 128; ++it) finish(q, p, row0, rows, n0 + first_of(it), v);
+                float v[W] = {};
+                for (int u = group; u < units; u += kGroups) finish(q, p, row0, rows, n0 + u * kStep, v);
                 continue;
             }
             if constexpr (P == 1) {
                 if (!(ok = wait())) break;
                 const uint32_t at = tmem + lanes + uint32_t(unit & 1) * 256u;
-                const int rounds = g.bn / (KIND == kHidden ? 64 : 128);
-                for (int it = 0; it < rounds; ++it) {
+                if (group >= units) done();
+                for (int u = group; u < units; u += kGroups) {
+                    const bool last = u + kGroups >= units;
                     if constexpr (KIND == kHidden) {
-                        float v[32];
-                        const int col = first_of(0) + it * 32;
-                        tmem_load32(at + col, v);
-                        if (it + 1 == rounds) done();
-                        spread(q, row0, rows, n0 + col, it + 1 == rounds ? q.n : n0 + col + 32, v);
+#pragma unroll 1
+                        for (int j = 0; j < W; j += 32) {
+                            const bool end = last && j + 32 == W;
+                            const int64_t col = n0 + u * W + j;
+                            const int64_t after = end ? q.n : j + 32 < W ? col + 32 : n0 + (u + kGroups) * W;
+                            spread(q, row0, rows, col, after,
+                                   [&](float(&x)[32]) {
+#pragma unroll
+                                       for (int i = 0; i < 32; i += 16) {
+                                           float v[16];
+                                           tmem_load16(at + u * W + j + i, v);
+#pragma unroll
+                                           for (int e = 0; e < 16; ++e) x[i + e] *= v[e];
+                                       }
+                                   },
+                                   [&]() {
+                                       if (end) done();
+                                   });
+                        }
                     } else {
-                        float v[64];
-                        load(at, first_of(it), v);
-                        if (it + 1 == rounds) done();
-                        finish(q, p, row0, rows, n0 + first_of(it), v);
+                        float v[W];
+                        if constexpr (KIND == kUp) {
+                            tmem_load(at + u * kStep, reinterpret_cast<float(&)[W / 2]>(v[0]));
+                            tmem_load(at + g.bn / 2 + u * kStep, reinterpret_cast<float(&)[W / 2]>(v[W / 2]));
+                        } else {
+                            tmem_load(at + u * kStep, v);
+                        }
+                        if (last) done();
+                        finish(q, p, row0, rows, n0 + u * kStep, v);
                     }
                 }
             } else {
-                float sum[64] = {};
+                constexpr int kUnits = 128 / W / kGroups;  // bn = 128
+                float sum[kUnits][W] = {};
                 for (int start = p.from; start < p.to; start += kSegment) {
                     if (!(ok = wait())) break;
                     const uint32_t at = tmem + lanes + uint32_t(unit & 1) * 256u;
 #pragma unroll
-                    for (int j = 0; j < 64; j += 32) {
-                        const uint32_t col = uint32_t(first_of(0)) + (KIND == kUp && j > 0 ? g.bn / 2 : j);
-                        float big[32], small[32];
-                        tmem_load32(at + col, big);
-                        tmem_load32(at + 128 + col, small);
+                    for (int u = 0; u < kUnits; ++u)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) sum[j + i] += big[i] + small[i];
-                    }
+                        for (int j = 0; j < W; j += 16) {
+                            const int col = (group + u * kGroups) * kStep + (KIND == kUp && j >= W / 2 ? 64 + j - W / 2 : j);
+                            float big[16], small[16];
+                            tmem_load16(at + col, big);
+                            tmem_load16(at + 128 + col, small);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) sum[u][j + i] += big[i] + small[i];
+                        }
                     done();
                 }
                 if (!ok) break;
-                finish(q, p, row0, rows, n0 + first_of(0), sum);
+#pragma unroll
+                for (int u = 0; u < kUnits; ++u) {
+                    const int64_t col = n0 + (group + u * kGroups) * kStep;
+                    if constexpr (KIND == kHidden)
+                        spread(q, row0, rows, col, u + 1 < kUnits ? col + kGroups * kStep : q.n,
+                               [&](float(&x)[32]) {
+#pragma unroll
+                                   for (int i = 0; i < 32; ++i) x[i] *= sum[u][i];
+                               },
+                               []() {});
+                    else
+                        finish(q, p, row0, rows, col, sum[u]);
+                }
             }
         }
     }
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) tmem_free<512>(tmem);
+    if (warp == S::kWarps + 1) tmem_free<512>(tmem);
     if (threadIdx.x == 0 && ctl.abort) raise_flag(g.flags, FMD_FLAG_WAIT_TIMEOUT);
 }
 
@@ -643,18 +689,24 @@ struct Plan {
     int bn, splits;
 };
 
-// The time of a launch in steps of 128 x 256 x 64: rounds of blocks, each its tile's steps and, besides, about four for
-// its start and end (its output for kinds that write much); the shares' sums are written and read again.
-Plan plan(const int64_t* m, const int64_t* n, int problems, int64_t steps, int planes, bool can_split) {
+// The time of a launch in steps of 128 x 256 x 64, about 0.3 us each: rounds of blocks, each its tile's steps and, besides,
+// about six for its start and end; the shares' sums are written and read again. unit: bn is a multiple of it (panels of 64
+// columns where the rows of B are the inner index; else any 32, so that few rows' weights are read by all SMs alike).
+Plan plan(const int64_t* m, const int64_t* n, int problems, int64_t steps, int planes, int unit, bool can_split) {
     Plan best{128, 1};
     double least = 1e300;
-    for (int bn = 128; bn <= (planes == 1 ? 256 : 128); bn *= 2) {
+    for (int bn = planes == 1 ? 64 : 128; bn <= (planes == 1 ? 256 : 128); bn += unit) {
         int64_t tiles = 0;
-        for (int i = 0; i < problems; ++i) tiles += ((m[i] + kM - 1) / kM) * ((n[i] + bn - 1) / bn);
+        double values = 0.0;
+        for (int i = 0; i < problems; ++i) {
+            tiles += ((m[i] + kM - 1) / kM) * ((n[i] + bn - 1) / bn);
+            values += double(m[i]) * double(n[i]);
+        }
         for (int splits = 1; splits <= (can_split ? 64 : 1) && (splits == 1 || 4 * splits <= steps); ++splits) {
             const int64_t rounds = (tiles * splits + kNumSMs - 1) / kNumSMs;
-            const double step = (planes == 1 ? 1.0 : 6.0) * (bn == 256 ? 1.0 : 0.6);
-            const double time = rounds * (((steps + splits - 1) / splits) * step + 4.0) + (splits > 1 ? 16.0 + splits : 0.0);
+            const double step = (planes == 1 ? 1.0 : 6.0) * (0.25 + 0.75 * bn / 256.0);
+            const double sums = splits > 1 ? 10.0 + (2.0 * splits + 1.0) * values * 4.0 / 6.5e6 / 0.3 : 0.0;
+            const double time = rounds * (((steps + splits - 1) / splits) * step + 6.0) + sums;
             if (time < least) {
                 least = time;
                 best = Plan{bn, splits};
@@ -670,12 +722,14 @@ struct Sizes {
     int64_t hidden_row, width_row, out_row;  // of the arrays made here
 };
 
-template <int KIND, int P>
-fmd_status launch(const Maps& maps, const Args& g, cudaStream_t s) {
-    constexpr size_t bytes = kRingBytes + kWorkers / 32 * kScratch + 1024;
-    const fmd_status st = grant_dynamic_smem((const void*)feed_kernel<KIND, P>, bytes, true);
+template <int KIND, int P, int W>
+fmd_status launch(const Maps& maps, Args& g, cudaStream_t s) {
+    using S = Shape<KIND, P>;
+    const fmd_status st = grant_dynamic_smem((const void*)feed_kernel<KIND, P, W>, S::kBytes, true);
     if (st != FMD_OK) return st;
-    feed_kernel<KIND, P><<<unsigned(g.tiles < kNumSMs ? g.tiles : kNumSMs), kThreads, bytes, s>>>(maps, g);
+    const int slots = int(S::kRing / (P * (kTileA + g.bn * 128)));
+    g.slots = slots < kMostSlots ? slots : kMostSlots;
+    feed_kernel<KIND, P, W><<<unsigned(g.tiles < kNumSMs ? g.tiles : kNumSMs), S::kThreads, S::kBytes, s>>>(maps, g);
     return check_launch();
 }
 
@@ -692,8 +746,6 @@ fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args&
     }
     g.bn = p.bn;
     g.splits = p.splits;
-    const int slots = int(kRingBytes / (planes * (kTileA + p.bn * 128)));
-    g.slots = slots < kMostSlots ? slots : kMostSlots;
     g.tiles = 0;
     for (int i = 0; i < g.problems; ++i) {
         Problem& q = g.problem[i];
@@ -704,7 +756,8 @@ fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args&
         g.tiles += q.m_tiles * q.n_tiles * p.splits;
     }
     if (g.tiles == 0) return FMD_OK;
-    fmd_status st = planes == 1 ? launch<KIND, 1>(maps, g, s) : launch<KIND, 3>(maps, g, s);
+    fmd_status st = planes == 3 ? launch<KIND, 3, 32>(maps, g, s)
+                    : g.bn == 256 ? launch<KIND, 1, 64>(maps, g, s) : launch<KIND, 1, 32>(maps, g, s);
     if (st != FMD_OK || p.splits == 1) return st;
     int64_t most = 0;
     for (int i = 0; i < g.problems; ++i) {
@@ -723,11 +776,11 @@ size_t part_bytes(const Plan& p, int64_t m, int64_t n) {
     return p.splits > 1 ? size_t(p.splits) * m * round_up(n, 8) * sizeof(float) : 0;
 }
 
-Plan down_plan(const Sizes& z) { return plan(&z.rows, &z.out, 1, steps_of(z.hidden), z.planes, true); }
-Plan input_plan(const Sizes& z) { return plan(&z.rows, &z.width, 1, 2 * steps_of(z.hidden), z.planes, true); }
+Plan down_plan(const Sizes& z) { return plan(&z.rows, &z.out, 1, steps_of(z.hidden), z.planes, 32, true); }
+Plan input_plan(const Sizes& z) { return plan(&z.rows, &z.width, 1, 2 * steps_of(z.hidden), z.planes, 64, true); }
 Plan weights_plan(const Sizes& z) {
     const int64_t m[3] = {z.hidden, z.hidden, z.out}, n[3] = {z.width, z.width, z.hidden};
-    return plan(m, n, 3, steps_of(z.rows), z.planes, true);
+    return plan(m, n, 3, steps_of(z.rows), z.planes, 64, true);
 }
 
 // Arrays in one buffer, each at a multiple of 256 bytes.
@@ -904,7 +957,7 @@ fmd_status fmd_gated_feed_forward(const fmd_feed_forward* problem, void* y, int3
     {
         const Matrix a[2] = {in.x, {}}, b[2] = {in.gate, in.up};
         const int64_t twice = 2 * z.hidden;  // two columns of sums for one of h
-        if ((st = run<kUp>(z.planes, a, b, 2, g, plan(&z.rows, &twice, 1, g.steps, z.planes, false), s)) != FMD_OK) return st;
+        if ((st = run<kUp>(z.planes, a, b, 2, g, plan(&z.rows, &twice, 1, g.steps, z.planes, 32, false), s)) != FMD_OK) return st;
     }
     g.problem[0].n = z.out;
     g.problem[0].out = y;
@@ -968,7 +1021,7 @@ fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kep
         args.problem[0].n = z.hidden;
         args.steps = int(steps_of(z.out));
         st = run<kHidden>(z.planes, &gm, &in.down, 1, args,
-                          plan(&z.rows, &z.hidden, 1, args.steps, z.planes, false), s);
+                          plan(&z.rows, &z.hidden, 1, args.steps, z.planes, 64, false), s);
         if (st != FMD_OK) return st;
     }
     const Matrix da{own + w.da, z.rows, z.hidden, z.hidden_row, z.planes}, db{own + w.db, z.rows, z.hidden, z.hidden_row, z.planes};
