@@ -35,8 +35,7 @@ namespace {
 
 constexpr int kM = 128, kK = 64;
 constexpr uint32_t kTileA = kM * kK * 2, kPanel = 64 * kK * 2;  // bytes of an operand's tile, of 64 columns of it
-constexpr int kMostSlots = 8;
-constexpr size_t kScratch = 4096;  // of each warp that stores
+constexpr int kMostSlots = 12;
 constexpr int kSegment = 2;
 constexpr float kBf16Max = 3.38953139e38f;
 
@@ -48,6 +47,7 @@ template <int KIND, int P>
 struct Shape {
     static constexpr int kWarps = P == 1 && (KIND == kUp || KIND == kHidden) ? 16 : 8;
     static constexpr int kThreads = 64 + 32 * kWarps;  // the takers first: a warp's part of TMEM goes by its number
+    static constexpr size_t kScratch = P == 1 && KIND == kUp ? 2048 : 4096;  // of each of these warps
     static constexpr size_t kRing = 224 * 1024 - kWarps * kScratch;
     static constexpr size_t kBytes = 225 * 1024;
 };
@@ -66,6 +66,7 @@ struct Args {
     int32_t problems, splits, tiles;
     int32_t steps, turn;  // of 64 along the inner index; from step `turn` on the second pair of maps (kInput)
     int32_t bn, slots, act;
+    int32_t tile_a;  // bytes of A's tile in a slot
     // h, da and db: [planes][rows][row]; what is kept: [rows][row] FP32
     __nv_bfloat16 *h, *da, *db;
     float *slope, *level;
@@ -160,7 +161,7 @@ __device__ __forceinline__ void activate(int act, float a, float& value, float& 
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 
-// A thread holds a row of the sums, memory wants rows side by side: what a warp stores or loads goes through 4 KB of shared
+// A thread holds a row of the sums, memory wants rows side by side: what a warp stores or loads goes through 2 or 4 KB of shared
 // memory of its own, W pieces of 16 bytes a row, so that W lanes reach into one row. The pieces of a row are turned by the
 // row's number, which keeps the banks apart both ways.
 template <int W>
@@ -298,7 +299,7 @@ __device__ __forceinline__ void put_result(unsigned char* scratch, const float (
     }
 }
 
-// W: columns of the sums that a warp takes at a time (64 where bn = 256; kUp: half of them a's, half b's).
+// W: columns of the sums that a warp takes at a time (kUp: half of them a's, half b's).
 template <int KIND, int P, int W>
 __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const __grid_constant__ Maps maps, const Args g) {
     using S = Shape<KIND, P>;
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
     __shared__ Ctrl ctl;
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t tile_b = uint32_t(g.bn) * 128u, slot_bytes = P * (kTileA + tile_b);
+    const uint32_t tile_b = uint32_t(g.bn) * 128u, tile_a = g.tile_a, slot_bytes = P * (tile_a + tile_b);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMostSlots; ++i) {
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                     const int k0 = (second ? step - g.turn : step) * kK;
                     const CUtensorMap *ma = &maps.a[second ? 1 : q.a], *mb = &maps.b[second ? 1 : q.b];
                     for (int i = 0; i < P; ++i) {
-                        const uint32_t a = at + i * kTileA, b = at + P * kTileA + uint32_t(i) * tile_b;
+                        const uint32_t a = at + P * tile_b + uint32_t(i) * tile_a, b = at + uint32_t(i) * tile_b;
                         if (kColumnsA) {
                             tma_load_3d(a, ma, bar, m0, k0, i);
                             tma_load_3d(a + kPanel, ma, bar, m0 + 64, k0, i);
@@ -383,7 +384,8 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             }
         }
     } else if (warp > S::kWarps) {
-        const uint32_t base = uniform(tmem), first = uniform(ring), bytes = uniform(slot_bytes), b_bytes = uniform(tile_b);
+        const uint32_t base = uniform(tmem), first = uniform(ring), bytes = uniform(slot_bytes), b_bytes = uniform(tile_b),
+                       a_bytes = uniform(tile_a);
         const int slots = uniform(g.slots), bn = uniform(g.bn);
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (kColumnsA ? 1u << 15 : 0u) |
                                (kColumnsB ? 1u << 16 : 0u) | (uint32_t(bn >> 3) << 17) | (uint32_t(kM >> 4) << 24);
@@ -407,7 +409,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                     tc_fence_after();
                     const uint32_t at = first + uint32_t(slot) * bytes;
                     if (elect_one()) {
-                        const uint32_t a = desc(at, kColumnsA), b = desc(at + P * kTileA, kColumnsB);
+                        const uint32_t a = desc(at + P * b_bytes, kColumnsA), b = desc(at, kColumnsB);
                         const bool add = step > start;
                         if (P == 1) {
                             mma2<kStepA, kStepB>(d, a, b, idesc, add);
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                             constexpr int kPa[6] = {2, 1, 0, 1, 0, 0}, kPb[6] = {0, 1, 2, 0, 1, 0};
 #pragma unroll
                             for (int i = 0; i < 6; ++i) {
-                                const uint32_t x = a + kPa[i] * (kTileA >> 4), y = b + kPb[i] * (b_bytes >> 4);
+                                const uint32_t x = a + kPa[i] * (a_bytes >> 4), y = b + kPb[i] * (b_bytes >> 4);
                                 const uint32_t to_sum = i < 5 ? d + 128 : d;
                                 mma2<kStepA, kStepB>(to_sum, x, y, idesc, add || (i > 0 && i < 5));
                                 mma2<kStepA, kStepB>(to_sum, x + 2 * kStepA, y + 2 * kStepB, idesc, true);
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
         using T = typename std::conditional<P == 1, __nv_bfloat16, float>::type;
         constexpr int kGroups = S::kWarps / 4, kStep = KIND == kUp ? W / 2 : W;  // kStep: columns of the result a unit
         const int group = warp >> 2, units = g.bn / W;
-        unsigned char* scratch = raw + (ring - su32(raw)) + S::kRing + warp * kScratch;
+        unsigned char* scratch = raw + (ring - su32(raw)) + S::kRing + warp * S::kScratch;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         int unit = 0;
         bool ok = true;
@@ -727,7 +729,7 @@ fmd_status launch(const Maps& maps, Args& g, cudaStream_t s) {
     using S = Shape<KIND, P>;
     const fmd_status st = grant_dynamic_smem((const void*)feed_kernel<KIND, P, W>, S::kBytes, true);
     if (st != FMD_OK) return st;
-    const int slots = int(S::kRing / (P * (kTileA + g.bn * 128)));
+    const int slots = int(S::kRing / (P * (g.tile_a + g.bn * 128)));
     g.slots = slots < kMostSlots ? slots : kMostSlots;
     feed_kernel<KIND, P, W><<<unsigned(g.tiles < kNumSMs ? g.tiles : kNumSMs), S::kThreads, S::kBytes, s>>>(maps, g);
     return check_launch();
@@ -737,9 +739,14 @@ template <int KIND>
 fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args& g, const Plan& p, cudaStream_t s) {
     Maps maps{};
     const bool columns_a = KIND == kWeights, columns_b = KIND == kHidden || KIND == kInput || KIND == kWeights;
+    // Few rows: the slots hold these alone, so that more of the weights are on their way (up of 8 rows, 4,096 x 11,000:
+    // 57 -> 36 us). The products read on to 128 rows, into what follows in shared memory, for rows of the result that
+    // nobody takes.
+    const int rows = g.problem[0].m < kM ? int(round_up(g.problem[0].m, 8)) : kM;
+    g.tile_a = columns_a ? int(kTileA) : rows * kK * 2;
     for (int i = 0; i < operands; ++i) {
         fmd_status st = FMD_OK;
-        if (a[i].data != nullptr) st = encode(&maps.a[i], a[i], columns_a ? kK : kM);
+        if (a[i].data != nullptr) st = encode(&maps.a[i], a[i], columns_a ? kK : rows);
         if (st == FMD_OK && b[i].data != nullptr)
             st = encode(&maps.b[i], b[i], columns_b ? kK : KIND == kUp ? p.bn / 2 : p.bn);
         if (st != FMD_OK) return st;
@@ -757,7 +764,7 @@ fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args&
     }
     if (g.tiles == 0) return FMD_OK;
     fmd_status st = planes == 3 ? launch<KIND, 3, 32>(maps, g, s)
-                    : g.bn == 256 ? launch<KIND, 1, 64>(maps, g, s) : launch<KIND, 1, 32>(maps, g, s);
+                    : KIND != kUp && g.bn == 256 ? launch<KIND, 1, KIND == kUp ? 32 : 64>(maps, g, s) : launch<KIND, 1, 32>(maps, g, s);
     if (st != FMD_OK || p.splits == 1) return st;
     int64_t most = 0;
     for (int i = 0; i < g.problems; ++i) {
