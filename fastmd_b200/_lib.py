@@ -218,8 +218,8 @@ KERNELS_PER_CALL = {"fmd_refilter_edges": 2, "fmd_refilter_edges_noalloc": 2, "f
                     "fmd_head_rotary_workspace_bytes": 0,
                     # up and down; hidden, input and weights (float32 planes and shares of a sum add one each)
                     "fmd_gated_feed_forward": 2, "fmd_gated_feed_forward_bwd": 3, "fmd_gated_feed_forward_bytes": 0,
-                    # segments add two a pass
-                    "fmd_decay_attention_bwd": 3, "fmd_decay_attention_workspace_bytes": 0}
+                    # the least: planes of float32 add one, segments two, the last matrices one
+                    "fmd_decay_attention_workspace_bytes": 0}
 
 
 def fused_step_kernels(n_layers: int) -> int:

@@ -2,6 +2,7 @@
 // the recurrence for single rows.
 
 #include "decay_attention.cuh"
+#include "tensor_cores.cuh"
 
 namespace fmd {
 namespace {
@@ -9,10 +10,11 @@ namespace {
 constexpr int kThreads = 256;
 
 // From what each segment adds to what it starts from, in place, and the matrix behind the last row. A block per sequence,
-// head and 1,024 of the matrix's values (four a thread), which it takes through the segments one after the other; the next
-// ones are loaded ahead.
-__global__ void __launch_bounds__(kThreads) carry_kernel(const Decay d) {
-    constexpr int kAhead = 8;
+// head and 1,024 of the matrix's values (four a thread), which it takes through the segments one after the other, sixteen
+// loaded at a time.
+__global__ void __launch_bounds__(kThreads) carry_kernel(const __grid_constant__ Decays all) {
+    constexpr int kAhead = 16;
+    const Decay& d = all.d[blockIdx.z];
     const int b = blockIdx.x / d.heads, head = blockIdx.x % d.heads;
     const int size = d.dim * d.dim, at = (blockIdx.y * kThreads + threadIdx.x) * 4;
     const float l2 = log2_decay(d, head);
@@ -22,7 +24,7 @@ __global__ void __launch_bounds__(kThreads) carry_kernel(const Decay d) {
     const int64_t n = hi - lo, most = decay_segments(d);
     // bad offsets do not lead out of the array
     const int64_t first = min(max(r0 / d.length + b, int64_t(0)), most);
-    const int64_t count = min((n + d.length - 1) / d.length, most - first);
+    const int count = int(min((n + d.length - 1) / d.length, most - first));
     const int64_t mine = (int64_t(b) * d.heads + head) * size;
     const int row = at / d.dim, col = at - row * d.dim;
     float4 state = f4_zero();
@@ -34,10 +36,10 @@ __global__ void __launch_bounds__(kThreads) carry_kernel(const Decay d) {
             state = ldg4(d.start + mine + at);
         }
     }
-    const float whole = exp2f(float(d.length) * l2);
+    const float whole = exp2f(float(d.length) * l2), last = exp2f(float(n - (count - 1) * d.length) * l2);
     float* p = d.states + (first * d.heads + head) * size + at;
     const int64_t step = int64_t(d.heads) * size;
-    for (int64_t i = 0; i < count; i += kAhead) {
+    for (int i = 0; i < count; i += kAhead) {
         float4 added[kAhead];
 #pragma unroll
         for (int e = 0; e < kAhead; ++e)
@@ -45,8 +47,7 @@ __global__ void __launch_bounds__(kThreads) carry_kernel(const Decay d) {
 #pragma unroll
         for (int e = 0; e < kAhead; ++e) {
             if (i + e >= count) break;
-            const int64_t rows = min(d.length, n - (i + e) * d.length);
-            const float keep = rows == d.length ? whole : exp2f(float(rows) * l2);
+            const float keep = i + e + 1 < count ? whole : last;
             st4(p + (i + e) * step, state);
             state = make_float4(fmaf(keep, state.x, added[e].x), fmaf(keep, state.y, added[e].y),
                                 fmaf(keep, state.z, added[e].z), fmaf(keep, state.w, added[e].w));
@@ -58,6 +59,30 @@ __global__ void __launch_bounds__(kThreads) carry_kernel(const Decay d) {
         q[0] = state.x, q[d.dim] = state.y, q[2 * d.dim] = state.z, q[3 * d.dim] = state.w;
     } else {
         st4(d.after + mine + at, state);
+    }
+}
+
+// float32 [rows, heads, dim] as three planes [3][rows][heads][dim] of bfloat16, up to four arrays (blockIdx.y).
+struct SplitArgs {
+    const float* x[4];
+    __nv_bfloat16* to[4];
+    int64_t row[4], head[4];
+    int64_t rows;
+    int32_t heads, dim;
+};
+
+__global__ void __launch_bounds__(kThreads) split_kernel(const SplitArgs a) {
+    const int t = blockIdx.y, per = a.dim / 8;
+    const int64_t heads = a.rows * a.heads, all = heads * per;
+    for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < all; i += int64_t(gridDim.x) * kThreads) {
+        const int64_t r = i / per, row = r / a.heads;
+        const float* x = a.x[t] + row * a.row[t] + (r - row * a.heads) * a.head[t] + (i - r * per) * 8;
+        const float4 p = ldg4(x), q = ldg4(x + 4);
+        float v[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+        uint4* to = reinterpret_cast<uint4*>(a.to[t]) + i;
+        to[0] = first_plane8(v);
+        to[all] = next_plane8(v);
+        to[2 * all] = next_plane8(v);
     }
 }
 
@@ -134,43 +159,101 @@ fmd_status check_rows(const fmd_decay& p, Decay& d) {
     return FMD_OK;
 }
 
-// Rows of a segment: whole sequences where these are blocks enough for the GPU or short; else so many that there are
-// about two blocks an SM.
-int64_t segment_length(const Decay& d) {
-    if (d.batch == 0) return kWhole;
-    const int64_t blocks = int64_t(d.batch) * d.heads, mean = d.rows / d.batch;
-    if (blocks >= 2 * kNumSMs || mean <= 512) return kWhole;
-    const int64_t want = (2 * kNumSMs + d.heads - 1) / d.heads;  // segments of all sequences together
-    int64_t length = (d.rows / want + 127) / 128 * 128;
+// How the recurrence runs, from the sizes alone.
+enum Path { kMma, kPlanes, kSimt };
+
+// float32 heads of up to 64 values go through planes on the tensor cores, wider ones stay on the FP32 cores: the planes of a
+// chunk of 128 rows do not fit beside those of the matrix.
+Path path_of(const Decay& d, int type) { return type == FMD_BF16 ? kMma : d.dim <= 64 ? kPlanes : kSimt; }
+
+// Rows of a segment: whole sequences where these are blocks enough for the GPU or short; else so many that the segments fill
+// it once (the sequences' last ones are half a segment long on average). Segments cost a second look at two of the three
+// inputs and two more launches.
+int64_t segment_length(const Decay& d, Path path) {
+    const int64_t places = (path == kMma && d.dim <= 64 ? 2 : 1) * kNumSMs;
+    if (d.batch == 0 || d.rows / d.batch <= 512 || 10 * int64_t(d.batch) * d.heads >= 6 * places) return kWhole;
+    const int64_t want = 2 * places / d.heads - d.batch;  // twice the segments, less the sequences' last ones
+    const int64_t length = (2 * d.rows / (want > 1 ? want : 1) + 127) / 128 * 128;
     return length < 256 ? 256 : length;
 }
 
 size_t matrices(const Decay& d, int64_t n) { return size_t(n) * d.heads * d.dim * d.dim * sizeof(float); }
 
-// One pass of the recurrence: with segments, or where the last matrix is wanted, what the segments add comes first.
-fmd_status mix(Decay d, bool bf16, void* workspace, cudaStream_t s) {
-    d.length = segment_length(d);
-    const bool carried = d.length < kWhole || d.after != nullptr;
-    const int64_t segments = decay_segments(d);
-    if (segments * d.heads > INT32_MAX) return FMD_ERR_UNSUPPORTED;
-    fmd_status st = FMD_OK;
-    if (carried && d.batch > 0) {
-        d.states = static_cast<float*>(workspace);
-        if (d.rows > 0) st = bf16 ? decay_states_mma(d, s) : decay_states_simt(d, s);
-        if (st != FMD_OK) return st;
-        const int64_t blocks = int64_t(d.batch) * d.heads;
-        if (blocks > INT32_MAX) return FMD_ERR_UNSUPPORTED;
-        carry_kernel<<<dim3(unsigned(blocks), unsigned((d.dim * d.dim + 4 * kThreads - 1) / (4 * kThreads))), kThreads, 0,
-                       s>>>(d);
-        if ((st = check_launch()) != FMD_OK) return st;
-    }
-    if (d.rows == 0 || d.out == nullptr) return FMD_OK;
-    return bf16 ? decay_rows_mma(d, carried, s) : decay_rows_simt(d, carried, s);
+size_t plane_bytes(const Decay& d) { return (size_t(d.rows) * d.heads * d.dim * 6 + 255) / 256 * 256; }
+
+// Planes of `arrays` inputs, and what the segments of `passes` passes add.
+size_t workspace_of(Decay d, int type, int arrays, int passes) {
+    const Path path = path_of(d, type);
+    d.length = segment_length(d, path);
+    return (path == kPlanes ? arrays * plane_bytes(d) : 0) +
+           (d.length < kWhole ? passes * matrices(d, decay_segments(d)) : 0);
 }
 
-size_t mix_bytes(Decay d, bool after) {
-    d.length = segment_length(d);
-    return d.length < kWhole || after ? matrices(d, decay_segments(d)) : 0;
+// The inputs as the kernels read them: in float32 their planes, which `split` makes.
+struct Input {
+    const void* data;
+    int64_t row, head;
+};
+
+fmd_status make_planes(const Decay& d, Path path, Input* inputs, int count, char*& workspace, cudaStream_t s) {
+    if (path != kPlanes || d.rows == 0) return FMD_OK;
+    SplitArgs a{};
+    a.rows = d.rows;
+    a.heads = d.heads;
+    a.dim = d.dim;
+    for (int i = 0; i < count; ++i) {
+        a.x[i] = static_cast<const float*>(inputs[i].data);
+        a.row[i] = inputs[i].row;
+        a.head[i] = inputs[i].head;
+        a.to[i] = reinterpret_cast<__nv_bfloat16*>(workspace);
+        inputs[i] = Input{workspace, int64_t(d.heads) * d.dim, d.dim};
+        workspace += plane_bytes(d);
+    }
+    split_kernel<<<dim3(unsigned(grid_for(d.rows * d.heads * (d.dim / 8), kThreads)), unsigned(count)), kThreads, 0, s>>>(a);
+    return check_launch();
+}
+
+void read_from(Decay& d, const Input& a, const Input& b, const Input& c) {
+    d.a = a.data, d.a_row = a.row, d.a_head = a.head;
+    d.b = b.data, d.b_row = b.row, d.b_head = b.head;
+    d.c = c.data, d.c_row = c.row, d.c_head = c.head;
+}
+
+fmd_status run_states(const Decays& d, Path path, cudaStream_t s) {
+    return path == kMma ? decay_states_mma(d, s) : path == kPlanes ? decay_states_planes(d, s) : decay_states_simt(d, s);
+}
+
+// Passes of the recurrence over the same rows, side by side: with segments what these add comes first.
+fmd_status mix(Decays all, Path path, char* workspace, cudaStream_t s) {
+    const Decay& d = all.d[0];
+    if (all.count == 0 || d.batch == 0) return FMD_OK;
+    int64_t length = segment_length(d, path);
+    if (d.rows == 0) length = 1;  // nothing but the matrices to hand on
+    for (int i = 0; i < all.count; ++i) all.d[i].length = length;
+    const int64_t segments = decay_segments(d);
+    if (segments * d.heads * all.count > INT32_MAX || int64_t(d.batch) * d.heads > INT32_MAX) return FMD_ERR_UNSUPPORTED;
+    fmd_status st = FMD_OK;
+    if (length < kWhole) {
+        for (int i = 0; i < all.count; ++i) {
+            all.d[i].states = reinterpret_cast<float*>(workspace);
+            workspace += d.rows > 0 ? matrices(d, segments) : 0;
+        }
+        if (d.rows > 0 && (st = run_states(all, path, s)) != FMD_OK) return st;
+        carry_kernel<<<dim3(unsigned(d.batch) * d.heads, unsigned((d.dim * d.dim + 4 * kThreads - 1) / (4 * kThreads)),
+                            unsigned(all.count)),
+                       kThreads, 0, s>>>(all);
+        if ((st = check_launch()) != FMD_OK) return st;
+    } else {
+        Decays ends{};  // those whose last matrix is asked for
+        for (int i = 0; i < all.count; ++i)
+            if (all.d[i].after != nullptr) ends.d[ends.count++] = all.d[i];
+        if (ends.count > 0 && (st = run_states(ends, path, s)) != FMD_OK) return st;
+    }
+    Decays rows{};
+    for (int i = 0; i < all.count; ++i)
+        if (all.d[i].out != nullptr) rows.d[rows.count++] = all.d[i];
+    if (d.rows == 0 || rows.count == 0) return FMD_OK;
+    return path == kMma ? decay_rows_mma(rows, s) : path == kPlanes ? decay_rows_planes(rows, s) : decay_rows_simt(rows, s);
 }
 
 }  // namespace
@@ -181,11 +264,11 @@ using namespace fmd;
 
 extern "C" {
 
-fmd_status fmd_decay_attention_workspace_bytes(const fmd_decay* problem, int32_t after, size_t* bytes) {
+fmd_status fmd_decay_attention_workspace_bytes(const fmd_decay* problem, int32_t backward, size_t* bytes) {
     Decay d;
     if (problem == nullptr || bytes == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     const fmd_status st = check_rows(*problem, d);
-    if (st == FMD_OK) *bytes = mix_bytes(d, after != 0);
+    if (st == FMD_OK) *bytes = workspace_of(d, problem->type, backward ? 4 : 3, backward ? 3 : 1);
     return st;
 }
 
@@ -193,21 +276,26 @@ fmd_status fmd_decay_attention(const fmd_decay* problem, const float* state, voi
                                size_t workspace_bytes, int32_t* flags, void* stream) {
     Decay d;
     if (problem == nullptr) return FMD_ERR_INVALID_ARGUMENT;
-    const fmd_status st = check_rows(*problem, d);
+    fmd_status st = check_rows(*problem, d);
     if (st != FMD_OK) return st;
     const fmd_decay& p = *problem;
     if (p.rows > 0 && out == nullptr) return FMD_ERR_INVALID_ARGUMENT;
-    const size_t need = mix_bytes(d, after != nullptr);
+    const size_t need = workspace_of(d, p.type, 3, 1);
     if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return FMD_ERR_WORKSPACE;
     if (!aligned16(out) || !aligned16(state) || !aligned16(after) || !aligned16(workspace)) return FMD_ERR_UNSUPPORTED;
-    d.a = p.q, d.b = p.k, d.c = p.v, d.out = out;
-    d.a_row = p.q_row, d.a_head = p.q_head, d.b_row = p.k_row, d.b_head = p.k_head, d.c_row = p.v_row, d.c_head = p.v_head;
+    const cudaStream_t s = as_stream(stream);
+    const Path path = path_of(d, p.type);
+    char* at = static_cast<char*>(workspace);
+    Input in[3] = {{p.q, p.q_row, p.q_head}, {p.k, p.k_row, p.k_head}, {p.v, p.v_row, p.v_head}};
+    if ((st = make_planes(d, path, in, 3, at, s)) != FMD_OK) return st;
+    read_from(d, in[0], in[1], in[2]);
+    d.out = out;
     d.start = state;
     d.after = after;
     d.flags = flags;
     d.near = d.far = p.scale;
     d.add = 1.0f;
-    return mix(d, p.type == FMD_BF16, workspace, as_stream(stream));
+    return mix(Decays{{d}, 1}, path, at, s);
 }
 
 fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state, const void* g, int64_t g_row,
@@ -218,45 +306,53 @@ fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state,
     fmd_status st = check_rows(*problem, d);
     if (st != FMD_OK) return st;
     const fmd_decay& p = *problem;
-    const bool bf16 = p.type == FMD_BF16;
     if (p.rows > 0 && g == nullptr) return FMD_ERR_INVALID_ARGUMENT;
-    const size_t need = mix_bytes(d, dstate != nullptr);
+    const size_t need = workspace_of(d, p.type, 4, 3);
     if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return FMD_ERR_WORKSPACE;
     if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(state) || !aligned16(gafter) ||
-        !aligned16(dstate) || !aligned16(workspace) || (p.rows > 0 && !vector_rows(g, g_row, g_head, bf16 ? 2 : 4)))
+        !aligned16(dstate) || !aligned16(workspace) ||
+        (p.rows > 0 && !vector_rows(g, g_row, g_head, p.type == FMD_BF16 ? 2 : 4)))
         return FMD_ERR_UNSUPPORTED;
     const cudaStream_t s = as_stream(stream);
+    const Path path = path_of(d, p.type);
+    char* at = static_cast<char*>(workspace);
+    Input in[4] = {{p.q, p.q_row, p.q_head}, {p.k, p.k_row, p.k_head}, {p.v, p.v_row, p.v_head}, {g, g_row, g_head}};
+    if ((st = make_planes(d, path, in, 4, at, s)) != FMD_OK) return st;
+    const Input &q = in[0], &k = in[1], &v = in[2], &go = in[3];
     d.flags = flags;
     d.near = p.scale;
+    Decays all{};
+    if (dk != nullptr || dv != nullptr || dstate != nullptr) {  // from the last row to the first
+        Decay m = d;
+        m.later = 1;
+        m.add = p.scale;
+        m.far = 1.0f;
+        m.start = gafter;
+        if (dv != nullptr || dstate != nullptr) {
+            read_from(m, k, q, go);
+            m.out = dv;
+            m.after = dstate;
+            all.d[all.count++] = m;
+        }
+        if (dk != nullptr) {
+            read_from(m, v, go, q);
+            m.out = dk;
+            m.after = nullptr;
+            m.transposed = 1;
+            all.d[all.count++] = m;
+        }
+    }
     if (dq != nullptr) {
         Decay m = d;
-        m.a = g, m.b = p.v, m.c = p.k, m.out = dq;
-        m.a_row = g_row, m.a_head = g_head, m.b_row = p.v_row, m.b_head = p.v_head, m.c_row = p.k_row, m.c_head = p.k_head;
+        read_from(m, go, v, k);
+        m.out = dq;
         m.start = state;
         m.transposed = 1;
         m.add = 1.0f;
         m.far = p.scale;
-        if ((st = mix(m, bf16, workspace, s)) != FMD_OK) return st;
+        all.d[all.count++] = m;
     }
-    d.later = 1;
-    d.add = p.scale;
-    d.far = 1.0f;
-    d.start = gafter;
-    if (dk != nullptr) {
-        Decay m = d;
-        m.a = p.v, m.b = g, m.c = p.q, m.out = dk;
-        m.a_row = p.v_row, m.a_head = p.v_head, m.b_row = g_row, m.b_head = g_head, m.c_row = p.q_row, m.c_head = p.q_head;
-        m.transposed = 1;
-        if ((st = mix(m, bf16, workspace, s)) != FMD_OK) return st;
-    }
-    if (dv != nullptr || dstate != nullptr) {
-        Decay m = d;
-        m.a = p.k, m.b = p.q, m.c = g, m.out = dv;
-        m.a_row = p.k_row, m.a_head = p.k_head, m.b_row = p.q_row, m.b_head = p.q_head, m.c_row = g_row, m.c_head = g_head;
-        m.after = dstate;
-        if ((st = mix(m, bf16, workspace, s)) != FMD_OK) return st;
-    }
-    return FMD_OK;
+    return mix(all, path, at, s);
 }
 
 fmd_status fmd_decay_attention_step(const fmd_decay* problem, float* state, void* out, void* stream) {

@@ -25,7 +25,7 @@ namespace fmd {
 
 struct Decay {
     const void *a, *b, *c;       // [rows, heads, dim]
-    void* out;                   // [rows, heads, dim] contiguous
+    void* out;                   // [rows, heads, dim] contiguous, or null
     const float* log_decay;      // [heads]
     const int64_t* offsets;      // [batch + 1]
     const float* start;          // [batch, heads, dim, dim]: S_0, or null for zeros
@@ -34,11 +34,24 @@ struct Decay {
     int32_t* flags;
     int64_t rows;
     int64_t a_row, a_head, b_row, b_head, c_row, c_head;
-    int64_t length;              // rows of a segment
+    int64_t length;              // rows of a segment; kWhole: a segment is a sequence
     float near, add, far;
     int32_t batch, heads, dim, later;
     int32_t transposed;          // start and after: indexed [c][b] for [b][c]
 };
+
+// Up to three of them, of the same rows, that run side by side.
+struct Decays {
+    Decay d[3];
+    int32_t count;
+};
+
+constexpr int64_t kWhole = int64_t(1) << 40;  // a segment that holds any sequence
+
+// Places for segments (tiles of `length` rows): some may have nothing to do.
+__host__ __device__ inline int64_t decay_segments(const Decay& d) {
+    return d.length >= kWhole ? d.batch : d.rows / d.length + d.batch;
+}
 
 // The place of one block: rows [row0, row0 + rows) of a sequence that has `all`, its number among the segments.
 struct Stretch {
@@ -49,15 +62,40 @@ struct Stretch {
 // Segment `index` of the map that counts them by sequence (as tiles of `length` rows); rows == 0: nothing to do. All 32
 // lanes of a warp. Offsets that do not start at 0, fall or end elsewhere than at the last row raise FMD_FLAG_INDEX_RANGE.
 __device__ __forceinline__ Stretch stretch_of(const Decay& d, int64_t index) {
-    const int b = find_sequence(d.offsets, d.batch, d.length, index);
+    int b;
+    if (d.length >= kWhole && d.batch <= 32) {  // the longest first: the GPU waits for the block that ends last
+        const int lane = threadIdx.x & 31;
+        const int64_t mine = lane < d.batch ? d.offsets[lane + 1] - d.offsets[lane] : -1;
+        int rank = 0;
+        for (int i = 0; i < d.batch; ++i) {
+            const int64_t other = __shfl_sync(0xffffffffu, mine, i);
+            rank += other > mine || (other == mine && i < lane);
+        }
+        b = __ffs(__ballot_sync(0xffffffffu, lane < d.batch && rank == index)) - 1;
+    } else {
+        b = find_sequence(d.offsets, d.batch, d.length, index);
+    }
     const int64_t r0 = d.offsets[b], r1 = d.offsets[b + 1];
     const int64_t lo = min(max(r0, int64_t(0)), d.rows), hi = min(max(r1, lo), d.rows);
-    const int64_t from = (index - (r0 / d.length + b)) * d.length, n = hi - lo;
+    const int64_t from = d.length >= kWhole ? 0 : (index - (r0 / d.length + b)) * d.length, n = hi - lo;
     Stretch s{b, lo, 0, index};
     if (from < 0 || from >= n) return s;
     s.rows = min(d.length, n - from);
     s.row0 = d.later ? hi - from - s.rows : lo + from;
     return s;
+}
+
+// The matrix that a stretch starts from, or null for zeros.
+__device__ __forceinline__ const float* start_of(const Decay& d, const Stretch& s, int head) {
+    const int64_t size = int64_t(d.dim) * d.dim;
+    if (d.length < kWhole) return d.states + (s.index * d.heads + head) * size;
+    return d.start != nullptr ? d.start + (int64_t(s.b) * d.heads + head) * size : nullptr;
+}
+
+// Its value (row, col): whole sequences may have it transposed.
+__device__ __forceinline__ float start_at(const Decay& d, const float* start, int row, int col) {
+    if (start == nullptr || row >= d.dim || col >= d.dim) return 0.0f;
+    return start[d.length >= kWhole && d.transposed ? col * d.dim + row : row * d.dim + col];
 }
 
 // Looks at sequence b's offsets.
@@ -72,19 +110,14 @@ __device__ __forceinline__ float log2_decay(const Decay& d, int head) {
     return fmaxf(fminf(d.log_decay[head], 0.0f), -1.0e4f) * kLog2e;
 }
 
-constexpr int64_t kWhole = int64_t(1) << 40;  // a segment that holds any sequence
-
-// Places for segments (tiles of `length` rows): some may have nothing to do.
-__host__ __device__ inline int64_t decay_segments(const Decay& d) {
-    return d.length >= kWhole ? d.batch : d.rows / d.length + d.batch;
-}
-
-// What the segments add to the matrix, and the rows. carried: a segment starts from its place in `states`, else from
-// `start`. bfloat16:
-fmd_status decay_states_mma(const Decay& d, cudaStream_t s);
-fmd_status decay_rows_mma(const Decay& d, bool carried, cudaStream_t s);
-// float32
-fmd_status decay_states_simt(const Decay& d, cudaStream_t s);
-fmd_status decay_rows_simt(const Decay& d, bool carried, cudaStream_t s);
+// What the segments add to the matrix (whole sequences: the matrix behind them, in `after`), and the rows. bfloat16:
+fmd_status decay_states_mma(const Decays& d, cudaStream_t s);
+fmd_status decay_rows_mma(const Decays& d, cudaStream_t s);
+// float32, heads of up to 64 values: a, b and c are three planes of bfloat16, [3][rows][heads][dim]
+fmd_status decay_states_planes(const Decays& d, cudaStream_t s);
+fmd_status decay_rows_planes(const Decays& d, cudaStream_t s);
+// float32, wider heads
+fmd_status decay_states_simt(const Decays& d, cudaStream_t s);
+fmd_status decay_rows_simt(const Decays& d, cudaStream_t s);
 
 }  // namespace fmd

@@ -1,4 +1,4 @@
-// Decay attention in float32, on the FP32 cores.
+// Decay attention in float32 for heads of more than 64 values, on the FP32 cores.
 //
 // A block of 256 threads walks over the chunks of 64 rows of one segment and head; the chunk's rows of a, b and c and the
 // matrix lie in shared memory in FP32, padded to DP columns. A thread owns pieces of 4 x 4 pairs, of 4 rows x DP / 16
@@ -9,7 +9,7 @@
 namespace fmd {
 namespace {
 
-constexpr int kThreads = 256, kChunk = 64;
+constexpr int kThreads = 256, kChunk = 64, kDim = 128;
 
 template <int DP>
 struct Tiles {
@@ -75,17 +75,25 @@ __device__ __forceinline__ int64_t chunk_row(const Decay& d, const Stretch& s, i
     return d.later ? s.row0 + s.rows - done - count : s.row0 + done;
 }
 
-template <int DP>
-__global__ void __launch_bounds__(kThreads) states_kernel(const Decay d) {
+__global__ void __launch_bounds__(kThreads) states_kernel(const __grid_constant__ Decays all) {
+    constexpr int DP = kDim;
+    const Decay& d = all.d[blockIdx.x % unsigned(all.count)];
+    const int64_t place = blockIdx.x / unsigned(all.count);
     constexpr int kPer = DP / 16, kLd = Tiles<DP>::kLd;
     extern __shared__ float smem[];
     float *b = smem, *c = b + kChunk * kLd, *weight = c + kChunk * kLd;
-    const int head = blockIdx.x % d.heads;
-    const Stretch s = stretch_of(d, blockIdx.x / d.heads);
-    if (s.rows == 0) return;
+    const int head = int(place % d.heads);
+    const Stretch s = stretch_of(d, place / d.heads);
+    const bool whole = d.length >= kWhole;
+    if (s.rows == 0 && !whole) return;
     const float l2 = log2_decay(d, head);
     const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-    float state[kPer][kPer] = {};
+    const float* start = whole ? start_of(d, s, head) : nullptr;
+    float state[kPer][kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) state[i][e] = start_at(d, start, ty * kPer + i, tx * kPer + e);
     for (int64_t done = 0; done < s.rows; done += kChunk) {
         const int count = int(min(int64_t(kChunk), s.rows - done));
         const int64_t row = chunk_row(d, s, done, count);
@@ -104,38 +112,41 @@ __global__ void __launch_bounds__(kThreads) states_kernel(const Decay d) {
             for (int e = 0; e < kPer; ++e) state[i][e] *= keep;
         add_outer<DP>(b, c, weight, count, ty, tx, state);
     }
-    float* out = d.states + (s.index * d.heads + head) * d.dim * d.dim;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-#pragma unroll
-        for (int e = 0; e < kPer; ++e)
-            if (ty * kPer + i < d.dim && tx * kPer + e < d.dim) out[(ty * kPer + i) * d.dim + tx * kPer + e] = state[i][e];
-}
-
-template <int DP>
-__global__ void __launch_bounds__(kThreads) rows_kernel(const Decay d, bool carried) {
-    constexpr int kPer = DP / 16, kLd = Tiles<DP>::kLd, kPairs = kChunk + 4;
-    extern __shared__ float smem[];
-    float *a = smem, *b = a + kChunk * kLd, *c = b + kChunk * kLd, *matrix = c + kChunk * kLd, *pairs = matrix + DP * kLd,
-          *weight = pairs + kChunk * kPairs;
-    const int head = blockIdx.x % d.heads;
-    const int64_t index = blockIdx.x / d.heads;
-    if (head == 0 && threadIdx.x == 32 && index < d.batch) check_offsets(d, index);
-    const Stretch s = stretch_of(d, index);
-    if (s.rows == 0) return;
-    const float l2 = log2_decay(d, head);
-    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-    float state[kPer][kPer] = {};
-    const float* start = carried ? d.states + (index * d.heads + head) * d.dim * d.dim
-                         : d.start != nullptr ? d.start + (int64_t(s.b) * d.heads + head) * d.dim * d.dim : nullptr;
-    const bool turn = !carried && d.transposed;
+    float* out = (whole ? d.after + int64_t(s.b) * d.heads * d.dim * d.dim : d.states + s.index * d.heads * d.dim * d.dim) +
+                 int64_t(head) * d.dim * d.dim;
+    const bool turn = whole && d.transposed;
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
             const int r = ty * kPer + i, col = tx * kPer + e;
-            if (start != nullptr && r < d.dim && col < d.dim) state[i][e] = start[turn ? col * d.dim + r : r * d.dim + col];
-            matrix[r * kLd + col] = state[i][e];
+            if (r < d.dim && col < d.dim) out[turn ? col * d.dim + r : r * d.dim + col] = state[i][e];
+        }
+}
+
+__global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ Decays all) {
+    constexpr int DP = kDim;
+    const Decay& d = all.d[blockIdx.x % unsigned(all.count)];
+    const int64_t place = blockIdx.x / unsigned(all.count);
+    constexpr int kPer = DP / 16, kLd = Tiles<DP>::kLd, kPairs = kChunk + 4;
+    extern __shared__ float smem[];
+    float *a = smem, *b = a + kChunk * kLd, *c = b + kChunk * kLd, *matrix = c + kChunk * kLd, *pairs = matrix + DP * kLd,
+          *weight = pairs + kChunk * kPairs;
+    const int head = int(place % d.heads);
+    const int64_t index = place / d.heads;
+    if (head == 0 && threadIdx.x == 32 && index < d.batch) check_offsets(d, index);
+    const Stretch s = stretch_of(d, index);
+    if (s.rows == 0) return;
+    const float l2 = log2_decay(d, head);
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    const float* start = start_of(d, s, head);
+    float state[kPer][kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            state[i][e] = start_at(d, start, ty * kPer + i, tx * kPer + e);
+            matrix[(ty * kPer + i) * kLd + tx * kPer + e] = state[i][e];
         }
     for (int64_t done = 0; done < s.rows; done += kChunk) {
         const int count = int(min(int64_t(kChunk), s.rows - done));
@@ -224,27 +235,21 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Decay d, bool carr
     }
 }
 
-template <int DP>
-fmd_status launch(const Decay& d, bool states, bool carried, cudaStream_t s) {
-    const size_t bytes = states ? Tiles<DP>::kStates : Tiles<DP>::kRows;
-    const void* kernel = states ? (const void*)states_kernel<DP> : (const void*)rows_kernel<DP>;
+fmd_status launch(const Decays& d, bool states, cudaStream_t s) {
+    const size_t bytes = states ? Tiles<kDim>::kStates : Tiles<kDim>::kRows;
+    const void* kernel = states ? (const void*)states_kernel : (const void*)rows_kernel;
     const fmd_status st = grant_dynamic_smem(kernel, bytes, true);
     if (st != FMD_OK) return st;
-    const unsigned blocks = unsigned(decay_segments(d) * d.heads);
-    if (states) states_kernel<DP><<<blocks, kThreads, bytes, s>>>(d);
-    else rows_kernel<DP><<<blocks, kThreads, bytes, s>>>(d, carried);
+    const unsigned blocks = unsigned(decay_segments(d.d[0]) * d.d[0].heads * d.count);
+    if (states) states_kernel<<<blocks, kThreads, bytes, s>>>(d);
+    else rows_kernel<<<blocks, kThreads, bytes, s>>>(d);
     return check_launch();
-}
-
-fmd_status launch_for(const Decay& d, bool states, bool carried, cudaStream_t s) {
-    return d.dim <= 32 ? launch<32>(d, states, carried, s) : d.dim <= 64 ? launch<64>(d, states, carried, s)
-                                                                         : launch<128>(d, states, carried, s);
 }
 
 }  // namespace
 
-fmd_status decay_states_simt(const Decay& d, cudaStream_t s) { return launch_for(d, true, false, s); }
+fmd_status decay_states_simt(const Decays& d, cudaStream_t s) { return launch(d, true, s); }
 
-fmd_status decay_rows_simt(const Decay& d, bool carried, cudaStream_t s) { return launch_for(d, false, carried, s); }
+fmd_status decay_rows_simt(const Decays& d, cudaStream_t s) { return launch(d, false, s); }
 
 }  // namespace fmd

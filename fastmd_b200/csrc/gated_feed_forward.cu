@@ -37,7 +37,6 @@ constexpr int kM = 128, kK = 64;
 constexpr uint32_t kTileA = kM * kK * 2, kPanel = 64 * kK * 2;  // bytes of an operand's tile, of 64 columns of it
 constexpr int kMostSlots = 12;
 constexpr int kSegment = 2;
-constexpr float kBf16Max = 3.38953139e38f;
 
 enum Kind { kUp, kDown, kHidden, kInput, kWeights };
 
@@ -213,29 +212,6 @@ __device__ __forceinline__ void turn_rows(unsigned char* scratch, const float4 (
         const float4 y = *reinterpret_cast<const float4*>(piece_at<8>(scratch, lane, i));
         v[4 * i] = y.x, v[4 * i + 1] = y.y, v[4 * i + 2] = y.z, v[4 * i + 3] = y.w;
     }
-}
-
-__device__ __forceinline__ uint4 pack8(const float* v) {
-    return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-}
-
-// Eight values' first plane; `v` becomes what is left of them. Held to the largest bfloat16: finite values stay finite.
-__device__ __forceinline__ uint4 first_plane8(float* v) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        w[i] = pack_bf16(fminf(fmaxf(v[2 * i], -kBf16Max), kBf16Max), fminf(fmaxf(v[2 * i + 1], -kBf16Max), kBf16Max));
-        const float2 part = unpack_bf16(w[i]);
-        v[2 * i] -= part.x;
-        v[2 * i + 1] -= part.y;
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-__device__ __forceinline__ uint4 next_plane8(float* v) {
-    uint32_t w[4];
-    next_plane<4>(v, w);
-    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // N values a row as P planes, `plane` values apart; rows are padded to multiples of 8 columns. The values are used up.

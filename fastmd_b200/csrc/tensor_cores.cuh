@@ -134,6 +134,15 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
         : "memory");
 }
 
+// 8 columns, in the same way
+__device__ __forceinline__ void tmem_load8(uint32_t addr, float (&v)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+        : "r"(addr)
+        : "memory");
+}
+
 // 16 columns: 32 bfloat16 of this thread's lane
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
     asm volatile(
@@ -142,6 +151,13 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[
         "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
         "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
         : "memory");
+}
+
+// 8 columns: 16 bfloat16 of this thread's lane
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(addr)
+                 : "memory");
 }
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -172,6 +188,31 @@ __device__ __forceinline__ void next_plane(float* y, uint32_t (&w)[N]) {
         y[2 * i] = left.x;
         y[2 * i + 1] = left.y;
     }
+}
+
+constexpr float kMostBf16 = 3.38953139e38f;  // the largest finite one
+
+__device__ __forceinline__ uint4 pack8(const float* v) {
+    return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
+// Eight values' first plane; `v` becomes what is left of them. Held to the largest bfloat16: finite values stay finite.
+__device__ __forceinline__ uint4 first_plane8(float* v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = pack_bf16(fminf(fmaxf(v[2 * i], -kMostBf16), kMostBf16), fminf(fmaxf(v[2 * i + 1], -kMostBf16), kMostBf16));
+        const float2 part = unpack_bf16(w[i]);
+        v[2 * i] -= part.x;
+        v[2 * i + 1] -= part.y;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ uint4 next_plane8(float* v) {
+    uint32_t w[4];
+    next_plane<4>(v, w);
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Zeros rows [first, last) of `panels` panels that lie `stride` bytes apart (the swizzle keeps a row's 128 bytes in

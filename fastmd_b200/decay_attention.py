@@ -24,9 +24,9 @@ def _problem(q, k, v, log_decay, offsets, scale) -> FmdDecay:
                     offsets.shape[0] - 1 if offsets is not None else 0, q.shape[1], q.shape[2])
 
 
-def _workspace(problem: FmdDecay, after: bool, device) -> tuple[Tensor | None, int]:
+def _workspace(problem: FmdDecay, backward: bool, device) -> tuple[Tensor | None, int]:
     nbytes = c_size_t()
-    call("fmd_decay_attention_workspace_bytes", problem, after, nbytes)
+    call("fmd_decay_attention_workspace_bytes", problem, backward, nbytes)
     size = nbytes.value
     return (torch.empty(size, device=device, dtype=torch.uint8) if size else None), size
 
@@ -39,7 +39,7 @@ def _forward(q, k, v, log_decay, offsets, state, scale, keep):
     device = q.device
     out, after = _like(q), _states(q, offsets) if keep else None
     problem = _problem(q, k, v, log_decay, offsets, scale)
-    workspace, size = _workspace(problem, keep, device)
+    workspace, size = _workspace(problem, False, device)
     call("fmd_decay_attention", problem, ptr(state), out.data_ptr(), ptr(after), ptr(workspace), size,
          _lib.flags_word(device).data_ptr(), stream(device))
     return out, after
@@ -66,7 +66,7 @@ class _DecayAttention(Function):
         dq, dk, dv = (_like(t) if n else None for t, n in zip((q, k, v), need))
         dstate = torch.empty_like(state) if need[5] else None
         problem = _problem(q, k, v, log_decay, offsets, ctx.scale)
-        workspace, size = _workspace(problem, need[5], q.device)
+        workspace, size = _workspace(problem, True, q.device)
         call("fmd_decay_attention_bwd", problem, ptr(state), g.data_ptr(), g.stride(0), g.stride(1), ptr(gafter), ptr(dq),
              ptr(dk), ptr(dv), ptr(dstate), ptr(workspace), size, _lib.flags_word(q.device).data_ptr(), stream(q.device))
         dq, dk, dv, dstate = first_order("decay_attention", (dq, dk, dv, dstate), inputs)

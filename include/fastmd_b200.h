@@ -1186,10 +1186,9 @@ typedef struct fmd_decay {
     int32_t type, batch, heads, dim, _pad;
 } fmd_decay;
 
-/* Workspace of the forward pass, or of the backward pass, where the matrix
- * behind the last row (the gradient of the first state) is asked for
- * (after = 1) or not; 0 for none. It starts at a multiple of 16 bytes. */
-FMD_API fmd_status fmd_decay_attention_workspace_bytes(const fmd_decay* problem, int32_t after, size_t* bytes);
+/* Workspace of the forward pass (backward = 0) or of the backward pass (1),
+ * from the sizes alone; 0 for none. It starts at a multiple of 16 bytes. */
+FMD_API fmd_status fmd_decay_attention_workspace_bytes(const fmd_decay* problem, int32_t backward, size_t* bytes);
 
 /* out [rows, heads, dim] and `after`, the states behind the last rows (NULL:
  * not written), from the states before the first ones (NULL: zeros). No
