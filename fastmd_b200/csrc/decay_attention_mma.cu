@@ -17,8 +17,13 @@
 // Warps, after the workers (8 or 16 of them: thread = row of the chunk and a part of the pairs or columns; for the matrix
 // its row, and a part of its columns):
 //   TMA: a, b, c of one chunk after the other through a ring of slots
-//   one thread issues the products: s, f | (b' ready) b'^T c | (p ready) p c | s of the next chunk, (S ready) f
-// What lies in TMEM: s and p in its place (each thread overwrites what it has read), n, and f with b'^T c in its place.
+//   one thread issues the products, each as soon as what it needs is there: f (S of this chunk), b'^T c (b'), s of the next
+//   chunk, n (p). What goes from chunk to chunk is S alone: while f runs the workers weigh the pairs.
+// What lies in TMEM: s and p in its place (each thread overwrites what it has read; where there is room two by turns), f,
+// and b'^T c and n one after the other.
+//
+// Three of four blocks of 32 x 32 pairs lie to one side of the diagonal: nothing is computed above it, and below it a weight
+// is the product of one factor of the row and one of the column (a table), l^{t-u} = l^{t-a} l^{a-u}, neither above 1.
 //
 // Rows of a tile that lie behind a chunk's end belong to others: their pairs are zeros, b' is zero there, and c is set to
 // zero, whatever their values. A head of up to 64 values is one panel; b' is read as two, the second from what follows in
@@ -56,8 +61,9 @@ struct RowsShape : Shape<KS, P> {
     static constexpr uint32_t kMatrix = kPlanes * kPlane > kPanelBytes ? kPlanes * kPlane : kPanelBytes;
     static constexpr size_t kBytes = kSlots * S::kSlotBytes + kMatrix + 1024;
     static constexpr uint32_t kTmem = kBlocks == 2 ? 256 : 512;
-    static constexpr uint32_t kThird = 128;                  // columns: the pairs at 0, their third plane, n, f
-    static constexpr uint32_t kNear = P == 3 ? 192 : 128, kFar = kNear + S::kDim;
+    static constexpr int kBuffers = kBlocks == 2 ? 1 : 2;    // of the pairs
+    // columns: the pairs at 0, their third plane, n (before it b'^T c), f
+    static constexpr uint32_t kThird = 128 * kBuffers, kNear = kThird + (P == 3 ? 64 : 0), kFar = kNear + S::kDim;
 };
 
 // PLANES: of b'.
@@ -75,7 +81,7 @@ struct StatesShape : Shape<KS, P> {
 template <int SLOTS>
 struct Ctrl {
     Ring<SLOTS> ring;
-    uint64_t pairs, ready, weights, added, out, matrix;
+    uint64_t pairs, far, ready, weights, added, out, matrix;
     uint64_t drain;
     uint32_t tmem;
     int32_t abort;
@@ -123,43 +129,45 @@ __device__ __forceinline__ void tmem_read(uint32_t at, float (&v)[N]) {
     if constexpr (N % 16 != 0) tmem_load8(at + N / 16 * 16, reinterpret_cast<float(&)[8]>(v[N / 16 * 16]));
 }
 
-__device__ __forceinline__ void add8(float (&v)[8], const uint4& x) {
-    const float2 y[4] = {unpack_bf16(x.x), unpack_bf16(x.y), unpack_bf16(x.z), unpack_bf16(x.w)};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[2 * e] += y[e].x;
-        v[2 * e + 1] += y[e].y;
-    }
-}
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
 
 // Row r of a tile of P planes times `weight` as OUT planes: the first P in place, the others from `more` on. A group takes
-// every GROUPS-th eight of the row, in an order that keeps the banks apart; the swizzle moves eights within a panel's row.
+// eights that lie side by side, in an order that keeps the banks apart; the swizzle moves eights within a panel's row.
 template <int KS, int P, int OUT, int GROUPS>
 __device__ __forceinline__ void weigh_row(unsigned char* tile, unsigned char* more, int r, int group, float weight, bool real) {
     using S = Shape<KS, P>;
-    constexpr int kEach = 8 * S::kPanels / GROUPS;  // eights of this group, side by side in a panel
+    constexpr int kEach = 8 * S::kPanels / GROUPS;
+    const float2 w2 = twice(weight);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         const int eight = group * kEach + i;
         const uint32_t at = uint32_t(eight / 8) * kPanelBytes + uint32_t(r) * 128 + uint32_t(((eight % 8) ^ (r & 7)) * 16);
-        float v[8] = {};
-        if (real) {  // exact: the planes are the parts of one FP32 number, the small ones first
+        float2 v[4];
+        uint4 x = *reinterpret_cast<const uint4*>(tile + (P - 1) * S::kTileBytes + at);
+        v[0] = unpack_bf16(x.x), v[1] = unpack_bf16(x.y), v[2] = unpack_bf16(x.z), v[3] = unpack_bf16(x.w);
 #pragma unroll
-            for (int q = P - 1; q >= 0; --q) add8(v, *reinterpret_cast<const uint4*>(tile + q * S::kTileBytes + at));
+        for (int q = P - 2; q >= 0; --q) {  // exact: the planes are the parts of one FP32 number, the small ones first
+            x = *reinterpret_cast<const uint4*>(tile + q * S::kTileBytes + at);
+            v[0] = add2(v[0], unpack_bf16(x.x)), v[1] = add2(v[1], unpack_bf16(x.y));
+            v[2] = add2(v[2], unpack_bf16(x.z)), v[3] = add2(v[3], unpack_bf16(x.w));
+        }
+        float y[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= weight;
+        for (int e = 0; e < 4; ++e) {
+            v[e] = mul2(v[e], w2);
+            y[2 * e] = v[e].x;
+            y[2 * e + 1] = v[e].y;
+        }
+        if (!real) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = 0.0f;
         }
 #pragma unroll
         for (int q = 0; q < OUT; ++q) {
-            const uint4 w = q + 1 == OUT ? pack8(v) : q == 0 ? first_plane8(v) : next_plane8(v);
+            const uint4 w = q + 1 == OUT ? pack8(y) : q == 0 && P == 3 ? first_plane8(y) : next_plane8(y);
             *reinterpret_cast<uint4*>((q < P ? tile + q * S::kTileBytes : more + (q - P) * S::kTileBytes) + at) = w;
         }
     }
-}
-
-// The decay of row j of a chunk of `count` as it enters the matrix.
-__device__ __forceinline__ float weight_of(const Decay& d, int j, int count, float l2) {
-    return d.add * ex2(float(d.later ? j + 1 : count - 1 - j) * l2);
 }
 
 // The thread's row of the matrix, columns from col0 on: as planes in shared memory.
@@ -176,7 +184,7 @@ __device__ __forceinline__ void store_matrix(unsigned char* to, int r, int col0,
 #pragma unroll
         for (int q = 0; q < S::kPlanes; ++q)
             *reinterpret_cast<uint4*>(p + q * S::kPlane) =
-                q + 1 == S::kPlanes ? pack8(v) : q == 0 ? first_plane8(v) : next_plane8(v);
+                q + 1 == S::kPlanes ? pack8(v) : q == 0 && P == 3 ? first_plane8(v) : next_plane8(v);
     }
 }
 
@@ -185,8 +193,13 @@ template <int N>
 __device__ __forceinline__ void add_columns(uint32_t at, float keep, float (&state)[N]) {
     float x[N];
     tmem_read(at, x);
+    const float2 k = twice(keep);
 #pragma unroll
-    for (int e = 0; e < N; ++e) state[e] = fmaf(keep, state[e], x[e]);
+    for (int e = 0; e < N; e += 2) {
+        const float2 y = fma2(k, make_float2(state[e], state[e + 1]), make_float2(x[e], x[e + 1]));
+        state[e] = y.x;
+        state[e + 1] = y.y;
+    }
 }
 
 template <int SLOTS>
@@ -194,6 +207,7 @@ __device__ __forceinline__ void open_block(Ctrl<SLOTS>& ctl, int workers) {
     if (threadIdx.x == 0) {
         init_ring(ctl.ring);
         mbar_init(&ctl.pairs, 1);
+        mbar_init(&ctl.far, 1);
         mbar_init(&ctl.ready, uint32_t(workers));
         mbar_init(&ctl.weights, uint32_t(workers));
         mbar_init(&ctl.added, 1);
@@ -275,14 +289,11 @@ __device__ __forceinline__ void load_start(const Decay& d, const Stretch& s, int
 
 // Chunk i of a stretch: its rows, and the first of them.
 struct Walk {
-    int64_t row0, rows;
-    int chunks, later;
+    int row0, rows, chunks, later;
     __device__ __forceinline__ Walk(const Stretch& s, const Decay& d)
-        : row0(s.row0), rows(s.rows), chunks(int((s.rows + kTile - 1) / kTile)), later(d.later) {}
-    __device__ __forceinline__ int count(int i) const { return int(min(int64_t(kTile), rows - int64_t(i) * kTile)); }
-    __device__ __forceinline__ int64_t first(int i) const {
-        return later ? row0 + rows - int64_t(i) * kTile - count(i) : row0 + int64_t(i) * kTile;
-    }
+        : row0(int(s.row0)), rows(int(s.rows)), chunks((rows + kTile - 1) / kTile), later(d.later) {}
+    __device__ __forceinline__ int count(int i) const { return min(kTile, rows - i * kTile); }
+    __device__ __forceinline__ int first(int i) const { return later ? row0 + max(0, rows - (i + 1) * kTile) : row0 + i * kTile; }
 };
 
 template <int KS, int P>
@@ -294,6 +305,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     unsigned char* matrix = ring + S::kSlots * S::kSlotBytes;
     __shared__ Ctrl<S::kSlots> ctl;
+    __shared__ alignas(16) float table[32];  // l^{31 - e}, going backwards l^e: of column e of a block of 32 pairs
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned which = blockIdx.x % unsigned(all.count), place = blockIdx.x / unsigned(all.count);
@@ -302,6 +314,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
     const int head = int(place % unsigned(d.heads));
     const int64_t index = place / unsigned(d.heads);
 
+    if (threadIdx.x < 32) table[lane] = exp2f(float(d.later ? lane : 31 - lane) * log2_decay(d, head));
     if (head == 0 && threadIdx.x == 32 && index < d.batch) check_offsets(d, index);
     const Stretch s = block_stretch(d, index);
     if (s.rows == 0) return;
@@ -327,19 +340,22 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                        add_desc = out_desc | 1u << 15;
         auto slot = [&](int i) { return first_slot + uint32_t(i % S::kSlots) * S::kSlotBytes; };
         bool ok = true, issued = false;
-        auto pairs = [&](int i) {  // over the pairs of the chunk before, whose product has been issued
+        auto at_pairs = [&](int i) { return base + uint32_t(i % S::kBuffers) * 128u; };
+        auto pairs = [&](int i) {  // over pairs whose product has been issued
             ok = ok && landed(ctl.ring, 3 * i, abort) && landed(ctl.ring, 3 * i + 1, abort);
             if (!ok) return;
             tc_fence_after();
-            const uint32_t a = slot(3 * i), b = slot(3 * i + 1);
+            const uint32_t a = slot(3 * i), b = slot(3 * i + 1), to = at_pairs(i);
             if (elect_one()) {
                 if (P == 1) {
-                    product_rows<KS>(base, a, b, pairs_desc);
+                    product_rows<KS>(to, a, b, pairs_desc);
                 } else {
 #pragma unroll
                     for (int q = 0; q < 6; ++q)
-                        product_rows<KS>(base, a + first_plane(q) * S::kTileBytes, b + second_plane(q) * S::kTileBytes, pairs_desc, q > 0);
+                        product_rows<KS>(to, a + first_plane(q) * S::kTileBytes, b + second_plane(q) * S::kTileBytes, pairs_desc,
+                                         q > 0);
                 }
+                tc_commit(&ctl.pairs);
             }
             issued = true;
         };
@@ -348,18 +364,18 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
             ok = warp_wait(&ctl.matrix, uint32_t(i) & 1u, abort);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t a = slot(3 * i), b = slot(3 * i + 1), c = slot(3 * i + 2);
+            const uint32_t a = slot(3 * i), b = slot(3 * i + 1), c = slot(3 * i + 2), far = base + S::kFar, near = base + S::kNear;
             if (elect_one()) {
                 if (P == 1) {
-                    product_matrix<KS>(base + S::kFar, a, planes + S::kPlane, S::kPanel, out_desc, false);
-                    product_matrix<KS>(base + S::kFar, a, planes, S::kPanel, out_desc, true);
+                    product_matrix<KS>(far, a, planes + S::kPlane, S::kPanel, out_desc, false);
+                    product_matrix<KS>(far, a, planes, S::kPanel, out_desc, true);
                 } else {
 #pragma unroll
                     for (int q = 0; q < 6; ++q)
-                        product_matrix<KS>(base + S::kFar, a + first_plane(q) * S::kTileBytes, planes + second_plane(q) * S::kPlane,
+                        product_matrix<KS>(far, a + first_plane(q) * S::kTileBytes, planes + second_plane(q) * S::kPlane,
                                            S::kPanel, out_desc, q > 0);
                 }
-                tc_commit(&ctl.pairs);
+                tc_commit(&ctl.far);
                 tc_commit(&ctl.ring.empty[(3 * i) % S::kSlots]);
             }
             ok = landed(ctl.ring, 3 * i + 2, abort) && warp_wait(&ctl.ready, uint32_t(i) & 1u, abort);
@@ -369,18 +385,24 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
             if (elect_one()) {
 #pragma unroll
                 for (int q = P == 1 ? 5 : 0; q < 6; ++q)
-                    product_columns(base + S::kFar, b + first_plane(q) * S::kTileBytes, c + second_plane(q) * S::kTileBytes, steps,
-                                    add_desc, P != 1 && q > 0);
+                    product_columns(near, b + first_plane(q) * S::kTileBytes, c + second_plane(q) * S::kTileBytes, steps, add_desc,
+                                    P != 1 && q > 0);
                 tc_commit(&ctl.added);
                 tc_commit(&ctl.ring.empty[(3 * i + 1) % S::kSlots]);
             }
-            ok = warp_wait(&ctl.weights, uint32_t(i) & 1u, abort);
+            // the next pairs before what the workers still prepare, if their tiles have landed
+            bool early = S::kBuffers == 2 && i + 1 < count;
+            for (int e = 3; e < 5 && early; ++e)
+                early = __all_sync(0xffffffffu, mbar_try_wait(su32(&ctl.ring.full[(3 * i + e) % S::kSlots]),
+                                                              uint32_t((3 * i + e) / S::kSlots) & 1u));
+            if (early) pairs(i + 1);
+            ok = ok && warp_wait(&ctl.weights, uint32_t(i) & 1u, abort);
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
-                const uint32_t near = base + S::kNear;
+                const uint32_t p = at_pairs(i);
                 if (P == 1) {
-                    product_weights<8, S::kPairs / 16, S::kPairs>(near, base, c, steps, out_desc, false);
+                    product_weights<8, S::kPairs / 16, S::kPairs>(near, p, c, steps, out_desc, false);
                 } else {
 #pragma unroll
                     for (int q = 0; q < 6; ++q) {
@@ -388,13 +410,13 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                         if (first_plane(q) == 2)
                             product_weights<8, 8, 0>(near, base + S::kThird, from, steps, out_desc, q > 0);
                         else
-                            product_weights<8, 2, 32>(near, base + 16 * first_plane(q), from, steps, out_desc, q > 0);
+                            product_weights<8, 2, 32>(near, p + 16 * first_plane(q), from, steps, out_desc, q > 0);
                     }
                 }
                 tc_commit(&ctl.out);
                 tc_commit(&ctl.ring.empty[(3 * i + 2) % S::kSlots]);
             }
-            if (i + 1 < count) pairs(i + 1);
+            if (!early && i + 1 < count) pairs(i + 1);
         }
         if (!ok && issued) {  // the products in flight end before TMEM is freed
             if (elect_one()) tc_commit(&ctl.drain);
@@ -404,77 +426,98 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
         using T = typename std::conditional<P == 1, __nv_bfloat16, float>::type;
         const int group = warp >> 2, r = threadIdx.x & 127, col0 = group * kColumns, pair0 = group * S::kPairs;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t at_pairs = tmem + lanes + pair0, at_third = tmem + lanes + S::kThird + pair0 / 2,
-                       at_near = tmem + lanes + S::kNear + col0, at_far = tmem + lanes + S::kFar + col0;
+        const uint32_t at_third = tmem + lanes + S::kThird + pair0 / 2, at_near = tmem + lanes + S::kNear + col0,
+                       at_far = tmem + lanes + S::kFar + col0;
         const float l2 = log2_decay(d, head), way = d.later ? -1.0f : 1.0f;
+        auto power = [&](int n) { return P == 1 ? ex2(float(n) * l2) : exp2f(float(n) * l2); };
         const bool holds = r < S::kDim;
         float state[kColumns];
         load_start(d, s, head, r, col0, state);
         if (holds) store_matrix<KS, P>(matrix, r, col0, state);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         warp_arrive(&ctl.matrix);
+        // the weights of 32 pairs from column `first` on
+        auto weigh_pairs = [&](int first, int count, float(&x)[32]) {
+            const int beside = (first / 32 - (warp & 3)) * (d.later ? -1 : 1);  // blocks above the diagonal
+            if (beside < 0 && first + 32 <= count) {
+                const float2 row = twice(d.near * power(d.later ? first - r : r - first - 31));
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(table + e);
+                    const float2 u = mul2(make_float2(x[e], x[e + 1]), mul2(row, make_float2(y.x, y.y)));
+                    const float2 v = mul2(make_float2(x[e + 2], x[e + 3]), mul2(row, make_float2(y.z, y.w)));
+                    x[e] = u.x, x[e + 1] = u.y, x[e + 2] = v.x, x[e + 3] = v.y;
+                }
+            } else {
+                const float t = way * float(r - first);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const float gap = fmaf(float(e), -way, t);
+                    const float w = (P == 1 ? ex2(gap * l2) : exp2f(gap * l2)) * d.near;
+                    x[e] = gap >= 0.0f && e < count - first ? x[e] * w : 0.0f;
+                }
+            }
+        };
+        auto above = [&](int first) { return d.later ? first / 32 < (warp & 3) : first / 32 > (warp & 3); };
+        // of a whole chunk; the last one has its own
+        float enters = d.add * power(d.later ? r + 1 : kTile - 1 - r), keep = power(kTile),
+              reach = d.far * power(d.later ? kTile - 1 - r : r + 1);
         for (int i = 0; i < walk.chunks; ++i) {
             const int count = walk.count(i);
-            const uint32_t parity = uint32_t(i) & 1u;
+            if (count < kTile) {
+                enters = d.add * power(d.later ? r + 1 : count - 1 - r);
+                keep = power(count);
+                reach = d.far * power(d.later ? count - 1 - r : r + 1);
+            }
+            const uint32_t parity = uint32_t(i) & 1u, at_pairs = tmem + lanes + uint32_t(i % S::kBuffers) * 128u + pair0;
             if (!worker_wait(&ctl.pairs, parity, abort)) break;
-            tc_fence_after();
-            float far[kColumns];
-            tmem_read(at_far, far);
             const int tile_b = 3 * i + 1, tile_c = 3 * i + 2;
             if (!worker_wait(&ctl.ring.full[tile_b % S::kSlots], uint32_t(tile_b / S::kSlots) & 1u, abort)) break;
-            weigh_row<KS, P, P, S::kGroups>(ring + (tile_b % S::kSlots) * S::kSlotBytes, nullptr, r, group,
-                                            weight_of(d, r, count, l2), r < count);
+            tc_fence_after();
+            weigh_row<KS, P, P, S::kGroups>(ring + (tile_b % S::kSlots) * S::kSlotBytes, nullptr, r, group, enters, r < count);
             if (count < kTile) {
                 if (!worker_wait(&ctl.ring.full[tile_c % S::kSlots], uint32_t(tile_c / S::kSlots) & 1u, abort)) break;
                 zero_rows(ring + (tile_c % S::kSlots) * S::kSlotBytes, P * S::kPanels, kPanelBytes, count, (count + 15) & ~15,
                           threadIdx.x, S::kWorkers);
             }
-            tc_fence_before();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(&ctl.ready);
 
-            const float t = way * float(r - pair0);
-            auto weigh = [&](int first, auto& x) {
 #pragma unroll
-                for (int e = 0; e < int(sizeof(x) / sizeof(x[0])); ++e) {
-                    const float gap = fmaf(float(first + e), -way, t);
-                    const float w = (P == 1 ? ex2(gap * l2) : exp2f(gap * l2)) * d.near;
-                    x[e] = gap >= 0.0f && first + e < count - pair0 ? x[e] * w : 0.0f;
-                }
-            };
-            if constexpr (P == 1) {
-#pragma unroll
-                for (int ch = 0; ch < S::kPairs; ch += 16) {
-                    float x[16];
-                    uint32_t p[8];
-                    tmem_load16(at_pairs + ch, x);
-                    weigh(ch, x);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
-                    tmem_store8(at_pairs + ch / 2, p);
-                }
-            } else {
-                float x[32];
+            for (int ch = 0; ch < S::kPairs; ch += 32) {
                 uint32_t p[16];
-                tmem_load32(at_pairs, x);
-                weigh(0, x);
+                const uint32_t at = at_pairs + (P == 1 ? ch / 2 : 0);
+                if (above(pair0 + ch)) {
 #pragma unroll
-                for (int q = 0; q < 3; ++q) {
+                    for (int e = 0; e < 16; ++e) p[e] = 0;
+#pragma unroll
+                    for (int q = 0; q < P; ++q) tmem_store16(q == 2 ? at_third : at + 16 * q, p);
+                    continue;
+                }
+                float x[32];
+                tmem_load32(at_pairs + ch, x);
+                weigh_pairs(pair0 + ch, count, x);
+#pragma unroll
+                for (int q = 0; q < P; ++q) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
-                        const uint4 w = q == 0 ? first_plane8(x + e) : next_plane8(x + e);
+                        const uint4 w = P == 1 ? pack8(x + e) : q == 0 ? first_plane8(x + e) : next_plane8(x + e);
                         p[e / 2] = w.x, p[e / 2 + 1] = w.y, p[e / 2 + 2] = w.z, p[e / 2 + 3] = w.w;
                     }
-                    tmem_store16(q == 2 ? at_third : at_pairs + 16 * q, p);
+                    tmem_store16(q == 2 ? at_third : at + 16 * q, p);
                 }
             }
+            if (!worker_wait(&ctl.added, parity, abort)) break;
+            tc_fence_after();
+            add_columns(at_near, keep, state);
             tmem_wait_st();
             tc_fence_before();
             warp_arrive(&ctl.weights);
 
-            if (!worker_wait(&ctl.added, parity, abort)) break;
+            if (!worker_wait(&ctl.far, parity, abort)) break;
             tc_fence_after();
-            add_columns(at_far, P == 1 ? ex2(float(count) * l2) : exp2f(float(count) * l2), state);
+            float far[kColumns];
+            tmem_read(at_far, far);
             if (i + 1 < walk.chunks) {
                 if (holds) store_matrix<KS, P>(matrix, r, col0, state);
                 tc_fence_before();
@@ -484,24 +527,27 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
 
             if (!worker_wait(&ctl.out, parity, abort)) break;
             tc_fence_after();
-            float near[kColumns];
-            tmem_read(at_near, near);
-            if (r < count) {
-                const float reach = d.far * exp2f(float(d.later ? count - 1 - r : r + 1) * l2);
-                T* out = static_cast<T*>(d.out) + ((walk.first(i) + r) * d.heads + head) * d.dim + col0;
+            T* out = static_cast<T*>(d.out) + (int64_t(walk.first(i) + r) * d.heads + head) * d.dim + col0;
+            const float2 reach2 = twice(reach);
 #pragma unroll
-                for (int e = 0; e < kColumns; ++e) near[e] = fmaf(reach, far[e], near[e]);
+            for (int e = 0; e < kColumns; e += 8) {
+                float near[8];
+                tmem_load8(at_near + e, near);
 #pragma unroll
-                for (int e = 0; e < kColumns; e += 8) {
-                    if (col0 + e >= d.dim) break;
-                    if constexpr (P == 1) {
-                        *reinterpret_cast<uint4*>(out + e) = pack8(near + e);
-                    } else {
-                        st4(out + e, make_float4(near[e], near[e + 1], near[e + 2], near[e + 3]));
-                        st4(out + e + 4, make_float4(near[e + 4], near[e + 5], near[e + 6], near[e + 7]));
-                    }
+                for (int o = 0; o < 8; o += 2) {
+                    const float2 y = fma2(reach2, make_float2(far[e + o], far[e + o + 1]), make_float2(near[o], near[o + 1]));
+                    near[o] = y.x;
+                    near[o + 1] = y.y;
+                }
+                if (r >= count || col0 + e >= d.dim) continue;
+                if constexpr (P == 1) {
+                    *reinterpret_cast<uint4*>(out + e) = pack8(near);
+                } else {
+                    st4(out + e, make_float4(near[0], near[1], near[2], near[3]));
+                    st4(out + e + 4, make_float4(near[4], near[5], near[6], near[7]));
                 }
             }
+            tc_fence_before();
         }
     }
 
