@@ -17,6 +17,7 @@
 // Warps, after the workers (8 or 16 of them: thread = row of the chunk and a part of the pairs or columns; for the matrix
 // its row, and a part of its columns):
 //   TMA: a, b, c of one chunk after the other through a ring of slots
+//   one thread hands c's slot back, through which the output has left (rows side by side)
 //   one thread issues the products, each as soon as what it needs is there: f (S of this chunk), b'^T c (b'), s of the next
 //   chunk, n (p). What goes from chunk to chunk is S alone: while f runs the workers weigh the pairs.
 // What lies in TMEM: s and p in its place (each thread overwrites what it has read; where there is room two by turns), f,
@@ -52,7 +53,7 @@ struct RowsShape : Shape<KS, P> {
     using S = Shape<KS, P>;
     // Two blocks an SM where they fit, of eight workers each; else sixteen in one block, which hide each other's waits.
     static constexpr int kBlocks = P == 1 && KS <= 4 ? 2 : 1;
-    static constexpr int kGroups = kBlocks == 2 ? 2 : 4, kWorkers = 128 * kGroups, kThreads = kWorkers + 64;
+    static constexpr int kGroups = kBlocks == 2 ? 2 : 4, kWorkers = 128 * kGroups, kThreads = kWorkers + 96;
     static constexpr int kColumns = S::kDim / kGroups, kPairs = kTile / kGroups;  // of a thread
     static constexpr int kSlots = P == 3 ? 4 : 5;
     static constexpr int kPlanes = P == 3 ? 3 : 2;           // of the matrix
@@ -81,7 +82,7 @@ struct StatesShape : Shape<KS, P> {
 template <int SLOTS>
 struct Ctrl {
     Ring<SLOTS> ring;
-    uint64_t pairs, far, ready, weights, added, out, matrix;
+    uint64_t pairs, far, ready, weights, added, out, matrix, stored;
     uint64_t drain;
     uint32_t tmem;
     int32_t abort;
@@ -137,19 +138,27 @@ template <int KS, int P, int OUT, int GROUPS>
 __device__ __forceinline__ void weigh_row(unsigned char* tile, unsigned char* more, int r, int group, float weight, bool real) {
     using S = Shape<KS, P>;
     constexpr int kEach = 8 * S::kPanels / GROUPS;
-    const float2 w2 = twice(weight);
+    const float2 w2 = twice(real ? weight : 0.0f);
+    uint32_t at[kEach];
+    uint4 x[kEach][P];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         const int eight = group * kEach + i;
-        const uint32_t at = uint32_t(eight / 8) * kPanelBytes + uint32_t(r) * 128 + uint32_t(((eight % 8) ^ (r & 7)) * 16);
-        float2 v[4];
-        uint4 x = *reinterpret_cast<const uint4*>(tile + (P - 1) * S::kTileBytes + at);
-        v[0] = unpack_bf16(x.x), v[1] = unpack_bf16(x.y), v[2] = unpack_bf16(x.z), v[3] = unpack_bf16(x.w);
+        at[i] = uint32_t(eight / 8) * kPanelBytes + uint32_t(r) * 128 + uint32_t(((eight % 8) ^ (r & 7)) * 16);
 #pragma unroll
-        for (int q = P - 2; q >= 0; --q) {  // exact: the planes are the parts of one FP32 number, the small ones first
-            x = *reinterpret_cast<const uint4*>(tile + q * S::kTileBytes + at);
-            v[0] = add2(v[0], unpack_bf16(x.x)), v[1] = add2(v[1], unpack_bf16(x.y));
-            v[2] = add2(v[2], unpack_bf16(x.z)), v[3] = add2(v[3], unpack_bf16(x.w));
+        for (int q = 0; q < P; ++q) {
+            x[i][q] = *reinterpret_cast<const uint4*>(tile + q * S::kTileBytes + at[i]);
+            if (!real) x[i][q] = make_uint4(0, 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        float2 v[4];
+#pragma unroll
+        for (int q = P - 1; q >= 0; --q) {  // exact: the planes are the parts of one FP32 number, the small ones first
+            const float2 y[4] = {unpack_bf16(x[i][q].x), unpack_bf16(x[i][q].y), unpack_bf16(x[i][q].z), unpack_bf16(x[i][q].w)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = q == P - 1 ? y[e] : add2(v[e], y[e]);
         }
         float y[8];
 #pragma unroll
@@ -158,14 +167,10 @@ __device__ __forceinline__ void weigh_row(unsigned char* tile, unsigned char* mo
             y[2 * e] = v[e].x;
             y[2 * e + 1] = v[e].y;
         }
-        if (!real) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = 0.0f;
-        }
 #pragma unroll
         for (int q = 0; q < OUT; ++q) {
             const uint4 w = q + 1 == OUT ? pack8(y) : q == 0 && P == 3 ? first_plane8(y) : next_plane8(y);
-            *reinterpret_cast<uint4*>((q < P ? tile + q * S::kTileBytes : more + (q - P) * S::kTileBytes) + at) = w;
+            *reinterpret_cast<uint4*>((q < P ? tile + q * S::kTileBytes : more + (q - P) * S::kTileBytes) + at[i]) = w;
         }
     }
 }
@@ -213,6 +218,7 @@ __device__ __forceinline__ void open_block(Ctrl<SLOTS>& ctl, int workers) {
         mbar_init(&ctl.added, 1);
         mbar_init(&ctl.out, 1);
         mbar_init(&ctl.matrix, uint32_t(workers));
+        mbar_init(&ctl.stored, uint32_t(workers));
         mbar_init(&ctl.drain, 1);
         ctl.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -305,7 +311,8 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     unsigned char* matrix = ring + S::kSlots * S::kSlotBytes;
     __shared__ Ctrl<S::kSlots> ctl;
-    __shared__ alignas(16) float table[32];  // l^{31 - e}, going backwards l^e: of column e of a block of 32 pairs
+    // near l^n at 31 + n, zeros before it; and the factors of the columns of a block of 32 pairs: l^{31 - e}, backwards l^e
+    __shared__ alignas(16) float powers[64], table[32];
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned which = blockIdx.x % unsigned(all.count), place = blockIdx.x / unsigned(all.count);
@@ -314,7 +321,12 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
     const int head = int(place % unsigned(d.heads));
     const int64_t index = place / unsigned(d.heads);
 
-    if (threadIdx.x < 32) table[lane] = exp2f(float(d.later ? lane : 31 - lane) * log2_decay(d, head));
+    if (threadIdx.x < 32) {
+        const float l2 = log2_decay(d, head);
+        table[lane] = exp2f(float(d.later ? lane : 31 - lane) * l2);
+        if (lane < 31) powers[lane] = 0.0f;
+        powers[lane + 31] = d.near * exp2f(float(lane) * l2);
+    }
     if (head == 0 && threadIdx.x == 32 && index < d.batch) check_offsets(d, index);
     const Stretch s = block_stretch(d, index);
     if (s.rows == 0) return;
@@ -333,6 +345,10 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                 load_tile<KS, P>(su32(ring + slot * S::kSlotBytes), what == 0 ? &maps.a : what == 1 ? &maps.b : &maps.c, bar,
                                  head, walk.first(chunk), d.rows);
             });
+    } else if (warp == kFeeder + 2) {
+        if (lane == 0)
+            for (int i = 0; i < walk.chunks && mbar_wait(&ctl.stored, uint32_t(i) & 1u, abort); ++i)
+                mbar_arrive(&ctl.ring.empty[(3 * i + 2) % S::kSlots]);
     } else if (warp > kFeeder) {
         const uint32_t base = uniform(tmem), first_slot = uniform(su32(ring)), planes = uniform(su32(matrix));
         const int count = uniform(walk.chunks), last = uniform(walk.count(walk.chunks - 1));
@@ -414,7 +430,6 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                     }
                 }
                 tc_commit(&ctl.out);
-                tc_commit(&ctl.ring.empty[(3 * i + 2) % S::kSlots]);
             }
             if (!early && i + 1 < count) pairs(i + 1);
         }
@@ -428,7 +443,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         const uint32_t at_third = tmem + lanes + S::kThird + pair0 / 2, at_near = tmem + lanes + S::kNear + col0,
                        at_far = tmem + lanes + S::kFar + col0;
-        const float l2 = log2_decay(d, head), way = d.later ? -1.0f : 1.0f;
+        const float l2 = log2_decay(d, head);
         auto power = [&](int n) { return P == 1 ? ex2(float(n) * l2) : exp2f(float(n) * l2); };
         const bool holds = r < S::kDim;
         float state[kColumns];
@@ -448,13 +463,13 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                     const float2 v = mul2(make_float2(x[e + 2], x[e + 3]), mul2(row, make_float2(y.z, y.w)));
                     x[e] = u.x, x[e + 1] = u.y, x[e + 2] = v.x, x[e + 3] = v.y;
                 }
-            } else {
-                const float t = way * float(r - first);
+            } else {  // on the diagonal, or in the last chunk
+                const int t = r - first, from = d.later ? max(0, t) : 0, to = min(count - first, d.later ? 32 : t + 1);
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                    const float gap = fmaf(float(e), -way, t);
-                    const float w = (P == 1 ? ex2(gap * l2) : exp2f(gap * l2)) * d.near;
-                    x[e] = gap >= 0.0f && e < count - first ? x[e] * w : 0.0f;
+                    const int gap = d.later ? e - t : t - e;
+                    const float w = beside == 0 ? powers[(31 + gap) & 63] : d.near * power(gap);
+                    x[e] = e >= from && e < to ? x[e] * w : 0.0f;
                 }
             }
         };
@@ -527,7 +542,8 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
 
             if (!worker_wait(&ctl.out, parity, abort)) break;
             tc_fence_after();
-            T* out = static_cast<T*>(d.out) + (int64_t(walk.first(i) + r) * d.heads + head) * d.dim + col0;
+            constexpr int kPieces = kColumns * int(sizeof(T)) / 16, kWide = kPieces > 2 ? 4 : kPieces;
+            uint4 row[kWide] = {};
             const float2 reach2 = twice(reach);
 #pragma unroll
             for (int e = 0; e < kColumns; e += 8) {
@@ -539,15 +555,23 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                     near[o] = y.x;
                     near[o + 1] = y.y;
                 }
-                if (r >= count || col0 + e >= d.dim) continue;
                 if constexpr (P == 1) {
-                    *reinterpret_cast<uint4*>(out + e) = pack8(near);
+                    row[e / 8] = pack8(near);
                 } else {
-                    st4(out + e, make_float4(near[0], near[1], near[2], near[3]));
-                    st4(out + e + 4, make_float4(near[4], near[5], near[6], near[7]));
+#pragma unroll
+                    for (int o = 0; o < 8; o += 4)
+                        row[(e + o) / 4] = make_uint4(__float_as_uint(near[o]), __float_as_uint(near[o + 1]),
+                                                      __float_as_uint(near[o + 2]), __float_as_uint(near[o + 3]));
                 }
             }
             tc_fence_before();
+            // through the slot of c, which nobody reads any more
+            const int first_row = (warp & 3) * 32, left = min(kColumns, d.dim - col0) * int(sizeof(T)) / 16;
+            T* out = static_cast<T*>(d.out) + (int64_t(walk.first(i) + first_row) * d.heads + head) * d.dim + col0;
+            put_rows<kWide>(ring + (tile_c % S::kSlots) * S::kSlotBytes + warp * (kWide * 512), row, out,
+                            int64_t(d.heads) * d.dim * int(sizeof(T)), count - first_row, left);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            warp_arrive(&ctl.stored);
         }
     }
 

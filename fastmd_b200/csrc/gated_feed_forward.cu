@@ -160,34 +160,6 @@ __device__ __forceinline__ void activate(int act, float a, float& value, float& 
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 
-// A thread holds a row of the sums, memory wants rows side by side: what a warp stores or loads goes through 2 or 4 KB of shared
-// memory of its own, W pieces of 16 bytes a row, so that W lanes reach into one row. The pieces of a row are turned by the
-// row's number, which keeps the banks apart both ways.
-template <int W>
-__device__ __forceinline__ uint4* piece_at(unsigned char* scratch, int row, int piece) {
-    constexpr int kShift = W == 8 ? 0 : W == 4 ? 1 : 2;
-    return reinterpret_cast<uint4*>(scratch + (row * W + (piece ^ (row >> kShift & (W - 1)))) * 16);
-}
-
-// The first `pieces` of each of the first `rows` rows to `to` and on, rows `stride` bytes apart.
-template <int W>
-__device__ __forceinline__ void put_rows(unsigned char* scratch, const uint4* w, void* to, int64_t stride, int rows, int pieces) {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < W; ++i) *piece_at<W>(scratch, lane, i) = w[i];
-    __syncwarp();
-    if (lane % W >= pieces) return;
-    char* p = static_cast<char*>(to) + (lane / W) * stride + (lane % W) * 16;
-    const int left = rows - lane / W;
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-        if (i * (32 / W) < left)
-            *reinterpret_cast<uint4*>(p) = *piece_at<W>(scratch, i * (32 / W) + lane / W, lane % W);
-        p += (32 / W) * stride;
-    }
-}
-
 // 32 columns of FP32 of 32 rows: the loads (a lane holds pieces of eight rows) ..
 __device__ __forceinline__ void fetch_rows(const float* from, int64_t stride, int rows, int pieces, float4 (&x)[8]) {
     const int lane = threadIdx.x & 31, left = lane % 8 < pieces ? rows - lane / 8 : 0;

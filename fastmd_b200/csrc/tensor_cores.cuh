@@ -215,6 +215,34 @@ __device__ __forceinline__ uint4 next_plane8(float* v) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// A thread holds a row of a result, memory wants rows side by side: what a warp stores or loads goes through shared memory of
+// its own (32 rows), W pieces of 16 bytes a row, so that W lanes reach into one row. The pieces of a row are turned by the
+// row's number, which keeps the banks apart both ways.
+template <int W>
+__device__ __forceinline__ uint4* piece_at(unsigned char* scratch, int row, int piece) {
+    constexpr int kShift = W == 8 ? 0 : W == 4 ? 1 : 2;
+    return reinterpret_cast<uint4*>(scratch + (row * W + (piece ^ (row >> kShift & (W - 1)))) * 16);
+}
+
+// The first `pieces` of each of the first `rows` rows to `to` and on, rows `stride` bytes apart.
+template <int W>
+__device__ __forceinline__ void put_rows(unsigned char* scratch, const uint4* w, void* to, int64_t stride, int rows, int pieces) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < W; ++i) *piece_at<W>(scratch, lane, i) = w[i];
+    __syncwarp();
+    if (lane % W >= pieces) return;
+    char* p = static_cast<char*>(to) + (lane / W) * stride + (lane % W) * 16;
+    const int left = rows - lane / W;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        if (i * (32 / W) < left)
+            *reinterpret_cast<uint4*>(p) = *piece_at<W>(scratch, i * (32 / W) + lane / W, lane % W);
+        p += (32 / W) * stride;
+    }
+}
+
 // Zeros rows [first, last) of `panels` panels that lie `stride` bytes apart (the swizzle keeps a row's 128 bytes in
 // place), by `count` threads; then visible to the tensor cores after the barrier that follows.
 __device__ __forceinline__ void zero_rows(unsigned char* tile, int panels, uint32_t stride, int first, int last,
