@@ -132,6 +132,13 @@ __device__ __forceinline__ void tmem_read(uint32_t at, float (&v)[N]) {
 
 __device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
 
+// Two bfloat16 times a weight in two planes, rounded once (but for 2^-18).
+__device__ __forceinline__ uint32_t times(uint32_t x, uint32_t high, uint32_t low) {
+    uint32_t y;
+    asm("{\n\t.reg .b32 t;\n\tmul.rn.bf16x2 t, %1, %3;\n\tfma.rn.bf16x2 %0, %1, %2, t;\n\t}" : "=r"(y) : "r"(x), "r"(high), "r"(low));
+    return y;
+}
+
 // Row r of a tile of P planes times `weight` as OUT planes: the first P in place, the others from `more` on. A group takes
 // eights that lie side by side, in an order that keeps the banks apart; the swizzle moves eights within a panel's row.
 template <int KS, int P, int OUT, int GROUPS>
@@ -139,6 +146,7 @@ __device__ __forceinline__ void weigh_row(unsigned char* tile, unsigned char* mo
     using S = Shape<KS, P>;
     constexpr int kEach = 8 * S::kPanels / GROUPS;
     const float2 w2 = twice(real ? weight : 0.0f);
+    const uint32_t high = pack_bf16(w2.x, w2.x), low = pack_bf16(w2.x - unpack_bf16(high).x, w2.x - unpack_bf16(high).x);
     uint32_t at[kEach];
     uint4 x[kEach][P];
 #pragma unroll
@@ -153,24 +161,30 @@ __device__ __forceinline__ void weigh_row(unsigned char* tile, unsigned char* mo
     }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        float2 v[4];
+        if constexpr (OUT == 1) {
+            *reinterpret_cast<uint4*>(tile + at[i]) = make_uint4(times(x[i][0].x, high, low), times(x[i][0].y, high, low),
+                                                                 times(x[i][0].z, high, low), times(x[i][0].w, high, low));
+        } else {
+            float2 v[4];
 #pragma unroll
-        for (int q = P - 1; q >= 0; --q) {  // exact: the planes are the parts of one FP32 number, the small ones first
-            const float2 y[4] = {unpack_bf16(x[i][q].x), unpack_bf16(x[i][q].y), unpack_bf16(x[i][q].z), unpack_bf16(x[i][q].w)};
+            for (int q = P - 1; q >= 0; --q) {  // exact: the planes are the parts of one FP32 number, the small ones first
+                const float2 y[4] = {unpack_bf16(x[i][q].x), unpack_bf16(x[i][q].y), unpack_bf16(x[i][q].z),
+                                     unpack_bf16(x[i][q].w)};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = q == P - 1 ? y[e] : add2(v[e], y[e]);
-        }
-        float y[8];
+                for (int e = 0; e < 4; ++e) v[e] = q == P - 1 ? y[e] : add2(v[e], y[e]);
+            }
+            float y[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[e] = mul2(v[e], w2);
-            y[2 * e] = v[e].x;
-            y[2 * e + 1] = v[e].y;
-        }
+            for (int e = 0; e < 4; ++e) {
+                v[e] = mul2(v[e], w2);
+                y[2 * e] = v[e].x;
+                y[2 * e + 1] = v[e].y;
+            }
 #pragma unroll
-        for (int q = 0; q < OUT; ++q) {
-            const uint4 w = q + 1 == OUT ? pack8(y) : q == 0 && P == 3 ? first_plane8(y) : next_plane8(y);
-            *reinterpret_cast<uint4*>((q < P ? tile + q * S::kTileBytes : more + (q - P) * S::kTileBytes) + at[i]) = w;
+            for (int q = 0; q < OUT; ++q) {
+                const uint4 w = q + 1 == OUT ? pack8(y) : q == 0 && P == 3 ? first_plane8(y) : next_plane8(y);
+                *reinterpret_cast<uint4*>((q < P ? tile + q * S::kTileBytes : more + (q - P) * S::kTileBytes) + at[i]) = w;
+            }
         }
     }
 }
@@ -463,13 +477,25 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                     const float2 v = mul2(make_float2(x[e + 2], x[e + 3]), mul2(row, make_float2(y.z, y.w)));
                     x[e] = u.x, x[e + 1] = u.y, x[e + 2] = v.x, x[e + 3] = v.y;
                 }
-            } else {  // on the diagonal, or in the last chunk
+            } else {
+                // on the diagonal, or in the last chunk: the pairs of the columns [from, to)
                 const int t = r - first, from = d.later ? max(0, t) : 0, to = min(count - first, d.later ? 32 : t + 1);
+                const uint32_t seen = to > from ? (to >= 32 ? 0xffffffffu : (1u << to) - 1u) & (0xffffffffu << from) : 0u;
+                // every weight is computed and then chosen: a choice of what to compute would be a branch for every pair
+                float w[32];
+                if (beside == 0) {
+                    const float* from_t = powers + 31 + (d.later ? -t : t);
+                    const int step = d.later ? 1 : -1;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) w[e] = from_t[step * e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) w[e] = d.near * power(d.later ? e - t : t - e);
+                }
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                    const int gap = d.later ? e - t : t - e;
-                    const float w = beside == 0 ? powers[(31 + gap) & 63] : d.near * power(gap);
-                    x[e] = e >= from && e < to ? x[e] * w : 0.0f;
+                    const float y = x[e] * w[e];
+                    x[e] = seen >> e & 1u ? y : 0.0f;
                 }
             }
         };
@@ -545,33 +571,32 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
             constexpr int kPieces = kColumns * int(sizeof(T)) / 16, kWide = kPieces > 2 ? 4 : kPieces;
             uint4 row[kWide] = {};
             const float2 reach2 = twice(reach);
+            constexpr int kStep = kColumns % 16 == 0 ? 16 : 8;
 #pragma unroll
-            for (int e = 0; e < kColumns; e += 8) {
-                float near[8];
-                tmem_load8(at_near + e, near);
+            for (int e = 0; e < kColumns; e += kStep) {
+                float near[kStep];
+                tmem_read(at_near + e, near);
 #pragma unroll
-                for (int o = 0; o < 8; o += 2) {
+                for (int o = 0; o < kStep; o += 2) {
                     const float2 y = fma2(reach2, make_float2(far[e + o], far[e + o + 1]), make_float2(near[o], near[o + 1]));
                     near[o] = y.x;
                     near[o + 1] = y.y;
                 }
-                if constexpr (P == 1) {
-                    row[e / 8] = pack8(near);
-                } else {
+                constexpr int kValues = 16 / int(sizeof(T));  // of a piece
 #pragma unroll
-                    for (int o = 0; o < 8; o += 4)
-                        row[(e + o) / 4] = make_uint4(__float_as_uint(near[o]), __float_as_uint(near[o + 1]),
-                                                      __float_as_uint(near[o + 2]), __float_as_uint(near[o + 3]));
-                }
+                for (int o = 0; o < kStep; o += kValues)
+                    row[(e + o) / kValues] = P == 1 ? pack8(near + o)
+                                                    : make_uint4(__float_as_uint(near[o]), __float_as_uint(near[o + 1]),
+                                                                 __float_as_uint(near[o + 2]), __float_as_uint(near[o + 3]));
             }
             tc_fence_before();
             // through the slot of c, which nobody reads any more
             const int first_row = (warp & 3) * 32, left = min(kColumns, d.dim - col0) * int(sizeof(T)) / 16;
-            T* out = static_cast<T*>(d.out) + (int64_t(walk.first(i) + first_row) * d.heads + head) * d.dim + col0;
-            put_rows<kWide>(ring + (tile_c % S::kSlots) * S::kSlotBytes + warp * (kWide * 512), row, out,
-                            int64_t(d.heads) * d.dim * int(sizeof(T)), count - first_row, left);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            turn_pieces<kWide>(ring + (tile_c % S::kSlots) * S::kSlotBytes + warp * (kWide * 512), row);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stores: it waits for those too
             warp_arrive(&ctl.stored);
+            T* out = static_cast<T*>(d.out) + (int64_t(walk.first(i) + first_row) * d.heads + head) * d.dim + col0;
+            store_pieces<kWide>(row, out, int64_t(d.heads) * d.dim * int(sizeof(T)), count - first_row, left);
         }
     }
 

@@ -224,23 +224,34 @@ __device__ __forceinline__ uint4* piece_at(unsigned char* scratch, int row, int 
     return reinterpret_cast<uint4*>(scratch + (row * W + (piece ^ (row >> kShift & (W - 1)))) * 16);
 }
 
-// The first `pieces` of each of the first `rows` rows to `to` and on, rows `stride` bytes apart.
+// From a row a lane to W lanes a row: piece i becomes piece lane % W of row i (32 / W) + lane / W.
 template <int W>
-__device__ __forceinline__ void put_rows(unsigned char* scratch, const uint4* w, void* to, int64_t stride, int rows, int pieces) {
+__device__ __forceinline__ void turn_pieces(unsigned char* scratch, uint4 (&w)[W]) {
     const int lane = threadIdx.x & 31;
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < W; ++i) *piece_at<W>(scratch, lane, i) = w[i];
     __syncwarp();
-    if (lane % W >= pieces) return;
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = *piece_at<W>(scratch, i * (32 / W) + lane / W, lane % W);
+}
+
+// Turned pieces: the first `pieces` of each of the first `rows` rows to `to` and on, rows `stride` bytes apart.
+template <int W>
+__device__ __forceinline__ void store_pieces(const uint4 (&w)[W], void* to, int64_t stride, int rows, int pieces) {
+    const int lane = threadIdx.x & 31, left = lane % W < pieces ? rows - lane / W : 0;
     char* p = static_cast<char*>(to) + (lane / W) * stride + (lane % W) * 16;
-    const int left = rows - lane / W;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        if (i * (32 / W) < left)
-            *reinterpret_cast<uint4*>(p) = *piece_at<W>(scratch, i * (32 / W) + lane / W, lane % W);
+        if (i * (32 / W) < left) *reinterpret_cast<uint4*>(p) = w[i];
         p += (32 / W) * stride;
     }
+}
+
+template <int W>
+__device__ __forceinline__ void put_rows(unsigned char* scratch, uint4 (&w)[W], void* to, int64_t stride, int rows, int pieces) {
+    turn_pieces<W>(scratch, w);
+    store_pieces<W>(w, to, stride, rows, pieces);
 }
 
 // Zeros rows [first, last) of `panels` panels that lie `stride` bytes apart (the swizzle keeps a row's 128 bytes in
