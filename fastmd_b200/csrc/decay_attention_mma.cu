@@ -17,7 +17,7 @@
 // Warps, after the workers (8 or 16 of them: thread = row of the chunk and a part of the pairs or columns; for the matrix
 // its row, and a part of its columns):
 //   TMA: a, b, c of one chunk after the other through a ring of slots
-//   one thread hands c's slot back, through which the output has left (rows side by side)
+//   TMA: the output, out of c's slot, which then goes back to the ring (the last chunk's rows by the workers themselves)
 //   one thread issues the products, each as soon as what it needs is there: f (S of this chunk), b'^T c (b'), s of the next
 //   chunk, n (p). What goes from chunk to chunk is S alone: while f runs the workers weigh the pairs.
 // What lies in TMEM: s and p in its place (each thread overwrites what it has read; where there is room two by turns), f,
@@ -55,6 +55,7 @@ struct RowsShape : Shape<KS, P> {
     static constexpr int kBlocks = P == 1 && KS <= 4 ? 2 : 1;
     static constexpr int kGroups = kBlocks == 2 ? 2 : 4, kWorkers = 128 * kGroups, kThreads = kWorkers + 96;
     static constexpr int kColumns = S::kDim / kGroups, kPairs = kTile / kGroups;  // of a thread
+    static constexpr int kSize = P == 3 ? 4 : 2, kOutPanels = (S::kDim * kSize + 127) / 128;  // of the output
     static constexpr int kSlots = P == 3 ? 4 : 5;
     static constexpr int kPlanes = P == 3 ? 3 : 2;           // of the matrix
     static constexpr uint32_t kPanel = S::kDim * 128;        // of the matrix: kDim rows x 64 columns
@@ -89,7 +90,7 @@ struct Ctrl {
 };
 
 struct Maps {
-    CUtensorMap a, b, c;
+    CUtensorMap a, b, c, out;
 };
 
 struct AllMaps {
@@ -361,8 +362,17 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
             });
     } else if (warp == kFeeder + 2) {
         if (lane == 0)
-            for (int i = 0; i < walk.chunks && mbar_wait(&ctl.stored, uint32_t(i) & 1u, abort); ++i)
-                mbar_arrive(&ctl.ring.empty[(3 * i + 2) % S::kSlots]);
+            for (int i = 0; i < walk.chunks && mbar_wait(&ctl.stored, uint32_t(i) & 1u, abort); ++i) {
+                const int slot = (3 * i + 2) % S::kSlots;
+                if (walk.count(i) == kTile) {
+                    for (int p = 0; p < S::kOutPanels; ++p)
+                        tma_store_4d(&maps.out, su32(ring + slot * S::kSlotBytes + p * kPanelBytes), p * (128 / S::kSize), 0,
+                                     head, walk.first(i));
+                    asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+                }
+                mbar_arrive(&ctl.ring.empty[slot]);
+            }
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     } else if (warp > kFeeder) {
         const uint32_t base = uniform(tmem), first_slot = uniform(su32(ring)), planes = uniform(su32(matrix));
         const int count = uniform(walk.chunks), last = uniform(walk.count(walk.chunks - 1));
@@ -568,7 +578,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
 
             if (!worker_wait(&ctl.out, parity, abort)) break;
             tc_fence_after();
-            constexpr int kPieces = kColumns * int(sizeof(T)) / 16, kWide = kPieces > 2 ? 4 : kPieces;
+            constexpr int kPieces = kColumns * S::kSize / 16, kWide = kPieces > 2 ? 4 : kPieces;
             uint4 row[kWide] = {};
             const float2 reach2 = twice(reach);
             constexpr int kStep = kColumns % 16 == 0 ? 16 : 8;
@@ -590,13 +600,25 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                                                                  __float_as_uint(near[o + 2]), __float_as_uint(near[o + 3]));
             }
             tc_fence_before();
-            // through the slot of c, which nobody reads any more
-            const int first_row = (warp & 3) * 32, left = min(kColumns, d.dim - col0) * int(sizeof(T)) / 16;
-            turn_pieces<kWide>(ring + (tile_c % S::kSlots) * S::kSlotBytes + warp * (kWide * 512), row);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stores: it waits for those too
+            // by way of c's slot, which nobody reads any more: as TMA stores it, or turned for the workers' own stores. The fence
+            // comes before those: it would wait for them.
+            unsigned char* slot = ring + (tile_c % S::kSlots) * S::kSlotBytes;
+            if (count == kTile) {
+#pragma unroll
+                for (int e = 0; e < kPieces; ++e) {
+                    const int piece = col0 * S::kSize / 16 + e;
+                    *reinterpret_cast<uint4*>(slot + (piece / 8) * kPanelBytes + r * 128 + ((piece % 8) ^ (r & 7)) * 16) = row[e];
+                }
+            } else {
+                turn_pieces<kWide>(slot + warp * (kWide * 512), row);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(&ctl.stored);
-            T* out = static_cast<T*>(d.out) + (int64_t(walk.first(i) + first_row) * d.heads + head) * d.dim + col0;
-            store_pieces<kWide>(row, out, int64_t(d.heads) * d.dim * int(sizeof(T)), count - first_row, left);
+            if (count < kTile) {
+                const int first_row = (warp & 3) * 32, left = min(kColumns, d.dim - col0) * S::kSize / 16;
+                T* out = static_cast<T*>(d.out) + (int64_t(walk.first(i) + first_row) * d.heads + head) * d.dim + col0;
+                store_pieces<kWide>(row, out, int64_t(d.heads) * d.dim * S::kSize, count - first_row, left);
+            }
         }
     }
 
@@ -728,6 +750,18 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
     if (threadIdx.x == 0 && ctl.abort) raise_flag(d.flags, FMD_FLAG_WAIT_TIMEOUT);
 }
 
+// The output, [rows, heads, dim] contiguous: panels of 128 bytes and 128 rows of a head.
+fmd_status encode_out(const DriverCalls& drv, CUtensorMap* map, const Decay& d, bool f32) {
+    const cuuint64_t size = f32 ? 4 : 2;
+    const cuuint64_t dims[4] = {cuuint64_t(d.dim), 1, cuuint64_t(d.heads), cuuint64_t(d.rows)};
+    const cuuint64_t strides[3] = {d.dim * size, d.dim * size, d.heads * d.dim * size};
+    const cuuint32_t box[4] = {cuuint32_t(128 / size), 1, 1, cuuint32_t(kTile)}, step[4] = {1, 1, 1, 1};
+    const CUresult r = drv.encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, d.out, dims,
+                                  strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? FMD_OK : record_error_text(FMD_ERR_CUDA, "cuTensorMapEncodeTiled failed, CUresult", r);
+}
+
 fmd_status encode(AllMaps& maps, const Decays& all, bool rows, int planes) {
     const DriverCalls& drv = driver_calls();
     if (drv.encode == nullptr || drv.ctx_get_current == nullptr)
@@ -737,6 +771,7 @@ fmd_status encode(AllMaps& maps, const Decays& all, bool rows, int planes) {
         const Decay& d = all.d[i];
         const int64_t n = d.rows * planes;
         if (st == FMD_OK && rows) st = encode_packed(drv, &maps.m[i].a, d.a, n, d.heads, 1, d.dim, d.a_row, d.a_head, kTile);
+        if (st == FMD_OK && rows) st = encode_out(drv, &maps.m[i].out, d, planes == 3);
         if (st == FMD_OK) st = encode_packed(drv, &maps.m[i].b, d.b, n, d.heads, 1, d.dim, d.b_row, d.b_head, kTile);
         if (st == FMD_OK) st = encode_packed(drv, &maps.m[i].c, d.c, n, d.heads, 1, d.dim, d.c_row, d.c_head, kTile);
     }

@@ -15,6 +15,13 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int x, int y, int z, int w) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(src), "r"(x), "r"(y), "r"(z), "r"(w)
+                 : "memory");
+}
+
 // The products are issued by one thread of a warp whose lanes all walk through the same waits: only there, with every
 // operand the same in all lanes, does the compiler keep descriptors and addresses in uniform registers. Under a branch
 // on the lane each product took about 115 cycles to issue, twice what the tensor cores need for it.
