@@ -154,7 +154,8 @@ _SIGNATURES: dict[str, list] = {
     "fmd_packed_attention_workspace_bytes": [POINTER(FmdAttention), _I32, POINTER(c_size_t)],
     "fmd_packed_attention": [POINTER(FmdAttention), _P, _P, _P, c_size_t, _P, _P],
     "fmd_packed_attention_bwd": [POINTER(FmdAttention), _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, c_size_t, _P, _P],
-    "fmd_gated_feed_forward_bytes": [POINTER(FmdFeedForward), _I32, POINTER(c_size_t), POINTER(c_size_t)],
+    "fmd_gated_feed_forward_bytes": [POINTER(FmdFeedForward), _I32, POINTER(c_size_t), POINTER(c_size_t),
+                                     POINTER(c_size_t)],
     "fmd_gated_feed_forward": [POINTER(FmdFeedForward), _P, _I32, _P, c_size_t, _P, c_size_t, _P, _P],
     "fmd_gated_feed_forward_bwd": [POINTER(FmdFeedForward), _P, c_size_t, _P, _I64, _P, _P, _P, _P, _P, c_size_t, _P, _P],
     "fmd_decay_attention_workspace_bytes": [POINTER(FmdDecay), _I32, POINTER(c_size_t)],

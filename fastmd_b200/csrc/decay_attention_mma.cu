@@ -298,13 +298,20 @@ __device__ __forceinline__ Stretch block_stretch(const Decay& d, int64_t index) 
 template <int N>
 __device__ __forceinline__ void load_start(const Decay& d, const Stretch& s, int head, int r, int col0, float (&state)[N]) {
     const float* from = start_of(d, s, head);
-    const bool turn = d.length >= kWhole && d.transposed;
-    const int step = turn ? d.dim : 1;
-    if (from != nullptr) from += turn ? r + col0 * d.dim : r * d.dim + col0;
+    const bool turn = d.length >= kWhole && d.transposed, here = from != nullptr && r < d.dim;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        state[i] = from != nullptr && r < d.dim && col0 + i < d.dim ? *from : 0.0f;
-        from += step;
+    for (int i = 0; i < N; i += 4) {
+        const int col = col0 + i;
+        float4 x = f4_zero();
+        if (here && col < d.dim) {
+            if (turn) {
+                const float* p = from + col * d.dim + r;
+                x = make_float4(p[0], p[d.dim], p[2 * d.dim], p[3 * d.dim]);
+            } else {
+                x = ldg4(from + r * d.dim + col);
+            }
+        }
+        state[i] = x.x, state[i + 1] = x.y, state[i + 2] = x.z, state[i + 3] = x.w;
     }
 }
 

@@ -27,6 +27,7 @@
 // flight, frees its TMEM and returns.
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include "tensor_cores.cuh"
 
@@ -46,29 +47,33 @@ template <int KIND, int P>
 struct Shape {
     static constexpr int kWarps = P == 1 && (KIND == kUp || KIND == kHidden) ? 16 : 8;
     static constexpr int kThreads = 64 + 32 * kWarps;  // the takers first: a warp's part of TMEM goes by its number
-    static constexpr size_t kScratch = P == 1 && KIND == kUp ? 2048 : 4096;  // of each of these warps
+    static constexpr size_t kScratch = kWarps == 16 ? 2048 : 4096;  // of each of these warps
     static constexpr size_t kRing = 224 * 1024 - kWarps * kScratch;
     static constexpr size_t kBytes = 225 * 1024;
 };
 
-// One product [m, n] of a launch.
+// One product [m, n] of a launch; `out` null (kinds with one): not asked for, its tiles are passed over.
 struct Problem {
     void* out;
-    float* part;  // [splits, m, part_row]: sums of the splits
-    int64_t m, n, part_row;
+    int64_t m, n;
     int32_t a, b;  // maps
     int32_t m_tiles, n_tiles;
 };
 
 struct Args {
     Problem problem[3];
-    int32_t problems, splits, tiles;
+    int32_t problems;
+    int32_t tiles, whole, splits;  // tiles of all problems; those from `whole` on are shared out along the inner index
+    float* part;                   // [tiles - whole][splits][128][bn]: the shares' sums
     int32_t steps, turn;  // of 64 along the inner index; from step `turn` on the second pair of maps (kInput)
     int32_t bn, slots, act;
     int32_t tile_a;  // bytes of A's tile in a slot
-    // h, da and db: [planes][rows][row]; what is kept: [rows][row] FP32
-    __nv_bfloat16 *h, *da, *db;
-    float *slope, *level;
+    __nv_bfloat16 *h, *da, *db;  // [planes][rows][row]
+    // What the gradients are multiplied by, b act'(a) and act(a) [rows][row]: float32, or in 16 bits float16 times a power of
+    // two of each row's 16 columns, `unit` [row / 16][rows] (11 bits, over 2^-29 of the largest of the 16; else the rest of
+    // the kernel waits for memory, and one rounding to bfloat16 here would cost the gradients as much as their own)
+    void *slope, *level;
+    float2* unit;
     int64_t row, plane;
     int32_t* flags;
 };
@@ -109,30 +114,43 @@ __device__ __forceinline__ void mma2(uint32_t d, uint32_t a, uint32_t b, uint32_
         : "memory");
 }
 
-// The place of tile t: its problem, rows and columns, and the steps of its share of the inner index.
+// The place of a block's turn: its problem, rows and columns, the steps of its share of the inner index, and which of the
+// shares it is (part: its place among them; -1: a whole tile).
 struct Place {
-    int problem, m, n, split, from, to;
+    int problem, m, n, part, from, to;
 };
+
+__device__ __forceinline__ int turns_of(const Args& g) { return g.whole + (g.tiles - g.whole) * g.splits; }
 
 __device__ __forceinline__ Place place_of(const Args& g, int t) {
     Place p;
     p.problem = 0;
+    p.part = -1;
+    p.from = 0;
+    p.to = g.steps;
+    if (t >= g.whole && g.splits > 1) {
+        const int shared = g.tiles - g.whole, split = (t - g.whole) / shared, share = (g.steps + g.splits - 1) / g.splits;
+        t -= split * shared;
+        p.part = (t - g.whole) * g.splits + split;
+        p.from = min(g.steps, split * share);
+        p.to = min(g.steps, p.from + share);
+    }
     while (p.problem + 1 < g.problems) {
-        const int here = g.problem[p.problem].m_tiles * g.problem[p.problem].n_tiles * g.splits;
+        const int here = g.problem[p.problem].m_tiles * g.problem[p.problem].n_tiles;
         if (t < here) break;
         t -= here;
         ++p.problem;
     }
     const Problem& q = g.problem[p.problem];
-    const int all = q.m_tiles * q.n_tiles;
-    p.split = t / all;
-    t -= p.split * all;
     p.m = t / q.n_tiles;
     p.n = t - p.m * q.n_tiles;
-    const int share = (g.steps + g.splits - 1) / g.splits;
-    p.from = min(g.steps, p.split * share);
-    p.to = min(g.steps, p.from + share);
     return p;
+}
+
+// Whether anybody wants the problem.
+template <int KIND>
+__device__ __forceinline__ bool wanted(const Problem& q) {
+    return KIND != kWeights || q.out != nullptr;
 }
 
 __device__ __forceinline__ float rcp(float x) {
@@ -185,6 +203,46 @@ __device__ __forceinline__ void turn_rows(unsigned char* scratch, const float4 (
         v[4 * i] = y.x, v[4 * i + 1] = y.y, v[4 * i + 2] = y.z, v[4 * i + 3] = y.w;
     }
 }
+
+// 32 columns of float16 of 32 rows in the same way: four lanes a row.
+__device__ __forceinline__ void fetch_halves(const __half* from, int64_t stride, int rows, int pieces, uint4 (&x)[4]) {
+    const int lane = threadIdx.x & 31, left = lane % 4 < pieces ? rows - lane / 4 : 0;
+    const __half* p = from + (lane / 4) * stride + (lane % 4) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[i] = i * 8 < left ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+        p += 8 * stride;
+    }
+}
+
+__device__ __forceinline__ void turn_halves(unsigned char* scratch, uint4 (&x)[4]) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *piece_at<4>(scratch, i * 8 + lane / 4, lane % 4) = x[i];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *piece_at<4>(scratch, lane, i);
+}
+
+// The power of two that takes 16 values to float16's upper range, and those values; `unit`: its inverse.
+__device__ __forceinline__ void pack_halves(const float* v, uint4 (&w)[2], float& unit) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(v[i]));
+    const int e = int(__float_as_uint(most) >> 23);
+    const int shift = e == 255 ? 0 : min(127 + 14 - e, 100);  // the largest becomes 2^14 .. 2^15
+    const float up = __uint_as_float(uint32_t(127 + shift) << 23);
+    unit = __uint_as_float(uint32_t(127 - shift) << 23);
+    uint32_t* p = reinterpret_cast<uint32_t*>(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const __half2 h = __floats2half2_rn(v[2 * i] * up, v[2 * i + 1] * up);
+        p[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+__device__ __forceinline__ float2 unpack_half(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
 // N values a row as P planes, `plane` values apart; rows are padded to multiples of 8 columns. The values are used up.
 template <int P, int N>
@@ -283,9 +341,10 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             int slot = 0;
             uint32_t phase = 0, armed = 0;  // armed: slots with a copy that nobody may have waited for
             bool ok = true;
-            for (int t = blockIdx.x; t < g.tiles && ok; t += gridDim.x) {
+            for (int t = blockIdx.x; t < turns_of(g) && ok; t += gridDim.x) {
                 const Place p = place_of(g, t);
                 const Problem& q = g.problem[p.problem];
+                if (!wanted<KIND>(q)) continue;
                 const int m0 = p.m * kM, n0 = p.n * (KIND == kUp ? g.bn / 2 : g.bn);
                 for (int step = p.from; step < p.to; ++step) {
                     if (!mbar_wait(&ctl.empty[slot], phase ^ 1u, abort)) {
@@ -344,8 +403,9 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
         int slot = 0, unit = 0;
         uint32_t phase = 0;
         bool ok = true, issued = false;
-        for (int t = blockIdx.x; t < g.tiles && ok; t += gridDim.x) {
+        for (int t = blockIdx.x; t < turns_of(g) && ok; t += gridDim.x) {
             const Place p = place_of(g, t);
+            if (!wanted<KIND>(g.problem[p.problem])) continue;
             const int from = uniform(p.from), to = uniform(p.to);
             for (int start = from; start < to && ok; ++unit) {
                 const int end = P == 1 ? to : min(to, start + kSegment);
@@ -410,26 +470,39 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             warp_arrive(&ctl.taken[unit & 1]);
             ++unit;
         };
-        // kHidden: the factors of the next 32 columns are on their way while the last ones are stored
+        // kHidden, float32: the factors of the next 32 columns are on their way while the last ones are stored
         float4 ahead[8];
-        auto fetch = [&](const float* factor, int64_t row0, int64_t col, int rows, int64_t n) {
+        auto fetch = [&](const void* factor, int64_t row0, int64_t col, int rows, int64_t n) {
             const int pieces = int(max(int64_t(0), min(int64_t(8), (n - col + 7) / 8 * 2)));
-            fetch_rows(factor + row0 * g.row + col, g.row, rows, pieces, ahead);
+            fetch_rows(static_cast<const float*>(factor) + row0 * g.row + col, g.row, rows, pieces, ahead);
         };
-        // dh of 32 columns by `take(i, v)`, 16 at a time
-        auto spread = [&](const Problem& q, int64_t row0, int rows, int64_t col, int64_t after, auto take, auto taken) {
+        auto spread = [&](const Problem& q, int64_t row0, int rows, int64_t col, int64_t after, const float* v) {
             const int columns = int(max(int64_t(0), min(int64_t(32), q.n - col)));
             const int64_t at = row0 * g.row + col;
             float x[32];
             turn_rows(scratch, ahead, x);
             fetch(g.level, row0, col, rows, q.n);
-            take(x);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] *= v[i];
             put_planes<P, 32>(scratch, x, g.da + at, g.row, g.plane, rows, columns);
             turn_rows(scratch, ahead, x);
             fetch(g.slope, row0, after, rows, q.n);
-            take(x);
-            taken();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] *= v[i];
             put_planes<P, 32>(scratch, x, g.db + at, g.row, g.plane, rows, columns);
+        };
+        // the same in 16 bits, of both factors at once
+        uint4 slopes[4], levels[4];
+        float2 unit_of[2];
+        auto fetch_both = [&](int64_t row0, int64_t col, int rows, int64_t n) {
+            const int pieces = int(max(int64_t(0), min(int64_t(4), (n - col + 7) / 8)));
+            fetch_halves(static_cast<const __half*>(g.slope) + row0 * g.row + col, g.row, rows, pieces, slopes);
+            fetch_halves(static_cast<const __half*>(g.level) + row0 * g.row + col, g.row, rows, pieces, levels);
+            const int lane = threadIdx.x & 31;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                unit_of[i] = lane < rows && 2 * i < pieces ? __ldg(g.unit + (col / 16 + i) * g.problem[0].m + row0 + lane)
+                                                           : make_float2(0.0f, 0.0f);
         };
         // What follows the W sums of column `col` and on (kUp: of the hidden units).
         auto finish = [&](const Problem& q, const Place& p, int64_t row0, int rows, int64_t col, float(&v)[W]) {
@@ -453,25 +526,42 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                 else
                     put_planes<P, kH>(scratch, h, g.h + at, g.row, g.plane, rows, columns);
                 if (g.slope != nullptr) {
-                    put_floats<kH>(scratch, v + kH, g.slope + at, g.row, rows, (columns + 7) & ~7);
-                    put_floats<kH>(scratch, v, g.level + at, g.row, rows, (columns + 7) & ~7);
+                    if constexpr (P == 1) {
+                        uint4 w[2];
+                        float2 unit;
+                        pack_halves(v + kH, w, unit.x);
+                        put_rows<2>(scratch, w, static_cast<__half*>(g.slope) + at, g.row * 2, rows, (columns + 7) / 8);
+                        pack_halves(v, w, unit.y);
+                        put_rows<2>(scratch, w, static_cast<__half*>(g.level) + at, g.row * 2, rows, (columns + 7) / 8);
+                        const int lane = threadIdx.x & 31;
+                        if (lane < rows && columns > 0) g.unit[col / 16 * q.m + row0 + lane] = unit;
+                    } else {
+                        put_floats<kH>(scratch, v + kH, static_cast<float*>(g.slope) + at, g.row, rows, (columns + 7) & ~7);
+                        put_floats<kH>(scratch, v, static_cast<float*>(g.level) + at, g.row, rows, (columns + 7) & ~7);
+                    }
                 }
             } else if constexpr (KIND != kHidden) {
-                const bool parts = g.splits > 1;
-                const int64_t n = parts ? q.part_row : q.n;
-                const int columns = int(max(int64_t(0), min(int64_t(W), n - col)));
-                if (parts)
-                    put_result<W>(scratch, v, q.part + (int64_t(p.split) * q.m + row0) * n + col, n, rows, columns, true);
+                const int columns = int(max(int64_t(0), min(int64_t(W), q.n - col)));
+                if (p.part >= 0)
+                    put_result<W>(scratch, v, g.part + (int64_t(p.part) * kM + (warp & 3) * 32) * g.bn + (col - int64_t(p.n) * g.bn),
+                                  g.bn, rows, W, true);
                 else
-                    put_result<W>(scratch, v, static_cast<T*>(q.out) + row0 * n + col, n, rows, columns, n % 8 == 0);
+                    put_result<W>(scratch, v, static_cast<T*>(q.out) + row0 * q.n + col, q.n, rows, columns, q.n % 8 == 0);
             }
         };
-        for (int t = blockIdx.x; t < g.tiles && ok; t += gridDim.x) {
+        for (int t = blockIdx.x; t < turns_of(g) && ok; t += gridDim.x) {
             const Place p = place_of(g, t);
             const Problem& q = g.problem[p.problem];
+            if (!wanted<KIND>(q)) continue;
             const int64_t row0 = int64_t(p.m) * kM + (warp & 3) * 32, n0 = int64_t(p.n) * (KIND == kUp ? g.bn / 2 : g.bn);
             const int rows = int(max(int64_t(0), min(int64_t(32), q.m - row0)));
-            if (KIND == kHidden && group < units) fetch(g.slope, row0, n0 + group * kStep, rows, q.n);
+            if constexpr (KIND == kHidden) {
+                if (P == 1) {
+                    if (group < units) fetch_both(row0, n0 + group * kStep, rows, q.n);
+                } else {
+                    fetch(g.slope, row0, n0 + group * kStep, rows, q.n);
+                }
+            }
             if (p.from >= p.to) {  // a split without a share: sums of zero
                 float v[W] = {};
                 for (int u = group; u < units; u += kGroups) finish(q, p, row0, rows, n0 + u * kStep, v);
@@ -484,25 +574,30 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                 for (int u = group; u < units; u += kGroups) {
                     const bool last = u + kGroups >= units;
                     if constexpr (KIND == kHidden) {
-#pragma unroll 1
-                        for (int j = 0; j < W; j += 32) {
-                            const bool end = last && j + 32 == W;
-                            const int64_t col = n0 + u * W + j;
-                            const int64_t after = end ? q.n : j + 32 < W ? col + 32 : n0 + (u + kGroups) * W;
-                            spread(q, row0, rows, col, after,
-                                   [&](float(&x)[32]) {
+                        const int64_t col = n0 + u * 32;
+                        const int columns = int(max(int64_t(0), min(int64_t(32), q.n - col)));
+                        turn_halves(scratch, slopes);
+                        turn_halves(scratch, levels);
+                        uint4 da[4], db[4];
+                        const uint32_t *s = reinterpret_cast<const uint32_t*>(slopes), *l = reinterpret_cast<const uint32_t*>(levels);
 #pragma unroll
-                                       for (int i = 0; i < 32; i += 16) {
-                                           float v[16];
-                                           tmem_load16(at + u * W + j + i, v);
+                        for (int j = 0; j < 2; ++j) {
+                            float v[16], x[16], y[16];
+                            tmem_load16(at + u * 32 + j * 16, v);
 #pragma unroll
-                                           for (int e = 0; e < 16; ++e) x[i + e] *= v[e];
-                                       }
-                                   },
-                                   [&]() {
-                                       if (end) done();
-                                   });
+                            for (int i = 0; i < 16; i += 2) {
+                                const float2 f = unpack_half(s[j * 8 + i / 2]), h = unpack_half(l[j * 8 + i / 2]);
+                                x[i] = v[i] * (f.x * unit_of[j].x), x[i + 1] = v[i + 1] * (f.y * unit_of[j].x);
+                                y[i] = v[i] * (h.x * unit_of[j].y), y[i + 1] = v[i + 1] * (h.y * unit_of[j].y);
+                            }
+                            da[2 * j] = pack8(x), da[2 * j + 1] = pack8(x + 8);
+                            db[2 * j] = pack8(y), db[2 * j + 1] = pack8(y + 8);
                         }
+                        if (last) done();
+                        else fetch_both(row0, col + kGroups * 32, rows, q.n);
+                        const int64_t to = row0 * g.row + col;
+                        put_rows<4>(scratch, da, g.da + to, g.row * 2, rows, (columns + 7) / 8);
+                        put_rows<4>(scratch, db, g.db + to, g.row * 2, rows, (columns + 7) / 8);
                     } else {
                         float v[W];
                         if constexpr (KIND == kUp) {
@@ -516,35 +611,33 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                     }
                 }
             } else {
-                constexpr int kUnits = 128 / W / kGroups;  // bn = 128
+                constexpr int kUnits = 128 / W / kGroups;  // at most: bn is up to 128
                 float sum[kUnits][W] = {};
                 for (int start = p.from; start < p.to; start += kSegment) {
                     if (!(ok = wait())) break;
                     const uint32_t at = tmem + lanes + uint32_t(unit & 1) * 256u;
 #pragma unroll
-                    for (int u = 0; u < kUnits; ++u)
+                    for (int u = 0; u < kUnits; ++u) {
+                        if (group + u * kGroups >= units) break;
 #pragma unroll
                         for (int j = 0; j < W; j += 16) {
-                            const int col = (group + u * kGroups) * kStep + (KIND == kUp && j >= W / 2 ? 64 + j - W / 2 : j);
+                            const int col = (group + u * kGroups) * kStep + (KIND == kUp && j >= W / 2 ? g.bn / 2 + j - W / 2 : j);
                             float big[16], small[16];
                             tmem_load16(at + col, big);
                             tmem_load16(at + 128 + col, small);
 #pragma unroll
                             for (int i = 0; i < 16; ++i) sum[u][j + i] += big[i] + small[i];
                         }
+                    }
                     done();
                 }
                 if (!ok) break;
 #pragma unroll
                 for (int u = 0; u < kUnits; ++u) {
+                    if (group + u * kGroups >= units) break;
                     const int64_t col = n0 + (group + u * kGroups) * kStep;
                     if constexpr (KIND == kHidden)
-                        spread(q, row0, rows, col, u + 1 < kUnits ? col + kGroups * kStep : q.n,
-                               [&](float(&x)[32]) {
-#pragma unroll
-                                   for (int i = 0; i < 32; ++i) x[i] *= sum[u][i];
-                               },
-                               []() {});
+                        spread(q, row0, rows, col, group + (u + 1) * kGroups < units ? col + kGroups * kStep : q.n, sum[u]);
                     else
                         finish(q, p, row0, rows, col, sum[u]);
                 }
@@ -591,23 +684,31 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitArgs a) {
     }
 }
 
-// out [m, n] = the sum of the splits' parts, in their order; a thread per four columns, blockIdx.y: the problem.
+// The tiles that were shared out: the sums of their shares, in their order. blockIdx.y: the tile; a thread per four columns.
 template <typename T>
 __global__ void __launch_bounds__(256) add_kernel(const Args g) {
-    const Problem& q = g.problem[blockIdx.y];
-    const int64_t per = (q.n + 3) / 4, all = q.m * per;
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += int64_t(gridDim.x) * 256) {
-        const int64_t row = i / per;
-        const int64_t col = (i - row * per) * 4;
-        float4 sum = f4_zero();
+    Place p = place_of(g, g.whole + int(blockIdx.y));
+    const Problem& q = g.problem[p.problem];
+    if (q.out == nullptr) return;
+    const int per = g.bn / 4, at = int(blockIdx.x) * 256 + int(threadIdx.x), row = at / per, col = (at - row * per) * 4;
+    if (row >= kM) return;
+    const float* part = g.part + (int64_t(blockIdx.y) * g.splits * kM + row) * g.bn + col;
+    float4 sum = f4_zero();
 #pragma unroll 4
-        for (int z = 0; z < g.splits; ++z)
-            sum = f4_add(sum, *reinterpret_cast<const float4*>(q.part + (int64_t(z) * q.m + row) * q.part_row + col));
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-        T* out = static_cast<T*>(q.out) + row * q.n + col;
+    for (int z = 0; z < g.splits; ++z) sum = f4_add(sum, *reinterpret_cast<const float4*>(part + int64_t(z) * kM * g.bn));
+    const int64_t m = int64_t(p.m) * kM + row, n = int64_t(p.n) * g.bn + col;
+    if (m >= q.m) return;
+    T* out = static_cast<T*>(q.out) + m * q.n + n;
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+    if (q.n % 4 == 0 && n < q.n) {
+        if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+        else
+            st4(out, sum);
+    } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (col + e < q.n) store1(out + e, v[e]);
+            if (n + e < q.n) store1(out + e, v[e]);
     }
 }
 
@@ -634,32 +735,38 @@ fmd_status encode(CUtensorMap* map, const Matrix& x, int box_rows) {
 
 int64_t round_up(int64_t v, int64_t unit) { return (v + unit - 1) / unit * unit; }
 
-// How a product runs: columns of a tile, and shares of the inner index.
+// How a launch runs: columns of a tile, the tiles that are not shared out, shares of the others along the inner index.
 struct Plan {
-    int bn, splits;
+    int bn, tiles, whole, splits;
+    size_t bytes() const { return splits > 1 ? size_t(tiles - whole) * splits * kM * bn * sizeof(float) : 0; }
 };
 
 // The time of a launch in steps of 128 x 256 x 64, about 0.3 us each: rounds of blocks, each its tile's steps and, besides,
-// about six for its start and end; the shares' sums are written and read again. unit: bn is a multiple of it (panels of 64
-// columns where the rows of B are the inner index; else any 32, so that few rows' weights are read by all SMs alike).
+// about six for its start and end. Tiles are shared out along the inner index where that ends sooner: all of them, or those
+// of the last round, which do not fill the GPU; the shares' sums are written and read again. unit: bn is a multiple of it
+// (panels of 64 columns where the rows of B are the inner index; else any 32, so that few rows' weights are read by all
+// SMs alike).
 Plan plan(const int64_t* m, const int64_t* n, int problems, int64_t steps, int planes, int unit, bool can_split) {
-    Plan best{128, 1};
+    Plan best{128, 0, 0, 1};
     double least = 1e300;
-    for (int bn = planes == 1 ? 64 : 128; bn <= (planes == 1 ? 256 : 128); bn += unit) {
+    for (int bn = unit; bn <= (planes == 1 ? 256 : 128); bn += unit) {
         int64_t tiles = 0;
-        double values = 0.0;
-        for (int i = 0; i < problems; ++i) {
-            tiles += ((m[i] + kM - 1) / kM) * ((n[i] + bn - 1) / bn);
-            values += double(m[i]) * double(n[i]);
-        }
-        for (int splits = 1; splits <= (can_split ? 64 : 1) && (splits == 1 || 4 * splits <= steps); ++splits) {
-            const int64_t rounds = (tiles * splits + kNumSMs - 1) / kNumSMs;
-            const double step = (planes == 1 ? 1.0 : 6.0) * (0.25 + 0.75 * bn / 256.0);
-            const double sums = splits > 1 ? 10.0 + (2.0 * splits + 1.0) * values * 4.0 / 6.5e6 / 0.3 : 0.0;
-            const double time = rounds * (((steps + splits - 1) / splits) * step + 6.0) + sums;
-            if (time < least) {
-                least = time;
-                best = Plan{bn, splits};
+        for (int i = 0; i < problems; ++i) tiles += ((m[i] + kM - 1) / kM) * ((n[i] + bn - 1) / bn);
+        const double step = (planes == 1 ? 1.0 : 6.0) * (0.25 + 0.75 * bn / 256.0);
+        for (int full = 0; full < (can_split && tiles > kNumSMs ? 2 : 1); ++full) {
+            const int64_t whole = full ? tiles / kNumSMs * kNumSMs : 0, rest = tiles - whole;
+            const double before = whole / kNumSMs * (steps * step + 6.0);
+            // shares beyond four rounds of blocks even nothing out any more
+            for (int splits = 1; splits <= (can_split ? 64 : 1) &&
+                                 (splits == 1 || (4 * splits <= steps && rest * (splits - 1) < 4 * kNumSMs)); ++splits) {
+                const int64_t rounds = (rest * splits + kNumSMs - 1) / kNumSMs;
+                const double moved = (2.0 * splits + 1.0) * rest * kM * bn * 4.0;
+                const double sums = splits > 1 ? 10.0 + moved / 6.5e6 / 0.3 : 0.0;
+                const double time = before + rounds * (((steps + splits - 1) / splits) * step + 6.0) + sums;
+                if (time < least) {
+                    least = time;
+                    best = Plan{bn, int(tiles), int(splits > 1 ? whole : tiles), splits};
+                }
             }
         }
     }
@@ -679,7 +786,8 @@ fmd_status launch(const Maps& maps, Args& g, cudaStream_t s) {
     if (st != FMD_OK) return st;
     const int slots = int(S::kRing / (P * (g.tile_a + g.bn * 128)));
     g.slots = slots < kMostSlots ? slots : kMostSlots;
-    feed_kernel<KIND, P, W><<<unsigned(g.tiles < kNumSMs ? g.tiles : kNumSMs), S::kThreads, S::kBytes, s>>>(maps, g);
+    const int64_t turns = g.whole + int64_t(g.tiles - g.whole) * g.splits;
+    feed_kernel<KIND, P, W><<<unsigned(turns < kNumSMs ? turns : kNumSMs), S::kThreads, S::kBytes, s>>>(maps, g);
     return check_launch();
 }
 
@@ -700,36 +808,27 @@ fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args&
         if (st != FMD_OK) return st;
     }
     g.bn = p.bn;
+    g.tiles = p.tiles;
+    g.whole = p.whole;
     g.splits = p.splits;
-    g.tiles = 0;
     for (int i = 0; i < g.problems; ++i) {
         Problem& q = g.problem[i];
         const int columns = KIND == kUp ? p.bn / 2 : p.bn;
         q.m_tiles = int((q.m + kM - 1) / kM);
         q.n_tiles = int((q.n + columns - 1) / columns);
-        q.part_row = round_up(q.n, 8);
-        g.tiles += q.m_tiles * q.n_tiles * p.splits;
     }
-    if (g.tiles == 0) return FMD_OK;
-    fmd_status st = planes == 3 ? launch<KIND, 3, 32>(maps, g, s)
-                    : KIND != kUp && g.bn == 256 ? launch<KIND, 1, KIND == kUp ? 32 : 64>(maps, g, s) : launch<KIND, 1, 32>(maps, g, s);
+    constexpr int kWide = KIND == kUp || KIND == kHidden ? 32 : 64;
+    const fmd_status st = planes == 3   ? launch<KIND, 3, 32>(maps, g, s)
+                          : g.bn == 256 ? launch<KIND, 1, kWide>(maps, g, s)
+                                        : launch<KIND, 1, 32>(maps, g, s);
     if (st != FMD_OK || p.splits == 1) return st;
-    int64_t most = 0;
-    for (int i = 0; i < g.problems; ++i) {
-        const int64_t all = g.problem[i].m * ((g.problem[i].n + 3) / 4);
-        most = all > most ? all : most;
-    }
-    const dim3 grid(unsigned(grid_for(most, 256)), unsigned(g.problems));
+    const dim3 grid(unsigned((kM * p.bn / 4 + 255) / 256), unsigned(p.tiles - p.whole));
     if (planes == 1) add_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(g);
     else add_kernel<float><<<grid, 256, 0, s>>>(g);
     return check_launch();
 }
 
 int64_t steps_of(int64_t k) { return (k + kK - 1) / kK; }
-
-size_t part_bytes(const Plan& p, int64_t m, int64_t n) {
-    return p.splits > 1 ? size_t(p.splits) * m * round_up(n, 8) * sizeof(float) : 0;
-}
 
 Plan down_plan(const Sizes& z) { return plan(&z.rows, &z.out, 1, steps_of(z.hidden), z.planes, 32, true); }
 Plan input_plan(const Sizes& z) { return plan(&z.rows, &z.width, 1, 2 * steps_of(z.hidden), z.planes, 64, true); }
@@ -750,7 +849,7 @@ struct Layout {
 
 // What the forward pass keeps for the backward pass: h, FP32 factors, and in float32 the planes of what it was given.
 struct Kept {
-    size_t h, slope, level, x, gate, up, down, bytes;
+    size_t h, slope, level, unit, x, gate, up, down, bytes;
 };
 
 Kept kept_layout(const Sizes& z, bool factors) {
@@ -759,8 +858,10 @@ Kept kept_layout(const Sizes& z, bool factors) {
     const size_t hidden = size_t(z.rows) * z.hidden_row;
     k.h = at.take(hidden * z.planes * 2);
     if (factors) {
-        k.slope = at.take(hidden * 4);
-        k.level = at.take(hidden * 4);
+        const size_t size = z.planes == 3 ? 4 : 2;
+        k.slope = at.take(hidden * size);
+        k.level = at.take(hidden * size);
+        if (z.planes == 1) k.unit = at.take(size_t(z.rows) * ((z.hidden + 15) / 16) * sizeof(float2));
     }
     if (z.planes == 3) {
         k.x = at.take(size_t(z.rows) * z.width_row * 6);
@@ -784,9 +885,7 @@ Scratch scratch_layout(const Sizes& z) {
     k.da = at.take(hidden);
     k.db = at.take(hidden);
     if (z.planes == 3) k.g = at.take(size_t(z.rows) * z.out_row * 6);
-    const Plan w = weights_plan(z);
-    const size_t weights = 2 * part_bytes(w, z.hidden, z.width) + part_bytes(w, z.out, z.hidden);
-    const size_t input = part_bytes(input_plan(z), z.rows, z.width);
+    const size_t weights = weights_plan(z).bytes(), input = input_plan(z).bytes();
     k.part = at.take(weights > input ? weights : input);
     k.bytes = at.bytes;
     return k;
@@ -856,15 +955,15 @@ using namespace fmd;
 
 extern "C" {
 
-fmd_status fmd_gated_feed_forward_bytes(const fmd_feed_forward* problem, int32_t backward, size_t* kept,
-                                        size_t* workspace) {
+fmd_status fmd_gated_feed_forward_bytes(const fmd_feed_forward* problem, int32_t keep, size_t* kept, size_t* forward,
+                                        size_t* backward) {
     Sizes z;
-    if (problem == nullptr || kept == nullptr || workspace == nullptr) return FMD_ERR_INVALID_ARGUMENT;
+    if (problem == nullptr || kept == nullptr || forward == nullptr || backward == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     const fmd_status st = check(*problem, z);
     if (st != FMD_OK) return st;
-    *kept = kept_layout(z, backward != 0).bytes;
-    if (backward) *workspace = z.rows > 0 ? scratch_layout(z).bytes : 0;
-    else *workspace = part_bytes(down_plan(z), z.rows, z.out);
+    *kept = z.rows > 0 ? kept_layout(z, keep != 0).bytes : 0;
+    *forward = z.rows > 0 ? down_plan(z).bytes() : 0;
+    *backward = z.rows > 0 && keep ? scratch_layout(z).bytes : 0;
     return FMD_OK;
 }
 
@@ -877,7 +976,7 @@ fmd_status fmd_gated_feed_forward(const fmd_feed_forward* problem, void* y, int3
     const Kept k = kept_layout(z, keep != 0);
     const Plan down = down_plan(z);
     if (y == nullptr) return FMD_ERR_INVALID_ARGUMENT;
-    if (kept_bytes < k.bytes || kept == nullptr || workspace_bytes < part_bytes(down, z.rows, z.out) ||
+    if (kept_bytes < k.bytes || kept == nullptr || workspace_bytes < down.bytes() ||
         (down.splits > 1 && workspace == nullptr))
         return FMD_ERR_WORKSPACE;
     if (!aligned16(y) || !aligned16(kept) || !aligned16(workspace)) return FMD_ERR_UNSUPPORTED;
@@ -903,8 +1002,9 @@ fmd_status fmd_gated_feed_forward(const fmd_feed_forward* problem, void* y, int3
     g.row = z.hidden_row;
     g.plane = z.rows * z.hidden_row;
     if (keep) {
-        g.slope = reinterpret_cast<float*>(at + k.slope);
-        g.level = reinterpret_cast<float*>(at + k.level);
+        g.slope = at + k.slope;
+        g.level = at + k.level;
+        g.unit = reinterpret_cast<float2*>(at + k.unit);
     }
     g.problem[0].m = z.rows;
     g.problem[0].n = z.hidden;
@@ -916,7 +1016,7 @@ fmd_status fmd_gated_feed_forward(const fmd_feed_forward* problem, void* y, int3
     }
     g.problem[0].n = z.out;
     g.problem[0].out = y;
-    g.problem[0].part = static_cast<float*>(workspace);
+    g.part = static_cast<float*>(workspace);
     g.steps = int(steps_of(z.hidden));
     const Matrix h{at + k.h, z.rows, z.hidden, z.hidden_row, z.planes};
     return run<kDown>(z.planes, &h, &in.down, 1, g, down, s);
@@ -965,11 +1065,12 @@ fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kep
     args.flags = flags;
     args.row = z.hidden_row;
     args.plane = z.rows * z.hidden_row;
-    args.slope = reinterpret_cast<float*>(at + k.slope);
-    args.level = reinterpret_cast<float*>(at + k.level);
+    args.slope = at + k.slope;
+    args.level = at + k.level;
+    args.unit = reinterpret_cast<float2*>(at + k.unit);
     args.da = reinterpret_cast<__nv_bfloat16*>(own + w.da);
     args.db = reinterpret_cast<__nv_bfloat16*>(own + w.db);
-    float* part = reinterpret_cast<float*>(own + w.part);
+    args.part = reinterpret_cast<float*>(own + w.part);
     if (dx != nullptr || dgate != nullptr || dup != nullptr) {
         args.problems = 1;
         args.problem[0].m = z.rows;
@@ -984,7 +1085,6 @@ fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kep
         args.problems = 1;
         args.problem[0].n = z.width;
         args.problem[0].out = dx;
-        args.problem[0].part = part;
         args.turn = int(steps_of(z.hidden));
         args.steps = 2 * args.turn;
         const Matrix a[2] = {da, db}, b[2] = {in.gate, in.up};
@@ -995,20 +1095,19 @@ fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kep
     const Matrix h{at + k.h, z.rows, z.hidden, z.hidden_row, z.planes};
     const Matrix a[3] = {da, db, gm}, b[3] = {in.x, in.x, h};
     void* const out[3] = {dgate, dup, ddown};
-    args.problems = 0;
+    // all three have their places whichever are asked for, so that each has the same bits
+    args.problems = 3;
     for (int i = 0; i < 3; ++i) {
-        if (out[i] == nullptr) continue;
-        Problem& q = args.problem[args.problems++];
+        Problem& q = args.problem[i];
         q = Problem{};
         q.out = out[i];
         q.m = i < 2 ? z.hidden : z.out;
         q.n = i < 2 ? z.width : z.hidden;
-        q.part = part;
         q.a = q.b = i;
-        part += part_bytes(p, q.m, q.n) / sizeof(float);
     }
     args.steps = int(steps_of(z.rows));
-    return args.problems > 0 ? run<kWeights>(z.planes, a, b, 3, args, p, s) : FMD_OK;
+    if (dgate == nullptr && dup == nullptr && ddown == nullptr) return FMD_OK;
+    return run<kWeights>(z.planes, a, b, 3, args, p, s);
 }
 
 }  // extern "C"

@@ -39,33 +39,26 @@ def _problem(x, gate, up, down, activation) -> FmdFeedForward:
                           TYPES[x.dtype], activation)
 
 
-def _bytes(problem: FmdFeedForward, backward: bool) -> tuple[int, int]:
-    kept, workspace = c_size_t(), c_size_t()
-    call("fmd_gated_feed_forward_bytes", problem, backward, kept, workspace)
-    return kept.value, workspace.value
-
-
-def _room(size: int, device) -> Tensor | None:
-    return torch.empty(size, device=device, dtype=torch.uint8) if size else None
-
-
 def _forward(x, gate, up, down, activation, keep):
     device = x.device
     y = torch.empty(x.shape[0], down.shape[0], device=device, dtype=x.dtype)
     problem = _problem(x, gate, up, down, activation)
-    size, more = _bytes(problem, False)
-    if keep:
-        size, _ = _bytes(problem, True)
-    kept, workspace = _room(size, device), _room(more, device)
-    call("fmd_gated_feed_forward", problem, y.data_ptr(), keep, ptr(kept), size, ptr(workspace), more,
+    kept, forward, backward = c_size_t(), c_size_t(), c_size_t()
+    call("fmd_gated_feed_forward_bytes", problem, keep, kept, forward, backward)
+    size, more = kept.value, forward.value
+    # as scratch of the call the two are one buffer (sizes are multiples of 256)
+    room = torch.empty(size if keep else size + more, device=device, dtype=torch.uint8)
+    workspace = torch.empty(more, device=device, dtype=torch.uint8) if keep and more else None
+    start = room.data_ptr()
+    call("fmd_gated_feed_forward", problem, y.data_ptr(), keep, start, size, ptr(workspace) if keep else start + size, more,
          _lib.flags_word(device).data_ptr(), stream(device))
-    return y, kept
+    return y, room, backward.value
 
 
 class _GatedFeedForward(Function):
     @staticmethod
     def forward(ctx, x, gate, up, down, activation):
-        y, kept = _forward(x, gate, up, down, activation, True)
+        y, kept, ctx.size = _forward(x, gate, up, down, activation, True)
         ctx.save_for_backward(x, gate, up, down, kept)
         ctx.activation = activation
         return y
@@ -78,11 +71,10 @@ class _GatedFeedForward(Function):
         g = _rows(g)
         grads = [torch.empty(t.shape, device=device, dtype=t.dtype) if need else None
                  for t, need in zip(like, ctx.needs_input_grad)]
-        problem = _problem(x, gate, up, down, ctx.activation)
-        _, size = _bytes(problem, True)
-        workspace = _room(size, device)
-        call("fmd_gated_feed_forward_bwd", problem, ptr(kept), 0 if kept is None else kept.numel(), g.data_ptr(), g.stride(0),
-             *(ptr(t) for t in grads), ptr(workspace), size, _lib.flags_word(device).data_ptr(), stream(device))
+        workspace = torch.empty(ctx.size, device=device, dtype=torch.uint8)
+        call("fmd_gated_feed_forward_bwd", _problem(x, gate, up, down, ctx.activation), kept.data_ptr(), kept.numel(),
+             g.data_ptr(), g.stride(0), *(ptr(t) for t in grads), workspace.data_ptr(), ctx.size,
+             _lib.flags_word(device).data_ptr(), stream(device))
         return *first_order("gated_feed_forward", grads, inputs), None
 
 
@@ -98,7 +90,7 @@ def gated_feed_forward(x: Tensor, gate: Tensor, up: Tensor, down: Tensor, *, act
     held in 32 bits; in bfloat16 the gated product and the gradients of the two projections are rounded to bfloat16 as
     operands of the next product, each of which costs a result about as much as its own rounding. In float32 each product
     is six of bfloat16 planes; an infinity gives NaN where the formula may have an infinity. For the backward pass a call
-    keeps 10 bytes a row and hidden unit (float32: 14, and one and a half times the bytes of x and the weights)."""
+    keeps 6.5 bytes a row and hidden unit (float32: 14, and one and a half times the bytes of x and the weights)."""
     _lib.require_cuda(x, gate, up, down)
     if x.dim() < 1 or gate.dim() != 2 or up.shape != gate.shape or down.dim() != 2 or x.shape[-1] != gate.shape[1] \
             or down.shape[1] != gate.shape[0]:
@@ -122,7 +114,7 @@ def gated_feed_forward(x: Tensor, gate: Tensor, up: Tensor, down: Tensor, *, act
         if (trains and torch.is_grad_enabled()) or has_tangent(x, gate, up, down):
             y = _GatedFeedForward.apply(*args)
         else:
-            y, _ = _forward(*args, False)
+            y = _forward(*args, False)[0]
     return y if x.dim() == 2 else y.view(shape)
 
 

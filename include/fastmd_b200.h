@@ -1143,12 +1143,10 @@ typedef struct fmd_feed_forward {
 } fmd_feed_forward;
 
 /* From the sizes alone: `kept`, the bytes that the forward pass fills (with
- * backward = 1 for fmd_gated_feed_forward_bwd, else as scratch of its own),
- * and `workspace`: of the forward pass (backward = 0) or of the backward pass
- * (1). Both buffers start at a multiple of 16 bytes. The forward pass's
- * workspace is the same whether it keeps or not. */
-FMD_API fmd_status fmd_gated_feed_forward_bytes(const fmd_feed_forward* problem, int32_t backward, size_t* kept,
-                                                size_t* workspace);
+ * keep = 1 for fmd_gated_feed_forward_bwd, else as scratch of its own), and
+ * the workspaces of both passes. The buffers start at multiples of 16 bytes. */
+FMD_API fmd_status fmd_gated_feed_forward_bytes(const fmd_feed_forward* problem, int32_t keep, size_t* kept,
+                                                size_t* forward, size_t* backward);
 
 /* y [rows, out] contiguous. keep = 1: `kept` is left for the backward pass.
  * FP32 sums, deterministic; h = act(..) * (..) is rounded to the type before
