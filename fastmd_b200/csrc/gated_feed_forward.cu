@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                     const uint32_t at = tmem + lanes + uint32_t(unit & 1) * 256u;
 #pragma unroll
                     for (int u = 0; u < kUnits; ++u) {
-                        if (group + u * kGroups >= units) break;
+                        if (KIND != kHidden && group + u * kGroups >= units) break;
 #pragma unroll
                         for (int j = 0; j < W; j += 16) {
                             const int col = (group + u * kGroups) * kStep + (KIND == kUp && j >= W / 2 ? g.bn / 2 + j - W / 2 : j);
@@ -634,10 +634,10 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                 if (!ok) break;
 #pragma unroll
                 for (int u = 0; u < kUnits; ++u) {
-                    if (group + u * kGroups >= units) break;
+                    if (KIND != kHidden && group + u * kGroups >= units) break;
                     const int64_t col = n0 + (group + u * kGroups) * kStep;
                     if constexpr (KIND == kHidden)
-                        spread(q, row0, rows, col, group + (u + 1) * kGroups < units ? col + kGroups * kStep : q.n, sum[u]);
+                        spread(q, row0, rows, col, u + 1 < kUnits ? col + kGroups * kStep : q.n, sum[u]);
                     else
                         finish(q, p, row0, rows, col, sum[u]);
                 }
@@ -741,7 +741,7 @@ struct Plan {
     size_t bytes() const { return splits > 1 ? size_t(tiles - whole) * splits * kM * bn * sizeof(float) : 0; }
 };
 
-// The time of a launch in steps of 128 x 256 x 64, about 0.3 us each: rounds of blocks, each its tile's steps and, besides,
+// The time of a launch in steps of 128 x 256 x 64, about 0.4 us each: rounds of blocks, each its tile's steps and, besides,
 // about six for its start and end. Tiles are shared out along the inner index where that ends sooner: all of them, or those
 // of the last round, which do not fill the GPU; the shares' sums are written and read again. unit: bn is a multiple of it
 // (panels of 64 columns where the rows of B are the inner index; else any 32, so that few rows' weights are read by all
@@ -752,7 +752,8 @@ Plan plan(const int64_t* m, const int64_t* n, int problems, int64_t steps, int p
     for (int bn = unit; bn <= (planes == 1 ? 256 : 128); bn += unit) {
         int64_t tiles = 0;
         for (int i = 0; i < problems; ++i) tiles += ((m[i] + kM - 1) / kM) * ((n[i] + bn - 1) / bn);
-        const double step = (planes == 1 ? 1.0 : 6.0) * (0.25 + 0.75 * bn / 256.0);
+        // narrower tiles wait for their operands and barriers all the same (steps of 64 columns: 0.39 us, of 256: 0.45)
+        const double step = planes == 1 ? 0.7 + 0.3 * bn / 256.0 : 1.0 + 4.0 * bn / 256.0;
         for (int full = 0; full < (can_split && tiles > kNumSMs ? 2 : 1); ++full) {
             const int64_t whole = full ? tiles / kNumSMs * kNumSMs : 0, rest = tiles - whole;
             const double before = whole / kNumSMs * (steps * step + 6.0);
@@ -761,7 +762,7 @@ Plan plan(const int64_t* m, const int64_t* n, int problems, int64_t steps, int p
                                  (splits == 1 || (4 * splits <= steps && rest * (splits - 1) < 4 * kNumSMs)); ++splits) {
                 const int64_t rounds = (rest * splits + kNumSMs - 1) / kNumSMs;
                 const double moved = (2.0 * splits + 1.0) * rest * kM * bn * 4.0;
-                const double sums = splits > 1 ? 10.0 + moved / 6.5e6 / 0.3 : 0.0;
+                const double sums = splits > 1 ? 10.0 + moved / 6.5e6 / 0.4 : 0.0;
                 const double time = before + rounds * (((steps + splits - 1) / splits) * step + 6.0) + sums;
                 if (time < least) {
                     least = time;
@@ -1077,7 +1078,7 @@ fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kep
         args.problem[0].n = z.hidden;
         args.steps = int(steps_of(z.out));
         st = run<kHidden>(z.planes, &gm, &in.down, 1, args,
-                          plan(&z.rows, &z.hidden, 1, args.steps, z.planes, 64, false), s);
+                          plan(&z.rows, &z.hidden, 1, args.steps, z.planes, z.planes == 1 ? 64 : 128, false), s);
         if (st != FMD_OK) return st;
     }
     const Matrix da{own + w.da, z.rows, z.hidden, z.hidden_row, z.planes}, db{own + w.db, z.rows, z.hidden, z.hidden_row, z.planes};

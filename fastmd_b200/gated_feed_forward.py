@@ -92,30 +92,32 @@ def gated_feed_forward(x: Tensor, gate: Tensor, up: Tensor, down: Tensor, *, act
     is six of bfloat16 planes; an infinity gives NaN where the formula may have an infinity. For the backward pass a call
     keeps 6.5 bytes a row and hidden unit (float32: 14, and one and a half times the bytes of x and the weights)."""
     _lib.require_cuda(x, gate, up, down)
-    if x.dim() < 1 or gate.dim() != 2 or up.shape != gate.shape or down.dim() != 2 or x.shape[-1] != gate.shape[1] \
-            or down.shape[1] != gate.shape[0]:
+    lead, weights, last = x.shape, gate.shape, down.shape
+    if x.dim() < 1 or gate.dim() != 2 or up.shape != weights or down.dim() != 2 or lead[-1] != weights[1] \
+            or last[1] != weights[0]:
         raise ValueError("x must be [.., width], gate and up [hidden, width] and down [out, hidden], got "
-                         f"{tuple(x.shape)}, {tuple(gate.shape)}, {tuple(up.shape)} and {tuple(down.shape)}")
-    if x.dtype not in TYPES or not x.dtype == gate.dtype == up.dtype == down.dtype:
+                         f"{tuple(lead)}, {tuple(weights)}, {tuple(up.shape)} and {tuple(last)}")
+    kind = x.dtype
+    if kind not in TYPES or gate.dtype != kind or up.dtype != kind or down.dtype != kind:
         raise ValueError("x and the weights must all be float32 or bfloat16, got "
-                         f"{x.dtype}, {gate.dtype}, {up.dtype} and {down.dtype}")
-    if not x.device == gate.device == up.device == down.device:
+                         f"{kind}, {gate.dtype}, {up.dtype} and {down.dtype}")
+    index = x.get_device()
+    if gate.get_device() != index or up.get_device() != index or down.get_device() != index:
         raise ValueError("x and the weights must be on one device")
-    if min(gate.shape) < 1 or down.shape[0] < 1 or max(*gate.shape, down.shape[0]) > 2 ** 20:
-        raise ValueError(f"width, hidden and out must be between 1 and 2^20, got {gate.shape[1]}, {gate.shape[0]} and "
-                         f"{down.shape[0]}")
+    hidden, width, out = *weights, last[0]
+    if not (0 < width <= 2 ** 20 and 0 < hidden <= 2 ** 20 and 0 < out <= 2 ** 20):
+        raise ValueError(f"width, hidden and out must be between 1 and 2^20, got {width}, {hidden} and {out}")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
-    shape = (*x.shape[:-1], down.shape[0])
-    flat = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+    flat = x if len(lead) == 2 else x.reshape(-1, width)
     args = (_rows(flat), _rows(gate), _rows(up), _rows(down), ACTIVATIONS[activation])
-    trains = x.requires_grad or gate.requires_grad or up.requires_grad or down.requires_grad
     with on_device(x.device):
-        if (trains and torch.is_grad_enabled()) or has_tangent(x, gate, up, down):
+        if (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or up.requires_grad or down.requires_grad)) \
+                or has_tangent(x, gate, up, down):
             y = _GatedFeedForward.apply(*args)
         else:
             y = _forward(*args, False)[0]
-    return y if x.dim() == 2 else y.view(shape)
+    return y if len(lead) == 2 else y.view(*lead[:-1], out)
 
 
 __all__ = ["gated_feed_forward"]
