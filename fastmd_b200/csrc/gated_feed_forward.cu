@@ -23,6 +23,11 @@
 // each), one thread of another issues the products, 8 or 16 take the sums from one of two accumulators in TMEM while the
 // other one is filled: thread = row and part of the columns.
 //
+// Pairs of blocks: where a launch has enough tiles, the two SMs of a cluster work on 256 x 256 together, each with its own 128
+// rows of A and half of B's columns, since one block's tile of 128 x 256 takes 48 KB a step of 512 cycles of products and an
+// SM gets about 64 bytes a cycle (1,230 TFLOP/s). The first block of the pair issues the products of both; copies of both
+// arrive on its barriers, its commits on both blocks'.
+//
 // Every wait is bounded: on expiry the block raises FMD_FLAG_WAIT_TIMEOUT, waits (bounded) for its copies and products in
 // flight, frees its TMEM and returns.
 
@@ -65,6 +70,7 @@ struct Args {
     int32_t problems;
     int32_t tiles, whole, splits;  // tiles of all problems; those from `whole` on are shared out along the inner index
     float* part;                   // [tiles - whole][splits][128][bn]: the shares' sums
+    int32_t tile_m;                // rows of a tile: 128, of a pair 256
     int32_t steps, turn;  // of 64 along the inner index; from step `turn` on the second pair of maps (kInput)
     int32_t bn, slots, act;
     int32_t tile_a;  // bytes of A's tile in a slot
@@ -90,29 +96,100 @@ struct Ctrl {
     int32_t abort;
 };
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(su32(bar))
-        : "memory");
-}
-
 __device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[16]) { tmem_load16(at, v); }
 __device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[32]) { tmem_load32(at, v); }
 __device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[64]) { tmem_load64(at, v); }
 
-// Two steps of 16 of D (+)= A B^T; `astep`, `bstep`: how far a step is, in descriptor units.
-template <int ASTEP, int BSTEP>
+#define FMD_MMA2(GROUP)                                                                                            \
+    asm volatile(                                                                                                  \
+        "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 u, v, w, z;\n\t"                                         \
+        "setp.ne.b32 p, %5, 0;\n\tadd.u32 x, %1, %6;\n\tadd.u32 y, %2, %7;\n\t"                                     \
+        "mov.b64 u, {%1, %3};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 w, {x, %3};\n\tmov.b64 z, {y, %3};\n\t"             \
+        "tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], u, v, %4, p;\n\t"                                         \
+        "tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], w, z, %4, 1;\n\t}" ::"r"(d),                              \
+        "r"(a), "r"(b), "r"(kDescHigh), "r"(idesc), "r"(add), "n"(ASTEP), "n"(BSTEP)                               \
+        : "memory")
+
+// Two steps of 16 of D (+)= A B^T; ASTEP, BSTEP: how far a step is, in descriptor units. PAIR: of both blocks' rows.
+template <bool PAIR, int ASTEP, int BSTEP>
 __device__ __forceinline__ void mma2(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 u, v, w, z;\n\t"
-        "setp.ne.b32 p, %5, 0;\n\tadd.u32 x, %1, %6;\n\tadd.u32 y, %2, %7;\n\t"
-        "mov.b64 u, {%1, %3};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 w, {x, %3};\n\tmov.b64 z, {y, %3};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], u, v, %4, p;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], w, z, %4, 1;\n\t}" ::"r"(d),
-        "r"(a), "r"(b), "r"(kDescHigh), "r"(idesc), "r"(add), "n"(ASTEP), "n"(BSTEP)
-        : "memory");
+    if constexpr (PAIR) FMD_MMA2("2");
+    else FMD_MMA2("1");
 }
+
+// What a single block does by itself and a pair together.
+template <bool PAIR>
+struct Group {
+    __device__ static uint32_t rank() {
+        uint32_t r = 0;
+        if (PAIR) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+        return r;
+    }
+    // the first block's copy of a barrier
+    __device__ static uint32_t first(uint64_t* bar) {
+        uint32_t a = su32(bar);
+        if (PAIR) asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(a));
+        return a;
+    }
+    __device__ static void sync() {
+        __syncwarp();
+        if (PAIR)
+            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        else
+            __syncthreads();
+    }
+    __device__ static void load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+        if (PAIR)
+            asm volatile(
+                "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
+                "{%2, %3, %4}], [%5];" ::"r"(dst),
+                "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+                : "memory");
+        else
+            asm volatile(
+                "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+                "[%5];" ::"r"(dst),
+                "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+                : "memory");
+    }
+    // all products so far: an arrival on the barrier, in both blocks
+    __device__ static void commit(uint64_t* bar) {
+        if (PAIR)
+            asm volatile(
+                "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                    su32(bar)),
+                "h"(uint16_t(3))
+                : "memory");
+        else
+            tc_commit(bar);
+    }
+    // a warp's arrival on the first block's barrier
+    __device__ static void arrive(uint64_t* bar) {
+        __syncwarp();
+        if ((threadIdx.x & 31) != 0) return;
+        if (PAIR)
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(first(bar)) : "memory");
+        else
+            mbar_arrive(bar);
+    }
+    __device__ static void alloc(uint32_t* address) {
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(address)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            tmem_alloc<512>(address);
+        }
+    }
+    __device__ static void free(uint32_t address) {
+        if (PAIR) {
+            __syncwarp();
+            tc_fence_after();
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(address) : "memory");
+        } else {
+            tmem_free<512>(address);
+        }
+    }
+};
 
 // The place of a block's turn: its problem, rows and columns, the steps of its share of the inner index, and which of the
 // shares it is (part: its place among them; -1: a whole tile).
@@ -306,16 +383,20 @@ __device__ __forceinline__ void put_result(unsigned char* scratch, const float (
 }
 
 // W: columns of the sums that a warp takes at a time (kUp: half of them a's, half b's).
-template <int KIND, int P, int W>
+template <int KIND, int P, int W, bool PAIR>
 __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const __grid_constant__ Maps maps, const Args g) {
     using S = Shape<KIND, P>;
+    using G = Group<PAIR>;
     constexpr bool kColumnsA = KIND == kWeights, kColumnsB = KIND == kHidden || KIND == kInput || KIND == kWeights;
     extern __shared__ unsigned char raw[];
     const uint32_t ring = (su32(raw) + 1023u) & ~1023u;
     __shared__ Ctrl ctl;
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t tile_b = uint32_t(g.bn) * 128u, tile_a = g.tile_a, slot_bytes = P * (tile_a + tile_b);
+    const uint32_t rank = G::rank();
+    const int first_turn = PAIR ? int(blockIdx.x) / 2 : int(blockIdx.x), turns = PAIR ? int(gridDim.x) / 2 : int(gridDim.x);
+    const int columns = PAIR ? g.bn / 2 : g.bn;  // of B in this block
+    const uint32_t tile_b = uint32_t(columns) * 128u, tile_a = g.tile_a, slot_bytes = P * (tile_a + tile_b);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMostSlots; ++i) {
@@ -324,15 +405,15 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctl.sums[i], 1);
-            mbar_init(&ctl.taken[i], S::kWarps);
+            mbar_init(&ctl.taken[i], PAIR ? 2 * S::kWarps : S::kWarps);
         }
         mbar_init(&ctl.drain, 1);
         ctl.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == S::kWarps + 1) tmem_alloc<512>(&ctl.tmem);
+    if (warp == S::kWarps + 1) G::alloc(&ctl.tmem);
     tc_fence_before();
-    __syncthreads();
+    G::sync();
     tc_fence_after();
     const uint32_t tmem = ctl.tmem;
 
@@ -341,18 +422,19 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             int slot = 0;
             uint32_t phase = 0, armed = 0;  // armed: slots with a copy that nobody may have waited for
             bool ok = true;
-            for (int t = blockIdx.x; t < turns_of(g) && ok; t += gridDim.x) {
+            for (int t = first_turn; t < turns_of(g) && ok; t += turns) {
                 const Place p = place_of(g, t);
                 const Problem& q = g.problem[p.problem];
                 if (!wanted<KIND>(q)) continue;
-                const int m0 = p.m * kM, n0 = p.n * (KIND == kUp ? g.bn / 2 : g.bn);
+                const int m0 = p.m * g.tile_m + int(rank) * kM, n0 = p.n * (KIND == kUp ? g.bn / 2 : g.bn) +
+                                                                     (PAIR && KIND != kUp ? int(rank) * columns : 0);
                 for (int step = p.from; step < p.to; ++step) {
                     if (!mbar_wait(&ctl.empty[slot], phase ^ 1u, abort)) {
                         ok = false;
                         break;
                     }
-                    uint64_t* bar = &ctl.full[slot];
-                    mbar_expect_tx(bar, slot_bytes);
+                    const uint32_t bar = G::first(&ctl.full[slot]);
+                    if (!PAIR || rank == 0) mbar_expect_tx(&ctl.full[slot], PAIR ? 2 * slot_bytes : slot_bytes);
                     armed |= 1u << slot;
                     const uint32_t at = ring + uint32_t(slot) * slot_bytes;
                     const bool second = KIND == kInput && step >= g.turn;
@@ -361,19 +443,20 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                     for (int i = 0; i < P; ++i) {
                         const uint32_t a = at + P * tile_b + uint32_t(i) * tile_a, b = at + uint32_t(i) * tile_b;
                         if (kColumnsA) {
-                            tma_load_3d(a, ma, bar, m0, k0, i);
-                            tma_load_3d(a + kPanel, ma, bar, m0 + 64, k0, i);
+                            G::load(a, ma, bar, m0, k0, i);
+                            G::load(a + kPanel, ma, bar, m0 + 64, k0, i);
                         } else {
-                            tma_load_3d(a, ma, bar, k0, m0, i);
+                            G::load(a, ma, bar, k0, m0, i);
                         }
-                        if (KIND == kUp) {
-                            tma_load_3d(b, &maps.b[0], bar, k0, n0, i);
-                            tma_load_3d(b + tile_b / 2, &maps.b[1], bar, k0, n0, i);
+                        if (KIND == kUp && PAIR) {
+                            G::load(b, &maps.b[rank], bar, k0, n0, i);
+                        } else if (KIND == kUp) {
+                            G::load(b, &maps.b[0], bar, k0, n0, i);
+                            G::load(b + tile_b / 2, &maps.b[1], bar, k0, n0, i);
                         } else if (kColumnsB) {
-                            for (int c = 0; c < g.bn / 64; ++c)
-                                tma_load_3d(b + c * kPanel, mb, bar, n0 + 64 * c, k0, i);
+                            for (int c = 0; c < columns / 64; ++c) G::load(b + c * kPanel, mb, bar, n0 + 64 * c, k0, i);
                         } else {
-                            tma_load_3d(b, mb, bar, k0, n0, i);
+                            G::load(b, mb, bar, k0, n0, i);
                         }
                     }
                     if (++slot == g.slots) {
@@ -384,18 +467,21 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             }
             // the block ends after the copies in flight and, where all went well, after the products that read them
             for (int i = 0; i < g.slots; ++i) {
-                const uint32_t turns = phase + (i < slot ? 1u : 0u);  // parity of the number of uses of slot i
+                const uint32_t uses = phase + (i < slot ? 1u : 0u);  // parity of the number of uses of slot i
                 if (!(armed >> i & 1u)) continue;
-                if (ok) ok = mbar_wait(&ctl.empty[i], (turns ^ 1u) & 1u, abort);
-                if (!ok) mbar_wait(&ctl.full[i], (turns ^ 1u) & 1u, abort, true);
+                if (ok) ok = mbar_wait(&ctl.empty[i], (uses ^ 1u) & 1u, abort);
+                if (!ok && rank == 0) mbar_wait(&ctl.full[i], (uses ^ 1u) & 1u, abort, true);
             }
+            if (PAIR && !ok)  // copies whose barrier the other block has not armed or does not look at
+                for (const unsigned long long t0 = global_ns(); global_ns() - t0 < 1000000ull;) {
+                }
         }
-    } else if (warp > S::kWarps) {
+    } else if (warp > S::kWarps && rank == 0) {
         const uint32_t base = uniform(tmem), first = uniform(ring), bytes = uniform(slot_bytes), b_bytes = uniform(tile_b),
                        a_bytes = uniform(tile_a);
         const int slots = uniform(g.slots), bn = uniform(g.bn);
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (kColumnsA ? 1u << 15 : 0u) |
-                               (kColumnsB ? 1u << 16 : 0u) | (uint32_t(bn >> 3) << 17) | (uint32_t(kM >> 4) << 24);
+                               (kColumnsB ? 1u << 16 : 0u) | (uint32_t(bn >> 3) << 17) | (uint32_t((PAIR ? 2 * kM : kM) >> 4) << 24);
         constexpr int kStepA = kColumnsA ? 128 : 2, kStepB = kColumnsB ? 128 : 2;
         auto desc = [](uint32_t at, bool columns) {
             return ((at & 0x3FFFFu) >> 4) | (columns ? (kPanel >> 4) << 16 : 1u << 16);
@@ -403,7 +489,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
         int slot = 0, unit = 0;
         uint32_t phase = 0;
         bool ok = true, issued = false;
-        for (int t = blockIdx.x; t < turns_of(g) && ok; t += gridDim.x) {
+        for (int t = first_turn; t < turns_of(g) && ok; t += turns) {
             const Place p = place_of(g, t);
             if (!wanted<KIND>(g.problem[p.problem])) continue;
             const int from = uniform(p.from), to = uniform(p.to);
@@ -420,20 +506,20 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                         const uint32_t a = desc(at + P * b_bytes, kColumnsA), b = desc(at, kColumnsB);
                         const bool add = step > start;
                         if (P == 1) {
-                            mma2<kStepA, kStepB>(d, a, b, idesc, add);
-                            mma2<kStepA, kStepB>(d, a + 2 * kStepA, b + 2 * kStepB, idesc, true);
+                            mma2<PAIR, kStepA, kStepB>(d, a, b, idesc, add);
+                            mma2<PAIR, kStepA, kStepB>(d, a + 2 * kStepA, b + 2 * kStepB, idesc, true);
                         } else {  // the small products first, into sums of their own
                             constexpr int kPa[6] = {2, 1, 0, 1, 0, 0}, kPb[6] = {0, 1, 2, 0, 1, 0};
 #pragma unroll
                             for (int i = 0; i < 6; ++i) {
                                 const uint32_t x = a + kPa[i] * (a_bytes >> 4), y = b + kPb[i] * (b_bytes >> 4);
                                 const uint32_t to_sum = i < 5 ? d + 128 : d;
-                                mma2<kStepA, kStepB>(to_sum, x, y, idesc, add || (i > 0 && i < 5));
-                                mma2<kStepA, kStepB>(to_sum, x + 2 * kStepA, y + 2 * kStepB, idesc, true);
+                                mma2<PAIR, kStepA, kStepB>(to_sum, x, y, idesc, add || (i > 0 && i < 5));
+                                mma2<PAIR, kStepA, kStepB>(to_sum, x + 2 * kStepA, y + 2 * kStepB, idesc, true);
                             }
                         }
-                        tc_commit(&ctl.empty[slot]);
-                        if (step + 1 == end) tc_commit(&ctl.sums[unit & 1]);
+                        G::commit(&ctl.empty[slot]);
+                        if (step + 1 == end) G::commit(&ctl.sums[unit & 1]);
                     }
                     issued = true;
                     if (++slot == slots) {
@@ -445,10 +531,10 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             }
         }
         if (!ok && issued) {  // the products in flight end before TMEM is freed
-            if (elect_one()) tc_commit(&ctl.drain);
+            if (elect_one()) G::commit(&ctl.drain);
             warp_wait(&ctl.drain, 0, abort, true);
         }
-    } else {
+    } else if (warp < S::kWarps) {
         using T = typename std::conditional<P == 1, __nv_bfloat16, float>::type;
         constexpr int kGroups = S::kWarps / 4, kStep = KIND == kUp ? W / 2 : W;  // kStep: columns of the result a unit
         const int group = warp >> 2, units = g.bn / W;
@@ -467,7 +553,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
         };
         auto done = [&]() {
             tc_fence_before();
-            warp_arrive(&ctl.taken[unit & 1]);
+            G::arrive(&ctl.taken[unit & 1]);
             ++unit;
         };
         // kHidden, float32: the factors of the next 32 columns are on their way while the last ones are stored
@@ -543,17 +629,17 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             } else if constexpr (KIND != kHidden) {
                 const int columns = int(max(int64_t(0), min(int64_t(W), q.n - col)));
                 if (p.part >= 0)
-                    put_result<W>(scratch, v, g.part + (int64_t(p.part) * kM + (warp & 3) * 32) * g.bn + (col - int64_t(p.n) * g.bn),
+                    put_result<W>(scratch, v, g.part + (int64_t(p.part) * g.tile_m + rank * kM + (warp & 3) * 32) * g.bn + (col - int64_t(p.n) * g.bn),
                                   g.bn, rows, W, true);
                 else
                     put_result<W>(scratch, v, static_cast<T*>(q.out) + row0 * q.n + col, q.n, rows, columns, q.n % 8 == 0);
             }
         };
-        for (int t = blockIdx.x; t < turns_of(g) && ok; t += gridDim.x) {
+        for (int t = first_turn; t < turns_of(g) && ok; t += turns) {
             const Place p = place_of(g, t);
             const Problem& q = g.problem[p.problem];
             if (!wanted<KIND>(q)) continue;
-            const int64_t row0 = int64_t(p.m) * kM + (warp & 3) * 32, n0 = int64_t(p.n) * (KIND == kUp ? g.bn / 2 : g.bn);
+            const int64_t row0 = int64_t(p.m) * g.tile_m + rank * kM + (warp & 3) * 32, n0 = int64_t(p.n) * (KIND == kUp ? g.bn / 2 : g.bn);
             const int rows = int(max(int64_t(0), min(int64_t(32), q.m - row0)));
             if constexpr (KIND == kHidden) {
                 if (P == 1) {
@@ -646,8 +732,8 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
     }
 
     tc_fence_before();
-    __syncthreads();
-    if (warp == S::kWarps + 1) tmem_free<512>(tmem);
+    G::sync();
+    if (warp == S::kWarps + 1) G::free(tmem);
     if (threadIdx.x == 0 && ctl.abort) raise_flag(g.flags, FMD_FLAG_WAIT_TIMEOUT);
 }
 
@@ -691,12 +777,12 @@ __global__ void __launch_bounds__(256) add_kernel(const Args g) {
     const Problem& q = g.problem[p.problem];
     if (q.out == nullptr) return;
     const int per = g.bn / 4, at = int(blockIdx.x) * 256 + int(threadIdx.x), row = at / per, col = (at - row * per) * 4;
-    if (row >= kM) return;
-    const float* part = g.part + (int64_t(blockIdx.y) * g.splits * kM + row) * g.bn + col;
+    if (row >= g.tile_m) return;
+    const float* part = g.part + (int64_t(blockIdx.y) * g.splits * g.tile_m + row) * g.bn + col;
     float4 sum = f4_zero();
 #pragma unroll 4
-    for (int z = 0; z < g.splits; ++z) sum = f4_add(sum, *reinterpret_cast<const float4*>(part + int64_t(z) * kM * g.bn));
-    const int64_t m = int64_t(p.m) * kM + row, n = int64_t(p.n) * g.bn + col;
+    for (int z = 0; z < g.splits; ++z) sum = f4_add(sum, *reinterpret_cast<const float4*>(part + int64_t(z) * g.tile_m * g.bn));
+    const int64_t m = int64_t(p.m) * g.tile_m + row, n = int64_t(p.n) * g.bn + col;
     if (m >= q.m) return;
     T* out = static_cast<T*>(q.out) + m * q.n + n;
     const float v[4] = {sum.x, sum.y, sum.z, sum.w};
@@ -735,42 +821,48 @@ fmd_status encode(CUtensorMap* map, const Matrix& x, int box_rows) {
 
 int64_t round_up(int64_t v, int64_t unit) { return (v + unit - 1) / unit * unit; }
 
-// How a launch runs: columns of a tile, the tiles that are not shared out, shares of the others along the inner index.
+// How a launch runs: rows (256: pairs of blocks) and columns of a tile, the tiles that are not shared out, shares of the
+// others along the inner index.
 struct Plan {
-    int bn, tiles, whole, splits;
-    size_t bytes() const { return splits > 1 ? size_t(tiles - whole) * splits * kM * bn * sizeof(float) : 0; }
+    int tile_m, bn, tiles, whole, splits;
+    size_t bytes() const { return splits > 1 ? size_t(tiles - whole) * splits * tile_m * bn * sizeof(float) : 0; }
 };
 
 // The time of a launch in steps of 128 x 256 x 64, about 0.4 us each: rounds of blocks, each its tile's steps and, besides,
-// about six for its start and end. Tiles are shared out along the inner index where that ends sooner: all of them, or those
-// of the last round, which do not fill the GPU; the shares' sums are written and read again. unit: bn is a multiple of it
-// (panels of 64 columns where the rows of B are the inner index; else any 32, so that few rows' weights are read by all
-// SMs alike).
+// about six for its start and end. Narrower tiles wait for their operands and barriers all the same (steps of 64 columns:
+// 0.39 us, of 256: 0.45); a pair's step of 256 x 256 takes 0.75 of one. Tiles are shared out along the inner index where that
+// ends sooner: all of them, or those of the last round, which do not fill the GPU; the shares' sums are written and read
+// again. unit: bn is a multiple of it (panels of 64 columns where the rows of B are the inner index; else any 32, so that few
+// rows' weights are read by all SMs alike).
 Plan plan(const int64_t* m, const int64_t* n, int problems, int64_t steps, int planes, int unit, bool can_split) {
-    Plan best{128, 0, 0, 1};
+    Plan best{kM, 128, 0, 0, 1};
     double least = 1e300;
-    for (int bn = unit; bn <= (planes == 1 ? 256 : 128); bn += unit) {
+    auto look = [&](int tile_m, int bn) {
         int64_t tiles = 0;
-        for (int i = 0; i < problems; ++i) tiles += ((m[i] + kM - 1) / kM) * ((n[i] + bn - 1) / bn);
-        // narrower tiles wait for their operands and barriers all the same (steps of 64 columns: 0.39 us, of 256: 0.45)
-        const double step = planes == 1 ? 0.7 + 0.3 * bn / 256.0 : 1.0 + 4.0 * bn / 256.0;
-        for (int full = 0; full < (can_split && tiles > kNumSMs ? 2 : 1); ++full) {
-            const int64_t whole = full ? tiles / kNumSMs * kNumSMs : 0, rest = tiles - whole;
-            const double before = whole / kNumSMs * (steps * step + 6.0);
+        for (int i = 0; i < problems; ++i) tiles += ((m[i] + tile_m - 1) / tile_m) * ((n[i] + bn - 1) / bn);
+        const int64_t places = kNumSMs * kM / tile_m;
+        const double step = planes == 3 ? 1.0 + 4.0 * bn / 256.0 : tile_m > kM ? 0.75 : 0.7 + 0.3 * bn / 256.0;
+        for (int full = 0; full < (can_split && tiles > places ? 2 : 1); ++full) {
+            const int64_t whole = full ? tiles / places * places : 0, rest = tiles - whole;
+            const double before = whole / places * (steps * step + 6.0);
             // shares beyond four rounds of blocks even nothing out any more
             for (int splits = 1; splits <= (can_split ? 64 : 1) &&
-                                 (splits == 1 || (4 * splits <= steps && rest * (splits - 1) < 4 * kNumSMs)); ++splits) {
-                const int64_t rounds = (rest * splits + kNumSMs - 1) / kNumSMs;
-                const double moved = (2.0 * splits + 1.0) * rest * kM * bn * 4.0;
+                                 (splits == 1 || (4 * splits <= steps && rest * (splits - 1) < 4 * places)); ++splits) {
+                const int64_t rounds = (rest * splits + places - 1) / places;
+                const double moved = (2.0 * splits + 1.0) * rest * tile_m * bn * 4.0;
                 const double sums = splits > 1 ? 10.0 + moved / 6.5e6 / 0.4 : 0.0;
                 const double time = before + rounds * (((steps + splits - 1) / splits) * step + 6.0) + sums;
                 if (time < least) {
                     least = time;
-                    best = Plan{bn, int(tiles), int(splits > 1 ? whole : tiles), splits};
+                    best = Plan{tile_m, bn, int(tiles), int(splits > 1 ? whole : tiles), splits};
                 }
             }
         }
-    }
+    };
+    for (int bn = unit; bn <= (planes == 1 ? 256 : 128); bn += unit) look(kM, bn);
+    int64_t most = 0;
+    for (int i = 0; i < problems; ++i) most = m[i] > most ? m[i] : most;
+    if (planes == 1 && most > kM) look(2 * kM, 256);
     return best;
 }
 
@@ -780,16 +872,33 @@ struct Sizes {
     int64_t hidden_row, width_row, out_row;  // of the arrays made here
 };
 
-template <int KIND, int P, int W>
+template <int KIND, int P, int W, bool PAIR>
 fmd_status launch(const Maps& maps, Args& g, cudaStream_t s) {
     using S = Shape<KIND, P>;
-    const fmd_status st = grant_dynamic_smem((const void*)feed_kernel<KIND, P, W>, S::kBytes, true);
+    const fmd_status st = grant_dynamic_smem((const void*)feed_kernel<KIND, P, W, PAIR>, S::kBytes, true);
     if (st != FMD_OK) return st;
-    const int slots = int(S::kRing / (P * (g.tile_a + g.bn * 128)));
+    const int slots = int(S::kRing / (P * (g.tile_a + (PAIR ? g.bn / 2 : g.bn) * 128)));
     g.slots = slots < kMostSlots ? slots : kMostSlots;
-    const int64_t turns = g.whole + int64_t(g.tiles - g.whole) * g.splits;
-    feed_kernel<KIND, P, W><<<unsigned(turns < kNumSMs ? turns : kNumSMs), S::kThreads, S::kBytes, s>>>(maps, g);
-    return check_launch();
+    const int64_t turns = g.whole + int64_t(g.tiles - g.whole) * g.splits, places = PAIR ? kNumSMs / 2 : kNumSMs;
+    const unsigned blocks = unsigned((turns < places ? turns : places) * (PAIR ? 2 : 1));
+    if constexpr (!PAIR) {
+        feed_kernel<KIND, P, W, PAIR><<<blocks, S::kThreads, S::kBytes, s>>>(maps, g);
+        return check_launch();
+    } else {
+        cudaLaunchAttribute pair{};
+        pair.id = cudaLaunchAttributeClusterDimension;
+        pair.val.clusterDim.x = 2;
+        pair.val.clusterDim.y = pair.val.clusterDim.z = 1;
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(blocks);
+        config.blockDim = dim3(unsigned(S::kThreads));
+        config.dynamicSmemBytes = S::kBytes;
+        config.stream = s;
+        config.attrs = &pair;
+        config.numAttrs = 1;
+        const cudaError_t err = cudaLaunchKernelEx(&config, feed_kernel<KIND, P, W, PAIR>, maps, g);
+        return err == cudaSuccess ? check_launch() : record_cuda_error(err);
+    }
 }
 
 template <int KIND>
@@ -805,9 +914,10 @@ fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args&
         fmd_status st = FMD_OK;
         if (a[i].data != nullptr) st = encode(&maps.a[i], a[i], columns_a ? kK : rows);
         if (st == FMD_OK && b[i].data != nullptr)
-            st = encode(&maps.b[i], b[i], columns_b ? kK : KIND == kUp ? p.bn / 2 : p.bn);
+            st = encode(&maps.b[i], b[i], columns_b ? kK : KIND == kUp || p.tile_m > kM ? p.bn / 2 : p.bn);
         if (st != FMD_OK) return st;
     }
+    g.tile_m = p.tile_m;
     g.bn = p.bn;
     g.tiles = p.tiles;
     g.whole = p.whole;
@@ -815,15 +925,16 @@ fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args&
     for (int i = 0; i < g.problems; ++i) {
         Problem& q = g.problem[i];
         const int columns = KIND == kUp ? p.bn / 2 : p.bn;
-        q.m_tiles = int((q.m + kM - 1) / kM);
+        q.m_tiles = int((q.m + p.tile_m - 1) / p.tile_m);
         q.n_tiles = int((q.n + columns - 1) / columns);
     }
     constexpr int kWide = KIND == kUp || KIND == kHidden ? 32 : 64;
-    const fmd_status st = planes == 3   ? launch<KIND, 3, 32>(maps, g, s)
-                          : g.bn == 256 ? launch<KIND, 1, kWide>(maps, g, s)
-                                        : launch<KIND, 1, 32>(maps, g, s);
+    const fmd_status st = planes == 3       ? launch<KIND, 3, 32, false>(maps, g, s)
+                          : p.tile_m > kM   ? launch<KIND, 1, kWide, true>(maps, g, s)
+                          : g.bn == 256     ? launch<KIND, 1, kWide, false>(maps, g, s)
+                                            : launch<KIND, 1, 32, false>(maps, g, s);
     if (st != FMD_OK || p.splits == 1) return st;
-    const dim3 grid(unsigned((kM * p.bn / 4 + 255) / 256), unsigned(p.tiles - p.whole));
+    const dim3 grid(unsigned((p.tile_m * p.bn / 4 + 255) / 256), unsigned(p.tiles - p.whole));
     if (planes == 1) add_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(g);
     else add_kernel<float><<<grid, 256, 0, s>>>(g);
     return check_launch();
