@@ -62,6 +62,7 @@ struct Problem {
     void* out;
     int64_t m, n;
     int32_t a, b;  // maps
+    int32_t a_panels, b_panels;  // whether the operands' maps go by panels of 64 columns
     int32_t m_tiles, n_tiles;
 };
 
@@ -74,13 +75,18 @@ struct Args {
     int32_t steps, turn;  // of 64 along the inner index; from step `turn` on the second pair of maps (kInput)
     int32_t bn, slots, act;
     int32_t tile_a;  // bytes of A's tile in a slot
-    __nv_bfloat16 *h, *da, *db;  // [planes][rows][row]
-    // What the gradients are multiplied by, b act'(a) and act(a) [rows][row]: float32, or in 16 bits float16 times a power of
-    // two of each row's 16 columns, `unit` [row / 16][rows] (11 bits, over 2^-29 of the largest of the 16; else the rest of
-    // the kernel waits for memory, and one rounding to bfloat16 here would cost the gradients as much as their own)
+    // h, da and db in panels of 64 hidden units, [planes][panels][rows][64]: a warp's store and a tile's copy are each in one
+    // piece of memory. The last panel is filled up with zeros.
+    __nv_bfloat16 *h, *da, *db;
+    int64_t plane;  // values of a plane
+    int32_t panels;
+    // What the gradients are multiplied by, b act'(a) and act(a), as the threads hold it: blocks of 32 rows x 16 units,
+    // [unit / 16][row / 32][piece of 16 bytes][row % 32]. FP32; in 16 bits float16 times a power of two of each row's 16
+    // units, whose inverse is `unit` [unit / 16][row] (11 bits, for values over 2^-29 of the largest of the 16: a rounding to
+    // bfloat16 would cost the gradients as much as their own, and FP32 the kernels that wait for memory a fifth)
     void *slope, *level;
     float2* unit;
-    int64_t row, plane;
+    int32_t blocks;  // of 32 rows
     int32_t* flags;
 };
 
@@ -138,18 +144,18 @@ struct Group {
         else
             __syncthreads();
     }
-    __device__ static void load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    __device__ static void load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
         if (PAIR)
             asm volatile(
-                "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
-                "{%2, %3, %4}], [%5];" ::"r"(dst),
-                "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+                "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
+                "{%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
                 : "memory");
         else
             asm volatile(
-                "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-                "[%5];" ::"r"(dst),
-                "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+                "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+                "%5}], [%6];" ::"r"(dst),
+                "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
                 : "memory");
     }
     // all products so far: an arrival on the barrier, in both blocks
@@ -255,53 +261,6 @@ __device__ __forceinline__ void activate(int act, float a, float& value, float& 
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 
-// 32 columns of FP32 of 32 rows: the loads (a lane holds pieces of eight rows) ..
-__device__ __forceinline__ void fetch_rows(const float* from, int64_t stride, int rows, int pieces, float4 (&x)[8]) {
-    const int lane = threadIdx.x & 31, left = lane % 8 < pieces ? rows - lane / 8 : 0;
-    const float* p = from + (lane / 8) * stride + (lane % 8) * 4;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        x[i] = i * 4 < left ? ldg4(p) : f4_zero();
-        p += 4 * stride;
-    }
-}
-
-// .. and the turn to a row a lane.
-__device__ __forceinline__ void turn_rows(unsigned char* scratch, const float4 (&x)[8], float (&v)[32]) {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        *reinterpret_cast<float4*>(piece_at<8>(scratch, i * 4 + lane / 8, lane % 8)) = x[i];
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float4 y = *reinterpret_cast<const float4*>(piece_at<8>(scratch, lane, i));
-        v[4 * i] = y.x, v[4 * i + 1] = y.y, v[4 * i + 2] = y.z, v[4 * i + 3] = y.w;
-    }
-}
-
-// 32 columns of float16 of 32 rows in the same way: four lanes a row.
-__device__ __forceinline__ void fetch_halves(const __half* from, int64_t stride, int rows, int pieces, uint4 (&x)[4]) {
-    const int lane = threadIdx.x & 31, left = lane % 4 < pieces ? rows - lane / 4 : 0;
-    const __half* p = from + (lane / 4) * stride + (lane % 4) * 8;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[i] = i * 8 < left ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
-        p += 8 * stride;
-    }
-}
-
-__device__ __forceinline__ void turn_halves(unsigned char* scratch, uint4 (&x)[4]) {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *piece_at<4>(scratch, i * 8 + lane / 4, lane % 4) = x[i];
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = *piece_at<4>(scratch, lane, i);
-}
-
 // The power of two that takes 16 values to float16's upper range, and those values; `unit`: its inverse.
 __device__ __forceinline__ void pack_halves(const float* v, uint4 (&w)[2], float& unit) {
     float most = 0.0f;
@@ -321,7 +280,11 @@ __device__ __forceinline__ void pack_halves(const float* v, uint4 (&w)[2], float
 
 __device__ __forceinline__ float2 unpack_half(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// N values a row as P planes, `plane` values apart; rows are padded to multiples of 8 columns. The values are used up.
+__device__ __forceinline__ uint4 as_piece(const float* v) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+
+// N values a row as P planes, `plane` values apart. The values are used up.
 template <int P, int N>
 __device__ __forceinline__ void put_planes(unsigned char* scratch, float* v, __nv_bfloat16* to, int64_t row, int64_t plane,
                                            int rows, int columns) {
@@ -419,6 +382,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
 
     if (warp == S::kWarps) {
         if (lane == 0) {
+            const uint32_t first_full = G::first(ctl.full);
             int slot = 0;
             uint32_t phase = 0, armed = 0;  // armed: slots with a copy that nobody may have waited for
             bool ok = true;
@@ -428,40 +392,53 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                 if (!wanted<KIND>(q)) continue;
                 const int m0 = p.m * g.tile_m + int(rank) * kM, n0 = p.n * (KIND == kUp ? g.bn / 2 : g.bn) +
                                                                      (PAIR && KIND != kUp ? int(rank) * columns : 0);
-                for (int step = p.from; step < p.to; ++step) {
-                    if (!mbar_wait(&ctl.empty[slot], phase ^ 1u, abort)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t bar = G::first(&ctl.full[slot]);
-                    if (!PAIR || rank == 0) mbar_expect_tx(&ctl.full[slot], PAIR ? 2 * slot_bytes : slot_bytes);
-                    armed |= 1u << slot;
-                    const uint32_t at = ring + uint32_t(slot) * slot_bytes;
-                    const bool second = KIND == kInput && step >= g.turn;
-                    const int k0 = (second ? step - g.turn : step) * kK;
-                    const CUtensorMap *ma = &maps.a[second ? 1 : q.a], *mb = &maps.b[second ? 1 : q.b];
-                    for (int i = 0; i < P; ++i) {
-                        const uint32_t a = at + P * tile_b + uint32_t(i) * tile_a, b = at + uint32_t(i) * tile_b;
-                        if (kColumnsA) {
-                            G::load(a, ma, bar, m0, k0, i);
-                            G::load(a + kPanel, ma, bar, m0 + 64, k0, i);
-                        } else {
-                            G::load(a, ma, bar, k0, m0, i);
+                const bool pa = q.a_panels != 0, pb = q.b_panels != 0;
+                for (int half = 0; half < (KIND == kInput ? 2 : 1) && ok; ++half) {  // kInput: da and gate, db and up
+                    const int base = half * g.turn, from = max(p.from, base);
+                    const int to = KIND == kInput && half == 0 ? min(p.to, g.turn) : p.to;
+                    const CUtensorMap *ma = &maps.a[half > 0 ? 1 : q.a], *mb = &maps.b[half > 0 ? 1 : q.b];
+                    const CUtensorMap* up = &maps.b[KIND == kUp && PAIR ? rank : 1];
+                    for (int step = from; step < to; ++step) {
+                        if (!mbar_wait(&ctl.empty[slot], phase ^ 1u, abort)) {
+                            ok = false;
+                            break;
                         }
-                        if (KIND == kUp && PAIR) {
-                            G::load(b, &maps.b[rank], bar, k0, n0, i);
-                        } else if (KIND == kUp) {
-                            G::load(b, &maps.b[0], bar, k0, n0, i);
-                            G::load(b + tile_b / 2, &maps.b[1], bar, k0, n0, i);
-                        } else if (kColumnsB) {
-                            for (int c = 0; c < columns / 64; ++c) G::load(b + c * kPanel, mb, bar, n0 + 64 * c, k0, i);
-                        } else {
-                            G::load(b, mb, bar, k0, n0, i);
+                        const uint32_t bar = first_full + uint32_t(slot) * 8u;
+                        if (!PAIR || rank == 0) mbar_expect_tx(&ctl.full[slot], PAIR ? 2 * slot_bytes : slot_bytes);
+                        armed |= 1u << slot;
+                        const uint32_t at = ring + uint32_t(slot) * slot_bytes;
+                        const int k = step - base, k0 = k * kK;
+#pragma unroll
+                        for (int i = 0; i < P; ++i) {
+                            const uint32_t a = at + P * tile_b + uint32_t(i) * tile_a, b = at + uint32_t(i) * tile_b;
+                            if (kColumnsA) {
+                                if (pa) {
+                                    G::load(a, ma, bar, 0, k0, m0 / 64, i);
+                                } else {
+                                    G::load(a, ma, bar, m0, k0, 0, i);
+                                    G::load(a + kPanel, ma, bar, m0 + 64, k0, 0, i);
+                                }
+                            } else {
+                                G::load(a, ma, bar, pa ? 0 : k0, m0, pa ? k : 0, i);
+                            }
+                            if (KIND == kUp && PAIR) {
+                                G::load(b, up, bar, pb ? 0 : k0, n0, pb ? k : 0, i);
+                            } else if (KIND == kUp) {
+                                G::load(b, mb, bar, pb ? 0 : k0, n0, pb ? k : 0, i);
+                                G::load(b + tile_b / 2, up, bar, pb ? 0 : k0, n0, pb ? k : 0, i);
+                            } else if (kColumnsB) {
+                                if (pb)
+                                    G::load(b, mb, bar, 0, k0, n0 / 64, i);
+                                else
+                                    for (int c = 0; c < columns / 64; ++c) G::load(b + c * kPanel, mb, bar, n0 + 64 * c, k0, 0, i);
+                            } else {
+                                G::load(b, mb, bar, pb ? 0 : k0, n0, pb ? k : 0, i);
+                            }
                         }
-                    }
-                    if (++slot == g.slots) {
-                        slot = 0;
-                        phase ^= 1u;
+                        if (++slot == g.slots) {
+                            slot = 0;
+                            phase ^= 1u;
+                        }
                     }
                 }
             }
@@ -556,46 +533,50 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             G::arrive(&ctl.taken[unit & 1]);
             ++unit;
         };
-        // kHidden, float32: the factors of the next 32 columns are on their way while the last ones are stored
-        float4 ahead[8];
-        auto fetch = [&](const void* factor, int64_t row0, int64_t col, int rows, int64_t n) {
-            const int pieces = int(max(int64_t(0), min(int64_t(8), (n - col + 7) / 8 * 2)));
-            fetch_rows(static_cast<const float*>(factor) + row0 * g.row + col, g.row, rows, pieces, ahead);
-        };
-        auto spread = [&](const Problem& q, int64_t row0, int rows, int64_t col, int64_t after, const float* v) {
-            const int columns = int(max(int64_t(0), min(int64_t(32), q.n - col)));
-            const int64_t at = row0 * g.row + col;
-            float x[32];
-            turn_rows(scratch, ahead, x);
-            fetch(g.level, row0, col, rows, q.n);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] *= v[i];
-            put_planes<P, 32>(scratch, x, g.da + at, g.row, g.plane, rows, columns);
-            turn_rows(scratch, ahead, x);
-            fetch(g.slope, row0, after, rows, q.n);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] *= v[i];
-            put_planes<P, 32>(scratch, x, g.db + at, g.row, g.plane, rows, columns);
-        };
-        // the same in 16 bits, of both factors at once
-        uint4 slopes[4], levels[4];
+        const int lane32 = lane;
+        // the block of 32 rows from row0 on and 16 hidden units from col on, this lane's first piece
+        constexpr int kPieces = P == 1 ? 2 : 4;
+        auto block_at = [&](int64_t row0, int64_t col) { return ((col / 16 * g.blocks + row0 / 32) * kPieces) * 32 + lane32; };
+        auto panel_at = [&](int64_t row0, int64_t col, int64_t rows) { return (col / 64 * rows + row0) * 64 + col % 64; };
+        // kHidden: factors of 32 columns, those of the next ones on their way while the last ones are stored
+        uint4 slopes[2 * kPieces], levels[P == 1 ? 2 * kPieces : 1];
         float2 unit_of[2];
-        auto fetch_both = [&](int64_t row0, int64_t col, int rows, int64_t n) {
-            const int pieces = int(max(int64_t(0), min(int64_t(4), (n - col + 7) / 8)));
-            fetch_halves(static_cast<const __half*>(g.slope) + row0 * g.row + col, g.row, rows, pieces, slopes);
-            fetch_halves(static_cast<const __half*>(g.level) + row0 * g.row + col, g.row, rows, pieces, levels);
-            const int lane = threadIdx.x & 31;
+        auto fetch = [&](const void* factor, int64_t row0, int64_t col, int64_t n, uint4* to) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint4* p = static_cast<const uint4*>(factor) + block_at(row0, col + 16 * i);
+                const bool here = col + 16 * i < n;
+#pragma unroll
+                for (int e = 0; e < kPieces; ++e) to[i * kPieces + e] = here ? __ldg(p + 32 * e) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto fetch_both = [&](int64_t row0, int64_t col, int64_t n) {
+            fetch(g.slope, row0, col, n, slopes);
+            fetch(g.level, row0, col, n, levels);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                unit_of[i] = lane < rows && 2 * i < pieces ? __ldg(g.unit + (col / 16 + i) * g.problem[0].m + row0 + lane)
-                                                           : make_float2(0.0f, 0.0f);
+                unit_of[i] = col + 16 * i < n ? __ldg(g.unit + (col / 16 + i) * g.blocks * 32 + row0 + lane32) : make_float2(0.0f, 0.0f);
+        };
+        // float32: one factor after the other
+        auto spread = [&](const Problem& q, int64_t row0, int rows, int64_t col, int64_t after, const float* v) {
+            __nv_bfloat16* const to[2] = {g.da, g.db};
+            const int columns = col < g.panels * 64 ? 32 : 0;
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                float x[32];
+                const float* f = reinterpret_cast<const float*>(slopes);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[i] = f[i] * v[i];
+                if (o == 0) fetch(g.level, row0, col, rows > 0 ? q.n : 0, slopes);
+                else fetch(g.slope, row0, after, rows > 0 ? q.n : 0, slopes);
+                put_planes<P, 32>(scratch, x, to[o] + panel_at(row0, col, q.m), 64, g.plane, rows, columns);
+            }
         };
         // What follows the W sums of column `col` and on (kUp: of the hidden units).
         auto finish = [&](const Problem& q, const Place& p, int64_t row0, int rows, int64_t col, float(&v)[W]) {
             if constexpr (KIND == kUp) {
                 constexpr int kH = W / 2;
-                const int columns = int(max(int64_t(0), min(int64_t(kH), q.n - col)));
-                const int64_t at = row0 * g.row + col;
+                const int columns = col < g.panels * 64 ? kH : 0;
                 uint4 first[kH / 8];
                 float h[P == 3 ? kH : 8];
 #pragma unroll
@@ -607,23 +588,28 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                     v[kH + i] *= slope;
                     if (P == 1 && i % 8 == 7) first[i / 8] = pack8(h);
                 }
+                const int64_t at = panel_at(row0, col, q.m);
                 if constexpr (P == 1)
-                    put_rows<kH / 8>(scratch, first, g.h + at, g.row * 2, rows, (columns + 7) / 8);
+                    put_rows<kH / 8>(scratch, first, g.h + at, 128, rows, columns / 8);
                 else
-                    put_planes<P, kH>(scratch, h, g.h + at, g.row, g.plane, rows, columns);
-                if (g.slope != nullptr) {
+                    put_planes<P, kH>(scratch, h, g.h + at, 64, g.plane, rows, columns);
+                if (g.slope != nullptr && col < q.n && rows > 0) {
+                    uint4 *slope = static_cast<uint4*>(g.slope) + block_at(row0, col),
+                          *level = static_cast<uint4*>(g.level) + block_at(row0, col);
                     if constexpr (P == 1) {
                         uint4 w[2];
                         float2 unit;
                         pack_halves(v + kH, w, unit.x);
-                        put_rows<2>(scratch, w, static_cast<__half*>(g.slope) + at, g.row * 2, rows, (columns + 7) / 8);
+                        slope[0] = w[0], slope[32] = w[1];
                         pack_halves(v, w, unit.y);
-                        put_rows<2>(scratch, w, static_cast<__half*>(g.level) + at, g.row * 2, rows, (columns + 7) / 8);
-                        const int lane = threadIdx.x & 31;
-                        if (lane < rows && columns > 0) g.unit[col / 16 * q.m + row0 + lane] = unit;
+                        level[0] = w[0], level[32] = w[1];
+                        g.unit[col / 16 * g.blocks * 32 + row0 + lane32] = unit;
                     } else {
-                        put_floats<kH>(scratch, v + kH, static_cast<float*>(g.slope) + at, g.row, rows, (columns + 7) & ~7);
-                        put_floats<kH>(scratch, v, static_cast<float*>(g.level) + at, g.row, rows, (columns + 7) & ~7);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            slope[32 * i] = as_piece(v + kH + 4 * i);
+                            level[32 * i] = as_piece(v + 4 * i);
+                        }
                     }
                 }
             } else if constexpr (KIND != kHidden) {
@@ -642,12 +628,17 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             const int64_t row0 = int64_t(p.m) * g.tile_m + rank * kM + (warp & 3) * 32, n0 = int64_t(p.n) * (KIND == kUp ? g.bn / 2 : g.bn);
             const int rows = int(max(int64_t(0), min(int64_t(32), q.m - row0)));
             if constexpr (KIND == kHidden) {
-                if (P == 1) {
-                    if (group < units) fetch_both(row0, n0 + group * kStep, rows, q.n);
+                if constexpr (P == 1) {
+                    if (group < units) fetch_both(row0, n0 + group * kStep, rows > 0 ? q.n : 0);
                 } else {
-                    fetch(g.slope, row0, n0 + group * kStep, rows, q.n);
+                    fetch(g.slope, row0, n0 + group * kStep, rows > 0 ? q.n : 0, slopes);
                 }
             }
+            if (KIND == kUp && p.n + 1 == q.n_tiles)  // what the last tile leaves of the last panel
+                for (int64_t col = n0 + g.bn / 2 + group * 16; col < g.panels * 64; col += kGroups * 16) {
+                    float v[16] = {};
+                    put_planes<P, 16>(scratch, v, g.h + panel_at(row0, col, q.m), 64, g.plane, rows, 16);
+                }
             if (p.from >= p.to) {  // a split without a share: sums of zero
                 float v[W] = {};
                 for (int u = group; u < units; u += kGroups) finish(q, p, row0, rows, n0 + u * kStep, v);
@@ -661,9 +652,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                     const bool last = u + kGroups >= units;
                     if constexpr (KIND == kHidden) {
                         const int64_t col = n0 + u * 32;
-                        const int columns = int(max(int64_t(0), min(int64_t(32), q.n - col)));
-                        turn_halves(scratch, slopes);
-                        turn_halves(scratch, levels);
+                        const int columns = col < g.panels * 64 ? 32 : 0;
                         uint4 da[4], db[4];
                         const uint32_t *s = reinterpret_cast<const uint32_t*>(slopes), *l = reinterpret_cast<const uint32_t*>(levels);
 #pragma unroll
@@ -680,10 +669,10 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                             db[2 * j] = pack8(y), db[2 * j + 1] = pack8(y + 8);
                         }
                         if (last) done();
-                        else fetch_both(row0, col + kGroups * 32, rows, q.n);
-                        const int64_t to = row0 * g.row + col;
-                        put_rows<4>(scratch, da, g.da + to, g.row * 2, rows, (columns + 7) / 8);
-                        put_rows<4>(scratch, db, g.db + to, g.row * 2, rows, (columns + 7) / 8);
+                        else fetch_both(row0, col + kGroups * 32, rows > 0 ? q.n : 0);
+                        const int64_t to = panel_at(row0, col, q.m);
+                        put_rows<4>(scratch, da, g.da + to, 128, rows, columns / 8);
+                        put_rows<4>(scratch, db, g.db + to, 128, rows, columns / 8);
                     } else {
                         float v[W];
                         if constexpr (KIND == kUp) {
@@ -800,20 +789,28 @@ __global__ void __launch_bounds__(256) add_kernel(const Args g) {
 
 // ------------------------------------------------------------------- host
 
-// A matrix of bfloat16 as TMA reads it: `planes` of [rows, columns] with rows `row` apart.
+// A matrix of bfloat16 as TMA reads it: `planes` of [rows, columns] with rows `row` apart, or (panels > 0) in panels of 64
+// columns, [planes][panels][rows][64].
 struct Matrix {
     const void* data;
     int64_t rows, columns, row;
-    int planes;
+    int planes, panels;
+    // Read panel by panel, so that one copy takes several: any matrix of whole panels. Else a copy is at most 64 columns,
+    // and what lies behind the last column is filled with zeros.
+    bool by_panels() const { return panels > 0 || columns % 64 == 0; }
 };
 
-fmd_status encode(CUtensorMap* map, const Matrix& x, int box_rows) {
+fmd_status encode(CUtensorMap* map, const Matrix& x, int box_rows, int box_panels) {
     const DriverCalls& drv = driver_calls();
-    const int64_t row = x.rows == 1 ? (x.columns + 7) / 8 * 8 : x.row;
-    const cuuint64_t dims[3] = {cuuint64_t(x.columns), cuuint64_t(x.rows), cuuint64_t(x.planes)};
-    const cuuint64_t strides[2] = {cuuint64_t(row) * 2, cuuint64_t(x.planes == 1 ? row * x.rows : x.row * x.rows) * 2};
-    const cuuint32_t box[3] = {64, cuuint32_t(box_rows), 1}, step[3] = {1, 1, 1};
-    const CUresult r = drv.encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(x.data), dims, strides, box,
+    const int64_t row = x.panels > 0 ? 64 : x.rows == 1 ? (x.columns + 7) / 8 * 8 : x.row;
+    const int64_t panel = x.panels > 0 ? 64 * x.rows : 64, count = x.panels > 0 ? x.panels : x.columns / 64;
+    const bool panels = x.by_panels();
+    const cuuint64_t dims[4] = {cuuint64_t(panels ? 64 : x.columns), cuuint64_t(x.rows), cuuint64_t(panels ? count : 1),
+                                cuuint64_t(x.planes)};
+    const cuuint64_t strides[3] = {cuuint64_t(row) * 2, cuuint64_t(panels ? panel : row * x.rows) * 2,
+                                   cuuint64_t(x.panels > 0 ? panel * count : row * x.rows) * 2};
+    const cuuint32_t box[4] = {64, cuuint32_t(box_rows), cuuint32_t(panels ? box_panels : 1), 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = drv.encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(x.data), dims, strides, box,
                                   step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? FMD_OK : record_error_text(FMD_ERR_CUDA, "cuTensorMapEncodeTiled failed, CUresult", r);
@@ -869,7 +866,9 @@ Plan plan(const int64_t* m, const int64_t* n, int problems, int64_t steps, int p
 struct Sizes {
     int64_t rows, width, hidden, out;
     int planes;  // 3: float32
-    int64_t hidden_row, width_row, out_row;  // of the arrays made here
+    int64_t hidden_row, width_row, out_row;  // of planes of what is given
+    int panels, blocks;                      // of h, da and db; of 32 rows, of the factors
+    size_t values() const { return size_t(rows) * panels * 64; }
 };
 
 template <int KIND, int P, int W, bool PAIR>
@@ -912,9 +911,10 @@ fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args&
     g.tile_a = columns_a ? int(kTileA) : rows * kK * 2;
     for (int i = 0; i < operands; ++i) {
         fmd_status st = FMD_OK;
-        if (a[i].data != nullptr) st = encode(&maps.a[i], a[i], columns_a ? kK : rows);
+        if (a[i].data != nullptr) st = encode(&maps.a[i], a[i], columns_a ? kK : rows, columns_a ? kM / 64 : 1);
         if (st == FMD_OK && b[i].data != nullptr)
-            st = encode(&maps.b[i], b[i], columns_b ? kK : KIND == kUp || p.tile_m > kM ? p.bn / 2 : p.bn);
+            st = encode(&maps.b[i], b[i], columns_b ? kK : KIND == kUp || p.tile_m > kM ? p.bn / 2 : p.bn,
+                        columns_b ? (p.tile_m > kM ? p.bn / 2 : p.bn) / 64 : 1);
         if (st != FMD_OK) return st;
     }
     g.tile_m = p.tile_m;
@@ -925,6 +925,8 @@ fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args&
     for (int i = 0; i < g.problems; ++i) {
         Problem& q = g.problem[i];
         const int columns = KIND == kUp ? p.bn / 2 : p.bn;
+        q.a_panels = a[q.a].by_panels();
+        q.b_panels = b[q.b].by_panels();
         q.m_tiles = int((q.m + p.tile_m - 1) / p.tile_m);
         q.n_tiles = int((q.n + columns - 1) / columns);
     }
@@ -967,13 +969,12 @@ struct Kept {
 Kept kept_layout(const Sizes& z, bool factors) {
     Layout at;
     Kept k{};
-    const size_t hidden = size_t(z.rows) * z.hidden_row;
-    k.h = at.take(hidden * z.planes * 2);
+    k.h = at.take(z.values() * z.planes * 2);
     if (factors) {
-        const size_t size = z.planes == 3 ? 4 : 2;
-        k.slope = at.take(hidden * size);
-        k.level = at.take(hidden * size);
-        if (z.planes == 1) k.unit = at.take(size_t(z.rows) * ((z.hidden + 15) / 16) * sizeof(float2));
+        const size_t blocks = size_t(z.blocks) * ((z.hidden + 15) / 16);  // of 32 rows x 16 units
+        k.slope = at.take(blocks * 512 * (z.planes == 3 ? 4 : 2));
+        k.level = at.take(blocks * 512 * (z.planes == 3 ? 4 : 2));
+        if (z.planes == 1) k.unit = at.take(blocks * 32 * sizeof(float2));
     }
     if (z.planes == 3) {
         k.x = at.take(size_t(z.rows) * z.width_row * 6);
@@ -993,7 +994,7 @@ struct Scratch {
 Scratch scratch_layout(const Sizes& z) {
     Layout at;
     Scratch k{};
-    const size_t hidden = size_t(z.rows) * z.hidden_row * z.planes * 2;
+    const size_t hidden = z.values() * z.planes * 2;
     k.da = at.take(hidden);
     k.db = at.take(hidden);
     if (z.planes == 3) k.g = at.take(size_t(z.rows) * z.out_row * 6);
@@ -1016,7 +1017,7 @@ fmd_status check(const fmd_feed_forward& f, Sizes& z) {
          !vector_rows(f.down, f.out > 1 ? f.down_row : 0, 0, 2)))
         return FMD_ERR_UNSUPPORTED;
     z = Sizes{f.rows, f.width, f.hidden, f.out, f.type == FMD_F32 ? 3 : 1, round_up(f.hidden, 8), round_up(f.width, 8),
-              round_up(f.out, 8)};
+              round_up(f.out, 8), int((f.hidden + 63) / 64), int((f.rows + 31) / 32)};
     // tiles are counted in 32 bits
     if (((z.rows + 127) / 128) * ((z.hidden + 63) / 64 + (z.width + 63) / 64 + (z.out + 63) / 64) * 64 > INT32_MAX)
         return FMD_ERR_UNSUPPORTED;
@@ -1054,10 +1055,10 @@ struct Inputs {
 
 Inputs inputs_of(const fmd_feed_forward& f, const Sizes& z, const Kept& k, char* kept) {
     if (z.planes == 1)
-        return Inputs{{f.x, z.rows, z.width, f.x_row, 1}, {f.gate, z.hidden, z.width, f.gate_row, 1},
-                      {f.up, z.hidden, z.width, f.up_row, 1}, {f.down, z.out, z.hidden, f.down_row, 1}};
-    return Inputs{{kept + k.x, z.rows, z.width, z.width_row, 3}, {kept + k.gate, z.hidden, z.width, z.width_row, 3},
-                  {kept + k.up, z.hidden, z.width, z.width_row, 3}, {kept + k.down, z.out, z.hidden, z.hidden_row, 3}};
+        return Inputs{{f.x, z.rows, z.width, f.x_row, 1, 0}, {f.gate, z.hidden, z.width, f.gate_row, 1, 0},
+                      {f.up, z.hidden, z.width, f.up_row, 1, 0}, {f.down, z.out, z.hidden, f.down_row, 1, 0}};
+    return Inputs{{kept + k.x, z.rows, z.width, z.width_row, 3, 0}, {kept + k.gate, z.hidden, z.width, z.width_row, 3, 0},
+                  {kept + k.up, z.hidden, z.width, z.width_row, 3, 0}, {kept + k.down, z.out, z.hidden, z.hidden_row, 3, 0}};
 }
 
 }  // namespace
@@ -1111,8 +1112,9 @@ fmd_status fmd_gated_feed_forward(const fmd_feed_forward* problem, void* y, int3
     g.flags = flags;
     g.act = f.activation;
     g.h = reinterpret_cast<__nv_bfloat16*>(at + k.h);
-    g.row = z.hidden_row;
-    g.plane = z.rows * z.hidden_row;
+    g.plane = int64_t(z.values());
+    g.panels = z.panels;
+    g.blocks = z.blocks;
     if (keep) {
         g.slope = at + k.slope;
         g.level = at + k.level;
@@ -1130,7 +1132,7 @@ fmd_status fmd_gated_feed_forward(const fmd_feed_forward* problem, void* y, int3
     g.problem[0].out = y;
     g.part = static_cast<float*>(workspace);
     g.steps = int(steps_of(z.hidden));
-    const Matrix h{at + k.h, z.rows, z.hidden, z.hidden_row, z.planes};
+    const Matrix h{at + k.h, z.rows, z.hidden, 64, z.planes, z.panels};
     return run<kDown>(z.planes, &h, &in.down, 1, g, down, s);
 }
 
@@ -1165,18 +1167,19 @@ fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kep
     if ((st = ready()) != FMD_OK) return st;
     char *at = static_cast<char*>(kept), *own = static_cast<char*>(workspace);
     const Inputs in = inputs_of(f, z, k, at);
-    Matrix gm{g, z.rows, z.out, g_row, 1};
+    Matrix gm{g, z.rows, z.out, g_row, 1, 0};
     if (z.planes == 3) {
         SplitArgs a{};
         int count = 0;
         add_split(a, count, g, own + w.g, z.rows, z.out, g_row, z.out_row);
         if ((st = split(a, count, s)) != FMD_OK) return st;
-        gm = Matrix{own + w.g, z.rows, z.out, z.out_row, 3};
+        gm = Matrix{own + w.g, z.rows, z.out, z.out_row, 3, 0};
     }
     Args args{};
     args.flags = flags;
-    args.row = z.hidden_row;
-    args.plane = z.rows * z.hidden_row;
+    args.plane = int64_t(z.values());
+    args.panels = z.panels;
+    args.blocks = z.blocks;
     args.slope = at + k.slope;
     args.level = at + k.level;
     args.unit = reinterpret_cast<float2*>(at + k.unit);
@@ -1192,7 +1195,7 @@ fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kep
                           plan(&z.rows, &z.hidden, 1, args.steps, z.planes, z.planes == 1 ? 64 : 128, false), s);
         if (st != FMD_OK) return st;
     }
-    const Matrix da{own + w.da, z.rows, z.hidden, z.hidden_row, z.planes}, db{own + w.db, z.rows, z.hidden, z.hidden_row, z.planes};
+    const Matrix da{own + w.da, z.rows, z.hidden, 64, z.planes, z.panels}, db{own + w.db, z.rows, z.hidden, 64, z.planes, z.panels};
     if (dx != nullptr) {
         args.problems = 1;
         args.problem[0].n = z.width;
@@ -1204,7 +1207,7 @@ fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kep
     }
     // the products of the weights' gradients that are asked for
     const Plan p = weights_plan(z);
-    const Matrix h{at + k.h, z.rows, z.hidden, z.hidden_row, z.planes};
+    const Matrix h{at + k.h, z.rows, z.hidden, 64, z.planes, z.panels};
     const Matrix a[3] = {da, db, gm}, b[3] = {in.x, in.x, h};
     void* const out[3] = {dgate, dup, ddown};
     // all three have their places whichever are asked for, so that each has the same bits
