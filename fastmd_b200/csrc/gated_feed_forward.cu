@@ -47,10 +47,11 @@ constexpr int kSegment = 2;
 enum Kind { kUp, kDown, kHidden, kInput, kWeights };
 
 // Warps that take the sums: sixteen where much follows them, which eight did not get through in the time of a tile's products
-// (up of 32,000 x 1,024 x 4,096 with its factors 718 us, hidden 923); float32 has six times the products and needs the slots.
+// (up of 32,000 x 1,024 x 4,096 with its factors 718 us, hidden 923); hidden in float32 has six times the products, and needs
+// the registers.
 template <int KIND, int P>
 struct Shape {
-    static constexpr int kWarps = P == 1 && (KIND == kUp || KIND == kHidden) ? 16 : 8;
+    static constexpr int kWarps = KIND == kUp || (P == 1 && KIND == kHidden) ? 16 : 8;
     static constexpr int kThreads = 64 + 32 * kWarps;  // the takers first: a warp's part of TMEM goes by its number
     static constexpr size_t kScratch = kWarps == 16 ? 2048 : 4096;  // of each of these warps
     static constexpr size_t kRing = 224 * 1024 - kWarps * kScratch;
@@ -686,7 +687,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                     }
                 }
             } else {
-                constexpr int kUnits = 128 / W / kGroups;  // at most: bn is up to 128
+                constexpr int kUnits = 128 / W / kGroups > 0 ? 128 / W / kGroups : 1;  // at most: bn is up to 128
                 float sum[kUnits][W] = {};
                 for (int start = p.from; start < p.to; start += kSegment) {
                     if (!(ok = wait())) break;
