@@ -160,7 +160,7 @@ _SIGNATURES: dict[str, list] = {
     "fmd_gated_feed_forward_bwd": [POINTER(FmdFeedForward), _P, c_size_t, _P, _I64, _P, _P, _P, _P, _P, c_size_t, _P, _P],
     "fmd_decay_attention_workspace_bytes": [POINTER(FmdDecay), _I32, POINTER(c_size_t)],
     "fmd_decay_attention": [POINTER(FmdDecay), _P, _P, _P, _P, c_size_t, _P, _P],
-    "fmd_decay_attention_bwd": [POINTER(FmdDecay), _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, c_size_t, _P, _P],
+    "fmd_decay_attention_bwd": [POINTER(FmdDecay), _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, c_size_t, _P, _P],
     "fmd_decay_attention_step": [POINTER(FmdDecay), _P, _P, _P],
     "fmd_nhc_pre_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P],
     "fmd_nhc_post_pre_force": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P],

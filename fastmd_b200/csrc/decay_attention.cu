@@ -195,21 +195,26 @@ struct Input {
     int64_t row, head;
 };
 
-fmd_status make_planes(const Decay& d, Path path, Input* inputs, int count, char*& workspace, cudaStream_t s) {
+// The planes of `inputs`, the first `made` of which are there already, at `made_at`; their room stays in the workspace.
+fmd_status make_planes(const Decay& d, Path path, Input* inputs, int count, int made, const void* made_at, char*& workspace,
+                       cudaStream_t s) {
     if (path != kPlanes || d.rows == 0) return FMD_OK;
     SplitArgs a{};
     a.rows = d.rows;
     a.heads = d.heads;
     a.dim = d.dim;
     for (int i = 0; i < count; ++i) {
-        a.x[i] = static_cast<const float*>(inputs[i].data);
-        a.row[i] = inputs[i].row;
-        a.head[i] = inputs[i].head;
-        a.to[i] = reinterpret_cast<__nv_bfloat16*>(workspace);
-        inputs[i] = Input{workspace, int64_t(d.heads) * d.dim, d.dim};
+        if (i >= made) {
+            a.x[i - made] = static_cast<const float*>(inputs[i].data);
+            a.row[i - made] = inputs[i].row;
+            a.head[i - made] = inputs[i].head;
+            a.to[i - made] = reinterpret_cast<__nv_bfloat16*>(workspace);
+        }
+        const void* at = i < made ? static_cast<const char*>(made_at) + i * plane_bytes(d) : workspace;
+        inputs[i] = Input{at, int64_t(d.heads) * d.dim, d.dim};
         workspace += plane_bytes(d);
     }
-    split_kernel<<<dim3(unsigned(grid_for(d.rows * d.heads * (d.dim / 8), kThreads)), unsigned(count)), kThreads, 0, s>>>(a);
+    split_kernel<<<dim3(unsigned(grid_for(d.rows * d.heads * (d.dim / 8), kThreads)), unsigned(count - made)), kThreads, 0, s>>>(a);
     return check_launch();
 }
 
@@ -287,7 +292,7 @@ fmd_status fmd_decay_attention(const fmd_decay* problem, const float* state, voi
     const Path path = path_of(d, p.type);
     char* at = static_cast<char*>(workspace);
     Input in[3] = {{p.q, p.q_row, p.q_head}, {p.k, p.k_row, p.k_head}, {p.v, p.v_row, p.v_head}};
-    if ((st = make_planes(d, path, in, 3, at, s)) != FMD_OK) return st;
+    if ((st = make_planes(d, path, in, 3, 0, nullptr, at, s)) != FMD_OK) return st;
     read_from(d, in[0], in[1], in[2]);
     d.out = out;
     d.start = state;
@@ -298,9 +303,9 @@ fmd_status fmd_decay_attention(const fmd_decay* problem, const float* state, voi
     return mix(Decays{{d}, 1}, path, at, s);
 }
 
-fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state, const void* g, int64_t g_row,
-                                   int64_t g_head, const float* gafter, void* dq, void* dk, void* dv, float* dstate,
-                                   void* workspace, size_t workspace_bytes, int32_t* flags, void* stream) {
+fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state, const void* forward, const void* g,
+                                   int64_t g_row, int64_t g_head, const float* gafter, void* dq, void* dk, void* dv,
+                                   float* dstate, void* workspace, size_t workspace_bytes, int32_t* flags, void* stream) {
     Decay d;
     if (problem == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     fmd_status st = check_rows(*problem, d);
@@ -310,14 +315,14 @@ fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state,
     const size_t need = workspace_of(d, p.type, 4, 3);
     if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return FMD_ERR_WORKSPACE;
     if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(state) || !aligned16(gafter) ||
-        !aligned16(dstate) || !aligned16(workspace) ||
+        !aligned16(dstate) || !aligned16(workspace) || !aligned16(forward) ||
         (p.rows > 0 && !vector_rows(g, g_row, g_head, p.type == FMD_BF16 ? 2 : 4)))
         return FMD_ERR_UNSUPPORTED;
     const cudaStream_t s = as_stream(stream);
     const Path path = path_of(d, p.type);
     char* at = static_cast<char*>(workspace);
     Input in[4] = {{p.q, p.q_row, p.q_head}, {p.k, p.k_row, p.k_head}, {p.v, p.v_row, p.v_head}, {g, g_row, g_head}};
-    if ((st = make_planes(d, path, in, 4, at, s)) != FMD_OK) return st;
+    if ((st = make_planes(d, path, in, 4, forward != nullptr ? 3 : 0, forward, at, s)) != FMD_OK) return st;
     const Input &q = in[0], &k = in[1], &v = in[2], &go = in[3];
     d.flags = flags;
     d.near = p.scale;

@@ -727,6 +727,155 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
     if (threadIdx.x == 0 && ctl.abort) raise_flag(g.flags, FMD_FLAG_WAIT_TIMEOUT);
 }
 
+// ------------------------------------------------------------------- few rows in float32
+
+// A few rows in float32 without planes, whose making moves four times the weights' bytes: on the FP32 cores. A block takes R
+// rows of x and J rows of weights (GATED: J / 2 units, their gate and up rows) through the inner index in chunks of 256, which
+// lie in shared memory, one in use and one on its way; each of its eight warps takes 32 of a chunk, all R x J sums, a lane 4 x J R / 128 of them: 4 + C
+// vectors of shared memory for 16 C products. The warps' sums are added up at the end.
+constexpr int kFewThreads = 256, kFewChunk = 256, kFewLd = kFewChunk + 4;
+
+struct Few {
+    const float *x, *w0, *w1;  // w1: up
+    float* out;
+    int64_t x_row, w0_row, w1_row, out_row;
+    int32_t rows, inner, units, act;
+    bool vector_x, vector_w;  // rows start at multiples of 16 bytes, and the inner size is one of four values
+};
+
+template <int R, int J>
+struct FewShape {
+    static constexpr int kRowGroups = R / 4, kColumnGroups = 32 / kRowGroups, kC = J / kColumnGroups;
+    static constexpr int kStage = (R + J) * kFewLd;  // values of a chunk
+    static constexpr size_t kChunks = size_t(2) * kStage * 4, kSums = size_t(8) * R * J * 4;
+    static constexpr size_t kBytes = kChunks > kSums ? kChunks : kSums;
+};
+
+// Four bytes, or sixteen, to shared memory; zeros where there are none.
+__device__ __forceinline__ void copy4(float* to, const float* from, bool here) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(su32(to)), "l"(from), "r"(here ? 4 : 0) : "memory");
+}
+
+__device__ __forceinline__ void copy16(float* to, const float* from, bool here) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(su32(to)), "l"(from), "r"(here ? 16 : 0) : "memory");
+}
+
+// A chunk of `count` rows, row r at row_of(r): sixteen bytes a thread where rows start at multiples of them.
+template <typename RowOf>
+__device__ __forceinline__ void copy_rows(float* to, int count, int k0, int inner, bool vector, RowOf row_of) {
+    if (vector) {
+        const int k = k0 + int(threadIdx.x) % 64 * 4;
+        const bool here = k < inner;
+#pragma unroll 4
+        for (int r = int(threadIdx.x) / 64; r < count; r += 4)
+            copy16(to + r * kFewLd + int(threadIdx.x) % 64 * 4, row_of(r) + (here ? k : 0), here);
+    } else {
+        const int k = k0 + int(threadIdx.x);
+        const bool here = k < inner;
+#pragma unroll 8
+        for (int r = 0; r < count; ++r) copy4(to + r * kFewLd + threadIdx.x, row_of(r) + (here ? k : 0), here);
+    }
+}
+
+template <int R, int J, bool GATED>
+__global__ void __launch_bounds__(kFewThreads) few_kernel(const Few f) {
+    using S = FewShape<R, J>;
+    constexpr int kUnits = GATED ? J / 2 : J;
+    extern __shared__ float few_smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rg = lane % S::kRowGroups, cg = lane / S::kRowGroups;
+    const int unit0 = int(blockIdx.x) * kUnits, row0 = int(blockIdx.y) * R, chunks = (f.inner + kFewChunk - 1) / kFewChunk;
+    const int rows = min(R, f.rows - row0);
+    auto load = [&](int chunk) {
+        float *x = few_smem + chunk % 2 * S::kStage, *w = x + R * kFewLd;
+        copy_rows(w, J, chunk * kFewChunk, f.inner, f.vector_w, [&](int j) {
+            const int unit = min(unit0 + j % kUnits, f.units - 1);  // units behind the last one are computed and dropped
+            return GATED && j >= kUnits ? f.w1 + unit * f.w1_row : f.w0 + unit * f.w0_row;
+        });
+        copy_rows(x, rows, chunk * kFewChunk, f.inner, f.vector_x, [&](int r) { return f.x + (row0 + r) * f.x_row; });
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    float acc[4][S::kC] = {};
+    load(0);
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        if (chunk + 1 < chunks) {
+            load(chunk + 1);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+        __syncthreads();
+        const float *x = few_smem + chunk % 2 * S::kStage, *w = x + R * kFewLd;
+#pragma unroll 2
+        for (int e = 0; e < 32; e += 4) {
+            float4 a[4], b[S::kC];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                a[i] = *reinterpret_cast<const float4*>(x + (rg + S::kRowGroups * i) * kFewLd + warp * 32 + e);
+#pragma unroll
+            for (int c = 0; c < S::kC; ++c)
+                b[c] = *reinterpret_cast<const float4*>(w + (cg + S::kColumnGroups * c) * kFewLd + warp * 32 + e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < S::kC; ++c) {
+                    acc[i][c] = fmaf(a[i].x, b[c].x, acc[i][c]);
+                    acc[i][c] = fmaf(a[i].y, b[c].y, acc[i][c]);
+                    acc[i][c] = fmaf(a[i].z, b[c].z, acc[i][c]);
+                    acc[i][c] = fmaf(a[i].w, b[c].w, acc[i][c]);
+                }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < S::kC; ++c)
+            few_smem[(warp * R + rg + S::kRowGroups * i) * J + cg + S::kColumnGroups * c] = acc[i][c];
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * kUnits; i += kFewThreads) {
+        const int r = i / kUnits, u = i % kUnits, unit = unit0 + u;
+        if (row0 + r >= f.rows || unit >= f.units) continue;
+        float a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            a += few_smem[(q * R + r) * J + u];
+            if (GATED) b += few_smem[(q * R + r) * J + kUnits + u];
+        }
+        if (GATED) {
+            float level, slope;
+            activate<true>(f.act, a, level, slope);
+            a = level * b;
+        }
+        f.out[(row0 + r) * f.out_row + unit] = a;
+    }
+}
+
+template <int R, int J, bool GATED>
+fmd_status launch_few(const Few& f, cudaStream_t s) {
+    constexpr size_t bytes = FewShape<R, J>::kBytes;
+    const fmd_status st = grant_dynamic_smem((const void*)few_kernel<R, J, GATED>, bytes);
+    if (st != FMD_OK) return st;
+    const int units = GATED ? J / 2 : J;
+    few_kernel<R, J, GATED><<<dim3(unsigned((f.units + units - 1) / units), unsigned((f.rows + R - 1) / R)), kFewThreads, bytes,
+                             s>>>(f);
+    return check_launch();
+}
+
+// As many rows of weights a block, of sixteen at most, as leave a block for every SM.
+template <int R, bool GATED>
+fmd_status launch_few(const Few& f, cudaStream_t s) {
+    const int64_t rows = int64_t(f.units) * (GATED ? 2 : 1);
+    if (rows >= 16 * kNumSMs) return launch_few<R, 16, GATED>(f, s);
+    if constexpr (R >= 32)
+        if (rows < 8 * kNumSMs) return launch_few<R, 4, GATED>(f, s);
+    return launch_few<R, 8, GATED>(f, s);
+}
+
+template <bool GATED>
+fmd_status launch_few(const Few& f, cudaStream_t s) {
+    return f.rows <= 16 ? launch_few<16, GATED>(f, s) : launch_few<32, GATED>(f, s);
+}
+
 // ------------------------------------------------------------------- planes and sums of splits
 
 // float32 [rows, columns] as three planes [3][rows][row] of bfloat16, up to four arrays (blockIdx.y).
@@ -818,6 +967,12 @@ fmd_status encode(CUtensorMap* map, const Matrix& x, int box_rows, int box_panel
 }
 
 int64_t round_up(int64_t v, int64_t unit) { return (v + unit - 1) / unit * unit; }
+
+// Rows up to which float32 goes without planes where no backward pass follows: two blocks of 32 where the weights are small,
+// else one. us on the FP32 cores and by planes, width x hidden: 256 x 512, 32 rows 10 and 22, 64 rows 11 and 22; 512 x 1,365,
+// 32 rows 19 and 29, 64 rows 31 and 29 (with two launches less); 1,024 x 4,096, 16 rows 38 and 62, 32 rows 64 and 61, 64 rows
+// 125 and 61; 4,096 x 11,000, 1 row 217 and 440, 32 rows 363 and 439, 64 rows 707 and 449.
+int64_t few_limit(int64_t width, int64_t hidden) { return width * hidden <= (1 << 20) ? 64 : 32; }
 
 // How a launch runs: rows (256: pairs of blocks) and columns of a tile, the tiles that are not shared out, shares of the
 // others along the inner index.
@@ -1025,6 +1180,23 @@ fmd_status check(const fmd_feed_forward& f, Sizes& z) {
     return FMD_OK;
 }
 
+// A few rows: h alone, by rows.
+bool few_rows(const Sizes& z, bool keep) { return z.planes == 3 && !keep && z.rows > 0 && z.rows <= few_limit(z.width, z.hidden); }
+size_t few_bytes(const Sizes& z) { return (size_t(z.rows) * round_up(z.hidden, 4) * sizeof(float) + 255) / 256 * 256; }
+
+fmd_status run_few(const fmd_feed_forward& f, float* h, float* y, cudaStream_t s) {
+    const float *x = static_cast<const float*>(f.x), *gate = static_cast<const float*>(f.gate),
+                *up = static_cast<const float*>(f.up), *down = static_cast<const float*>(f.down);
+    auto whole = [](const float* p, int64_t row, int64_t inner) { return inner % 4 == 0 && row % 4 == 0 && aligned16(p); };
+    const int64_t h_row = round_up(f.hidden, 4);
+    const fmd_status st = launch_few<true>(
+        Few{x, gate, up, h, f.x_row, f.gate_row, f.up_row, h_row, int32_t(f.rows), f.width, f.hidden, f.activation,
+            whole(x, f.rows > 1 ? f.x_row : 0, f.width), whole(gate, f.gate_row, f.width) && whole(up, f.up_row, f.width)}, s);
+    if (st != FMD_OK) return st;
+    return launch_few<false>(Few{h, down, nullptr, y, h_row, f.down_row, 0, f.out, int32_t(f.rows), f.hidden, f.out, 0,
+                                 f.hidden % 4 == 0, whole(down, f.down_row, f.hidden)}, s);
+}
+
 fmd_status ready() {
     const DriverCalls& drv = driver_calls();
     if (drv.encode == nullptr || drv.ctx_get_current == nullptr)
@@ -1075,8 +1247,9 @@ fmd_status fmd_gated_feed_forward_bytes(const fmd_feed_forward* problem, int32_t
     if (problem == nullptr || kept == nullptr || forward == nullptr || backward == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     const fmd_status st = check(*problem, z);
     if (st != FMD_OK) return st;
-    *kept = z.rows > 0 ? kept_layout(z, keep != 0).bytes : 0;
-    *forward = z.rows > 0 ? down_plan(z).bytes() : 0;
+    const bool few = few_rows(z, keep);
+    *kept = few ? few_bytes(z) : z.rows > 0 ? kept_layout(z, keep != 0).bytes : 0;
+    *forward = few || z.rows == 0 ? 0 : down_plan(z).bytes();
     *backward = z.rows > 0 && keep ? scratch_layout(z).bytes : 0;
     return FMD_OK;
 }
@@ -1087,9 +1260,14 @@ fmd_status fmd_gated_feed_forward(const fmd_feed_forward* problem, void* y, int3
     if (problem == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     fmd_status st = check(*problem, z);
     if (st != FMD_OK || z.rows == 0) return st;
+    if (y == nullptr) return FMD_ERR_INVALID_ARGUMENT;
+    if (few_rows(z, keep)) {
+        if (kept == nullptr || kept_bytes < few_bytes(z)) return FMD_ERR_WORKSPACE;
+        if (!aligned16(y) || !aligned16(kept)) return FMD_ERR_UNSUPPORTED;
+        return run_few(*problem, static_cast<float*>(kept), static_cast<float*>(y), as_stream(stream));
+    }
     const Kept k = kept_layout(z, keep != 0);
     const Plan down = down_plan(z);
-    if (y == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     if (kept_bytes < k.bytes || kept == nullptr || workspace_bytes < down.bytes() ||
         (down.splits > 1 && workspace == nullptr))
         return FMD_ERR_WORKSPACE;

@@ -17,6 +17,9 @@ from ._first_order import first_order, has_tangent
 from ._lib import FmdDecay, c_size_t, call, on_device, ptr, stream
 from .head_rotary import TYPES, _head_rows, _like
 
+#: float32 heads of up to this many values go through planes, which the forward pass hands to the backward pass
+PLANES_DIM = 64
+
 
 def _problem(q, k, v, log_decay, offsets, scale) -> FmdDecay:
     return FmdDecay(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), ptr(offsets), q.shape[0], q.stride(0),
@@ -42,21 +45,23 @@ def _forward(q, k, v, log_decay, offsets, state, scale, keep):
     workspace, size = _workspace(problem, False, device)
     call("fmd_decay_attention", problem, ptr(state), out.data_ptr(), ptr(after), ptr(workspace), size,
          _lib.flags_word(device).data_ptr(), stream(device))
-    return out, after
+    return out, after, workspace
 
 
 class _DecayAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, offsets, state, scale, keep):
-        out, after = _forward(q, k, v, log_decay, offsets, state, scale, keep)
-        ctx.save_for_backward(q, k, v, log_decay, offsets, state)
+        out, after, workspace = _forward(q, k, v, log_decay, offsets, state, scale, keep)
+        if q.dtype != torch.float32 or q.shape[2] > PLANES_DIM:
+            workspace = None
+        ctx.save_for_backward(q, k, v, log_decay, offsets, state, workspace)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return out, after
 
     @staticmethod
     def backward(ctx, g, gafter):
-        q, k, v, log_decay, offsets, state = ctx.saved_tensors
+        q, k, v, log_decay, offsets, state, forward = ctx.saved_tensors
         if g is None and gafter is None:
             return (None,) * 8
         inputs = (g, gafter, q, k, v, state)
@@ -67,7 +72,7 @@ class _DecayAttention(Function):
         dstate = torch.empty_like(state) if need[5] else None
         problem = _problem(q, k, v, log_decay, offsets, ctx.scale)
         workspace, size = _workspace(problem, True, q.device)
-        call("fmd_decay_attention_bwd", problem, ptr(state), g.data_ptr(), g.stride(0), g.stride(1), ptr(gafter), ptr(dq),
+        call("fmd_decay_attention_bwd", problem, ptr(state), ptr(forward), g.data_ptr(), g.stride(0), g.stride(1), ptr(gafter), ptr(dq),
              ptr(dk), ptr(dv), ptr(dstate), ptr(workspace), size, _lib.flags_word(q.device).data_ptr(), stream(q.device))
         dq, dk, dv, dstate = first_order("decay_attention", (dq, dk, dv, dstate), inputs)
         return dq, dk, dv, None, None, dstate, None, None
@@ -145,7 +150,7 @@ def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, offsets:
         if (torch.is_grad_enabled() and trains) or has_tangent(q, k, v, log_decay, state):
             out, after = _DecayAttention.apply(*args)
         else:
-            out, after = _forward(*args)
+            out, after, _ = _forward(*args)
     return (out, after) if return_state else out
 
 

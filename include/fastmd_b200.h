@@ -1185,7 +1185,8 @@ typedef struct fmd_decay {
 } fmd_decay;
 
 /* Workspace of the forward pass (backward = 0) or of the backward pass (1),
- * from the sizes alone; 0 for none. It starts at a multiple of 16 bytes. */
+ * from the sizes alone; 0 for none. It starts at a multiple of 16 bytes. The
+ * forward pass's may be handed to the backward pass of the same problem. */
 FMD_API fmd_status fmd_decay_attention_workspace_bytes(const fmd_decay* problem, int32_t backward, size_t* bytes);
 
 /* out [rows, heads, dim] and `after`, the states behind the last rows (NULL:
@@ -1196,11 +1197,13 @@ FMD_API fmd_status fmd_decay_attention(const fmd_decay* problem, const float* st
 
 /* Gradients of q, k, v (contiguous) and of the first states, each may be
  * NULL, from those of out (g, strides g_row, g_head) and of the last states
- * (gafter, NULL: none). Deterministic. */
-FMD_API fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state, const void* g, int64_t g_row,
-                                           int64_t g_head, const float* gafter, void* dq, void* dk, void* dv,
-                                           float* dstate, void* workspace, size_t workspace_bytes, int32_t* flags,
-                                           void* stream);
+ * (gafter, NULL: none). `forward`: the forward pass's workspace as it left it
+ * (the planes of q, k and v that float32 heads of up to 64 values need), or
+ * NULL. Deterministic. */
+FMD_API fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state, const void* forward,
+                                           const void* g, int64_t g_row, int64_t g_head, const float* gafter, void* dq,
+                                           void* dk, void* dv, float* dstate, void* workspace, size_t workspace_bytes,
+                                           int32_t* flags, void* stream);
 
 /* One row of each of `rows` sequences: state [rows, heads, dim, dim] moves on
  * in place. offsets and batch are not used; any strides. */

@@ -449,9 +449,9 @@ def test_bad_arguments_of_the_entry_points_launch_nothing():
     assert lib.fmd_decay_attention(f, None, None, None, None, 0, None, None) == 1
     assert lib.fmd_decay_attention(problem(rows=4000, type=0), None, p, p, p, 8, None, None) == 4
     assert lib.fmd_decay_attention(f, odd, p, None, None, 0, None, None) == 3
-    assert lib.fmd_decay_attention_bwd(f, None, None, 32, 16, None, p, p, p, None, None, 0, None, None) == 1
-    assert lib.fmd_decay_attention_bwd(f, None, p, 33, 16, None, p, p, p, None, None, 0, None, None) == 3
-    assert lib.fmd_decay_attention_bwd(problem(rows=4000, type=0), None, p, 32, 16, None, p, p, p, p, p, need - 1, None, None) == 4
+    assert lib.fmd_decay_attention_bwd(f, None, None, None, 32, 16, None, p, p, p, None, None, 0, None, None) == 1
+    assert lib.fmd_decay_attention_bwd(f, None, None, p, 33, 16, None, p, p, p, None, None, 0, None, None) == 3
+    assert lib.fmd_decay_attention_bwd(problem(rows=4000, type=0), None, None, p, 32, 16, None, p, p, p, p, p, need - 1, None, None) == 4
     assert lib.fmd_decay_attention_step(f, None, p, None) == 1
     assert lib.fmd_decay_attention_step(f, odd, p, None) == 3
     assert lib.fmd_decay_attention_step(problem(rows=0), None, None, None) == 0

@@ -3,7 +3,8 @@
 The bounds follow the roundings: u = half the distance of neighbouring values of the stored type (2^-24 or 2^-8 relative),
 for the result and for h, da and db, which are operands of further products; and the sums: n products of bfloat16 are added
 16 at a time into FP32 that is cut off, 2^-23 a step; in float32 a sum starts anew every 128 values (8 steps for the large
-products, and what the small ones and the planes leave out is below 8 units of 2^-24), and the partial sums are added."""
+products, and what the small ones and the planes leave out is below 8 units of 2^-24), and the partial sums are added; a few
+rows are added up on the FP32 cores, 32 sums side by side."""
 import ctypes
 import math
 
@@ -21,7 +22,7 @@ E32 = 2.0 ** -24
 
 def sums(n, dtype):
     """Units of sum |a||b| that a sum of n products may be off by."""
-    return E32 * (n / 8 + 8 if dtype == B16 else 24 + n / 128)
+    return E32 * (n / 8 + 8 if dtype == B16 else 24 + n / 32)
 
 
 def act_of(a, kind):
