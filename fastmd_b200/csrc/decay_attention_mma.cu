@@ -12,12 +12,14 @@
 // small ones first.
 //
 // states_kernel does the last line alone, for what a segment adds to the matrix or for the matrix behind a sequence; in
-// bfloat16 with three planes of b' where the matrix itself is a result, so that it is exact to FP32.
+// bfloat16 with three planes of b' where the matrix itself is a result, so that it is exact to FP32. There is room for one
+// chunk's planes, so a chunk goes by halves: one half's rows are weighed while the other's products run, and its sums are
+// taken a chunk later.
 //
 // Warps, after the workers (8 or 16 of them: thread = row of the chunk and a part of the pairs or columns; for the matrix
 // its row, and a part of its columns):
-//   TMA: a, b, c of one chunk after the other through a ring of slots
-//   TMA: the output, out of c's slot, which then goes back to the ring (the last chunk's rows by the workers themselves)
+//   TMA: a, b, c of one chunk after the other through a ring of slots; the output out of c's slot before that is filled again
+//   (the last chunk's rows by the workers themselves)
 //   one thread issues the products, each as soon as what it needs is there: f (S of this chunk), b'^T c (b'), s of the next
 //   chunk, n (p). What goes from chunk to chunk is S alone: while f runs the workers weigh the pairs.
 // What lies in TMEM: s and p in its place (each thread overwrites what it has read; where there is room two by turns), f,
@@ -53,7 +55,7 @@ struct RowsShape : Shape<KS, P> {
     using S = Shape<KS, P>;
     // Two blocks an SM where they fit, of eight workers each; else sixteen in one block, which hide each other's waits.
     static constexpr int kBlocks = P == 1 && KS <= 4 ? 2 : 1;
-    static constexpr int kGroups = kBlocks == 2 ? 2 : 4, kWorkers = 128 * kGroups, kThreads = kWorkers + 96;
+    static constexpr int kGroups = kBlocks == 2 ? 2 : 4, kWorkers = 128 * kGroups, kThreads = kWorkers + 64;
     static constexpr int kColumns = S::kDim / kGroups, kPairs = kTile / kGroups;  // of a thread
     static constexpr int kSize = P == 3 ? 4 : 2, kOutPanels = (S::kDim * kSize + 127) / 128;  // of the output
     static constexpr int kSlots = P == 3 ? 4 : 5;
@@ -77,13 +79,24 @@ struct StatesShape : Shape<KS, P> {
     static constexpr int kMore = PLANES - P;                 // planes of b' beside the slots
     static constexpr int kSlots = P == 3 || PLANES == 3 ? 4 : 6;
     static constexpr size_t kBytes = kSlots * S::kSlotBytes + kMore * S::kTileBytes + kPanelBytes + 1024;
-    static constexpr uint32_t kTmem = KS <= 2 ? 32 : KS <= 4 ? 64 : 128;
+    static constexpr uint32_t kTmem = KS <= 2 ? 64 : KS <= 4 ? 128 : 256;  // two sums by turns
 };
 
 template <int SLOTS>
 struct Ctrl {
     Ring<SLOTS> ring;
     uint64_t pairs, far, ready, weights, added, out, matrix, stored;
+    uint64_t drain;
+    uint32_t tmem;
+    int32_t abort;
+};
+
+// ready, freed: of the halves of a chunk; added, taken: of two sums by turns, since nobody may run a phase of a barrier ahead of
+// a wait that has not looked yet.
+template <int SLOTS>
+struct StatesCtrl {
+    Ring<SLOTS> ring;
+    uint64_t ready[2], freed[2], added[2], taken[2];
     uint64_t drain;
     uint32_t tmem;
     int32_t abort;
@@ -109,10 +122,10 @@ __device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t
         : "memory");
 }
 
-// D (+)= A^T B over `steps` steps of 16 rows of both: the columns of A are the product's M index.
-__device__ __forceinline__ void product_columns(uint32_t d, uint32_t a, uint32_t b, int steps, uint32_t idesc, bool add) {
+// D (+)= A^T B over steps [from, to) of 16 rows of both: the columns of A are the product's M index.
+__device__ __forceinline__ void product_columns(uint32_t d, uint32_t a, uint32_t b, int from, int to, uint32_t idesc, bool add) {
     const uint32_t ad = columns_desc(a), bd = columns_desc(b);
-    for (int k = 0; k < steps; ++k) mma(d, ad + k * 128, bd + k * 128, idesc, add || k > 0);
+    for (int k = from; k < to; ++k) mma(d, ad + k * 128, bd + k * 128, idesc, add || k > from);
 }
 
 // D (+)= A B: the rows of A the product's M index, those of B (panels `panel` bytes apart) its inner index.
@@ -241,8 +254,9 @@ __device__ __forceinline__ void open_block(Ctrl<SLOTS>& ctl, int workers) {
 }
 
 // The copies of a walk, tile i by load(i, slot, barrier); then until their slots are released, or have landed.
-template <int SLOTS, typename Load>
-__device__ __forceinline__ void feed_tiles(Ctrl<SLOTS>& ctl, volatile int32_t* abort, int count, uint32_t bytes, Load load) {
+template <typename Control, typename Load>
+__device__ __forceinline__ void feed_tiles(Control& ctl, volatile int32_t* abort, int count, uint32_t bytes, Load load) {
+    constexpr int SLOTS = sizeof(ctl.ring.full) / sizeof(ctl.ring.full[0]);
     int slot = 0, armed = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -361,25 +375,42 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
     const uint32_t tmem = ctl.tmem;
 
     if (warp == kFeeder) {
-        if (lane == 0)
-            feed_tiles(ctl, abort, 3 * walk.chunks, S::kSlotBytes, [&](int i, int slot, uint64_t* bar) {
-                const int chunk = i / 3, what = i - 3 * chunk;
-                load_tile<KS, P>(su32(ring + slot * S::kSlotBytes), what == 0 ? &maps.a : what == 1 ? &maps.b : &maps.c, bar,
-                                 head, walk.first(chunk), d.rows);
-            });
-    } else if (warp == kFeeder + 2) {
-        if (lane == 0)
-            for (int i = 0; i < walk.chunks && mbar_wait(&ctl.stored, uint32_t(i) & 1u, abort); ++i) {
-                const int slot = (3 * i + 2) % S::kSlots;
-                if (walk.count(i) == kTile) {
+        if (lane == 0) {
+            const int tiles = 3 * walk.chunks;
+            uint32_t phases = 0;  // of the slots' releases after a and b
+            // tile i's slot is free again: after c's, once the output has left it
+            auto released = [&](int i) {
+                const int slot = i % S::kSlots, chunk = i / 3;
+                if (i % 3 != 2) {
+                    const bool got = mbar_wait(&ctl.ring.empty[slot], phases >> slot & 1u, abort);
+                    phases ^= 1u << slot;
+                    return got;
+                }
+                if (!mbar_wait(&ctl.stored, uint32_t(chunk) & 1u, abort)) return false;
+                if (walk.count(chunk) == kTile) {
                     for (int p = 0; p < S::kOutPanels; ++p)
                         tma_store_4d(&maps.out, su32(ring + slot * S::kSlotBytes + p * kPanelBytes), p * (128 / S::kSize), 0,
-                                     head, walk.first(i));
+                                     head, walk.first(chunk));
                     asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
                 }
-                mbar_arrive(&ctl.ring.empty[slot]);
+                return true;
+            };
+            bool ok = true;
+            int armed = 0;
+            for (int i = 0; i < tiles && ok; ++i) {
+                const int slot = i % S::kSlots, chunk = i / 3, what = i - 3 * chunk;
+                if (i >= S::kSlots && !(ok = released(i - S::kSlots))) break;
+                mbar_expect_tx(&ctl.ring.full[slot], S::kSlotBytes);
+                load_tile<KS, P>(su32(ring + slot * S::kSlotBytes), what == 0 ? &maps.a : what == 1 ? &maps.b : &maps.c,
+                                 &ctl.ring.full[slot], head, walk.first(chunk), d.rows);
+                armed = i + 1;
             }
-        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+            for (int i = max(0, armed - S::kSlots); i < armed; ++i) {
+                if (ok) ok = released(i);
+                if (!ok) mbar_wait(&ctl.ring.full[i % S::kSlots], uint32_t(i / S::kSlots) & 1u, abort, true);
+            }
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        }
     } else if (warp > kFeeder) {
         const uint32_t base = uniform(tmem), first_slot = uniform(su32(ring)), planes = uniform(su32(matrix));
         const int count = uniform(walk.chunks), last = uniform(walk.count(walk.chunks - 1));
@@ -432,7 +463,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
             if (elect_one()) {
 #pragma unroll
                 for (int q = P == 1 ? 5 : 0; q < 6; ++q)
-                    product_columns(near, b + first_plane(q) * S::kTileBytes, c + second_plane(q) * S::kTileBytes, steps, add_desc,
+                    product_columns(near, b + first_plane(q) * S::kTileBytes, c + second_plane(q) * S::kTileBytes, 0, steps, add_desc,
                                     P != 1 && q > 0);
                 tc_commit(&ctl.added);
                 tc_commit(&ctl.ring.empty[(3 * i + 1) % S::kSlots]);
@@ -643,7 +674,7 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
     extern __shared__ unsigned char raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     unsigned char* more = ring + S::kSlots * S::kSlotBytes;
-    __shared__ Ctrl<S::kSlots> ctl;
+    __shared__ StatesCtrl<S::kSlots> ctl;
     volatile int32_t* abort = &ctl.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned which = blockIdx.x % unsigned(all.count), place = blockIdx.x / unsigned(all.count);
@@ -655,7 +686,18 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
     const Stretch s = block_stretch(d, place / unsigned(d.heads));
     if (s.rows == 0 && !whole) return;
     const Walk walk(s, d);
-    open_block(ctl, kFeeder);
+    if (threadIdx.x == 0) {
+        init_ring(ctl.ring);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ctl.ready[i], kFeeder / 2);
+            mbar_init(&ctl.freed[i], 1);
+            mbar_init(&ctl.added[i], 1);
+            mbar_init(&ctl.taken[i], kFeeder);
+        }
+        mbar_init(&ctl.drain, 1);
+        ctl.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     if (warp == kFeeder + 1) tmem_alloc<S::kTmem>(&ctl.tmem);
     tc_fence_before();
     __syncthreads();
@@ -675,27 +717,37 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
         auto slot = [&](int i) { return first_slot + uint32_t(i % S::kSlots) * S::kSlotBytes; };
         bool ok = true, issued = false;
         for (int i = 0; i < count && ok; ++i) {
-            ok = landed(ctl.ring, 2 * i, abort) && landed(ctl.ring, 2 * i + 1, abort) &&
-                 warp_wait(&ctl.ready, uint32_t(i) & 1u, abort);
-            if (!ok) break;
-            tc_fence_after();
+            const uint32_t sum = base + uint32_t(i & 1) * S::kDim, b = slot(2 * i), c = slot(2 * i + 1);
             const int steps = ((i + 1 == count ? last : kTile) + 15) / 16;
-            const uint32_t b = slot(2 * i), c = slot(2 * i + 1);
-            if (elect_one()) {
-                if (P == 1) {
+            ok = landed(ctl.ring, 2 * i, abort) && landed(ctl.ring, 2 * i + 1, abort);
+            if (ok && i > 1) ok = warp_wait(&ctl.taken[i & 1], (uint32_t(i >> 1) & 1u) ^ 1u, abort);
 #pragma unroll
-                    for (int q = PLANES - 1; q >= 0; --q)
-                        product_columns(base, q == 0 ? b : planes + (q - 1) * S::kTileBytes, c, steps, desc, q < PLANES - 1);
-                } else {
+            for (int half = 0; half < 2; ++half) {
+                ok = ok && warp_wait(&ctl.ready[half], uint32_t(i) & 1u, abort);
+                if (!ok) break;
+                tc_fence_after();
+                const int from = 4 * half, to = min(4 * half + 4, steps);
+                if (elect_one()) {
+                    if (P == 1) {
 #pragma unroll
-                    for (int q = 0; q < 6; ++q)
-                        product_columns(base, b + first_plane(q) * S::kTileBytes, c + second_plane(q) * S::kTileBytes, steps, desc, q > 0);
+                        for (int q = PLANES - 1; q >= 0; --q)
+                            product_columns(sum, q == 0 ? b : planes + (q - 1) * S::kTileBytes, c, from, to, desc,
+                                            half > 0 || q < PLANES - 1);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 6; ++q)
+                            product_columns(sum, b + first_plane(q) * S::kTileBytes, c + second_plane(q) * S::kTileBytes, from, to,
+                                            desc, half > 0 || q > 0);
+                    }
+                    tc_commit(&ctl.freed[half]);
+                    if (half > 0) {
+                        tc_commit(&ctl.added[i & 1]);
+                        tc_commit(&ctl.ring.empty[(2 * i) % S::kSlots]);
+                        tc_commit(&ctl.ring.empty[(2 * i + 1) % S::kSlots]);
+                    }
                 }
-                tc_commit(&ctl.added);
-                tc_commit(&ctl.ring.empty[(2 * i) % S::kSlots]);
-                tc_commit(&ctl.ring.empty[(2 * i + 1) % S::kSlots]);
+                issued = true;
             }
-            issued = true;
         }
         if (!ok && issued) {
             if (elect_one()) tc_commit(&ctl.drain);
@@ -712,27 +764,38 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
 #pragma unroll
             for (int i = 0; i < kColumns; ++i) state[i] = 0.0f;
         }
+        const int half = r >> 6;
         bool ok = true;
-        for (int i = 0; i < walk.chunks; ++i) {
+        auto take = [&](int i) {  // the sums of chunk i
+            if (!worker_wait(&ctl.added[i & 1], uint32_t(i >> 1) & 1u, abort)) return false;
+            tc_fence_after();
+            add_columns(at + uint32_t(i & 1) * S::kDim, exp2f(float(walk.count(i)) * l2), state);
+            tc_fence_before();
+            warp_arrive(&ctl.taken[i & 1]);
+            return true;
+        };
+        for (int i = 0; i < walk.chunks && ok; ++i) {
             const int count = walk.count(i), tile_b = 2 * i, tile_c = 2 * i + 1;
             ok = worker_wait(&ctl.ring.full[tile_b % S::kSlots], uint32_t(tile_b / S::kSlots) & 1u, abort);
+            if (S::kMore > 0 && ok && i > 0) ok = worker_wait(&ctl.freed[half], uint32_t(i - 1) & 1u, abort);
             if (!ok) break;
             const float weight = d.add * exp2f(float(d.later ? r + 1 : count - 1 - r) * l2);
             weigh_row<KS, P, PLANES, S::kGroups>(ring + (tile_b % S::kSlots) * S::kSlotBytes, more, r, group, weight, r < count);
             if (count < kTile) {
                 ok = worker_wait(&ctl.ring.full[tile_c % S::kSlots], uint32_t(tile_c / S::kSlots) & 1u, abort);
                 if (!ok) break;
-                zero_rows(ring + (tile_c % S::kSlots) * S::kSlotBytes, P * S::kPanels, kPanelBytes, count, (count + 15) & ~15,
-                          threadIdx.x, S::kWorkers);
+                const int first = max(count, 64 * half), end = min((count + 15) & ~15, 64 * half + 64);
+                if (first < end)
+                    zero_rows(ring + (tile_c % S::kSlots) * S::kSlotBytes, P * S::kPanels, kPanelBytes, first, end,
+                              group * 64 + (r & 63), S::kWorkers / 2);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            warp_arrive(&ctl.ready);
-            ok = worker_wait(&ctl.added, uint32_t(i) & 1u, abort);
+            if (S::kMore == 0 && i > 0) ok = worker_wait(&ctl.freed[half], uint32_t(i - 1) & 1u, abort);
             if (!ok) break;
-            tc_fence_after();
-            add_columns(at, exp2f(float(count) * l2), state);
-            tc_fence_before();
+            warp_arrive(&ctl.ready[half]);
+            if (i > 0) ok = take(i - 1);
         }
+        if (ok && walk.chunks > 0) ok = take(walk.chunks - 1);
         if (ok && r < d.dim) {
             const int64_t size = int64_t(d.dim) * d.dim;
             float* out = whole ? d.after + (int64_t(s.b) * d.heads + head) * size
