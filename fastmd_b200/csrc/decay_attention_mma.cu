@@ -20,10 +20,9 @@
 // its row, and a part of its columns):
 //   TMA: a, b, c of one chunk after the other through a ring of slots; the output out of c's slot before that is filled again
 //   (the last chunk's rows by the workers themselves)
-//   one thread issues the products, each as soon as what it needs is there: f (S of this chunk), b'^T c (b'), s of the next
-//   chunk, n (p). What goes from chunk to chunk is S alone: while f runs the workers weigh the pairs.
-// What lies in TMEM: s and p in its place (each thread overwrites what it has read; where there is room two by turns), f,
-// and b'^T c and n one after the other.
+//   one thread issues the products, each as soon as what it needs is there: f (S of this chunk), b'^T c (b'), n (p), s of the
+//   next chunk. What goes from chunk to chunk is S alone: while f runs the workers weigh the pairs.
+// What lies in TMEM: s and p in its place (each thread overwrites what it has read), n, f, b'^T c.
 //
 // Three of four blocks of 32 x 32 pairs lie to one side of the diagonal: nothing is computed above it, and below it a weight
 // is the product of one factor of the row and one of the column (a table), l^{t-u} = l^{t-a} l^{a-u}, neither above 1.
@@ -65,9 +64,9 @@ struct RowsShape : Shape<KS, P> {
     static constexpr uint32_t kMatrix = kPlanes * kPlane > kPanelBytes ? kPlanes * kPlane : kPanelBytes;
     static constexpr size_t kBytes = kSlots * S::kSlotBytes + kMatrix + 1024;
     static constexpr uint32_t kTmem = kBlocks == 2 ? 256 : 512;
-    static constexpr int kBuffers = kBlocks == 2 ? 1 : 2;    // of the pairs
-    // columns: the pairs at 0, their third plane, n (before it b'^T c), f
-    static constexpr uint32_t kThird = 128 * kBuffers, kNear = kThird + (P == 3 ? 64 : 0), kFar = kNear + S::kDim;
+    // columns: the pairs at 0, their third plane, n, f, and b'^T c (where two blocks share TMEM: in n's place before it)
+    static constexpr uint32_t kThird = 128, kNear = kThird + (P == 3 ? 64 : 0), kFar = kNear + S::kDim;
+    static constexpr uint32_t kSum = kBlocks == 2 ? kNear : kFar + S::kDim;
 };
 
 // PLANES: of b'.
@@ -418,19 +417,18 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                        add_desc = out_desc | 1u << 15;
         auto slot = [&](int i) { return first_slot + uint32_t(i % S::kSlots) * S::kSlotBytes; };
         bool ok = true, issued = false;
-        auto at_pairs = [&](int i) { return base + uint32_t(i % S::kBuffers) * 128u; };
         auto pairs = [&](int i) {  // over pairs whose product has been issued
             ok = ok && landed(ctl.ring, 3 * i, abort) && landed(ctl.ring, 3 * i + 1, abort);
             if (!ok) return;
             tc_fence_after();
-            const uint32_t a = slot(3 * i), b = slot(3 * i + 1), to = at_pairs(i);
+            const uint32_t a = slot(3 * i), b = slot(3 * i + 1);
             if (elect_one()) {
                 if (P == 1) {
-                    product_rows<KS>(to, a, b, pairs_desc);
+                    product_rows<KS>(base, a, b, pairs_desc);
                 } else {
 #pragma unroll
                     for (int q = 0; q < 6; ++q)
-                        product_rows<KS>(to, a + first_plane(q) * S::kTileBytes, b + second_plane(q) * S::kTileBytes, pairs_desc,
+                        product_rows<KS>(base, a + first_plane(q) * S::kTileBytes, b + second_plane(q) * S::kTileBytes, pairs_desc,
                                          q > 0);
                 }
                 tc_commit(&ctl.pairs);
@@ -442,7 +440,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
             ok = warp_wait(&ctl.matrix, uint32_t(i) & 1u, abort);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t a = slot(3 * i), b = slot(3 * i + 1), c = slot(3 * i + 2), far = base + S::kFar, near = base + S::kNear;
+            const uint32_t a = slot(3 * i), b = slot(3 * i + 1), c = slot(3 * i + 2), far = base + S::kFar, near = base + S::kNear, sum = base + S::kSum;
             if (elect_one()) {
                 if (P == 1) {
                     product_matrix<KS>(far, a, planes + S::kPlane, S::kPanel, out_desc, false);
@@ -463,24 +461,17 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
             if (elect_one()) {
 #pragma unroll
                 for (int q = P == 1 ? 5 : 0; q < 6; ++q)
-                    product_columns(near, b + first_plane(q) * S::kTileBytes, c + second_plane(q) * S::kTileBytes, 0, steps, add_desc,
+                    product_columns(sum, b + first_plane(q) * S::kTileBytes, c + second_plane(q) * S::kTileBytes, 0, steps, add_desc,
                                     P != 1 && q > 0);
                 tc_commit(&ctl.added);
                 tc_commit(&ctl.ring.empty[(3 * i + 1) % S::kSlots]);
             }
-            // the next pairs before what the workers still prepare, if their tiles have landed
-            bool early = S::kBuffers == 2 && i + 1 < count;
-            for (int e = 3; e < 5 && early; ++e)
-                early = __all_sync(0xffffffffu, mbar_try_wait(su32(&ctl.ring.full[(3 * i + e) % S::kSlots]),
-                                                              uint32_t((3 * i + e) / S::kSlots) & 1u));
-            if (early) pairs(i + 1);
             ok = ok && warp_wait(&ctl.weights, uint32_t(i) & 1u, abort);
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
-                const uint32_t p = at_pairs(i);
                 if (P == 1) {
-                    product_weights<8, S::kPairs / 16, S::kPairs>(near, p, c, steps, out_desc, false);
+                    product_weights<8, S::kPairs / 16, S::kPairs>(near, base, c, steps, out_desc, false);
                 } else {
 #pragma unroll
                     for (int q = 0; q < 6; ++q) {
@@ -488,12 +479,12 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                         if (first_plane(q) == 2)
                             product_weights<8, 8, 0>(near, base + S::kThird, from, steps, out_desc, q > 0);
                         else
-                            product_weights<8, 2, 32>(near, p + 16 * first_plane(q), from, steps, out_desc, q > 0);
+                            product_weights<8, 2, 32>(near, base + 16 * first_plane(q), from, steps, out_desc, q > 0);
                     }
                 }
                 tc_commit(&ctl.out);
             }
-            if (!early && i + 1 < count) pairs(i + 1);
+            if (i + 1 < count) pairs(i + 1);  // not before n: the workers wait for that (5 % slower)
         }
         if (!ok && issued) {  // the products in flight end before TMEM is freed
             if (elect_one()) tc_commit(&ctl.drain);
@@ -503,8 +494,8 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
         using T = typename std::conditional<P == 1, __nv_bfloat16, float>::type;
         const int group = warp >> 2, r = threadIdx.x & 127, col0 = group * kColumns, pair0 = group * S::kPairs;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t at_third = tmem + lanes + S::kThird + pair0 / 2, at_near = tmem + lanes + S::kNear + col0,
-                       at_far = tmem + lanes + S::kFar + col0;
+        const uint32_t at_pairs = tmem + lanes + pair0, at_third = tmem + lanes + S::kThird + pair0 / 2, at_near = tmem + lanes + S::kNear + col0,
+                       at_far = tmem + lanes + S::kFar + col0, at_sum = tmem + lanes + S::kSum + col0;
         const float l2 = log2_decay(d, head);
         auto power = [&](int n) { return P == 1 ? ex2(float(n) * l2) : exp2f(float(n) * l2); };
         const bool holds = r < S::kDim;
@@ -558,7 +549,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                 keep = power(count);
                 reach = d.far * power(d.later ? count - 1 - r : r + 1);
             }
-            const uint32_t parity = uint32_t(i) & 1u, at_pairs = tmem + lanes + uint32_t(i % S::kBuffers) * 128u + pair0;
+            const uint32_t parity = uint32_t(i) & 1u;
             if (!worker_wait(&ctl.pairs, parity, abort)) break;
             const int tile_b = 3 * i + 1, tile_c = 3 * i + 2;
             if (!worker_wait(&ctl.ring.full[tile_b % S::kSlots], uint32_t(tile_b / S::kSlots) & 1u, abort)) break;
@@ -596,12 +587,18 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                     tmem_store16(q == 2 ? at_third : at + 16 * q, p);
                 }
             }
+            tmem_wait_st();
+            if (S::kSum != S::kNear) {
+                tc_fence_before();
+                warp_arrive(&ctl.weights);
+            }
             if (!worker_wait(&ctl.added, parity, abort)) break;
             tc_fence_after();
-            add_columns(at_near, keep, state);
-            tmem_wait_st();
-            tc_fence_before();
-            warp_arrive(&ctl.weights);
+            add_columns(at_sum, keep, state);
+            if (S::kSum == S::kNear) {
+                tc_fence_before();
+                warp_arrive(&ctl.weights);
+            }
 
             if (!worker_wait(&ctl.far, parity, abort)) break;
             tc_fence_after();
