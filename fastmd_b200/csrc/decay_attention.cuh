@@ -105,9 +105,10 @@ __device__ __forceinline__ void check_offsets(const Decay& d, int64_t b) {
         raise_flag(d.flags, FMD_FLAG_INDEX_RANGE);
 }
 
-// l^n; a logarithm above zero counts as zero, and nothing of -inf is left after a row.
+// l^n; a logarithm above zero counts as zero, and nothing of -inf is left after a row. NaN stays NaN.
 __device__ __forceinline__ float log2_decay(const Decay& d, int head) {
-    return fmaxf(fminf(d.log_decay[head], 0.0f), -1.0e4f) * kLog2e;
+    const float log = d.log_decay[head];
+    return (log != log ? log : fmaxf(fminf(log, 0.0f), -1.0e4f)) * kLog2e;
 }
 
 // What the segments add to the matrix (whole sequences: the matrix behind them, in `after`), and the rows. bfloat16:

@@ -81,10 +81,12 @@ struct StatesShape : Shape<KS, P> {
     static constexpr uint32_t kTmem = KS <= 2 ? 64 : KS <= 4 ? 128 : 256;  // two sums by turns
 };
 
+// stored: of two chunks by turns. Nothing but the time of a copy keeps the workers from finishing the next chunk before the
+// warp that copies has looked at the last one; they cannot finish two, since the copies of the second come after that look.
 template <int SLOTS>
 struct Ctrl {
     Ring<SLOTS> ring;
-    uint64_t pairs, far, ready, weights, added, out, matrix, stored;
+    uint64_t pairs, far, ready, weights, added, out, matrix, stored[2];
     uint64_t drain;
     uint32_t tmem;
     int32_t abort;
@@ -245,7 +247,7 @@ __device__ __forceinline__ void open_block(Ctrl<SLOTS>& ctl, int workers) {
         mbar_init(&ctl.added, 1);
         mbar_init(&ctl.out, 1);
         mbar_init(&ctl.matrix, uint32_t(workers));
-        mbar_init(&ctl.stored, uint32_t(workers));
+        for (int i = 0; i < 2; ++i) mbar_init(&ctl.stored[i], uint32_t(workers));
         mbar_init(&ctl.drain, 1);
         ctl.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -385,7 +387,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                     phases ^= 1u << slot;
                     return got;
                 }
-                if (!mbar_wait(&ctl.stored, uint32_t(chunk) & 1u, abort)) return false;
+                if (!mbar_wait(&ctl.stored[chunk & 1], uint32_t(chunk >> 1) & 1u, abort)) return false;
                 if (walk.count(chunk) == kTile) {
                     for (int p = 0; p < S::kOutPanels; ++p)
                         tma_store_4d(&maps.out, su32(ring + slot * S::kSlotBytes + p * kPanelBytes), p * (128 / S::kSize), 0,
@@ -648,7 +650,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                 turn_pieces<kWide>(slot + warp * (kWide * 512), row);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            warp_arrive(&ctl.stored);
+            warp_arrive(&ctl.stored[i & 1]);
             if (count < kTile) {
                 const int first_row = (warp & 3) * 32, left = min(kColumns, d.dim - col0) * S::kSize / 16;
                 T* out = static_cast<T*>(d.out) + (int64_t(walk.first(i) + first_row) * d.heads + head) * d.dim + col0;

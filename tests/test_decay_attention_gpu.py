@@ -240,6 +240,44 @@ def test_strong_and_no_decay(cuda, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,dim", [(F32, 64), (F32, 72), (B16, 64)], ids=["planes", "f32", "b16"])
+def test_a_decay_of_nan_gives_nan(cuda, dtype, dim):
+    """It is not taken for one of the values that count as 0, and other heads do not see it."""
+    q, k, v, _, state, _, offsets = make([300, 7], 2, dim, dtype)
+    log = torch.tensor([math.nan, -0.1], device="cuda")
+    want = decay_attention(q, k, v, log.nan_to_num(), offsets, state, return_state=True)
+    got = decay_attention(q, k, v, log, offsets, state, return_state=True)
+    for x, y in zip(got, want):
+        assert torch.equal(x[:, 1], y[:, 1])
+    assert torch.isnan(got[1][0, 0]).all() and torch.isnan(got[0][:, 0]).all()
+    now = state.clone()
+    assert torch.isnan(decay_attention_step(q[:2], k[:2], v[:2], log, now)[:, 0]).all() and torch.isfinite(now[:, 1]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,heads,dim", [(F32, 17, 64), (F32, 17, 128), (B16, 17, 128)], ids=["planes", "f32", "b16"])
+def test_arrays_past_32_bits(cuda, dtype, heads, dim):
+    """More than 2^31 values an array: the last sequence's rows and those of its first state."""
+    tail = 300
+    rows = 2 ** 31 // (heads * dim) + 5000
+    x = torch.zeros(rows, heads, dim, device="cuda", dtype=dtype)
+    q, k, v, g, state, gafter, _ = make([tail], heads, dim, dtype)
+    x[-tail:] = q
+    y = x.clone()
+    y[-tail:] = k
+    offsets = torch.tensor([0, 900, rows - tail, rows], device="cuda")
+    states = torch.cat((torch.zeros_like(state), torch.zeros_like(state), state))
+    log = decays(heads)
+    want, err = reference(q, k, k, log, [tail], state, dim ** -0.5)
+    out, after = decay_attention(x, y, y, log, offsets, states, return_state=True)
+    check(out[-tail:], want["out"], err["out"], "out")
+    check(after[2:], want["after"], err["after"], "after")
+    assert not out[:-tail].any() and not after[:2].any()
+    del x, y, out
+    torch.cuda.empty_cache()
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
 def test_strides_and_parts(cuda, dtype):
     sizes, heads, dim = [100, 61], 3, 40
