@@ -267,8 +267,14 @@ __device__ __forceinline__ void pack_halves(const float* v, uint4 (&w)[2], float
     float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(v[i]));
-    const int e = int(__float_as_uint(most) >> 23);
-    const int shift = e == 255 ? 0 : min(127 + 14 - e, 100);  // the largest becomes 2^14 .. 2^15
+    int e = int(__float_as_uint(most) >> 23);
+    if (e == 255) {  // of the finite ones
+        most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(v[i]) < __int_as_float(0x7f800000) ? fabsf(v[i]) : 0.0f);
+        e = int(__float_as_uint(most) >> 23);
+    }
+    const int shift = min(127 + 14 - e, 100);  // the largest becomes 2^14 .. 2^15
     const float up = __uint_as_float(uint32_t(127 + shift) << 23);
     unit = __uint_as_float(uint32_t(127 - shift) << 23);
     uint32_t* p = reinterpret_cast<uint32_t*>(w);

@@ -210,6 +210,44 @@ def test_values_that_are_not_finite_stay_in_their_row(cuda, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+def test_an_infinite_weight_leaves_other_units_their_gradients(cuda, kind):
+    """act(a) of one hidden unit is infinite in some rows, those of its neighbours small or beyond float16: bfloat16."""
+    x, wg, wu, wd, g = make(40, 16, 32, 24, B16)
+    x = x.abs() + 0.1
+    wg[5] = wg[5].abs() * 1e5
+    wg[6] = wg[6].abs() * 1e-2
+    wg[7, 0] = float("inf")
+    leaves = [t.requires_grad_() for t in (x, wg, wu, wd)]
+    (dup,) = torch.autograd.grad(gated_feed_forward(*leaves, activation=kind), leaves[2:3], g)
+    others = [i for i in range(32) if i != 7]
+    want, err = reference(x, wg[others], wu[others], wd[:, others], g, kind)
+    check(dup[others], want["dup"], err["dup"], "dup", 40)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+def test_arrays_past_32_bits(cuda, dtype):
+    """More than 2^31 values of the hidden rows: the last rows of the result and their gradient."""
+    hidden, tail = 8200, 200
+    rows = 2 ** 31 // hidden + 1000
+    x, wg, wu, wd, g = make(tail, 16, hidden, 16, dtype)
+    many, more = (torch.zeros(rows, 16, device="cuda", dtype=dtype) for _ in range(2))
+    many[-tail:], more[-tail:] = x, g
+    want, err = reference(x, wg, wu, wd, g, "silu")
+    leaves = [t.requires_grad_() for t in (many, wg, wu, wd)]
+    y = gated_feed_forward(*leaves)
+    grads = torch.autograd.grad(y, leaves, more)
+    check(y.detach()[-tail:], want["y"], err["y"], "y", tail * hidden)
+    check(grads[0][-tail:], want["dx"], err["dx"], "dx", tail * hidden)
+    for name, got in zip(("dgate", "dup", "ddown"), grads[1:]):
+        check(got, want[name], err[name], name, tail * hidden)
+    assert not y[:-tail].any() and not grads[0][:-tail].any()
+    del y, grads, got
+    torch.cuda.empty_cache()
+
+
+@gpu
 def test_large_values(cuda):
     """Projections far beyond the activations' range, and finite values beyond the largest bfloat16."""
     for dtype in (F32, B16):
