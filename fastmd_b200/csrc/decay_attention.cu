@@ -14,6 +14,8 @@ constexpr int kThreads = 256;
 // loaded at a time.
 __global__ void __launch_bounds__(kThreads) carry_kernel(const __grid_constant__ Decays all) {
     constexpr int kAhead = 16;
+    dependents_may_start();
+    wait_for_the_kernel_ahead();
     const Decay& d = all.d[blockIdx.z];
     const int b = blockIdx.x / d.heads, head = blockIdx.x % d.heads;
     const int size = d.dim * d.dim, at = (blockIdx.y * kThreads + threadIdx.x) * 4;
@@ -72,6 +74,7 @@ struct SplitArgs {
 };
 
 __global__ void __launch_bounds__(kThreads) split_kernel(const SplitArgs a) {
+    dependents_may_start();
     const int t = blockIdx.y, per = a.dim / 8;
     const int64_t heads = a.rows * a.heads, all = heads * per;
     for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < all; i += int64_t(gridDim.x) * kThreads) {
@@ -224,8 +227,10 @@ void read_from(Decay& d, const Input& a, const Input& b, const Input& c) {
     d.c = c.data, d.c_row = c.row, d.c_head = c.head;
 }
 
-fmd_status run_states(const Decays& d, Path path, cudaStream_t s) {
-    return path == kMma ? decay_states_mma(d, s) : path == kPlanes ? decay_states_planes(d, s) : decay_states_simt(d, s);
+fmd_status run_states(const Decays& d, Path path, bool early, cudaStream_t s) {
+    return path == kMma      ? decay_states_mma(d, early, s)
+           : path == kPlanes ? decay_states_planes(d, early, s)
+                             : decay_states_simt(d, s);
 }
 
 // Passes of the recurrence over the same rows, side by side: with segments what these add comes first.
@@ -238,27 +243,31 @@ fmd_status mix(Decays all, Path path, char* workspace, cudaStream_t s) {
     const int64_t segments = decay_segments(d);
     if (segments * d.heads * all.count > INT32_MAX || int64_t(d.batch) * d.heads > INT32_MAX) return FMD_ERR_UNSUPPORTED;
     fmd_status st = FMD_OK;
+    bool early = path == kPlanes && d.rows > 0;  // behind the kernel that makes the planes
     if (length < kWhole) {
         for (int i = 0; i < all.count; ++i) {
             all.d[i].states = reinterpret_cast<float*>(workspace);
             workspace += d.rows > 0 ? matrices(d, segments) : 0;
         }
-        if (d.rows > 0 && (st = run_states(all, path, s)) != FMD_OK) return st;
-        carry_kernel<<<dim3(unsigned(d.batch) * d.heads, unsigned((d.dim * d.dim + 4 * kThreads - 1) / (4 * kThreads)),
-                            unsigned(all.count)),
-                       kThreads, 0, s>>>(all);
-        if ((st = check_launch()) != FMD_OK) return st;
+        if (d.rows > 0 && (st = run_states(all, path, early, s)) != FMD_OK) return st;
+        const dim3 grid(unsigned(d.batch) * d.heads, unsigned((d.dim * d.dim + 4 * kThreads - 1) / (4 * kThreads)),
+                        unsigned(all.count));
+        if ((st = launch_early(carry_kernel, grid, kThreads, 0, s, all)) != FMD_OK) return st;
+        early = true;
     } else {
         Decays ends{};  // those whose last matrix is asked for
         for (int i = 0; i < all.count; ++i)
             if (all.d[i].after != nullptr) ends.d[ends.count++] = all.d[i];
-        if (ends.count > 0 && (st = run_states(ends, path, s)) != FMD_OK) return st;
+        if (ends.count > 0 && (st = run_states(ends, path, early, s)) != FMD_OK) return st;
+        early = early || ends.count > 0;
     }
     Decays rows{};
     for (int i = 0; i < all.count; ++i)
         if (all.d[i].out != nullptr) rows.d[rows.count++] = all.d[i];
     if (d.rows == 0 || rows.count == 0) return FMD_OK;
-    return path == kMma ? decay_rows_mma(rows, s) : path == kPlanes ? decay_rows_planes(rows, s) : decay_rows_simt(rows, s);
+    return path == kMma      ? decay_rows_mma(rows, early, s)
+           : path == kPlanes ? decay_rows_planes(rows, early, s)
+                             : decay_rows_simt(rows, s);
 }
 
 }  // namespace

@@ -111,12 +111,13 @@ __device__ __forceinline__ float log2_decay(const Decay& d, int head) {
     return (log != log ? log : fmaxf(fminf(log, 0.0f), -1.0e4f)) * kLog2e;
 }
 
-// What the segments add to the matrix (whole sequences: the matrix behind them, in `after`), and the rows. bfloat16:
-fmd_status decay_states_mma(const Decays& d, cudaStream_t s);
-fmd_status decay_rows_mma(const Decays& d, cudaStream_t s);
+// What the segments add to the matrix (whole sequences: the matrix behind them, in `after`), and the rows; early: behind
+// another kernel of the same call, which they may overlap until they need its results. bfloat16:
+fmd_status decay_states_mma(const Decays& d, bool early, cudaStream_t s);
+fmd_status decay_rows_mma(const Decays& d, bool early, cudaStream_t s);
 // float32, heads of up to 64 values: a, b and c are three planes of bfloat16, [3][rows][heads][dim]
-fmd_status decay_states_planes(const Decays& d, cudaStream_t s);
-fmd_status decay_rows_planes(const Decays& d, cudaStream_t s);
+fmd_status decay_states_planes(const Decays& d, bool early, cudaStream_t s);
+fmd_status decay_rows_planes(const Decays& d, bool early, cudaStream_t s);
 // float32, wider heads
 fmd_status decay_states_simt(const Decays& d, cudaStream_t s);
 fmd_status decay_rows_simt(const Decays& d, cudaStream_t s);

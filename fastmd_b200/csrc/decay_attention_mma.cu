@@ -366,7 +366,10 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
     }
     if (head == 0 && threadIdx.x == 32 && index < d.batch) check_offsets(d, index);
     const Stretch s = block_stretch(d, index);
-    if (s.rows == 0) return;
+    if (s.rows == 0) {
+        wait_for_the_kernel_ahead();
+        return;
+    }
     const Walk walk(s, d);
     open_block(ctl, kFeeder);
     if (warp == kFeeder + 1) tmem_alloc<S::kTmem>(&ctl.tmem);
@@ -374,6 +377,8 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl.tmem;
+    dependents_may_start();  // with this block's TMEM in hand: they take theirs and hold it until this kernel ends
+    wait_for_the_kernel_ahead();
 
     if (warp == kFeeder) {
         if (lane == 0) {
@@ -683,7 +688,10 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
     const bool whole = d.length >= kWhole;
 
     const Stretch s = block_stretch(d, place / unsigned(d.heads));
-    if (s.rows == 0 && !whole) return;
+    if (s.rows == 0 && !whole) {
+        wait_for_the_kernel_ahead();
+        return;
+    }
     const Walk walk(s, d);
     if (threadIdx.x == 0) {
         init_ring(ctl.ring);
@@ -702,6 +710,8 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl.tmem;
+    dependents_may_start();  // with this block's TMEM in hand: they take theirs and hold it until this kernel ends
+    wait_for_the_kernel_ahead();
 
     if (warp == kFeeder) {
         if (lane == 0)
@@ -850,62 +860,64 @@ fmd_status encode(AllMaps& maps, const Decays& all, bool rows, int planes) {
 unsigned blocks_of(const Decays& d) { return unsigned(decay_segments(d.d[0]) * d.d[0].heads * d.count); }
 
 template <int KS, int P>
-fmd_status launch_rows(const AllMaps& maps, const Decays& d, cudaStream_t s) {
+fmd_status launch_rows(const AllMaps& maps, const Decays& d, bool early, cudaStream_t s) {
     using S = RowsShape<KS, P>;
     const fmd_status st = grant_dynamic_smem((const void*)rows_kernel<KS, P>, S::kBytes, true);
     if (st != FMD_OK) return st;
+    if (early) return launch_early(rows_kernel<KS, P>, blocks_of(d), S::kThreads, S::kBytes, s, maps, d);
     rows_kernel<KS, P><<<blocks_of(d), S::kThreads, S::kBytes, s>>>(maps, d);
     return check_launch();
 }
 
 template <int KS, int P, int PLANES>
-fmd_status launch_states(const AllMaps& maps, const Decays& d, cudaStream_t s) {
+fmd_status launch_states(const AllMaps& maps, const Decays& d, bool early, cudaStream_t s) {
     using S = StatesShape<KS, P, PLANES>;
     const fmd_status st = grant_dynamic_smem((const void*)states_kernel<KS, P, PLANES>, S::kBytes, true);
     if (st != FMD_OK) return st;
+    if (early) return launch_early(states_kernel<KS, P, PLANES>, blocks_of(d), S::kThreads, S::kBytes, s, maps, d);
     states_kernel<KS, P, PLANES><<<blocks_of(d), S::kThreads, S::kBytes, s>>>(maps, d);
     return check_launch();
 }
 
 template <int KS>
-fmd_status launch_states(const AllMaps& maps, const Decays& d, cudaStream_t s) {
+fmd_status launch_states(const AllMaps& maps, const Decays& d, bool early, cudaStream_t s) {
     bool after = false;
     for (int i = 0; i < d.count; ++i) after = after || d.d[i].after != nullptr;
-    return after ? launch_states<KS, 1, 3>(maps, d, s) : launch_states<KS, 1, 1>(maps, d, s);
+    return after ? launch_states<KS, 1, 3>(maps, d, early, s) : launch_states<KS, 1, 1>(maps, d, early, s);
 }
 
 }  // namespace
 
-fmd_status decay_states_mma(const Decays& d, cudaStream_t s) {
+fmd_status decay_states_mma(const Decays& d, bool early, cudaStream_t s) {
     AllMaps maps{};
     const fmd_status st = encode(maps, d, false, 1);
     if (st != FMD_OK) return st;
     const int dim = d.d[0].dim;
-    return dim <= 32 ? launch_states<2>(maps, d, s) : dim <= 64 ? launch_states<4>(maps, d, s)
-         : dim <= 96 ? launch_states<6>(maps, d, s) : launch_states<8>(maps, d, s);
+    return dim <= 32 ? launch_states<2>(maps, d, early, s) : dim <= 64 ? launch_states<4>(maps, d, early, s)
+         : dim <= 96 ? launch_states<6>(maps, d, early, s) : launch_states<8>(maps, d, early, s);
 }
 
-fmd_status decay_rows_mma(const Decays& d, cudaStream_t s) {
+fmd_status decay_rows_mma(const Decays& d, bool early, cudaStream_t s) {
     AllMaps maps{};
     const fmd_status st = encode(maps, d, true, 1);
     if (st != FMD_OK) return st;
     const int dim = d.d[0].dim;
-    return dim <= 32 ? launch_rows<2, 1>(maps, d, s) : dim <= 64 ? launch_rows<4, 1>(maps, d, s)
-         : dim <= 96 ? launch_rows<6, 1>(maps, d, s) : launch_rows<8, 1>(maps, d, s);
+    return dim <= 32 ? launch_rows<2, 1>(maps, d, early, s) : dim <= 64 ? launch_rows<4, 1>(maps, d, early, s)
+         : dim <= 96 ? launch_rows<6, 1>(maps, d, early, s) : launch_rows<8, 1>(maps, d, early, s);
 }
 
-fmd_status decay_states_planes(const Decays& d, cudaStream_t s) {
+fmd_status decay_states_planes(const Decays& d, bool early, cudaStream_t s) {
     AllMaps maps{};
     const fmd_status st = encode(maps, d, false, 3);
     if (st != FMD_OK) return st;
-    return d.d[0].dim <= 32 ? launch_states<2, 3, 3>(maps, d, s) : launch_states<4, 3, 3>(maps, d, s);
+    return d.d[0].dim <= 32 ? launch_states<2, 3, 3>(maps, d, early, s) : launch_states<4, 3, 3>(maps, d, early, s);
 }
 
-fmd_status decay_rows_planes(const Decays& d, cudaStream_t s) {
+fmd_status decay_rows_planes(const Decays& d, bool early, cudaStream_t s) {
     AllMaps maps{};
     const fmd_status st = encode(maps, d, true, 3);
     if (st != FMD_OK) return st;
-    return d.d[0].dim <= 32 ? launch_rows<2, 3>(maps, d, s) : launch_rows<4, 3>(maps, d, s);
+    return d.d[0].dim <= 32 ? launch_rows<2, 3>(maps, d, early, s) : launch_rows<4, 3>(maps, d, early, s);
 }
 
 }  // namespace fmd

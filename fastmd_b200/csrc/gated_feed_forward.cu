@@ -386,6 +386,20 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
     G::sync();
     tc_fence_after();
     const uint32_t tmem = ctl.tmem;
+    dependents_may_start();  // with this block's TMEM in hand: they take theirs and hold it until this kernel ends
+    // down in 16 bits: its weights were there before the kernel ahead, so that the first of them come while that one ends
+    constexpr bool kAhead = KIND == kDown && P == 1 && !PAIR;
+    int ahead = 0;
+    if (kAhead && warp == S::kWarps && lane == 0 && first_turn < turns_of(g)) {
+        const Place p = place_of(g, first_turn);
+        const bool pb = g.problem[0].b_panels != 0;
+        for (; ahead < min(g.slots, p.to - p.from); ++ahead) {
+            const int k = p.from + ahead;
+            mbar_expect_tx(&ctl.full[ahead], slot_bytes);
+            G::load(ring + uint32_t(ahead) * slot_bytes, &maps.b[0], su32(&ctl.full[ahead]), pb ? 0 : k * kK, p.n * g.bn, pb ? k : 0, 0);
+        }
+    }
+    wait_for_the_kernel_ahead();
 
     if (warp == S::kWarps) {
         if (lane == 0) {
@@ -411,7 +425,9 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                             break;
                         }
                         const uint32_t bar = first_full + uint32_t(slot) * 8u;
-                        if (!PAIR || rank == 0) mbar_expect_tx(&ctl.full[slot], PAIR ? 2 * slot_bytes : slot_bytes);
+                        const bool given = kAhead && ahead > 0;  // B is there, or on its way
+                        if (given) --ahead;
+                        else if (!PAIR || rank == 0) mbar_expect_tx(&ctl.full[slot], PAIR ? 2 * slot_bytes : slot_bytes);
                         armed |= 1u << slot;
                         const uint32_t at = ring + uint32_t(slot) * slot_bytes;
                         const int k = step - base, k0 = k * kK;
@@ -438,7 +454,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                                     G::load(b, mb, bar, 0, k0, n0 / 64, i);
                                 else
                                     for (int c = 0; c < columns / 64; ++c) G::load(b + c * kPanel, mb, bar, n0 + 64 * c, k0, 0, i);
-                            } else {
+                            } else if (!given) {
                                 G::load(b, mb, bar, pb ? 0 : k0, n0, pb ? k : 0, i);
                             }
                         }
@@ -456,7 +472,8 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                 if (ok) ok = mbar_wait(&ctl.empty[i], (uses ^ 1u) & 1u, abort);
                 if (!ok && rank == 0) mbar_wait(&ctl.full[i], (uses ^ 1u) & 1u, abort, true);
             }
-            if (PAIR && !ok)  // copies whose barrier the other block has not armed or does not look at
+            // copies whose barrier the other block has not armed or does not look at, or that came ahead of a step not taken
+            if (!ok && (PAIR || ahead > 0))
                 for (const unsigned long long t0 = global_ns(); global_ns() - t0 < 1000000ull;) {
                 }
         }
@@ -893,6 +910,7 @@ struct SplitArgs {
 };
 
 __global__ void __launch_bounds__(256) split_kernel(const SplitArgs a) {
+    dependents_may_start();
     const int t = blockIdx.y, per = int(a.row[t] / 8), n = a.columns[t];
     const int64_t all = a.rows[t] * per, plane = a.rows[t] * a.row[t];
     const bool vector = a.from_row[t] % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x[t]) & 15u) == 0;
@@ -918,7 +936,9 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitArgs a) {
 // The tiles that were shared out: the sums of their shares, in their order. blockIdx.y: the tile; a thread per four columns.
 template <typename T>
 __global__ void __launch_bounds__(256) add_kernel(const Args g) {
-    Place p = place_of(g, g.whole + int(blockIdx.y));
+    dependents_may_start();
+    wait_for_the_kernel_ahead();
+    const Place p = place_of(g, g.whole + int(blockIdx.y));
     const Problem& q = g.problem[p.problem];
     if (q.out == nullptr) return;
     const int per = g.bn / 4, at = int(blockIdx.x) * 256 + int(threadIdx.x), row = at / per, col = (at - row * per) * 4;
@@ -1033,8 +1053,10 @@ struct Sizes {
     size_t values() const { return size_t(rows) * panels * 64; }
 };
 
+// early: behind another kernel of the same call, which it may overlap. Not for pairs of blocks: placed as SMs become free they
+// took 4 % longer over many tiles (feed_frames_bf16 2018 -> 2095 us), and few are left to gain.
 template <int KIND, int P, int W, bool PAIR>
-fmd_status launch(const Maps& maps, Args& g, cudaStream_t s) {
+fmd_status launch(const Maps& maps, Args& g, bool early, cudaStream_t s) {
     using S = Shape<KIND, P>;
     const fmd_status st = grant_dynamic_smem((const void*)feed_kernel<KIND, P, W, PAIR>, S::kBytes, true);
     if (st != FMD_OK) return st;
@@ -1042,28 +1064,27 @@ fmd_status launch(const Maps& maps, Args& g, cudaStream_t s) {
     g.slots = slots < kMostSlots ? slots : kMostSlots;
     const int64_t turns = g.whole + int64_t(g.tiles - g.whole) * g.splits, places = PAIR ? kNumSMs / 2 : kNumSMs;
     const unsigned blocks = unsigned((turns < places ? turns : places) * (PAIR ? 2 : 1));
-    if constexpr (!PAIR) {
-        feed_kernel<KIND, P, W, PAIR><<<blocks, S::kThreads, S::kBytes, s>>>(maps, g);
-        return check_launch();
-    } else {
-        cudaLaunchAttribute pair{};
-        pair.id = cudaLaunchAttributeClusterDimension;
-        pair.val.clusterDim.x = 2;
-        pair.val.clusterDim.y = pair.val.clusterDim.z = 1;
-        cudaLaunchConfig_t config{};
-        config.gridDim = dim3(blocks);
-        config.blockDim = dim3(unsigned(S::kThreads));
-        config.dynamicSmemBytes = S::kBytes;
-        config.stream = s;
-        config.attrs = &pair;
-        config.numAttrs = 1;
-        const cudaError_t err = cudaLaunchKernelEx(&config, feed_kernel<KIND, P, W, PAIR>, maps, g);
-        return err == cudaSuccess ? check_launch() : record_cuda_error(err);
+    cudaLaunchAttribute attributes[2]{};
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(blocks);
+    config.blockDim = dim3(unsigned(S::kThreads));
+    config.dynamicSmemBytes = S::kBytes;
+    config.stream = s;
+    config.attrs = attributes;
+    if (early && !PAIR) {
+        attributes[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attributes[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
+    if (PAIR) {
+        attributes[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attributes[config.numAttrs++].val.clusterDim = {2, 1, 1};
+    }
+    const cudaError_t err = cudaLaunchKernelEx(&config, feed_kernel<KIND, P, W, PAIR>, maps, g);
+    return err == cudaSuccess ? check_launch() : record_cuda_error(err);
 }
 
 template <int KIND>
-fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args& g, const Plan& p, cudaStream_t s) {
+fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args& g, const Plan& p, bool early, cudaStream_t s) {
     Maps maps{};
     const bool columns_a = KIND == kWeights, columns_b = KIND == kHidden || KIND == kInput || KIND == kWeights;
     // Few rows: the slots hold these alone, so that more of the weights are on their way (up of 8 rows, 4,096 x 11,000:
@@ -1093,15 +1114,13 @@ fmd_status run(int planes, const Matrix* a, const Matrix* b, int operands, Args&
         q.n_tiles = int((q.n + columns - 1) / columns);
     }
     constexpr int kWide = KIND == kUp || KIND == kHidden ? 32 : 64;
-    const fmd_status st = planes == 3       ? launch<KIND, 3, 32, false>(maps, g, s)
-                          : p.tile_m > kM   ? launch<KIND, 1, kWide, true>(maps, g, s)
-                          : g.bn == 256     ? launch<KIND, 1, kWide, false>(maps, g, s)
-                                            : launch<KIND, 1, 32, false>(maps, g, s);
+    const fmd_status st = planes == 3       ? launch<KIND, 3, 32, false>(maps, g, early, s)
+                          : p.tile_m > kM   ? launch<KIND, 1, kWide, true>(maps, g, early, s)
+                          : g.bn == 256     ? launch<KIND, 1, kWide, false>(maps, g, early, s)
+                                            : launch<KIND, 1, 32, false>(maps, g, early, s);
     if (st != FMD_OK || p.splits == 1) return st;
     const dim3 grid(unsigned((p.tile_m * p.bn / 4 + 255) / 256), unsigned(p.tiles - p.whole));
-    if (planes == 1) add_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(g);
-    else add_kernel<float><<<grid, 256, 0, s>>>(g);
-    return check_launch();
+    return launch_early(planes == 1 ? add_kernel<__nv_bfloat16> : add_kernel<float>, grid, 256, 0, s, g);
 }
 
 int64_t steps_of(int64_t k) { return (k + kK - 1) / kK; }
@@ -1311,14 +1330,15 @@ fmd_status fmd_gated_feed_forward(const fmd_feed_forward* problem, void* y, int3
     {
         const Matrix a[2] = {in.x, {}}, b[2] = {in.gate, in.up};
         const int64_t twice = 2 * z.hidden;  // two columns of sums for one of h
-        if ((st = run<kUp>(z.planes, a, b, 2, g, plan(&z.rows, &twice, 1, g.steps, z.planes, 32, false), s)) != FMD_OK) return st;
+        if ((st = run<kUp>(z.planes, a, b, 2, g, plan(&z.rows, &twice, 1, g.steps, z.planes, 32, false),
+                           z.planes == 3, s)) != FMD_OK) return st;
     }
     g.problem[0].n = z.out;
     g.problem[0].out = y;
     g.part = static_cast<float*>(workspace);
     g.steps = int(steps_of(z.hidden));
     const Matrix h{at + k.h, z.rows, z.hidden, 64, z.planes, z.panels};
-    return run<kDown>(z.planes, &h, &in.down, 1, g, down, s);
+    return run<kDown>(z.planes, &h, &in.down, 1, g, down, true, s);
 }
 
 fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kept, size_t kept_bytes, const void* g,
@@ -1371,13 +1391,14 @@ fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kep
     args.da = reinterpret_cast<__nv_bfloat16*>(own + w.da);
     args.db = reinterpret_cast<__nv_bfloat16*>(own + w.db);
     args.part = reinterpret_cast<float*>(own + w.part);
-    if (dx != nullptr || dgate != nullptr || dup != nullptr) {
+    const bool hidden = dx != nullptr || dgate != nullptr || dup != nullptr;
+    if (hidden) {
         args.problems = 1;
         args.problem[0].m = z.rows;
         args.problem[0].n = z.hidden;
         args.steps = int(steps_of(z.out));
         st = run<kHidden>(z.planes, &gm, &in.down, 1, args,
-                          plan(&z.rows, &z.hidden, 1, args.steps, z.planes, z.planes == 1 ? 64 : 128, false), s);
+                          plan(&z.rows, &z.hidden, 1, args.steps, z.planes, z.planes == 1 ? 64 : 128, false), z.planes == 3, s);
         if (st != FMD_OK) return st;
     }
     const Matrix da{own + w.da, z.rows, z.hidden, 64, z.planes, z.panels}, db{own + w.db, z.rows, z.hidden, 64, z.planes, z.panels};
@@ -1388,7 +1409,7 @@ fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kep
         args.turn = int(steps_of(z.hidden));
         args.steps = 2 * args.turn;
         const Matrix a[2] = {da, db}, b[2] = {in.gate, in.up};
-        if ((st = run<kInput>(z.planes, a, b, 2, args, input_plan(z), s)) != FMD_OK) return st;
+        if ((st = run<kInput>(z.planes, a, b, 2, args, input_plan(z), true, s)) != FMD_OK) return st;
     }
     // the products of the weights' gradients that are asked for
     const Plan p = weights_plan(z);
@@ -1407,7 +1428,7 @@ fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kep
     }
     args.steps = int(steps_of(z.rows));
     if (dgate == nullptr && dup == nullptr && ddown == nullptr) return FMD_OK;
-    return run<kWeights>(z.planes, a, b, 3, args, p, s);
+    return run<kWeights>(z.planes, a, b, 3, args, p, z.planes == 3 || hidden, s);
 }
 
 }  // extern "C"

@@ -344,6 +344,10 @@ __device__ __forceinline__ void tmem_free(uint32_t address) {
 
 __device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;"); }
 
+// Waits for the kernel ahead, whose results are to be seen; every block of a kernel launched early comes here, so that its end
+// is also the end of all before it.
+__device__ __forceinline__ void wait_for_the_kernel_ahead() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ------------------------------------------------------------------- host
 
 // Launches `kernel` so that it may start before the one ahead of it in the stream is complete.
