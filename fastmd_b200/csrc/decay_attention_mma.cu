@@ -28,8 +28,7 @@
 // is the product of one factor of the row and one of the column (a table), l^{t-u} = l^{t-a} l^{a-u}, neither above 1.
 //
 // Rows of a tile that lie behind a chunk's end belong to others: their pairs are zeros, b' is zero there, and c is set to
-// zero, whatever their values. A head of up to 64 values is one panel; b' is read as two, the second from what follows in
-// shared memory, for rows of the matrix that nobody takes.
+// zero, whatever their values.
 //
 // Every wait is bounded: on expiry the block raises FMD_FLAG_WAIT_TIMEOUT, waits (bounded) for its copies and products in
 // flight, frees its TMEM and returns.
@@ -47,6 +46,16 @@ struct Shape {
     static constexpr int kPanels = (KS + 3) / 4;
     static constexpr uint32_t kTileBytes = kPanels * kPanelBytes;  // of a plane
     static constexpr uint32_t kSlotBytes = P * kTileBytes;
+    // Rows of the product that the matrix is summed up by: 64 are enough for heads of up to 64 values, and read half as much of
+    // b'. They lie in the first 16 lanes of each of TMEM's quarters.
+    static constexpr int kRows = KS <= 4 ? 64 : 128;
+    static constexpr uint32_t kSumDesc = (uint32_t(kRows) >> 4) << 24 | 1u << 15;
+    // The row of the matrix that a thread holds, or kDim for none.
+    __device__ static int matrix_row() {
+        const int quarter = int(threadIdx.x >> 5) & 3, lane = int(threadIdx.x) & 31;
+        if (KS > 4) return quarter * 32 + lane < kDim ? quarter * 32 + lane : kDim;
+        return lane < 16 && quarter * 16 + lane < kDim ? quarter * 16 + lane : kDim;
+    }
 };
 
 template <int KS, int P>
@@ -61,7 +70,7 @@ struct RowsShape : Shape<KS, P> {
     static constexpr int kPlanes = P == 3 ? 3 : 2;           // of the matrix
     static constexpr uint32_t kPanel = S::kDim * 128;        // of the matrix: kDim rows x 64 columns
     static constexpr uint32_t kPlane = S::kPanels * kPanel;
-    static constexpr uint32_t kMatrix = kPlanes * kPlane > kPanelBytes ? kPlanes * kPlane : kPanelBytes;
+    static constexpr uint32_t kMatrix = kPlanes * kPlane;
     static constexpr size_t kBytes = kSlots * S::kSlotBytes + kMatrix + 1024;
     static constexpr uint32_t kTmem = kBlocks == 2 ? 256 : 512;
     // columns: the pairs at 0, their third plane, n, f, and b'^T c (where two blocks share TMEM: in n's place before it)
@@ -77,7 +86,7 @@ struct StatesShape : Shape<KS, P> {
     static constexpr int kColumns = S::kDim / kGroups;
     static constexpr int kMore = PLANES - P;                 // planes of b' beside the slots
     static constexpr int kSlots = P == 3 || PLANES == 3 ? 4 : 6;
-    static constexpr size_t kBytes = kSlots * S::kSlotBytes + kMore * S::kTileBytes + kPanelBytes + 1024;
+    static constexpr size_t kBytes = kSlots * S::kSlotBytes + kMore * S::kTileBytes + 1024;
     static constexpr uint32_t kTmem = KS <= 2 ? 64 : KS <= 4 ? 128 : 256;  // two sums by turns
 };
 
@@ -421,7 +430,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
         const uint32_t base = uniform(tmem), first_slot = uniform(su32(ring)), planes = uniform(su32(matrix));
         const int count = uniform(walk.chunks), last = uniform(walk.count(walk.chunks - 1));
         const uint32_t pairs_desc = bf16_idesc(kTile, false), out_desc = bf16_idesc(S::kDim, true),
-                       add_desc = out_desc | 1u << 15;
+                       add_desc = (out_desc & 0xFFFFFFu) | S::kSumDesc;
         auto slot = [&](int i) { return first_slot + uint32_t(i % S::kSlots) * S::kSlotBytes; };
         bool ok = true, issued = false;
         auto pairs = [&](int i) {  // over pairs whose product has been issued
@@ -505,10 +514,11 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                        at_far = tmem + lanes + S::kFar + col0, at_sum = tmem + lanes + S::kSum + col0;
         const float l2 = log2_decay(d, head);
         auto power = [&](int n) { return P == 1 ? ex2(float(n) * l2) : exp2f(float(n) * l2); };
-        const bool holds = r < S::kDim;
+        const int matrix_row = S::matrix_row();
+        const bool holds = matrix_row < S::kDim;
         float state[kColumns];
-        load_start(d, s, head, r, col0, state);
-        if (holds) store_matrix<KS, P>(matrix, r, col0, state);
+        load_start(d, s, head, matrix_row, col0, state);
+        if (holds) store_matrix<KS, P>(matrix, matrix_row, col0, state);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         warp_arrive(&ctl.matrix);
         // the weights of 32 pairs from column `first` on
@@ -612,7 +622,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
             float far[kColumns];
             tmem_read(at_far, far);
             if (i + 1 < walk.chunks) {
-                if (holds) store_matrix<KS, P>(matrix, r, col0, state);
+                if (holds) store_matrix<KS, P>(matrix, matrix_row, col0, state);
                 tc_fence_before();
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 warp_arrive(&ctl.matrix);
@@ -722,7 +732,7 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
     } else if (warp > kFeeder) {
         const uint32_t base = uniform(tmem), first_slot = uniform(su32(ring)), planes = uniform(su32(more));
         const int count = uniform(walk.chunks), last = count > 0 ? uniform(walk.count(walk.chunks - 1)) : 0;
-        const uint32_t desc = bf16_idesc(S::kDim, true) | 1u << 15;
+        const uint32_t desc = (bf16_idesc(S::kDim, true) & 0xFFFFFFu) | S::kSumDesc;
         auto slot = [&](int i) { return first_slot + uint32_t(i % S::kSlots) * S::kSlotBytes; };
         bool ok = true, issued = false;
         for (int i = 0; i < count && ok; ++i) {
@@ -767,8 +777,9 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
         const uint32_t at = tmem + (uint32_t((warp & 3) * 32) << 16) + col0;
         const float l2 = log2_decay(d, head);
         float state[kColumns];
+        const int matrix_row = S::matrix_row();
         if (whole) {
-            load_start(d, s, head, r, col0, state);
+            load_start(d, s, head, matrix_row, col0, state);
         } else {
 #pragma unroll
             for (int i = 0; i < kColumns; ++i) state[i] = 0.0f;
@@ -805,7 +816,7 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
             if (i > 0) ok = take(i - 1);
         }
         if (ok && walk.chunks > 0) ok = take(walk.chunks - 1);
-        if (ok && r < d.dim) {
+        if (ok && matrix_row < d.dim) {
             const int64_t size = int64_t(d.dim) * d.dim;
             float* out = whole ? d.after + (int64_t(s.b) * d.heads + head) * size
                                : d.states + (s.index * d.heads + head) * size;
@@ -815,9 +826,9 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
                 if (col0 + i >= d.dim) break;
                 if (turn) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) out[(col0 + i + e) * d.dim + r] = state[i + e];
+                    for (int e = 0; e < 4; ++e) out[(col0 + i + e) * d.dim + matrix_row] = state[i + e];
                 } else {
-                    st4(out + r * d.dim + col0 + i, make_float4(state[i], state[i + 1], state[i + 2], state[i + 3]));
+                    st4(out + matrix_row * d.dim + col0 + i, make_float4(state[i], state[i + 1], state[i + 2], state[i + 3]));
                 }
             }
         }
