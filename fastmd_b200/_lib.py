@@ -296,5 +296,6 @@ def flags_word(device) -> torch.Tensor:
 c_int32_t, c_int64_t = c_int32, c_int64
 c_void_p_t = c_void_p
 
-__all__ = ["FastMDLibraryError", "FmdAttention", "FmdCatPart", "FmdDecay", "FmdFeedForward", "FmdHeadRotarySide", "call", "check", "declare", "flags_word", "lib", "on_device", "ptr",
+__all__ = ["FastMDLibraryError", "FmdAttention", "FmdCatPart", "FmdDecay", "FmdFeedForward", "FmdHeadRotarySide", "call",
+           "check", "declare", "flags_word", "lib", "on_device", "ptr",
            "require_cuda", "stream", "c_double", "c_float", "c_int32", "c_int64", "c_void_p", "ctypes"]

@@ -30,6 +30,12 @@
 // Rows of a tile that lie behind a chunk's end belong to others: their pairs are zeros, b' is zero there, and c is set to
 // zero, whatever their values.
 //
+// What bounds it is the traffic of shared memory, 128 bytes a cycle. A chunk of a head of 128 in bfloat16: the products'
+// operands 2,300 cycles (f, with two planes of S, 1,000), copies in and out 1,000, what the workers read and write 1,300 (b' and
+// S 500 each, the output 250); it takes 5,500 (products alone 2,560). Of a float32 head of 64: 5,000, 1,400 and 1,200; about
+// 9,000. Measured and not kept: eight workers for the pairs and the output beside eight for the matrix (rows of 50,000 x 16
+// heads of 128: 163 -> 200 us), one lane that waits for its warp (163 -> 170).
+//
 // Every wait is bounded: on expiry the block raises FMD_FLAG_WAIT_TIMEOUT, waits (bounded) for its copies and products in
 // flight, frees its TMEM and returns.
 
@@ -159,7 +165,9 @@ __device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
 // Two bfloat16 times a weight in two planes, rounded once (but for 2^-18).
 __device__ __forceinline__ uint32_t times(uint32_t x, uint32_t high, uint32_t low) {
     uint32_t y;
-    asm("{\n\t.reg .b32 t;\n\tmul.rn.bf16x2 t, %1, %3;\n\tfma.rn.bf16x2 %0, %1, %2, t;\n\t}" : "=r"(y) : "r"(x), "r"(high), "r"(low));
+    asm("{\n\t.reg .b32 t;\n\tmul.rn.bf16x2 t, %1, %3;\n\tfma.rn.bf16x2 %0, %1, %2, t;\n\t}"
+        : "=r"(y)
+        : "r"(x), "r"(high), "r"(low));
     return y;
 }
 
@@ -348,6 +356,9 @@ struct Walk {
     __device__ __forceinline__ int first(int i) const { return later ? row0 + max(0, rows - (i + 1) * kTile) : row0 + i * kTile; }
 };
 
+// us: 50,000 rows, 16 heads of 128 in bfloat16, in segments 162 (802 MB, 5.0 TB/s); 16 sequences of 100 to 2,000 rows, 16 heads
+// of 128, the output 66 (256 blocks of up to 16 chunks on 148 SMs) and three gradients 178; in float32 64 sequences of 100 to
+// 500 rows, 8 heads of 64, 88 and 225.
 template <int KS, int P>
 __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::kBlocks)
     rows_kernel(const __grid_constant__ AllMaps all_maps, const __grid_constant__ Decays all) {
@@ -444,8 +455,8 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                 } else {
 #pragma unroll
                     for (int q = 0; q < 6; ++q)
-                        product_rows<KS>(base, a + first_plane(q) * S::kTileBytes, b + second_plane(q) * S::kTileBytes, pairs_desc,
-                                         q > 0);
+                        product_rows<KS>(base, a + first_plane(q) * S::kTileBytes, b + second_plane(q) * S::kTileBytes,
+                                         pairs_desc, q > 0);
                 }
                 tc_commit(&ctl.pairs);
             }
@@ -456,7 +467,8 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
             ok = warp_wait(&ctl.matrix, uint32_t(i) & 1u, abort);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t a = slot(3 * i), b = slot(3 * i + 1), c = slot(3 * i + 2), far = base + S::kFar, near = base + S::kNear, sum = base + S::kSum;
+            const uint32_t a = slot(3 * i), b = slot(3 * i + 1), c = slot(3 * i + 2);
+            const uint32_t far = base + S::kFar, near = base + S::kNear, sum = base + S::kSum;
             if (elect_one()) {
                 if (P == 1) {
                     product_matrix<KS>(far, a, planes + S::kPlane, S::kPanel, out_desc, false);
@@ -477,8 +489,8 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
             if (elect_one()) {
 #pragma unroll
                 for (int q = P == 1 ? 5 : 0; q < 6; ++q)
-                    product_columns(sum, b + first_plane(q) * S::kTileBytes, c + second_plane(q) * S::kTileBytes, 0, steps, add_desc,
-                                    P != 1 && q > 0);
+                    product_columns(sum, b + first_plane(q) * S::kTileBytes, c + second_plane(q) * S::kTileBytes, 0, steps,
+                                    add_desc, P != 1 && q > 0);
                 tc_commit(&ctl.added);
                 tc_commit(&ctl.ring.empty[(3 * i + 1) % S::kSlots]);
             }
@@ -510,8 +522,9 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
         using T = typename std::conditional<P == 1, __nv_bfloat16, float>::type;
         const int group = warp >> 2, r = threadIdx.x & 127, col0 = group * kColumns, pair0 = group * S::kPairs;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t at_pairs = tmem + lanes + pair0, at_third = tmem + lanes + S::kThird + pair0 / 2, at_near = tmem + lanes + S::kNear + col0,
-                       at_far = tmem + lanes + S::kFar + col0, at_sum = tmem + lanes + S::kSum + col0;
+        const uint32_t at_pairs = tmem + lanes + pair0, at_third = tmem + lanes + S::kThird + pair0 / 2;
+        const uint32_t at_near = tmem + lanes + S::kNear + col0, at_far = tmem + lanes + S::kFar + col0,
+                       at_sum = tmem + lanes + S::kSum + col0;
         const float l2 = log2_decay(d, head);
         auto power = [&](int n) { return P == 1 ? ex2(float(n) * l2) : exp2f(float(n) * l2); };
         const int matrix_row = S::matrix_row();
@@ -680,6 +693,8 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
     if (threadIdx.x == 0 && ctl.abort) raise_flag(d.flags, FMD_FLAG_WAIT_TIMEOUT);
 }
 
+// 50,000 rows, 16 heads of 128 in bfloat16, three planes of b': 102 us (410 MB, 4.0 TB/s). A chunk's traffic of shared memory is
+// 3,100 cycles, 70 us in all; the rest is the start and the waits for memory of one block an SM.
 template <int KS, int P, int PLANES>
 __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
     states_kernel(const __grid_constant__ AllMaps all_maps, const __grid_constant__ Decays all) {
@@ -755,8 +770,8 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
                     } else {
 #pragma unroll
                         for (int q = 0; q < 6; ++q)
-                            product_columns(sum, b + first_plane(q) * S::kTileBytes, c + second_plane(q) * S::kTileBytes, from, to,
-                                            desc, half > 0 || q > 0);
+                            product_columns(sum, b + first_plane(q) * S::kTileBytes, c + second_plane(q) * S::kTileBytes,
+                                            from, to, desc, half > 0 || q > 0);
                     }
                     tc_commit(&ctl.freed[half]);
                     if (half > 0) {

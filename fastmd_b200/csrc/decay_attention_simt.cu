@@ -2,7 +2,9 @@
 //
 // A block of 256 threads walks over the chunks of 64 rows of one segment and head; the chunk's rows of a, b and c and the
 // matrix lie in shared memory in FP32, padded to DP columns. A thread owns pieces of 4 x 4 pairs, of 4 rows x DP / 16
-// values of the output, and of DP / 16 x DP / 16 of the matrix, which it also keeps in registers.
+// values of the output, and of DP / 16 x DP / 16 of the matrix, which it also keeps in registers. Bound by the FP32 cores and
+// the shared memory that feeds them, a block an SM: 64 sequences of 100 to 500 rows, 8 heads of 128, forward and backward,
+// 2,700 us (heads of 64 by planes 360); one of 20,000 rows, 16 heads of 128, forward, 1,850.
 
 #include "decay_attention.cuh"
 

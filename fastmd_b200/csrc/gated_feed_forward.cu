@@ -4,16 +4,20 @@
 //   dh = g Wd;  da = dh (b act'(a)), db = dh act(a)
 //   dx = da Wg + db Wu;  dWg = da^T x, dWu = db^T x, dWd = g^T h
 //
-// Five products, each a kernel of the one form below; they differ in how operands lie and in what follows the sums:
-//   up       x [Wg; Wu]^T: a tile's columns are half a's and half b's, so that h follows where the sums are; where a
-//            backward pass follows, b act'(a) and act(a) are kept in FP32
-//   down     h Wd^T
-//   hidden   g Wd, times what was kept: da and db
-//   input    [da, db] [Wg; Wu]: one sum over both
-//   weights  da^T x, db^T x, g^T h: three problems of one launch
+// Five products, each a kernel of the one form below; they differ in how operands lie and in what follows the sums. us and
+// TFLOP/s of 32,000 x 1,024 x 4,096 in bfloat16, forward and backward (1,816 in all, 1,330 TFLOP/s):
+//   up       x [Wg; Wu]^T: a tile's columns are half a's and half b's, so that h follows where the sums are; where a backward
+//            pass follows, b act'(a) and act(a) are kept too                                          416 us, 1,290 TFLOP/s
+//   down     h Wd^T                                                                                   181 us, 1,490
+//   hidden   g Wd, times what was kept: da and db; 1.1 GB of memory, 170 us by itself                 304 us,   880
+//   input    [da, db] [Wg; Wu]: one sum over both                                                     347 us, 1,550
+//   weights  da^T x, db^T x, g^T h: three problems of one launch                                      546 us, 1,480
+// Many rows are bound by the tensor cores (up and hidden by what follows the sums: waits for memory, 16 warps an SM), a few by
+// the weights' bytes: up of 8 x 4,096 x 11,000 takes 36 us, 5.0 TB/s.
 //
 // Roundings: h, da and db are operands of further products and are stored in bfloat16; each costs the result as much as its
-// own last rounding, 1.4 of it in all. What the gradients are multiplied by stays in FP32, which would add as much again.
+// own last rounding, 1.4 of it in all. What the gradients are multiplied by has 11 bits or more, which costs next to nothing;
+// as bfloat16 it would cost as much again.
 //
 // float32: every operand is three planes of bfloat16 (x = x0 + x1 + x2, 24 bits) and a product is the six of its planes
 // that count: x0 w0 apart from the five small ones, because the tensor cores cut off what does not fit as they add. For the
@@ -311,9 +315,7 @@ __device__ __forceinline__ void put_floats(unsigned char* scratch, const float* 
                                            int columns) {
     uint4 w[N / 4];
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i)
-        w[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
-                          __float_as_uint(v[4 * i + 3]));
+    for (int i = 0; i < N / 4; ++i) w[i] = as_piece(v + 4 * i);
     put_rows<N / 4>(scratch, w, to, row * 4, rows, (columns + 3) / 4);
 }
 
@@ -396,7 +398,8 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
         for (; ahead < min(g.slots, p.to - p.from); ++ahead) {
             const int k = p.from + ahead;
             mbar_expect_tx(&ctl.full[ahead], slot_bytes);
-            G::load(ring + uint32_t(ahead) * slot_bytes, &maps.b[0], su32(&ctl.full[ahead]), pb ? 0 : k * kK, p.n * g.bn, pb ? k : 0, 0);
+            G::load(ring + uint32_t(ahead) * slot_bytes, &maps.b[0], su32(&ctl.full[ahead]), pb ? 0 : k * kK, p.n * g.bn,
+                    pb ? k : 0, 0);
         }
     }
     wait_for_the_kernel_ahead();
@@ -453,7 +456,8 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                                 if (pb)
                                     G::load(b, mb, bar, 0, k0, n0 / 64, i);
                                 else
-                                    for (int c = 0; c < columns / 64; ++c) G::load(b + c * kPanel, mb, bar, n0 + 64 * c, k0, 0, i);
+                                    for (int c = 0; c < columns / 64; ++c)
+                                        G::load(b + c * kPanel, mb, bar, n0 + 64 * c, k0, 0, i);
                             } else if (!given) {
                                 G::load(b, mb, bar, pb ? 0 : k0, n0, pb ? k : 0, i);
                             }
@@ -482,7 +486,8 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                        a_bytes = uniform(tile_a);
         const int slots = uniform(g.slots), bn = uniform(g.bn);
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (kColumnsA ? 1u << 15 : 0u) |
-                               (kColumnsB ? 1u << 16 : 0u) | (uint32_t(bn >> 3) << 17) | (uint32_t((PAIR ? 2 * kM : kM) >> 4) << 24);
+                               (kColumnsB ? 1u << 16 : 0u) | (uint32_t(bn >> 3) << 17) |
+                               (uint32_t((PAIR ? 2 * kM : kM) >> 4) << 24);
         constexpr int kStepA = kColumnsA ? 128 : 2, kStepB = kColumnsB ? 128 : 2;
         auto desc = [](uint32_t at, bool columns) {
             return ((at & 0x3FFFFu) >> 4) | (columns ? (kPanel >> 4) << 16 : 1u << 16);
@@ -557,10 +562,9 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             G::arrive(&ctl.taken[unit & 1]);
             ++unit;
         };
-        const int lane32 = lane;
         // the block of 32 rows from row0 on and 16 hidden units from col on, this lane's first piece
         constexpr int kPieces = P == 1 ? 2 : 4;
-        auto block_at = [&](int64_t row0, int64_t col) { return ((col / 16 * g.blocks + row0 / 32) * kPieces) * 32 + lane32; };
+        auto block_at = [&](int64_t row0, int64_t col) { return ((col / 16 * g.blocks + row0 / 32) * kPieces) * 32 + lane; };
         auto panel_at = [&](int64_t row0, int64_t col, int64_t rows) { return (col / 64 * rows + row0) * 64 + col % 64; };
         // kHidden: factors of 32 columns, those of the next ones on their way while the last ones are stored
         uint4 slopes[2 * kPieces], levels[P == 1 ? 2 * kPieces : 1];
@@ -579,7 +583,8 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             fetch(g.level, row0, col, n, levels);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                unit_of[i] = col + 16 * i < n ? __ldg(g.unit + (col / 16 + i) * g.blocks * 32 + row0 + lane32) : make_float2(0.0f, 0.0f);
+                unit_of[i] = col + 16 * i < n ? __ldg(g.unit + (col / 16 + i) * g.blocks * 32 + row0 + lane)
+                                              : make_float2(0.0f, 0.0f);
         };
         // float32: one factor after the other
         auto spread = [&](const Problem& q, int64_t row0, int rows, int64_t col, int64_t after, const float* v) {
@@ -627,7 +632,7 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                         slope[0] = w[0], slope[32] = w[1];
                         pack_halves(v, w, unit.y);
                         level[0] = w[0], level[32] = w[1];
-                        g.unit[col / 16 * g.blocks * 32 + row0 + lane32] = unit;
+                        g.unit[col / 16 * g.blocks * 32 + row0 + lane] = unit;
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -639,7 +644,9 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             } else if constexpr (KIND != kHidden) {
                 const int columns = int(max(int64_t(0), min(int64_t(W), q.n - col)));
                 if (p.part >= 0)
-                    put_result<W>(scratch, v, g.part + (int64_t(p.part) * g.tile_m + rank * kM + (warp & 3) * 32) * g.bn + (col - int64_t(p.n) * g.bn),
+                    put_result<W>(scratch, v,
+                                  g.part + (int64_t(p.part) * g.tile_m + rank * kM + (warp & 3) * 32) * g.bn +
+                                      (col - int64_t(p.n) * g.bn),
                                   g.bn, rows, W, true);
                 else
                     put_result<W>(scratch, v, static_cast<T*>(q.out) + row0 * q.n + col, q.n, rows, columns, q.n % 8 == 0);
@@ -649,7 +656,8 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
             const Place p = place_of(g, t);
             const Problem& q = g.problem[p.problem];
             if (!wanted<KIND>(q)) continue;
-            const int64_t row0 = int64_t(p.m) * g.tile_m + rank * kM + (warp & 3) * 32, n0 = int64_t(p.n) * (KIND == kUp ? g.bn / 2 : g.bn);
+            const int64_t row0 = int64_t(p.m) * g.tile_m + rank * kM + (warp & 3) * 32,
+                          n0 = int64_t(p.n) * (KIND == kUp ? g.bn / 2 : g.bn);
             const int rows = int(max(int64_t(0), min(int64_t(32), q.m - row0)));
             if constexpr (KIND == kHidden) {
                 if constexpr (P == 1) {
@@ -678,7 +686,8 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                         const int64_t col = n0 + u * 32;
                         const int columns = col < g.panels * 64 ? 32 : 0;
                         uint4 da[4], db[4];
-                        const uint32_t *s = reinterpret_cast<const uint32_t*>(slopes), *l = reinterpret_cast<const uint32_t*>(levels);
+                        const uint32_t *s = reinterpret_cast<const uint32_t*>(slopes),
+                                       *l = reinterpret_cast<const uint32_t*>(levels);
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             float v[16], x[16], y[16];
@@ -720,7 +729,8 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
                         if (KIND != kHidden && group + u * kGroups >= units) break;
 #pragma unroll
                         for (int j = 0; j < W; j += 16) {
-                            const int col = (group + u * kGroups) * kStep + (KIND == kUp && j >= W / 2 ? g.bn / 2 + j - W / 2 : j);
+                            const int col = (group + u * kGroups) * kStep +
+                                            (KIND == kUp && j >= W / 2 ? g.bn / 2 + j - W / 2 : j);
                             float big[16], small[16];
                             tmem_load16(at + col, big);
                             tmem_load16(at + 128 + col, small);
@@ -754,8 +764,10 @@ __global__ void __launch_bounds__(Shape<KIND, P>::kThreads, 1) feed_kernel(const
 
 // A few rows in float32 without planes, whose making moves four times the weights' bytes: on the FP32 cores. A block takes R
 // rows of x and J rows of weights (GATED: J / 2 units, their gate and up rows) through the inner index in chunks of 256, which
-// lie in shared memory, one in use and one on its way; each of its eight warps takes 32 of a chunk, all R x J sums, a lane 4 x J R / 128 of them: 4 + C
-// vectors of shared memory for 16 C products. The warps' sums are added up at the end.
+// lie in shared memory, one in use and one on its way; each of its eight warps takes 32 of a chunk, all R x J sums, a lane
+// 4 x C of them (C = J R / 128): 4 + C vectors of shared memory for 16 C products. The warps' sums are added up at the end.
+// 33 rows of 512 x 1,365: 13.7 and 13.5 us, of which reading the weights, 8.4 MB, would be one each: start, end, and chunks
+// that wait for memory by turns.
 constexpr int kFewThreads = 256, kFewChunk = 256, kFewLd = kFewChunk + 4;
 
 struct Few {
@@ -1142,7 +1154,7 @@ struct Layout {
     }
 };
 
-// What the forward pass keeps for the backward pass: h, FP32 factors, and in float32 the planes of what it was given.
+// What the forward pass keeps for the backward pass: h, the factors, and in float32 the planes of what it was given.
 struct Kept {
     size_t h, slope, level, unit, x, gate, up, down, bytes;
 };
@@ -1206,7 +1218,10 @@ fmd_status check(const fmd_feed_forward& f, Sizes& z) {
 }
 
 // A few rows: h alone, by rows.
-bool few_rows(const Sizes& z, bool keep) { return z.planes == 3 && !keep && z.rows > 0 && z.rows <= few_limit(z.width, z.hidden); }
+bool few_rows(const Sizes& z, bool keep) {
+    return z.planes == 3 && !keep && z.rows > 0 && z.rows <= few_limit(z.width, z.hidden);
+}
+
 size_t few_bytes(const Sizes& z) { return (size_t(z.rows) * round_up(z.hidden, 4) * sizeof(float) + 255) / 256 * 256; }
 
 fmd_status run_few(const fmd_feed_forward& f, float* h, float* y, cudaStream_t s) {
@@ -1401,7 +1416,8 @@ fmd_status fmd_gated_feed_forward_bwd(const fmd_feed_forward* problem, void* kep
                           plan(&z.rows, &z.hidden, 1, args.steps, z.planes, z.planes == 1 ? 64 : 128, false), z.planes == 3, s);
         if (st != FMD_OK) return st;
     }
-    const Matrix da{own + w.da, z.rows, z.hidden, 64, z.planes, z.panels}, db{own + w.db, z.rows, z.hidden, 64, z.planes, z.panels};
+    const Matrix da{own + w.da, z.rows, z.hidden, 64, z.planes, z.panels};
+    const Matrix db{own + w.db, z.rows, z.hidden, 64, z.planes, z.panels};
     if (dx != nullptr) {
         args.problems = 1;
         args.problem[0].n = z.width;

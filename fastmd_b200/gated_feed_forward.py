@@ -89,8 +89,10 @@ def gated_feed_forward(x: Tensor, gate: Tensor, up: Tensor, down: Tensor, *, act
     Differentiable in all four (first derivatives in reverse mode: others raise), with the same bits on every run. Sums are
     held in 32 bits; in bfloat16 the gated product and the gradients of the two projections are rounded to bfloat16 as
     operands of the next product, each of which costs a result about as much as its own rounding. In float32 each product
-    is six of bfloat16 planes; an infinity gives NaN where the formula may have an infinity. For the backward pass a call
-    keeps 6.5 bytes a row and hidden unit (float32: 14, and one and a half times the bytes of x and the weights)."""
+    is six of bfloat16 planes (a few rows without gradients: FP32). Rows do not see each other's values, finite or not; within
+    a row an infinity may give NaN where the formula has an infinity. For the backward pass a call keeps 6.5 bytes a row and
+    hidden unit (float32: 14, and one and a half times the bytes of x and the weights). As for any autograd function, a
+    backward pass is captured in a CUDA graph only while no eager graph of the same leaves is alive."""
     _lib.require_cuda(x, gate, up, down)
     lead, weights, last = x.shape, gate.shape, down.shape
     if x.dim() < 1 or gate.dim() != 2 or up.shape != weights or down.dim() != 2 or lead[-1] != weights[1] \
