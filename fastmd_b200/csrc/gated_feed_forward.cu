@@ -247,6 +247,15 @@ __device__ __forceinline__ float rcp(float x) {
     return y;
 }
 
+// The normal distribution's share below a, with density = e^{-a a / 2}, to 10^-7: Abramowitz and Stegun, Handbook of
+// Mathematical Functions, 7.1.26. Half of up's instructions were the library's erfc (10,007 x 264 x 1,000: 47 -> 34 us).
+__device__ __forceinline__ float normal_share(float a, float density) {
+    const float t = rcp(fmaf(fabsf(a), 0.3275911f * 0.7071067811865476f, 1.0f));
+    const float sum = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
+    const float tail = 0.5f * density * t * sum;
+    return a < 0.0f ? tail : 1.0f - tail;
+}
+
 // act(a) and act'(a). EXACT: to FP32's last bits; else to 2^-20 or so, for results in 16 bits.
 template <bool EXACT>
 __device__ __forceinline__ void activate(int act, float a, float& value, float& slope) {
@@ -257,9 +266,10 @@ __device__ __forceinline__ void activate(int act, float a, float& value, float& 
         value = low * turn;
         slope = fmaf(held * turn, 1.0f - turn, turn);
     } else {
-        const float share = 0.5f * erfcf(-0.7071067811865476f * a);
+        const float density = EXACT ? expf(-0.5f * a * a) : ex2(-0.7213475204444817f * a * a);
+        const float share = EXACT ? 0.5f * erfcf(-0.7071067811865476f * a) : normal_share(a, density);
         value = low * share;
-        slope = fmaf(held, 0.3989422804014327f * (EXACT ? expf(-0.5f * a * a) : ex2(-0.7213475204444817f * a * a)), share);
+        slope = fmaf(held, 0.3989422804014327f * density, share);
     }
 }
 
