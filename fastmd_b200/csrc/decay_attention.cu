@@ -164,20 +164,13 @@ fmd_status check_rows(const fmd_decay& p, Decay& d) {
     return FMD_OK;
 }
 
-// How the recurrence runs, from the sizes alone.
-enum Path { kMma, kPlanes, kSimt };
-
-// float32 heads of up to 64 values go through planes on the tensor cores, wider ones stay on the FP32 cores: the planes of a
-// chunk of 128 rows do not fit beside those of the matrix.
-Path path_of(const Decay& d, int type) { return type == FMD_BF16 ? kMma : d.dim <= 64 ? kPlanes : kSimt; }
-
 // Rows of a segment: whole sequences where these are blocks enough for the GPU or short; else so many that the segments fill
 // it once (the sequences' last ones are half a segment long on average). Segments cost a second look at two of the three
 // inputs and two more launches.
-int64_t segment_length(const Decay& d, Path path) {
-    const int64_t places = (path == kMma && d.dim <= 64 ? 2 : 1) * kNumSMs;
-    if (d.batch == 0 || d.rows / d.batch <= 512 || 10 * int64_t(d.batch) * d.heads >= 6 * places) return kWhole;
-    const int64_t want = 2 * places / d.heads - d.batch;  // twice the segments, less the sequences' last ones
+int64_t segment_length(const Decay& d, bool planes) {
+    const int64_t heads = d.heads * (planes && d.dim > 64 ? 2 : 1);  // blocks for a sequence
+    if (d.batch == 0 || d.rows / d.batch <= 512 || 10 * d.batch * heads >= 6 * kNumSMs) return kWhole;
+    const int64_t want = 2 * kNumSMs / heads - d.batch;  // twice the segments, less the sequences' last ones
     const int64_t length = (2 * d.rows / (want > 1 ? want : 1) + 127) / 128 * 128;
     return length < 256 ? 256 : length;
 }
@@ -186,12 +179,11 @@ size_t matrices(const Decay& d, int64_t n) { return size_t(n) * d.heads * d.dim 
 
 size_t plane_bytes(const Decay& d) { return (size_t(d.rows) * d.heads * d.dim * 6 + 255) / 256 * 256; }
 
-// Planes of `arrays` inputs, and what the segments of `passes` passes add.
+// Planes of `arrays` inputs (float32), and what the segments of `passes` passes add.
 size_t workspace_of(Decay d, int type, int arrays, int passes) {
-    const Path path = path_of(d, type);
-    d.length = segment_length(d, path);
-    return (path == kPlanes ? arrays * plane_bytes(d) : 0) +
-           (d.length < kWhole ? passes * matrices(d, decay_segments(d)) : 0);
+    const bool planes = type == FMD_F32;
+    d.length = segment_length(d, planes);
+    return (planes ? arrays * plane_bytes(d) : 0) + (d.length < kWhole ? passes * matrices(d, decay_segments(d)) : 0);
 }
 
 // The inputs as the kernels read them: in float32 their planes, which `split` makes.
@@ -201,9 +193,9 @@ struct Input {
 };
 
 // The planes of `inputs`, the first `made` of which are there already, at `made_at`; their room stays in the workspace.
-fmd_status make_planes(const Decay& d, Path path, Input* inputs, int count, int made, const void* made_at, char*& workspace,
+fmd_status make_planes(const Decay& d, Input* inputs, int count, int made, const void* made_at, char*& workspace,
                        cudaStream_t s) {
-    if (path != kPlanes || d.rows == 0) return FMD_OK;
+    if (d.rows == 0) return FMD_OK;
     SplitArgs a{};
     a.rows = d.rows;
     a.heads = d.heads;
@@ -230,29 +222,27 @@ void read_from(Decay& d, const Input& a, const Input& b, const Input& c) {
     d.c = c.data, d.c_row = c.row, d.c_head = c.head;
 }
 
-fmd_status run_states(const Decays& d, Path path, bool early, cudaStream_t s) {
-    return path == kMma      ? decay_states_mma(d, early, s)
-           : path == kPlanes ? decay_states_planes(d, early, s)
-                             : decay_states_simt(d, s);
+fmd_status run_states(const Decays& d, bool planes, bool early, cudaStream_t s) {
+    return planes ? decay_states_planes(d, early, s) : decay_states_mma(d, early, s);
 }
 
 // Passes of the recurrence over the same rows, side by side: with segments what these add comes first.
-fmd_status mix(Decays all, Path path, char* workspace, cudaStream_t s) {
+fmd_status mix(Decays all, bool planes, char* workspace, cudaStream_t s) {
     const Decay& d = all.d[0];
     if (all.count == 0 || d.batch == 0) return FMD_OK;
-    int64_t length = segment_length(d, path);
+    int64_t length = segment_length(d, planes);
     if (d.rows == 0) length = 1;  // nothing but the matrices to hand on
     for (int i = 0; i < all.count; ++i) all.d[i].length = length;
     const int64_t segments = decay_segments(d);
-    if (segments * d.heads * all.count > INT32_MAX || int64_t(d.batch) * d.heads > INT32_MAX) return FMD_ERR_UNSUPPORTED;
+    if (4 * segments * d.heads * all.count > INT32_MAX || int64_t(d.batch) * d.heads > INT32_MAX) return FMD_ERR_UNSUPPORTED;
     fmd_status st = FMD_OK;
-    bool early = path == kPlanes && d.rows > 0;  // behind the kernel that makes the planes
+    bool early = planes && d.rows > 0;  // behind the kernel that makes the planes
     if (length < kWhole) {
         for (int i = 0; i < all.count; ++i) {
             all.d[i].states = reinterpret_cast<float*>(workspace);
             workspace += d.rows > 0 ? matrices(d, segments) : 0;
         }
-        if (d.rows > 0 && (st = run_states(all, path, early, s)) != FMD_OK) return st;
+        if (d.rows > 0 && (st = run_states(all, planes, early, s)) != FMD_OK) return st;
         const dim3 grid(unsigned(d.batch) * d.heads, unsigned((d.dim * d.dim + 4 * kThreads - 1) / (4 * kThreads)),
                         unsigned(all.count));
         if ((st = launch_early(carry_kernel, grid, kThreads, 0, s, all)) != FMD_OK) return st;
@@ -261,16 +251,14 @@ fmd_status mix(Decays all, Path path, char* workspace, cudaStream_t s) {
         Decays ends{};  // those whose last matrix is asked for
         for (int i = 0; i < all.count; ++i)
             if (all.d[i].after != nullptr) ends.d[ends.count++] = all.d[i];
-        if (ends.count > 0 && (st = run_states(ends, path, early, s)) != FMD_OK) return st;
+        if (ends.count > 0 && (st = run_states(ends, planes, early, s)) != FMD_OK) return st;
         early = early || ends.count > 0;
     }
     Decays rows{};
     for (int i = 0; i < all.count; ++i)
         if (all.d[i].out != nullptr) rows.d[rows.count++] = all.d[i];
     if (d.rows == 0 || rows.count == 0) return FMD_OK;
-    return path == kMma      ? decay_rows_mma(rows, early, s)
-           : path == kPlanes ? decay_rows_planes(rows, early, s)
-                             : decay_rows_simt(rows, s);
+    return planes ? decay_rows_planes(rows, early, s) : decay_rows_mma(rows, early, s);
 }
 
 }  // namespace
@@ -301,10 +289,10 @@ fmd_status fmd_decay_attention(const fmd_decay* problem, const float* state, voi
     if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return FMD_ERR_WORKSPACE;
     if (!aligned16(out) || !aligned16(state) || !aligned16(after) || !aligned16(workspace)) return FMD_ERR_UNSUPPORTED;
     const cudaStream_t s = as_stream(stream);
-    const Path path = path_of(d, p.type);
+    const bool planes = p.type == FMD_F32;
     char* at = static_cast<char*>(workspace);
     Input in[3] = {{p.q, p.q_row, p.q_head}, {p.k, p.k_row, p.k_head}, {p.v, p.v_row, p.v_head}};
-    if ((st = make_planes(d, path, in, 3, 0, nullptr, at, s)) != FMD_OK) return st;
+    if (planes && (st = make_planes(d, in, 3, 0, nullptr, at, s)) != FMD_OK) return st;
     read_from(d, in[0], in[1], in[2]);
     d.out = out;
     d.start = state;
@@ -312,7 +300,7 @@ fmd_status fmd_decay_attention(const fmd_decay* problem, const float* state, voi
     d.flags = flags;
     d.near = d.far = p.scale;
     d.add = 1.0f;
-    return mix(Decays{{d}, 1}, path, at, s);
+    return mix(Decays{{d}, 1}, planes, at, s);
 }
 
 fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state, const void* forward, const void* g,
@@ -331,10 +319,10 @@ fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state,
         (p.rows > 0 && !vector_rows(g, g_row, g_head, p.type == FMD_BF16 ? 2 : 4)))
         return FMD_ERR_UNSUPPORTED;
     const cudaStream_t s = as_stream(stream);
-    const Path path = path_of(d, p.type);
+    const bool planes = p.type == FMD_F32;
     char* at = static_cast<char*>(workspace);
     Input in[4] = {{p.q, p.q_row, p.q_head}, {p.k, p.k_row, p.k_head}, {p.v, p.v_row, p.v_head}, {g, g_row, g_head}};
-    if ((st = make_planes(d, path, in, 4, forward != nullptr ? 3 : 0, forward, at, s)) != FMD_OK) return st;
+    if (planes && (st = make_planes(d, in, 4, forward != nullptr ? 3 : 0, forward, at, s)) != FMD_OK) return st;
     const Input &q = in[0], &k = in[1], &v = in[2], &go = in[3];
     d.flags = flags;
     d.near = p.scale;
@@ -369,7 +357,7 @@ fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state,
         m.far = p.scale;
         all.d[all.count++] = m;
     }
-    return mix(all, path, at, s);
+    return mix(all, planes, at, s);
 }
 
 fmd_status fmd_decay_attention_step(const fmd_decay* problem, float* state, void* out, void* stream) {

@@ -92,12 +92,6 @@ __device__ __forceinline__ const float* start_of(const Decay& d, const Stretch& 
     return d.start != nullptr ? d.start + (int64_t(s.b) * d.heads + head) * size : nullptr;
 }
 
-// Its value (row, col): whole sequences may have it transposed.
-__device__ __forceinline__ float start_at(const Decay& d, const float* start, int row, int col) {
-    if (start == nullptr || row >= d.dim || col >= d.dim) return 0.0f;
-    return start[d.length >= kWhole && d.transposed ? col * d.dim + row : row * d.dim + col];
-}
-
 // Looks at sequence b's offsets.
 __device__ __forceinline__ void check_offsets(const Decay& d, int64_t b) {
     const int64_t r0 = d.offsets[b], r1 = d.offsets[b + 1];
@@ -115,11 +109,8 @@ __device__ __forceinline__ float log2_decay(const Decay& d, int head) {
 // another kernel of the same call, which they may overlap until they need its results. bfloat16:
 fmd_status decay_states_mma(const Decays& d, bool early, cudaStream_t s);
 fmd_status decay_rows_mma(const Decays& d, bool early, cudaStream_t s);
-// float32, heads of up to 64 values: a, b and c are three planes of bfloat16, [3][rows][heads][dim]
+// float32: a, b and c are three planes of bfloat16, [3][rows][heads][dim]
 fmd_status decay_states_planes(const Decays& d, bool early, cudaStream_t s);
 fmd_status decay_rows_planes(const Decays& d, bool early, cudaStream_t s);
-// float32, wider heads
-fmd_status decay_states_simt(const Decays& d, cudaStream_t s);
-fmd_status decay_rows_simt(const Decays& d, cudaStream_t s);
 
 }  // namespace fmd

@@ -1,4 +1,4 @@
-// Decay attention on the tensor cores: bfloat16, and float32 for heads of up to 64 values as planes of bfloat16.
+// Decay attention on the tensor cores: bfloat16, and float32 as planes of bfloat16.
 //
 // A block walks over the chunks of 128 rows of one segment and head. Of a chunk (rows t, u of it, l the decay):
 //   pairs   s = a b^T;  p_tu = near l^{t-u} s_tu for u <= t, as bfloat16 back into TMEM;  near part  n = p c
@@ -9,14 +9,16 @@
 // an output about as much as its own rounding: 1.4 of it in all. One plane of S would cost as much again.
 //
 // float32: a, b, c, p, b' and S are three planes each (24 bits) and a product is the six of its planes that count, the
-// small ones first.
+// small ones first. There is room for heads of up to 64 values. Wider ones go in parts of 64, since the output is linear in the
+// pairs: its values fall into two (blocks of their own), a . b into two sums, of which a second launch adds the second to the
+// output that the first one left.
 //
 // states_kernel does the last line alone, for what a segment adds to the matrix or for the matrix behind a sequence; in
 // bfloat16 with three planes of b' where the matrix itself is a result, so that it is exact to FP32. There is room for one
 // chunk's planes, so a chunk goes by halves: one half's rows are weighed while the other's products run, and its sums are
 // taken a chunk later.
 //
-// Warps, after the workers (8 or 16 of them: thread = row of the chunk and a part of the pairs or columns; for the matrix
+// Warps, after the workers (16 of them: thread = row of the chunk and a part of the pairs or columns; for the matrix
 // its row, and a part of its columns):
 //   TMA: a, b, c of one chunk after the other through a ring of slots; the output out of c's slot before that is filled again
 //   (the last chunk's rows by the workers themselves)
@@ -67,9 +69,9 @@ struct Shape {
 template <int KS, int P>
 struct RowsShape : Shape<KS, P> {
     using S = Shape<KS, P>;
-    // Two blocks an SM where they fit, of eight workers each; else sixteen in one block, which hide each other's waits.
-    static constexpr int kBlocks = P == 1 && KS <= 4 ? 2 : 1;
-    static constexpr int kGroups = kBlocks == 2 ? 2 : 4, kWorkers = 128 * kGroups, kThreads = kWorkers + 64;
+    // Sixteen workers hide each other's waits: two blocks an SM of eight each, which heads of up to 64 values in bfloat16 leave
+    // room for, took up to 9 % longer (4 sequences of 3,000 to 8,000 rows, 8 heads of 64, forward and backward: 233 us, 214).
+    static constexpr int kGroups = 4, kWorkers = 128 * kGroups, kThreads = kWorkers + 64;
     static constexpr int kColumns = S::kDim / kGroups, kPairs = kTile / kGroups;  // of a thread
     static constexpr int kSize = P == 3 ? 4 : 2, kOutPanels = (S::kDim * kSize + 127) / 128;  // of the output
     static constexpr int kSlots = P == 3 ? 4 : 5;
@@ -78,10 +80,9 @@ struct RowsShape : Shape<KS, P> {
     static constexpr uint32_t kPlane = S::kPanels * kPanel;
     static constexpr uint32_t kMatrix = kPlanes * kPlane;
     static constexpr size_t kBytes = kSlots * S::kSlotBytes + kMatrix + 1024;
-    static constexpr uint32_t kTmem = kBlocks == 2 ? 256 : 512;
-    // columns: the pairs at 0, their third plane, n, f, and b'^T c (where two blocks share TMEM: in n's place before it)
-    static constexpr uint32_t kThird = 128, kNear = kThird + (P == 3 ? 64 : 0), kFar = kNear + S::kDim;
-    static constexpr uint32_t kSum = kBlocks == 2 ? kNear : kFar + S::kDim;
+    // columns: the pairs at 0, their third plane, n, f, and b'^T c
+    static constexpr uint32_t kTmem = 512;
+    static constexpr uint32_t kThird = 128, kNear = kThird + (P == 3 ? 64 : 0), kFar = kNear + S::kDim, kSum = kFar + S::kDim;
 };
 
 // PLANES: of b'.
@@ -298,14 +299,42 @@ __device__ __forceinline__ void feed_tiles(Control& ctl, volatile int32_t* abort
     }
 }
 
-// One tile: P planes of `panels` panels each, rows from `row` on of `all`.
+// One tile: P planes of `panels` panels each, rows from `row` on of `all`, the head's values from `first` on.
 template <int KS, int P>
 __device__ __forceinline__ void load_tile(uint32_t to, const CUtensorMap* map, uint64_t* bar, int head, int64_t row,
-                                          int64_t all) {
+                                          int64_t all, int first) {
     using S = Shape<KS, P>;
     for (int q = 0; q < P; ++q)
         for (int p = 0; p < S::kPanels; ++p)
-            tma_load_4d(to + q * S::kTileBytes + p * kPanelBytes, map, bar, p * 64, 0, head, int(q * all + row));
+            tma_load_4d(to + q * S::kTileBytes + p * kPanelBytes, map, bar, first + p * 64, 0, head, int(q * all + row));
+}
+
+// The values of a head in parts of 64 (float32 heads of more than that): those of c and the output, and those of a and b, which
+// each add to the output.
+__host__ __device__ constexpr int parts_of(int planes, int dim) { return planes == 3 && dim > 64 ? 2 : 1; }
+
+// Adds a tile of shared memory to memory.
+__device__ __forceinline__ void tma_add_4d(const CUtensorMap* map, uint32_t src, int x, int y, int z, int w) {
+    asm volatile("cp.reduce.async.bulk.tensor.4d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(src), "r"(x), "r"(y), "r"(z), "r"(w)
+                 : "memory");
+}
+
+// What store_pieces overwrites next, added to the pieces (FP32).
+template <int W>
+__device__ __forceinline__ void add_pieces(uint4 (&w)[W], const void* from, int64_t stride, int rows, int pieces) {
+    const int lane = threadIdx.x & 31, left = lane % W < pieces ? rows - lane / W : 0;
+    const char* p = static_cast<const char*>(from) + (lane / W) * stride + (lane % W) * 16;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        if (i * (32 / W) < left) {
+            const float4 x = *reinterpret_cast<const float4*>(p);
+            w[i] = make_uint4(__float_as_uint(__uint_as_float(w[i].x) + x.x), __float_as_uint(__uint_as_float(w[i].y) + x.y),
+                              __float_as_uint(__uint_as_float(w[i].z) + x.z), __float_as_uint(__uint_as_float(w[i].w) + x.w));
+        }
+        p += (32 / W) * stride;
+    }
 }
 
 __device__ __forceinline__ bool worker_wait(uint64_t* bar, uint32_t parity, volatile int32_t* abort) {
@@ -326,7 +355,7 @@ __device__ __forceinline__ Stretch block_stretch(const Decay& d, int64_t index) 
     return place;
 }
 
-// What a stretch starts from: row r of the matrix, columns from col0 on.
+// What a stretch starts from: row r of the matrix (dim or more: none), columns from col0 on.
 template <int N>
 __device__ __forceinline__ void load_start(const Decay& d, const Stretch& s, int head, int r, int col0, float (&state)[N]) {
     const float* from = start_of(d, s, head);
@@ -358,10 +387,11 @@ struct Walk {
 
 // us: 50,000 rows, 16 heads of 128 in bfloat16, in segments 162 (802 MB, 5.0 TB/s); 16 sequences of 100 to 2,000 rows, 16 heads
 // of 128, the output 66 (256 blocks of up to 16 chunks on 148 SMs) and three gradients 178; in float32 64 sequences of 100 to
-// 500 rows, 8 heads of 64, 88 and 225.
+// 500 rows, 8 heads of 64, 88 and 225, heads of 128 four times that (1,275 with the planes; 2,700 on the FP32 cores).
+// part: of a's and b's values.
 template <int KS, int P>
-__global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::kBlocks)
-    rows_kernel(const __grid_constant__ AllMaps all_maps, const __grid_constant__ Decays all) {
+__global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, 1)
+    rows_kernel(const __grid_constant__ AllMaps all_maps, const __grid_constant__ Decays all, const int part) {
     using S = RowsShape<KS, P>;
     constexpr int kColumns = S::kColumns, kFeeder = S::kWorkers / 32;
     extern __shared__ unsigned char raw[];
@@ -375,8 +405,9 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
     const unsigned which = blockIdx.x % unsigned(all.count), place = blockIdx.x / unsigned(all.count);
     const Decay& d = all.d[which];
     const Maps& maps = all_maps.m[which];
-    const int head = int(place % unsigned(d.heads));
-    const int64_t index = place / unsigned(d.heads);
+    const unsigned parts = parts_of(P, d.dim);
+    const int head = int(place / parts % unsigned(d.heads)), first_in = 64 * part, first_out = 64 * int(place % parts);
+    const int64_t index = place / parts / unsigned(d.heads);
 
     if (threadIdx.x < 32) {
         const float l2 = log2_decay(d, head);
@@ -414,9 +445,13 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                 }
                 if (!mbar_wait(&ctl.stored[chunk & 1], uint32_t(chunk >> 1) & 1u, abort)) return false;
                 if (walk.count(chunk) == kTile) {
-                    for (int p = 0; p < S::kOutPanels; ++p)
-                        tma_store_4d(&maps.out, su32(ring + slot * S::kSlotBytes + p * kPanelBytes), p * (128 / S::kSize), 0,
-                                     head, walk.first(chunk));
+                    for (int p = 0; p < S::kOutPanels; ++p) {
+                        const uint32_t from = su32(ring + slot * S::kSlotBytes + p * kPanelBytes);
+                        const int x = first_out + p * (128 / S::kSize);
+                        if (x >= d.dim) break;
+                        if (P == 3 && part > 0) tma_add_4d(&maps.out, from, x, 0, head, walk.first(chunk));
+                        else tma_store_4d(&maps.out, from, x, 0, head, walk.first(chunk));
+                    }
                     asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
                 }
                 return true;
@@ -428,7 +463,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                 if (i >= S::kSlots && !(ok = released(i - S::kSlots))) break;
                 mbar_expect_tx(&ctl.ring.full[slot], S::kSlotBytes);
                 load_tile<KS, P>(su32(ring + slot * S::kSlotBytes), what == 0 ? &maps.a : what == 1 ? &maps.b : &maps.c,
-                                 &ctl.ring.full[slot], head, walk.first(chunk), d.rows);
+                                 &ctl.ring.full[slot], head, walk.first(chunk), d.rows, what == 2 ? first_out : first_in);
                 armed = i + 1;
             }
             for (int i = max(0, armed - S::kSlots); i < armed; ++i) {
@@ -530,7 +565,7 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
         const int matrix_row = S::matrix_row();
         const bool holds = matrix_row < S::kDim;
         float state[kColumns];
-        load_start(d, s, head, matrix_row, col0, state);
+        load_start(d, s, head, holds ? first_in + matrix_row : d.dim, first_out + col0, state);
         if (holds) store_matrix<KS, P>(matrix, matrix_row, col0, state);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         warp_arrive(&ctl.matrix);
@@ -618,17 +653,11 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
                 }
             }
             tmem_wait_st();
-            if (S::kSum != S::kNear) {
-                tc_fence_before();
-                warp_arrive(&ctl.weights);
-            }
+            tc_fence_before();
+            warp_arrive(&ctl.weights);
             if (!worker_wait(&ctl.added, parity, abort)) break;
             tc_fence_after();
             add_columns(at_sum, keep, state);
-            if (S::kSum == S::kNear) {
-                tc_fence_before();
-                warp_arrive(&ctl.weights);
-            }
 
             if (!worker_wait(&ctl.far, parity, abort)) break;
             tc_fence_after();
@@ -680,8 +709,10 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, RowsShape<KS, P>::
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(&ctl.stored[i & 1]);
             if (count < kTile) {
-                const int first_row = (warp & 3) * 32, left = min(kColumns, d.dim - col0) * S::kSize / 16;
-                T* out = static_cast<T*>(d.out) + (int64_t(walk.first(i) + first_row) * d.heads + head) * d.dim + col0;
+                const int first_row = (warp & 3) * 32, left = min(kColumns, d.dim - first_out - col0) * S::kSize / 16;
+                T* out = static_cast<T*>(d.out) + (int64_t(walk.first(i) + first_row) * d.heads + head) * d.dim + first_out + col0;
+                if (P == 3 && part > 0)
+                    add_pieces<kWide>(row, out, int64_t(d.heads) * d.dim * S::kSize, count - first_row, left);
                 store_pieces<kWide>(row, out, int64_t(d.heads) * d.dim * S::kSize, count - first_row, left);
             }
         }
@@ -709,10 +740,12 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
     const unsigned which = blockIdx.x % unsigned(all.count), place = blockIdx.x / unsigned(all.count);
     const Decay& d = all.d[which];
     const Maps& maps = all_maps.m[which];
-    const int head = int(place % unsigned(d.heads));
+    const unsigned parts = parts_of(P, d.dim);
+    const int head = int(place / (parts * parts) % unsigned(d.heads)), first_c = 64 * int(place % parts),
+              first_b = 64 * int(place / parts % parts);
     const bool whole = d.length >= kWhole;
 
-    const Stretch s = block_stretch(d, place / unsigned(d.heads));
+    const Stretch s = block_stretch(d, place / (parts * parts) / unsigned(d.heads));
     if (s.rows == 0 && !whole) {
         wait_for_the_kernel_ahead();
         return;
@@ -742,7 +775,7 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
         if (lane == 0)
             feed_tiles(ctl, abort, 2 * walk.chunks, S::kSlotBytes, [&](int i, int slot, uint64_t* bar) {
                 load_tile<KS, P>(su32(ring + slot * S::kSlotBytes), i & 1 ? &maps.c : &maps.b, bar, head, walk.first(i >> 1),
-                                 d.rows);
+                                 d.rows, i & 1 ? first_c : first_b);
             });
     } else if (warp > kFeeder) {
         const uint32_t base = uniform(tmem), first_slot = uniform(su32(ring)), planes = uniform(su32(more));
@@ -792,9 +825,9 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
         const uint32_t at = tmem + (uint32_t((warp & 3) * 32) << 16) + col0;
         const float l2 = log2_decay(d, head);
         float state[kColumns];
-        const int matrix_row = S::matrix_row();
+        const int matrix_row = S::matrix_row() < S::kDim ? first_b + S::matrix_row() : d.dim;  // of the whole head's
         if (whole) {
-            load_start(d, s, head, matrix_row, col0, state);
+            load_start(d, s, head, matrix_row, first_c + col0, state);
         } else {
 #pragma unroll
             for (int i = 0; i < kColumns; ++i) state[i] = 0.0f;
@@ -838,12 +871,13 @@ __global__ void __launch_bounds__(StatesShape<KS, P, PLANES>::kThreads, 1)
             const bool turn = whole && d.transposed;
 #pragma unroll
             for (int i = 0; i < kColumns; i += 4) {
-                if (col0 + i >= d.dim) break;
+                const int col = first_c + col0 + i;
+                if (col >= d.dim) break;
                 if (turn) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) out[(col0 + i + e) * d.dim + matrix_row] = state[i + e];
+                    for (int e = 0; e < 4; ++e) out[(col + e) * d.dim + matrix_row] = state[i + e];
                 } else {
-                    st4(out + matrix_row * d.dim + col0 + i, make_float4(state[i], state[i + 1], state[i + 2], state[i + 3]));
+                    st4(out + matrix_row * d.dim + col, make_float4(state[i], state[i + 1], state[i + 2], state[i + 3]));
                 }
             }
         }
@@ -883,16 +917,22 @@ fmd_status encode(AllMaps& maps, const Decays& all, bool rows, int planes) {
     return st;
 }
 
-unsigned blocks_of(const Decays& d) { return unsigned(decay_segments(d.d[0]) * d.d[0].heads * d.count); }
+unsigned blocks_of(const Decays& d, int parts) { return unsigned(decay_segments(d.d[0]) * d.d[0].heads * d.count * parts); }
 
 template <int KS, int P>
 fmd_status launch_rows(const AllMaps& maps, const Decays& d, bool early, cudaStream_t s) {
     using S = RowsShape<KS, P>;
     const fmd_status st = grant_dynamic_smem((const void*)rows_kernel<KS, P>, S::kBytes, true);
     if (st != FMD_OK) return st;
-    if (early) return launch_early(rows_kernel<KS, P>, blocks_of(d), S::kThreads, S::kBytes, s, maps, d);
-    rows_kernel<KS, P><<<blocks_of(d), S::kThreads, S::kBytes, s>>>(maps, d);
-    return check_launch();
+    const int parts = parts_of(P, d.d[0].dim);
+    const unsigned blocks = blocks_of(d, parts);
+    if (early) {
+        const fmd_status first = launch_early(rows_kernel<KS, P>, blocks, S::kThreads, S::kBytes, s, maps, d, 0);
+        if (first != FMD_OK) return first;
+    } else {
+        rows_kernel<KS, P><<<blocks, S::kThreads, S::kBytes, s>>>(maps, d, 0);
+    }
+    return parts > 1 ? launch_early(rows_kernel<KS, P>, blocks, S::kThreads, S::kBytes, s, maps, d, 1) : check_launch();
 }
 
 template <int KS, int P, int PLANES>
@@ -900,8 +940,10 @@ fmd_status launch_states(const AllMaps& maps, const Decays& d, bool early, cudaS
     using S = StatesShape<KS, P, PLANES>;
     const fmd_status st = grant_dynamic_smem((const void*)states_kernel<KS, P, PLANES>, S::kBytes, true);
     if (st != FMD_OK) return st;
-    if (early) return launch_early(states_kernel<KS, P, PLANES>, blocks_of(d), S::kThreads, S::kBytes, s, maps, d);
-    states_kernel<KS, P, PLANES><<<blocks_of(d), S::kThreads, S::kBytes, s>>>(maps, d);
+    const int parts = parts_of(P, d.d[0].dim);
+    const unsigned blocks = blocks_of(d, parts * parts);
+    if (early) return launch_early(states_kernel<KS, P, PLANES>, blocks, S::kThreads, S::kBytes, s, maps, d);
+    states_kernel<KS, P, PLANES><<<blocks, S::kThreads, S::kBytes, s>>>(maps, d);
     return check_launch();
 }
 

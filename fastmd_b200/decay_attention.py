@@ -17,9 +17,6 @@ from ._first_order import first_order, has_tangent
 from ._lib import FmdDecay, c_size_t, call, on_device, ptr, stream
 from .head_rotary import TYPES, _head_rows, _like
 
-#: float32 heads of up to this many values go through planes, which the forward pass hands to the backward pass
-PLANES_DIM = 64
-
 
 def _problem(q, k, v, log_decay, offsets, scale) -> FmdDecay:
     return FmdDecay(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), ptr(offsets), q.shape[0], q.stride(0),
@@ -52,7 +49,7 @@ class _DecayAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, offsets, state, scale, keep):
         out, after, workspace = _forward(q, k, v, log_decay, offsets, state, scale, keep)
-        if q.dtype != torch.float32 or q.shape[2] > PLANES_DIM:
+        if q.dtype != torch.float32:
             workspace = None
         ctx.save_for_backward(q, k, v, log_decay, offsets, state, workspace)
         ctx.scale = scale
@@ -136,7 +133,7 @@ def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, offsets:
     (1.4 of it in all). Sequences do not see each other's values, finite or not; within a sequence a value that is not finite
     may reach earlier rows too (0 * inf), and an infinity may give NaN. A ``log_decay`` of NaN gives NaN. Sequences are taken
     in chunks and, where they are few and long, in segments that run side by side. For the backward pass a call in float32
-    with ``dim`` up to 64 keeps the planes of q, k and v (6 bytes a value). As for any autograd function, a backward pass is
+    keeps the planes of q, k and v (6 bytes a value). As for any autograd function, a backward pass is
     captured in a CUDA graph only while no eager graph of the same leaves is alive."""
     _lib.require_cuda(q, k, v, log_decay, offsets, state)
     scale = _check(q, k, v, log_decay, scale)

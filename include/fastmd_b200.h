@@ -1198,8 +1198,7 @@ FMD_API fmd_status fmd_decay_attention(const fmd_decay* problem, const float* st
 /* Gradients of q, k, v (contiguous) and of the first states, each may be
  * NULL, from those of out (g, strides g_row, g_head) and of the last states
  * (gafter, NULL: none). `forward`: the forward pass's workspace as it left it
- * (the planes of q, k and v that float32 heads of up to 64 values need), or
- * NULL. Deterministic. */
+ * (in float32 the planes of q, k and v), or NULL. Deterministic. */
 FMD_API fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state, const void* forward,
                                            const void* g, int64_t g_row, int64_t g_head, const float* gafter, void* dq,
                                            void* dk, void* dv, float* dstate, void* workspace, size_t workspace_bytes,
