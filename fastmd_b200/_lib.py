@@ -56,6 +56,12 @@ class FmdFeedForward(ctypes.Structure):
                 ("_pad", c_int32)]
 
 
+class FmdPadded(ctypes.Structure):
+    """A matrix and where its rows go, for fmd_pad_rows."""
+    _fields_ = [("source", c_void_p), ("to", c_void_p), ("rows", c_int64), ("columns", c_int64), ("from_row", c_int64),
+                ("from_column", c_int64), ("to_row", c_int64)]
+
+
 class FmdDecay(ctypes.Structure):
     """The problem of fmd_decay_attention, its backward pass and its step."""
     _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("log_decay", c_void_p), ("offsets", c_void_p),
@@ -156,6 +162,7 @@ _SIGNATURES: dict[str, list] = {
     "fmd_packed_attention_bwd": [POINTER(FmdAttention), _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, c_size_t, _P, _P],
     "fmd_gated_feed_forward_bytes": [POINTER(FmdFeedForward), _I32, POINTER(c_size_t), POINTER(c_size_t),
                                      POINTER(c_size_t)],
+    "fmd_pad_rows": [POINTER(FmdPadded), _I32, _P],
     "fmd_gated_feed_forward": [POINTER(FmdFeedForward), _P, _I32, _P, c_size_t, _P, c_size_t, _P, _P],
     "fmd_gated_feed_forward_bwd": [POINTER(FmdFeedForward), _P, c_size_t, _P, _I64, _P, _P, _P, _P, _P, c_size_t, _P, _P],
     "fmd_decay_attention_workspace_bytes": [POINTER(FmdDecay), _I32, POINTER(c_size_t)],
@@ -296,6 +303,7 @@ def flags_word(device) -> torch.Tensor:
 c_int32_t, c_int64_t = c_int32, c_int64
 c_void_p_t = c_void_p
 
-__all__ = ["FastMDLibraryError", "FmdAttention", "FmdCatPart", "FmdDecay", "FmdFeedForward", "FmdHeadRotarySide", "call",
+__all__ = ["FastMDLibraryError", "FmdAttention", "FmdCatPart", "FmdDecay", "FmdFeedForward", "FmdHeadRotarySide",
+           "FmdPadded", "call",
            "check", "declare", "flags_word", "lib", "on_device", "ptr",
            "require_cuda", "stream", "c_double", "c_float", "c_int32", "c_int64", "c_void_p", "ctypes"]

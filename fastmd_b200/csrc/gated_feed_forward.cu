@@ -329,7 +329,8 @@ __device__ __forceinline__ void put_floats(unsigned char* scratch, const float* 
     put_rows<N / 4>(scratch, w, to, row * 4, rows, (columns + 3) / 4);
 }
 
-// N columns of a result's rows, `columns` of which exist; rows start anywhere unless `vector`.
+// N columns of a result's rows, `columns` of which exist. Rows start at multiples of 16 bytes (`vector`), else in 16 bits at
+// words where they are of even length, or anywhere.
 template <int N, typename T>
 __device__ __forceinline__ void put_result(unsigned char* scratch, const float (&v)[N], T* to, int64_t row, int rows, int columns,
                                            bool vector) {
@@ -358,6 +359,14 @@ __device__ __forceinline__ void put_result(unsigned char* scratch, const float (
 #pragma unroll
                 for (int i = 0; i < 32; ++i) cells[(lane - turn) * 33 + i] = v[part + i];
             __syncwarp();
+            if (sizeof(T) == 2 && row % 2 == 0) {  // two rows at a time
+                const int c = lane % 16 * 2;
+                for (int r = lane / 16; r < 16 && turn + r < rows; r += 2)
+                    if (part + c < columns)
+                        *reinterpret_cast<uint32_t*>(to + (turn + r) * row + part + c) =
+                            pack_bf16(cells[r * 33 + c], cells[r * 33 + c + 1]);
+                continue;
+            }
             for (int r = 0; r < 16 && turn + r < rows; ++r)
                 if (part + lane < columns) store1(to + (turn + r) * row + part + lane, cells[r * 33 + lane]);
         }
@@ -955,6 +964,28 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitArgs a) {
     }
 }
 
+// Matrices of 16-bit values with any strides, up to four (blockIdx.y), as rows that TMA reads: `row` values apart, a multiple
+// of 8, with zeros behind their columns. 27,341 rows of 1,812: 49 us, 4.1 TB/s.
+struct PadArgs {
+    fmd_padded x[4];
+};
+
+__global__ void __launch_bounds__(256) pad_kernel(const PadArgs a) {
+    const fmd_padded& x = a.x[blockIdx.y];
+    const int per = int(x.to_row / 8);
+    const int64_t all = x.rows * per;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += int64_t(gridDim.x) * 256) {
+        const int64_t row = i / per;
+        const int c = int(i - row * per) * 8;
+        const uint16_t* from = static_cast<const uint16_t*>(x.from) + row * x.from_row + c * x.from_column;
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = c + e < x.columns ? __ldg(from + e * x.from_column) : 0u;
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(x.to) + row * x.to_row + c) =
+            make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+    }
+}
+
 // The tiles that were shared out: the sums of their shares, in their order. blockIdx.y: the tile; a thread per four columns.
 template <typename T>
 __global__ void __launch_bounds__(256) add_kernel(const Args g) {
@@ -1302,6 +1333,23 @@ fmd_status fmd_gated_feed_forward_bytes(const fmd_feed_forward* problem, int32_t
     *forward = few || z.rows == 0 ? 0 : down_plan(z).bytes();
     *backward = z.rows > 0 && keep ? scratch_layout(z).bytes : 0;
     return FMD_OK;
+}
+
+fmd_status fmd_pad_rows(const fmd_padded* x, int32_t count, void* stream) {
+    if (x == nullptr || count < 1 || count > 4) return FMD_ERR_INVALID_ARGUMENT;
+    PadArgs a{};
+    int64_t most = 0;
+    for (int i = 0; i < count; ++i) {
+        if (x[i].rows < 0 || x[i].columns < 1 || x[i].columns > (1 << 20) || x[i].to_row < x[i].columns || x[i].to_row % 8 != 0 ||
+            (x[i].rows > 0 && (x[i].from == nullptr || x[i].to == nullptr)))
+            return FMD_ERR_INVALID_ARGUMENT;
+        if (!aligned16(x[i].to) || x[i].to_row > (1 << 24) || x[i].rows > (1 << 28)) return FMD_ERR_UNSUPPORTED;
+        a.x[i] = x[i];
+        most = x[i].rows * (x[i].to_row / 8) > most ? x[i].rows * (x[i].to_row / 8) : most;
+    }
+    if (most == 0) return FMD_OK;
+    pad_kernel<<<dim3(unsigned(grid_for(most, 256)), unsigned(count)), 256, 0, as_stream(stream)>>>(a);
+    return check_launch();
 }
 
 fmd_status fmd_gated_feed_forward(const fmd_feed_forward* problem, void* y, int32_t keep, void* kept, size_t kept_bytes,

@@ -13,24 +13,39 @@ from torch.autograd import Function
 
 from . import _lib
 from ._first_order import first_order, has_tangent
-from ._lib import FmdFeedForward, c_size_t, call, on_device, ptr, stream
+from ._lib import FmdFeedForward, FmdPadded, c_size_t, call, on_device, ptr, stream
 from .head_rotary import TYPES
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
 
 
-def _rows(x: Tensor) -> Tensor:
-    """``x`` with unit stride inside a row and, in 16 bits, rows that start at multiples of 16 bytes; copied only when
-    needed."""
+def _ready(x: Tensor) -> bool:
+    """Whether the kernels read ``x`` as it is: unit stride inside a row and, in 16 bits, rows at multiples of 16 bytes."""
     row, unit = x.stride()
     rows, columns = x.shape
     whole = (unit == 1 or columns == 1) and (row >= columns or rows <= 1)
-    if x.dtype == torch.float32:
-        return x if whole else x.contiguous()
-    if whole and not (x.data_ptr() % 16 or (row % 8 and rows > 1)):
-        return x
-    room = torch.empty(rows, (columns + 7) // 8 * 8, device=x.device, dtype=x.dtype)
-    return room[:, :columns].copy_(x)
+    return whole and (x.dtype == torch.float32 or not (x.data_ptr() % 16 or (row % 8 and rows > 1)))
+
+
+def _rows(*tensors: Tensor) -> tuple[Tensor, ...]:
+    """The tensors as the kernels read them; those that are not are copied, in 16 bits by one kernel, to padded rows. Not for
+    autograd to see: the gradients belong to the tensors themselves."""
+    some = [t for t in tensors if not _ready(t)]
+    if not some:
+        return tensors
+    if some[0].dtype == torch.float32:
+        copies = iter([t.contiguous() for t in some])
+    else:
+        wide = [(t.shape[1] + 7) // 8 * 8 for t in some]
+        starts = [0]
+        for t, row in zip(some, wide):
+            starts.append(starts[-1] + (t.shape[0] * row + 127) // 128 * 128)
+        room = torch.empty(starts[-1], device=some[0].device, dtype=some[0].dtype)
+        made = [room.as_strided(t.shape, (row, 1), at) for t, row, at in zip(some, wide, starts)]
+        call("fmd_pad_rows", (FmdPadded * len(some))(*((t.data_ptr(), m.data_ptr(), *t.shape, *t.stride(), row)
+                                                       for t, m, row in zip(some, made, wide))), len(some), stream(room.device))
+        copies = iter(made)
+    return tuple(t if _ready(t) else next(copies) for t in tensors)
 
 
 def _problem(x, gate, up, down, activation) -> FmdFeedForward:
@@ -58,17 +73,19 @@ def _forward(x, gate, up, down, activation, keep):
 class _GatedFeedForward(Function):
     @staticmethod
     def forward(ctx, x, gate, up, down, activation):
-        y, kept, ctx.size = _forward(x, gate, up, down, activation, True)
-        ctx.save_for_backward(x, gate, up, down, kept)
+        given = (x, gate, up, down)
+        rows = _rows(*given)
+        y, kept, ctx.size = _forward(*rows, activation, True)
+        ctx.save_for_backward(*given, kept, *(None if a is b else a for a, b in zip(rows, given)))
         ctx.activation = activation
         return y
 
     @staticmethod
     def backward(ctx, g):
-        x, gate, up, down, kept = ctx.saved_tensors
-        like, device = (x, gate, up, down), x.device
-        inputs = (g, *like)
-        g = _rows(g)
+        *like, kept, x, gate, up, down = ctx.saved_tensors
+        x, gate, up, down = (b if a is None else a for a, b in zip((x, gate, up, down), like))
+        device, inputs = x.device, (g, *like)
+        g, = _rows(g)
         grads = [torch.empty(t.shape, device=device, dtype=t.dtype) if need else None
                  for t, need in zip(like, ctx.needs_input_grad)]
         workspace = torch.empty(ctx.size, device=device, dtype=torch.uint8)
@@ -112,13 +129,13 @@ def gated_feed_forward(x: Tensor, gate: Tensor, up: Tensor, down: Tensor, *, act
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
     flat = x if len(lead) == 2 else x.reshape(-1, width)
-    args = (_rows(flat), _rows(gate), _rows(up), _rows(down), ACTIVATIONS[activation])
+    args, kind = (flat, gate, up, down), ACTIVATIONS[activation]
     with on_device(x.device):
         if (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or up.requires_grad or down.requires_grad)) \
                 or has_tangent(x, gate, up, down):
-            y = _GatedFeedForward.apply(*args)
+            y = _GatedFeedForward.apply(*args, kind)
         else:
-            y = _forward(*args, False)[0]
+            y = _forward(*_rows(*args), kind, False)[0]
     return y if len(lead) == 2 else y.view(*lead[:-1], out)
 
 

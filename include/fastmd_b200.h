@@ -1142,6 +1142,18 @@ typedef struct fmd_feed_forward {
     int32_t width, hidden, out, type, activation, _pad;
 } fmd_feed_forward;
 
+/* A matrix of 16-bit values with any strides and where its rows go: to_row
+ * values apart, a multiple of 8, zeros behind the columns. */
+typedef struct fmd_padded {
+    const void* from;
+    void* to;
+    int64_t rows, columns, from_row, from_column, to_row;
+} fmd_padded;
+
+/* Copies of up to four such matrices, as fmd_gated_feed_forward reads them;
+ * `to` starts at a multiple of 16 bytes. */
+FMD_API fmd_status fmd_pad_rows(const fmd_padded* x, int32_t count, void* stream);
+
 /* From the sizes alone: `kept`, the bytes that the forward pass fills (with
  * keep = 1 for fmd_gated_feed_forward_bwd, else as scratch of its own), and
  * the workspaces of both passes. The buffers start at multiples of 16 bytes. */

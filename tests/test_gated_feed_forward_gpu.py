@@ -152,6 +152,25 @@ def test_strides_and_shapes(cuda, dtype):
 
 
 @gpu
+def test_rows_of_odd_length(cuda):
+    """bfloat16 rows that are copied first, transposed ones among them: the bits of padded storage, gradients of the tensors
+    themselves, and no second derivatives either."""
+    given = make(50, 37, 51, 29, B16)
+    padded = [torch.zeros(t.shape[0], 64, device="cuda", dtype=B16)[:, :t.shape[1]].copy_(t) for t in given]
+    turned = [t.T.contiguous().T for t in given]
+    results = []
+    for *leaves, g in (given, padded, turned):
+        leaves = [t.detach().requires_grad_() for t in leaves]
+        y = gated_feed_forward(*leaves)
+        grads = torch.autograd.grad(y, leaves, g, retain_graph=True, create_graph=True)
+        with pytest.raises(RuntimeError, match="first derivatives"):
+            torch.autograd.grad(grads[0].float().square().sum(), leaves[0])
+        results.append((y.detach(), gated_feed_forward(*(t.detach() for t in leaves)), *(x.detach() for x in grads)))
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
 def test_gradients_on_their_own(cuda, dtype):
     """Each gradient asked for by itself has the bits that it has among all, on every run."""
@@ -369,3 +388,12 @@ def test_bad_arguments_of_the_entry_points_launch_nothing():
     assert lib.fmd_gated_feed_forward_bwd(f, p, 8, p, 16, p, p, p, p, p, 1 << 20, None, None) == 4
     assert lib.fmd_gated_feed_forward_bwd(f, p, 1 << 20, p, 16, p, p, p, p, p, 8, None, None) == 4
     assert lib.fmd_gated_feed_forward_bwd(f, p, 1 << 20, p, 17, p, p, p, p, p, 1 << 20, None, None) == 3
+    one = dict(source=(1 << 20) + 2, to=1 << 20, rows=5, columns=17, from_row=17, from_column=1, to_row=24)
+
+    def pad(count=1, **change):
+        return lib.fmd_pad_rows((_lib.FmdPadded * 4)(_lib.FmdPadded(**{**one, **change})), count, None)
+
+    assert lib.fmd_pad_rows(None, 1, None) == 1 and pad(0) == 1 and pad(5) == 1
+    for change in (dict(rows=-1), dict(columns=0), dict(to_row=16), dict(to_row=25), dict(source=None), dict(to=None)):
+        assert pad(**change) == 1, change
+    assert pad(to=(1 << 20) + 8) == 3 and pad(rows=0, source=None, to=None) == 0
