@@ -1,5 +1,5 @@
 // C entry points of decay attention: argument checks, the cut into segments, what is carried from segment to segment, and
-// the recurrence for single rows.
+// the recurrence row by row, for single rows and for sequences of a few.
 
 #include "decay_attention.cuh"
 #include "tensor_cores.cuh"
@@ -135,6 +135,120 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const Decay d, float* st
     write(static_cast<T*>(d.out) + (b * d.heads + head) * dim + threadIdx.x, d.far * out);
 }
 
+__device__ __forceinline__ float4 read4(const float* p) { return ldg4(p); }
+__device__ __forceinline__ float4 read4(const __nv_bfloat16* p) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+    const float2 x = unpack_bf16(w.x), y = unpack_bf16(w.y);
+    return make_float4(x.x, x.y, y.x, y.y);
+}
+__device__ __forceinline__ void write4(float* p, float4 v) { st4(p, v); }
+__device__ __forceinline__ void write4(__nv_bfloat16* p, float4 v) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+}
+
+// Sequences of a few rows, row by row: the step above, with the matrix in registers from the first row to the last and in either
+// direction. A block per sequence, head, pass and 32 columns of the matrix (which do not see each other); a thread holds four
+// columns of every 32nd row. It takes four rows at a time, whose sums over the matrix's rows are joined together.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) few_rows_kernel(const __grid_constant__ Decays all) {
+    constexpr int kRows = 4, kQuads = 8, kGroups = kThreads / kQuads, kMost = 128 / kGroups;
+    __shared__ alignas(16) float2 ab[kRows][128];
+    __shared__ float4 c[kRows][kQuads], sums[kThreads / 32][kRows][kQuads];
+    const Decay& d = all.d[blockIdx.x % unsigned(all.count)];
+    const int dim = d.dim, quads = dim / 4, parts = (quads + kQuads - 1) / kQuads;
+    const unsigned place = blockIdx.x / unsigned(all.count), whose = place / unsigned(parts);
+    const int head = int(whose % unsigned(d.heads)), seq = int(whose / unsigned(d.heads));
+    const int quad0 = int(place % unsigned(parts)) * kQuads;
+    if (head == 0 && quad0 == 0 && threadIdx.x == 0) check_offsets(d, seq);
+    const int64_t lo = min(max(d.offsets[seq], int64_t(0)), d.rows), hi = min(max(d.offsets[seq + 1], lo), d.rows), n = hi - lo;
+    const int x = int(threadIdx.x), quad = x % kQuads, group = x / kQuads;
+    const bool here = quad0 + quad < quads;
+    const float keep = exp2f(log2_decay(d, head));
+    // who brings what of the next four rows: four warps a and b, a fifth c
+    const bool brings_ab = x < 128 && x % 32 < quads, brings_c = x >= 128 && x < 160 && here;
+    const int row_of = brings_c ? x / kQuads % kRows : x / 32;
+    auto row_at = [&](int64_t i) { return d.later ? hi - 1 - i : lo + i; };
+    float4 next[2] = {};
+    auto fetch = [&](int64_t i) {
+        if (i + row_of >= n) return;
+        const int64_t t = row_at(i + row_of);
+        if (brings_ab) {
+            next[0] = read4(static_cast<const T*>(d.a) + t * d.a_row + head * d.a_head + x % 32 * 4);
+            next[1] = read4(static_cast<const T*>(d.b) + t * d.b_row + head * d.b_head + x % 32 * 4);
+        } else if (brings_c) {
+            next[0] = read4(static_cast<const T*>(d.c) + t * d.c_row + head * d.c_head + (quad0 + quad) * 4);
+        }
+    };
+    fetch(0);
+    // value (r, col) of a given matrix lies at r * down + col * right
+    const int64_t mine = (int64_t(seq) * d.heads + head) * dim * dim;
+    const int down = d.transposed ? 1 : dim, right = d.transposed ? dim : 1;
+    float4 s[kMost];
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        const int r = group + i * kGroups;
+        s[i] = f4_zero();
+        if (d.start != nullptr && here && r < dim) {
+            const float* p = d.start + mine + r * down + 4 * (quad0 + quad) * right;
+            s[i] = d.transposed ? make_float4(p[0], p[dim], p[2 * dim], p[3 * dim]) : ldg4(p);
+        }
+    }
+    for (int64_t i = 0; i < n; i += kRows) {
+        if (brings_ab) {
+            const float4 p = next[0], q = next[1];
+            float2* to = &ab[row_of][x % 32 * 4];
+            to[0] = make_float2(p.x, d.add * q.x), to[1] = make_float2(p.y, d.add * q.y);
+            to[2] = make_float2(p.z, d.add * q.z), to[3] = make_float2(p.w, d.add * q.w);
+        } else if (brings_c) {
+            c[row_of][quad] = next[0];
+        }
+        __syncthreads();
+        fetch(i + kRows);
+        const int rows = int(min(int64_t(kRows), n - i));
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+            if (j >= rows) break;
+            const float w = d.later && i + j == 0 ? 1.0f : keep;
+            const float4 y = c[j][quad];
+            float4 sum = f4_zero();
+#pragma unroll
+            for (int m = 0; m < kMost; ++m) {
+                const int r = group + m * kGroups;
+                if (r >= dim) break;
+                const float2 u = ab[j][r];
+                s[m] = make_float4(fmaf(w, s[m].x, u.y * y.x), fmaf(w, s[m].y, u.y * y.y), fmaf(w, s[m].z, u.y * y.z),
+                                   fmaf(w, s[m].w, u.y * y.w));
+                sum = make_float4(fmaf(u.x, s[m].x, sum.x), fmaf(u.x, s[m].y, sum.y), fmaf(u.x, s[m].z, sum.z),
+                                  fmaf(u.x, s[m].w, sum.w));
+            }
+#pragma unroll
+            for (int e = kQuads; e < 32; e *= 2)
+                sum = f4_add(sum, make_float4(__shfl_xor_sync(0xffffffffu, sum.x, e), __shfl_xor_sync(0xffffffffu, sum.y, e),
+                                              __shfl_xor_sync(0xffffffffu, sum.z, e), __shfl_xor_sync(0xffffffffu, sum.w, e)));
+            if (x % 32 < kQuads) sums[x / 32][j][quad] = sum;
+        }
+        __syncthreads();
+        const int j = x / kQuads;
+        if (d.out == nullptr || !here || j >= rows) continue;
+        float4 out = f4_zero();
+#pragma unroll
+        for (int g = 0; g < kThreads / 32; ++g) out = f4_add(out, sums[g][j][quad]);
+        write4(static_cast<T*>(d.out) + (row_at(i + j) * d.heads + head) * dim + 4 * (quad0 + quad),
+               make_float4(d.far * out.x, d.far * out.y, d.far * out.z, d.far * out.w));
+    }
+    if (d.after == nullptr || !here) return;
+    const float w = d.later && n > 0 ? keep : 1.0f;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        const int r = group + i * kGroups;
+        if (r >= dim) break;
+        float* p = d.after + mine + r * down + 4 * (quad0 + quad) * right;
+        const float4 v = make_float4(w * s[i].x, w * s[i].y, w * s[i].z, w * s[i].w);
+        if (d.transposed) p[0] = v.x, p[dim] = v.y, p[2 * dim] = v.z, p[3 * dim] = v.w;
+        else st4(p, v);
+    }
+}
+
 fmd_status check(const fmd_decay& p, Decay& d, bool rows_aligned) {
     if ((p.type != FMD_F32 && p.type != FMD_BF16) || p.rows < 0 || p.batch < 0 || p.heads < 1 || p.dim < 8 || p.dim > 128 ||
         p.dim % 8 || !(p.scale >= 0.0f && p.scale <= 1.0e38f) || p.log_decay == nullptr ||
@@ -164,12 +278,30 @@ fmd_status check_rows(const fmd_decay& p, Decay& d) {
     return FMD_OK;
 }
 
+// Whether the sequences are taken row by row: up to 16 rows each on average, in float32 32. us row by row and by chunks, 23
+// sequences with states, 32 heads: heads of 128 in bfloat16, 1 row 25 and 134, 16 rows 64 and 137, 33 rows 115 and 142, with
+// gradients 237 and 377, 435 and 386; in float32 1 row 25 and 348, 33 rows 106 and 386, with gradients 411 and 1,220; heads of 64
+// in bfloat16 28 and 71 (16 rows), 48 and 73 (33). Four sequences, 8 heads: 23 and 27 (16 rows, bfloat16), 22 and 34 (33,
+// float32), what the host needs. All rows may be one sequence's, which then takes 0.3 us a row: 500 rows 156 and 43 (32 heads
+// of 128, bfloat16).
+bool few_rows(const Decay& d, int type) { return d.rows <= (type == FMD_F32 ? 32 : 16) * int64_t(d.batch); }
+
+fmd_status run_few(const Decays& all, int type, cudaStream_t s) {
+    const Decay& d = all.d[0];
+    if (all.count == 0 || d.batch == 0) return FMD_OK;
+    const int64_t blocks = int64_t(d.batch) * d.heads * all.count * ((d.dim + 31) / 32);
+    if (blocks > INT32_MAX) return FMD_ERR_UNSUPPORTED;
+    if (type == FMD_BF16) few_rows_kernel<__nv_bfloat16><<<unsigned(blocks), kThreads, 0, s>>>(all);
+    else few_rows_kernel<float><<<unsigned(blocks), kThreads, 0, s>>>(all);
+    return check_launch();
+}
+
 // Rows of a segment: whole sequences where these are blocks enough for the GPU or short; else so many that the segments fill
 // it once (the sequences' last ones are half a segment long on average). Segments cost a second look at two of the three
 // inputs and two more launches.
 int64_t segment_length(const Decay& d, bool planes) {
     const int64_t heads = d.heads * (planes && d.dim > 64 ? 2 : 1);  // blocks for a sequence
-    if (d.batch == 0 || d.rows / d.batch <= 512 || 10 * d.batch * heads >= 6 * kNumSMs) return kWhole;
+    if (d.rows / d.batch <= 512 || 10 * d.batch * heads >= 6 * kNumSMs) return kWhole;
     const int64_t want = 2 * kNumSMs / heads - d.batch;  // twice the segments, less the sequences' last ones
     const int64_t length = (2 * d.rows / (want > 1 ? want : 1) + 127) / 128 * 128;
     return length < 256 ? 256 : length;
@@ -181,6 +313,7 @@ size_t plane_bytes(const Decay& d) { return (size_t(d.rows) * d.heads * d.dim * 
 
 // Planes of `arrays` inputs (float32), and what the segments of `passes` passes add.
 size_t workspace_of(Decay d, int type, int arrays, int passes) {
+    if (few_rows(d, type)) return 0;
     const bool planes = type == FMD_F32;
     d.length = segment_length(d, planes);
     return (planes ? arrays * plane_bytes(d) : 0) + (d.length < kWhole ? passes * matrices(d, decay_segments(d)) : 0);
@@ -195,7 +328,6 @@ struct Input {
 // The planes of `inputs`, the first `made` of which are there already, at `made_at`; their room stays in the workspace.
 fmd_status make_planes(const Decay& d, Input* inputs, int count, int made, const void* made_at, char*& workspace,
                        cudaStream_t s) {
-    if (d.rows == 0) return FMD_OK;
     SplitArgs a{};
     a.rows = d.rows;
     a.heads = d.heads;
@@ -229,20 +361,19 @@ fmd_status run_states(const Decays& d, bool planes, bool early, cudaStream_t s) 
 // Passes of the recurrence over the same rows, side by side: with segments what these add comes first.
 fmd_status mix(Decays all, bool planes, char* workspace, cudaStream_t s) {
     const Decay& d = all.d[0];
-    if (all.count == 0 || d.batch == 0) return FMD_OK;
-    int64_t length = segment_length(d, planes);
-    if (d.rows == 0) length = 1;  // nothing but the matrices to hand on
+    if (all.count == 0) return FMD_OK;
+    const int64_t length = segment_length(d, planes);
     for (int i = 0; i < all.count; ++i) all.d[i].length = length;
     const int64_t segments = decay_segments(d);
     if (4 * segments * d.heads * all.count > INT32_MAX || int64_t(d.batch) * d.heads > INT32_MAX) return FMD_ERR_UNSUPPORTED;
     fmd_status st = FMD_OK;
-    bool early = planes && d.rows > 0;  // behind the kernel that makes the planes
+    bool early = planes;  // behind the kernel that makes them
     if (length < kWhole) {
         for (int i = 0; i < all.count; ++i) {
             all.d[i].states = reinterpret_cast<float*>(workspace);
-            workspace += d.rows > 0 ? matrices(d, segments) : 0;
+            workspace += matrices(d, segments);
         }
-        if (d.rows > 0 && (st = run_states(all, planes, early, s)) != FMD_OK) return st;
+        if ((st = run_states(all, planes, early, s)) != FMD_OK) return st;
         const dim3 grid(unsigned(d.batch) * d.heads, unsigned((d.dim * d.dim + 4 * kThreads - 1) / (4 * kThreads)),
                         unsigned(all.count));
         if ((st = launch_early(carry_kernel, grid, kThreads, 0, s, all)) != FMD_OK) return st;
@@ -257,7 +388,7 @@ fmd_status mix(Decays all, bool planes, char* workspace, cudaStream_t s) {
     Decays rows{};
     for (int i = 0; i < all.count; ++i)
         if (all.d[i].out != nullptr) rows.d[rows.count++] = all.d[i];
-    if (d.rows == 0 || rows.count == 0) return FMD_OK;
+    if (rows.count == 0) return FMD_OK;
     return planes ? decay_rows_planes(rows, early, s) : decay_rows_mma(rows, early, s);
 }
 
@@ -289,7 +420,7 @@ fmd_status fmd_decay_attention(const fmd_decay* problem, const float* state, voi
     if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return FMD_ERR_WORKSPACE;
     if (!aligned16(out) || !aligned16(state) || !aligned16(after) || !aligned16(workspace)) return FMD_ERR_UNSUPPORTED;
     const cudaStream_t s = as_stream(stream);
-    const bool planes = p.type == FMD_F32;
+    const bool few = few_rows(d, p.type), planes = p.type == FMD_F32 && !few;
     char* at = static_cast<char*>(workspace);
     Input in[3] = {{p.q, p.q_row, p.q_head}, {p.k, p.k_row, p.k_head}, {p.v, p.v_row, p.v_head}};
     if (planes && (st = make_planes(d, in, 3, 0, nullptr, at, s)) != FMD_OK) return st;
@@ -300,7 +431,7 @@ fmd_status fmd_decay_attention(const fmd_decay* problem, const float* state, voi
     d.flags = flags;
     d.near = d.far = p.scale;
     d.add = 1.0f;
-    return mix(Decays{{d}, 1}, planes, at, s);
+    return few ? run_few(Decays{{d}, 1}, p.type, s) : mix(Decays{{d}, 1}, planes, at, s);
 }
 
 fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state, const void* forward, const void* g,
@@ -319,7 +450,7 @@ fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state,
         (p.rows > 0 && !vector_rows(g, g_row, g_head, p.type == FMD_BF16 ? 2 : 4)))
         return FMD_ERR_UNSUPPORTED;
     const cudaStream_t s = as_stream(stream);
-    const bool planes = p.type == FMD_F32;
+    const bool few = few_rows(d, p.type), planes = p.type == FMD_F32 && !few;
     char* at = static_cast<char*>(workspace);
     Input in[4] = {{p.q, p.q_row, p.q_head}, {p.k, p.k_row, p.k_head}, {p.v, p.v_row, p.v_head}, {g, g_row, g_head}};
     if (planes && (st = make_planes(d, in, 4, forward != nullptr ? 3 : 0, forward, at, s)) != FMD_OK) return st;
@@ -357,7 +488,7 @@ fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state,
         m.far = p.scale;
         all.d[all.count++] = m;
     }
-    return mix(all, planes, at, s);
+    return few ? run_few(all, p.type, s) : mix(all, planes, at, s);
 }
 
 fmd_status fmd_decay_attention_step(const fmd_decay* problem, float* state, void* out, void* stream) {

@@ -710,7 +710,8 @@ __global__ void __launch_bounds__(RowsShape<KS, P>::kThreads, 1)
             warp_arrive(&ctl.stored[i & 1]);
             if (count < kTile) {
                 const int first_row = (warp & 3) * 32, left = min(kColumns, d.dim - first_out - col0) * S::kSize / 16;
-                T* out = static_cast<T*>(d.out) + (int64_t(walk.first(i) + first_row) * d.heads + head) * d.dim + first_out + col0;
+                T* out = static_cast<T*>(d.out) + (int64_t(walk.first(i) + first_row) * d.heads + head) * d.dim + first_out +
+                         col0;
                 if (P == 3 && part > 0)
                     add_pieces<kWide>(row, out, int64_t(d.heads) * d.dim * S::kSize, count - first_row, left);
                 store_pieces<kWide>(row, out, int64_t(d.heads) * d.dim * S::kSize, count - first_row, left);

@@ -131,10 +131,10 @@ def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, offsets:
     run. Sums and matrices are held in 32 bits, and states are exact to FP32 in both types; in bfloat16 the weights of the
     pairs of rows and the decayed rows are rounded once as operands, which costs an output about as much as its own rounding
     (1.4 of it in all). Sequences do not see each other's values, finite or not; within a sequence a value that is not finite
-    may reach earlier rows too (0 * inf), and an infinity may give NaN. A ``log_decay`` of NaN gives NaN. Sequences are taken
-    in chunks and, where they are few and long, in segments that run side by side. For the backward pass a call in float32
-    keeps the planes of q, k and v (6 bytes a value). As for any autograd function, a backward pass is
-    captured in a CUDA graph only while no eager graph of the same leaves is alive."""
+    may reach earlier rows too (0 * inf), and an infinity may give NaN. A ``log_decay`` of NaN gives NaN. Sequences of a
+    few rows are taken row by row, others in chunks and, where they are few and long, in segments that run side by side. For
+    the backward pass a call in float32 keeps the planes of q, k and v (6 bytes a value). As for any autograd function, a
+    backward pass is captured in a CUDA graph only while no eager graph of the same leaves is alive."""
     _lib.require_cuda(q, k, v, log_decay, offsets, state)
     scale = _check(q, k, v, log_decay, scale)
     if offsets.dim() != 1 or offsets.shape[0] < 1 or offsets.dtype != torch.int64:

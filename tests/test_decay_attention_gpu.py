@@ -133,7 +133,7 @@ def run_case(sizes, heads, dim, dtype, with_state, seed=0):
 
 SEQUENCES = {
     "one": [1], "two": [2, 1], "frames": [135, 135, 135], "edges": [63, 64, 65, 1, 0, 127, 128, 129, 255, 0],
-    "ragged": [5, 200, 0, 3, 311], "long": [1500], "zeros": [0, 0, 70],
+    "ragged": [5, 200, 0, 3, 311], "long": [1500], "zeros": [0, 0, 70], "short": [3, 0, 17, 1, 40, 5, 4, 8, 9], "single": [1] * 5,
 }
 
 
@@ -144,6 +144,13 @@ SEQUENCES = {
 @pytest.mark.parametrize("heads,dim", [(1, 8), (3, 64), (4, 128), (2, 32)])
 def test_against_the_formulas(cuda, heads, dim, name, with_state, dtype):
     run_case(SEQUENCES[name], heads, dim, dtype, with_state, seed=dim + heads)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+@pytest.mark.parametrize("dim", [16, 24, 40, 48, 56, 72, 80, 88, 96, 104, 112, 120])
+def test_every_head_size_row_by_row(cuda, dim, dtype):
+    run_case([5, 13, 0, 8, 1], 2, dim, dtype, True)
 
 
 @gpu
@@ -237,6 +244,42 @@ def test_strong_and_no_decay(cuda, dtype):
     now = state.clone()
     decay_attention_step(q[:1], k[:1], v[:1], log, now)
     assert torch.isfinite(now).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+def test_row_by_row_and_by_chunks(cuda, dtype):
+    """The same rows as a batch of short sequences and beside a long one: decays at their limits, values of other sequences
+    that are not finite, parts of the gradients, and offsets that do not fit."""
+    sizes, heads, dim = [7, 0, 12, 1, 4], 4, 72
+    q, k, v, g, state, gafter, offsets = make(sizes + [900], heads, dim, dtype)
+    log = torch.tensor([0.0, -math.inf, -200.0, 1.0], device="cuda")
+    q.data[3:5], state[2] = float("nan"), float("inf")  # of sequences 0 and 2
+
+    def run(q, k, v, state, offsets, g, gafter):
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k, v, state)]
+        out, after = decay_attention(*leaves[:3], log, offsets, leaves[3], return_state=True)
+        grads = torch.autograd.grad((out, after), leaves, (g, gafter), retain_graph=True)
+        (dv,) = torch.autograd.grad(out, leaves[2], g, retain_graph=True)
+        (dstate,) = torch.autograd.grad(after, leaves[3], gafter)
+        return out.detach(), after.detach(), *grads, dv, dstate
+
+    rows, places = slice(19, 24), [3, 4]  # of the two sequences that are finite
+    args = [t[rows] for t in (q, k, v)], torch.tensor([0.0, -1e4, -200.0, 0.0], device="cuda"), [1, 4], state[places]
+    bounds = [reference(*args[0], *args[1:], dim ** -0.5, *grads)
+              for grads in ((g[rows], gafter[places]), (g[rows], None), (None, gafter[places]))]
+    for got in (run(q[:24], k[:24], v[:24], state[:5], offsets[:6], g[:24], gafter[:5]),
+                run(q, k, v, state, offsets, g, gafter)):
+        for i, (name, x) in enumerate(zip(("out", "after", "dq", "dk", "dv", "dstate", "dv", "dstate"), got)):
+            want, err = bounds[max(0, i - 5)]
+            check(x[places if x.dim() == 4 else rows], want[name], err[name], f"{i} {name}")
+        assert torch.equal(got[1][1], state[1])  # nothing happened there
+    flags = _lib.flags_word(q.device)
+    for bad in ([0, 9, 7, 24], [1, 5, 9, 24], [0, 5, 9, 20], [0, 5, 9, 90], [0, -9, 9, 24], [0, 2 ** 60, 9, 24]):
+        flags.zero_()
+        decay_attention(q[:24], k[:24], v[:24], log, torch.tensor(bad, device="cuda"), return_state=True)
+        assert int(flags.item()) & 1, bad
+    flags.zero_()
 
 
 @gpu
