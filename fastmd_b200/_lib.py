@@ -273,11 +273,13 @@ def stream(device=None) -> int:
 
 
 _HERE = contextlib.nullcontext()
+_device_index = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def on_device(device):
-    """A context in which ``device`` is the current one, for launches on tensors that may lie elsewhere."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    """A context in which ``device``, that of a CUDA tensor, is the current one, for launches on tensors that may lie
+    elsewhere."""
+    return _HERE if device.index == _device_index() else torch.cuda.device(device)
 
 
 def require_cuda(*tensors) -> None:

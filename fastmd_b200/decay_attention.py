@@ -83,21 +83,24 @@ def _aligned_state(state: Tensor | None) -> Tensor | None:
     return state.clone() if state.data_ptr() % 16 else state
 
 
-def _check(q, k, v, log_decay, scale) -> float:
-    if q.dim() != 3 or k.shape != q.shape or v.shape != q.shape:
+def _check(q, k, v, log_decay, scale, *others) -> float:
+    shape, kind, index = q.shape, q.dtype, q.get_device()
+    if index < 0 or k.get_device() != index or v.get_device() != index or log_decay.get_device() != index \
+            or any(t is not None and t.get_device() != index for t in others):
+        _lib.require_cuda(q, k, v, log_decay, *others)
+        raise ValueError("all tensors must be on the device of q")
+    if len(shape) != 3 or k.shape != shape or v.shape != shape:
         raise ValueError("q, k and v must all be [rows, heads, dim], got "
-                         f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
-    if q.dtype not in TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError(f"q, k and v must all be float32 or bfloat16, got {q.dtype}, {k.dtype} and {v.dtype}")
-    heads, dim = q.shape[1:]
+                         f"{tuple(shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    if kind not in TYPES or k.dtype != kind or v.dtype != kind:
+        raise ValueError(f"q, k and v must all be float32 or bfloat16, got {kind}, {k.dtype} and {v.dtype}")
+    _, heads, dim = shape
     if dim % 8 or not 8 <= dim <= 128:
         raise ValueError(f"the head size must be a multiple of 8 up to 128, got {dim}")
     if not 1 <= heads <= 1024:
         raise ValueError(f"between 1 and 1024 heads, got {heads}")
     if log_decay.shape != (heads,) or log_decay.dtype != torch.float32:
         raise ValueError(f"log_decay must be float32 [{heads}], got {log_decay.dtype} {tuple(log_decay.shape)}")
-    if not q.device == k.device == v.device == log_decay.device:
-        raise ValueError("q, k, v and log_decay must be on one device")
     scale = dim ** -0.5 if scale is None else float(scale)
     if not 0.0 <= scale <= 1e38:
         raise ValueError(f"scale must be between 0 and 1e38, got {scale}")
@@ -105,11 +108,9 @@ def _check(q, k, v, log_decay, scale) -> float:
 
 
 def _check_state(state, batch, q) -> None:
-    shape = (batch, q.shape[1], q.shape[2], q.shape[2])
-    if tuple(state.shape) != shape or state.dtype != torch.float32:
-        raise ValueError(f"state must be float32 {list(shape)}, got {state.dtype} {list(state.shape)}")
-    if state.device != q.device:
-        raise ValueError("state must be on the device of q")
+    _, heads, dim = q.shape
+    if state.shape != (batch, heads, dim, dim) or state.dtype != torch.float32:
+        raise ValueError(f"state must be float32 {[batch, heads, dim, dim]}, got {state.dtype} {list(state.shape)}")
 
 
 def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, offsets: Tensor, state: Tensor | None = None, *,
@@ -135,12 +136,9 @@ def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, offsets:
     few rows are taken row by row, others in chunks and, where they are few and long, in segments that run side by side. For
     the backward pass a call in float32 keeps the planes of q, k and v (6 bytes a value). As for any autograd function, a
     backward pass is captured in a CUDA graph only while no eager graph of the same leaves is alive."""
-    _lib.require_cuda(q, k, v, log_decay, offsets, state)
-    scale = _check(q, k, v, log_decay, scale)
+    scale = _check(q, k, v, log_decay, scale, offsets, state)
     if offsets.dim() != 1 or offsets.shape[0] < 1 or offsets.dtype != torch.int64:
         raise ValueError(f"offsets must be int64 [sequences + 1], got {offsets.dtype} {tuple(offsets.shape)}")
-    if offsets.device != q.device:
-        raise ValueError("offsets must be on the device of q")
     if offsets.shape[0] == 1 and q.shape[0]:
         raise ValueError("rows without a sequence: offsets holds one value")
     if state is not None:
@@ -165,19 +163,24 @@ def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, sta
     q, k and v ``[sequences, heads, dim]`` and ``log_decay`` as for ``decay_attention``; any strides. ``state`` is
     contiguous float32 ``[sequences, heads, dim, dim]`` and is the caller's: it moves on by a row each call. Not
     differentiable: where an argument requires a gradient the call raises (``decay_attention`` takes single rows too)."""
-    _lib.require_cuda(q, k, v, log_decay, state)
-    scale = _check(q, k, v, log_decay, scale)
+    scale = _check(q, k, v, log_decay, scale, state)
     _check_state(state, q.shape[0], q)
     if not state.is_contiguous() or state.data_ptr() % 16:
         raise ValueError("state must be contiguous and start at a multiple of 16 bytes: it is changed in place")
-    tensors = (q, k, v, log_decay, state)
-    if (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or has_tangent(*tensors):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+                                     or state.requires_grad)) or has_tangent(q, k, v, log_decay, state):
         raise ValueError("decay_attention_step has no gradient: call it under torch.no_grad(), or decay_attention")
-    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
-    out = _like(q)
-    with on_device(q.device):
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    if k.stride(2) != 1:
+        k = k.contiguous()
+    if v.stride(2) != 1:
+        v = v.contiguous()
+    device = q.device
+    out = torch.empty(q.shape, device=device, dtype=q.dtype)
+    with on_device(device):
         call("fmd_decay_attention_step", _problem(q, k, v, log_decay.contiguous(), None, scale), state.data_ptr(),
-             out.data_ptr(), stream(q.device))
+             out.data_ptr(), stream(device))
     if not state.is_inference():
         torch.autograd.graph.increment_version(state)
     return out
