@@ -373,10 +373,12 @@ def test_gradients_against_differences(cuda):
 
 
 @gpu
-@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
-def test_captured_and_repeated(cuda, dtype):
+@pytest.mark.parametrize("dtype,sizes,dim", [(F32, [600, 250], 64), (B16, [600, 250], 64), (F32, [600, 250], 104),
+                                             (F32, [900, 1400], 72), (F32, [9, 3], 72), (B16, [9, 3], 64)],
+                         ids=["f32", "b16", "f32-parts", "f32-segments", "f32-few", "b16-few"])
+def test_captured_and_repeated(cuda, dtype, sizes, dim):
     """Forward, backward and steps in a graph, replayed on other values and lengths; the same bits on every run."""
-    sizes, heads, dim = [600, 250], 3, 64
+    heads = 3
     q, k, v, g, state, gafter, offsets = make(sizes, heads, dim, dtype)
     log = decays(heads)
     leaves = [t.requires_grad_() for t in (q, k, v)]
@@ -397,7 +399,7 @@ def test_captured_and_repeated(cuda, dtype):
         got = work()
     with torch.no_grad():
         q.mul_(-1.5)
-        offsets[1] = 130
+        offsets[1] = 130 if sizes[0] > 130 else 4
         moving.copy_(state)
     graph.replay()
     moving.copy_(state)
