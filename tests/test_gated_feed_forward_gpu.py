@@ -288,6 +288,42 @@ def test_large_values(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+@pytest.mark.parametrize("rows", [4, 300])
+def test_gates_far_below_zero(cuda, rows, kind):
+    """act(a) and act'(a) for a in [-9, -5], where they are 10^-6 to 10^-18 (GELU): bfloat16 keeps their leading bits. One
+    value of x reaches each projection, down is the identity and every unit has a gradient in one row, so that nothing is
+    summed: y is h as it was rounded (2^-8 of itself), dup and dgate are db and da (2^-8, and 2^-11 of the factor they are
+    multiplied by). The functions' own errors count 2^-16 (the exponent of e^{-a a / 2}, up to 58, has 24 bits; the rest is
+    2^-20), and act' is a difference whose smaller part is a thirtieth of the other."""
+    hidden, width = 512, 8
+    gen = torch.Generator().manual_seed(rows)
+    x = torch.zeros(rows, width)
+    x[:, 0] = 1.0
+    gate, up = torch.zeros(hidden, width), torch.zeros(hidden, width)
+    gate[:, 0] = torch.linspace(-9, -5, hidden)
+    up[:, 0] = torch.randn(hidden, generator=gen)
+    g = torch.zeros(rows, hidden)
+    unit = torch.arange(hidden)
+    g[unit % rows, unit] = torch.randn(hidden, generator=gen)
+    x, gate, up, down, g = (t.to(B16).cuda() for t in (x, gate, up, torch.eye(hidden), g))
+    leaves = [t.requires_grad_() for t in (gate, up)]
+    y = gated_feed_forward(x, gate, up, down, activation=kind)
+    dgate, dup = torch.autograd.grad(y, leaves, g)
+    a, b, own = gate.detach()[:, 0].double(), up.detach()[:, 0].double(), g.sum(0).double()
+    share = torch.sigmoid(a) if kind == "silu" else 0.5 * torch.special.erfc(-a * math.sqrt(0.5))
+    level = a * share
+    slope = share + (level * (1 - share) if kind == "silu" else a * torch.exp(-a * a / 2) / math.sqrt(2 * math.pi))
+    step, function, factor = 2.0 ** -8, 2.0 ** -16, 2.0 ** -11
+    for name, got, want, most in (("y", y.detach(), (level * b).expand(rows, hidden), step + 2 * function),
+                                  ("dup", dup[:, 0], own * level, step + factor + 2 * function),
+                                  ("dgate", dgate[:, 0], own * b * slope, step + factor + 4 * function)):
+        off = ((got.double() - want).abs() / want.abs()).amax()
+        assert float(off) <= most * (1 + step), f"{name}: off by {float(off):.4f} of itself, {most:.4f} allowed"
+    assert not dgate[:, 1:].any() and not dup[:, 1:].any()
+
+
+@gpu
 def test_captured_with_gradients(cuda):
     """Forward and backward in a graph, replayed on other values, two graphs with workspaces of their own."""
     *leaves, g = make(500, 136, 320, 136, B16)
