@@ -14,7 +14,7 @@ from torch.autograd import Function
 from . import _lib
 from ._first_order import first_order, has_tangent
 from ._lib import FmdFeedForward, FmdPadded, c_size_t, call, on_device, ptr, stream
-from .head_rotary import TYPES
+from .head_rotary import TYPES, _aligned
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
 
@@ -86,6 +86,8 @@ class _GatedFeedForward(Function):
         x, gate, up, down = (b if a is None else a for a, b in zip((x, gate, up, down), like))
         device, inputs = x.device, (g, *like)
         g, = _rows(g)
+        # a hook may have moved what was saved: without the padding of its rows, or to another start
+        kept, (x, gate, up, down) = _aligned(kept), _rows(x, gate, up, down)
         grads = [torch.empty(t.shape, device=device, dtype=t.dtype) if need else None
                  for t, need in zip(like, ctx.needs_input_grad)]
         workspace = torch.empty(ctx.size, device=device, dtype=torch.uint8)

@@ -170,6 +170,34 @@ def test_rows_of_odd_length(cuda):
         assert all(torch.equal(a, b) for a, b in zip(results[0], other))
 
 
+class Elsewhere(torch.autograd.graph.saved_tensors_hooks):
+    """Brings what is saved back in memory that starts one value further than a tensor of its own."""
+
+    def __init__(self):
+        super().__init__(lambda t: t.detach().cpu(), self.back)
+
+    @staticmethod
+    def back(t):
+        return torch.empty(t.numel() + 1, device="cuda", dtype=t.dtype)[1:].view(t.shape).copy_(t)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+@pytest.mark.parametrize("width,hidden,out", [(67, 101, 67), (72, 136, 72), (1, 1, 1)])
+def test_saved_tensors_that_come_back_otherwise(cuda, width, hidden, out, dtype):
+    """Hooks that move what is saved (to the host and back) may give it other strides and another start: padded rows come back
+    without their padding. The gradients are those of the tensors as they were, to the bit."""
+    *leaves, g = make(90, width, hidden, out, dtype)
+    views = [torch.zeros(t.shape[0], t.shape[1] + 16, device="cuda", dtype=dtype)[:, 8:8 + t.shape[1]].copy_(t) for t in leaves]
+    for some in (leaves, views, [t.T.contiguous().T for t in leaves]):
+        some = [t.detach().requires_grad_() for t in some]
+        want = torch.autograd.grad(gated_feed_forward(*some), some, g)
+        for hook in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True), Elsewhere()):
+            with hook:
+                y = gated_feed_forward(*some)
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, some, g), want))
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
 def test_gradients_on_their_own(cuda, dtype):
