@@ -15,7 +15,7 @@ from torch.autograd import Function
 from . import _lib
 from ._first_order import first_order, has_tangent
 from ._lib import FmdDecay, c_size_t, call, on_device, ptr, stream
-from .head_rotary import TYPES, _head_rows, _like
+from .head_rotary import TYPES, _aligned, _head_rows, _like
 
 
 def _problem(q, k, v, log_decay, offsets, scale) -> FmdDecay:
@@ -62,6 +62,9 @@ class _DecayAttention(Function):
         if g is None and gafter is None:
             return (None,) * 8
         inputs = (g, gafter, q, k, v, state)
+        # a hook may have moved what was saved to another start
+        q, k, v, log_decay, offsets = _head_rows(q), _head_rows(k), _head_rows(v), log_decay.contiguous(), offsets.contiguous()
+        state, forward = _aligned_state(state), _aligned_state(forward)
         g = torch.zeros_like(q, memory_format=torch.contiguous_format) if g is None else _head_rows(g)
         gafter = _aligned_state(gafter)
         need = ctx.needs_input_grad
@@ -77,10 +80,7 @@ class _DecayAttention(Function):
 
 
 def _aligned_state(state: Tensor | None) -> Tensor | None:
-    if state is None:
-        return None
-    state = state.contiguous()
-    return state.clone() if state.data_ptr() % 16 else state
+    return None if state is None else _aligned(state)
 
 
 def _check(q, k, v, log_decay, scale, *others) -> float:

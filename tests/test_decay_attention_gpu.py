@@ -352,6 +352,37 @@ def test_strides_and_parts(cuda, dtype):
     assert torch.equal(broad, ones)
 
 
+class Elsewhere(torch.autograd.graph.saved_tensors_hooks):
+    """Brings what is saved back in memory that starts one value further than a tensor of its own."""
+
+    def __init__(self):
+        super().__init__(lambda t: t.detach().cpu(), self.back)
+
+    @staticmethod
+    def back(t):
+        return torch.empty(t.numel() + 1, device="cuda", dtype=t.dtype)[1:].view(t.shape).copy_(t)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+@pytest.mark.parametrize("sizes", [[9, 3], [100, 61], [2000]], ids=["rows", "chunks", "segments"])
+def test_saved_tensors_that_come_back_otherwise(cuda, sizes, dtype):
+    """Hooks that move what is saved (to the host and back) may give it another start: the gradients are the same, to the bit."""
+    heads, dim = 3, 72
+    q, k, v, g, state, gafter, offsets = make(sizes, heads, dim, dtype)
+    leaves, grads = [t.requires_grad_() for t in (q, k, v, state)], (g, gafter)
+    log = decays(heads)
+
+    def call():
+        return decay_attention(q, k, v, log, offsets, state, return_state=True)
+
+    want = torch.autograd.grad(call(), leaves, grads)
+    for hook in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True), Elsewhere()):
+        with hook:
+            both = call()
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(both, leaves, grads), want))
+
+
 @gpu
 def test_gradients_against_differences(cuda):
     q, k, v, g, state, gafter, offsets = make([9, 40], 2, 16, F32)
