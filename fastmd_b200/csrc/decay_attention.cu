@@ -100,7 +100,7 @@ __device__ __forceinline__ void write(__nv_bfloat16* p, float v) { *p = __float2
 // 1.08 GB of 512 rows, 16 heads of 128, in 186 us, 5.8 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) step_kernel(const Decay d, float* state) {
-    __shared__ float q[128], k[128], v[128];
+    __shared__ alignas(16) float q[128], k[128], v[128];
     __shared__ float4 sums[kThreads];
     const int64_t b = blockIdx.x / unsigned(d.heads);
     const int head = int(blockIdx.x - b * d.heads), dim = d.dim, quads = dim / 4;

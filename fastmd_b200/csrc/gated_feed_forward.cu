@@ -845,7 +845,7 @@ template <int R, int J, bool GATED>
 __global__ void __launch_bounds__(kFewThreads) few_kernel(const Few f) {
     using S = FewShape<R, J>;
     constexpr int kUnits = GATED ? J / 2 : J;
-    extern __shared__ float few_smem[];
+    extern __shared__ __align__(16) float few_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rg = lane % S::kRowGroups, cg = lane / S::kRowGroups;
     const int unit0 = int(blockIdx.x) * kUnits, row0 = int(blockIdx.y) * R, chunks = (f.inner + kFewChunk - 1) / kFewChunk;
     const int rows = min(R, f.rows - row0);
