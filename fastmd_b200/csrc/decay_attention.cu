@@ -325,7 +325,7 @@ struct Input {
     int64_t row, head;
 };
 
-// The planes of `inputs`, the first `made` of which are there already, at `made_at`; their room stays in the workspace.
+// The planes of `inputs`, the first `made` of which are there already, at `made_at`: the workspace holds those of the others.
 fmd_status make_planes(const Decay& d, Input* inputs, int count, int made, const void* made_at, char*& workspace,
                        cudaStream_t s) {
     SplitArgs a{};
@@ -341,7 +341,7 @@ fmd_status make_planes(const Decay& d, Input* inputs, int count, int made, const
         }
         const void* at = i < made ? static_cast<const char*>(made_at) + i * plane_bytes(d) : workspace;
         inputs[i] = Input{at, int64_t(d.heads) * d.dim, d.dim};
-        workspace += plane_bytes(d);
+        if (i >= made) workspace += plane_bytes(d);
     }
     const dim3 grid(unsigned(grid_for(d.rows * d.heads * (d.dim / 8), kThreads)), unsigned(count - made));
     split_kernel<<<grid, kThreads, 0, s>>>(a);
@@ -404,7 +404,7 @@ fmd_status fmd_decay_attention_workspace_bytes(const fmd_decay* problem, int32_t
     Decay d;
     if (problem == nullptr || bytes == nullptr) return FMD_ERR_INVALID_ARGUMENT;
     const fmd_status st = check_rows(*problem, d);
-    if (st == FMD_OK) *bytes = workspace_of(d, problem->type, backward ? 4 : 3, backward ? 3 : 1);
+    if (st == FMD_OK) *bytes = workspace_of(d, problem->type, backward == 2 ? 1 : backward ? 4 : 3, backward ? 3 : 1);
     return st;
 }
 
@@ -443,7 +443,7 @@ fmd_status fmd_decay_attention_bwd(const fmd_decay* problem, const float* state,
     if (st != FMD_OK) return st;
     const fmd_decay& p = *problem;
     if (p.rows > 0 && g == nullptr) return FMD_ERR_INVALID_ARGUMENT;
-    const size_t need = workspace_of(d, p.type, 4, 3);
+    const size_t need = workspace_of(d, p.type, forward != nullptr ? 1 : 4, 3);
     if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return FMD_ERR_WORKSPACE;
     if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(state) || !aligned16(gafter) ||
         !aligned16(dstate) || !aligned16(workspace) || !aligned16(forward) ||

@@ -24,7 +24,8 @@ def _problem(q, k, v, log_decay, offsets, scale) -> FmdDecay:
                     offsets.shape[0] - 1 if offsets is not None else 0, q.shape[1], q.shape[2])
 
 
-def _workspace(problem: FmdDecay, backward: bool, device) -> tuple[Tensor | None, int]:
+def _workspace(problem: FmdDecay, backward: int, device) -> tuple[Tensor | None, int]:
+    """Of the forward pass (0), of the backward pass (1), or of one that is handed the forward pass's (2)."""
     nbytes = c_size_t()
     call("fmd_decay_attention_workspace_bytes", problem, backward, nbytes)
     size = nbytes.value
@@ -39,7 +40,7 @@ def _forward(q, k, v, log_decay, offsets, state, scale, keep):
     device = q.device
     out, after = _like(q), _states(q, offsets) if keep else None
     problem = _problem(q, k, v, log_decay, offsets, scale)
-    workspace, size = _workspace(problem, False, device)
+    workspace, size = _workspace(problem, 0, device)
     call("fmd_decay_attention", problem, ptr(state), out.data_ptr(), ptr(after), ptr(workspace), size,
          _lib.flags_word(device).data_ptr(), stream(device))
     return out, after, workspace
@@ -71,7 +72,7 @@ class _DecayAttention(Function):
         dq, dk, dv = (_like(t) if n else None for t, n in zip((q, k, v), need))
         dstate = torch.empty_like(state) if need[5] else None
         problem = _problem(q, k, v, log_decay, offsets, ctx.scale)
-        workspace, size = _workspace(problem, True, q.device)
+        workspace, size = _workspace(problem, 1 if forward is None else 2, q.device)
         call("fmd_decay_attention_bwd", problem, ptr(state), ptr(forward), g.data_ptr(), g.stride(0), g.stride(1),
              ptr(gafter), ptr(dq), ptr(dk), ptr(dv), ptr(dstate), ptr(workspace), size,
              _lib.flags_word(q.device).data_ptr(), stream(q.device))
@@ -134,8 +135,9 @@ def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, offsets:
     (1.4 of it in all). Sequences do not see each other's values, finite or not; within a sequence a value that is not finite
     may reach earlier rows too (0 * inf), and an infinity may give NaN. A ``log_decay`` of NaN gives NaN. Sequences of a
     few rows are taken row by row, others in chunks and, where they are few and long, in segments that run side by side. For
-    the backward pass a call in float32 keeps the planes of q, k and v (6 bytes a value). As for any autograd function, a
-    backward pass is captured in a CUDA graph only while no eager graph of the same leaves is alive."""
+    the backward pass a call in float32 keeps the planes of q, k and v (6 bytes a value) and, with segments, their matrices (13 MB
+    at most). As for any autograd function, a backward pass is captured in a CUDA graph only while no eager graph of the same
+    leaves is alive."""
     scale = _check(q, k, v, log_decay, scale, offsets, state)
     if offsets.dim() != 1 or offsets.shape[0] < 1 or offsets.dtype != torch.int64:
         raise ValueError(f"offsets must be int64 [sequences + 1], got {offsets.dtype} {tuple(offsets.shape)}")

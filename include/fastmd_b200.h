@@ -1196,9 +1196,10 @@ typedef struct fmd_decay {
     int32_t type, batch, heads, dim, _pad;
 } fmd_decay;
 
-/* Workspace of the forward pass (backward = 0) or of the backward pass (1),
- * from the sizes alone; 0 for none. It starts at a multiple of 16 bytes. The
- * forward pass's may be handed to the backward pass of the same problem. */
+/* Workspace of the forward pass (backward = 0), of the backward pass (1) or
+ * of a backward pass of the same problem that is handed the forward pass's
+ * workspace (2: smaller in float32), from the sizes alone; 0 for none. It
+ * starts at a multiple of 16 bytes. */
 FMD_API fmd_status fmd_decay_attention_workspace_bytes(const fmd_decay* problem, int32_t backward, size_t* bytes);
 
 /* out [rows, heads, dim] and `after`, the states behind the last rows (NULL:

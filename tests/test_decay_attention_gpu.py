@@ -441,6 +441,63 @@ def test_captured_and_repeated(cuda, dtype, sizes, dim):
 
 
 @gpu
+@pytest.mark.parametrize("sizes", [[64] * 100, [6000, 400]], ids=["chunks", "segments"])
+def test_planes_that_are_handed_over_take_no_room(cuda, sizes):
+    """float32: the forward pass's planes of q, k and v are not given room again. The backward pass allocates its gradients, the
+    planes of the output's gradient (6 bytes a value) and the segments' matrices, and writes nothing behind its workspace."""
+    heads, dim = 3, 72
+    q, k, v, g, state, gafter, offsets = make(sizes, heads, dim, F32)
+    log, leaves = decays(heads), [t.requires_grad_() for t in (q, k, v, state)]
+
+    def step():
+        both = decay_attention(q, k, v, log, offsets, state, return_state=True)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        grads = torch.autograd.grad(both, leaves, (g, gafter))
+        return grads, torch.cuda.max_memory_allocated() - before
+
+    step()
+    want, used = step()
+    values, matrices = q.numel(), 3 * (sum(sizes) // 256 + len(sizes)) * heads * dim * dim * 4
+    assert used <= 3 * 4 * values + state.numel() * 4 + 6 * values + matrices + 2 ** 20
+
+    def problem():
+        return _lib.FmdDecay(q.data_ptr(), k.data_ptr(), v.data_ptr(), log.data_ptr(), offsets.data_ptr(), q.shape[0],
+                             heads * dim, dim, heads * dim, dim, heads * dim, dim, dim ** -0.5, 0, len(sizes), heads, dim)
+
+    def room(backward, guard=0):
+        nbytes = ctypes.c_size_t()
+        _lib.call("fmd_decay_attention_workspace_bytes", problem(), backward, nbytes)
+        return torch.full((nbytes.value + guard,), 0xA5, device="cuda", dtype=torch.uint8), nbytes.value
+
+    forward, size = room(0)
+    flags, stream = _lib.flags_word(q.device).data_ptr(), _lib.stream(q.device)
+    out, grads = torch.empty_like(q), [torch.empty_like(t) for t in leaves]
+    _lib.call("fmd_decay_attention", problem(), state.data_ptr(), out.data_ptr(), None, forward.data_ptr(), size, flags, stream)
+    for handed in (forward.data_ptr(), None):
+        work, size = room(2 if handed else 1, 4096)
+        for t in grads:
+            t.fill_(float("nan"))
+        _lib.call("fmd_decay_attention_bwd", problem(), state.data_ptr(), handed, g.data_ptr(), heads * dim, dim,
+                  gafter.data_ptr(), *(t.data_ptr() for t in grads), work.data_ptr(), size, flags, stream)
+        assert bool((work[size:] == 0xA5).all())
+        assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+def test_the_workspace_of_a_backward_pass_with_planes():
+    lib, one, all_ = _lib.lib(), ctypes.c_size_t(), ctypes.c_size_t()
+    for kind, rows, batch in ((0, 4000, 2), (0, 4000, 200), (0, 40, 2), (1, 4000, 2)):
+        f = _lib.FmdDecay(1 << 20, 1 << 20, 1 << 20, 1 << 20, 1 << 20, rows, 32, 16, 32, 16, 32, 16, 1.0, kind, batch, 2, 16)
+        assert lib.fmd_decay_attention_workspace_bytes(f, 1, all_) == 0 and lib.fmd_decay_attention_workspace_bytes(f, 2, one) == 0
+        planes = rows * 32 * 6 if kind == 0 and rows > 32 * batch else 0
+        assert all_.value - one.value == 3 * planes and one.value >= planes
+        p = ctypes.c_void_p(1 << 20)
+        if one.value:
+            assert lib.fmd_decay_attention_bwd(f, None, p, p, 32, 16, None, p, p, p, None, p, one.value - 1, None, None) == 4
+
+
+@gpu
 def test_two_streams_at_once(cuda):
     q, k, v, g, state, gafter, offsets = make([2100, 1300, 5], 6, 64, B16)
     log = decays(6)
