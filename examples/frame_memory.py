@@ -61,10 +61,17 @@ class MemoryModel(nn.Module):
         super().__init__()
         self.embed, self.read = nn.Linear(features, width), nn.Linear(width, features)
         self.blocks = nn.ModuleList(MemoryBlock(width, heads, dim, hidden) for _ in range(layers))
-        self.to(device=device, dtype=dtype)
         # half-lives from one frame to some hundreds
         rate = 2.0 ** -(1 + 8 * (torch.arange(heads, device=device, dtype=torch.float64) + 0.5) / heads)
-        self.log_decay = torch.log1p(-rate).float()
+        self.register_buffer("log_decay", torch.log1p(-rate).float())
+        self.to(device=device, dtype=dtype)
+
+    def _apply(self, fn, *args, **kwargs):
+        # the decays move with the model, but stay in FP32 whatever its type becomes
+        given = self.log_decay
+        super()._apply(fn, *args, **kwargs)
+        self.log_decay = given.to(self.log_decay.device)
+        return self
 
     def forward(self, frames, offsets, states=None, return_states=False):
         """Predictions after every frame: frames ``[rows, features]`` packed by ``offsets``. ``states``, one a block, are those

@@ -129,3 +129,20 @@ def test_the_decays_on_the_host():
     rate = 1 - model.log_decay.double().exp()
     assert bool((rate.diff() < 0).all()) and 0.2 < float(rate[0]) < 0.5 and float(rate[-1]) < 0.01
     assert [s.shape for s in model.new_states(2)] == [(2, 8, 8, 8)]
+
+
+def test_the_decays_belong_to_the_model():
+    """They move with it and are saved with it, and no change of its type rounds them: the operators take them in FP32."""
+    def make(heads):
+        return load().MemoryModel(3, width=16, heads=heads, dim=8, hidden=24, layers=1, device="cpu")
+
+    model, want = make(8), make(8).log_decay.clone()
+    assert "log_decay" not in dict(model.named_parameters())
+    for kind in (torch.bfloat16, torch.float64, torch.float32):
+        model.to(kind)
+        assert model.embed.weight.dtype == kind and torch.equal(model.log_decay, want) and model.log_decay.dtype == torch.float32
+    saved = model.state_dict()
+    saved["log_decay"] = 0.5 * want
+    model.load_state_dict(saved)
+    assert torch.equal(model.log_decay, 0.5 * want)
+    assert model.to("meta").log_decay.device.type == "meta"
