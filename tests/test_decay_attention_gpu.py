@@ -553,6 +553,70 @@ def test_bad_offsets_are_flagged(cuda, offsets, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,sizes,dim", [(B16, [900, 1400], 64), (F32, [900, 1400], 64), (B16, [2300], 128)],
+                         ids=["b16", "f32", "b16-one"])
+def test_captured_segments(cuda, dtype, sizes, dim):
+    """The same where sequences are cut into segments, and where they become so few rows that most segments are empty."""
+    if len(sizes) == 2:
+        test_captured_and_repeated(cuda, dtype, sizes, dim)
+        return
+    q, k, v, g, state, gafter, offsets = make(sizes, 3, dim, dtype)
+    log, leaves = decays(3), [t.requires_grad_() for t in (q, k, v, state)]
+
+    def work():
+        out, after = decay_attention(q, k, v, log, offsets, state, return_state=True)
+        return out, after, *torch.autograd.grad((out, after), leaves, (g, gafter))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for _ in range(2):
+        with torch.no_grad():
+            v.mul_(-0.5)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, work()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, B16], ids=["f32", "b16"])
+@pytest.mark.parametrize("sizes,heads,dim", [([200] + [0] * 20 + [3] * 5, 2, 64), ([0] * 15 + [1, 180], 3, 128),
+                                             ([2000] + [50] * 30, 2, 64), ([40] * 9 + [1700] + [35] * 9, 3, 72)],
+                         ids=["row_by_row", "last", "chunks", "between"])
+def test_one_long_log_among_short_ones(cuda, sizes, heads, dim, dtype):
+    """The choice of kernels goes by the average length. Row by row a decay l^n is a product of n numbers that are rounded once,
+    n / 2 units of 2^-24: for the 200 rows here less than the 128 units of a chunk's sum, which is not taken."""
+    run_case(sizes, heads, dim, dtype, True, seed=dim)
+
+
+@gpu
+@pytest.mark.parametrize("offsets", [[0, 900, 700, 2300], [5, 900, 1400, 2300], [0, 900, 1400, 2200], [0, 900, 1400, 2400],
+                                     [0, -9, 1400, 2300], [0, 2 ** 40, 1400, 2300], [-(2 ** 40), 900, 1400, 2300],
+                                     [0, 2300, 0, 2300], [2300, 2300, 2300, 2300]])
+@pytest.mark.parametrize("dtype,dim", [(F32, 16), (F32, 72), (B16, 64)], ids=["planes", "parts", "b16"])
+def test_bad_offsets_are_flagged_with_segments(cuda, offsets, dtype, dim):
+    """Nothing outside the arrays is touched: sequences cut into segments, forward and backward."""
+    sizes, heads = [900, 500, 900], 3
+    q, k, v, g, state, gafter, good = make(sizes, heads, dim, dtype)
+    word, log = _lib.flags_word(q.device), decays(heads)
+    want = decay_attention(q, k, v, log, good, state)
+    bad = torch.tensor(offsets, device="cuda")
+    for keep in (False, True):
+        word.zero_()
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, state)]
+        out = decay_attention(*leaves[:3], log, bad, leaves[3], return_state=keep)
+        assert int(word.item()) & 1
+        torch.autograd.grad(out, leaves, (g, gafter) if keep else g)
+        torch.cuda.synchronize()
+    word.zero_()
+    assert torch.equal(decay_attention(q, k, v, log, good, state), want) and int(word.item()) == 0
+
+
+@gpu
 def test_refusals(cuda):
     q, k, v, _, state, _, offsets = make([5, 3], 2, 16, B16)
     log = decays(2)
