@@ -282,8 +282,8 @@ fmd_status check_rows(const fmd_decay& p, Decay& d) {
 // sequences with states, 32 heads: heads of 128 in bfloat16, 1 row 25 and 134, 16 rows 64 and 137, 33 rows 115 and 142, with
 // gradients 237 and 377, 435 and 386; in float32 1 row 25 and 348, 33 rows 106 and 386, with gradients 411 and 1,220; heads of 64
 // in bfloat16 28 and 71 (16 rows), 48 and 73 (33). Four sequences, 8 heads: 23 and 27 (16 rows, bfloat16), 22 and 34 (33,
-// float32), what the host needs. All rows may be one sequence's, which then takes 0.3 us a row: 500 rows 156 and 43 (32 heads
-// of 128, bfloat16).
+// float32), what the host needs. All rows may be one sequence's, which then takes 0.2 to 0.3 us a row, without a bound but theirs:
+// 500 rows 156 and 43 (32 heads of 128, bfloat16), 7,681 beside 511 single ones 1,960 (8 heads of 64; by itself 38).
 bool few_rows(const Decay& d, int type) { return d.rows <= (type == FMD_F32 ? 32 : 16) * int64_t(d.batch); }
 
 fmd_status run_few(const Decays& all, int type, cudaStream_t s) {
@@ -296,9 +296,10 @@ fmd_status run_few(const Decays& all, int type, cudaStream_t s) {
     return check_launch();
 }
 
-// Rows of a segment: whole sequences where these are blocks enough for the GPU or short; else so many that the segments fill
-// it once (the sequences' last ones are half a segment long on average). Segments cost a second look at two of the three
-// inputs and two more launches.
+// Rows of a segment: whole sequences where these are blocks enough for the GPU or short, both on average; else so many that the
+// segments fill it once (the sequences' last ones are half a segment long on average). Segments cost a second look at two of the
+// three inputs and two more launches. A long sequence among short ones is walked by its heads' blocks alone: 30,000 rows beside
+// 63 of 50, 8 heads of 64, take 485 us in bfloat16 and 1,190 in float32, by themselves 61 and 199.
 int64_t segment_length(const Decay& d, bool planes) {
     const int64_t heads = d.heads * (planes && d.dim > 64 ? 2 : 1);  // blocks for a sequence
     if (d.rows / d.batch <= 512 || 10 * d.batch * heads >= 6 * kNumSMs) return kWhole;

@@ -32,10 +32,14 @@
 // Rows of a tile that lie behind a chunk's end belong to others: their pairs are zeros, b' is zero there, and c is set to
 // zero, whatever their values.
 //
-// What bounds it is the traffic of shared memory, 128 bytes a cycle. A chunk of a head of 128 in bfloat16: the products'
+// What bounds it. A chunk among those of all SMs, whole sequences of one length, at 1,965 MHz: a head of 128 in bfloat16 3.5 us,
+// with 5.4 TB/s of memory, a float32 head of 64 6.1 us; and a block takes some 6 us besides, for its offsets, TMEM, first copies
+// and last output, in which its SM does nothing else (148 blocks of 1, 4 and 16 chunks 9.3, 19.6 and 62.7 us; eight times as many
+// of 1 chunk 74). By itself a chunk is bound by the traffic of shared memory, 128 bytes a cycle: in bfloat16 the products'
 // operands 2,300 cycles (f, with two planes of S, 1,000), copies in and out 1,000, what the workers read and write 1,300 (b' and
-// S 500 each, the output 250); it takes 5,500 (products alone 2,560). Of a float32 head of 64: 5,000, 1,400 and 1,200; about
-// 9,000. Measured and not kept: eight workers for the pairs and the output beside eight for the matrix (rows of 50,000 x 16
+// S 500 each, the output 250), of 5,500 (products alone 2,560); in float32 5,000, 1,400 and 1,200 of about 9,000. Not in this
+// account: the registers that heads of 128 spill, 160 bytes stored and 140 read a thread, up to 1,200 cycles were all of them
+// in the walk. Measured and not kept: eight workers for the pairs and the output beside eight for the matrix (rows of 50,000 x 16
 // heads of 128: 163 -> 200 us), one lane that waits for its warp (163 -> 170).
 //
 // Every wait is bounded: on expiry the block raises FMD_FLAG_WAIT_TIMEOUT, waits (bounded) for its copies and products in

@@ -16,8 +16,8 @@
 // the weights' bytes: up of 8 x 4,096 x 11,000 takes 36 us, 5.0 TB/s.
 //
 // Roundings: h, da and db are operands of further products and are stored in bfloat16; each costs the result as much as its
-// own last rounding, 1.4 of it in all. What the gradients are multiplied by has 11 bits or more, which costs next to nothing;
-// as bfloat16 it would cost as much again.
+// own last rounding, 1.4 of it in all. What the gradients are multiplied by is kept in 11 bits, beside the largest of a row's 16
+// units (Args), which costs next to nothing; as bfloat16 it would cost as much again.
 //
 // float32: every operand is three planes of bfloat16 (x = x0 + x1 + x2, 24 bits) and a product is the six of its planes
 // that count: x0 w0 apart from the five small ones, because the tensor cores cut off what does not fit as they add. For the
@@ -87,8 +87,9 @@ struct Args {
     int32_t panels;
     // What the gradients are multiplied by, b act'(a) and act(a), as the threads hold it: blocks of 32 rows x 16 units,
     // [unit / 16][row / 32][piece of 16 bytes][row % 32]. FP32; in 16 bits float16 times a power of two of each row's 16
-    // units, whose inverse is `unit` [unit / 16][row] (11 bits, for values over 2^-29 of the largest of the 16: a rounding to
-    // bfloat16 would cost the gradients as much as their own, and FP32 the kernels that wait for memory a fifth)
+    // units, whose inverse is `unit` [unit / 16][row] (11 bits, for values over 2^-29 of the largest of the 16, fewer below and
+    // none under 2^-39, where a unit adds next to nothing to what its neighbours do: a rounding to bfloat16 would cost the
+    // gradients as much as their own, and FP32 the kernels that wait for memory a fifth)
     void *slope, *level;
     float2* unit;
     int32_t blocks;  // of 32 rows
@@ -265,8 +266,8 @@ __device__ __forceinline__ float normal_share(float a, float density) {
     return a < 0.0f ? tail : 1.0f - tail;
 }
 
-// act(a) and act'(a). EXACT: to FP32's last bits; else, for results in 16 bits, to 2^-20 or so of themselves, and far below
-// zero to 2^-17 (a = -9) or what the exponent of e^{-a a / 2} or e^a keeps.
+// act(a) and act'(a). EXACT: to FP32's last bits; else, for results in 16 bits, to 2^-20 or so. Of themselves, that is, but far
+// below zero, where both keep what the rounding of e^{-a a / 2}'s or e^a's exponent leaves (2^-17 at a = -9).
 template <bool EXACT>
 __device__ __forceinline__ void activate(int act, float a, float& value, float& slope) {
     // held where a factor of 0 stands for the limit, so that an infinity gives its limit too

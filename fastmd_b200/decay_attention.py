@@ -132,12 +132,14 @@ def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, offsets:
     Differentiable in q, k, v and ``state`` (first derivatives in reverse mode: others raise), with the same bits on every
     run. Sums and matrices are held in 32 bits, and states are exact to FP32 in both types; in bfloat16 the weights of the
     pairs of rows and the decayed rows are rounded once as operands, which costs an output about as much as its own rounding
-    (1.4 of it in all). Sequences do not see each other's values, finite or not; within a sequence a value that is not finite
-    may reach earlier rows too (0 * inf), and an infinity may give NaN. A ``log_decay`` of NaN gives NaN. Sequences of a
-    few rows are taken row by row, others in chunks and, where they are few and long, in segments that run side by side. For
-    the backward pass a call in float32 keeps the planes of q, k and v (6 bytes a value) and, with segments, their matrices (13 MB
-    at most). As for any autograd function, a backward pass is captured in a CUDA graph only while no eager graph of the same
-    leaves is alive."""
+    (1.4 of it in all). Row by row the decay is one FP32 number, so that n rows' is off by up to n / 2 of its last bits.
+    Sequences do not see each other's values, finite or not; within a sequence a value that is not finite may reach earlier
+    rows too (0 * inf), and an infinity may give NaN. A ``log_decay`` of NaN gives NaN. Sequences of a few rows are taken row
+    by row, others in chunks and, where they are few and long, in segments that run side by side. Which of these goes by the
+    average length alone: one long sequence among many short ones takes its rows one after the other (0.2 us a row, or 2 to 5
+    a chunk of 128), however many there are; a call of its own is faster for it. For the backward pass a call in float32
+    keeps the planes of q, k and v (6 bytes a value) and, with segments, their matrices (13 MB at most). As for any autograd
+    function, a backward pass is captured in a CUDA graph only while no eager graph of the same leaves is alive."""
     scale = _check(q, k, v, log_decay, scale, offsets, state)
     if offsets.dim() != 1 or offsets.shape[0] < 1 or offsets.dtype != torch.int64:
         raise ValueError(f"offsets must be int64 [sequences + 1], got {offsets.dtype} {tuple(offsets.shape)}")
@@ -163,8 +165,8 @@ def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, sta
     """One new row of every sequence: ``state = exp(log_decay) state + k v^T`` in place, ``out = scale * q state``.
 
     q, k and v ``[sequences, heads, dim]`` and ``log_decay`` as for ``decay_attention``; any strides. ``state`` is
-    contiguous float32 ``[sequences, heads, dim, dim]`` and is the caller's: it moves on by a row each call. Not
-    differentiable: where an argument requires a gradient the call raises (``decay_attention`` takes single rows too)."""
+    contiguous float32 ``[sequences, heads, dim, dim]`` and is the caller's: it moves on by a row each call, by a decay that is
+    one FP32 number (of a ``log_decay`` below some 10^-7 nothing is left of it). Not differentiable: where an argument requires a gradient the call raises (``decay_attention`` takes single rows too)."""
     scale = _check(q, k, v, log_decay, scale, state)
     _check_state(state, q.shape[0], q)
     if not state.is_contiguous() or state.data_ptr() % 16:
